@@ -1,0 +1,539 @@
+// Losses on a language model's logits that need only the log-probability of one token per row: log-probabilities
+// themselves, the clipped policy objective with its KL term, the loss of paired log ratios.
+//
+//   row:         m = max z,  s = sum exp((z - m) / T),  lp = (z[t] - m) / T - log s
+//   policy:      r = exp(lp - old),  l = max(-A r, -A clamp(r, 1 - c, 1 + c')) + k (exp(ref - lp) - (ref - lp) - 1)
+//                dl/dlp = (-A r where the unclipped term is the larger, else 0) + k (1 - exp(ref - lp))
+//   preference:  S = sum lp over an answer,  h = beta ((S_c - ref_c) - (S_r - ref_r)),
+//                l = -(1 - e) log sigmoid(h) - e log sigmoid(-h),  dl/dh = e - sigmoid(-h)
+//   logits:      dz[j] = g / T ([j = t] - exp((z[j] - m) / T) / s)
+//
+// Three kinds of kernels: one reads every row that counts once and keeps (m, log2 s) of it; one block joins the rows
+// into the loss, in a fixed order and in 64 bits (the sum of an answer's log-probabilities runs into the thousands, its
+// difference to the reference's is of order one); one writes the gradient.  Nothing of the size of the logits is kept
+// between the two passes but the logits.  A row that does not count (its token is the ignored index) is not read, so
+// whatever it holds reaches nothing, and its gradient is zero.
+#include <cooperative_groups.h>
+#include "sm100_ptx.cuh"
+#include "common.cuh"
+
+namespace gb {
+namespace tl {
+
+namespace cg = cooperative_groups;
+
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr int SITE_TOKEN = 7;                      // where a bad index was found (native.py: _raise_status)
+
+// Row r of the logits starts at z + (r / inner) * s_outer + (r % inner) * s_inner elements: a [B, T, V] slice is read in place.
+struct RowMap {
+  long long inner, s_outer, s_inner;
+  __device__ __forceinline__ long long at(long long r) const { return (r / inner) * s_outer + (r % inner) * s_inner; }
+};
+
+struct Policy {
+  const float* old;            // [rows]; null: log-probabilities alone are wanted
+  const float* adv;            // one per `adv_div` rows
+  const float* ref;            // [rows] or null
+  float* loss;                 // [rows]
+  float* coef;                 // [rows] dl/dlp
+  long long adv_div;
+  float lo, hi, kl;            // 1 - c, 1 + c', k
+};
+
+struct MaxSum { float m, s; };
+
+// (max, sum) pairs of two parts; c = log2(e) / T.  A part of -inf alone (or of nothing) is (-inf, 0).
+__device__ __forceinline__ MaxSum join(MaxSum a, MaxSum b, float c) {
+  const float m = fmaxf(a.m, b.m);
+  if (m == -INFINITY) return MaxSum{m, a.s + b.s};                 // (a NaN sum stays one)
+  return MaxSum{m, a.s * exp2f((a.m - m) * c) + b.s * exp2f((b.m - m) * c)};
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+template <typename T> struct Two;
+template <> struct Two<__nv_bfloat16> {
+  typedef __nv_bfloat162 P;
+  static __device__ __forceinline__ float2 f(P a) { return __bfloat1622float2(a); }
+  static __device__ __forceinline__ uint32_t pack(float a, float b) { return pack2c<true>(a, b); }
+};
+template <> struct Two<__half> {
+  typedef __half2 P;
+  static __device__ __forceinline__ float2 f(P a) { return __half22float2(a); }
+  static __device__ __forceinline__ uint32_t pack(float a, float b) { return pack2c<false>(a, b); }
+};
+
+// 16 bytes of a row as floats, in pairs
+template <typename T>
+__device__ __forceinline__ void unpack(const uint4& v, float2 (&f)[8 / sizeof(T)]) {
+  if constexpr (sizeof(T) == 4) {
+    f[0] = make_float2(__uint_as_float(v.x), __uint_as_float(v.y));
+    f[1] = make_float2(__uint_as_float(v.z), __uint_as_float(v.w));
+  } else {
+    const typename Two<T>::P* p = reinterpret_cast<const typename Two<T>::P*>(&v);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = Two<T>::f(p[i]);
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ float vec_max(const uint4& v) {
+  if constexpr (sizeof(T) == 4) {
+    return fmaxf(fmaxf(__uint_as_float(v.x), __uint_as_float(v.y)), fmaxf(__uint_as_float(v.z), __uint_as_float(v.w)));
+  } else {
+    const typename Two<T>::P* p = reinterpret_cast<const typename Two<T>::P*>(&v);
+    const float2 f = Two<T>::f(__hmax2(__hmax2(p[0], p[1]), __hmax2(p[2], p[3])));
+    return fmaxf(f.x, f.y);
+  }
+}
+
+// What thread `t` of `G` sees of the `n` elements at p: running maximum and sum, 32 bytes at a time.  Elements before the
+// first 16-byte boundary and behind the last are taken one by one, so rows of odd length cost no more than aligned ones.
+template <typename T, int G>
+__device__ __forceinline__ MaxSum scan(const T* p, int n, float c, int t) {
+  constexpr int V = 16 / sizeof(T), H = V / 2;
+  MaxSum a{-INFINITY, 0.f};
+  auto raise = [&](float mx) {
+    if (mx > a.m) { a.s *= ex2((a.m - mx) * c); a.m = mx; }
+  };
+  auto one = [&](T x) {
+    const float z = Cvt<T>::to_f(x);
+    raise(z);
+    if (z != -INFINITY) a.s += ex2((z - a.m) * c);                 // (NaN comes through: NaN - m)
+  };
+  const float2 c2 = make_float2(c, c);
+  auto add = [&](const uint4& v) {
+    float2 f[H], sum = make_float2(0.f, 0.f);
+    unpack<T>(v, f);
+    const float2 nm = make_float2(-a.m, -a.m);
+#pragma unroll
+    for (int i = 0; i < H; ++i) {
+      float2 e = mul2(add2(f[i], nm), c2);
+      e.x = ex2(e.x); e.y = ex2(e.y);
+      sum = add2(sum, e);
+    }
+    a.s += sum.x + sum.y;
+  };
+  // all of a vector -inf and nothing larger before it: -inf - -inf would be NaN, so only a NaN among them may add
+  auto low = [&](const uint4& v) {
+    float2 f[H];
+    unpack<T>(v, f);
+#pragma unroll
+    for (int i = 0; i < H; ++i) {
+      if (f[i].x != f[i].x) a.s += f[i].x;
+      if (f[i].y != f[i].y) a.s += f[i].y;
+    }
+  };
+  const int mis = (int)((reinterpret_cast<uintptr_t>(p) & 15) / sizeof(T));
+  int head = mis ? V - mis : 0;
+  if (head > n) head = n;
+  if (t < head) one(p[t]);
+  const uint4* v = reinterpret_cast<const uint4*>(p + head);
+  const int nv = (n - head) / V;
+  int i = t;
+  for (; i + G < nv; i += 2 * G) {
+    const uint4 x = v[i], y = v[i + G];
+    raise(fmaxf(vec_max<T>(x), vec_max<T>(y)));
+    if (a.m == -INFINITY) { low(x); low(y); continue; }
+    add(x); add(y);
+  }
+  if (i < nv) {
+    const uint4 x = v[i];
+    raise(vec_max<T>(x));
+    if (a.m == -INFINITY) low(x); else add(x);
+  }
+  const int rest = head + nv * V + t;
+  if (rest < n) one(p[rest]);
+  return a;
+}
+
+__device__ __forceinline__ MaxSum warp_join(MaxSum a, float c) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    MaxSum b;
+    b.m = __shfl_xor_sync(0xffffffffu, a.m, o);
+    b.s = __shfl_xor_sync(0xffffffffu, a.s, o);
+    a = join(a, b, c);
+  }
+  return a;
+}
+
+// The token of a row; false where the row does not count.  A token outside the vocabulary is reported and does not count.
+template <typename TI>
+__device__ __forceinline__ bool counts(const TI* tokens, long long r, long long cols, long long ignore, long long& t) {
+  t = (long long)tokens[r];
+  return t != ignore && t >= 0 && t < cols;
+}
+
+// One row's results, by one thread
+template <typename T, typename TI>
+__device__ __forceinline__ void finish_row(MaxSum a, const T* p, long long t, long long r, long long rows, float temperature,
+                                           float* lp_out, float* stats, const Policy& q) {
+  // differences before products: z[t] - m is exact or nearly so where the token is likely
+  const float lp = (Cvt<T>::to_f(p[t]) - a.m) / temperature - logf(a.s);
+  lp_out[r] = lp;
+  stats[r] = a.m;
+  stats[rows + r] = log2f(a.s);
+  if (q.old != nullptr) {
+    const float A = q.adv[r / q.adv_div];
+    const float ratio = expf(lp - q.old[r]);
+    const float plain = -A * ratio, clipped = -A * fminf(fmaxf(ratio, q.lo), q.hi);
+    float loss = fmaxf(plain, clipped), coef = plain >= clipped ? plain : 0.f;
+    if (plain != plain || clipped != clipped) { loss = plain + clipped; coef = loss; }      // NaN stays NaN
+    if (q.ref != nullptr) {
+      const float d = q.ref[r] - lp, e = expf(d);
+      loss += q.kl * (e - d - 1.f);
+      coef += q.kl * (1.f - e);
+    }
+    q.loss[r] = loss;
+    q.coef[r] = coef;
+  }
+}
+
+__device__ __forceinline__ void skip_row(long long r, long long rows, float* lp_out, float* stats, const Policy& q) {
+  lp_out[r] = 0.f;
+  stats[r] = 0.f;
+  stats[rows + r] = 0.f;
+  if (q.old != nullptr) { q.loss[r] = 0.f; q.coef[r] = 0.f; }
+}
+
+// Rows of up to a few KB: one warp each.
+template <typename T, typename TI>
+__global__ void __launch_bounds__(256)
+token_rows_warp_kernel(const T* __restrict__ z, RowMap map, const TI* __restrict__ tokens, float* __restrict__ lp,
+                       float* __restrict__ stats, long long rows, int cols, long long ignore, float temperature, float c,
+                       Policy q, int* status) {
+  const int lane = threadIdx.x & 31;
+  const long long r = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (r >= rows) return;
+  long long t;
+  if (!counts(tokens, r, cols, ignore, t)) {
+    if (lane == 0) {
+      if (t != ignore) report_error(status, GB_ERR_BAD_INDEX, SITE_TOKEN, (int)t);
+      skip_row(r, rows, lp, stats, q);
+    }
+    return;
+  }
+  const T* p = z + map.at(r);
+  const MaxSum a = warp_join(scan<T, 32>(p, cols, c, lane), c);
+  if (lane == 0) finish_row<T, TI>(a, p, t, r, rows, temperature, lp, stats, q);
+}
+
+constexpr int FWD_THREADS = 512;
+
+// Long rows: one CTA each, or, where rows are few, the CTAs of a cluster share one and rank 0 joins their parts through
+// distributed shared memory.
+template <typename T, typename TI>
+__global__ void __launch_bounds__(FWD_THREADS, 3)
+token_rows_kernel(const T* __restrict__ z, RowMap map, const TI* __restrict__ tokens, float* __restrict__ lp,
+                  float* __restrict__ stats, long long rows, int cols, long long ignore, float temperature, float c,
+                  Policy q, int* status, int parts) {
+  __shared__ float2 sh[FWD_THREADS / 32];
+  __shared__ float2 mine;
+  const long long r = blockIdx.x / parts;
+  const int part = blockIdx.x % parts;
+  long long t;
+  if (!counts(tokens, r, cols, ignore, t)) {                       // (alike in all CTAs of the cluster)
+    if (part == 0 && threadIdx.x == 0) {
+      if (t != ignore) report_error(status, GB_ERR_BAD_INDEX, SITE_TOKEN, (int)t);
+      skip_row(r, rows, lp, stats, q);
+    }
+    return;
+  }
+  const T* p = z + map.at(r);
+  int lo = 0, n = cols;
+  if (parts > 1) {
+    const int step = ((cols + parts - 1) / parts + 7) & ~7;
+    lo = min(part * step, cols);
+    n = min(step, cols - lo);
+  }
+  MaxSum a = warp_join(scan<T, FWD_THREADS>(p + lo, n, c, threadIdx.x), c);
+  if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = make_float2(a.m, a.s);
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    a = MaxSum{-INFINITY, 0.f};
+    if (threadIdx.x < FWD_THREADS / 32) a = MaxSum{sh[threadIdx.x].x, sh[threadIdx.x].y};
+    a = warp_join(a, c);
+  }
+  if (parts > 1) {
+    cg::cluster_group cl = cg::this_cluster();
+    if (threadIdx.x == 0) mine = make_float2(a.m, a.s);
+    cl.sync();
+    if (part == 0 && threadIdx.x == 0) {
+      for (int k = 1; k < parts; ++k) {
+        const float2 o = *cl.map_shared_rank(&mine, k);
+        a = join(a, MaxSum{o.x, o.y}, c);
+      }
+    }
+    cl.sync();                                                     // nobody leaves while its part may still be read
+  }
+  if (part == 0 && threadIdx.x == 0) finish_row<T, TI>(a, p, t, r, rows, temperature, lp, stats, q);
+}
+
+__device__ __forceinline__ double block_sum64(double v, double* sh) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = (threadIdx.x & 31) < (blockDim.x >> 5) ? sh[threadIdx.x & 31] : 0.0;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// out[0] = sum of the rows' losses (over the number of rows that count), out[1] = the factor of every row's gradient
+template <typename TI>
+__global__ void __launch_bounds__(1024)
+policy_sum_kernel(const float* __restrict__ loss, const TI* __restrict__ tokens, long long rows, long long cols,
+                  long long ignore, int mean, float* __restrict__ out) {
+  __shared__ double sh[32];
+  double sum = 0.0, n = 0.0;
+  for (long long r = threadIdx.x; r < rows; r += 1024) {
+    long long t;
+    if (counts(tokens, r, cols, ignore, t)) { sum += (double)loss[r]; n += 1.0; }
+  }
+  sum = block_sum64(sum, sh);
+  n = block_sum64(n, sh);
+  if (threadIdx.x == 0) {
+    const double f = mean && n > 0.0 ? 1.0 / n : 1.0;
+    out[0] = (float)(sum * f);
+    out[1] = (float)f;
+  }
+}
+
+// Pair i: answers i (chosen) and pairs + i (rejected) of `len` rows each.  loss_each [pairs] or null; out[0] = their sum
+// (or mean); rewards [2 pairs] = beta (S - ref); gseq [2 pairs] = dl/dS.
+__global__ void __launch_bounds__(1024)
+preference_kernel(const float* __restrict__ lp, const float* __restrict__ ref, long long pairs, long long len, float beta,
+                  float smooth, int mean, float* __restrict__ loss_each, float* __restrict__ out, float* __restrict__ rewards,
+                  float* __restrict__ gseq) {
+  __shared__ double sh[32];
+  const int lane = threadIdx.x & 31;
+  for (long long s = threadIdx.x >> 5; s < 2 * pairs; s += 32) {
+    const float* p = lp + s * len;
+    double sum = 0.0;
+    for (long long i = lane; i < len; i += 32) sum += (double)p[i];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0) rewards[s] = (float)((double)beta * (sum - (double)ref[s]));
+  }
+  __syncthreads();
+  double total = 0.0;
+  for (long long i = threadIdx.x; i < pairs; i += 1024) {
+    const float h = rewards[i] - rewards[pairs + i];
+    // log(1 + exp(-|h|)) is common to both signs: -log sigmoid(h) = max(-h, 0) + it
+    const float l1 = log1pf(expf(-fabsf(h)));
+    const float loss = (1.f - smooth) * (fmaxf(-h, 0.f) + l1) + smooth * (fmaxf(h, 0.f) + l1) + (h != h ? h : 0.f);
+    const float g = beta * (smooth - 1.f / (1.f + expf(h)));
+    gseq[i] = g;
+    gseq[pairs + i] = -g;
+    if (loss_each != nullptr) loss_each[i] = loss;
+    total += (double)loss;
+  }
+  total = block_sum64(total, sh);
+  if (threadIdx.x == 0) out[0] = (float)(mean && pairs > 0 ? total / (double)pairs : total);
+}
+
+// A row's factor: base[r / base_div] * g[r / g_div % g_mod] * *dev_scale * scale, each pointer null for 1
+struct Factor {
+  const float* base; const float* g; const float* dev_scale;
+  long long base_div, g_div, g_mod;
+  float scale;
+  __device__ __forceinline__ float at(long long r) const {
+    float f = scale;
+    if (dev_scale != nullptr) f *= *dev_scale;
+    if (g != nullptr) f *= g[(r / g_div) % g_mod];
+    if (base != nullptr) f *= base[r / base_div];
+    return f;
+  }
+};
+
+constexpr int BWD_THREADS = 256;
+
+// Gradient of `n` elements of a row by `G` threads; `t` counts from the first of them.
+template <typename T, int G>
+__device__ __forceinline__ void grad_part(const T* p, T* d, int n, long long t, float m, float ls, float c, float f, int tid) {
+  constexpr int V = 16 / sizeof(T), H = V / 2, U = 4;
+  auto one = [&](int j) {
+    const float e = ex2(fmaf(Cvt<T>::to_f(p[j]) - m, c, -ls));
+    d[j] = Cvt<T>::from_f(f * ((j == t ? 1.f : 0.f) - e));
+  };
+  const int mis = (int)((reinterpret_cast<uintptr_t>(d) & 15) / sizeof(T));
+  int head = mis ? V - mis : 0;
+  if (head > n) head = n;
+  const bool same = ((reinterpret_cast<uintptr_t>(p) ^ reinterpret_cast<uintptr_t>(d)) & 15) == 0;
+  const int nv = same ? (n - head) / V : 0;
+  const uint4* src = reinterpret_cast<const uint4*>(p + head);
+  uint4* dst = reinterpret_cast<uint4*>(d + head);
+  const float2 nm = make_float2(-m, -m), c2 = make_float2(c, c), nl = make_float2(-ls, -ls), nf = make_float2(-f, -f);
+  const long long tv = t < head ? -1 : (t - head) / V;             // the vector that holds the token
+  auto vec = [&](const uint4& x, int i) {
+    float2 e[H];
+    unpack<T>(x, e);
+#pragma unroll
+    for (int k = 0; k < H; ++k) {
+      e[k] = fma2(add2(e[k], nm), c2, nl);
+      e[k].x = ex2(e[k].x); e[k].y = ex2(e[k].y);
+    }
+    if (i == tv) {
+      const int at = (int)((t - head) % V);
+#pragma unroll
+      for (int k = 0; k < H; ++k) {
+        if (2 * k == at) e[k].x -= 1.f;
+        if (2 * k + 1 == at) e[k].y -= 1.f;
+      }
+    }
+    uint4 o;
+    uint32_t* w = reinterpret_cast<uint32_t*>(&o);
+#pragma unroll
+    for (int k = 0; k < H; ++k) {
+      e[k] = mul2(e[k], nf);
+      if constexpr (sizeof(T) == 4) { w[2 * k] = __float_as_uint(e[k].x); w[2 * k + 1] = __float_as_uint(e[k].y); }
+      else w[k] = Two<T>::pack(e[k].x, e[k].y);
+    }
+    dst[i] = o;
+  };
+  if (same) {
+    if (tid < head) one(tid);
+    int i = tid;
+    for (; i + (U - 1) * G < nv; i += U * G) {
+      uint4 x[U];
+#pragma unroll
+      for (int k = 0; k < U; ++k) x[k] = src[i + k * G];
+#pragma unroll
+      for (int k = 0; k < U; ++k) vec(x[k], i + k * G);
+    }
+    for (; i < nv; i += G) vec(src[i], i);
+    const int rest = head + nv * V + tid;
+    if (rest < n) one(rest);
+  } else {
+    for (int j = tid; j < n; j += G) one(j);
+  }
+}
+
+template <typename T, int G>
+__device__ __forceinline__ void zero_part(T* d, int n, int tid) {
+  constexpr int V = 16 / sizeof(T);
+  const int mis = (int)((reinterpret_cast<uintptr_t>(d) & 15) / sizeof(T));
+  int head = mis ? V - mis : 0;
+  if (head > n) head = n;
+  const int nv = (n - head) / V;
+  if (tid < head) d[tid] = Cvt<T>::from_f(0.f);
+  uint4* dst = reinterpret_cast<uint4*>(d + head);
+  for (int i = tid; i < nv; i += G) dst[i] = make_uint4(0, 0, 0, 0);
+  const int rest = head + nv * V + tid;
+  if (rest < n) d[rest] = Cvt<T>::from_f(0.f);
+}
+
+// `G` threads per item; an item is `chunk` elements of one row.  Rows run from the last to the first: the forward pass
+// has left the last ones in L2.
+template <typename T, typename TI, int G>
+__global__ void __launch_bounds__(BWD_THREADS)
+token_grad_kernel(const T* __restrict__ z, RowMap map, const TI* __restrict__ tokens, const float* __restrict__ stats,
+                  T* __restrict__ dz, long long rows, int cols, long long ignore, float temperature, float c, Factor fac,
+                  int chunk, int chunks) {
+  const int tid = threadIdx.x % G;
+  const long long item = (long long)blockIdx.x * (BWD_THREADS / G) + threadIdx.x / G;
+  if (item >= rows * chunks) return;
+  const long long r = rows - 1 - item / chunks;
+  const int lo = (int)(item % chunks) * chunk;
+  const int n = min(chunk, cols - lo);
+  T* d = dz + r * cols + lo;
+  long long t;
+  const float f = counts(tokens, r, cols, ignore, t) ? fac.at(r) / temperature : 0.f;
+  if (f == 0.f) { zero_part<T, G>(d, n, tid); return; }
+  grad_part<T, G>(z + map.at(r) + lo, d, n, t - lo, stats[r], stats[rows + r], c, f, tid);
+}
+
+template <typename T, typename TI>
+static int rows_forward(const void* z, RowMap map, const void* tokens, float* lp, float* stats, long long rows, int cols,
+                        long long ignore, float temperature, const Policy& q, int* status, cudaStream_t st) {
+  const float c = LOG2E / temperature;
+  if (cols <= 1024) {
+    token_rows_warp_kernel<T, TI><<<(unsigned)((rows + 7) / 8), 256, 0, st>>>(
+        (const T*)z, map, (const TI*)tokens, lp, stats, rows, cols, ignore, temperature, c, q, status);
+    return (int)cudaGetLastError();
+  }
+  // a part has to be worth its cluster barriers: 4096 elements at least
+  int parts = 1;
+  while (parts < 8 && rows * parts * 2 <= 3ll * sm_count() && cols / (parts * 2) >= 4096) parts *= 2;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = parts; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+  cfg.gridDim = dim3((unsigned)(rows * parts)); cfg.blockDim = dim3(FWD_THREADS); cfg.stream = st;
+  cfg.attrs = attr; cfg.numAttrs = parts > 1 ? 1 : 0;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, token_rows_kernel<T, TI>, (const T*)z, map, (const TI*)tokens, lp, stats, rows,
+                                           cols, ignore, temperature, c, q, status, parts);
+  return e == cudaSuccess ? (int)cudaGetLastError() : (int)e;
+}
+
+template <typename T, typename TI>
+static int rows_backward(const void* z, RowMap map, const void* tokens, const float* stats, void* dz, long long rows, int cols,
+                         long long ignore, float temperature, const Factor& fac, cudaStream_t st) {
+  const float c = LOG2E / temperature;
+  if (cols <= 1024) {
+    token_grad_kernel<T, TI, 32><<<(unsigned)((rows + 7) / 8), BWD_THREADS, 0, st>>>(
+        (const T*)z, map, (const TI*)tokens, stats, (T*)dz, rows, cols, ignore, temperature, c, fac, cols, 1);
+    return (int)cudaGetLastError();
+  }
+  const int chunk = 16384 / (int)sizeof(T) * 2;
+  const int chunks = (cols + chunk - 1) / chunk;
+  if (rows * chunks > 0x7fffffffll) return -3;
+  token_grad_kernel<T, TI, BWD_THREADS><<<(unsigned)(rows * chunks), BWD_THREADS, 0, st>>>(
+      (const T*)z, map, (const TI*)tokens, stats, (T*)dz, rows, cols, ignore, temperature, c, fac, chunk, chunks);
+  return (int)cudaGetLastError();
+}
+
+}  // namespace tl
+}  // namespace gb
+
+using namespace gb;
+
+// Log-probabilities lp [rows] of `tokens` and the rows' (max, log2 sum) in stats [2, rows].  With `old` also the clipped
+// policy loss [rows] and its derivative by lp [rows].  Rows: see RowMap.
+extern "C" int gb_token_rows(const void* z, const void* tokens, float* lp, float* stats, long long rows, long long cols,
+                             long long inner, long long s_outer, long long s_inner, long long ignore, float temperature,
+                             const float* old, const float* adv, const float* ref, float* loss, float* coef,
+                             long long adv_div, float lo, float hi, float kl, int dt, int token_i64, int* status,
+                             cudaStream_t st) {
+  if (rows == 0) return 0;
+  if (cols < 1 || cols > 0x7fffffffll || rows > 0x0fffffffll || inner < 1 || adv_div < 1 || !(temperature > 0.f)) return -3;
+  const tl::RowMap map{inner, s_outer, s_inner};
+  const tl::Policy q{old, adv, ref, loss, coef, adv_div, lo, hi, kl};
+  if (token_i64) GB_DISPATCH_FLOAT(dt, T, return (tl::rows_forward<T, long long>(z, map, tokens, lp, stats, rows, (int)cols, ignore, temperature, q, status, st)));
+  GB_DISPATCH_FLOAT(dt, T, return (tl::rows_forward<T, int>(z, map, tokens, lp, stats, rows, (int)cols, ignore, temperature, q, status, st)));
+}
+
+extern "C" int gb_policy_sum(const float* loss, const void* tokens, long long rows, long long cols, long long ignore,
+                             int mean, float* out, int token_i64, cudaStream_t st) {
+  if (token_i64) tl::policy_sum_kernel<long long><<<1, 1024, 0, st>>>(loss, (const long long*)tokens, rows, cols, ignore, mean, out);
+  else tl::policy_sum_kernel<int><<<1, 1024, 0, st>>>(loss, (const int*)tokens, rows, cols, ignore, mean, out);
+  return (int)cudaGetLastError();
+}
+
+extern "C" int gb_preference(const float* lp, const float* ref, long long pairs, long long len, float beta, float smooth,
+                             int mean, float* loss_each, float* out, float* rewards, float* gseq, cudaStream_t st) {
+  tl::preference_kernel<<<1, 1024, 0, st>>>(lp, ref, pairs, len, beta, smooth, mean, loss_each, out, rewards, gseq);
+  return (int)cudaGetLastError();
+}
+
+// Gradient dz [rows, cols] (contiguous); a row's factor: see Factor.
+extern "C" int gb_token_grad(const void* z, const void* tokens, const float* stats, void* dz, long long rows, long long cols,
+                             long long inner, long long s_outer, long long s_inner, long long ignore, float temperature,
+                             const float* base, long long base_div, const float* g, long long g_div, long long g_mod,
+                             const float* dev_scale, float scale, int dt, int token_i64, cudaStream_t st) {
+  if (rows == 0) return 0;
+  if (cols < 1 || cols > 0x7fffffffll || rows > 0x0fffffffll || inner < 1 || base_div < 1 || g_div < 1 || g_mod < 1 ||
+      !(temperature > 0.f)) return -3;
+  const tl::RowMap map{inner, s_outer, s_inner};
+  const tl::Factor fac{base, g, dev_scale, base_div, g_div, g_mod, scale};
+  if (token_i64) GB_DISPATCH_FLOAT(dt, T, return (tl::rows_backward<T, long long>(z, map, tokens, stats, dz, rows, (int)cols, ignore, temperature, fac, st)));
+  GB_DISPATCH_FLOAT(dt, T, return (tl::rows_backward<T, int>(z, map, tokens, stats, dz, rows, (int)cols, ignore, temperature, fac, st)));
+}

@@ -954,6 +954,79 @@ class CrossEntropyFunction(Function):
         return K.cross_entropy_bwd(logits, target, lse, rows, ignore_index, inplace)
 
 
+class TokenLogProbsFunction(Function):
+    """Log-probabilities of given tokens; the backward pass writes g (onehot - softmax) / temperature in one pass."""
+    raw = True
+    amp_policy = AMPPolicy.PRESERVE
+
+    @staticmethod
+    def forward(ctx, logits, tokens, temperature, ignore_index):
+        logits = K.token_logits(logits)
+        lp, stats = K.token_rows(logits, tokens, ignore_index, temperature)
+        ctx.save_for_backward(logits, tokens, stats)
+        ctx.meta = (temperature, ignore_index)
+        return lp
+
+    @staticmethod
+    def backward(ctx, g):
+        logits, tokens, stats = ctx.saved_tensors
+        temperature, ignore_index = ctx.meta
+        return K.token_grad(logits, tokens, stats, ignore_index, temperature, g=K.contiguous(K.to_dtype(g, stats.dtype)),
+                            g_mod=_pymax(tokens.numel(), 1))
+
+
+class PolicyLossFunction(Function):
+    """Clipped policy objective with a KL term, from the logits: one pass over the rows forward, one backward."""
+    raw = True
+    amp_policy = AMPPolicy.PRESERVE
+
+    @staticmethod
+    def forward(ctx, logits, tokens, policy, temperature, ignore_index, reduction):
+        logits = K.token_logits(logits)
+        _, stats, loss, coef = K.token_rows(logits, tokens, ignore_index, temperature, policy)
+        total = None
+        if reduction != "none":
+            total = K.policy_sum(loss, tokens, logits.shape[-1], ignore_index, reduction == "mean")
+        ctx.save_for_backward(logits, tokens, stats, coef, total)
+        ctx.meta = (temperature, ignore_index)
+        return loss if total is None else total[0]
+
+    @staticmethod
+    def backward(ctx, g):
+        logits, tokens, stats, coef, total = ctx.saved_tensors
+        temperature, ignore_index = ctx.meta
+        return K.token_grad(logits, tokens, stats, ignore_index, temperature, base=coef,
+                            g=K.contiguous(K.to_dtype(g, stats.dtype)),
+                            g_mod=_pymax(tokens.numel(), 1) if total is None else 1,
+                            dev_scale=None if total is None else total[1:])
+
+
+class PreferenceLossFunction(Function):
+    """Loss of paired log ratios, from the logits of chosen and rejected answers."""
+    raw = True
+    amp_policy = AMPPolicy.PRESERVE
+
+    @staticmethod
+    def forward(ctx, logits, tokens, ref, beta, smoothing, ignore_index, reduction, rewards_out):
+        logits = K.token_logits(logits)
+        lp, stats = K.token_rows(logits, tokens, ignore_index, 1.0)
+        each, total, rewards, gseq = K.preference(lp, ref, beta, smoothing, reduction == "mean", reduction == "none")
+        rewards_out.append(rewards)
+        ctx.save_for_backward(logits, tokens, stats, gseq)
+        ctx.meta = (ignore_index, reduction)
+        return total if each is None else each
+
+    @staticmethod
+    def backward(ctx, g):
+        logits, tokens, stats, gseq = ctx.saved_tensors
+        ignore_index, reduction = ctx.meta
+        pairs, length = gseq.numel() // 2, _pymax(tokens.shape[1], 1)
+        return K.token_grad(logits, tokens, stats, ignore_index, 1.0, base=gseq, base_div=length,
+                            g=K.contiguous(K.to_dtype(g, stats.dtype)), g_div=length,
+                            g_mod=_pymax(pairs, 1) if reduction == "none" else 1,
+                            scale=1.0 / _pymax(pairs, 1) if reduction == "mean" else 1.0)
+
+
 # ============================= fused transformer ops ==============================
 class FusedRMSNormFunction(Function):
     raw = True
@@ -1507,6 +1580,106 @@ def cross_entropy(input, target, weight=None, ignore_index=-100, reduction="mean
 
 
 sparse_cross_entropy = cross_entropy
+
+
+def _token_args(name, logits, tokens, ignore_index, temperature=1.0):
+    """Checks what the losses on tokens' log-probabilities have in common; returns the raw tokens."""
+    if not (isinstance(logits, Tensor) and isinstance(tokens, Tensor)):
+        raise TypeError(f"{name}: logits and tokens must be Tensors")
+    z, t = logits._t, tokens._t
+    if not z.dtype.is_floating_point:
+        raise TypeError(f"{name}: logits must be floating-point, got {z.dtype}")
+    if t.dtype.is_floating_point or t.dtype.is_complex or t.dtype == torch.bool:
+        raise TypeError(f"{name}: tokens must be integers, got {t.dtype}")
+    if z.dim() < 1 or z.shape[-1] == 0 or tuple(t.shape) != tuple(z.shape[:-1]):
+        raise ValueError(f"{name}: logits [..., V] need tokens [...], got {tuple(z.shape)} and {tuple(t.shape)}")
+    if t.device != z.device:
+        raise ValueError(f"{name}: logits are on {z.device}, tokens on {t.device}")
+    if isinstance(ignore_index, bool) or not isinstance(ignore_index, int):
+        raise TypeError(f"{name}: ignore_index must be an int, got {ignore_index!r}")
+    if not 1e-6 <= float(temperature) < math.inf:
+        raise ValueError(f"{name}: temperature must be finite and at least 1e-6, got {temperature}")
+    if t.dtype not in (torch.int64, torch.int32):
+        t = t.long()
+    return K.contiguous(t)
+
+
+def _constant(name, what, x, shapes, z):
+    """A floating-point input through which no gradient flows, as contiguous numbers of the width the loss is computed in."""
+    if not isinstance(x, Tensor) or not x._t.dtype.is_floating_point:
+        raise TypeError(f"{name}: {what} must be a floating-point Tensor")
+    if x.requires_grad:
+        raise ValueError(f"{name}: {what} is a constant of the loss; pass a detached Tensor")
+    if tuple(x._t.shape) not in shapes:
+        raise ValueError(f"{name}: {what} has shape {tuple(x._t.shape)}, expected {' or '.join(map(str, shapes))}")
+    if x._t.device != z.device:
+        raise ValueError(f"{name}: logits are on {z.device}, {what} on {x._t.device}")
+    return K.contiguous(K.to_dtype(x._t, torch.float64 if z.dtype == torch.float64 else torch.float32))
+
+
+def _number(name, what, x, low, high):
+    if isinstance(x, bool) or not isinstance(x, (int, float)) or not low <= x <= high:
+        raise ValueError(f"{name}: {what} must be a number from {low} to {high}, got {x!r}")
+    return float(x)
+
+
+def token_log_probs(logits, tokens, temperature=1.0, ignore_index=-100):
+    """Log-probabilities of `tokens` [...] under softmax(logits [..., V] / temperature), in float32 (0 where ignored).
+
+    What a sampler's or a reference model's answers are scored by.  Logits are read once and in place (a `[:, :-1]` view is
+    not copied); rows whose token is `ignore_index` are not read.  A row that is -inf throughout gives NaN."""
+    t = _token_args("token_log_probs", logits, tokens, ignore_index, temperature)
+    return TokenLogProbsFunction.apply(logits, t, float(temperature), ignore_index)
+
+
+def policy_loss(logits, tokens, old_log_probs, advantages, ref_log_probs=None, clip=0.2, clip_high=None, kl_coef=0.0,
+                temperature=1.0, ignore_index=-100, reduction="mean"):
+    """Clipped policy objective with a KL penalty, from the policy's logits [..., V] for the `tokens` [...] it drew.
+
+    With lp the tokens' log-probabilities (of logits / temperature) and r = exp(lp - old_log_probs), every token's loss is
+    max(-A r, -A clamp(r, 1 - clip, 1 + clip_high)) + kl_coef (exp(d) - d - 1), d = ref_log_probs - lp.
+    `advantages` has one number per token, or one per sequence ([...] without the last dimension); `clip_high` is `clip`
+    unless given.  Tokens equal to `ignore_index` (prompts, padding) do not count, whatever the other inputs hold there;
+    "mean" is over those that do (0 if there are none).  Gradients flow to the logits alone; where both branches are
+    equal they flow through the first."""
+    name = "policy_loss"
+    if reduction not in ("mean", "sum", "none"):
+        raise ValueError(f"Invalid reduction mode: {reduction}")
+    t = _token_args(name, logits, tokens, ignore_index, temperature)
+    z, shape = logits._t, tuple(t.shape)
+    lo = 1.0 - _number(name, "clip", clip, 0.0, 1.0)
+    hi = 1.0 + _number(name, "clip_high", clip if clip_high is None else clip_high, 0.0, math.inf)
+    kl = _number(name, "kl_coef", kl_coef, 0.0, math.inf)
+    if (ref_log_probs is None) != (kl == 0.0):
+        raise ValueError(f"{name}: ref_log_probs and a positive kl_coef go together")
+    old = _constant(name, "old_log_probs", old_log_probs, (shape,), z)
+    adv = _constant(name, "advantages", advantages, (shape, shape[:-1]) if shape else (shape,), z)
+    ref = None if ref_log_probs is None else _constant(name, "ref_log_probs", ref_log_probs, (shape,), z)
+    div = 1 if tuple(adv.shape) == shape else _pymax(shape[-1], 1)
+    return PolicyLossFunction.apply(logits, t, (old, adv, div, ref, lo, hi, kl), float(temperature), ignore_index, reduction)
+
+
+def preference_loss(logits, tokens, ref_log_probs, beta=0.1, label_smoothing=0.0, ignore_index=-100, reduction="mean",
+                    return_rewards=False):
+    """Loss of paired log ratios, from the logits [2 P, T, V] of P chosen answers followed by the P rejected ones.
+
+    With S the sums of the answers' log-probabilities (tokens [2 P, T]; those equal to `ignore_index` do not count) and
+    reward = beta (S - ref_log_probs [2 P]), a pair's loss is -(1 - e) log sigmoid(h) - e log sigmoid(-h) with
+    h = reward(chosen) - reward(rejected) and e = label_smoothing.  "none" gives one loss per pair.  With
+    `return_rewards` also the rewards [2 P], through which no gradient flows."""
+    name = "preference_loss"
+    if reduction not in ("mean", "sum", "none"):
+        raise ValueError(f"Invalid reduction mode: {reduction}")
+    t = _token_args(name, logits, tokens, ignore_index)
+    z = logits._t
+    if z.dim() != 3 or z.shape[0] % 2:
+        raise ValueError(f"{name}: logits must be [2 P, T, V], chosen answers before rejected ones, got {tuple(z.shape)}")
+    beta = _number(name, "beta", beta, 0.0, math.inf)
+    smoothing = _number(name, "label_smoothing", label_smoothing, 0.0, 1.0)
+    ref = _constant(name, "ref_log_probs", ref_log_probs, ((z.shape[0],),), z)
+    rewards = []
+    loss = PreferenceLossFunction.apply(logits, t, ref, beta, smoothing, ignore_index, reduction, rewards)
+    return (loss, Tensor._wrap(rewards[0])) if return_rewards else loss
 
 
 def rms_norm(x, weight, eps=1e-6):

@@ -32,6 +32,33 @@ class CrossEntropyLoss(Module):
         return F.cross_entropy(input, target, weight=w, ignore_index=self.ignore_index, reduction=self.reduction)
 
 
+class PolicyLoss(Module):
+    """Clipped policy objective with a KL penalty: `F.policy_loss` with its settings kept."""
+
+    def __init__(self, clip=0.2, clip_high=None, kl_coef=0.0, temperature=1.0, ignore_index=-100, reduction="mean"):
+        super().__init__()
+        self.clip, self.clip_high, self.kl_coef = clip, clip_high, kl_coef
+        self.temperature, self.ignore_index, self.reduction = temperature, ignore_index, reduction
+
+    def forward(self, logits, tokens, old_log_probs, advantages, ref_log_probs=None):
+        return F.policy_loss(logits, tokens, old_log_probs, advantages, ref_log_probs, clip=self.clip,
+                             clip_high=self.clip_high, kl_coef=self.kl_coef, temperature=self.temperature,
+                             ignore_index=self.ignore_index, reduction=self.reduction)
+
+
+class PreferenceLoss(Module):
+    """Loss of paired log ratios: `F.preference_loss` with its settings kept."""
+
+    def __init__(self, beta=0.1, label_smoothing=0.0, ignore_index=-100, reduction="mean"):
+        super().__init__()
+        self.beta, self.label_smoothing = beta, label_smoothing
+        self.ignore_index, self.reduction = ignore_index, reduction
+
+    def forward(self, logits, tokens, ref_log_probs):
+        return F.preference_loss(logits, tokens, ref_log_probs, beta=self.beta, label_smoothing=self.label_smoothing,
+                                 ignore_index=self.ignore_index, reduction=self.reduction)
+
+
 class SoftmaxLoss(Module):
     def forward(self, logits, y):
         return F.cross_entropy(logits, y)

@@ -602,6 +602,101 @@ def cross_entropy_bwd(logits, target, lse, grad_rows, ignore_index, inplace=Fals
     return p.to(logits.dtype)
 
 
+def _check_tokens(tokens, vocab, ignore_index):
+    """Host check of the CPU path (the kernels report through the status word): which rows count."""
+    valid = tokens != ignore_index
+    if bool((valid & ((tokens < 0) | (tokens >= vocab))).any()):
+        raise IndexError(f"token outside the vocabulary of {vocab}")
+    return valid
+
+
+def token_logits(logits):
+    """The logits as the row kernels read them: themselves where their rows lie on two strides, else a copy."""
+    return contiguous(logits) if logits.is_cuda and N._row_map(logits) is None else logits
+
+
+def token_rows(logits, tokens, ignore_index, temperature, policy=None):
+    """Log-probabilities of `tokens` [...] under `logits` [..., V] / temperature (0 where ignored) and what the gradient
+    needs of the rows.  `policy` = (old, advantages, rows per advantage, ref or None, lowest ratio, highest ratio, KL
+    weight): also the clipped policy loss of every row and its derivative by the log-probability."""
+    if logits.is_cuda:
+        r = N.token_rows(logits, tokens, ignore_index, temperature, policy)
+        if r is not NotImplemented:
+            return r
+        _fell("token_rows")
+    acc = torch.float64 if logits.dtype == torch.float64 else _F32
+    valid = _check_tokens(tokens, logits.shape[-1], ignore_index)
+    z = logits.to(acc)
+    m = z.max(-1, keepdim=True).values
+    log_sum = torch.logsumexp((z - m) / temperature, -1, keepdim=True)
+    tok = torch.where(valid, tokens, torch.zeros_like(tokens)).long().unsqueeze(-1)
+    lp = ((z.gather(-1, tok) - m) / temperature - log_sum).squeeze(-1)
+    zero = torch.zeros_like(lp)
+    lp = torch.where(valid, lp, zero)
+    stats = torch.stack((m.reshape(-1), log_sum.reshape(-1) * math.log2(math.e)))
+    if policy is None:
+        return lp, stats
+    old, adv, div, ref, lo, hi, kl = policy
+    A = adv.reshape(-1).repeat_interleave(div).reshape(lp.shape).to(acc)
+    ratio = torch.exp(lp - old.reshape(lp.shape))
+    plain, clipped = -A * ratio, -A * ratio.clamp(lo, hi)
+    loss = torch.maximum(plain, clipped)
+    coef = torch.where(plain >= clipped, plain, zero)
+    coef = torch.where(torch.isnan(loss), loss, coef)
+    if ref is not None:
+        d = ref.reshape(lp.shape) - lp
+        e = torch.exp(d)
+        loss = loss + kl * (e - d - 1)
+        coef = coef + kl * (1 - e)
+    return lp, stats, torch.where(valid, loss, zero), torch.where(valid, coef, zero)
+
+
+def policy_sum(loss, tokens, vocab, ignore_index, mean):
+    """[sum (mean over the rows that count) of the rows' losses, the factor of their gradients]."""
+    if loss.is_cuda and loss.dtype == _F32:
+        return N.policy_sum(loss, tokens, vocab, ignore_index, mean)
+    n = int(((tokens != ignore_index) & (tokens >= 0) & (tokens < vocab)).sum())
+    f = 1.0 / n if mean and n else 1.0
+    return torch.stack(((loss.double().sum() * f).to(loss.dtype), torch.tensor(f, dtype=loss.dtype, device=loss.device)))
+
+
+def preference(lp, ref, beta, smoothing, mean, each):
+    """(loss per pair or None, loss, rewards [2 pairs], derivative of a pair's loss by every answer's sum [2 pairs])."""
+    if lp.is_cuda and lp.dtype == _F32:
+        return N.preference(lp, ref, beta, smoothing, mean, each)
+    n = ref.numel()
+    rewards = (beta * (lp.double().reshape(n, -1).sum(1) - ref.double())).to(lp.dtype)
+    h = rewards[:n // 2] - rewards[n // 2:]
+    lse = torch.log1p(torch.exp(-h.abs()))
+    loss = (1 - smoothing) * ((-h).clamp(min=0) + lse) + smoothing * (h.clamp(min=0) + lse)
+    g = beta * (smoothing - 1 / (1 + torch.exp(h)))
+    total = loss.double().sum()
+    total = (total / (n // 2) if mean and n else total).to(lp.dtype)
+    return loss if each else None, total, rewards, torch.cat((g, -g))
+
+
+def token_grad(logits, tokens, stats, ignore_index, temperature, base=None, base_div=1, g=None, g_div=1, g_mod=1,
+               dev_scale=None, scale=1.0):
+    """Gradient of the logits: row r's derivative by its token's log-probability is
+    base[r // base_div] * g[r // g_div % g_mod] * dev_scale * scale (None: 1); zero for ignored rows."""
+    if logits.is_cuda and logits.dtype != torch.float64:
+        return N.token_grad(logits, tokens, stats, ignore_index, temperature, base, base_div, g, g_div, g_mod, dev_scale, scale)
+    rows, V = tokens.numel(), logits.shape[-1]
+    r = torch.arange(rows, device=logits.device)
+    f = torch.full((rows,), scale, dtype=stats.dtype, device=logits.device)
+    for t, at in ((base, r // base_div), (g, r // g_div % g_mod), (dev_scale, r * 0)):
+        if t is not None:
+            f = f * t.reshape(-1)[at]
+    flat = tokens.reshape(-1)
+    valid = (flat != ignore_index) & (flat >= 0) & (flat < V)
+    f = torch.where(valid, f, torch.zeros_like(f)) / temperature
+    z = logits.reshape(rows, V).to(stats.dtype)
+    p = torch.exp2((z - stats[0, :, None]) * (math.log2(math.e) / temperature) - stats[1, :, None])
+    p.scatter_add_(1, torch.where(valid, flat, torch.zeros_like(flat)).long()[:, None], -torch.ones_like(f)[:, None])
+    d = torch.where((f == 0)[:, None], torch.zeros_like(p), p * -f[:, None])
+    return d.reshape(logits.shape).to(logits.dtype)
+
+
 # ============================== transformer pieces ===============================
 def swiglu_fwd(gate, up):
     if gate.is_cuda:
@@ -900,6 +995,53 @@ def sgd_step(params, grads, bufs, lr, momentum, weight_decay):
             g = g + weight_decay * p
         u.mul_(momentum).add_(g, alpha=1.0 - momentum)
         p.sub_(lr * u)
+
+
+def _newton_schulz_torch(x, steps, coefficients, eps):
+    a, b, c = coefficients
+    y = x if x.dtype == torch.float64 else x.to(_F32)
+    tall = y.shape[-2] > y.shape[-1]
+    y = y.transpose(-2, -1) if tall else y
+    y = y / (torch.linalg.vector_norm(y, dim=(-2, -1), keepdim=True, dtype=torch.float64) + eps).to(y.dtype)
+    for _ in range(steps):
+        A = y @ y.transpose(-2, -1)
+        y = a * y + (b * A + c * (A @ A)) @ y
+    return y.transpose(-2, -1) if tall else y
+
+
+def newton_schulz(x, steps, coefficients, eps, exponents):
+    """Orthogonalised matrices of x [batch, rows, cols], in its type."""
+    if x.is_cuda:
+        r = N.newton_schulz(contiguous(x), steps, coefficients, eps, exponents)
+        if r is not NotImplemented:
+            return r
+        _fell("newton_schulz")
+    return _newton_schulz_torch(x, steps, coefficients, eps).to(x.dtype).contiguous()
+
+
+def muon_step(params, grads, bufs, shape, lr, momentum, nesterov, weight_decay, scale, steps, coefficients, eps, exponents,
+              grad_scale=None, found_inf=None, dyn_lr=None):
+    """One Muon step, in place, on matrices of one shape; params / grads / bufs are lists of (tensor, index of the matrix
+    in the tensor's leading dimensions).  `grad_scale`, `found_inf`: as in `adamw_step`."""
+    if params[0][0].is_cuda:
+        r = N.muon_step(params, grads, bufs, shape, lr, momentum, nesterov, weight_decay, scale, steps, coefficients, eps,
+                        exponents, grad_scale, found_inf, dyn_lr)
+        if r is not NotImplemented:
+            return
+        _fell("muon_step")
+    if dyn_lr is not None:
+        raise RuntimeError("capturable optimizer state needs contiguous fp32 CUDA parameters and floating-point gradients")
+    if found_inf is not None and float(found_inf.item()) != 0.0:
+        return
+    for (p, i), (g, _), (u, _) in zip(params, grads, bufs):
+        p, g, u = (t.view(-1, *shape)[i] for t in (p, g, u))
+        g = g.to(u.dtype)
+        if grad_scale is not None:
+            g = g * grad_scale.to(g.dtype)
+        u.mul_(momentum).add_(g, alpha=1.0 - momentum)
+        y = momentum * u + (1.0 - momentum) * g if nesterov else u
+        o = _newton_schulz_torch(y, steps, coefficients, eps)
+        p.mul_(1.0 - lr * weight_decay).sub_((lr * scale * o).to(p.dtype))
 
 
 def unscale_and_check(grads, inv_scale, found_inf):

@@ -68,6 +68,11 @@ _SIGS = {
     "gb_index_put": "pp" + "d" + "ii" + "ppp" + "i" + "pp",
     "gb_cast_stack": "ppipip",
     "gb_masked_fill": "pp" + "d" + "ll" + "i" + "p", "gb_fill_elems": "pldip",
+    "gb_token_rows": "pppp" + "lllll" + "l" + "f" + "ppppp" + "l" + "fff" + "ii" + "pp",
+    "gb_policy_sum": "pp" + "lll" + "i" + "p" + "i" + "p", "gb_preference": "pp" + "ll" + "ff" + "i" + "pppp" + "p",
+    "gb_token_grad": "pppp" + "lllll" + "l" + "f" + "pl" + "pll" + "p" + "f" + "ii" + "p",
+    "gb_ns_workspace": "lllip", "gb_muon_momentum": "p" + "iiii" + "f" + "i" + "ppp" + "p",
+    "gb_newton_schulz": "pp" + "iiiii" + "fff" + "d" + "pp" + "fff" + "pp" + "pp" + "p",
 }
 
 _L = None
@@ -111,6 +116,26 @@ def _chk(rc, what):
         raise RuntimeError(f"{what} failed with code {rc}")
 
 
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+class _Here:
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        return False
+
+
+_here = _Here()
+
+
+def _on(dev):
+    """Launches inside go to `dev`, which may be another device than the current one."""
+    return _here if dev.index is None or dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+
+
 def _sms(dev):
     i = dev.index if dev.index is not None else torch.cuda.current_device()
     if i not in _sm_count:
@@ -142,7 +167,7 @@ def _raise_status(rec, what="native kernel"):
     if rec[0] == 4:
         raise IndexError(f"index out of range in a native kernel (site={rec[1]}: 1 row gather / embedding lookup, "
                          f"2 row scatter-add, 3 gather along a dim, 4 scatter along a dim, 5 indexed read, "
-                         f"6 indexed write; block={rec[2]}, index={rec[3]}); the access was skipped")
+                         f"6 indexed write, 7 token of a row of logits; block={rec[2]}, index={rec[3]}); the access was skipped")
     if rec[0] == 3 and rec[1] == 900:
         raise RuntimeError(f"{what}: expert-parallel receive buffer too small: this rank was sent {rec[3]} "
                            f"(tile-padded) rows; raise GENESIS_EP_CAPACITY (multiple of the balanced share)")
@@ -1850,3 +1875,150 @@ def masked_fill_(a, mask, value):
         _chk(lib().gb_masked_fill(a.data_ptr(), mask.data_ptr(), float(value), rows, inner, _ELEM_DT[a.dtype], _st()),
              "masked_fill")
     return a
+
+
+# =============================== losses on tokens' log-probabilities ===============================
+def _row_map(logits):
+    """(rows per outer step, outer stride, inner stride) of the rows of [..., V] logits, in elements, or None when they do
+    not lie on two strides or a row is not contiguous.  A `logits[:, :-1]` view does, so it is read in place."""
+    if logits.shape[-1] > 1 and logits.stride(-1) != 1:
+        return None
+    dims = []                                            # (size, stride) from the outermost, neighbours merged
+    for n, st in zip(logits.shape[:-1], logits.stride()[:-1]):
+        if n == 1:
+            continue
+        if dims and dims[-1][1] == n * st:
+            dims[-1] = (dims[-1][0] * n, st)
+        else:
+            dims.append((n, st))
+    if len(dims) > 2:
+        return None
+    if not dims:
+        return 1, 0, 0
+    if len(dims) == 1:
+        return dims[0][0], 0, dims[0][1]
+    return dims[1][0], dims[0][1], dims[1][1]
+
+
+_TOKEN_DT = (torch.int64, torch.int32)
+
+
+def token_rows(logits, tokens, ignore_index, temperature, policy=None):
+    """(log-probabilities, row statistics [2, rows]) of `tokens` under `logits` [..., V]; with `policy` =
+    (old, advantages, rows per advantage, ref or None, lowest ratio, highest ratio, KL weight) also (loss, derivative)."""
+    m = _row_map(logits)
+    if logits.dtype not in _FLOATS or m is None:
+        return NotImplemented
+    rows, dev = tokens.numel(), logits.device
+    lp = torch.empty(tokens.shape, dtype=F32, device=dev)
+    stats = torch.empty(2, rows, dtype=F32, device=dev)
+    old = adv = ref = loss = coef = None
+    div, lo, hi, kl = 1, 0.0, 0.0, 0.0
+    if policy is not None:
+        old, adv, div, ref, lo, hi, kl = policy
+        loss = torch.empty(tokens.shape, dtype=F32, device=dev)
+        coef = torch.empty(tokens.shape, dtype=F32, device=dev)
+    with _on(dev):
+        _chk(lib().gb_token_rows(logits.data_ptr(), tokens.data_ptr(), lp.data_ptr(), stats.data_ptr(), rows, logits.shape[-1],
+                                 *m, int(ignore_index), float(temperature), _ptr(old), _ptr(adv), _ptr(ref), _ptr(loss),
+                                 _ptr(coef), div, lo, hi, kl, _DT[logits.dtype], 1 if tokens.dtype == torch.int64 else 0,
+                                 status_tensor(dev).data_ptr(), _st()), "token_rows")
+    return (lp, stats) if policy is None else (lp, stats, loss, coef)
+
+
+def policy_sum(loss, tokens, vocab, ignore_index, mean):
+    """[sum of the rows' losses (over their number with `mean`), the factor of their gradients]."""
+    out = torch.empty(2, dtype=F32, device=loss.device)
+    with _on(loss.device):
+        _chk(lib().gb_policy_sum(loss.data_ptr(), tokens.data_ptr(), tokens.numel(), vocab, int(ignore_index), 1 if mean else 0,
+                                 out.data_ptr(), 1 if tokens.dtype == torch.int64 else 0, _st()), "policy_sum")
+    return out
+
+
+def preference(lp, ref, beta, smoothing, mean, each):
+    """(loss per pair or None, loss [], rewards [2 pairs], derivative by every answer's sum [2 pairs])."""
+    dev, n = lp.device, ref.numel()
+    loss = torch.empty(n // 2, dtype=F32, device=dev) if each else None
+    out = torch.empty((), dtype=F32, device=dev)
+    rewards = torch.empty(n, dtype=F32, device=dev)
+    gseq = torch.empty(n, dtype=F32, device=dev)
+    with _on(dev):
+        _chk(lib().gb_preference(lp.data_ptr(), ref.data_ptr(), n // 2, lp.numel() // n if n else 0, float(beta),
+                                 float(smoothing), 1 if mean else 0, _ptr(loss), out.data_ptr(), rewards.data_ptr(),
+                                 gseq.data_ptr(), _st()), "preference")
+    return loss, out, rewards, gseq
+
+
+def token_grad(logits, tokens, stats, ignore_index, temperature, base, base_div, g, g_div, g_mod, dev_scale, scale):
+    """Gradient of [..., V] logits; row r's derivative by its token's log-probability is
+    base[r // base_div] * g[r // g_div % g_mod] * dev_scale * scale (None: 1)."""
+    m = _row_map(logits)
+    out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    with _on(logits.device):
+        _chk(lib().gb_token_grad(logits.data_ptr(), tokens.data_ptr(), stats.data_ptr(), out.data_ptr(), tokens.numel(),
+                                 logits.shape[-1], *m, int(ignore_index), float(temperature), _ptr(base), base_div, _ptr(g),
+                                 g_div, g_mod, _ptr(dev_scale), float(scale), _DT[logits.dtype],
+                                 1 if tokens.dtype == torch.int64 else 0, _st()), "token_grad")
+    return out
+
+
+# =============================== orthogonalised updates ===============================
+def _ns_workspace(rows, cols, batch, with_y, dev):
+    size = ctypes.c_longlong()
+    lib().gb_ns_workspace(rows, cols, batch, 1 if with_y else 0, ctypes.addressof(size))
+    return torch.empty(size.value, dtype=torch.uint8, device=dev)
+
+
+def newton_schulz(x, steps, coefficients, eps, exponents):
+    """Orthogonalised matrices of contiguous x [batch, rows, cols], in its type."""
+    if x.dtype not in _FLOATS or not x.is_contiguous():
+        return NotImplemented
+    out = torch.empty_like(x)
+    batch, rows, cols = x.shape
+    per = _ns_batch(rows, cols)
+    ex = (ctypes.c_int * len(exponents))(*exponents)
+    with _on(x.device):
+        for i in range(0, batch, per):
+            n = min(per, batch - i)
+            ws = _ns_workspace(rows, cols, n, False, x.device)
+            _chk(lib().gb_newton_schulz(x[i].data_ptr(), out[i].data_ptr(), _DT[x.dtype], rows, cols, n, steps,
+                                        *coefficients, eps, ex, None, 0.0, 0.0, 0.0, None, None, ws.data_ptr(),
+                                        status_tensor(x.device).data_ptr(), _st()), "newton_schulz")
+    return out
+
+
+def _ns_batch(rows, cols):
+    """Matrices of one pass: the workspace holds 16 bytes per element of them, a GB or so is enough to fill the GPU."""
+    return max(1, min(4096, (1 << 28) // (rows * cols)))
+
+
+def muon_step(params, grads, bufs, shape, lr, momentum, nesterov, weight_decay, scale, steps, coefficients, eps, exponents,
+              grad_scale, found_inf, dyn_lr):
+    """One step on matrices of one shape.  params / grads / bufs: lists of (tensor, index of the matrix in it)."""
+    rows, cols = shape
+    for t, _ in params + bufs:
+        if t.dtype != F32 or not t.is_contiguous():
+            return NotImplemented
+    gdt = grads[0][0].dtype
+    if any(g.dtype != gdt or not g.is_contiguous() for g, _ in grads) or gdt not in _FLOATS:
+        return NotImplemented
+    dev = params[0][0].device
+    per = _ns_batch(rows, cols)
+    ex = (ctypes.c_int * len(exponents))(*exponents)
+
+    def at(pair):
+        return pair[0].data_ptr() + pair[1] * rows * cols * pair[0].element_size()
+
+    with _on(dev):
+        for i in range(0, len(params), per):
+            n = min(per, len(params) - i)
+            table = _meta([[at(x) for x in grads[i:i + n]], [at(x) for x in bufs[i:i + n]], [at(x) for x in params[i:i + n]]],
+                          n, dev)
+            ws = _ns_workspace(rows, cols, n, True, dev)
+            _chk(lib().gb_muon_momentum(table.data_ptr(), n, _DT[gdt], rows, cols, float(momentum), 1 if nesterov else 0,
+                                        _ptr(grad_scale), _ptr(found_inf), ws.data_ptr(), _st()), "muon_momentum")
+            _chk(lib().gb_newton_schulz(None, None, 0, rows, cols, n, steps, *coefficients, eps, ex,
+                                        table.data_ptr() + 16 * n, float(lr), float(weight_decay), float(scale),
+                                        _ptr(dyn_lr), _ptr(found_inf), ws.data_ptr(), status_tensor(dev).data_ptr(), _st()),
+                 "newton_schulz")
+    return True

@@ -1,3 +1,4 @@
 from .optimizer import Optimizer, SGD, Adam, AdamW
+from .muon import Muon, orthogonalize
 from . import lr_scheduler
 from . import adamw  # noqa: E402,F401
