@@ -14,9 +14,14 @@
 //
 // Work.  A and B are symmetric: only tiles on and below the diagonal are computed, the rest is written as their mirror
 // image by the same epilogue.  A step is three launches over all matrices of a batch, 128 x 128 tiles on persistent CTAs:
-//   warp 0 TMA producer, warp 1 issues tcgen05.mma, warps 2-9 epilogue; two accumulators in tensor memory.
+//   warp 0 TMA producer, warp 1 issues tcgen05.mma, warps 2-9 epilogue; four accumulators in tensor memory.
 // A stage holds both terms of both operands for 64 elements of the contraction (64 KB) and feeds three products, so an SM
 // reads 85 bytes a clock from L2 at the full tensor rate, as the single-product GEMM with tiles of 128 x 256 does.
+// Tiles too few to fill the GPU are shared by clusters of up to 8 CTAs, each with a part of the contraction.
+//
+// Sums.  The tensor cores round their accumulator towards zero, which adds up over a long contraction (4864 x 896: 1.6e-5 of
+// the result).  So an accumulator takes up 256 elements of the contraction and is then added, rounded to nearest, to the
+// sums that the epilogue's warps hold in registers; the products go on in the next of four accumulators meanwhile.
 #include "sm100_ptx.cuh"
 #include "common.cuh"
 
@@ -30,10 +35,13 @@ namespace ns {
 constexpr int BM = 128, BN = 128, BK = 64, STAGES = 3;
 constexpr int TILE_BYTES = 128 * 128;                 // 128 rows of 64 fp16, or 64 rows of 2 x 64
 constexpr int STAGE_BYTES = 4 * TILE_BYTES;           // hi and lo of both operands
-constexpr int BARRIER_OFFSET = STAGES * STAGE_BYTES;
-constexpr int SMEM_TOTAL = BARRIER_OFFSET + 1024;
-constexpr int PARTS = 64;                             // partial sums of squares per matrix
-constexpr int ACC_STRIDE = BN;
+constexpr int CHUNK_BYTES = 32 * 32 * 4;              // 32 x 32 results in fp32
+constexpr int SLAB_OFFSET = STAGES * STAGE_BYTES;     // one chunk per epilogue warp
+constexpr int BARRIER_OFFSET = SLAB_OFFSET + 8 * CHUNK_BYTES;
+constexpr int SMEM_TOTAL = BARRIER_OFFSET + 256;
+constexpr int PARTS = 256;                            // most partial sums of squares per matrix
+constexpr int ACCS = 4;                               // accumulators in tensor memory, BN columns each
+constexpr int DRAIN = 4;                              // stages that one accumulator takes up: see the header
 
 enum Mode : int { GRAM = 0, SQUARE = 1, APPLY = 2, APPLY_LAST = 3 };
 
@@ -49,10 +57,11 @@ struct Params {
   // APPLY_LAST: out[batch] in `out_dtype`, or the weights of an optimizer step through `weights`
   void* out;
   int out_dtype, tall;         // tall: the result goes out transposed, [n, m]
-  const long long* weights;    // [batch] addresses of fp32 weights, or null
-  float lr, decay, scale;      // w <- w (1 - lr decay) - lr scale o
+  const long long* weights;    // [batch] addresses of fp32 weights (+ 1 where the weight is tall), or null
+  float lr, decay, scale;      // w <- w (1 - lr decay) - lr o, or scale lr o where it is tall
   const float* dyn_lr;
   const float* found_inf;
+  int splits;                  // CTAs of a cluster that share a tile's contraction (1: whole tiles, persistent CTAs)
 };
 
 __device__ __forceinline__ void split(float x, __half& hi, __half& lo) {
@@ -60,36 +69,214 @@ __device__ __forceinline__ void split(float x, __half& hi, __half& lo) {
   lo = __float2half_rn(x - __half2float(hi));
 }
 
+// Byte offset of 16-byte unit `u` of row `r` of a 32 x 32 chunk in shared memory.  Eight neighbouring rows, and the eight
+// rows r, r + 4, .., put a unit into eight different bank groups: rows written lane by lane, read unit by unit, and
+// columns read four rows apart are all free of conflicts.
+__device__ __forceinline__ int chunk_at(int r, int u) { return r * 128 + ((u ^ r ^ (r >> 3)) & 7) * 16; }
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+}
+__device__ __forceinline__ float4 ld_peer(uint32_t addr, uint32_t rank) {
+  float4 v;
+  asm volatile("{\n\t.reg .u32 a;\n\tmapa.shared::cluster.u32 a, %4, %5;\n\tld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [a];\n\t}"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr), "r"(rank) : "memory");
+  return v;
+}
+
+__device__ __forceinline__ void store4(void* p, int dt, size_t i, const float* v, int n, bool whole) {
+  if (whole) {                                        // four elements, aligned
+    if (dt == DT_F32) *reinterpret_cast<float4*>(reinterpret_cast<float*>(p) + i) = make_float4(v[0], v[1], v[2], v[3]);
+    else *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(p) + i) = make_uint2(pack2(v[0], v[1], dt), pack2(v[2], v[3], dt));
+  } else {
+    for (int k = 0; k < n; ++k) store_from_float(p, dt, i + k, v[k]);
+  }
+}
+
+// What becomes of a 32 x 32 chunk of accumulators (rows row0.., columns col0.. of matrix z) that lies in shared memory.  A
+// lane takes four neighbouring columns of a row, eight lanes a row, so that memory sees whole 128-byte lines (64 of fp16).
 template <int MODE>
+struct Epilogue {
+  const Params& p;
+  int lane;
+  float keep, step;
+  bool skip, vec;              // vec: four elements of the result at a time
+  __device__ __forceinline__ Epilogue(const Params& q) : p(q), lane(threadIdx.x & 31), keep(1.f), step(0.f), skip(false), vec(false) {
+    if constexpr (MODE == APPLY_LAST) {
+      const float lr = p.dyn_lr != nullptr ? *p.dyn_lr : p.lr;
+      keep = 1.f - lr * p.decay;
+      step = lr;
+      skip = p.found_inf != nullptr && *p.found_inf != 0.f;
+      // (rows of a result of n, or m, elements start on a boundary of four; weights are looked at one by one)
+      vec = ((p.tall ? p.m : p.n) & 3) == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0;
+    }
+  }
+  __device__ __forceinline__ void run(const uint8_t* chunk, int z, int row0, int col0, bool mirror) const {
+    const int cols = MODE == GRAM || MODE == SQUARE ? p.m : p.n;
+    const int u = lane & 7, col = col0 + 4 * u;
+    if constexpr (MODE == GRAM || MODE == SQUARE) {
+      const size_t plane = (size_t)p.m * p.lda;
+      __half* hi = p.dst + (size_t)z * 2 * plane;
+      const __half* ah = p.a_planes + (size_t)z * 2 * plane;
+#pragma unroll
+      for (int it = 0; it < 8; ++it) {
+        const int r = 4 * it + (lane >> 3), row = row0 + r;
+        if (row < p.m && col < cols) {
+          const float4 a = *reinterpret_cast<const float4*>(chunk + chunk_at(r, u));
+          float v[4] = {a.x * p.f_acc, a.y * p.f_acc, a.z * p.f_acc, a.w * p.f_acc};
+          const size_t o = (size_t)row * p.lda + col;
+          if constexpr (MODE == SQUARE) add_a(v, ah + o, plane);
+          put(hi + o, plane, v);
+        }
+      }
+      if (mirror) {
+        // the transposed chunk: row `col0 + r` of the result, its columns row0 + 4 u .. + 3
+        const int i0 = row0 + 4 * u;
+#pragma unroll
+        for (int it = 0; it < 8; ++it) {
+          const int r = 4 * it + (lane >> 3), row = col0 + r;
+          if (row < cols && i0 < p.m) {
+            float v[4];
+            column(chunk, r, u, v);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[k] *= p.f_acc;
+            const size_t o = (size_t)row * p.lda + i0;
+            if constexpr (MODE == SQUARE) add_a(v, ah + o, plane);
+            put(hi + o, plane, v);
+          }
+        }
+      }
+    } else {
+      bool across = false;                                       // the result is the transpose
+      if constexpr (MODE == APPLY_LAST) across = p.weights != nullptr ? (p.weights[z] & 1) != 0 : p.tall != 0;
+      if (!across) {
+#pragma unroll
+        for (int it = 0; it < 8; ++it) {
+          const int r = 4 * it + (lane >> 3), row = row0 + r;
+          if (row < p.m && col < cols) {
+            const float4 a = *reinterpret_cast<const float4*>(chunk + chunk_at(r, u));
+            float* x = p.x + ((size_t)z * p.m + row) * p.ldx + col;
+            const float4 o = *reinterpret_cast<const float4*>(x);
+            float v[4] = {fmaf(a.x, p.f_acc, o.x * p.f_a), fmaf(a.y, p.f_acc, o.y * p.f_a), fmaf(a.z, p.f_acc, o.z * p.f_a),
+                          fmaf(a.w, p.f_acc, o.w * p.f_a)};
+            if constexpr (MODE == APPLY) {
+              *reinterpret_cast<float4*>(x) = make_float4(v[0], v[1], v[2], v[3]);
+              const size_t plane = (size_t)p.m * p.ldx;
+#pragma unroll
+              for (int k = 0; k < 4; ++k) v[k] *= p.next_scale;
+              put(p.dst + (size_t)z * 2 * plane + (size_t)row * p.ldx + col, plane, v);
+            } else {
+              result(z, (size_t)row * p.n + col, v, min(4, cols - col), step);
+            }
+          }
+        }
+      } else {
+        // X is read by rows as above and meets its accumulators in shared memory; then columns go out as rows
+        float4 o[8];
+#pragma unroll
+        for (int it = 0; it < 8; ++it) {
+          const int row = row0 + 4 * it + (lane >> 3);
+          o[it] = row < p.m && col < cols ? *reinterpret_cast<const float4*>(p.x + ((size_t)z * p.m + row) * p.ldx + col)
+                                          : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+#pragma unroll
+        for (int it = 0; it < 8; ++it) {
+          float4* a = reinterpret_cast<float4*>(const_cast<uint8_t*>(chunk) + chunk_at(4 * it + (lane >> 3), u));
+          const float4 b = *a;
+          *a = make_float4(fmaf(b.x, p.f_acc, o[it].x * p.f_a), fmaf(b.y, p.f_acc, o[it].y * p.f_a),
+                           fmaf(b.z, p.f_acc, o[it].z * p.f_a), fmaf(b.w, p.f_acc, o[it].w * p.f_a));
+        }
+        __syncwarp();
+        const int i0 = row0 + 4 * u;
+#pragma unroll
+        for (int it = 0; it < 8; ++it) {
+          const int r = 4 * it + (lane >> 3), row = col0 + r;
+          if (row < cols && i0 < p.m) {
+            float v[4];
+            column(chunk, r, u, v);
+            result(z, (size_t)row * p.m + i0, v, min(4, p.m - i0), step * p.scale);
+          }
+        }
+      }
+    }
+  }
+  // four rows 4 u .. of column `c` of the chunk
+  __device__ __forceinline__ void column(const uint8_t* chunk, int c, int u, float (&v)[4]) const {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = *reinterpret_cast<const float*>(chunk + chunk_at(4 * u + k, c >> 2) + (c & 3) * 4);
+  }
+  __device__ __forceinline__ void add_a(float (&v)[4], const __half* a, size_t plane) const {
+    const uint2 x = *reinterpret_cast<const uint2*>(a), y = *reinterpret_cast<const uint2*>(a + plane);
+    const float2 x0 = __half22float2(*reinterpret_cast<const __half2*>(&x.x)), x1 = __half22float2(*reinterpret_cast<const __half2*>(&x.y));
+    const float2 y0 = __half22float2(*reinterpret_cast<const __half2*>(&y.x)), y1 = __half22float2(*reinterpret_cast<const __half2*>(&y.y));
+    v[0] = fmaf(x0.x + y0.x, p.f_a, v[0]); v[1] = fmaf(x0.y + y0.y, p.f_a, v[1]);
+    v[2] = fmaf(x1.x + y1.x, p.f_a, v[2]); v[3] = fmaf(x1.y + y1.y, p.f_a, v[3]);
+  }
+  // both terms of four elements; the pitch is a multiple of 8, so what lies past the last column is padding
+  __device__ __forceinline__ void put(__half* hi, size_t plane, const float (&v)[4]) const {
+    uint2 h, l;
+    __half* h4 = reinterpret_cast<__half*>(&h);
+    __half* l4 = reinterpret_cast<__half*>(&l);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) split(v[k], h4[k], l4[k]);
+    *reinterpret_cast<uint2*>(hi) = h;
+    *reinterpret_cast<uint2*>(hi + plane) = l;
+  }
+  // up to four neighbouring elements of the result
+  __device__ __forceinline__ void result(int z, size_t at, const float (&v)[4], int n, float step) const {
+    if (p.weights != nullptr) {
+      if (skip) return;
+      float* w = reinterpret_cast<float*>(p.weights[z] & ~1ll) + at;
+      if (n == 4 && (reinterpret_cast<uintptr_t>(w) & 15) == 0) {
+        float4 o = *reinterpret_cast<const float4*>(w);
+        o.x = fmaf(o.x, keep, -step * v[0]); o.y = fmaf(o.y, keep, -step * v[1]);
+        o.z = fmaf(o.z, keep, -step * v[2]); o.w = fmaf(o.w, keep, -step * v[3]);
+        *reinterpret_cast<float4*>(w) = o;
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (k < n) w[k] = fmaf(w[k], keep, -step * v[k]);
+      }
+    } else {
+      store4(p.out, p.out_dtype, (size_t)z * p.m * p.n + at, v, n, n == 4 && vec);
+    }
+  }
+};
+
+template <int MODE, bool SPLIT>
 __global__ void __launch_bounds__(320, 1)
 ns_product_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_constant__ CUtensorMap tmapB, const Params p) {
   constexpr bool SYM = MODE == GRAM || MODE == SQUARE;
   constexpr bool B_MN = !SYM;                           // X as the right operand: its rows run along the contraction
   extern __shared__ __align__(1024) uint8_t smem[];
-  if (status_poisoned(p.status)) return;
-  if ((reinterpret_cast<uintptr_t>(smem) & 1023) != 0) {
-    if (threadIdx.x == 0) report_error(p.status, GB_ERR_BAD_ARG, 5, 0);
-    return;
-  }
   uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + BARRIER_OFFSET);
   uint64_t* empty_bar = full_bar + STAGES;
   uint64_t* tmem_full = empty_bar + STAGES;
-  uint64_t* tmem_empty = tmem_full + 2;
-  uint32_t* tmem_base_slot = reinterpret_cast<uint32_t*>(tmem_empty + 2);
+  uint64_t* tmem_empty = tmem_full + ACCS;
+  uint32_t* tmem_base_slot = reinterpret_cast<uint32_t*>(tmem_empty + ACCS);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_base_slot + 1);
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
   const int lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], 1); }
-    for (int a = 0; a < 2; ++a) { mbar_init(&tmem_full[a], 1); mbar_init(&tmem_empty[a], 8); }
-    *abort_flag = 0;
+    for (int a = 0; a < ACCS; ++a) { mbar_init(&tmem_full[a], 1); mbar_init(&tmem_empty[a], 8); }
+    // after an error no work is done, but every CTA of a cluster comes to its barriers
+    const bool aligned = (smem_u32(smem) & 1023) == 0;
+    if (!aligned) report_error(p.status, GB_ERR_BAD_ARG, 5, 0);
+    *abort_flag = !aligned || status_poisoned(p.status) ? 1 : 0;
     mbar_fence_init();
     tma_prefetch_desc(&tmapA);
     tma_prefetch_desc(&tmapB);
   }
   if (warp == 1) {
-    tmem_alloc(tmem_base_slot, 2 * ACC_STRIDE);
+    tmem_alloc(tmem_base_slot, ACCS * BN);
     tmem_relinquish();
   }
   tc_fence_before_sync();
@@ -100,7 +287,11 @@ ns_product_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_consta
   const int tm = (p.m + BM - 1) / BM, tn = (p.n + BN - 1) / BN;
   const int per = SYM ? tm * (tm + 1) / 2 : tm * tn;
   const long long total = (long long)per * p.batch;
-  const int K = MODE == GRAM ? p.n : p.m;
+  const int kblocks = ((MODE == GRAM ? p.n : p.m) + BK - 1) / BK;
+  // this CTA's tiles and its part of their contraction, in blocks of BK
+  const int splits = SPLIT ? p.splits : 1, rank = SPLIT ? (int)cluster_rank() : 0;
+  const long long first = blockIdx.x / splits, stride = gridDim.x / splits;
+  const int kb0 = kblocks * rank / splits, kb1 = kblocks * (rank + 1) / splits;
   // tile of matrix z: (mi, ni); the symmetric modes walk the lower triangle row by row
   auto decode = [&](long long t, int& mi, int& ni, int& z) {
     z = (int)(t / per);
@@ -120,11 +311,11 @@ ns_product_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_consta
     // =========================== TMA producer ===========================
     if (elect_one()) {
       uint32_t it = 0;
-      for (long long t = blockIdx.x; t < total && !*abort_flag; t += gridDim.x) {
+      for (long long t = first; t < total && !*abort_flag; t += stride) {
         int mi, ni, z;
         decode(t, mi, ni, z);
-        for (int k0 = 0; k0 < K; k0 += BK, ++it) {
-          const int s = it % STAGES;
+        for (int kb = kb0; kb < kb1; ++kb, ++it) {
+          const int s = it % STAGES, k0 = kb * BK;
           if (!mbar_wait(&empty_bar[s], ((it / STAGES) & 1) ^ 1, abort_flag, p.status, 110)) break;
           uint8_t* st = smem + s * STAGE_BYTES;
           mbar_expect_tx(&full_bar[s], STAGE_BYTES);
@@ -144,177 +335,130 @@ ns_product_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_consta
       }
       if (*abort_flag) drain_copies(full_bar, STAGES, it);
     }
+    __syncwarp();
   } else if (warp == 1) {
     // =========================== MMA issuer (converged warp, one elected lane) ===========================
     const uint32_t idesc = make_idesc(0u, 0u, B_MN ? 1u : 0u, BM, BN);
-    uint32_t it = 0, tile_no = 0;
-    for (long long t = blockIdx.x; t < total; t += gridDim.x) {
-      const uint32_t acc = tile_no & 1, acc_ph = (tile_no >> 1) & 1;
-      if (!__all_sync(0xffffffffu, mbar_wait(&tmem_empty[acc], acc_ph ^ 1, abort_flag, p.status, 210))) break;
-      tc_fence_after_sync();
-      const uint32_t d_tmem = tmem_base + acc * ACC_STRIDE;
-      bool ok = true;
-      for (int k0 = 0; k0 < K; k0 += BK, ++it) {
-        const int s = it % STAGES;
-        if (!__all_sync(0xffffffffu, mbar_wait(&full_bar[s], (it / STAGES) & 1, abort_flag, p.status, 211))) { ok = false; break; }
+    uint32_t it = 0, drains = 0;
+    bool ok = !*abort_flag;
+    ok = __all_sync(0xffffffffu, ok);
+    for (long long t = first; t < total && ok; t += stride) {
+      for (int kb = kb0; kb < kb1 && ok; kb += DRAIN, ++drains) {
+        const uint32_t acc = drains % ACCS;
+        if (!__all_sync(0xffffffffu, mbar_wait(&tmem_empty[acc], ((drains / ACCS) & 1) ^ 1, abort_flag, p.status, 210))) { ok = false; break; }
         tc_fence_after_sync();
-        const uint32_t a_addr = smem_u32(smem + s * STAGE_BYTES), b_addr = a_addr + 2 * TILE_BYTES;
-        const uint64_t da = make_smem_desc(a_addr, 16, 1024);
-        const uint64_t db = B_MN ? make_smem_desc(b_addr, BK * 128, 1024) : make_smem_desc(b_addr, 16, 1024);
-        if (elect_one()) {
+        const uint32_t d_tmem = tmem_base + acc * BN;
+        const int end = min(kb + DRAIN, kb1);
+        for (int k = kb; k < end; ++k, ++it) {
+          const int s = it % STAGES;
+          if (!__all_sync(0xffffffffu, mbar_wait(&full_bar[s], (it / STAGES) & 1, abort_flag, p.status, 211))) { ok = false; break; }
+          tc_fence_after_sync();
+          const uint32_t a_addr = smem_u32(smem + s * STAGE_BYTES), b_addr = a_addr + 2 * TILE_BYTES;
+          const uint64_t da = make_smem_desc(a_addr, 16, 1024);
+          const uint64_t db = B_MN ? make_smem_desc(b_addr, BK * 128, 1024) : make_smem_desc(b_addr, 16, 1024);
+          if (elect_one()) {
 #pragma unroll
-          for (int kk = 0; kk < BK / 16; ++kk) {
-            const uint64_t a = da + kk * 2, b = db + (B_MN ? kk * 128 : kk * 2);      // (16-byte units)
-            constexpr uint64_t LO = TILE_BYTES / 16;
-            umma_f16(d_tmem, a, b, idesc, (k0 == 0 && kk == 0) ? 0u : 1u);
-            umma_f16(d_tmem, a, b + LO, idesc, 1u);
-            umma_f16(d_tmem, a + LO, b, idesc, 1u);
+            for (int kk = 0; kk < BK / 16; ++kk) {
+              const uint64_t a = da + kk * 2, b = db + (B_MN ? kk * 128 : kk * 2);      // (16-byte units)
+              constexpr uint64_t LO = TILE_BYTES / 16;
+              umma_f16(d_tmem, a, b + LO, idesc, (k == kb && kk == 0) ? 0u : 1u);
+              umma_f16(d_tmem, a + LO, b, idesc, 1u);
+              umma_f16(d_tmem, a, b, idesc, 1u);
+            }
+            umma_commit(&empty_bar[s]);
           }
-          umma_commit(&empty_bar[s]);
+          __syncwarp();
         }
-        __syncwarp();
+        if (ok) {
+          if (elect_one()) umma_commit(&tmem_full[acc]);
+          __syncwarp();
+        }
       }
-      if (!ok) break;
-      if (elect_one()) umma_commit(&tmem_full[acc]);
-      __syncwarp();
-      ++tile_no;
     }
     __syncwarp();
   } else {
     // =========================== epilogue: 8 warps, 32 rows x 64 columns each ===========================
     const int q = warp & 3, half = (warp - 2) >> 2;
-    uint32_t tile_no = 0;
-    float keep = 0.f, step = 0.f;
-    bool skip = false;
-    if constexpr (MODE == APPLY_LAST) {
-      const float lr = p.dyn_lr != nullptr ? *p.dyn_lr : p.lr;
-      keep = 1.f - lr * p.decay;
-      step = lr * p.scale;
-      skip = p.found_inf != nullptr && *p.found_inf != 0.f;
-    }
-    for (long long t = blockIdx.x; t < total && !*abort_flag; t += gridDim.x) {
+    uint8_t* slab = smem + SLAB_OFFSET + (warp - 2) * CHUNK_BYTES;
+    const Epilogue<MODE> epi(p);
+    uint32_t drains = 0;
+    bool ok = true;
+    for (long long t = first; t < total; t += stride) {
       int mi, ni, z;
       decode(t, mi, ni, z);
-      const uint32_t acc = tile_no & 1, acc_ph = (tile_no >> 1) & 1;
-      if (!__all_sync(0xffffffffu, mbar_wait(&tmem_full[acc], acc_ph, abort_flag, p.status, 310))) break;
-      tc_fence_after_sync();
-      const int row = mi * BM + q * 32 + lane;
-      const int cols = SYM ? p.m : p.n;
-#pragma unroll 1
-      for (int c = half * 64; c < half * 64 + 64; c += 32) {
-        const int col0 = ni * BN + c;
-        __syncwarp();                                   // (the lanes part below where rows or columns end)
-        uint32_t r[32];
-        tmem_ld_32x32b_x32(tmem_base + ((uint32_t)(q * 32) << 16) + acc * ACC_STRIDE + c, r);
-        tmem_ld_wait();
-        if (row >= p.m || col0 >= cols) continue;
-        float v[32];
-        if constexpr (SYM) {
-          const size_t plane = (size_t)p.m * p.lda, base = (size_t)z * 2 * plane;
-          __half* hi = p.dst + base;
-          __half* lo = hi + plane;
+      float v[2][32];
 #pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]) * p.f_acc;
-          if constexpr (MODE == SQUARE) {
-            const __half* ah = p.a_planes + base + (size_t)row * p.lda + col0;
-            const __half* al = ah + plane;
+      for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-              if (col0 + 8 * g < cols) {
-                const uint4 x = *reinterpret_cast<const uint4*>(ah + 8 * g), y = *reinterpret_cast<const uint4*>(al + 8 * g);
-                const __half2* xh = reinterpret_cast<const __half2*>(&x);
-                const __half2* yh = reinterpret_cast<const __half2*>(&y);
+        for (int j = 0; j < 32; ++j) v[h][j] = 0.f;
+      for (int kb = kb0; kb < kb1; kb += DRAIN, ++drains) {
+        const uint32_t acc = drains % ACCS;
+        if (!__all_sync(0xffffffffu, mbar_wait(&tmem_full[acc], (drains / ACCS) & 1, abort_flag, p.status, 310))) { ok = false; break; }
+        tc_fence_after_sync();
+        const uint32_t at = tmem_base + ((uint32_t)(q * 32) << 16) + acc * BN + half * 64;
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                  const float2 f = __half22float2(xh[k]), e = __half22float2(yh[k]);
-                  v[8 * g + 2 * k] = fmaf(f.x + e.x, p.f_a, v[8 * g + 2 * k]);
-                  v[8 * g + 2 * k + 1] = fmaf(f.y + e.y, p.f_a, v[8 * g + 2 * k + 1]);
-                }
-              }
-            }
-          }
+        for (int h = 0; h < 2; ++h) {
+          uint32_t r[32];
+          tmem_ld_32x32b_x32(at + 32 * h, r);
+          tmem_ld_wait();
 #pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            if (col0 + 8 * g < cols) {                  // (the pitch is a multiple of 8: whole vectors fit)
-              uint4 oh, ol;
-              __half* h8 = reinterpret_cast<__half*>(&oh);
-              __half* l8 = reinterpret_cast<__half*>(&ol);
+          for (int j = 0; j < 32; ++j) v[h][j] += __uint_as_float(r[j]);
+        }
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&tmem_empty[acc]);
+      }
+      if (!ok) break;
 #pragma unroll
-              for (int k = 0; k < 8; ++k) split(v[8 * g + k], h8[k], l8[k]);
-              *reinterpret_cast<uint4*>(hi + (size_t)row * p.lda + col0 + 8 * g) = oh;
-              *reinterpret_cast<uint4*>(lo + (size_t)row * p.lda + col0 + 8 * g) = ol;
-              if (mi != ni) {
+      for (int h = 0; h < 2; ++h) {
+        // a part of the contraction waits in this CTA's stages, which all products have been read from by now
+        uint8_t* at = SPLIT ? smem + ((warp - 2) * 2 + h) * CHUNK_BYTES : slab;
+        __syncwarp();                                   // (the chunk before has been read)
 #pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                  if (col0 + 8 * g + k < cols) {
-                    hi[(size_t)(col0 + 8 * g + k) * p.lda + row] = h8[k];
-                    lo[(size_t)(col0 + 8 * g + k) * p.lda + row] = l8[k];
-                  }
-                }
-              }
-            }
-          }
-        } else {
-          float* x = p.x + ((size_t)z * p.m + row) * p.ldx + col0;
-#pragma unroll
-          for (int g = 0; g < 8; ++g) {
-            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (col0 + 4 * g < cols) o = *reinterpret_cast<const float4*>(x + 4 * g);
-            v[4 * g] = fmaf(__uint_as_float(r[4 * g]), p.f_acc, o.x * p.f_a);
-            v[4 * g + 1] = fmaf(__uint_as_float(r[4 * g + 1]), p.f_acc, o.y * p.f_a);
-            v[4 * g + 2] = fmaf(__uint_as_float(r[4 * g + 2]), p.f_acc, o.z * p.f_a);
-            v[4 * g + 3] = fmaf(__uint_as_float(r[4 * g + 3]), p.f_acc, o.w * p.f_a);
-          }
-          if constexpr (MODE == APPLY) {
-            const size_t plane = (size_t)p.m * p.ldx;
-            __half* hi = p.dst + (size_t)z * 2 * plane + (size_t)row * p.ldx + col0;
-            __half* lo = hi + plane;
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-              if (col0 + 8 * g < cols) {
-                uint4 oh, ol;
-                __half* h8 = reinterpret_cast<__half*>(&oh);
-                __half* l8 = reinterpret_cast<__half*>(&ol);
-#pragma unroll
-                for (int k = 0; k < 8; ++k) split(v[8 * g + k] * p.next_scale, h8[k], l8[k]);
-                *reinterpret_cast<uint4*>(hi + 8 * g) = oh;
-                *reinterpret_cast<uint4*>(lo + 8 * g) = ol;
-                *reinterpret_cast<float4*>(x + 8 * g) = make_float4(v[8 * g], v[8 * g + 1], v[8 * g + 2], v[8 * g + 3]);
-                *reinterpret_cast<float4*>(x + 8 * g + 4) = make_float4(v[8 * g + 4], v[8 * g + 5], v[8 * g + 6], v[8 * g + 7]);
-              }
-            }
-          } else {
-            // element (row, col) of X is (col, row) of a tall result
-            const size_t si = p.tall ? 1 : p.n, sj = p.tall ? p.m : 1;
-            const size_t at = (size_t)row * si + (size_t)col0 * sj;
-            if (p.weights != nullptr) {
-              float* w = reinterpret_cast<float*>(p.weights[z]) + at;
-              if (!skip) {
-#pragma unroll
-                for (int j = 0; j < 32; ++j)
-                  if (col0 + j < cols) w[j * sj] = fmaf(w[j * sj], keep, -step * v[j]);
-              }
-            } else {
-              const size_t o = (size_t)z * p.m * p.n + at;
-#pragma unroll
-              for (int j = 0; j < 32; ++j)
-                if (col0 + j < cols) store_from_float(p.out, p.out_dtype, o + j * sj, v[j]);
-            }
-          }
+        for (int u = 0; u < 8; ++u)
+          *reinterpret_cast<float4*>(at + chunk_at(lane, u)) = make_float4(v[h][4 * u], v[h][4 * u + 1], v[h][4 * u + 2], v[h][4 * u + 3]);
+        __syncwarp();
+        if constexpr (!SPLIT) {
+          const int col0 = ni * BN + half * 64 + h * 32;
+          epi.run(slab, z, mi * BM + q * 32, col0, SYM && mi != ni);
         }
       }
-      tc_fence_before_sync();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&tmem_empty[acc]);
-      ++tile_no;
     }
   }
 
+  if constexpr (SPLIT) {
+    // the parts of a tile meet: rank k adds up chunks k, k + splits, .., in the order of the ranks, one warp each
+    tc_fence_before_sync();
+    __syncthreads();
+    cluster_barrier();
+    const int c = rank + (warp - 2) * splits;
+    if (warp >= 2 && c < 16 && !*abort_flag) {
+      uint8_t* slab = smem + SLAB_OFFSET + (warp - 2) * CHUNK_BYTES;
+#pragma unroll
+      for (int it = 0; it < 8; ++it) {
+        const int off = chunk_at(4 * it + (lane >> 3), lane & 7);
+        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int k = 0; k < splits; ++k) {
+          const float4 o = ld_peer(smem_u32(smem) + c * CHUNK_BYTES + off, k);
+          sum.x += o.x; sum.y += o.y; sum.z += o.z; sum.w += o.w;
+        }
+        *reinterpret_cast<float4*>(slab + off) = sum;
+      }
+      __syncwarp();
+      int mi, ni, z;
+      decode(first, mi, ni, z);
+      const int w = (c >> 1) + 2;                        // the warp whose chunk this was
+      const int q = w & 3, col0 = ni * BN + ((w - 2) >> 2) * 64 + (c & 1) * 32;
+      const Epilogue<MODE> epi(p);
+      epi.run(slab, z, mi * BM + q * 32, col0, SYM && mi != ni);
+    }
+    cluster_barrier();                                   // nobody leaves while its part may still be read
+  }
   tc_fence_before_sync();
   __syncthreads();
   if (warp == 1) {
     tc_fence_after_sync();
-    tmem_dealloc(tmem_base, 2 * ACC_STRIDE);
+    tmem_dealloc(tmem_base, ACCS * BN);
   }
 }
 
@@ -329,14 +473,39 @@ __device__ __forceinline__ double block_sum256(double v, double* sh) {
   return v;
 }
 
-// Partial sums of squares, in 64 bits: 32 would overflow or vanish at half the exponent range of the elements
+__device__ __forceinline__ float4 load4(const void* p, int dt, size_t i) {
+  if (dt == DT_F32) return *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p) + i);
+  const uint2 w = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint16_t*>(p) + i);
+  return make_float4(half_bits_to_float((uint16_t)w.x, dt), half_bits_to_float((uint16_t)(w.x >> 16), dt),
+                     half_bits_to_float((uint16_t)w.y, dt), half_bits_to_float((uint16_t)(w.y >> 16), dt));
+}
+__device__ __forceinline__ bool aligned4(const void* p, int dt) {
+  return (reinterpret_cast<uintptr_t>(p) & (dt == DT_F32 ? 15 : 7)) == 0;
+}
+// (the squares in 64 bits: 32 would overflow or vanish at half the exponent range of the elements)
+__device__ __forceinline__ double square4(float4 v) {
+  return ((double)v.x * v.x + (double)v.y * v.y) + ((double)v.z * v.z + (double)v.w * v.w);
+}
+
+// Partial sums of squares of every matrix: gridDim.x of them, in an order that depends on the sizes alone
 __global__ void __launch_bounds__(256)
 ns_norm_kernel(const void* __restrict__ src, int dt, long long numel, double* __restrict__ partial) {
   __shared__ double sh[8];
-  const size_t base = (size_t)blockIdx.y * numel;
+  const void* p = reinterpret_cast<const uint8_t*>(src) + (size_t)blockIdx.y * numel * (dt == DT_F32 ? 4 : 2);
+  const long long step = 256ll * gridDim.x, me = (long long)blockIdx.x * 256 + threadIdx.x;
   double s = 0.0;
-  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < numel; i += 256 * PARTS) {
-    const double x = (double)load_as_float(src, dt, base + i);
+  const long long nv = aligned4(p, dt) ? numel / 4 : 0;
+  long long i = me;
+  for (; i + 3 * step < nv; i += 4 * step) {
+    float4 v[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = load4(p, dt, 4 * (i + k * step));
+#pragma unroll
+    for (int k = 0; k < 4; ++k) s += square4(v[k]);
+  }
+  for (; i < nv; i += step) s += square4(load4(p, dt, 4 * i));
+  for (i = 4 * nv + me; i < numel; i += step) {
+    const double x = (double)load_as_float(p, dt, i);
     s += x * x;
   }
   s = block_sum256(s, sh);
@@ -354,69 +523,149 @@ muon_momentum_kernel(const long long* __restrict__ table, int batch, int grad_dt
   const int z = blockIdx.y;
   const void* g = reinterpret_cast<const void*>(table[z]);
   float* u = reinterpret_cast<float*>(table[batch + z]);
-  const float gs = grad_scale != nullptr ? *grad_scale : 1.f;
+  float* yz = y + (size_t)z * numel;
+  const float gs = grad_scale != nullptr ? *grad_scale : 1.f, nu = 1.f - mu;
   const bool skip = found_inf != nullptr && *found_inf != 0.f;      // the step is cancelled: momentum stays as it is
   double s = 0.0;
-  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < numel; i += 256 * PARTS) {
-    const float gi = skip ? 0.f : load_as_float(g, grad_dt, i) * gs;
-    const float ui = mu * u[i] + (1.f - mu) * gi;
-    if (!skip) u[i] = ui;
-    const float yi = nesterov ? mu * ui + (1.f - mu) * gi : ui;
-    y[(size_t)z * numel + i] = yi;
+  const long long step = 256ll * gridDim.x, me = (long long)blockIdx.x * 256 + threadIdx.x;
+  auto update = [&](float g1, float& u1) {
+    const float gi = g1 * gs;
+    u1 = mu * u1 + nu * gi;
+    return nesterov ? mu * u1 + nu * gi : u1;
+  };
+  const bool vec = aligned4(g, grad_dt) && ((reinterpret_cast<uintptr_t>(u) | reinterpret_cast<uintptr_t>(yz)) & 15) == 0;
+  const long long nv = skip ? 0 : (vec ? numel / 4 : 0), n = skip ? 0 : numel;
+  auto four = [&](float4 gv, float4 uv, long long i) {
+    float4 o;
+    o.x = update(gv.x, uv.x); o.y = update(gv.y, uv.y); o.z = update(gv.z, uv.z); o.w = update(gv.w, uv.w);
+    *reinterpret_cast<float4*>(u + 4 * i) = uv;
+    *reinterpret_cast<float4*>(yz + 4 * i) = o;
+    s += square4(o);
+  };
+  long long i = me;
+  for (; i + step < nv; i += 2 * step) {
+    const float4 g0 = load4(g, grad_dt, 4 * i), g1 = load4(g, grad_dt, 4 * (i + step));
+    const float4 u0 = *reinterpret_cast<const float4*>(u + 4 * i), u1 = *reinterpret_cast<const float4*>(u + 4 * (i + step));
+    four(g0, u0, i);
+    four(g1, u1, i + step);
+  }
+  if (i < nv) four(load4(g, grad_dt, 4 * i), *reinterpret_cast<const float4*>(u + 4 * i), i);
+  for (i = 4 * nv + me; i < n; i += step) {
+    float ui = u[i];
+    const float yi = update(load_as_float(g, grad_dt, i), ui);
+    u[i] = ui;
+    yz[i] = yi;
     s += (double)yi * (double)yi;
   }
   s = block_sum256(s, sh);
   if (threadIdx.x == 0) partial[z * PARTS + blockIdx.x] = s;
 }
 
-// X = G / (|G| + eps), in 32 bits and as fp16 terms, transposed where G [rows, cols] is tall
+// X = G / (|G| + eps), in 32 bits and as fp16 terms; a tall G [n, m] is transposed on the way.  A block: 32 x 128 of X.
 __global__ void __launch_bounds__(256)
-ns_prepare_kernel(const void* __restrict__ src, int dt, int rows, int cols, int tall, const double* __restrict__ partial,
-                  double eps, float scale, float* __restrict__ x, __half* __restrict__ planes, int ldx) {
-  __shared__ float tile[32][33];
-  __shared__ double inv;
-  const int z = blockIdx.z;
-  if (threadIdx.x == 0) {
-    double s = 0.0;
-    for (int i = 0; i < PARTS; ++i) s += partial[z * PARTS + i];
-    inv = 1.0 / (sqrt(s) + eps);
-  }
-  __syncthreads();
-  const int r0 = blockIdx.y * 32, c0 = blockIdx.x * 32;
-  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-#pragma unroll
-  for (int k = 0; k < 32; k += 8) {
-    const int r = r0 + ty + k, c = c0 + tx;
-    if (r < rows && c < cols)
-      tile[ty + k][tx] = (float)((double)load_as_float(src, dt, ((size_t)z * rows + r) * cols + c) * inv);
-  }
-  __syncthreads();
-  const int m = tall ? cols : rows;
+ns_prepare_kernel(const void* __restrict__ src, int dt, int m, int n, int tall, const long long* __restrict__ weights,
+                  const double* __restrict__ partial, int parts, double eps, float scale, float* __restrict__ x,
+                  __half* __restrict__ planes, int ldx) {
+  __shared__ float tile[128][33];
+  __shared__ double sh[8];
+  const int z = blockIdx.z, i0 = blockIdx.y * 32, j0 = blockIdx.x * 128;
+  const double inv = 1.0 / (sqrt(block_sum256((int)threadIdx.x < parts ? partial[z * PARTS + threadIdx.x] : 0.0, sh)) + eps);
+  const void* g = reinterpret_cast<const uint8_t*>(src) + (size_t)z * m * n * (dt == DT_F32 ? 4 : 2);
+  if (weights != nullptr) tall = (int)(weights[z] & 1);
   const size_t plane = (size_t)m * ldx;
-#pragma unroll
-  for (int k = 0; k < 32; k += 8) {
-    int i, j;
-    float v;
-    if (tall) { i = c0 + ty + k; j = r0 + tx; v = tile[tx][ty + k]; if (i >= cols || j >= rows) continue; }
-    else { i = r0 + ty + k; j = c0 + tx; v = tile[ty + k][tx]; if (i >= rows || j >= cols) continue; }
+  float* xz = x + (size_t)z * plane;
+  __half* hi = planes + (size_t)z * 2 * plane;
+  const int u = threadIdx.x & 31, w = threadIdx.x >> 5;
+  auto put = [&](int i, int j, float4 v) {               // (the pitch is a multiple of 8: four elements stay inside it)
     const size_t o = (size_t)i * ldx + j;
-    __half hi, lo;
-    split(v * scale, hi, lo);
-    x[(size_t)z * plane + o] = v;
-    planes[(size_t)z * 2 * plane + o] = hi;
-    planes[(size_t)z * 2 * plane + plane + o] = lo;
+    *reinterpret_cast<float4*>(xz + o) = v;
+    uint2 h, l;
+    __half* h4 = reinterpret_cast<__half*>(&h);
+    __half* l4 = reinterpret_cast<__half*>(&l);
+    split(v.x * scale, h4[0], l4[0]); split(v.y * scale, h4[1], l4[1]);
+    split(v.z * scale, h4[2], l4[2]); split(v.w * scale, h4[3], l4[3]);
+    *reinterpret_cast<uint2*>(hi + o) = h;
+    *reinterpret_cast<uint2*>(hi + plane + o) = l;
+  };
+  auto norm = [&](float a) { return (float)((double)a * inv); };
+  if (!tall) {
+    const bool vec = (n & 3) == 0 && aligned4(g, dt);
+    const int j = j0 + 4 * u;
+    float4 v[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int i = i0 + w + 8 * k;
+      v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (i < m && j < n) {
+        const size_t o = (size_t)i * n + j;
+        if (vec) v[k] = load4(g, dt, o);
+        else {
+          v[k].x = load_as_float(g, dt, o);
+          if (j + 1 < n) v[k].y = load_as_float(g, dt, o + 1);
+          if (j + 2 < n) v[k].z = load_as_float(g, dt, o + 2);
+          if (j + 3 < n) v[k].w = load_as_float(g, dt, o + 3);
+        }
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int i = i0 + w + 8 * k;
+      if (i < m && j < n) put(i, j, make_float4(norm(v[k].x), norm(v[k].y), norm(v[k].z), norm(v[k].w)));
+    }
+  } else {
+    float v[16];
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+      const int j = j0 + w + 8 * k, i = i0 + u;
+      v[k] = i < m && j < n ? load_as_float(g, dt, (size_t)j * m + i) : 0.f;
+    }
+#pragma unroll
+    for (int k = 0; k < 16; ++k) tile[w + 8 * k][u] = v[k];
+    __syncthreads();
+    const int j = j0 + 4 * u;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int r = w + 8 * k, i = i0 + r;
+      if (i < m && j < n)
+        put(i, j, make_float4(norm(tile[4 * u][r]), norm(tile[4 * u + 1][r]), norm(tile[4 * u + 2][r]), norm(tile[4 * u + 3][r])));
+    }
   }
 }
 
+// How many partial sums a matrix gets: 16 K elements each, up to 256
+static inline int norm_parts(long long numel) {
+  const long long p = (numel + 16383) / 16384;
+  return (int)(p < PARTS ? p : PARTS);
+}
+
 template <int MODE>
-static int product(const CUtensorMap& ta, const CUtensorMap& tb, const Params& p, cudaStream_t st) {
-  static unsigned long long configured = 0;
-  if (int e = smem_opt_in(ns_product_kernel<MODE>, SMEM_TOTAL, configured)) return e;
+static int product(const CUtensorMap& ta, const CUtensorMap& tb, Params p, cudaStream_t st) {
+  constexpr bool SYM = MODE == GRAM || MODE == SQUARE;
   const int tm = (p.m + BM - 1) / BM, tn = (p.n + BN - 1) / BN;
-  const long long total = (long long)(MODE == GRAM || MODE == SQUARE ? tm * (tm + 1) / 2 : tm * tn) * p.batch;
-  const int sms = sm_count();
-  ns_product_kernel<MODE><<<(unsigned)(total < sms ? total : sms), 320, SMEM_TOTAL, st>>>(ta, tb, p);
-  return (int)cudaGetLastError();
+  const long long total = (long long)(SYM ? tm * (tm + 1) / 2 : tm * tn) * p.batch;
+  const int sms = sm_count(), kblocks = ((MODE == GRAM ? p.n : p.m) + BK - 1) / BK;
+  // tiles that leave most SMs idle: clusters share their contraction
+  int splits = 1;
+  while (splits < 8 && total * splits * 2 <= sms && kblocks >= 4 * splits) splits *= 2;
+  p.splits = splits;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = splits; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+  cfg.blockDim = dim3(320); cfg.dynamicSmemBytes = SMEM_TOTAL; cfg.stream = st; cfg.attrs = attr;
+  cudaError_t e;
+  if (splits > 1) {
+    static unsigned long long configured = 0;
+    if (int r = smem_opt_in(ns_product_kernel<MODE, true>, SMEM_TOTAL, configured)) return r;
+    cfg.gridDim = dim3((unsigned)(total * splits)); cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, ns_product_kernel<MODE, true>, ta, tb, p);
+  } else {
+    static unsigned long long configured = 0;
+    if (int r = smem_opt_in(ns_product_kernel<MODE, false>, SMEM_TOTAL, configured)) return r;
+    cfg.gridDim = dim3((unsigned)(total < sms ? total : sms)); cfg.numAttrs = 0;
+    e = cudaLaunchKernelEx(&cfg, ns_product_kernel<MODE, false>, ta, tb, p);
+  }
+  return e == cudaSuccess ? (int)cudaGetLastError() : (int)e;
 }
 
 static inline long long up256(long long b) { return (b + 255) & ~255ll; }
@@ -444,43 +693,45 @@ struct Workspace {
 
 using namespace gb;
 
-// Bytes of workspace that a batch of `batch` matrices needs (with_y: an optimizer step, which keeps its update there)
-extern "C" int gb_ns_workspace(long long rows, long long cols, long long batch, int with_y, long long* bytes) {
-  *bytes = ns::Workspace(nullptr, rows < cols ? rows : cols, rows < cols ? cols : rows, batch, with_y != 0).bytes;
+// Bytes of workspace that `batch` matrices m x n, m <= n, need (with_y: an optimizer step, which keeps its updates there)
+extern "C" int gb_ns_workspace(long long m, long long n, long long batch, int with_y, long long* bytes) {
+  *bytes = ns::Workspace(nullptr, m, n, batch, with_y != 0).bytes;
   return 0;
 }
 
 // First half of an optimizer step: see muon_momentum_kernel.  The update and its partial sums stay in the workspace.
-extern "C" int gb_muon_momentum(const long long* table, int batch, int grad_dt, int rows, int cols, float mu, int nesterov,
+extern "C" int gb_muon_momentum(const long long* table, int batch, int grad_dt, int m, int n, float mu, int nesterov,
                                 const float* grad_scale, const float* found_inf, void* workspace, cudaStream_t st) {
-  if (batch <= 0 || rows <= 0 || cols <= 0) return 0;
-  if (batch > 65535) return -3;
-  const ns::Workspace w((uint8_t*)workspace, rows < cols ? rows : cols, rows < cols ? cols : rows, batch, true);
-  ns::muon_momentum_kernel<<<dim3(ns::PARTS, batch), 256, 0, st>>>(table, batch, grad_dt, (long long)rows * cols, mu, nesterov,
-                                                                   grad_scale, found_inf, w.y, w.partial);
+  if (batch <= 0 || m <= 0 || n <= 0) return 0;
+  if (batch > 32767 || m > n) return -3;
+  const ns::Workspace w((uint8_t*)workspace, m, n, batch, true);
+  const long long numel = (long long)m * n;
+  ns::muon_momentum_kernel<<<dim3(ns::norm_parts(numel), batch), 256, 0, st>>>(table, batch, grad_dt, numel, mu, nesterov,
+                                                                               grad_scale, found_inf, w.y, w.partial);
   return (int)cudaGetLastError();
 }
 
-// Orthogonalises `batch` matrices [rows, cols].  `src` (contiguous, dtype dt) with `out` of the same type, or null for the
-// update that gb_muon_momentum has left in the workspace, which goes into the weights at `weights` [batch].
+// Orthogonalises `batch` matrices [m, n], or [n, m] (tall), m <= n.  `src` (contiguous, dtype dt) with `out` of the same type;
+// or src null for the updates that gb_muon_momentum has left in the workspace, which go into the weights whose addresses
+// `weights` [batch] holds (+ 1 for a tall one).
 // exponents [3 steps]: powers of two by which X, A and B of each step are scaled in fp16 (host: from the coefficients).
-extern "C" int gb_newton_schulz(const void* src, void* out, int dt, int rows, int cols, int batch, int steps, float a, float b,
-                                float c, double eps, const int* exponents, const long long* weights, float lr, float decay,
-                                float scale, const float* dyn_lr, const float* found_inf, void* workspace, int* status,
-                                cudaStream_t st) {
-  if (batch <= 0 || rows <= 0 || cols <= 0) return 0;
-  if (batch > 32767 || steps < 1 || (src == nullptr) != (weights != nullptr) || (reinterpret_cast<uintptr_t>(workspace) & 255) != 0)
-    return -3;
-  const int tall = rows > cols, m = tall ? cols : rows, n = tall ? rows : cols;
+extern "C" int gb_newton_schulz(const void* src, void* out, int dt, int m, int n, int tall, int batch, int steps, float a,
+                                float b, float c, double eps, const int* exponents, const long long* weights, float lr,
+                                float decay, float scale, const float* dyn_lr, const float* found_inf, void* workspace,
+                                int* status, cudaStream_t st) {
+  if (batch <= 0 || m <= 0 || n <= 0) return 0;
+  if (batch > 32767 || m > n || steps < 1 || (src == nullptr) != (weights != nullptr) ||
+      (reinterpret_cast<uintptr_t>(workspace) & 255) != 0) return -3;
   const int ldx = (n + 7) & ~7, lda = (m + 7) & ~7;
   const ns::Workspace w((uint8_t*)workspace, m, n, batch, src == nullptr);
-  if (src != nullptr) ns::ns_norm_kernel<<<dim3(ns::PARTS, batch), 256, 0, st>>>(src, dt, (long long)rows * cols, w.partial);
-  const dim3 grid((cols + 31) / 32, (rows + 31) / 32, batch);
+  const int parts = ns::norm_parts((long long)m * n);
+  const dim3 grid((n + 127) / 128, (m + 31) / 32, batch);
   if (grid.y > 65535) return -3;
-  ns::ns_prepare_kernel<<<grid, 256, 0, st>>>(src != nullptr ? src : w.y, src != nullptr ? dt : (int)DT_F32, rows, cols, tall,
-                                              w.partial, eps, ldexpf(1.f, exponents[0]), w.x, w.xp[0], ldx);
+  if (src != nullptr) ns::ns_norm_kernel<<<dim3(parts, batch), 256, 0, st>>>(src, dt, (long long)m * n, w.partial);
+  ns::ns_prepare_kernel<<<grid, 256, 0, st>>>(src != nullptr ? src : w.y, src != nullptr ? dt : (int)DT_F32, m, n, tall, weights,
+                                              w.partial, parts, eps, ldexpf(1.f, exponents[0]), w.x, w.xp[0], ldx);
   if (const int e = (int)cudaGetLastError()) return e;
-  // maps: X as left or right operand of X X^T (rows of the contraction), X as right operand of B X, A, B
+  // maps: X as left or right operand of X X^T, X as right operand of B X (64 rows of the contraction at a time), A, B
   CUtensorMap mx[2], mxr[2], ma, mb;
   int r;
   for (int i = 0; i < 2; ++i) {

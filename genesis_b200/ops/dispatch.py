@@ -1021,8 +1021,9 @@ def newton_schulz(x, steps, coefficients, eps, exponents):
 
 def muon_step(params, grads, bufs, shape, lr, momentum, nesterov, weight_decay, scale, steps, coefficients, eps, exponents,
               grad_scale=None, found_inf=None, dyn_lr=None):
-    """One Muon step, in place, on matrices of one shape; params / grads / bufs are lists of (tensor, index of the matrix
-    in the tensor's leading dimensions).  `grad_scale`, `found_inf`: as in `adamw_step`."""
+    """One Muon step, in place, on matrices of `shape` = (m, n), m <= n, and (n, m), whose update is scaled by `scale`;
+    params / grads / bufs are lists of (tensor, index of the matrix in the tensor's leading dimensions).  `grad_scale`,
+    `found_inf`: as in `adamw_step`."""
     if params[0][0].is_cuda:
         r = N.muon_step(params, grads, bufs, shape, lr, momentum, nesterov, weight_decay, scale, steps, coefficients, eps,
                         exponents, grad_scale, found_inf, dyn_lr)
@@ -1034,14 +1035,15 @@ def muon_step(params, grads, bufs, shape, lr, momentum, nesterov, weight_decay, 
     if found_inf is not None and float(found_inf.item()) != 0.0:
         return
     for (p, i), (g, _), (u, _) in zip(params, grads, bufs):
-        p, g, u = (t.view(-1, *shape)[i] for t in (p, g, u))
+        p, g, u = (t.view(-1, *t.shape[-2:])[i] for t in (p, g, u))
         g = g.to(u.dtype)
         if grad_scale is not None:
             g = g * grad_scale.to(g.dtype)
         u.mul_(momentum).add_(g, alpha=1.0 - momentum)
         y = momentum * u + (1.0 - momentum) * g if nesterov else u
         o = _newton_schulz_torch(y, steps, coefficients, eps)
-        p.mul_(1.0 - lr * weight_decay).sub_((lr * scale * o).to(p.dtype))
+        step = lr * scale if p.shape[0] > p.shape[1] else lr
+        p.mul_(1.0 - lr * weight_decay).sub_((step * o).to(p.dtype))
 
 
 def unscale_and_check(grads, inv_scale, found_inf):

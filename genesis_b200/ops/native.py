@@ -72,7 +72,7 @@ _SIGS = {
     "gb_policy_sum": "pp" + "lll" + "i" + "p" + "i" + "p", "gb_preference": "pp" + "ll" + "ff" + "i" + "pppp" + "p",
     "gb_token_grad": "pppp" + "lllll" + "l" + "f" + "pl" + "pll" + "p" + "f" + "ii" + "p",
     "gb_ns_workspace": "lllip", "gb_muon_momentum": "p" + "iiii" + "f" + "i" + "ppp" + "p",
-    "gb_newton_schulz": "pp" + "iiiii" + "fff" + "d" + "pp" + "fff" + "pp" + "pp" + "p",
+    "gb_newton_schulz": "pp" + "iiiiii" + "fff" + "d" + "pp" + "fff" + "pp" + "pp" + "p",
 }
 
 _L = None
@@ -1963,10 +1963,15 @@ def token_grad(logits, tokens, stats, ignore_index, temperature, base, base_div,
 
 
 # =============================== orthogonalised updates ===============================
-def _ns_workspace(rows, cols, batch, with_y, dev):
+def _ns_workspace(m, n, batch, with_y, dev):
     size = ctypes.c_longlong()
-    lib().gb_ns_workspace(rows, cols, batch, 1 if with_y else 0, ctypes.addressof(size))
+    lib().gb_ns_workspace(m, n, batch, 1 if with_y else 0, ctypes.addressof(size))
     return torch.empty(size.value, dtype=torch.uint8, device=dev)
+
+
+def _ns_batch(m, n):
+    """Matrices of one pass: the workspace holds 16 bytes per element of them, some GB are enough to fill the GPU."""
+    return max(1, min(4096, (1 << 28) // (m * n)))
 
 
 def newton_schulz(x, steps, coefficients, eps, exponents):
@@ -1975,27 +1980,24 @@ def newton_schulz(x, steps, coefficients, eps, exponents):
         return NotImplemented
     out = torch.empty_like(x)
     batch, rows, cols = x.shape
-    per = _ns_batch(rows, cols)
+    m, n = min(rows, cols), max(rows, cols)
+    per = _ns_batch(m, n)
     ex = (ctypes.c_int * len(exponents))(*exponents)
     with _on(x.device):
         for i in range(0, batch, per):
-            n = min(per, batch - i)
-            ws = _ns_workspace(rows, cols, n, False, x.device)
-            _chk(lib().gb_newton_schulz(x[i].data_ptr(), out[i].data_ptr(), _DT[x.dtype], rows, cols, n, steps,
-                                        *coefficients, eps, ex, None, 0.0, 0.0, 0.0, None, None, ws.data_ptr(),
+            count = min(per, batch - i)
+            ws = _ns_workspace(m, n, count, False, x.device)
+            _chk(lib().gb_newton_schulz(x[i].data_ptr(), out[i].data_ptr(), _DT[x.dtype], m, n, 1 if rows > cols else 0, count,
+                                        steps, *coefficients, eps, ex, None, 0.0, 0.0, 0.0, None, None, ws.data_ptr(),
                                         status_tensor(x.device).data_ptr(), _st()), "newton_schulz")
     return out
 
 
-def _ns_batch(rows, cols):
-    """Matrices of one pass: the workspace holds 16 bytes per element of them, a GB or so is enough to fill the GPU."""
-    return max(1, min(4096, (1 << 28) // (rows * cols)))
-
-
 def muon_step(params, grads, bufs, shape, lr, momentum, nesterov, weight_decay, scale, steps, coefficients, eps, exponents,
               grad_scale, found_inf, dyn_lr):
-    """One step on matrices of one shape.  params / grads / bufs: lists of (tensor, index of the matrix in it)."""
-    rows, cols = shape
+    """One step on matrices of shape (m, n) or (n, m), m <= n.  params / grads / bufs: lists of (tensor, index of the
+    matrix in it)."""
+    m, n = shape
     for t, _ in params + bufs:
         if t.dtype != F32 or not t.is_contiguous():
             return NotImplemented
@@ -2003,22 +2005,22 @@ def muon_step(params, grads, bufs, shape, lr, momentum, nesterov, weight_decay, 
     if any(g.dtype != gdt or not g.is_contiguous() for g, _ in grads) or gdt not in _FLOATS:
         return NotImplemented
     dev = params[0][0].device
-    per = _ns_batch(rows, cols)
+    per = _ns_batch(m, n)
     ex = (ctypes.c_int * len(exponents))(*exponents)
 
     def at(pair):
-        return pair[0].data_ptr() + pair[1] * rows * cols * pair[0].element_size()
+        return pair[0].data_ptr() + pair[1] * m * n * pair[0].element_size()
 
     with _on(dev):
         for i in range(0, len(params), per):
-            n = min(per, len(params) - i)
-            table = _meta([[at(x) for x in grads[i:i + n]], [at(x) for x in bufs[i:i + n]], [at(x) for x in params[i:i + n]]],
-                          n, dev)
-            ws = _ns_workspace(rows, cols, n, True, dev)
-            _chk(lib().gb_muon_momentum(table.data_ptr(), n, _DT[gdt], rows, cols, float(momentum), 1 if nesterov else 0,
+            count = min(per, len(params) - i)
+            table = _meta([[at(x) for x in grads[i:i + count]], [at(x) for x in bufs[i:i + count]],
+                           [at(x) + (1 if x[0].shape[-2] > x[0].shape[-1] else 0) for x in params[i:i + count]]], 3, dev)
+            ws = _ns_workspace(m, n, count, True, dev)
+            _chk(lib().gb_muon_momentum(table.data_ptr(), count, _DT[gdt], m, n, float(momentum), 1 if nesterov else 0,
                                         _ptr(grad_scale), _ptr(found_inf), ws.data_ptr(), _st()), "muon_momentum")
-            _chk(lib().gb_newton_schulz(None, None, 0, rows, cols, n, steps, *coefficients, eps, ex,
-                                        table.data_ptr() + 16 * n, float(lr), float(weight_decay), float(scale),
+            _chk(lib().gb_newton_schulz(None, None, 0, m, n, 0, count, steps, *coefficients, eps, ex,
+                                        table.data_ptr() + 16 * count, float(lr), float(weight_decay), float(scale),
                                         _ptr(dyn_lr), _ptr(found_inf), ws.data_ptr(), status_tensor(dev).data_ptr(), _st()),
                  "newton_schulz")
     return True

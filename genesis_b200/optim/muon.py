@@ -3,7 +3,7 @@
     u <- mu u + (1 - mu) g,   y = mu u + (1 - mu) g (Nesterov) or u,   o = orthogonalize(y)
     w <- w (1 - lr decay) - lr sqrt(max(1, rows / cols)) o
 
-The orthogonalisation (`csrc/newton_schulz.cu`) works on all matrices of one shape at once.  Vectors, embeddings and
+The orthogonalisation (`csrc/newton_schulz.cu`) works on all matrices of one shape, and its transpose, at once.  Vectors, embeddings and
 output heads are left to AdamW: `Muon` takes tensors of two and more dimensions, whose last two are the matrix.
 """
 import functools
@@ -132,12 +132,12 @@ class Muon(Optimizer):
             if g.shape != p.shape or g.device != p.device:
                 raise ValueError(f"gradient of shape {tuple(g.shape)} on {g.device} for a parameter of shape "
                                  f"{tuple(p.shape)} on {p.device}")
-            members = groups.setdefault((tuple(p.shape[-2:]), g.dtype, p.device), [])
+            members = groups.setdefault((tuple(sorted(p.shape[-2:])), g.dtype, p.device), [])
             g, u = K.contiguous(g), self._state(self.u, i)
             members += [((p, k), (g, k), (u, k)) for k in range(p.numel() // (p.shape[-2] * p.shape[-1]))]
         for (shape, _, _), members in groups.items():
             ps, gs, us = (list(x) for x in zip(*members))
             K.muon_step(ps, gs, us, shape, self.lr, self.momentum, self.nesterov, self.weight_decay,
-                        math.sqrt(max(1.0, shape[0] / shape[1])), self.steps, self.coefficients, self.eps, exponents,
+                        math.sqrt(shape[1] / shape[0]), self.steps, self.coefficients, self.eps, exponents,
                         self._grad_scale, self._found_inf, self._dyn_lr_t)
         self._touched(idx)
