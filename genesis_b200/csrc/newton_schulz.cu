@@ -14,7 +14,7 @@
 //
 // Work.  A and B are symmetric: only tiles on and below the diagonal are computed, the rest is written as their mirror
 // image by the same epilogue.  A step is three launches over all matrices of a batch, 128 x 128 tiles on persistent CTAs:
-//   warp 0 TMA producer, warp 1 issues tcgen05.mma, warps 2-9 epilogue; four accumulators in tensor memory.
+//   warp 0 TMA producer, warp 1 issues tcgen05.mma, warps 4-11 epilogue; accumulators in all of tensor memory.
 // A stage holds both terms of both operands for 64 elements of the contraction (64 KB) and feeds three products, so an SM
 // reads 85 bytes a clock from L2 at the full tensor rate, as the single-product GEMM with tiles of 128 x 256 does.
 // Tiles too few to fill the GPU are shared by clusters of up to 8 CTAs, each with a part of the contraction.
@@ -32,16 +32,16 @@ int make_tmap_3d(CUtensorMap* out, const void* base, int dtype, long long inner,
 
 namespace ns {
 
-constexpr int BM = 128, BN = 128, BK = 64, STAGES = 3;
-constexpr int TILE_BYTES = 128 * 128;                 // 128 rows of 64 fp16, or 64 rows of 2 x 64
-constexpr int STAGE_BYTES = 4 * TILE_BYTES;           // hi and lo of both operands
+constexpr int BM = 128, BK = 64;
+constexpr int A_BYTES = BM * 128;                     // 128 rows of 64 fp16
+constexpr int RING_BYTES = 4 * 48 * 1024;
 constexpr int CHUNK_BYTES = 32 * 32 * 4;              // 32 x 32 results in fp32
-constexpr int SLAB_OFFSET = STAGES * STAGE_BYTES;     // one chunk per epilogue warp
+constexpr int SLAB_OFFSET = RING_BYTES;               // one chunk per epilogue warp
 constexpr int BARRIER_OFFSET = SLAB_OFFSET + 8 * CHUNK_BYTES;
 constexpr int SMEM_TOTAL = BARRIER_OFFSET + 256;
+constexpr int THREADS = 384;                          // warps 0 TMA, 1 MMA, 2 and 3 idle, 4-11 epilogue
 constexpr int PARTS = 256;                            // most partial sums of squares per matrix
-constexpr int ACCS = 4;                               // accumulators in tensor memory, BN columns each
-constexpr int DRAIN = 4;                              // stages that one accumulator takes up: see the header
+constexpr int DRAIN = 4;                              // blocks of BK that one accumulator takes up: see the header
 
 enum Mode : int { GRAM = 0, SQUARE = 1, APPLY = 2, APPLY_LAST = 3 };
 
@@ -95,7 +95,9 @@ __device__ __forceinline__ void store4(void* p, int dt, size_t i, const float* v
     if (dt == DT_F32) *reinterpret_cast<float4*>(reinterpret_cast<float*>(p) + i) = make_float4(v[0], v[1], v[2], v[3]);
     else *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(p) + i) = make_uint2(pack2(v[0], v[1], dt), pack2(v[2], v[3], dt));
   } else {
-    for (int k = 0; k < n; ++k) store_from_float(p, dt, i + k, v[k]);
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (k < n) store_from_float(p, dt, i + k, v[k]);
   }
 }
 
@@ -113,106 +115,140 @@ struct Epilogue {
       keep = 1.f - lr * p.decay;
       step = lr;
       skip = p.found_inf != nullptr && *p.found_inf != 0.f;
-      // (rows of a result of n, or m, elements start on a boundary of four; weights are looked at one by one)
+      // rows of n, or m, elements start on a boundary of four, and end on one
       vec = ((p.tall ? p.m : p.n) & 3) == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0;
     }
   }
-  __device__ __forceinline__ void run(const uint8_t* chunk, int z, int row0, int col0, bool mirror) const {
+  __device__ __forceinline__ void run(uint8_t* chunk, int z, int row0, int col0) const {
     const int cols = MODE == GRAM || MODE == SQUARE ? p.m : p.n;
-    const int u = lane & 7, col = col0 + 4 * u;
+    if (row0 >= p.m || col0 >= cols) return;
+    // symmetric results: blocks of 128 below the diagonal are written twice, those above it not at all
+    if ((MODE == GRAM || MODE == SQUARE) && col0 / BM > row0 / BM) return;
+    const bool mirror = col0 / BM < row0 / BM;
+    const int u = lane & 7, r0 = lane >> 3, col = col0 + 4 * u;
+    // everything that is read comes before the first store: eight loads of a lane are in flight together
     if constexpr (MODE == GRAM || MODE == SQUARE) {
-      const size_t plane = (size_t)p.m * p.lda;
-      __half* hi = p.dst + (size_t)z * 2 * plane;
-      const __half* ah = p.a_planes + (size_t)z * 2 * plane;
+      const size_t plane = (size_t)p.m * p.lda, zo = (size_t)z * 2 * plane;
+#pragma unroll 1
+      for (int pass = 0; pass <= (mirror ? 1 : 0); ++pass) {
+        // second pass, the transposed chunk: row col0 + r of the result, its columns row0 + 4 u .. + 3
+        const int i0 = pass ? col0 : row0, j = pass ? row0 + 4 * u : col;
+        __half* dst = p.dst + zo + (size_t)(i0 + r0) * p.lda + j;
+        const int rows = j < p.m ? p.m - i0 - r0 : 0;
+        uint2 ah[8], al[8];
+        if constexpr (MODE == SQUARE) {
+          const __half* a = p.a_planes + zo + (size_t)(i0 + r0) * p.lda + j;
 #pragma unroll
-      for (int it = 0; it < 8; ++it) {
-        const int r = 4 * it + (lane >> 3), row = row0 + r;
-        if (row < p.m && col < cols) {
-          const float4 a = *reinterpret_cast<const float4*>(chunk + chunk_at(r, u));
-          float v[4] = {a.x * p.f_acc, a.y * p.f_acc, a.z * p.f_acc, a.w * p.f_acc};
-          const size_t o = (size_t)row * p.lda + col;
-          if constexpr (MODE == SQUARE) add_a(v, ah + o, plane);
-          put(hi + o, plane, v);
+          for (int it = 0; it < 8; ++it) {
+            ah[it] = al[it] = make_uint2(0u, 0u);
+            if (4 * it < rows) {
+              ah[it] = *reinterpret_cast<const uint2*>(a + (size_t)(4 * it) * p.lda);
+              al[it] = *reinterpret_cast<const uint2*>(a + (size_t)(4 * it) * p.lda + plane);
+            }
+          }
         }
-      }
-      if (mirror) {
-        // the transposed chunk: row `col0 + r` of the result, its columns row0 + 4 u .. + 3
-        const int i0 = row0 + 4 * u;
 #pragma unroll
         for (int it = 0; it < 8; ++it) {
-          const int r = 4 * it + (lane >> 3), row = col0 + r;
-          if (row < cols && i0 < p.m) {
+          if (4 * it < rows) {
             float v[4];
-            column(chunk, r, u, v);
+            if (pass) column(chunk, 4 * it + r0, u, v);
+            else row4(chunk, 4 * it + r0, u, v);
 #pragma unroll
             for (int k = 0; k < 4; ++k) v[k] *= p.f_acc;
-            const size_t o = (size_t)row * p.lda + i0;
-            if constexpr (MODE == SQUARE) add_a(v, ah + o, plane);
-            put(hi + o, plane, v);
+            if constexpr (MODE == SQUARE) add_a(v, ah[it], al[it]);
+            put(dst + (size_t)(4 * it) * p.lda, plane, v);
           }
         }
       }
     } else {
       bool across = false;                                       // the result is the transpose
       if constexpr (MODE == APPLY_LAST) across = p.weights != nullptr ? (p.weights[z] & 1) != 0 : p.tall != 0;
-      if (!across) {
+      const int rows = col < cols ? p.m - row0 - r0 : 0;
+      float* x = p.x + ((size_t)z * p.m + row0 + r0) * p.ldx + col;
+      float4 o[8];
 #pragma unroll
-        for (int it = 0; it < 8; ++it) {
-          const int r = 4 * it + (lane >> 3), row = row0 + r;
-          if (row < p.m && col < cols) {
-            const float4 a = *reinterpret_cast<const float4*>(chunk + chunk_at(r, u));
-            float* x = p.x + ((size_t)z * p.m + row) * p.ldx + col;
-            const float4 o = *reinterpret_cast<const float4*>(x);
-            float v[4] = {fmaf(a.x, p.f_acc, o.x * p.f_a), fmaf(a.y, p.f_acc, o.y * p.f_a), fmaf(a.z, p.f_acc, o.z * p.f_a),
-                          fmaf(a.w, p.f_acc, o.w * p.f_a)};
-            if constexpr (MODE == APPLY) {
-              *reinterpret_cast<float4*>(x) = make_float4(v[0], v[1], v[2], v[3]);
-              const size_t plane = (size_t)p.m * p.ldx;
+      for (int it = 0; it < 8; ++it)
+        o[it] = 4 * it < rows ? *reinterpret_cast<const float4*>(x + (size_t)(4 * it) * p.ldx) : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-              for (int k = 0; k < 4; ++k) v[k] *= p.next_scale;
-              put(p.dst + (size_t)z * 2 * plane + (size_t)row * p.ldx + col, plane, v);
-            } else {
-              result(z, (size_t)row * p.n + col, v, min(4, cols - col), step);
+      for (int it = 0; it < 8; ++it) {
+        float4* a = reinterpret_cast<float4*>(chunk + chunk_at(4 * it + r0, u));
+        const float4 b = *a;
+        const float v[4] = {fmaf(b.x, p.f_acc, o[it].x * p.f_a), fmaf(b.y, p.f_acc, o[it].y * p.f_a),
+                            fmaf(b.z, p.f_acc, o[it].z * p.f_a), fmaf(b.w, p.f_acc, o[it].w * p.f_a)};
+        if constexpr (MODE == APPLY) {
+          if (4 * it < rows) {
+            *reinterpret_cast<float4*>(x + (size_t)(4 * it) * p.ldx) = make_float4(v[0], v[1], v[2], v[3]);
+            const size_t plane = (size_t)p.m * p.ldx;
+            const float w[4] = {v[0] * p.next_scale, v[1] * p.next_scale, v[2] * p.next_scale, v[3] * p.next_scale};
+            put(p.dst + (size_t)z * 2 * plane + (size_t)(row0 + r0 + 4 * it) * p.ldx + col, plane, w);
+          }
+        } else {
+          *a = make_float4(v[0], v[1], v[2], v[3]);
+        }
+      }
+      if constexpr (MODE == APPLY_LAST) {
+        __syncwarp();
+        const int i0 = across ? col0 : row0, j = across ? row0 + 4 * u : col;
+        const int ld = across ? p.m : p.n, count = ld - j;       // elements of a row from here on
+        const int left = count > 0 ? (across ? p.n : p.m) - i0 - r0 : 0;
+        const float st = across ? step * p.scale : step;
+        const size_t at = (size_t)(i0 + r0) * ld + j;
+        if (p.weights != nullptr) {
+          float* w = reinterpret_cast<float*>(p.weights[z] & ~1ll) + at;
+          if (skip) return;
+          if ((ld & 3) == 0 && (reinterpret_cast<uintptr_t>(w) & 15) == 0) {
+#pragma unroll
+            for (int it = 0; it < 8; ++it)
+              if (4 * it < left) o[it] = *reinterpret_cast<const float4*>(w + (size_t)(4 * it) * ld);
+#pragma unroll
+            for (int it = 0; it < 8; ++it) {
+              if (4 * it < left) {
+                float v[4];
+                if (across) column(chunk, 4 * it + r0, u, v);
+                else row4(chunk, 4 * it + r0, u, v);
+                *reinterpret_cast<float4*>(w + (size_t)(4 * it) * ld) =
+                    make_float4(fmaf(o[it].x, keep, -st * v[0]), fmaf(o[it].y, keep, -st * v[1]),
+                                fmaf(o[it].z, keep, -st * v[2]), fmaf(o[it].w, keep, -st * v[3]));
+              }
+            }
+          } else {
+#pragma unroll 1
+            for (int it = 0; it < 8; ++it) {
+              if (4 * it < left) {
+                float v[4];
+                if (across) column(chunk, 4 * it + r0, u, v);
+                else row4(chunk, 4 * it + r0, u, v);
+                float* q = w + (size_t)(4 * it) * ld;
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                  if (k < count) q[k] = fmaf(q[k], keep, -st * v[k]);
+              }
             }
           }
-        }
-      } else {
-        // X is read by rows as above and meets its accumulators in shared memory; then columns go out as rows
-        float4 o[8];
+        } else {
 #pragma unroll
-        for (int it = 0; it < 8; ++it) {
-          const int row = row0 + 4 * it + (lane >> 3);
-          o[it] = row < p.m && col < cols ? *reinterpret_cast<const float4*>(p.x + ((size_t)z * p.m + row) * p.ldx + col)
-                                          : make_float4(0.f, 0.f, 0.f, 0.f);
-        }
-#pragma unroll
-        for (int it = 0; it < 8; ++it) {
-          float4* a = reinterpret_cast<float4*>(const_cast<uint8_t*>(chunk) + chunk_at(4 * it + (lane >> 3), u));
-          const float4 b = *a;
-          *a = make_float4(fmaf(b.x, p.f_acc, o[it].x * p.f_a), fmaf(b.y, p.f_acc, o[it].y * p.f_a),
-                           fmaf(b.z, p.f_acc, o[it].z * p.f_a), fmaf(b.w, p.f_acc, o[it].w * p.f_a));
-        }
-        __syncwarp();
-        const int i0 = row0 + 4 * u;
-#pragma unroll
-        for (int it = 0; it < 8; ++it) {
-          const int r = 4 * it + (lane >> 3), row = col0 + r;
-          if (row < cols && i0 < p.m) {
-            float v[4];
-            column(chunk, r, u, v);
-            result(z, (size_t)row * p.m + i0, v, min(4, p.m - i0), step * p.scale);
+          for (int it = 0; it < 8; ++it) {
+            if (4 * it < left) {
+              float v[4];
+              if (across) column(chunk, 4 * it + r0, u, v);
+              else row4(chunk, 4 * it + r0, u, v);
+              store4(p.out, p.out_dtype, (size_t)z * p.m * p.n + at + (size_t)(4 * it) * ld, v, count, vec);
+            }
           }
         }
       }
     }
+  }
+  __device__ __forceinline__ void row4(const uint8_t* chunk, int r, int u, float (&v)[4]) const {
+    const float4 a = *reinterpret_cast<const float4*>(chunk + chunk_at(r, u));
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
   }
   // four rows 4 u .. of column `c` of the chunk
   __device__ __forceinline__ void column(const uint8_t* chunk, int c, int u, float (&v)[4]) const {
 #pragma unroll
     for (int k = 0; k < 4; ++k) v[k] = *reinterpret_cast<const float*>(chunk + chunk_at(4 * u + k, c >> 2) + (c & 3) * 4);
   }
-  __device__ __forceinline__ void add_a(float (&v)[4], const __half* a, size_t plane) const {
-    const uint2 x = *reinterpret_cast<const uint2*>(a), y = *reinterpret_cast<const uint2*>(a + plane);
+  __device__ __forceinline__ void add_a(float (&v)[4], const uint2& x, const uint2& y) const {
     const float2 x0 = __half22float2(*reinterpret_cast<const __half2*>(&x.x)), x1 = __half22float2(*reinterpret_cast<const __half2*>(&x.y));
     const float2 y0 = __half22float2(*reinterpret_cast<const __half2*>(&y.x)), y1 = __half22float2(*reinterpret_cast<const __half2*>(&y.y));
     v[0] = fmaf(x0.x + y0.x, p.f_a, v[0]); v[1] = fmaf(x0.y + y0.y, p.f_a, v[1]);
@@ -228,36 +264,31 @@ struct Epilogue {
     *reinterpret_cast<uint2*>(hi) = h;
     *reinterpret_cast<uint2*>(hi + plane) = l;
   }
-  // up to four neighbouring elements of the result
-  __device__ __forceinline__ void result(int z, size_t at, const float (&v)[4], int n, float step) const {
-    if (p.weights != nullptr) {
-      if (skip) return;
-      float* w = reinterpret_cast<float*>(p.weights[z] & ~1ll) + at;
-      if (n == 4 && (reinterpret_cast<uintptr_t>(w) & 15) == 0) {
-        float4 o = *reinterpret_cast<const float4*>(w);
-        o.x = fmaf(o.x, keep, -step * v[0]); o.y = fmaf(o.y, keep, -step * v[1]);
-        o.z = fmaf(o.z, keep, -step * v[2]); o.w = fmaf(o.w, keep, -step * v[3]);
-        *reinterpret_cast<float4*>(w) = o;
-      } else {
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          if (k < n) w[k] = fmaf(w[k], keep, -step * v[k]);
-      }
-    } else {
-      store4(p.out, p.out_dtype, (size_t)z * p.m * p.n + at, v, n, n == 4 && vec);
-    }
-  }
 };
 
-template <int MODE, bool SPLIT>
-__global__ void __launch_bounds__(320, 1)
+// Tiles of BM x BN: for the symmetric modes those that hold a block of 128 x 128 on or below the diagonal, row by row
+template <int BN>
+__host__ __device__ constexpr long long tiles_of(bool sym, long long m, long long n) {
+  const long long tm = (m + BM - 1) / BM;
+  if (!sym) return tm * ((n + BN - 1) / BN);
+  return BN == 128 ? tm * (tm + 1) / 2 : (tm + 1) / 2 * (tm + 1 - (tm + 1) / 2);
+}
+
+template <int MODE, int BN, bool SPLIT>
+__global__ void __launch_bounds__(THREADS, 1)
 ns_product_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_constant__ CUtensorMap tmapB, const Params p) {
   constexpr bool SYM = MODE == GRAM || MODE == SQUARE;
   constexpr bool B_MN = !SYM;                           // X as the right operand: its rows run along the contraction
+  constexpr int B_BYTES = BN * 128;
+  // Ring of half stages: (A hi, B lo) and (A lo, B hi) of a block of the contraction.  The three products of a block run in
+  // the order hi lo, hi hi, lo hi, so the first half is free before the block is done.
+  constexpr int HALF_BYTES = A_BYTES + B_BYTES, HALVES = RING_BYTES / HALF_BYTES / 2 * 2;
+  constexpr int ACCS = 512 / BN;                        // accumulators in tensor memory
+  constexpr int CHUNKS = BN / 64;                       // of 32 x 32 results, per epilogue warp
   extern __shared__ __align__(1024) uint8_t smem[];
   uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + BARRIER_OFFSET);
-  uint64_t* empty_bar = full_bar + STAGES;
-  uint64_t* tmem_full = empty_bar + STAGES;
+  uint64_t* empty_bar = full_bar + HALVES;
+  uint64_t* tmem_full = empty_bar + HALVES;
   uint64_t* tmem_empty = tmem_full + ACCS;
   uint32_t* tmem_base_slot = reinterpret_cast<uint32_t*>(tmem_empty + ACCS);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_base_slot + 1);
@@ -265,7 +296,7 @@ ns_product_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_consta
   const int lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < STAGES; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], 1); }
+    for (int s = 0; s < HALVES; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], 1); }
     for (int a = 0; a < ACCS; ++a) { mbar_init(&tmem_full[a], 1); mbar_init(&tmem_empty[a], 8); }
     // after an error no work is done, but every CTA of a cluster comes to its barriers
     const bool aligned = (smem_u32(smem) & 1023) == 0;
@@ -276,7 +307,7 @@ ns_product_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_consta
     tma_prefetch_desc(&tmapB);
   }
   if (warp == 1) {
-    tmem_alloc(tmem_base_slot, ACCS * BN);
+    tmem_alloc(tmem_base_slot, 512);
     tmem_relinquish();
   }
   tc_fence_before_sync();
@@ -284,64 +315,82 @@ ns_product_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_consta
   tc_fence_after_sync();
   const uint32_t tmem_base = *tmem_base_slot;
 
-  const int tm = (p.m + BM - 1) / BM, tn = (p.n + BN - 1) / BN;
-  const int per = SYM ? tm * (tm + 1) / 2 : tm * tn;
+  const int tm = (p.m + BM - 1) / BM;
+  const int per = (int)tiles_of<BN>(SYM, p.m, p.n);
   const long long total = (long long)per * p.batch;
   const int kblocks = ((MODE == GRAM ? p.n : p.m) + BK - 1) / BK;
   // this CTA's tiles and its part of their contraction, in blocks of BK
   const int splits = SPLIT ? p.splits : 1, rank = SPLIT ? (int)cluster_rank() : 0;
   const long long first = blockIdx.x / splits, stride = gridDim.x / splits;
   const int kb0 = kblocks * rank / splits, kb1 = kblocks * (rank + 1) / splits;
-  // tile of matrix z: (mi, ni); the symmetric modes walk the lower triangle row by row
+  // tile of matrix z: (mi, ni)
   auto decode = [&](long long t, int& mi, int& ni, int& z) {
     z = (int)(t / per);
     const int r = (int)(t % per);
     if constexpr (SYM) {
-      mi = (int)((sqrtf(8.f * (float)r + 1.f) - 1.f) * 0.5f);
-      while (mi * (mi + 1) / 2 > r) --mi;
-      while ((mi + 1) * (mi + 2) / 2 <= r) ++mi;
-      ni = r - mi * (mi + 1) / 2;
+      if constexpr (BN == 128) {
+        mi = (int)((sqrtf(8.f * (float)r + 1.f) - 1.f) * 0.5f);
+        while (mi * (mi + 1) / 2 > r) --mi;
+        while ((mi + 1) * (mi + 2) / 2 <= r) ++mi;
+        ni = r - mi * (mi + 1) / 2;
+      } else {
+        // rows 2 g and 2 g + 1 have g + 1 tiles each; g (g + 1) tiles lie before row 2 g
+        int g = (int)((sqrtf(4.f * (float)r + 1.f) - 1.f) * 0.5f);
+        while (g * (g + 1) > r) --g;
+        while ((g + 1) * (g + 2) <= r) ++g;
+        const int o = r - g * (g + 1);
+        mi = 2 * g + (o > g ? 1 : 0);
+        ni = o > g ? o - g - 1 : o;
+      }
     } else {
       ni = r / tm;
       mi = r % tm;
     }
   };
 
-  if (warp == 0) {
+  // The sums of a 128 x 256 tile take 128 registers of every epilogue thread: of 384 x 168 at launch, the first four warps
+  // keep 56 each and the others get 224 (128 x 56 + 256 x 224 = 384 x 168).
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (warp == 0) {
     // =========================== TMA producer ===========================
     if (elect_one()) {
       uint32_t it = 0;
       for (long long t = first; t < total && !*abort_flag; t += stride) {
         int mi, ni, z;
         decode(t, mi, ni, z);
-        for (int kb = kb0; kb < kb1; ++kb, ++it) {
-          const int s = it % STAGES, k0 = kb * BK;
-          if (!mbar_wait(&empty_bar[s], ((it / STAGES) & 1) ^ 1, abort_flag, p.status, 110)) break;
-          uint8_t* st = smem + s * STAGE_BYTES;
-          mbar_expect_tx(&full_bar[s], STAGE_BYTES);
+        for (int kh = 2 * kb0; kh < 2 * kb1; ++kh, ++it) {
+          const int s = it % HALVES, k0 = (kh >> 1) * BK, h = kh & 1;        // h: A's term (0 = hi); B's is the other
+          if (!mbar_wait(&empty_bar[s], ((it / HALVES) & 1) ^ 1, abort_flag, p.status, 110)) break;
+          uint8_t* sa = smem + s * HALF_BYTES;
+          uint8_t* sb = sa + A_BYTES;
+          mbar_expect_tx(&full_bar[s], HALF_BYTES);
+          tma_load_3d(sa, &tmapA, &full_bar[s], k0, mi * BM, 2 * z + h);
+          if constexpr (!B_MN) {
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            tma_load_3d(st + h * TILE_BYTES, &tmapA, &full_bar[s], k0, mi * BM, 2 * z + h);
-            uint8_t* sb = st + (2 + h) * TILE_BYTES;
-            if constexpr (!B_MN) {
-              tma_load_3d(sb, &tmapB, &full_bar[s], k0, ni * BN, 2 * z + h);
-            } else {
+            for (int c = 0; c < BN / 128; ++c)
+              tma_load_3d(sb + c * A_BYTES, &tmapB, &full_bar[s], k0, ni * BN + c * 128, 2 * z + 1 - h);
+          } else {
 #pragma unroll
-              for (int c = 0; c < BN / 64; ++c)
-                tma_load_3d(sb + c * (BK * 128), &tmapB, &full_bar[s], ni * BN + c * 64, k0, 2 * z + h);
-            }
+            for (int c = 0; c < BN / 64; ++c)
+              tma_load_3d(sb + c * (BK * 128), &tmapB, &full_bar[s], ni * BN + c * 64, k0, 2 * z + 1 - h);
           }
         }
       }
-      if (*abort_flag) drain_copies(full_bar, STAGES, it);
+      if (*abort_flag) drain_copies(full_bar, HALVES, it);
     }
     __syncwarp();
   } else if (warp == 1) {
     // =========================== MMA issuer (converged warp, one elected lane) ===========================
     const uint32_t idesc = make_idesc(0u, 0u, B_MN ? 1u : 0u, BM, BN);
     uint32_t it = 0, drains = 0;
-    bool ok = !*abort_flag;
-    ok = __all_sync(0xffffffffu, ok);
+    bool ok = __all_sync(0xffffffffu, *abort_flag == 0);
+    auto b_desc = [&](uint32_t addr) { return B_MN ? make_smem_desc(addr, BK * 128, 1024) : make_smem_desc(addr, 16, 1024); };
+    auto multiply = [&](uint32_t d, uint64_t a, uint64_t b, bool fresh) {
+#pragma unroll
+      for (int kk = 0; kk < BK / 16; ++kk)                                   // (descriptors count 16-byte units)
+        umma_f16(d, a + kk * 2, b + (B_MN ? kk * 128 : kk * 2), idesc, fresh && kk == 0 ? 0u : 1u);
+    };
     for (long long t = first; t < total && ok; t += stride) {
       for (int kb = kb0; kb < kb1 && ok; kb += DRAIN, ++drains) {
         const uint32_t acc = drains % ACCS;
@@ -349,23 +398,23 @@ ns_product_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_consta
         tc_fence_after_sync();
         const uint32_t d_tmem = tmem_base + acc * BN;
         const int end = min(kb + DRAIN, kb1);
-        for (int k = kb; k < end; ++k, ++it) {
-          const int s = it % STAGES;
-          if (!__all_sync(0xffffffffu, mbar_wait(&full_bar[s], (it / STAGES) & 1, abort_flag, p.status, 211))) { ok = false; break; }
+        for (int k = kb; k < end; ++k, it += 2) {
+          const int s = it % HALVES;                                         // (even: HALVES is)
+          const uint32_t ph = (it / HALVES) & 1;
+          if (!__all_sync(0xffffffffu, mbar_wait(&full_bar[s], ph, abort_flag, p.status, 211))) { ok = false; break; }
           tc_fence_after_sync();
-          const uint32_t a_addr = smem_u32(smem + s * STAGE_BYTES), b_addr = a_addr + 2 * TILE_BYTES;
-          const uint64_t da = make_smem_desc(a_addr, 16, 1024);
-          const uint64_t db = B_MN ? make_smem_desc(b_addr, BK * 128, 1024) : make_smem_desc(b_addr, 16, 1024);
+          const uint32_t x_addr = smem_u32(smem + s * HALF_BYTES), y_addr = x_addr + HALF_BYTES;
+          const uint64_t a_hi = make_smem_desc(x_addr, 16, 1024), b_lo = b_desc(x_addr + A_BYTES);
+          const uint64_t a_lo = make_smem_desc(y_addr, 16, 1024), b_hi = b_desc(y_addr + A_BYTES);
+          if (elect_one()) multiply(d_tmem, a_hi, b_lo, k == kb);
+          __syncwarp();
+          if (!__all_sync(0xffffffffu, mbar_wait(&full_bar[s + 1], ph, abort_flag, p.status, 212))) { ok = false; break; }
+          tc_fence_after_sync();
           if (elect_one()) {
-#pragma unroll
-            for (int kk = 0; kk < BK / 16; ++kk) {
-              const uint64_t a = da + kk * 2, b = db + (B_MN ? kk * 128 : kk * 2);      // (16-byte units)
-              constexpr uint64_t LO = TILE_BYTES / 16;
-              umma_f16(d_tmem, a, b + LO, idesc, (k == kb && kk == 0) ? 0u : 1u);
-              umma_f16(d_tmem, a + LO, b, idesc, 1u);
-              umma_f16(d_tmem, a, b, idesc, 1u);
-            }
+            multiply(d_tmem, a_hi, b_hi, false);
             umma_commit(&empty_bar[s]);
+            multiply(d_tmem, a_lo, b_hi, false);
+            umma_commit(&empty_bar[s + 1]);
           }
           __syncwarp();
         }
@@ -376,33 +425,41 @@ ns_product_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_consta
       }
     }
     __syncwarp();
+    }
+    if constexpr (SPLIT) {                               // (the epilogue's three barriers, see there)
+      tc_fence_before_sync();
+      __syncthreads();
+      cluster_barrier();
+      cluster_barrier();
+    }
   } else {
-    // =========================== epilogue: 8 warps, 32 rows x 64 columns each ===========================
-    const int q = warp & 3, half = (warp - 2) >> 2;
-    uint8_t* slab = smem + SLAB_OFFSET + (warp - 2) * CHUNK_BYTES;
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+    // =========================== epilogue: 8 warps, 32 rows x BN / 2 columns each ===========================
+    const int q = warp & 3, half = (warp - 4) >> 2;
+    uint8_t* slab = smem + SLAB_OFFSET + (warp - 4) * CHUNK_BYTES;
     const Epilogue<MODE> epi(p);
     uint32_t drains = 0;
     bool ok = true;
     for (long long t = first; t < total; t += stride) {
       int mi, ni, z;
       decode(t, mi, ni, z);
-      float v[2][32];
+      float v[CHUNKS][32];
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
+      for (int h = 0; h < CHUNKS; ++h)
 #pragma unroll
         for (int j = 0; j < 32; ++j) v[h][j] = 0.f;
       for (int kb = kb0; kb < kb1; kb += DRAIN, ++drains) {
         const uint32_t acc = drains % ACCS;
         if (!__all_sync(0xffffffffu, mbar_wait(&tmem_full[acc], (drains / ACCS) & 1, abort_flag, p.status, 310))) { ok = false; break; }
         tc_fence_after_sync();
-        const uint32_t at = tmem_base + ((uint32_t)(q * 32) << 16) + acc * BN + half * 64;
+        const uint32_t at = tmem_base + ((uint32_t)(q * 32) << 16) + acc * BN + half * (BN / 2);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint32_t r[32];
-          tmem_ld_32x32b_x32(at + 32 * h, r);
+        for (int h = 0; h < 2 * CHUNKS; ++h) {
+          uint32_t r[16];
+          tmem_ld_32x32b_x16(at + 16 * h, r);
           tmem_ld_wait();
 #pragma unroll
-          for (int j = 0; j < 32; ++j) v[h][j] += __uint_as_float(r[j]);
+          for (int j = 0; j < 16; ++j) v[h >> 1][(h & 1) * 16 + j] += __uint_as_float(r[j]);
         }
         tc_fence_before_sync();
         __syncwarp();
@@ -410,55 +467,51 @@ ns_product_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_consta
       }
       if (!ok) break;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        // a part of the contraction waits in this CTA's stages, which all products have been read from by now
-        uint8_t* at = SPLIT ? smem + ((warp - 2) * 2 + h) * CHUNK_BYTES : slab;
+      for (int h = 0; h < CHUNKS; ++h) {
+        // a part of the contraction waits in this CTA's ring, which all products have been read from by now
+        uint8_t* at = SPLIT ? smem + ((warp - 4) * CHUNKS + h) * CHUNK_BYTES : slab;
         __syncwarp();                                   // (the chunk before has been read)
 #pragma unroll
         for (int u = 0; u < 8; ++u)
           *reinterpret_cast<float4*>(at + chunk_at(lane, u)) = make_float4(v[h][4 * u], v[h][4 * u + 1], v[h][4 * u + 2], v[h][4 * u + 3]);
         __syncwarp();
-        if constexpr (!SPLIT) {
-          const int col0 = ni * BN + half * 64 + h * 32;
-          epi.run(slab, z, mi * BM + q * 32, col0, SYM && mi != ni);
+        if constexpr (!SPLIT) epi.run(slab, z, mi * BM + q * 32, ni * BN + half * (BN / 2) + h * 32);
+      }
+    }
+    if constexpr (SPLIT) {
+      // the parts of a tile meet: rank k adds up chunks k, k + splits, .., in the order of the ranks, one warp each at a time
+      tc_fence_before_sync();
+      __syncthreads();
+      cluster_barrier();
+      if (!*abort_flag) {
+        int mi, ni, z;
+        decode(first, mi, ni, z);
+        for (int c = rank + (warp - 4) * splits; c < 8 * CHUNKS; c += 8 * splits) {
+          __syncwarp();
+  #pragma unroll
+          for (int it = 0; it < 8; ++it) {
+            const int off = chunk_at(4 * it + (lane >> 3), lane & 7);
+            float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int k = 0; k < splits; ++k) {
+              const float4 o = ld_peer(smem_u32(smem) + c * CHUNK_BYTES + off, k);
+              sum.x += o.x; sum.y += o.y; sum.z += o.z; sum.w += o.w;
+            }
+            *reinterpret_cast<float4*>(slab + off) = sum;
+          }
+          __syncwarp();
+          const int w = c / CHUNKS;                        // the warp whose chunk this was, and where its rows and columns are
+          epi.run(slab, z, mi * BM + (w & 3) * 32, ni * BN + (w >> 2) * (BN / 2) + (c % CHUNKS) * 32);
         }
       }
+      cluster_barrier();                                   // nobody leaves while its part may still be read
     }
   }
 
-  if constexpr (SPLIT) {
-    // the parts of a tile meet: rank k adds up chunks k, k + splits, .., in the order of the ranks, one warp each
-    tc_fence_before_sync();
-    __syncthreads();
-    cluster_barrier();
-    const int c = rank + (warp - 2) * splits;
-    if (warp >= 2 && c < 16 && !*abort_flag) {
-      uint8_t* slab = smem + SLAB_OFFSET + (warp - 2) * CHUNK_BYTES;
-#pragma unroll
-      for (int it = 0; it < 8; ++it) {
-        const int off = chunk_at(4 * it + (lane >> 3), lane & 7);
-        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int k = 0; k < splits; ++k) {
-          const float4 o = ld_peer(smem_u32(smem) + c * CHUNK_BYTES + off, k);
-          sum.x += o.x; sum.y += o.y; sum.z += o.z; sum.w += o.w;
-        }
-        *reinterpret_cast<float4*>(slab + off) = sum;
-      }
-      __syncwarp();
-      int mi, ni, z;
-      decode(first, mi, ni, z);
-      const int w = (c >> 1) + 2;                        // the warp whose chunk this was
-      const int q = w & 3, col0 = ni * BN + ((w - 2) >> 2) * 64 + (c & 1) * 32;
-      const Epilogue<MODE> epi(p);
-      epi.run(slab, z, mi * BM + q * 32, col0, SYM && mi != ni);
-    }
-    cluster_barrier();                                   // nobody leaves while its part may still be read
-  }
   tc_fence_before_sync();
   __syncthreads();
   if (warp == 1) {
     tc_fence_after_sync();
-    tmem_dealloc(tmem_base, ACCS * BN);
+    tmem_dealloc(tmem_base, 512);
   }
 }
 
@@ -638,34 +691,40 @@ static inline int norm_parts(long long numel) {
   return (int)(p < PARTS ? p : PARTS);
 }
 
-template <int MODE>
-static int product(const CUtensorMap& ta, const CUtensorMap& tb, Params p, cudaStream_t st) {
-  constexpr bool SYM = MODE == GRAM || MODE == SQUARE;
-  const int tm = (p.m + BM - 1) / BM, tn = (p.n + BN - 1) / BN;
-  const long long total = (long long)(SYM ? tm * (tm + 1) / 2 : tm * tn) * p.batch;
-  const int sms = sm_count(), kblocks = ((MODE == GRAM ? p.n : p.m) + BK - 1) / BK;
-  // tiles that leave most SMs idle: clusters share their contraction
-  int splits = 1;
-  while (splits < 8 && total * splits * 2 <= sms && kblocks >= 4 * splits) splits *= 2;
-  p.splits = splits;
+template <int MODE, int BN, bool SPLIT>
+static int launch(const CUtensorMap& ta, const CUtensorMap& tb, const Params& p, int grid, cudaStream_t st) {
+  static unsigned long long configured = 0;
+  if (int r = smem_opt_in(ns_product_kernel<MODE, BN, SPLIT>, SMEM_TOTAL, configured)) return r;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = splits; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
-  cfg.blockDim = dim3(320); cfg.dynamicSmemBytes = SMEM_TOTAL; cfg.stream = st; cfg.attrs = attr;
-  cudaError_t e;
-  if (splits > 1) {
-    static unsigned long long configured = 0;
-    if (int r = smem_opt_in(ns_product_kernel<MODE, true>, SMEM_TOTAL, configured)) return r;
-    cfg.gridDim = dim3((unsigned)(total * splits)); cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, ns_product_kernel<MODE, true>, ta, tb, p);
-  } else {
-    static unsigned long long configured = 0;
-    if (int r = smem_opt_in(ns_product_kernel<MODE, false>, SMEM_TOTAL, configured)) return r;
-    cfg.gridDim = dim3((unsigned)(total < sms ? total : sms)); cfg.numAttrs = 0;
-    e = cudaLaunchKernelEx(&cfg, ns_product_kernel<MODE, false>, ta, tb, p);
-  }
+  attr[0].val.clusterDim.x = p.splits; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+  cfg.gridDim = dim3((unsigned)grid); cfg.blockDim = dim3(THREADS); cfg.dynamicSmemBytes = SMEM_TOTAL; cfg.stream = st;
+  cfg.attrs = attr; cfg.numAttrs = SPLIT ? 1 : 0;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, ns_product_kernel<MODE, BN, SPLIT>, ta, tb, p);
   return e == cudaSuccess ? (int)cudaGetLastError() : (int)e;
+}
+
+template <int MODE>
+static int product(const CUtensorMap& ta, const CUtensorMap& tb, Params p, cudaStream_t st) {
+  constexpr bool SYM = MODE == GRAM || MODE == SQUARE;
+  const int sms = sm_count(), kblocks = ((MODE == GRAM ? p.n : p.m) + BK - 1) / BK;
+  // Tiles that leave most SMs idle: clusters of up to 8 CTAs share their contraction, two blocks of it each at least.  The
+  // width of the tiles is the one whose longest CTA has the fewer clocks: a block of the contraction takes 1700 with 256
+  // columns and 1080 with 128, bound by shared memory (160 and 213 bytes a clock at the full tensor rate, of 128).
+  int splits[2];
+  long long total[2], cost[2];
+  for (int w = 0; w < 2; ++w) {
+    total[w] = (w ? tiles_of<256>(SYM, p.m, p.n) : tiles_of<128>(SYM, p.m, p.n)) * p.batch;
+    splits[w] = 1;
+    while (splits[w] < 8 && total[w] * splits[w] * 2 <= sms && kblocks >= 4 * splits[w]) splits[w] *= 2;
+    cost[w] = (total[w] * splits[w] + sms - 1) / sms * ((kblocks + splits[w] - 1) / splits[w]) * (w ? 1700 : 1080);
+  }
+  const int w = cost[1] < cost[0] ? 1 : 0;
+  p.splits = splits[w];
+  const int grid = (int)(p.splits > 1 ? total[w] * p.splits : (total[w] < sms ? total[w] : sms));
+  if (w) return p.splits > 1 ? launch<MODE, 256, true>(ta, tb, p, grid, st) : launch<MODE, 256, false>(ta, tb, p, grid, st);
+  return p.splits > 1 ? launch<MODE, 128, true>(ta, tb, p, grid, st) : launch<MODE, 128, false>(ta, tb, p, grid, st);
 }
 
 static inline long long up256(long long b) { return (b + 255) & ~255ll; }
