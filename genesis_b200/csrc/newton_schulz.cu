@@ -41,7 +41,6 @@ constexpr int BARRIER_OFFSET = SLAB_OFFSET + 8 * CHUNK_BYTES;
 constexpr int SMEM_TOTAL = BARRIER_OFFSET + 256;
 constexpr int THREADS = 384;                          // warps 0 TMA, 1 MMA, 2 and 3 idle, 4-11 epilogue
 constexpr int PARTS = 256;                            // most partial sums of squares per matrix
-constexpr int DRAIN = 4;                              // blocks of BK that one accumulator takes up: see the header
 
 enum Mode : int { GRAM = 0, SQUARE = 1, APPLY = 2, APPLY_LAST = 3 };
 
@@ -64,10 +63,17 @@ struct Params {
   int splits;                  // CTAs of a cluster that share a tile's contraction (1: whole tiles, persistent CTAs)
 };
 
-__device__ __forceinline__ void split(float x, __half& hi, __half& lo) {
-  hi = __float2half_rn(x);
-  lo = __float2half_rn(x - __half2float(hi));
+// Terms of four numbers, x = hi + lo to 22 bits: (hi0 hi1, hi2 hi3, lo0 lo1, lo2 lo3)
+__device__ __forceinline__ uint4 split4(float a, float b, float c, float d) {
+  uint4 t;
+  t.x = pack2c<false>(a, b);
+  t.y = pack2c<false>(c, d);
+  const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&t.x)), y = __half22float2(*reinterpret_cast<const __half2*>(&t.y));
+  t.z = pack2c<false>(a - x.x, b - x.y);
+  t.w = pack2c<false>(c - y.x, d - y.y);
+  return t;
 }
+__device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
 
 // Byte offset of 16-byte unit `u` of row `r` of a 32 x 32 chunk in shared memory.  Eight neighbouring rows, and the eight
 // rows r, r + 4, .., put a unit into eight different bank groups: rows written lane by lane, read unit by unit, and
@@ -83,26 +89,19 @@ __device__ __forceinline__ void cluster_barrier() {
   asm volatile("barrier.cluster.arrive.release;" ::: "memory");
   asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
 }
-__device__ __forceinline__ float4 ld_peer(uint32_t addr, uint32_t rank) {
+__device__ __forceinline__ float4 ld_peer(uint32_t addr) {
   float4 v;
-  asm volatile("{\n\t.reg .u32 a;\n\tmapa.shared::cluster.u32 a, %4, %5;\n\tld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [a];\n\t}"
-               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr), "r"(rank) : "memory");
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
   return v;
 }
+// A launch of this chain may start while the one before it runs; nothing that it wrote is touched before this returns.
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
-__device__ __forceinline__ void store4(void* p, int dt, size_t i, const float* v, int n, bool whole) {
-  if (whole) {                                        // four elements, aligned
-    if (dt == DT_F32) *reinterpret_cast<float4*>(reinterpret_cast<float*>(p) + i) = make_float4(v[0], v[1], v[2], v[3]);
-    else *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(p) + i) = make_uint2(pack2(v[0], v[1], dt), pack2(v[2], v[3], dt));
-  } else {
-#pragma unroll
-    for (int k = 0; k < 4; ++k)
-      if (k < n) store_from_float(p, dt, i + k, v[k]);
-  }
-}
-
-// What becomes of a 32 x 32 chunk of accumulators (rows row0.., columns col0.. of matrix z) that lies in shared memory.  A
-// lane takes four neighbouring columns of a row, eight lanes a row, so that memory sees whole 128-byte lines (64 of fp16).
+// What becomes of a 32 x 32 chunk of accumulators (rows row0.., columns col0.. of matrix z).  A lane takes four neighbouring
+// columns of a row, eight lanes a row, so that memory sees whole 128-byte lines (64 of fp16): acc[i] is row 4 i + lane / 8,
+// columns 4 (lane % 8)...  `chunk` is the warp's shared memory, for what goes out transposed.  All loads of a chunk are
+// issued before its first store: otherwise each row would wait for its own (24 of 4864 x 896: 5366 us against ...).
 template <int MODE>
 struct Epilogue {
   const Params& p;
@@ -119,134 +118,172 @@ struct Epilogue {
       vec = ((p.tall ? p.m : p.n) & 3) == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0;
     }
   }
-  __device__ __forceinline__ void run(uint8_t* chunk, int z, int row0, int col0) const {
-    const int cols = MODE == GRAM || MODE == SQUARE ? p.m : p.n;
+  __device__ __forceinline__ void run(const float4 (&acc)[8], uint8_t* chunk, int z, int row0, int col0) const {
+    constexpr bool SYM = MODE == GRAM || MODE == SQUARE;
+    const int cols = SYM ? p.m : p.n;
     if (row0 >= p.m || col0 >= cols) return;
     // symmetric results: blocks of 128 below the diagonal are written twice, those above it not at all
-    if ((MODE == GRAM || MODE == SQUARE) && col0 / BM > row0 / BM) return;
-    const bool mirror = col0 / BM < row0 / BM;
+    if (SYM && col0 / BM > row0 / BM) return;
     const int u = lane & 7, r0 = lane >> 3, col = col0 + 4 * u;
-    // everything that is read comes before the first store: eight loads of a lane are in flight together
-    if constexpr (MODE == GRAM || MODE == SQUARE) {
-      const size_t plane = (size_t)p.m * p.lda, zo = (size_t)z * 2 * plane;
-#pragma unroll 1
-      for (int pass = 0; pass <= (mirror ? 1 : 0); ++pass) {
-        // second pass, the transposed chunk: row col0 + r of the result, its columns row0 + 4 u .. + 3
-        const int i0 = pass ? col0 : row0, j = pass ? row0 + 4 * u : col;
-        __half* dst = p.dst + zo + (size_t)(i0 + r0) * p.lda + j;
-        const int rows = j < p.m ? p.m - i0 - r0 : 0;
-        uint2 ah[8], al[8];
-        if constexpr (MODE == SQUARE) {
-          const __half* a = p.a_planes + zo + (size_t)(i0 + r0) * p.lda + j;
+    const int rows = col < cols ? p.m - row0 - r0 : 0;           // (rows 4 i of this lane below it are inside the matrix)
+    if constexpr (SYM) {
+      const bool mirror = col0 / BM < row0 / BM;
+      const size_t plane = (size_t)p.m * p.lda, zo = (size_t)z * 2 * plane, at = zo + (size_t)(row0 + r0) * p.lda + col;
+      const size_t pitch = 4 * (size_t)p.lda;
+      uint2 ah[8], al[8];
+      if constexpr (MODE == SQUARE) {
 #pragma unroll
-          for (int it = 0; it < 8; ++it) {
-            ah[it] = al[it] = make_uint2(0u, 0u);
-            if (4 * it < rows) {
-              ah[it] = *reinterpret_cast<const uint2*>(a + (size_t)(4 * it) * p.lda);
-              al[it] = *reinterpret_cast<const uint2*>(a + (size_t)(4 * it) * p.lda + plane);
-            }
+        for (int i = 0; i < 8; ++i) {
+          ah[i] = al[i] = make_uint2(0u, 0u);
+          if (4 * i < rows) {
+            ah[i] = *reinterpret_cast<const uint2*>(p.a_planes + at + i * pitch);
+            al[i] = *reinterpret_cast<const uint2*>(p.a_planes + at + i * pitch + plane);
           }
         }
+      }
+      uint4 t[8];
 #pragma unroll
-        for (int it = 0; it < 8; ++it) {
-          if (4 * it < rows) {
-            float v[4];
-            if (pass) column(chunk, 4 * it + r0, u, v);
-            else row4(chunk, 4 * it + r0, u, v);
+      for (int i = 0; i < 8; ++i) {
+        float v[4] = {acc[i].x * p.f_acc, acc[i].y * p.f_acc, acc[i].z * p.f_acc, acc[i].w * p.f_acc};
+        if constexpr (MODE == SQUARE) add_a(v, ah[i], al[i]);
+        t[i] = split4(v[0], v[1], v[2], v[3]);
+      }
+      if (mirror) {
+        // both terms of an element in the place of its sum; then columns are read as rows
+        __syncwarp();
 #pragma unroll
-            for (int k = 0; k < 4; ++k) v[k] *= p.f_acc;
-            if constexpr (MODE == SQUARE) add_a(v, ah[it], al[it]);
-            put(dst + (size_t)(4 * it) * p.lda, plane, v);
-          }
+        for (int i = 0; i < 8; ++i)
+          *reinterpret_cast<uint4*>(chunk + chunk_at(4 * i + r0, u)) =
+              make_uint4(__byte_perm(t[i].x, t[i].z, 0x5410), __byte_perm(t[i].x, t[i].z, 0x7632),
+                         __byte_perm(t[i].y, t[i].w, 0x5410), __byte_perm(t[i].y, t[i].w, 0x7632));
+        __syncwarp();
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (4 * i < rows) put(p.dst + at + i * pitch, plane, t[i]);
+      if (mirror) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          uint32_t w[4];
+          column(chunk, 4 * i + r0, u, w);
+          t[i] = make_uint4(__byte_perm(w[0], w[1], 0x5410), __byte_perm(w[2], w[3], 0x5410), __byte_perm(w[0], w[1], 0x7632),
+                            __byte_perm(w[2], w[3], 0x7632));
         }
+        const int j = row0 + 4 * u, left = j < p.m ? p.m - col0 - r0 : 0;
+        __half* out = p.dst + zo + (size_t)(col0 + r0) * p.lda + j;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (4 * i < left) put(out + i * pitch, plane, t[i]);
       }
     } else {
-      bool across = false;                                       // the result is the transpose
-      if constexpr (MODE == APPLY_LAST) across = p.weights != nullptr ? (p.weights[z] & 1) != 0 : p.tall != 0;
-      const int rows = col < cols ? p.m - row0 - r0 : 0;
       float* x = p.x + ((size_t)z * p.m + row0 + r0) * p.ldx + col;
-      float4 o[8];
+      const size_t pitch = 4 * (size_t)p.ldx;
+      float4 v[8];
 #pragma unroll
-      for (int it = 0; it < 8; ++it)
-        o[it] = 4 * it < rows ? *reinterpret_cast<const float4*>(x + (size_t)(4 * it) * p.ldx) : make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int i = 0; i < 8; ++i)
+        v[i] = 4 * i < rows ? *reinterpret_cast<const float4*>(x + i * pitch) : make_float4(0.f, 0.f, 0.f, 0.f);
+      if constexpr (MODE == APPLY) {
+        const size_t plane = (size_t)p.m * p.ldx;
+        __half* dst = p.dst + (size_t)z * 2 * plane + (size_t)(row0 + r0) * p.ldx + col;
 #pragma unroll
-      for (int it = 0; it < 8; ++it) {
-        float4* a = reinterpret_cast<float4*>(chunk + chunk_at(4 * it + r0, u));
-        const float4 b = *a;
-        const float v[4] = {fmaf(b.x, p.f_acc, o[it].x * p.f_a), fmaf(b.y, p.f_acc, o[it].y * p.f_a),
-                            fmaf(b.z, p.f_acc, o[it].z * p.f_a), fmaf(b.w, p.f_acc, o[it].w * p.f_a)};
-        if constexpr (MODE == APPLY) {
-          if (4 * it < rows) {
-            *reinterpret_cast<float4*>(x + (size_t)(4 * it) * p.ldx) = make_float4(v[0], v[1], v[2], v[3]);
-            const size_t plane = (size_t)p.m * p.ldx;
-            const float w[4] = {v[0] * p.next_scale, v[1] * p.next_scale, v[2] * p.next_scale, v[3] * p.next_scale};
-            put(p.dst + (size_t)z * 2 * plane + (size_t)(row0 + r0 + 4 * it) * p.ldx + col, plane, w);
+        for (int i = 0; i < 8; ++i) {
+          v[i] = combine(acc[i], v[i]);
+          if (4 * i < rows) {
+            *reinterpret_cast<float4*>(x + i * pitch) = v[i];
+            const float f = p.next_scale;
+            put(dst + i * pitch, plane, split4(v[i].x * f, v[i].y * f, v[i].z * f, v[i].w * f));
           }
-        } else {
-          *a = make_float4(v[0], v[1], v[2], v[3]);
         }
-      }
-      if constexpr (MODE == APPLY_LAST) {
-        __syncwarp();
+      } else {
+        const bool across = p.weights != nullptr ? (p.weights[z] & 1) != 0 : p.tall != 0;     // the result is the transpose
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = combine(acc[i], v[i]);
+        if (across) {
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 8; ++i) *reinterpret_cast<float4*>(chunk + chunk_at(4 * i + r0, u)) = v[i];
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            uint32_t w[4];
+            column(chunk, 4 * i + r0, u, w);
+            v[i] = make_float4(__uint_as_float(w[0]), __uint_as_float(w[1]), __uint_as_float(w[2]), __uint_as_float(w[3]));
+          }
+        }
         const int i0 = across ? col0 : row0, j = across ? row0 + 4 * u : col;
         const int ld = across ? p.m : p.n, count = ld - j;       // elements of a row from here on
         const int left = count > 0 ? (across ? p.n : p.m) - i0 - r0 : 0;
-        const float st = across ? step * p.scale : step;
-        const size_t at = (size_t)(i0 + r0) * ld + j;
+        const size_t at = (size_t)(i0 + r0) * ld + j, lp = 4 * (size_t)ld;
         if (p.weights != nullptr) {
-          float* w = reinterpret_cast<float*>(p.weights[z] & ~1ll) + at;
-          if (skip) return;
-          if ((ld & 3) == 0 && (reinterpret_cast<uintptr_t>(w) & 15) == 0) {
+          if (!skip) apply(reinterpret_cast<float*>(p.weights[z] & ~1ll) + at, lp, left, count, ld, across ? step * p.scale : step, v);
+        } else if (p.out_dtype == DT_F32) {
+          float* o = reinterpret_cast<float*>(p.out) + (size_t)z * p.m * p.n + at;
 #pragma unroll
-            for (int it = 0; it < 8; ++it)
-              if (4 * it < left) o[it] = *reinterpret_cast<const float4*>(w + (size_t)(4 * it) * ld);
-#pragma unroll
-            for (int it = 0; it < 8; ++it) {
-              if (4 * it < left) {
-                float v[4];
-                if (across) column(chunk, 4 * it + r0, u, v);
-                else row4(chunk, 4 * it + r0, u, v);
-                *reinterpret_cast<float4*>(w + (size_t)(4 * it) * ld) =
-                    make_float4(fmaf(o[it].x, keep, -st * v[0]), fmaf(o[it].y, keep, -st * v[1]),
-                                fmaf(o[it].z, keep, -st * v[2]), fmaf(o[it].w, keep, -st * v[3]));
-              }
-            }
-          } else {
-#pragma unroll 1
-            for (int it = 0; it < 8; ++it) {
-              if (4 * it < left) {
-                float v[4];
-                if (across) column(chunk, 4 * it + r0, u, v);
-                else row4(chunk, 4 * it + r0, u, v);
-                float* q = w + (size_t)(4 * it) * ld;
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-                  if (k < count) q[k] = fmaf(q[k], keep, -st * v[k]);
-              }
+          for (int i = 0; i < 8; ++i) {
+            if (4 * i >= left) continue;
+            if (vec) *reinterpret_cast<float4*>(o + i * lp) = v[i];
+            else {
+              o[i * lp] = v[i].x;
+              if (count > 1) o[i * lp + 1] = v[i].y;
+              if (count > 2) o[i * lp + 2] = v[i].z;
+              if (count > 3) o[i * lp + 3] = v[i].w;
             }
           }
         } else {
+          uint16_t* o = reinterpret_cast<uint16_t*>(p.out) + (size_t)z * p.m * p.n + at;
+          const bool bf = p.out_dtype == DT_BF16;
 #pragma unroll
-          for (int it = 0; it < 8; ++it) {
-            if (4 * it < left) {
-              float v[4];
-              if (across) column(chunk, 4 * it + r0, u, v);
-              else row4(chunk, 4 * it + r0, u, v);
-              store4(p.out, p.out_dtype, (size_t)z * p.m * p.n + at + (size_t)(4 * it) * ld, v, count, vec);
+          for (int i = 0; i < 8; ++i) {
+            if (4 * i >= left) continue;
+            uint2 w;
+            if (bf) { w.x = pack2c<true>(v[i].x, v[i].y); w.y = pack2c<true>(v[i].z, v[i].w); }
+            else { w.x = pack2c<false>(v[i].x, v[i].y); w.y = pack2c<false>(v[i].z, v[i].w); }
+            if (vec) *reinterpret_cast<uint2*>(o + i * lp) = w;
+            else {
+              o[i * lp] = (uint16_t)w.x;
+              if (count > 1) o[i * lp + 1] = (uint16_t)(w.x >> 16);
+              if (count > 2) o[i * lp + 2] = (uint16_t)w.y;
+              if (count > 3) o[i * lp + 3] = (uint16_t)(w.y >> 16);
             }
           }
         }
       }
     }
   }
-  __device__ __forceinline__ void row4(const uint8_t* chunk, int r, int u, float (&v)[4]) const {
-    const float4 a = *reinterpret_cast<const float4*>(chunk + chunk_at(r, u));
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+  // rows 4 i of the weights from `w` on, `left` of them below, `count` elements each from here on
+  __device__ __forceinline__ void apply(float* w, size_t pitch, int left, int count, int ld, float st, const float4 (&v)[8]) const {
+    if ((ld & 3) == 0 && (reinterpret_cast<uintptr_t>(w) & 15) == 0) {
+      float4 o[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (4 * i < left) o[i] = *reinterpret_cast<const float4*>(w + i * pitch);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (4 * i < left)
+          *reinterpret_cast<float4*>(w + i * pitch) = make_float4(fmaf(o[i].x, keep, -st * v[i].x), fmaf(o[i].y, keep, -st * v[i].y),
+                                                                  fmaf(o[i].z, keep, -st * v[i].z), fmaf(o[i].w, keep, -st * v[i].w));
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (4 * i >= left) continue;
+        float* q = w + i * pitch;
+        q[0] = fmaf(q[0], keep, -st * v[i].x);
+        if (count > 1) q[1] = fmaf(q[1], keep, -st * v[i].y);
+        if (count > 2) q[2] = fmaf(q[2], keep, -st * v[i].z);
+        if (count > 3) q[3] = fmaf(q[3], keep, -st * v[i].w);
+      }
+    }
+  }
+  __device__ __forceinline__ float4 combine(const float4& a, const float4& x) const {
+    return make_float4(fmaf(a.x, p.f_acc, x.x * p.f_a), fmaf(a.y, p.f_acc, x.y * p.f_a), fmaf(a.z, p.f_acc, x.z * p.f_a),
+                       fmaf(a.w, p.f_acc, x.w * p.f_a));
   }
   // four rows 4 u .. of column `c` of the chunk
-  __device__ __forceinline__ void column(const uint8_t* chunk, int c, int u, float (&v)[4]) const {
+  __device__ __forceinline__ void column(const uint8_t* chunk, int c, int u, uint32_t (&v)[4]) const {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) v[k] = *reinterpret_cast<const float*>(chunk + chunk_at(4 * u + k, c >> 2) + (c & 3) * 4);
+    for (int k = 0; k < 4; ++k) v[k] = *reinterpret_cast<const uint32_t*>(chunk + chunk_at(4 * u + k, c >> 2) + (c & 3) * 4);
   }
   __device__ __forceinline__ void add_a(float (&v)[4], const uint2& x, const uint2& y) const {
     const float2 x0 = __half22float2(*reinterpret_cast<const __half2*>(&x.x)), x1 = __half22float2(*reinterpret_cast<const __half2*>(&x.y));
@@ -254,15 +291,23 @@ struct Epilogue {
     v[0] = fmaf(x0.x + y0.x, p.f_a, v[0]); v[1] = fmaf(x0.y + y0.y, p.f_a, v[1]);
     v[2] = fmaf(x1.x + y1.x, p.f_a, v[2]); v[3] = fmaf(x1.y + y1.y, p.f_a, v[3]);
   }
-  // both terms of four elements; the pitch is a multiple of 8, so what lies past the last column is padding
-  __device__ __forceinline__ void put(__half* hi, size_t plane, const float (&v)[4]) const {
-    uint2 h, l;
-    __half* h4 = reinterpret_cast<__half*>(&h);
-    __half* l4 = reinterpret_cast<__half*>(&l);
-#pragma unroll
-    for (int k = 0; k < 4; ++k) split(v[k], h4[k], l4[k]);
-    *reinterpret_cast<uint2*>(hi) = h;
-    *reinterpret_cast<uint2*>(hi + plane) = l;
+  // (the pitch is a multiple of 8, so what lies past the last column is padding)
+  __device__ __forceinline__ void put(__half* hi, size_t plane, const uint4& t) const {
+    *reinterpret_cast<uint2*>(hi) = make_uint2(t.x, t.y);
+    *reinterpret_cast<uint2*>(hi + plane) = make_uint2(t.z, t.w);
+  }
+  // What this lane's warp will read of a chunk at its end is fetched into L2 while the products run: one line a lane
+  __device__ __forceinline__ void prefetch(int z, int row0, int col0) const {
+    if constexpr (MODE == APPLY || MODE == APPLY_LAST) {
+      if (row0 + lane < p.m && col0 < p.n) prefetch_l2(p.x + ((size_t)z * p.m + row0 + lane) * p.ldx + col0);
+      if constexpr (MODE == APPLY_LAST) {
+        if (p.weights != nullptr) {
+          const float* w = reinterpret_cast<const float*>(p.weights[z] & ~1ll);
+          if (p.weights[z] & 1) { if (col0 + lane < p.n && row0 < p.m) prefetch_l2(w + (size_t)(col0 + lane) * p.m + row0); }
+          else if (row0 + lane < p.m && col0 < p.n) prefetch_l2(w + (size_t)(row0 + lane) * p.n + col0);
+        }
+      }
+    }
   }
 };
 
@@ -284,6 +329,7 @@ ns_product_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_consta
   // the order hi lo, hi hi, lo hi, so the first half is free before the block is done.
   constexpr int HALF_BYTES = A_BYTES + B_BYTES, HALVES = RING_BYTES / HALF_BYTES / 2 * 2;
   constexpr int ACCS = 512 / BN;                        // accumulators in tensor memory
+  constexpr int DRAIN = 4;                              // blocks of BK that one accumulator takes up: see the header
   constexpr int CHUNKS = BN / 64;                       // of 32 x 32 results, per epilogue warp
   extern __shared__ __align__(1024) uint8_t smem[];
   uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + BARRIER_OFFSET);
@@ -314,6 +360,8 @@ ns_product_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_consta
   __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem_base = *tmem_base_slot;
+  let_next_start();
+  wait_for_previous();
 
   const int tm = (p.m + BM - 1) / BM;
   const int per = (int)tiles_of<BN>(SYM, p.m, p.n);
@@ -448,6 +496,8 @@ ns_product_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_consta
       for (int h = 0; h < CHUNKS; ++h)
 #pragma unroll
         for (int j = 0; j < 32; ++j) v[h][j] = 0.f;
+      if constexpr (!SPLIT)
+        for (int h = 0; h < CHUNKS; ++h) epi.prefetch(z, mi * BM + q * 32, ni * BN + half * (BN / 2) + h * 32);
       for (int kb = kb0; kb < kb1; kb += DRAIN, ++drains) {
         const uint32_t acc = drains % ACCS;
         if (!__all_sync(0xffffffffu, mbar_wait(&tmem_full[acc], (drains / ACCS) & 1, abort_flag, p.status, 310))) { ok = false; break; }
@@ -475,7 +525,12 @@ ns_product_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_consta
         for (int u = 0; u < 8; ++u)
           *reinterpret_cast<float4*>(at + chunk_at(lane, u)) = make_float4(v[h][4 * u], v[h][4 * u + 1], v[h][4 * u + 2], v[h][4 * u + 3]);
         __syncwarp();
-        if constexpr (!SPLIT) epi.run(slab, z, mi * BM + q * 32, ni * BN + half * (BN / 2) + h * 32);
+        if constexpr (!SPLIT) {
+          float4 acc[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) acc[i] = *reinterpret_cast<const float4*>(slab + chunk_at(4 * i + (lane >> 3), lane & 7));
+          epi.run(acc, slab, z, mi * BM + q * 32, ni * BN + half * (BN / 2) + h * 32);
+        }
       }
     }
     if constexpr (SPLIT) {
@@ -488,19 +543,21 @@ ns_product_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_consta
         decode(first, mi, ni, z);
         for (int c = rank + (warp - 4) * splits; c < 8 * CHUNKS; c += 8 * splits) {
           __syncwarp();
-  #pragma unroll
-          for (int it = 0; it < 8; ++it) {
-            const int off = chunk_at(4 * it + (lane >> 3), lane & 7);
-            float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-            for (int k = 0; k < splits; ++k) {
-              const float4 o = ld_peer(smem_u32(smem) + c * CHUNK_BYTES + off, k);
-              sum.x += o.x; sum.y += o.y; sum.z += o.z; sum.w += o.w;
-            }
-            *reinterpret_cast<float4*>(slab + off) = sum;
+            float4 sum[8];
+#pragma unroll
+          for (int it = 0; it < 8; ++it) sum[it] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+          for (int k = 0; k < splits; ++k) {
+            uint32_t peer;
+            asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(peer) : "r"(smem_u32(smem) + c * CHUNK_BYTES), "r"(k));
+            float4 o[8];
+#pragma unroll
+            for (int it = 0; it < 8; ++it) o[it] = ld_peer(peer + chunk_at(4 * it + (lane >> 3), lane & 7));
+#pragma unroll
+            for (int it = 0; it < 8; ++it) { sum[it].x += o[it].x; sum[it].y += o[it].y; sum[it].z += o[it].z; sum[it].w += o[it].w; }
           }
-          __syncwarp();
           const int w = c / CHUNKS;                        // the warp whose chunk this was, and where its rows and columns are
-          epi.run(slab, z, mi * BM + (w & 3) * 32, ni * BN + (w >> 2) * (BN / 2) + (c % CHUNKS) * 32);
+          epi.run(sum, slab, z, mi * BM + (w & 3) * 32, ni * BN + (w >> 2) * (BN / 2) + (c % CHUNKS) * 32);
         }
       }
       cluster_barrier();                                   // nobody leaves while its part may still be read
@@ -622,6 +679,8 @@ ns_prepare_kernel(const void* __restrict__ src, int dt, int m, int n, int tall, 
   __shared__ float tile[128][33];
   __shared__ double sh[8];
   const int z = blockIdx.z, i0 = blockIdx.y * 32, j0 = blockIdx.x * 128;
+  let_next_start();
+  wait_for_previous();
   const double inv = 1.0 / (sqrt(block_sum256((int)threadIdx.x < parts ? partial[z * PARTS + threadIdx.x] : 0.0, sh)) + eps);
   const void* g = reinterpret_cast<const uint8_t*>(src) + (size_t)z * m * n * (dt == DT_F32 ? 4 : 2);
   if (weights != nullptr) tall = (int)(weights[z] & 1);
@@ -632,13 +691,9 @@ ns_prepare_kernel(const void* __restrict__ src, int dt, int m, int n, int tall, 
   auto put = [&](int i, int j, float4 v) {               // (the pitch is a multiple of 8: four elements stay inside it)
     const size_t o = (size_t)i * ldx + j;
     *reinterpret_cast<float4*>(xz + o) = v;
-    uint2 h, l;
-    __half* h4 = reinterpret_cast<__half*>(&h);
-    __half* l4 = reinterpret_cast<__half*>(&l);
-    split(v.x * scale, h4[0], l4[0]); split(v.y * scale, h4[1], l4[1]);
-    split(v.z * scale, h4[2], l4[2]); split(v.w * scale, h4[3], l4[3]);
-    *reinterpret_cast<uint2*>(hi + o) = h;
-    *reinterpret_cast<uint2*>(hi + plane + o) = l;
+    const uint4 t = split4(v.x * scale, v.y * scale, v.z * scale, v.w * scale);
+    *reinterpret_cast<uint2*>(hi + o) = make_uint2(t.x, t.y);
+    *reinterpret_cast<uint2*>(hi + plane + o) = make_uint2(t.z, t.w);
   };
   auto norm = [&](float a) { return (float)((double)a * inv); };
   if (!tall) {
@@ -696,34 +751,62 @@ static int launch(const CUtensorMap& ta, const CUtensorMap& tb, const Params& p,
   static unsigned long long configured = 0;
   if (int r = smem_opt_in(ns_product_kernel<MODE, BN, SPLIT>, SMEM_TOTAL, configured)) return r;
   cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = p.splits; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = p.splits; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
   cfg.gridDim = dim3((unsigned)grid); cfg.blockDim = dim3(THREADS); cfg.dynamicSmemBytes = SMEM_TOTAL; cfg.stream = st;
-  cfg.attrs = attr; cfg.numAttrs = SPLIT ? 1 : 0;
+  cfg.attrs = attr; cfg.numAttrs = SPLIT ? 2 : 1;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, ns_product_kernel<MODE, BN, SPLIT>, ta, tb, p);
   return e == cudaSuccess ? (int)cudaGetLastError() : (int)e;
+}
+
+// How many clusters of 2, 4, 8 CTAs of this size the device holds at once: a cluster stays inside one group of SMs, and
+// groups differ in size, so it is less than the number of SMs allows (asked for once per device).
+static int max_clusters(int size) {
+  static int known[64][4] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  int& n = known[dev & 63][size == 2 ? 1 : size == 4 ? 2 : 3];
+  if (n == 0) {
+    auto kern = ns_product_kernel<GRAM, 128, true>;
+    static unsigned long long configured = 0;
+    if (smem_opt_in(kern, SMEM_TOTAL, configured)) return 1;
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = size; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    cfg.gridDim = dim3(size); cfg.blockDim = dim3(THREADS); cfg.dynamicSmemBytes = SMEM_TOTAL; cfg.attrs = attr; cfg.numAttrs = 1;
+    int got = 0;
+    if (cudaOccupancyMaxActiveClusters(&got, kern, &cfg) != cudaSuccess || got < 1) { cudaGetLastError(); got = 1; }
+    n = got;
+  }
+  return n;
 }
 
 template <int MODE>
 static int product(const CUtensorMap& ta, const CUtensorMap& tb, Params p, cudaStream_t st) {
   constexpr bool SYM = MODE == GRAM || MODE == SQUARE;
   const int sms = sm_count(), kblocks = ((MODE == GRAM ? p.n : p.m) + BK - 1) / BK;
-  // Tiles that leave most SMs idle: clusters of up to 8 CTAs share their contraction, two blocks of it each at least.  The
-  // width of the tiles is the one whose longest CTA has the fewer clocks: a block of the contraction takes 1700 with 256
-  // columns and 1080 with 128, bound by shared memory (160 and 213 bytes a clock at the full tensor rate, of 128).
-  int splits[2];
-  long long total[2], cost[2];
+  // Width of the tiles, and how many CTAs of a cluster share a tile's contraction where tiles are few: whatever has the
+  // fewest clocks on its longest CTA.  A block of the contraction takes 1700 clocks with 256 columns and 1080 with 128, bound
+  // by shared memory (160 and 213 bytes a clock at the full tensor rate, of 128); a start and its epilogue 8000 and 6000;
+  // the exchange of a cluster 4000.
+  int best_w = 0;
+  long long best = -1, best_total = 0;
+  p.splits = 1;
   for (int w = 0; w < 2; ++w) {
-    total[w] = (w ? tiles_of<256>(SYM, p.m, p.n) : tiles_of<128>(SYM, p.m, p.n)) * p.batch;
-    splits[w] = 1;
-    while (splits[w] < 8 && total[w] * splits[w] * 2 <= sms && kblocks >= 4 * splits[w]) splits[w] *= 2;
-    cost[w] = (total[w] * splits[w] + sms - 1) / sms * ((kblocks + splits[w] - 1) / splits[w]) * (w ? 1700 : 1080);
+    const long long total = (w ? tiles_of<256>(SYM, p.m, p.n) : tiles_of<128>(SYM, p.m, p.n)) * p.batch;
+    for (int s = 1; s == 1 || (s <= 8 && kblocks >= 2 * s); s *= 2) {
+      if (s > 1 && total > max_clusters(s)) break;              // clusters take one tile each: a single wave of them
+      const long long waves = s > 1 ? 1 : (total + sms - 1) / sms;
+      const long long t = waves * ((kblocks + s - 1) / s) * (w ? 1700 : 1080) + (w ? 8000 : 6000) + (s > 1 ? 4000 : 0);
+      if (best < 0 || t < best) { best = t; best_w = w; best_total = total; p.splits = s; }
+    }
   }
-  const int w = cost[1] < cost[0] ? 1 : 0;
-  p.splits = splits[w];
-  const int grid = (int)(p.splits > 1 ? total[w] * p.splits : (total[w] < sms ? total[w] : sms));
-  if (w) return p.splits > 1 ? launch<MODE, 256, true>(ta, tb, p, grid, st) : launch<MODE, 256, false>(ta, tb, p, grid, st);
+  const int grid = (int)(p.splits > 1 ? best_total * p.splits : (best_total < sms ? best_total : sms));
+  if (best_w) return p.splits > 1 ? launch<MODE, 256, true>(ta, tb, p, grid, st) : launch<MODE, 256, false>(ta, tb, p, grid, st);
   return p.splits > 1 ? launch<MODE, 128, true>(ta, tb, p, grid, st) : launch<MODE, 128, false>(ta, tb, p, grid, st);
 }
 
@@ -787,9 +870,15 @@ extern "C" int gb_newton_schulz(const void* src, void* out, int dt, int m, int n
   const dim3 grid((n + 127) / 128, (m + 31) / 32, batch);
   if (grid.y > 65535) return -3;
   if (src != nullptr) ns::ns_norm_kernel<<<dim3(parts, batch), 256, 0, st>>>(src, dt, (long long)m * n, w.partial);
-  ns::ns_prepare_kernel<<<grid, 256, 0, st>>>(src != nullptr ? src : w.y, src != nullptr ? dt : (int)DT_F32, m, n, tall, weights,
-                                              w.partial, parts, eps, ldexpf(1.f, exponents[0]), w.x, w.xp[0], ldx);
-  if (const int e = (int)cudaGetLastError()) return e;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = grid; cfg.blockDim = dim3(256); cfg.stream = st; cfg.attrs = attr; cfg.numAttrs = 1;
+  const void* g = src != nullptr ? src : (const void*)w.y;
+  const int g_dt = src != nullptr ? dt : (int)DT_F32;
+  if (const cudaError_t e = cudaLaunchKernelEx(&cfg, ns::ns_prepare_kernel, g, g_dt, m, n, tall, weights, (const double*)w.partial,
+                                               parts, eps, ldexpf(1.f, exponents[0]), w.x, w.xp[0], ldx)) return (int)e;
   // maps: X as left or right operand of X X^T, X as right operand of B X (64 rows of the contraction at a time), A, B
   CUtensorMap mx[2], mxr[2], ma, mb;
   int r;
