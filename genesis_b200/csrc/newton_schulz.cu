@@ -20,9 +20,10 @@
 // Tiles too few to fill the GPU are shared by clusters of up to 8 CTAs, each with a part of the contraction.
 //
 // Sums.  The tensor cores round their accumulator towards zero, which adds up over a long contraction (4864 x 896: 1.6e-5 of
-// the result).  So an accumulator takes up 256 elements of the contraction and is then added, rounded to nearest, to the
+// the result).  So an accumulator takes up 512 elements of the contraction (256 in tiles of 128 columns) and is then added, rounded to nearest, to the
 // sums that the epilogue's warps hold in registers; the products go on in the next of four accumulators meanwhile.
 #include "sm100_ptx.cuh"
+#include "sm100_pair.cuh"
 #include "common.cuh"
 
 namespace gb {
@@ -80,15 +81,6 @@ __device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefe
 // columns read four rows apart are all free of conflicts.
 __device__ __forceinline__ int chunk_at(int r, int u) { return r * 128 + ((u ^ r ^ (r >> 3)) & 7) * 16; }
 
-__device__ __forceinline__ uint32_t cluster_rank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ void cluster_barrier() {
-  asm volatile("barrier.cluster.arrive.release;" ::: "memory");
-  asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
-}
 __device__ __forceinline__ float4 ld_peer(uint32_t addr) {
   float4 v;
   asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
@@ -100,8 +92,9 @@ __device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.
 
 // What becomes of a 32 x 32 chunk of accumulators (rows row0.., columns col0.. of matrix z).  A lane takes four neighbouring
 // columns of a row, eight lanes a row, so that memory sees whole 128-byte lines (64 of fp16): acc[i] is row 4 i + lane / 8,
-// columns 4 (lane % 8)...  `chunk` is the warp's shared memory, for what goes out transposed.  All loads of a chunk are
-// issued before its first store: otherwise each row would wait for its own (24 of 4864 x 896: 5366 us against ...).
+// columns 4 (lane % 8)...  `chunk` is the warp's shared memory, for what goes out transposed.  What a chunk reads is fetched
+// while the chunk before it is worked on: with the loads of a row behind the stores of the row before it, each row waited
+// for its own, and an epilogue took twice as long as the products of its tile.
 template <int MODE>
 struct Epilogue {
   const Params& p;
@@ -118,34 +111,46 @@ struct Epilogue {
       vec = ((p.tall ? p.m : p.n) & 3) == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0;
     }
   }
-  __device__ __forceinline__ void run(const float4 (&acc)[8], uint8_t* chunk, int z, int row0, int col0) const {
+  // symmetric results: blocks of 128 below the diagonal are written twice, those above it not at all
+  __device__ __forceinline__ bool outside(int row0, int col0) const {
+    constexpr bool SYM = MODE == GRAM || MODE == SQUARE;
+    return row0 >= p.m || col0 >= (SYM ? p.m : p.n) || (SYM && col0 / BM > row0 / BM);
+  }
+  // What a chunk's results are made from besides its sums: X, or both terms of A
+  __device__ __forceinline__ void fetch(uint4 (&in)[8], int z, int row0, int col0) const {
+    const int u = lane & 7, r0 = lane >> 3, col = col0 + 4 * u;
+    if constexpr (MODE != GRAM) {
+      const int rows = outside(row0, col0) || col >= (MODE == SQUARE ? p.m : p.n) ? 0 : p.m - row0 - r0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        in[i] = make_uint4(0u, 0u, 0u, 0u);
+        if (4 * i >= rows) continue;
+        if constexpr (MODE == SQUARE) {
+          const size_t plane = (size_t)p.m * p.lda;
+          const __half* a = p.a_planes + (size_t)z * 2 * plane + (size_t)(row0 + r0 + 4 * i) * p.lda + col;
+          const uint2 hi = *reinterpret_cast<const uint2*>(a), lo = *reinterpret_cast<const uint2*>(a + plane);
+          in[i] = make_uint4(hi.x, hi.y, lo.x, lo.y);
+        } else {
+          in[i] = *reinterpret_cast<const uint4*>(p.x + ((size_t)z * p.m + row0 + r0 + 4 * i) * p.ldx + col);
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ void run(const float4 (&acc)[8], const uint4 (&in)[8], uint8_t* chunk, int z, int row0, int col0) const {
     constexpr bool SYM = MODE == GRAM || MODE == SQUARE;
     const int cols = SYM ? p.m : p.n;
-    if (row0 >= p.m || col0 >= cols) return;
-    // symmetric results: blocks of 128 below the diagonal are written twice, those above it not at all
-    if (SYM && col0 / BM > row0 / BM) return;
+    if (outside(row0, col0)) return;
     const int u = lane & 7, r0 = lane >> 3, col = col0 + 4 * u;
     const int rows = col < cols ? p.m - row0 - r0 : 0;           // (rows 4 i of this lane below it are inside the matrix)
     if constexpr (SYM) {
       const bool mirror = col0 / BM < row0 / BM;
       const size_t plane = (size_t)p.m * p.lda, zo = (size_t)z * 2 * plane, at = zo + (size_t)(row0 + r0) * p.lda + col;
       const size_t pitch = 4 * (size_t)p.lda;
-      uint2 ah[8], al[8];
-      if constexpr (MODE == SQUARE) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          ah[i] = al[i] = make_uint2(0u, 0u);
-          if (4 * i < rows) {
-            ah[i] = *reinterpret_cast<const uint2*>(p.a_planes + at + i * pitch);
-            al[i] = *reinterpret_cast<const uint2*>(p.a_planes + at + i * pitch + plane);
-          }
-        }
-      }
       uint4 t[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         float v[4] = {acc[i].x * p.f_acc, acc[i].y * p.f_acc, acc[i].z * p.f_acc, acc[i].w * p.f_acc};
-        if constexpr (MODE == SQUARE) add_a(v, ah[i], al[i]);
+        if constexpr (MODE == SQUARE) add_a(v, make_uint2(in[i].x, in[i].y), make_uint2(in[i].z, in[i].w));
         t[i] = split4(v[0], v[1], v[2], v[3]);
       }
       if (mirror) {
@@ -181,7 +186,7 @@ struct Epilogue {
       float4 v[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        v[i] = 4 * i < rows ? *reinterpret_cast<const float4*>(x + i * pitch) : make_float4(0.f, 0.f, 0.f, 0.f);
+        v[i] = make_float4(__uint_as_float(in[i].x), __uint_as_float(in[i].y), __uint_as_float(in[i].z), __uint_as_float(in[i].w));
       if constexpr (MODE == APPLY) {
         const size_t plane = (size_t)p.m * p.ldx;
         __half* dst = p.dst + (size_t)z * 2 * plane + (size_t)(row0 + r0) * p.ldx + col;
@@ -311,72 +316,87 @@ struct Epilogue {
   }
 };
 
-// Tiles of BM x BN: for the symmetric modes those that hold a block of 128 x 128 on or below the diagonal, row by row
-template <int BN>
-__host__ __device__ constexpr long long tiles_of(bool sym, long long m, long long n) {
-  const long long tm = (m + BM - 1) / BM;
-  if (!sym) return tm * ((n + BN - 1) / BN);
-  return BN == 128 ? tm * (tm + 1) / 2 : (tm + 1) / 2 * (tm + 1 - (tm + 1) / 2);
+// How CTAs work on tiles: each on whole ones; the CTAs of a cluster each on a part of the contraction of one tile; two CTAs
+// on a tile of twice the rows, through the tensor instructions of CTA pairs.
+enum Kind : int { WHOLE = 0, SPLIT = 1, PAIR = 2 };
+
+// Tiles of `rows` x BN: for the symmetric modes those that hold a block of 128 x 128 on or below the diagonal, row by row
+__host__ __device__ constexpr long long tiles_of(bool sym, long long m, long long n, int rows, int bn) {
+  const long long tm = (m + rows - 1) / rows;
+  if (!sym) return tm * ((n + bn - 1) / bn);
+  return bn == rows ? tm * (tm + 1) / 2 : (tm + 1) / 2 * (tm + 1 - (tm + 1) / 2);
 }
 
-template <int MODE, int BN, bool SPLIT>
+template <int MODE, int BN, int KIND>
 __global__ void __launch_bounds__(THREADS, 1)
 ns_product_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_constant__ CUtensorMap tmapB, const Params p) {
   constexpr bool SYM = MODE == GRAM || MODE == SQUARE;
   constexpr bool B_MN = !SYM;                           // X as the right operand: its rows run along the contraction
-  constexpr int B_BYTES = BN * 128;
+  constexpr int TM = KIND == PAIR ? 2 * BM : BM;        // rows of a tile
+  constexpr int BNC = KIND == PAIR ? BN / 2 : BN;       // columns of the right operand that a CTA loads
   // Ring of half stages: (A hi, B lo) and (A lo, B hi) of a block of the contraction.  The three products of a block run in
   // the order hi lo, hi hi, lo hi, so the first half is free before the block is done.
-  constexpr int HALF_BYTES = A_BYTES + B_BYTES, HALVES = RING_BYTES / HALF_BYTES / 2 * 2;
+  constexpr int HALF_BYTES = A_BYTES + BNC * 128, HALVES = RING_BYTES / HALF_BYTES / 2 * 2;
   constexpr int ACCS = 512 / BN;                        // accumulators in tensor memory
-  constexpr int DRAIN = 4;                              // blocks of BK that one accumulator takes up: see the header
+  constexpr int DRAIN = BN == 256 ? 8 : 4;              // blocks of BK that one accumulator takes up: see the header
   constexpr int CHUNKS = BN / 64;                       // of 32 x 32 results, per epilogue warp
   extern __shared__ __align__(1024) uint8_t smem[];
-  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + BARRIER_OFFSET);
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + BARRIER_OFFSET);       // (a pair: those of CTA 0 count both CTAs' loads)
   uint64_t* empty_bar = full_bar + HALVES;
   uint64_t* tmem_full = empty_bar + HALVES;
-  uint64_t* tmem_empty = tmem_full + ACCS;
+  uint64_t* tmem_empty = tmem_full + ACCS;                                       // (a pair: those of CTA 0 count both epilogues)
   uint32_t* tmem_base_slot = reinterpret_cast<uint32_t*>(tmem_empty + ACCS);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_base_slot + 1);
+  uint32_t* poison_slot = tmem_base_slot + 2;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
   const int lane = threadIdx.x & 31;
+  const int rank = KIND == WHOLE ? 0 : (int)g2::cta_rank_in_cluster();
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < HALVES; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], 1); }
-    for (int a = 0; a < ACCS; ++a) { mbar_init(&tmem_full[a], 1); mbar_init(&tmem_empty[a], 8); }
+    for (int a = 0; a < ACCS; ++a) { mbar_init(&tmem_full[a], 1); mbar_init(&tmem_empty[a], KIND == PAIR ? 16 : 8); }
     // after an error no work is done, but every CTA of a cluster comes to its barriers
     const bool aligned = (smem_u32(smem) & 1023) == 0;
     if (!aligned) report_error(p.status, GB_ERR_BAD_ARG, 5, 0);
     *abort_flag = !aligned || status_poisoned(p.status) ? 1 : 0;
+    *poison_slot = (uint32_t)*abort_flag;
     mbar_fence_init();
     tma_prefetch_desc(&tmapA);
     tma_prefetch_desc(&tmapB);
   }
   if (warp == 1) {
-    tmem_alloc(tmem_base_slot, 512);
-    tmem_relinquish();
+    if constexpr (KIND == PAIR) { g2::tmem_alloc2(tmem_base_slot, 512); g2::tmem_relinquish2(); }
+    else { tmem_alloc(tmem_base_slot, 512); tmem_relinquish(); }
   }
   tc_fence_before_sync();
   __syncthreads();
+  if constexpr (KIND == PAIR) {
+    // the two decide alike whether they work
+    g2::cluster_sync_all();
+    const uint32_t other = g2::ld_cluster_u32(g2::map_to_cta(smem_u32(poison_slot), rank ^ 1));
+    if (threadIdx.x == 0 && other != 0) *abort_flag = 1;
+    __syncthreads();
+  }
   tc_fence_after_sync();
   const uint32_t tmem_base = *tmem_base_slot;
   let_next_start();
   wait_for_previous();
 
-  const int tm = (p.m + BM - 1) / BM;
-  const int per = (int)tiles_of<BN>(SYM, p.m, p.n);
+  const int tm = (p.m + TM - 1) / TM;
+  const int per = (int)tiles_of(SYM, p.m, p.n, TM, BN);
   const long long total = (long long)per * p.batch;
   const int kblocks = ((MODE == GRAM ? p.n : p.m) + BK - 1) / BK;
   // this CTA's tiles and its part of their contraction, in blocks of BK
-  const int splits = SPLIT ? p.splits : 1, rank = SPLIT ? (int)cluster_rank() : 0;
-  const long long first = blockIdx.x / splits, stride = gridDim.x / splits;
-  const int kb0 = kblocks * rank / splits, kb1 = kblocks * (rank + 1) / splits;
+  const int splits = KIND == SPLIT ? p.splits : 1, group = KIND == PAIR ? 2 : splits;
+  const long long first = blockIdx.x / group, stride = gridDim.x / group;
+  const int kb0 = KIND == SPLIT ? kblocks * rank / splits : 0, kb1 = KIND == SPLIT ? kblocks * (rank + 1) / splits : kblocks;
+  const int row_in_tile = KIND == PAIR ? rank * BM : 0;
   // tile of matrix z: (mi, ni)
   auto decode = [&](long long t, int& mi, int& ni, int& z) {
     z = (int)(t / per);
     const int r = (int)(t % per);
     if constexpr (SYM) {
-      if constexpr (BN == 128) {
+      if constexpr (BN == TM) {
         mi = (int)((sqrtf(8.f * (float)r + 1.f) - 1.f) * 0.5f);
         while (mi * (mi + 1) / 2 > r) --mi;
         while ((mi + 1) * (mi + 2) / 2 <= r) ++mi;
@@ -395,90 +415,120 @@ ns_product_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_consta
       mi = r % tm;
     }
   };
+  // a role that gives up takes the pair with it
+  auto give_up = [&]() {
+    if constexpr (KIND == PAIR) g2::st_cluster_u32(g2::map_to_cta(smem_u32(const_cast<int*>(abort_flag)), rank ^ 1), 1u);
+  };
 
   // The sums of a 128 x 256 tile take 128 registers of every epilogue thread: of 384 x 168 at launch, the first four warps
   // keep 56 each and the others get 224 (128 x 56 + 256 x 224 = 384 x 168).
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     if (warp == 0) {
-    // =========================== TMA producer ===========================
-    if (elect_one()) {
-      uint32_t it = 0;
-      for (long long t = first; t < total && !*abort_flag; t += stride) {
-        int mi, ni, z;
-        decode(t, mi, ni, z);
-        for (int kh = 2 * kb0; kh < 2 * kb1; ++kh, ++it) {
-          const int s = it % HALVES, k0 = (kh >> 1) * BK, h = kh & 1;        // h: A's term (0 = hi); B's is the other
-          if (!mbar_wait(&empty_bar[s], ((it / HALVES) & 1) ^ 1, abort_flag, p.status, 110)) break;
-          uint8_t* sa = smem + s * HALF_BYTES;
-          uint8_t* sb = sa + A_BYTES;
-          mbar_expect_tx(&full_bar[s], HALF_BYTES);
-          tma_load_3d(sa, &tmapA, &full_bar[s], k0, mi * BM, 2 * z + h);
-          if constexpr (!B_MN) {
+      // =========================== TMA producer ===========================
+      if (elect_one()) {
+        uint32_t it = 0;
+        for (long long t = first; t < total && !*abort_flag; t += stride) {
+          int mi, ni, z;
+          decode(t, mi, ni, z);
+          const int m0 = mi * TM + row_in_tile, n0 = ni * BN + (KIND == PAIR ? rank * BNC : 0);
+          bool ok = true;
+          for (int kh = 2 * kb0; kh < 2 * kb1; ++kh, ++it) {
+            const int s = it % HALVES, k0 = (kh >> 1) * BK, h = kh & 1;      // h: A's term (0 = hi); B's is the other
+            if (!mbar_wait(&empty_bar[s], ((it / HALVES) & 1) ^ 1, abort_flag, p.status, 110)) { ok = false; break; }
+            uint8_t* sa = smem + s * HALF_BYTES;
+            uint8_t* sb = sa + A_BYTES;
+            if constexpr (KIND == PAIR) {
+              const uint32_t bar = g2::map_to_cta(smem_u32(&full_bar[s]), 0);
+              if (rank == 0) mbar_expect_tx(&full_bar[s], 2 * HALF_BYTES);
+              g2::tma2_load_3d(sa, &tmapA, bar, k0, m0, 2 * z + h);
+              if constexpr (!B_MN) {
+                g2::tma2_load_3d(sb, &tmapB, bar, k0, n0, 2 * z + 1 - h);
+              } else {
 #pragma unroll
-            for (int c = 0; c < BN / 128; ++c)
-              tma_load_3d(sb + c * A_BYTES, &tmapB, &full_bar[s], k0, ni * BN + c * 128, 2 * z + 1 - h);
-          } else {
+                for (int c = 0; c < BNC / 64; ++c) g2::tma2_load_3d(sb + c * (BK * 128), &tmapB, bar, n0 + c * 64, k0, 2 * z + 1 - h);
+              }
+            } else {
+              mbar_expect_tx(&full_bar[s], HALF_BYTES);
+              tma_load_3d(sa, &tmapA, &full_bar[s], k0, m0, 2 * z + h);
+              if constexpr (!B_MN) {
 #pragma unroll
-            for (int c = 0; c < BN / 64; ++c)
-              tma_load_3d(sb + c * (BK * 128), &tmapB, &full_bar[s], ni * BN + c * 64, k0, 2 * z + 1 - h);
+                for (int c = 0; c < BNC / 128; ++c)
+                  tma_load_3d(sb + c * A_BYTES, &tmapB, &full_bar[s], k0, n0 + c * 128, 2 * z + 1 - h);
+              } else {
+#pragma unroll
+                for (int c = 0; c < BNC / 64; ++c) tma_load_3d(sb + c * (BK * 128), &tmapB, &full_bar[s], n0 + c * 64, k0, 2 * z + 1 - h);
+              }
+            }
+          }
+          if (!ok) { give_up(); break; }
+        }
+        if (*abort_flag && (KIND != PAIR || rank == 0)) drain_copies(full_bar, HALVES, it);
+      }
+      __syncwarp();
+    } else if (warp == 1 && (KIND != PAIR || rank == 0)) {
+      // =========================== MMA issuer (converged warp, one elected lane) ===========================
+      const uint32_t idesc = make_idesc(0u, 0u, B_MN ? 1u : 0u, TM, BN);
+      uint32_t it = 0, drains = 0;
+      bool ok = __all_sync(0xffffffffu, *abort_flag == 0);
+      auto b_desc = [&](uint32_t addr) { return B_MN ? make_smem_desc(addr, BK * 128, 1024) : make_smem_desc(addr, 16, 1024); };
+      auto multiply = [&](uint32_t d, uint64_t a, uint64_t b, bool fresh) {
+#pragma unroll
+        for (int kk = 0; kk < BK / 16; ++kk) {                               // (descriptors count 16-byte units)
+          const uint64_t bk = b + (B_MN ? kk * 128 : kk * 2);
+          if constexpr (KIND == PAIR) g2::umma2_f16(d, a + kk * 2, bk, idesc, fresh && kk == 0 ? 0u : 1u);
+          else umma_f16(d, a + kk * 2, bk, idesc, fresh && kk == 0 ? 0u : 1u);
+        }
+      };
+      auto commit = [&](uint64_t* bar) {                                     // (in both CTAs of a pair)
+        if constexpr (KIND == PAIR) {
+          g2::umma2_commit(smem_u32(bar));
+          g2::umma2_commit(g2::map_to_cta(smem_u32(bar), 1));
+        } else {
+          umma_commit(bar);
+        }
+      };
+      for (long long t = first; t < total && ok; t += stride) {
+        for (int kb = kb0; kb < kb1 && ok; kb += DRAIN, ++drains) {
+          const uint32_t acc = drains % ACCS;
+          if (!__all_sync(0xffffffffu, mbar_wait(&tmem_empty[acc], ((drains / ACCS) & 1) ^ 1, abort_flag, p.status, 210))) { ok = false; break; }
+          tc_fence_after_sync();
+          const uint32_t d_tmem = tmem_base + acc * BN;
+          const int end = min(kb + DRAIN, kb1);
+          for (int k = kb; k < end; ++k, it += 2) {
+            const int s = it % HALVES;                                       // (even: HALVES is)
+            const uint32_t ph = (it / HALVES) & 1;
+            if (!__all_sync(0xffffffffu, mbar_wait(&full_bar[s], ph, abort_flag, p.status, 211))) { ok = false; break; }
+            tc_fence_after_sync();
+            const uint32_t x_addr = smem_u32(smem + s * HALF_BYTES), y_addr = x_addr + HALF_BYTES;
+            const uint64_t a_hi = make_smem_desc(x_addr, 16, 1024), b_lo = b_desc(x_addr + A_BYTES);
+            const uint64_t a_lo = make_smem_desc(y_addr, 16, 1024), b_hi = b_desc(y_addr + A_BYTES);
+            if (elect_one()) multiply(d_tmem, a_hi, b_lo, k == kb);
+            __syncwarp();
+            if (!__all_sync(0xffffffffu, mbar_wait(&full_bar[s + 1], ph, abort_flag, p.status, 212))) { ok = false; break; }
+            tc_fence_after_sync();
+            if (elect_one()) {
+              multiply(d_tmem, a_hi, b_hi, false);
+              commit(&empty_bar[s]);
+              multiply(d_tmem, a_lo, b_hi, false);
+              commit(&empty_bar[s + 1]);
+            }
+            __syncwarp();
+          }
+          if (ok) {
+            if (elect_one()) commit(&tmem_full[acc]);
+            __syncwarp();
           }
         }
       }
-      if (*abort_flag) drain_copies(full_bar, HALVES, it);
+      if (!ok && lane == 0) give_up();
+      __syncwarp();
     }
-    __syncwarp();
-  } else if (warp == 1) {
-    // =========================== MMA issuer (converged warp, one elected lane) ===========================
-    const uint32_t idesc = make_idesc(0u, 0u, B_MN ? 1u : 0u, BM, BN);
-    uint32_t it = 0, drains = 0;
-    bool ok = __all_sync(0xffffffffu, *abort_flag == 0);
-    auto b_desc = [&](uint32_t addr) { return B_MN ? make_smem_desc(addr, BK * 128, 1024) : make_smem_desc(addr, 16, 1024); };
-    auto multiply = [&](uint32_t d, uint64_t a, uint64_t b, bool fresh) {
-#pragma unroll
-      for (int kk = 0; kk < BK / 16; ++kk)                                   // (descriptors count 16-byte units)
-        umma_f16(d, a + kk * 2, b + (B_MN ? kk * 128 : kk * 2), idesc, fresh && kk == 0 ? 0u : 1u);
-    };
-    for (long long t = first; t < total && ok; t += stride) {
-      for (int kb = kb0; kb < kb1 && ok; kb += DRAIN, ++drains) {
-        const uint32_t acc = drains % ACCS;
-        if (!__all_sync(0xffffffffu, mbar_wait(&tmem_empty[acc], ((drains / ACCS) & 1) ^ 1, abort_flag, p.status, 210))) { ok = false; break; }
-        tc_fence_after_sync();
-        const uint32_t d_tmem = tmem_base + acc * BN;
-        const int end = min(kb + DRAIN, kb1);
-        for (int k = kb; k < end; ++k, it += 2) {
-          const int s = it % HALVES;                                         // (even: HALVES is)
-          const uint32_t ph = (it / HALVES) & 1;
-          if (!__all_sync(0xffffffffu, mbar_wait(&full_bar[s], ph, abort_flag, p.status, 211))) { ok = false; break; }
-          tc_fence_after_sync();
-          const uint32_t x_addr = smem_u32(smem + s * HALF_BYTES), y_addr = x_addr + HALF_BYTES;
-          const uint64_t a_hi = make_smem_desc(x_addr, 16, 1024), b_lo = b_desc(x_addr + A_BYTES);
-          const uint64_t a_lo = make_smem_desc(y_addr, 16, 1024), b_hi = b_desc(y_addr + A_BYTES);
-          if (elect_one()) multiply(d_tmem, a_hi, b_lo, k == kb);
-          __syncwarp();
-          if (!__all_sync(0xffffffffu, mbar_wait(&full_bar[s + 1], ph, abort_flag, p.status, 212))) { ok = false; break; }
-          tc_fence_after_sync();
-          if (elect_one()) {
-            multiply(d_tmem, a_hi, b_hi, false);
-            umma_commit(&empty_bar[s]);
-            multiply(d_tmem, a_lo, b_hi, false);
-            umma_commit(&empty_bar[s + 1]);
-          }
-          __syncwarp();
-        }
-        if (ok) {
-          if (elect_one()) umma_commit(&tmem_full[acc]);
-          __syncwarp();
-        }
-      }
-    }
-    __syncwarp();
-    }
-    if constexpr (SPLIT) {                               // (the epilogue's three barriers, see there)
+    if constexpr (KIND == SPLIT) {                       // (the epilogue's three barriers, see there)
       tc_fence_before_sync();
       __syncthreads();
-      cluster_barrier();
-      cluster_barrier();
+      g2::cluster_sync_all();
+      g2::cluster_sync_all();
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
@@ -486,89 +536,105 @@ ns_product_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_consta
     const int q = warp & 3, half = (warp - 4) >> 2;
     uint8_t* slab = smem + SLAB_OFFSET + (warp - 4) * CHUNK_BYTES;
     const Epilogue<MODE> epi(p);
+    const uint32_t empty0 = KIND == PAIR ? g2::map_to_cta(smem_u32(&tmem_empty[0]), 0) : 0u;
     uint32_t drains = 0;
     bool ok = true;
     for (long long t = first; t < total; t += stride) {
       int mi, ni, z;
       decode(t, mi, ni, z);
+      const int row0 = mi * TM + row_in_tile + q * 32, col0 = ni * BN + half * (BN / 2);
       float v[CHUNKS][32];
 #pragma unroll
       for (int h = 0; h < CHUNKS; ++h)
 #pragma unroll
         for (int j = 0; j < 32; ++j) v[h][j] = 0.f;
-      if constexpr (!SPLIT)
-        for (int h = 0; h < CHUNKS; ++h) epi.prefetch(z, mi * BM + q * 32, ni * BN + half * (BN / 2) + h * 32);
+      uint4 in[8];
+      if constexpr (KIND != SPLIT)
+        for (int h = 0; h < CHUNKS; ++h) epi.prefetch(z, row0, col0 + h * 32);
       for (int kb = kb0; kb < kb1; kb += DRAIN, ++drains) {
         const uint32_t acc = drains % ACCS;
         if (!__all_sync(0xffffffffu, mbar_wait(&tmem_full[acc], (drains / ACCS) & 1, abort_flag, p.status, 310))) { ok = false; break; }
         tc_fence_after_sync();
         const uint32_t at = tmem_base + ((uint32_t)(q * 32) << 16) + acc * BN + half * (BN / 2);
+        if (kb + DRAIN >= kb1 && KIND != SPLIT) epi.fetch(in, z, row0, col0);
 #pragma unroll
-        for (int h = 0; h < 2 * CHUNKS; ++h) {
-          uint32_t r[16];
-          tmem_ld_32x32b_x16(at + 16 * h, r);
+        for (int h = 0; h < CHUNKS; ++h) {
+          uint32_t r[32];
+          tmem_ld_32x32b_x32(at + 32 * h, r);
           tmem_ld_wait();
 #pragma unroll
-          for (int j = 0; j < 16; ++j) v[h >> 1][(h & 1) * 16 + j] += __uint_as_float(r[j]);
+          for (int j = 0; j < 32; ++j) v[h][j] += __uint_as_float(r[j]);
         }
         tc_fence_before_sync();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&tmem_empty[acc]);
+        if (lane == 0) {
+          if constexpr (KIND == PAIR) g2::mbar_arrive_cluster(empty0 + acc * 8);
+          else mbar_arrive(&tmem_empty[acc]);
+        }
       }
-      if (!ok) break;
+      if (!ok) {
+        if (lane == 0) give_up();
+        break;
+      }
 #pragma unroll
       for (int h = 0; h < CHUNKS; ++h) {
         // a part of the contraction waits in this CTA's ring, which all products have been read from by now
-        uint8_t* at = SPLIT ? smem + ((warp - 4) * CHUNKS + h) * CHUNK_BYTES : slab;
+        uint8_t* at = KIND == SPLIT ? smem + ((warp - 4) * CHUNKS + h) * CHUNK_BYTES : slab;
         __syncwarp();                                   // (the chunk before has been read)
 #pragma unroll
         for (int u = 0; u < 8; ++u)
           *reinterpret_cast<float4*>(at + chunk_at(lane, u)) = make_float4(v[h][4 * u], v[h][4 * u + 1], v[h][4 * u + 2], v[h][4 * u + 3]);
         __syncwarp();
-        if constexpr (!SPLIT) {
+        if constexpr (KIND != SPLIT) {
           float4 acc[8];
+          uint4 now[8];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) acc[i] = *reinterpret_cast<const float4*>(slab + chunk_at(4 * i + (lane >> 3), lane & 7));
-          epi.run(acc, slab, z, mi * BM + q * 32, ni * BN + half * (BN / 2) + h * 32);
+          for (int i = 0; i < 8; ++i) { acc[i] = *reinterpret_cast<const float4*>(slab + chunk_at(4 * i + (lane >> 3), lane & 7)); now[i] = in[i]; }
+          if (h + 1 < CHUNKS) epi.fetch(in, z, row0, col0 + (h + 1) * 32);
+          epi.run(acc, now, slab, z, row0, col0 + h * 32);
         }
       }
     }
-    if constexpr (SPLIT) {
+    if constexpr (KIND == SPLIT) {
       // the parts of a tile meet: rank k adds up chunks k, k + splits, .., in the order of the ranks, one warp each at a time
       tc_fence_before_sync();
       __syncthreads();
-      cluster_barrier();
+      g2::cluster_sync_all();
       if (!*abort_flag) {
         int mi, ni, z;
         decode(first, mi, ni, z);
         for (int c = rank + (warp - 4) * splits; c < 8 * CHUNKS; c += 8 * splits) {
           __syncwarp();
-            float4 sum[8];
+          const int w = c / CHUNKS;                      // the warp whose chunk this was, and where its rows and columns are
+          const int row0 = mi * BM + (w & 3) * 32, col0 = ni * BN + (w >> 2) * (BN / 2) + (c % CHUNKS) * 32;
+          uint4 in[8];
+          epi.fetch(in, z, row0, col0);
+          float4 sum[8];
 #pragma unroll
-          for (int it = 0; it < 8; ++it) sum[it] = make_float4(0.f, 0.f, 0.f, 0.f);
+          for (int i = 0; i < 8; ++i) sum[i] = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
           for (int k = 0; k < splits; ++k) {
-            uint32_t peer;
-            asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(peer) : "r"(smem_u32(smem) + c * CHUNK_BYTES), "r"(k));
+            const uint32_t peer = g2::map_to_cta(smem_u32(smem) + c * CHUNK_BYTES, k);
             float4 o[8];
 #pragma unroll
-            for (int it = 0; it < 8; ++it) o[it] = ld_peer(peer + chunk_at(4 * it + (lane >> 3), lane & 7));
+            for (int i = 0; i < 8; ++i) o[i] = ld_peer(peer + chunk_at(4 * i + (lane >> 3), lane & 7));
 #pragma unroll
-            for (int it = 0; it < 8; ++it) { sum[it].x += o[it].x; sum[it].y += o[it].y; sum[it].z += o[it].z; sum[it].w += o[it].w; }
+            for (int i = 0; i < 8; ++i) { sum[i].x += o[i].x; sum[i].y += o[i].y; sum[i].z += o[i].z; sum[i].w += o[i].w; }
           }
-          const int w = c / CHUNKS;                        // the warp whose chunk this was, and where its rows and columns are
-          epi.run(sum, slab, z, mi * BM + (w & 3) * 32, ni * BN + (w >> 2) * (BN / 2) + (c % CHUNKS) * 32);
+          epi.run(sum, in, slab, z, row0, col0);
         }
       }
-      cluster_barrier();                                   // nobody leaves while its part may still be read
+      g2::cluster_sync_all();                            // nobody leaves while its part may still be read
     }
   }
 
   tc_fence_before_sync();
   __syncthreads();
+  if constexpr (KIND == PAIR) g2::cluster_sync_all();    // nobody leaves (or frees tensor memory) while the other may still signal it
   if (warp == 1) {
     tc_fence_after_sync();
-    tmem_dealloc(tmem_base, 512);
+    if constexpr (KIND == PAIR) g2::tmem_dealloc2(tmem_base, 512);
+    else tmem_dealloc(tmem_base, 512);
   }
 }
 
@@ -746,19 +812,19 @@ static inline int norm_parts(long long numel) {
   return (int)(p < PARTS ? p : PARTS);
 }
 
-template <int MODE, int BN, bool SPLIT>
+template <int MODE, int BN, int KIND>
 static int launch(const CUtensorMap& ta, const CUtensorMap& tb, const Params& p, int grid, cudaStream_t st) {
   static unsigned long long configured = 0;
-  if (int r = smem_opt_in(ns_product_kernel<MODE, BN, SPLIT>, SMEM_TOTAL, configured)) return r;
+  if (int r = smem_opt_in(ns_product_kernel<MODE, BN, KIND>, SMEM_TOTAL, configured)) return r;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = p.splits; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
+  attr[1].val.clusterDim.x = KIND == PAIR ? 2 : p.splits; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
   cfg.gridDim = dim3((unsigned)grid); cfg.blockDim = dim3(THREADS); cfg.dynamicSmemBytes = SMEM_TOTAL; cfg.stream = st;
-  cfg.attrs = attr; cfg.numAttrs = SPLIT ? 2 : 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, ns_product_kernel<MODE, BN, SPLIT>, ta, tb, p);
+  cfg.attrs = attr; cfg.numAttrs = KIND == WHOLE ? 1 : 2;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, ns_product_kernel<MODE, BN, KIND>, ta, tb, p);
   return e == cudaSuccess ? (int)cudaGetLastError() : (int)e;
 }
 
@@ -770,7 +836,7 @@ static int max_clusters(int size) {
   cudaGetDevice(&dev);
   int& n = known[dev & 63][size == 2 ? 1 : size == 4 ? 2 : 3];
   if (n == 0) {
-    auto kern = ns_product_kernel<GRAM, 128, true>;
+    auto kern = ns_product_kernel<GRAM, 128, SPLIT>;
     static unsigned long long configured = 0;
     if (smem_opt_in(kern, SMEM_TOTAL, configured)) return 1;
     cudaLaunchConfig_t cfg = {};
@@ -788,26 +854,31 @@ static int max_clusters(int size) {
 template <int MODE>
 static int product(const CUtensorMap& ta, const CUtensorMap& tb, Params p, cudaStream_t st) {
   constexpr bool SYM = MODE == GRAM || MODE == SQUARE;
-  const int sms = sm_count(), kblocks = ((MODE == GRAM ? p.n : p.m) + BK - 1) / BK;
-  // Width of the tiles, and how many CTAs of a cluster share a tile's contraction where tiles are few: whatever has the
-  // fewest clocks on its longest CTA.  A block of the contraction takes 1700 clocks with 256 columns and 1080 with 128, bound
-  // by shared memory (160 and 213 bytes a clock at the full tensor rate, of 128); a start and its epilogue 8000 and 6000;
-  // the exchange of a cluster 4000.
-  int best_w = 0;
-  long long best = -1, best_total = 0;
-  p.splits = 1;
-  for (int w = 0; w < 2; ++w) {
-    const long long total = (w ? tiles_of<256>(SYM, p.m, p.n) : tiles_of<128>(SYM, p.m, p.n)) * p.batch;
-    for (int s = 1; s == 1 || (s <= 8 && kblocks >= 2 * s); s *= 2) {
-      if (s > 1 && total > max_clusters(s)) break;              // clusters take one tile each: a single wave of them
-      const long long waves = s > 1 ? 1 : (total + sms - 1) / sms;
-      const long long t = waves * ((kblocks + s - 1) / s) * (w ? 1700 : 1080) + (w ? 8000 : 6000) + (s > 1 ? 4000 : 0);
-      if (best < 0 || t < best) { best = t; best_w = w; best_total = total; p.splits = s; }
-    }
+  const long long sms = sm_count(), kblocks = ((MODE == GRAM ? p.n : p.m) + BK - 1) / BK;
+  // Tiles of 128 x 128 or 128 x 256, whole or shared by the CTAs of a cluster, or of 256 x 256 on pairs: whatever has the
+  // fewest clocks on its longest CTA.  A block of the contraction takes 1080 clocks with 128 columns and 1700 with 256,
+  // bound by shared memory (213 and 160 bytes a clock at the full tensor rate, of 128), or 2100 where all SMs together
+  // read more than L2 gives (11 TB/s); pairs read two thirds of that and take 1600.  A start and its epilogue are 6000 to
+  // 10000, the exchange of a cluster 4000.
+  int kind = WHOLE, bn = 128;
+  long long best = -1, grid = 0;
+  auto offer = [&](long long clocks, int k, int width, int splits, long long ctas) {
+    if (best >= 0 && clocks >= best) return;
+    best = clocks; kind = k; bn = width; p.splits = splits; grid = ctas;
+  };
+  for (int width = 128; width <= 256; width += 128) {
+    const long long total = tiles_of(SYM, p.m, p.n, BM, width) * p.batch, waves = (total + sms - 1) / sms;
+    const long long block = width == 128 ? 1080 : total >= sms ? 2100 : 1700, ends = width == 128 ? 6000 : 8000;
+    offer(waves * kblocks * block + ends, WHOLE, width, 1, total < sms ? total : sms);
+    for (int s = 2; s <= 8 && kblocks >= 2 * s && total <= max_clusters(s); s *= 2)      // (one tile each: a single wave)
+      offer((kblocks + s - 1) / s * (width == 128 ? 1080 : 1700) + ends + 4000, SPLIT, width, s, total * s);
   }
-  const int grid = (int)(p.splits > 1 ? best_total * p.splits : (best_total < sms ? best_total : sms));
-  if (best_w) return p.splits > 1 ? launch<MODE, 256, true>(ta, tb, p, grid, st) : launch<MODE, 256, false>(ta, tb, p, grid, st);
-  return p.splits > 1 ? launch<MODE, 128, true>(ta, tb, p, grid, st) : launch<MODE, 128, false>(ta, tb, p, grid, st);
+  const long long pairs = tiles_of(SYM, p.m, p.n, 2 * BM, 256) * p.batch, at_once = max_clusters(2);
+  offer((pairs + at_once - 1) / at_once * kblocks * 1600 + 10000, PAIR, 256, 1, 2 * (pairs < at_once ? pairs : at_once));
+  const int g = (int)grid;
+  if (kind == PAIR) return launch<MODE, 256, PAIR>(ta, tb, p, g, st);
+  if (kind == SPLIT) return bn == 256 ? launch<MODE, 256, SPLIT>(ta, tb, p, g, st) : launch<MODE, 128, SPLIT>(ta, tb, p, g, st);
+  return bn == 256 ? launch<MODE, 256, WHOLE>(ta, tb, p, g, st) : launch<MODE, 128, WHOLE>(ta, tb, p, g, st);
 }
 
 static inline long long up256(long long b) { return (b + 255) & ~255ll; }

@@ -41,6 +41,29 @@ def test_orthogonalize(shape, kind):
     assert float(err.max()) < TOL, err
 
 
+def iterated(x, steps=5, coefficients=(3.4445, -4.7750, 2.0315), eps=1e-7):
+    """The iteration itself in 64 bits: a decomposition of large matrices takes too long."""
+    a, b, c = coefficients
+    y = x.double()
+    y = y.mT if y.shape[-2] > y.shape[-1] else y
+    y = y / (torch.linalg.matrix_norm(y, keepdim=True) + eps)
+    for _ in range(steps):
+        q = y @ y.mT
+        y = a * y + (b * q + c * (q @ q)) @ y
+    return y.mT if x.shape[-2] > x.shape[-1] else y
+
+
+@pytest.mark.parametrize("shape", [(12, 512, 1024), (12, 1000, 500), (2, 2560, 2560), (3, 1100, 2300), (1, 2400, 5100), (9, 896, 896),
+                                   (20, 129, 4000), (200, 70, 40)])
+def test_large_and_many(shape):
+    """Sizes at which tiles are whole, on CTA pairs, or shared by clusters, in each of the three products."""
+    x = matrix(*shape, kind="low").cuda()
+    with K.strict_native():
+        o = genesis.optim.orthogonalize(T(x))
+    err = torch.linalg.matrix_norm(o._t.double() - iterated(x))
+    assert float(err.max()) < TOL, err
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("shape", [(60, 90), (90, 60), (2, 131, 77), (1, 7)])
 def test_types(shape, dtype):
@@ -196,7 +219,10 @@ def test_post_training_steps_of_a_model():
     graphed[2].make_capturable()
     run = genesis.cuda.GraphedTrainStep(lambda: step(*graphed), graphed[1], [], warmup=3)
     again = [run().item() for _ in range(2)]
-    assert again == losses[3:]
+    # (the embedding's gradient is added up in memory in no fixed order: its last bits, 2^-24 of it, and through Adam's
+    # division the steps of weights whose gradient is about zero, differ from run to run.  To first order neither moves the loss:
+    # 1e-3 sum |g| over gradients of at most 1e-9, for 515 x 64 weights 3e-8, and rounding of the loss, 2^-24)
+    assert max(abs(a - b) for a, b in zip(again, losses[3:])) < 1e-6
     assert graphed[1].t == 5
     # the gradient of one weight against differences of the loss, along the gradient
     model = build()[0]
