@@ -22,7 +22,6 @@ namespace tl {
 
 namespace cg = cooperative_groups;
 
-constexpr float LOG2E = 1.4426950408889634f;
 constexpr int SITE_TOKEN = 7;                      // where a bad index was found (native.py: _raise_status)
 
 // Row r of the logits starts at z + (r / inner) * s_outer + (r % inner) * s_inner elements: a [B, T, V] slice is read in place.
@@ -43,11 +42,25 @@ struct Policy {
 
 struct MaxSum { float m, s; };
 
-// (max, sum) pairs of two parts; c = log2(e) / T.  A part of -inf alone (or of nothing) is (-inf, 0).
-__device__ __forceinline__ MaxSum join(MaxSum a, MaxSum b, float c) {
+// log2(e) / T as the sum of two floats: rounded to one, it would shift every log-probability the same way, by 1.3e-8 of
+// (z - m) / T, and the sum of an answer's log-probabilities by their number times that.  The high part is rounded down, so
+// that the low one is positive and -inf times either is -inf.
+struct Scale {
+  float hi, lo;
+  explicit Scale(double temperature) {
+    const double c = 1.4426950408889634 / temperature;
+    hi = (float)c;
+    if ((double)hi >= c) hi = nextafterf(hi, 0.f);
+    lo = (float)(c - (double)hi);
+  }
+  __device__ __forceinline__ float operator()(float d) const { return fmaf(d, hi, d * lo); }
+};
+
+// (max, sum) pairs of two parts.  A part of -inf alone (or of nothing) is (-inf, 0).
+__device__ __forceinline__ MaxSum join(MaxSum a, MaxSum b, const Scale& c) {
   const float m = fmaxf(a.m, b.m);
   if (m == -INFINITY) return MaxSum{m, a.s + b.s};                 // (a NaN sum stays one)
-  return MaxSum{m, a.s * exp2f((a.m - m) * c) + b.s * exp2f((b.m - m) * c)};
+  return MaxSum{m, a.s * exp2f(c(a.m - m)) + b.s * exp2f(c(b.m - m))};
 }
 
 __device__ __forceinline__ float ex2(float x) {
@@ -92,67 +105,101 @@ __device__ __forceinline__ float vec_max(const uint4& v) {
   }
 }
 
-// What thread `t` of `G` sees of the `n` elements at p: running maximum and sum, 32 bytes at a time.  Elements before the
-// first 16-byte boundary and behind the last are taken one by one, so rows of odd length cost no more than aligned ones.
-template <typename T, int G>
-__device__ __forceinline__ MaxSum scan(const T* p, int n, float c, int t) {
+__device__ __forceinline__ void copy16(uint32_t smem_dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copies_issued() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// What thread `t` of `G` sees of the `n` elements at p: running maximum and sum, two vectors of 16 bytes at a time.  Elements
+// before the first 16-byte boundary and behind the last are taken one by one, so rows of odd length cost no more than
+// aligned ones.  With RING > 0 the vectors come through a ring of RING pairs in shared memory that belongs to the thread
+// alone (asynchronous copies, no barriers): 16 RING * 2 bytes of every thread are always on their way, where plain loads
+// leave the memory idle while they are worked on.
+template <typename T, int G, int RING>
+__device__ __forceinline__ MaxSum scan(const T* p, int n, const Scale& c, int t, uint8_t* ring = nullptr) {
   constexpr int V = 16 / sizeof(T), H = V / 2;
   MaxSum a{-INFINITY, 0.f};
   auto raise = [&](float mx) {
-    if (mx > a.m) { a.s *= ex2((a.m - mx) * c); a.m = mx; }
+    if (mx > a.m) { a.s *= ex2(c(a.m - mx)); a.m = mx; }
   };
   auto one = [&](T x) {
     const float z = Cvt<T>::to_f(x);
     raise(z);
-    if (z != -INFINITY) a.s += ex2((z - a.m) * c);                 // (NaN comes through: NaN - m)
+    if (z != -INFINITY) a.s += ex2(c(z - a.m));                    // (NaN comes through: NaN - m)
   };
-  const float2 c2 = make_float2(c, c);
+  const float2 hi = make_float2(c.hi, c.hi), lo = make_float2(c.lo, c.lo);
   auto add = [&](const uint4& v) {
     float2 f[H], sum = make_float2(0.f, 0.f);
     unpack<T>(v, f);
-    const float2 nm = make_float2(-a.m, -a.m);
+    const float m = a.m == -INFINITY ? 0.f : a.m;                  // (all -inf so far: they add nothing to a sum of 0)
+    const float2 nm = make_float2(-m, -m);
 #pragma unroll
     for (int i = 0; i < H; ++i) {
-      float2 e = mul2(add2(f[i], nm), c2);
+      const float2 d = add2(f[i], nm);
+      float2 e = fma2(d, hi, mul2(d, lo));
       e.x = ex2(e.x); e.y = ex2(e.y);
       sum = add2(sum, e);
     }
     a.s += sum.x + sum.y;
   };
-  // all of a vector -inf and nothing larger before it: -inf - -inf would be NaN, so only a NaN among them may add
-  auto low = [&](const uint4& v) {
-    float2 f[H];
-    unpack<T>(v, f);
-#pragma unroll
-    for (int i = 0; i < H; ++i) {
-      if (f[i].x != f[i].x) a.s += f[i].x;
-      if (f[i].y != f[i].y) a.s += f[i].y;
-    }
-  };
   const int mis = (int)((reinterpret_cast<uintptr_t>(p) & 15) / sizeof(T));
   int head = mis ? V - mis : 0;
   if (head > n) head = n;
-  if (t < head) one(p[t]);
   const uint4* v = reinterpret_cast<const uint4*>(p + head);
-  const int nv = (n - head) / V;
-  int i = t;
-  for (; i + G < nv; i += 2 * G) {
-    const uint4 x = v[i], y = v[i + G];
-    raise(fmaxf(vec_max<T>(x), vec_max<T>(y)));
-    if (a.m == -INFINITY) { low(x); low(y); continue; }
-    add(x); add(y);
+  const int nv = (n - head) / V, rest = head + nv * V + t;
+  if constexpr (RING > 0) {
+    const uint32_t base = smem_u32(ring) + t * 16;                 // vector k of a pair in slot s: base + (2 s + k) * 16 G
+    auto fetch = [&](int i, int s) {
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+        if (i + k * G < nv) copy16(base + (2 * s + k) * 16 * G, v + i + k * G);
+      copies_issued();
+    };
+#pragma unroll
+    for (int s = 0; s < RING; ++s) fetch(t + s * 2 * G, s);
+    if (t < head) one(p[t]);
+    if (rest < n) one(p[rest]);
+    int s = 0;
+    for (int i = t; i < nv; i += 2 * G) {
+      copies_wait<RING - 1>();
+      const uint4* slot = reinterpret_cast<const uint4*>(ring + t * 16 + s * 32 * G);
+      const bool two = i + G < nv;
+      const uint4 x = slot[0], y = two ? slot[G] : x;
+      raise(fmaxf(vec_max<T>(x), vec_max<T>(y)));
+      fetch(i + RING * 2 * G, s);
+      add(x);
+      if (two) add(y);
+      s = s + 1 == RING ? 0 : s + 1;
+    }
+    copies_wait<0>();
+  } else {
+    constexpr int U = 4;
+    if (t < head) one(p[t]);
+    int i = t;
+    for (; i + (U - 1) * G < nv; i += U * G) {
+      uint4 x[U];
+      float mx = -INFINITY;
+#pragma unroll
+      for (int k = 0; k < U; ++k) x[k] = v[i + k * G];
+#pragma unroll
+      for (int k = 0; k < U; ++k) mx = fmaxf(mx, vec_max<T>(x[k]));
+      raise(mx);
+#pragma unroll
+      for (int k = 0; k < U; ++k) add(x[k]);
+    }
+    for (; i < nv; i += G) {
+      const uint4 x = v[i];
+      raise(vec_max<T>(x));
+      add(x);
+    }
+    if (rest < n) one(p[rest]);
   }
-  if (i < nv) {
-    const uint4 x = v[i];
-    raise(vec_max<T>(x));
-    if (a.m == -INFINITY) low(x); else add(x);
-  }
-  const int rest = head + nv * V + t;
-  if (rest < n) one(p[rest]);
   return a;
 }
 
-__device__ __forceinline__ MaxSum warp_join(MaxSum a, float c) {
+__device__ __forceinline__ MaxSum warp_join(MaxSum a, const Scale& c) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     MaxSum b;
@@ -206,7 +253,7 @@ __device__ __forceinline__ void skip_row(long long r, long long rows, float* lp_
 template <typename T, typename TI>
 __global__ void __launch_bounds__(256)
 token_rows_warp_kernel(const T* __restrict__ z, RowMap map, const TI* __restrict__ tokens, float* __restrict__ lp,
-                       float* __restrict__ stats, long long rows, int cols, long long ignore, float temperature, float c,
+                       float* __restrict__ stats, long long rows, int cols, long long ignore, float temperature, Scale c,
                        Policy q, int* status) {
   const int lane = threadIdx.x & 31;
   const long long r = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
@@ -220,20 +267,21 @@ token_rows_warp_kernel(const T* __restrict__ z, RowMap map, const TI* __restrict
     return;
   }
   const T* p = z + map.at(r);
-  const MaxSum a = warp_join(scan<T, 32>(p, cols, c, lane), c);
+  const MaxSum a = warp_join(scan<T, 32, 0>(p, cols, c, lane), c);
   if (lane == 0) finish_row<T, TI>(a, p, t, r, rows, temperature, lp, stats, q);
 }
 
-constexpr int FWD_THREADS = 512;
+constexpr int RING = 4;
 
-// Long rows: one CTA each, or, where rows are few, the CTAs of a cluster share one and rank 0 joins their parts through
-// distributed shared memory.
-template <typename T, typename TI>
-__global__ void __launch_bounds__(FWD_THREADS, 3)
+// Longer rows: one CTA of G threads each, or, where rows are few, the CTAs of a cluster share one and rank 0 joins their
+// parts through distributed shared memory.  G = 512 reads through the ring, three CTAs on an SM.
+template <typename T, typename TI, int G>
+__global__ void __launch_bounds__(G, G == 512 ? 3 : 8)
 token_rows_kernel(const T* __restrict__ z, RowMap map, const TI* __restrict__ tokens, float* __restrict__ lp,
-                  float* __restrict__ stats, long long rows, int cols, long long ignore, float temperature, float c,
+                  float* __restrict__ stats, long long rows, int cols, long long ignore, float temperature, Scale c,
                   Policy q, int* status, int parts) {
-  __shared__ float2 sh[FWD_THREADS / 32];
+  extern __shared__ __align__(16) uint8_t ring[];
+  __shared__ float2 sh[G / 32];
   __shared__ float2 mine;
   const long long r = blockIdx.x / parts;
   const int part = blockIdx.x % parts;
@@ -252,12 +300,12 @@ token_rows_kernel(const T* __restrict__ z, RowMap map, const TI* __restrict__ to
     lo = min(part * step, cols);
     n = min(step, cols - lo);
   }
-  MaxSum a = warp_join(scan<T, FWD_THREADS>(p + lo, n, c, threadIdx.x), c);
+  MaxSum a = warp_join(scan<T, G, G == 512 ? RING : 0>(p + lo, n, c, threadIdx.x, ring), c);
   if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = make_float2(a.m, a.s);
   __syncthreads();
   if (threadIdx.x < 32) {
     a = MaxSum{-INFINITY, 0.f};
-    if (threadIdx.x < FWD_THREADS / 32) a = MaxSum{sh[threadIdx.x].x, sh[threadIdx.x].y};
+    if (threadIdx.x < G / 32) a = MaxSum{sh[threadIdx.x].x, sh[threadIdx.x].y};
     a = warp_join(a, c);
   }
   if (parts > 1) {
@@ -454,22 +502,33 @@ token_grad_kernel(const T* __restrict__ z, RowMap map, const TI* __restrict__ to
 template <typename T, typename TI>
 static int rows_forward(const void* z, RowMap map, const void* tokens, float* lp, float* stats, long long rows, int cols,
                         long long ignore, float temperature, const Policy& q, int* status, cudaStream_t st) {
-  const float c = LOG2E / temperature;
-  if (cols <= 1024) {
+  const Scale c((double)temperature);
+  const long long bytes = (long long)cols * sizeof(T), sms = sm_count();
+  // A warp a row up to 8 KB, 128 threads up to 32 KB, else 512; fewer rows than warps, or CTAs, that the device holds take the
+  // next larger group.
+  if (bytes <= 2048 || (bytes <= 8192 && rows >= 32 * sms)) {
     token_rows_warp_kernel<T, TI><<<(unsigned)((rows + 7) / 8), 256, 0, st>>>(
         (const T*)z, map, (const TI*)tokens, lp, stats, rows, cols, ignore, temperature, c, q, status);
     return (int)cudaGetLastError();
   }
+  if (bytes <= 8192 || (bytes <= 32768 && rows >= 8 * sms)) {
+    token_rows_kernel<T, TI, 128><<<(unsigned)rows, 128, 0, st>>>(
+        (const T*)z, map, (const TI*)tokens, lp, stats, rows, cols, ignore, temperature, c, q, status, 1);
+    return (int)cudaGetLastError();
+  }
   // a part has to be worth its cluster barriers: 4096 elements at least
   int parts = 1;
-  while (parts < 8 && rows * parts * 2 <= 3ll * sm_count() && cols / (parts * 2) >= 4096) parts *= 2;
+  while (parts < 8 && rows * parts * 2 <= 3 * sms && cols / (parts * 2) >= 4096) parts *= 2;
+  constexpr int smem = RING * 32 * 512;
+  static unsigned long long configured = 0;
+  if (int r = smem_opt_in(token_rows_kernel<T, TI, 512>, smem, configured)) return r;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = parts; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
-  cfg.gridDim = dim3((unsigned)(rows * parts)); cfg.blockDim = dim3(FWD_THREADS); cfg.stream = st;
+  cfg.gridDim = dim3((unsigned)(rows * parts)); cfg.blockDim = dim3(512); cfg.dynamicSmemBytes = smem; cfg.stream = st;
   cfg.attrs = attr; cfg.numAttrs = parts > 1 ? 1 : 0;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, token_rows_kernel<T, TI>, (const T*)z, map, (const TI*)tokens, lp, stats, rows,
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, token_rows_kernel<T, TI, 512>, (const T*)z, map, (const TI*)tokens, lp, stats, rows,
                                            cols, ignore, temperature, c, q, status, parts);
   return e == cudaSuccess ? (int)cudaGetLastError() : (int)e;
 }
@@ -477,8 +536,8 @@ static int rows_forward(const void* z, RowMap map, const void* tokens, float* lp
 template <typename T, typename TI>
 static int rows_backward(const void* z, RowMap map, const void* tokens, const float* stats, void* dz, long long rows, int cols,
                          long long ignore, float temperature, const Factor& fac, cudaStream_t st) {
-  const float c = LOG2E / temperature;
-  if (cols <= 1024) {
+  const float c = (float)(1.4426950408889634 / (double)temperature);
+  if ((long long)cols * sizeof(T) <= 8192 && (cols <= 1024 || rows >= 32ll * sm_count())) {
     token_grad_kernel<T, TI, 32><<<(unsigned)((rows + 7) / 8), BWD_THREADS, 0, st>>>(
         (const T*)z, map, (const TI*)tokens, stats, (T*)dz, rows, cols, ignore, temperature, c, fac, cols, 1);
     return (int)cudaGetLastError();
@@ -491,36 +550,54 @@ static int rows_backward(const void* z, RowMap map, const void* tokens, const fl
   return (int)cudaGetLastError();
 }
 
+static int rows_any(const void* z, const void* tokens, float* lp, float* stats, long long rows, long long cols, RowMap map,
+                    long long ignore, float temperature, const Policy& q, int dt, int token_i64, int* status, cudaStream_t st) {
+  if (rows == 0) return 0;
+  if (cols < 1 || cols > 0x7fffffffll || rows > 0x0fffffffll || map.inner < 1 || !(temperature > 0.f)) return -3;
+  if (token_i64) GB_DISPATCH_FLOAT(dt, T, return (rows_forward<T, long long>(z, map, tokens, lp, stats, rows, (int)cols, ignore, temperature, q, status, st)));
+  GB_DISPATCH_FLOAT(dt, T, return (rows_forward<T, int>(z, map, tokens, lp, stats, rows, (int)cols, ignore, temperature, q, status, st)));
+}
+
 }  // namespace tl
 }  // namespace gb
 
 using namespace gb;
 
-// Log-probabilities lp [rows] of `tokens` and the rows' (max, log2 sum) in stats [2, rows].  With `old` also the clipped
-// policy loss [rows] and its derivative by lp [rows].  Rows: see RowMap.
+// Log-probabilities lp [rows] of `tokens` and the rows' (max, log2 sum) in stats [2, rows].  Rows: see RowMap.
 extern "C" int gb_token_rows(const void* z, const void* tokens, float* lp, float* stats, long long rows, long long cols,
                              long long inner, long long s_outer, long long s_inner, long long ignore, float temperature,
-                             const float* old, const float* adv, const float* ref, float* loss, float* coef,
-                             long long adv_div, float lo, float hi, float kl, int dt, int token_i64, int* status,
-                             cudaStream_t st) {
-  if (rows == 0) return 0;
-  if (cols < 1 || cols > 0x7fffffffll || rows > 0x0fffffffll || inner < 1 || adv_div < 1 || !(temperature > 0.f)) return -3;
-  const tl::RowMap map{inner, s_outer, s_inner};
-  const tl::Policy q{old, adv, ref, loss, coef, adv_div, lo, hi, kl};
-  if (token_i64) GB_DISPATCH_FLOAT(dt, T, return (tl::rows_forward<T, long long>(z, map, tokens, lp, stats, rows, (int)cols, ignore, temperature, q, status, st)));
-  GB_DISPATCH_FLOAT(dt, T, return (tl::rows_forward<T, int>(z, map, tokens, lp, stats, rows, (int)cols, ignore, temperature, q, status, st)));
+                             int dt, int token_i64, int* status, cudaStream_t st) {
+  return tl::rows_any(z, tokens, lp, stats, rows, cols, tl::RowMap{inner, s_outer, s_inner}, ignore, temperature, tl::Policy{},
+                      dt, token_i64, status, st);
 }
 
-extern "C" int gb_policy_sum(const float* loss, const void* tokens, long long rows, long long cols, long long ignore,
-                             int mean, float* out, int token_i64, cudaStream_t st) {
+// The same, and every row's clipped policy loss [rows] and its derivative by lp, coef [rows]; out [2] (or null) receives the
+// sum of the losses (over the number of rows that count with `mean`) and the factor of their gradients.
+extern "C" int gb_policy_loss(const void* z, const void* tokens, float* lp, float* stats, long long rows, long long cols,
+                              long long inner, long long s_outer, long long s_inner, long long ignore, float temperature,
+                              const float* old, const float* adv, const float* ref, float* loss, float* coef, long long adv_div,
+                              float lo, float hi, float kl, float* out, int mean, int dt, int token_i64, int* status,
+                              cudaStream_t st) {
+  if (adv_div < 1) return -3;
+  const tl::Policy q{old, adv, ref, loss, coef, adv_div, lo, hi, kl};
+  if (const int e = tl::rows_any(z, tokens, lp, stats, rows, cols, tl::RowMap{inner, s_outer, s_inner}, ignore, temperature, q,
+                                 dt, token_i64, status, st)) return e;
+  if (out == nullptr) return 0;
   if (token_i64) tl::policy_sum_kernel<long long><<<1, 1024, 0, st>>>(loss, (const long long*)tokens, rows, cols, ignore, mean, out);
   else tl::policy_sum_kernel<int><<<1, 1024, 0, st>>>(loss, (const int*)tokens, rows, cols, ignore, mean, out);
   return (int)cudaGetLastError();
 }
 
-extern "C" int gb_preference(const float* lp, const float* ref, long long pairs, long long len, float beta, float smooth,
-                             int mean, float* loss_each, float* out, float* rewards, float* gseq, cudaStream_t st) {
-  tl::preference_kernel<<<1, 1024, 0, st>>>(lp, ref, pairs, len, beta, smooth, mean, loss_each, out, rewards, gseq);
+// Log-probabilities as gb_token_rows gives them, and the loss of `pairs` pairs of answers of rows / (2 pairs) rows each: see
+// preference_kernel.
+extern "C" int gb_preference_loss(const void* z, const void* tokens, float* lp, float* stats, long long rows, long long cols,
+                                  long long inner, long long s_outer, long long s_inner, long long ignore, const float* ref,
+                                  long long pairs, float beta, float smooth, int mean, float* loss_each, float* out,
+                                  float* rewards, float* gseq, int dt, int token_i64, int* status, cudaStream_t st) {
+  if (const int e = tl::rows_any(z, tokens, lp, stats, rows, cols, tl::RowMap{inner, s_outer, s_inner}, ignore, 1.f, tl::Policy{},
+                                 dt, token_i64, status, st)) return e;
+  tl::preference_kernel<<<1, 1024, 0, st>>>(lp, ref, pairs, pairs > 0 ? rows / (2 * pairs) : 0, beta, smooth, mean, loss_each, out,
+                                            rewards, gseq);
   return (int)cudaGetLastError();
 }
 

@@ -971,7 +971,7 @@ class TokenLogProbsFunction(Function):
     def backward(ctx, g):
         logits, tokens, stats = ctx.saved_tensors
         temperature, ignore_index = ctx.meta
-        return K.token_grad(logits, tokens, stats, ignore_index, temperature, g=K.contiguous(K.to_dtype(g, stats.dtype)),
+        return K.token_grad(logits, tokens, stats, ignore_index, temperature, g=_as(g, stats.dtype),
                             g_mod=_pymax(tokens.numel(), 1))
 
 
@@ -983,22 +983,17 @@ class PolicyLossFunction(Function):
     @staticmethod
     def forward(ctx, logits, tokens, policy, temperature, ignore_index, reduction):
         logits = K.token_logits(logits)
-        _, stats, loss, coef = K.token_rows(logits, tokens, ignore_index, temperature, policy)
-        total = None
-        if reduction != "none":
-            total = K.policy_sum(loss, tokens, logits.shape[-1], ignore_index, reduction == "mean")
-        ctx.save_for_backward(logits, tokens, stats, coef, total)
+        loss, stats, factor = K.policy_loss(logits, tokens, ignore_index, temperature, policy, reduction)
+        ctx.save_for_backward(logits, tokens, stats, factor)
         ctx.meta = (temperature, ignore_index)
-        return loss if total is None else total[0]
+        return loss
 
     @staticmethod
     def backward(ctx, g):
-        logits, tokens, stats, coef, total = ctx.saved_tensors
+        logits, tokens, stats, factor = ctx.saved_tensors
         temperature, ignore_index = ctx.meta
-        return K.token_grad(logits, tokens, stats, ignore_index, temperature, base=coef,
-                            g=K.contiguous(K.to_dtype(g, stats.dtype)),
-                            g_mod=_pymax(tokens.numel(), 1) if total is None else 1,
-                            dev_scale=None if total is None else total[1:])
+        return K.token_grad(logits, tokens, stats, ignore_index, temperature, 1, _as(g, stats.dtype),
+                            g_mod=_pymax(tokens.numel(), 1) if factor is None else 1, dev_scale=factor)
 
 
 class PreferenceLossFunction(Function):
@@ -1009,22 +1004,25 @@ class PreferenceLossFunction(Function):
     @staticmethod
     def forward(ctx, logits, tokens, ref, beta, smoothing, ignore_index, reduction, rewards_out):
         logits = K.token_logits(logits)
-        lp, stats = K.token_rows(logits, tokens, ignore_index, 1.0)
-        each, total, rewards, gseq = K.preference(lp, ref, beta, smoothing, reduction == "mean", reduction == "none")
+        loss, rewards, stats = K.preference_loss(logits, tokens, ignore_index, ref, beta, smoothing, reduction)
         rewards_out.append(rewards)
-        ctx.save_for_backward(logits, tokens, stats, gseq)
-        ctx.meta = (ignore_index, reduction)
-        return total if each is None else each
+        ctx.save_for_backward(logits, tokens, stats)
+        ctx.meta = (ignore_index, reduction, ref.numel() // 2)
+        return loss
 
     @staticmethod
     def backward(ctx, g):
-        logits, tokens, stats, gseq = ctx.saved_tensors
-        ignore_index, reduction = ctx.meta
-        pairs, length = gseq.numel() // 2, _pymax(tokens.shape[1], 1)
-        return K.token_grad(logits, tokens, stats, ignore_index, 1.0, base=gseq, base_div=length,
-                            g=K.contiguous(K.to_dtype(g, stats.dtype)), g_div=length,
-                            g_mod=_pymax(pairs, 1) if reduction == "none" else 1,
+        logits, tokens, stats = ctx.saved_tensors
+        ignore_index, reduction, pairs = ctx.meta
+        length = _pymax(tokens.shape[1], 1)
+        return K.token_grad(logits, tokens, stats, ignore_index, 1.0, length, _as(g, stats.dtype), length,
+                            _pymax(pairs, 1) if reduction == "none" else 1,
                             scale=1.0 / _pymax(pairs, 1) if reduction == "mean" else 1.0)
+
+
+def _as(t, dtype):
+    """`t` contiguous and of `dtype`."""
+    return t if t.dtype == dtype and t.is_contiguous() else K.contiguous(K.to_dtype(t, dtype))
 
 
 # ============================= fused transformer ops ==============================
@@ -1614,7 +1612,7 @@ def _constant(name, what, x, shapes, z):
         raise ValueError(f"{name}: {what} has shape {tuple(x._t.shape)}, expected {' or '.join(map(str, shapes))}")
     if x._t.device != z.device:
         raise ValueError(f"{name}: logits are on {z.device}, {what} on {x._t.device}")
-    return K.contiguous(K.to_dtype(x._t, torch.float64 if z.dtype == torch.float64 else torch.float32))
+    return _as(x._t, torch.float64 if z.dtype == torch.float64 else torch.float32)
 
 
 def _number(name, what, x, low, high):

@@ -615,12 +615,11 @@ def token_logits(logits):
     return contiguous(logits) if logits.is_cuda and N._row_map(logits) is None else logits
 
 
-def token_rows(logits, tokens, ignore_index, temperature, policy=None):
-    """Log-probabilities of `tokens` [...] under `logits` [..., V] / temperature (0 where ignored) and what the gradient
-    needs of the rows.  `policy` = (old, advantages, rows per advantage, ref or None, lowest ratio, highest ratio, KL
-    weight): also the clipped policy loss of every row and its derivative by the log-probability."""
+def token_rows(logits, tokens, ignore_index, temperature):
+    """Log-probabilities of `tokens` [...] under `logits` [..., V] / temperature (0 where ignored), and the rows' maxima and
+    log2 of their sums [2 rows], which the gradient needs."""
     if logits.is_cuda:
-        r = N.token_rows(logits, tokens, ignore_index, temperature, policy)
+        r = N.token_rows(logits, tokens, ignore_index, temperature)
         if r is not NotImplemented:
             return r
         _fell("token_rows")
@@ -631,67 +630,80 @@ def token_rows(logits, tokens, ignore_index, temperature, policy=None):
     log_sum = torch.logsumexp((z - m) / temperature, -1, keepdim=True)
     tok = torch.where(valid, tokens, torch.zeros_like(tokens)).long().unsqueeze(-1)
     lp = ((z.gather(-1, tok) - m) / temperature - log_sum).squeeze(-1)
-    zero = torch.zeros_like(lp)
-    lp = torch.where(valid, lp, zero)
-    stats = torch.stack((m.reshape(-1), log_sum.reshape(-1) * math.log2(math.e)))
-    if policy is None:
-        return lp, stats
+    return torch.where(valid, lp, torch.zeros_like(lp)), torch.cat((m.reshape(-1), log_sum.reshape(-1) * math.log2(math.e)))
+
+
+def policy_loss(logits, tokens, ignore_index, temperature, policy, reduction):
+    """Clipped policy loss; `policy` = (old log-probabilities, advantages, rows per advantage, reference log-probabilities or
+    None, lowest ratio, highest ratio, KL weight).  Returns (loss, the rows' statistics as in `token_rows` followed by the
+    derivatives of their losses by the log-probabilities, a factor of all gradients [1] or None)."""
+    if logits.is_cuda:
+        r = N.policy_loss(logits, tokens, ignore_index, temperature, policy, reduction)
+        if r is not NotImplemented:
+            return r
     old, adv, div, ref, lo, hi, kl = policy
-    A = adv.reshape(-1).repeat_interleave(div).reshape(lp.shape).to(acc)
-    ratio = torch.exp(lp - old.reshape(lp.shape))
+    lp, stats = token_rows(logits, tokens, ignore_index, temperature)
+    valid, zero = tokens != ignore_index, torch.zeros_like(lp)
+    A = adv.reshape(-1).repeat_interleave(div).reshape(lp.shape)
+    ratio = torch.exp(lp - old)
     plain, clipped = -A * ratio, -A * ratio.clamp(lo, hi)
     loss = torch.maximum(plain, clipped)
     coef = torch.where(plain >= clipped, plain, zero)
     coef = torch.where(torch.isnan(loss), loss, coef)
     if ref is not None:
-        d = ref.reshape(lp.shape) - lp
+        d = ref - lp
         e = torch.exp(d)
         loss = loss + kl * (e - d - 1)
         coef = coef + kl * (1 - e)
-    return lp, stats, torch.where(valid, loss, zero), torch.where(valid, coef, zero)
+    loss = torch.where(valid, loss, zero)
+    stats = torch.cat((stats, torch.where(valid, coef, zero).reshape(-1)))
+    if reduction == "none":
+        return loss, stats, None
+    n = int(valid.sum())
+    f = 1.0 / n if reduction == "mean" and n else 1.0
+    return (loss.double().sum() * f).to(loss.dtype), stats, torch.tensor([f], dtype=loss.dtype, device=loss.device)
 
 
-def policy_sum(loss, tokens, vocab, ignore_index, mean):
-    """[sum (mean over the rows that count) of the rows' losses, the factor of their gradients]."""
-    if loss.is_cuda and loss.dtype == _F32:
-        return N.policy_sum(loss, tokens, vocab, ignore_index, mean)
-    n = int(((tokens != ignore_index) & (tokens >= 0) & (tokens < vocab)).sum())
-    f = 1.0 / n if mean and n else 1.0
-    return torch.stack(((loss.double().sum() * f).to(loss.dtype), torch.tensor(f, dtype=loss.dtype, device=loss.device)))
-
-
-def preference(lp, ref, beta, smoothing, mean, each):
-    """(loss per pair or None, loss, rewards [2 pairs], derivative of a pair's loss by every answer's sum [2 pairs])."""
-    if lp.is_cuda and lp.dtype == _F32:
-        return N.preference(lp, ref, beta, smoothing, mean, each)
+def preference_loss(logits, tokens, ignore_index, ref, beta, smoothing, reduction):
+    """(loss, rewards [2 pairs], the rows' statistics as in `token_rows` followed by the derivatives of a pair's loss by the
+    sums of its two answers' log-probabilities [2 pairs])."""
+    if logits.is_cuda:
+        r = N.preference_loss(logits, tokens, ignore_index, ref, beta, smoothing, reduction)
+        if r is not NotImplemented:
+            return r
+    lp, stats = token_rows(logits, tokens, ignore_index, 1.0)
     n = ref.numel()
-    rewards = (beta * (lp.double().reshape(n, -1).sum(1) - ref.double())).to(lp.dtype)
+    rewards = (beta * (lp.double().sum(-1) - ref.double())).to(lp.dtype)
     h = rewards[:n // 2] - rewards[n // 2:]
     lse = torch.log1p(torch.exp(-h.abs()))
     loss = (1 - smoothing) * ((-h).clamp(min=0) + lse) + smoothing * (h.clamp(min=0) + lse)
     g = beta * (smoothing - 1 / (1 + torch.exp(h)))
+    stats = torch.cat((stats, g, -g))
+    if reduction == "none":
+        return loss, rewards, stats
     total = loss.double().sum()
-    total = (total / (n // 2) if mean and n else total).to(lp.dtype)
-    return loss if each else None, total, rewards, torch.cat((g, -g))
+    return (total / (n // 2) if reduction == "mean" and n else total).to(lp.dtype), rewards, stats
 
 
-def token_grad(logits, tokens, stats, ignore_index, temperature, base=None, base_div=1, g=None, g_div=1, g_mod=1,
-               dev_scale=None, scale=1.0):
+def token_grad(logits, tokens, stats, ignore_index, temperature, base_div=0, g=None, g_div=1, g_mod=1, dev_scale=None,
+               scale=1.0):
     """Gradient of the logits: row r's derivative by its token's log-probability is
-    base[r // base_div] * g[r // g_div % g_mod] * dev_scale * scale (None: 1); zero for ignored rows."""
+    base[r // base_div] * g[r // g_div % g_mod] * dev_scale * scale, base being what follows the rows' statistics in `stats`
+    (base_div 0: 1; dev_scale None: 1); zero for ignored rows."""
     if logits.is_cuda and logits.dtype != torch.float64:
-        return N.token_grad(logits, tokens, stats, ignore_index, temperature, base, base_div, g, g_div, g_mod, dev_scale, scale)
+        return N.token_grad(logits, tokens, stats, ignore_index, temperature, base_div, g, g_div, g_mod, dev_scale, scale)
     rows, V = tokens.numel(), logits.shape[-1]
     r = torch.arange(rows, device=logits.device)
-    f = torch.full((rows,), scale, dtype=stats.dtype, device=logits.device)
-    for t, at in ((base, r // base_div), (g, r // g_div % g_mod), (dev_scale, r * 0)):
-        if t is not None:
-            f = f * t.reshape(-1)[at]
+    f = g.reshape(-1)[r // g_div % g_mod] * scale
+    if base_div:
+        f = f * stats[2 * rows:][r // base_div]
+    if dev_scale is not None:
+        f = f * dev_scale
     flat = tokens.reshape(-1)
     valid = (flat != ignore_index) & (flat >= 0) & (flat < V)
     f = torch.where(valid, f, torch.zeros_like(f)) / temperature
     z = logits.reshape(rows, V).to(stats.dtype)
-    p = torch.exp2((z - stats[0, :, None]) * (math.log2(math.e) / temperature) - stats[1, :, None])
+    p = torch.exp2((z - stats[:rows, None]) * (math.log2(math.e) / temperature) - stats[rows:2 * rows, None])
     p.scatter_add_(1, torch.where(valid, flat, torch.zeros_like(flat)).long()[:, None], -torch.ones_like(f)[:, None])
     d = torch.where((f == 0)[:, None], torch.zeros_like(p), p * -f[:, None])
     return d.reshape(logits.shape).to(logits.dtype)

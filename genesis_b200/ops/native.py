@@ -68,8 +68,9 @@ _SIGS = {
     "gb_index_put": "pp" + "d" + "ii" + "ppp" + "i" + "pp",
     "gb_cast_stack": "ppipip",
     "gb_masked_fill": "pp" + "d" + "ll" + "i" + "p", "gb_fill_elems": "pldip",
-    "gb_token_rows": "pppp" + "lllll" + "l" + "f" + "ppppp" + "l" + "fff" + "ii" + "pp",
-    "gb_policy_sum": "pp" + "lll" + "i" + "p" + "i" + "p", "gb_preference": "pp" + "ll" + "ff" + "i" + "pppp" + "p",
+    "gb_token_rows": "pppp" + "lllll" + "l" + "f" + "ii" + "pp",
+    "gb_policy_loss": "pppp" + "lllll" + "l" + "f" + "ppppp" + "l" + "fff" + "p" + "iii" + "pp",
+    "gb_preference_loss": "pppp" + "lllll" + "l" + "p" + "l" + "ff" + "i" + "pppp" + "ii" + "pp",
     "gb_token_grad": "pppp" + "lllll" + "l" + "f" + "pl" + "pll" + "p" + "f" + "ii" + "p",
     "gb_ns_workspace": "lllip", "gb_muon_momentum": "p" + "iiii" + "f" + "i" + "ppp" + "p",
     "gb_newton_schulz": "pp" + "iiiiii" + "fff" + "d" + "pp" + "fff" + "pp" + "pp" + "p",
@@ -1903,61 +1904,75 @@ def _row_map(logits):
 _TOKEN_DT = (torch.int64, torch.int32)
 
 
-def token_rows(logits, tokens, ignore_index, temperature, policy=None):
-    """(log-probabilities, row statistics [2, rows]) of `tokens` under `logits` [..., V]; with `policy` =
-    (old, advantages, rows per advantage, ref or None, lowest ratio, highest ratio, KL weight) also (loss, derivative)."""
+def token_rows(logits, tokens, ignore_index, temperature):
+    """(log-probabilities, row statistics [2, rows]) of `tokens` under `logits` [..., V]."""
     m = _row_map(logits)
     if logits.dtype not in _FLOATS or m is None:
         return NotImplemented
     rows, dev = tokens.numel(), logits.device
     lp = torch.empty(tokens.shape, dtype=F32, device=dev)
-    stats = torch.empty(2, rows, dtype=F32, device=dev)
-    old = adv = ref = loss = coef = None
-    div, lo, hi, kl = 1, 0.0, 0.0, 0.0
-    if policy is not None:
-        old, adv, div, ref, lo, hi, kl = policy
-        loss = torch.empty(tokens.shape, dtype=F32, device=dev)
-        coef = torch.empty(tokens.shape, dtype=F32, device=dev)
+    stats = torch.empty(2 * rows, dtype=F32, device=dev)
     with _on(dev):
         _chk(lib().gb_token_rows(logits.data_ptr(), tokens.data_ptr(), lp.data_ptr(), stats.data_ptr(), rows, logits.shape[-1],
-                                 *m, int(ignore_index), float(temperature), _ptr(old), _ptr(adv), _ptr(ref), _ptr(loss),
-                                 _ptr(coef), div, lo, hi, kl, _DT[logits.dtype], 1 if tokens.dtype == torch.int64 else 0,
+                                 *m, ignore_index, temperature, _DT[logits.dtype], 1 if tokens.dtype == torch.int64 else 0,
                                  status_tensor(dev).data_ptr(), _st()), "token_rows")
-    return (lp, stats) if policy is None else (lp, stats, loss, coef)
+    return lp, stats
 
 
-def policy_sum(loss, tokens, vocab, ignore_index, mean):
-    """[sum of the rows' losses (over their number with `mean`), the factor of their gradients]."""
-    out = torch.empty(2, dtype=F32, device=loss.device)
-    with _on(loss.device):
-        _chk(lib().gb_policy_sum(loss.data_ptr(), tokens.data_ptr(), tokens.numel(), vocab, int(ignore_index), 1 if mean else 0,
-                                 out.data_ptr(), 1 if tokens.dtype == torch.int64 else 0, _st()), "policy_sum")
-    return out
-
-
-def preference(lp, ref, beta, smoothing, mean, each):
-    """(loss per pair or None, loss [], rewards [2 pairs], derivative by every answer's sum [2 pairs])."""
-    dev, n = lp.device, ref.numel()
-    loss = torch.empty(n // 2, dtype=F32, device=dev) if each else None
-    out = torch.empty((), dtype=F32, device=dev)
-    rewards = torch.empty(n, dtype=F32, device=dev)
-    gseq = torch.empty(n, dtype=F32, device=dev)
-    with _on(dev):
-        _chk(lib().gb_preference(lp.data_ptr(), ref.data_ptr(), n // 2, lp.numel() // n if n else 0, float(beta),
-                                 float(smoothing), 1 if mean else 0, _ptr(loss), out.data_ptr(), rewards.data_ptr(),
-                                 gseq.data_ptr(), _st()), "preference")
-    return loss, out, rewards, gseq
-
-
-def token_grad(logits, tokens, stats, ignore_index, temperature, base, base_div, g, g_div, g_mod, dev_scale, scale):
-    """Gradient of [..., V] logits; row r's derivative by its token's log-probability is
-    base[r // base_div] * g[r // g_div % g_mod] * dev_scale * scale (None: 1)."""
+def policy_loss(logits, tokens, ignore_index, temperature, policy, reduction):
+    """(loss, rows' statistics [2, rows] followed by the derivatives of their losses [rows], factor of the gradients [1] or
+    None); `policy` as in `dispatch.policy_loss`."""
     m = _row_map(logits)
+    if logits.dtype not in _FLOATS or m is None:
+        return NotImplemented
+    old, adv, div, ref, lo, hi, kl = policy
+    rows, dev = tokens.numel(), logits.device
+    each = reduction == "none"
+    # one buffer: statistics, derivatives, log-probabilities, and the losses where they are not asked for
+    buf = torch.empty((4 if each else 5) * rows, dtype=F32, device=dev)
+    out = torch.empty(tokens.shape, dtype=F32, device=dev) if each else torch.empty(2, dtype=F32, device=dev)
+    at, op = buf.data_ptr(), out.data_ptr()
+    with _on(dev):
+        _chk(lib().gb_policy_loss(logits.data_ptr(), tokens.data_ptr(), at + 12 * rows, at, rows, logits.shape[-1], *m,
+                                  ignore_index, temperature, old.data_ptr(), adv.data_ptr(), _ptr(ref),
+                                  op if each else at + 16 * rows, at + 8 * rows, div, lo, hi, kl, None if each else op,
+                                  1 if reduction == "mean" else 0, _DT[logits.dtype], 1 if tokens.dtype == torch.int64 else 0,
+                                  status_tensor(dev).data_ptr(), _st()), "policy_loss")
+    return (out, buf, None) if each else (out[0], buf, out[1:])
+
+
+def preference_loss(logits, tokens, ignore_index, ref, beta, smoothing, reduction):
+    """(loss, rewards [2 pairs], rows' statistics [2, rows] followed by the derivatives by the answers' sums [2 pairs])."""
+    m = _row_map(logits)
+    if logits.dtype not in _FLOATS or m is None:
+        return NotImplemented
+    rows, n, dev = tokens.numel(), ref.numel(), logits.device
+    each = reduction == "none"
+    buf = torch.empty(3 * rows + n + 1, dtype=F32, device=dev)
+    out = torch.empty((n // 2,) if each else (), dtype=F32, device=dev)
+    rewards = torch.empty(n, dtype=F32, device=dev)
+    at, op = buf.data_ptr(), out.data_ptr()
+    with _on(dev):
+        _chk(lib().gb_preference_loss(logits.data_ptr(), tokens.data_ptr(), at + 8 * rows + 4 * n, at, rows, logits.shape[-1], *m,
+                                      ignore_index, ref.data_ptr(), n // 2, beta, smoothing, 1 if reduction == "mean" else 0,
+                                      op if each else None, at + 12 * rows + 4 * n if each else op, rewards.data_ptr(),
+                                      at + 8 * rows, _DT[logits.dtype], 1 if tokens.dtype == torch.int64 else 0,
+                                      status_tensor(dev).data_ptr(), _st()), "preference_loss")
+    return out, rewards, buf
+
+
+def token_grad(logits, tokens, stats, ignore_index, temperature, base_div, g, g_div, g_mod, dev_scale, scale):
+    """Gradient of [..., V] logits; row r's derivative by its token's log-probability is
+    base[r // base_div] * g[r // g_div % g_mod] * dev_scale * scale, base being what follows the rows' statistics in `stats`
+    (base_div 0: 1; dev_scale None: 1)."""
+    m = _row_map(logits)
+    rows = tokens.numel()
     out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    at = stats.data_ptr()
     with _on(logits.device):
-        _chk(lib().gb_token_grad(logits.data_ptr(), tokens.data_ptr(), stats.data_ptr(), out.data_ptr(), tokens.numel(),
-                                 logits.shape[-1], *m, int(ignore_index), float(temperature), _ptr(base), base_div, _ptr(g),
-                                 g_div, g_mod, _ptr(dev_scale), float(scale), _DT[logits.dtype],
+        _chk(lib().gb_token_grad(logits.data_ptr(), tokens.data_ptr(), at, out.data_ptr(), rows, logits.shape[-1], *m,
+                                 ignore_index, temperature, at + 8 * rows if base_div else None, base_div or 1, g.data_ptr(),
+                                 g_div, g_mod, _ptr(dev_scale), scale, _DT[logits.dtype],
                                  1 if tokens.dtype == torch.int64 else 0, _st()), "token_grad")
     return out
 
