@@ -56,11 +56,10 @@ struct Scale {
   __device__ __forceinline__ float operator()(float d) const { return fmaf(d, hi, d * lo); }
 };
 
-// (max, sum) pairs of two parts.  A part of -inf alone (or of nothing) is (-inf, 0).
-__device__ __forceinline__ MaxSum join(MaxSum a, MaxSum b, const Scale& c) {
-  const float m = fmaxf(a.m, b.m);
-  if (m == -INFINITY) return MaxSum{m, a.s + b.s};                 // (a NaN sum stays one)
-  return MaxSum{m, a.s * exp2f(c(a.m - m)) + b.s * exp2f(c(b.m - m))};
+// A part's sum relative to the maximum m of the whole; a part of -inf alone (or of nothing) is (-inf, 0).  expf here: the
+// hardware's exponential is 5e-8 of its result too small on average, and a sum passes through several of these.
+__device__ __forceinline__ float rescale(MaxSum a, float m, float temperature) {
+  return a.m == m || m == -INFINITY ? a.s : a.s * expf((a.m - m) / temperature);       // (a NaN sum stays one)
 }
 
 __device__ __forceinline__ float ex2(float x) {
@@ -199,15 +198,10 @@ __device__ __forceinline__ MaxSum scan(const T* p, int n, const Scale& c, int t,
   return a;
 }
 
-__device__ __forceinline__ MaxSum warp_join(MaxSum a, const Scale& c) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    MaxSum b;
-    b.m = __shfl_xor_sync(0xffffffffu, a.m, o);
-    b.s = __shfl_xor_sync(0xffffffffu, a.s, o);
-    a = join(a, b, c);
-  }
-  return a;
+// (max, sum) of the warp's parts, in every lane
+__device__ __forceinline__ MaxSum warp_join(MaxSum a, float temperature) {
+  const float m = warp_max(a.m);
+  return MaxSum{m, warp_sum(rescale(a, m, temperature))};
 }
 
 // The token of a row; false where the row does not count.  A token outside the vocabulary is reported and does not count.
@@ -221,8 +215,8 @@ __device__ __forceinline__ bool counts(const TI* tokens, long long r, long long 
 template <typename T, typename TI>
 __device__ __forceinline__ void finish_row(MaxSum a, const T* p, long long t, long long r, long long rows, float temperature,
                                            float* lp_out, float* stats, const Policy& q) {
-  // differences before products: z[t] - m is exact or nearly so where the token is likely
-  const float lp = (Cvt<T>::to_f(p[t]) - a.m) / temperature - logf(a.s);
+  // In 64 bits and rounded once.  Differences come before products: z[t] - m is small where the token is likely.
+  const float lp = (float)(((double)Cvt<T>::to_f(p[t]) - (double)a.m) / (double)temperature - log((double)a.s));
   lp_out[r] = lp;
   stats[r] = a.m;
   stats[rows + r] = log2f(a.s);
@@ -267,7 +261,7 @@ token_rows_warp_kernel(const T* __restrict__ z, RowMap map, const TI* __restrict
     return;
   }
   const T* p = z + map.at(r);
-  const MaxSum a = warp_join(scan<T, 32, 0>(p, cols, c, lane), c);
+  const MaxSum a = warp_join(scan<T, 32, 0>(p, cols, c, lane), temperature);
   if (lane == 0) finish_row<T, TI>(a, p, t, r, rows, temperature, lp, stats, q);
 }
 
@@ -300,23 +294,27 @@ token_rows_kernel(const T* __restrict__ z, RowMap map, const TI* __restrict__ to
     lo = min(part * step, cols);
     n = min(step, cols - lo);
   }
-  MaxSum a = warp_join(scan<T, G, G == 512 ? RING : 0>(p + lo, n, c, threadIdx.x, ring), c);
+  MaxSum a = warp_join(scan<T, G, G == 512 ? RING : 0>(p + lo, n, c, threadIdx.x, ring), temperature);
   if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = make_float2(a.m, a.s);
   __syncthreads();
   if (threadIdx.x < 32) {
     a = MaxSum{-INFINITY, 0.f};
     if (threadIdx.x < G / 32) a = MaxSum{sh[threadIdx.x].x, sh[threadIdx.x].y};
-    a = warp_join(a, c);
+    a = warp_join(a, temperature);
   }
   if (parts > 1) {
     cg::cluster_group cl = cg::this_cluster();
     if (threadIdx.x == 0) mine = make_float2(a.m, a.s);
     cl.sync();
     if (part == 0 && threadIdx.x == 0) {
+      float m = a.m;
+      for (int k = 1; k < parts; ++k) m = fmaxf(m, cl.map_shared_rank(&mine, k)->x);
+      float sum = rescale(a, m, temperature);
       for (int k = 1; k < parts; ++k) {
         const float2 o = *cl.map_shared_rank(&mine, k);
-        a = join(a, MaxSum{o.x, o.y}, c);
+        sum += rescale(MaxSum{o.x, o.y}, m, temperature);
       }
+      a = MaxSum{m, sum};
     }
     cl.sync();                                                     // nobody leaves while its part may still be read
   }

@@ -219,10 +219,10 @@ def test_post_training_steps_of_a_model():
     graphed[2].make_capturable()
     run = genesis.cuda.GraphedTrainStep(lambda: step(*graphed), graphed[1], [], warmup=3)
     again = [run().item() for _ in range(2)]
-    # (the embedding's gradient is added up in memory in no fixed order: its last bits, 2^-24 of it, and through Adam's
-    # division the steps of weights whose gradient is about zero, differ from run to run.  To first order neither moves the loss:
-    # 1e-3 sum |g| over gradients of at most 1e-9, for 515 x 64 weights 3e-8, and rounding of the loss, 2^-24)
-    assert max(abs(a - b) for a, b in zip(again, losses[3:])) < 1e-6
+    # The framework adds up the embedding's gradient in memory in no fixed order, so runs differ in its last bits (eager ones
+    # too), and the next step's gradients by some 1e-7 of themselves.  The iteration amplifies that by 485 at most: updates of
+    # 2-norm 0.02 * 485 * 1e-7 = 1e-6 for each of the 14 matrices, against gradients of 2-norm 0.5 at most: 7e-6 of the loss.
+    assert max(abs(a - b) for a, b in zip(again, losses[3:])) < 1e-5
     assert graphed[1].t == 5
     # the gradient of one weight against differences of the loss, along the gradient
     model = build()[0]
