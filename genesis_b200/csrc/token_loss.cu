@@ -104,20 +104,11 @@ __device__ __forceinline__ float vec_max(const uint4& v) {
   }
 }
 
-__device__ __forceinline__ void copy16(uint32_t smem_dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void copies_issued() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-
-// What thread `t` of `G` sees of the `n` elements at p: running maximum and sum, two vectors of 16 bytes at a time.  Elements
+// What thread `t` of `G` sees of the `n` elements at p: running maximum and sum, U vectors of 16 bytes at a time.  Elements
 // before the first 16-byte boundary and behind the last are taken one by one, so rows of odd length cost no more than
-// aligned ones.  With RING > 0 the vectors come through a ring of RING pairs in shared memory that belongs to the thread
-// alone (asynchronous copies, no barriers): 16 RING * 2 bytes of every thread are always on their way, where plain loads
-// leave the memory idle while they are worked on.
-template <typename T, int G, int RING>
-__device__ __forceinline__ MaxSum scan(const T* p, int n, const Scale& c, int t, uint8_t* ring = nullptr) {
+// aligned ones.
+template <typename T, int G, int U>
+__device__ __forceinline__ MaxSum scan(const T* p, int n, const Scale& c, int t) {
   constexpr int V = 16 / sizeof(T), H = V / 2;
   MaxSum a{-INFINITY, 0.f};
   auto raise = [&](float mx) {
@@ -148,53 +139,25 @@ __device__ __forceinline__ MaxSum scan(const T* p, int n, const Scale& c, int t,
   if (head > n) head = n;
   const uint4* v = reinterpret_cast<const uint4*>(p + head);
   const int nv = (n - head) / V, rest = head + nv * V + t;
-  if constexpr (RING > 0) {
-    const uint32_t base = smem_u32(ring) + t * 16;                 // vector k of a pair in slot s: base + (2 s + k) * 16 G
-    auto fetch = [&](int i, int s) {
+  if (t < head) one(p[t]);
+  int i = t;
+  for (; i + (U - 1) * G < nv; i += U * G) {
+    uint4 x[U];
+    float mx = -INFINITY;
 #pragma unroll
-      for (int k = 0; k < 2; ++k)
-        if (i + k * G < nv) copy16(base + (2 * s + k) * 16 * G, v + i + k * G);
-      copies_issued();
-    };
+    for (int k = 0; k < U; ++k) x[k] = v[i + k * G];
 #pragma unroll
-    for (int s = 0; s < RING; ++s) fetch(t + s * 2 * G, s);
-    if (t < head) one(p[t]);
-    if (rest < n) one(p[rest]);
-    int s = 0;
-    for (int i = t; i < nv; i += 2 * G) {
-      copies_wait<RING - 1>();
-      const uint4* slot = reinterpret_cast<const uint4*>(ring + t * 16 + s * 32 * G);
-      const bool two = i + G < nv;
-      const uint4 x = slot[0], y = two ? slot[G] : x;
-      raise(fmaxf(vec_max<T>(x), vec_max<T>(y)));
-      fetch(i + RING * 2 * G, s);
-      add(x);
-      if (two) add(y);
-      s = s + 1 == RING ? 0 : s + 1;
-    }
-    copies_wait<0>();
-  } else {
-    constexpr int U = 4;
-    if (t < head) one(p[t]);
-    int i = t;
-    for (; i + (U - 1) * G < nv; i += U * G) {
-      uint4 x[U];
-      float mx = -INFINITY;
+    for (int k = 0; k < U; ++k) mx = fmaxf(mx, vec_max<T>(x[k]));
+    raise(mx);
 #pragma unroll
-      for (int k = 0; k < U; ++k) x[k] = v[i + k * G];
-#pragma unroll
-      for (int k = 0; k < U; ++k) mx = fmaxf(mx, vec_max<T>(x[k]));
-      raise(mx);
-#pragma unroll
-      for (int k = 0; k < U; ++k) add(x[k]);
-    }
-    for (; i < nv; i += G) {
-      const uint4 x = v[i];
-      raise(vec_max<T>(x));
-      add(x);
-    }
-    if (rest < n) one(p[rest]);
+    for (int k = 0; k < U; ++k) add(x[k]);
   }
+  for (; i < nv; i += G) {
+    const uint4 x = v[i];
+    raise(vec_max<T>(x));
+    add(x);
+  }
+  if (rest < n) one(p[rest]);
   return a;
 }
 
@@ -261,20 +224,20 @@ token_rows_warp_kernel(const T* __restrict__ z, RowMap map, const TI* __restrict
     return;
   }
   const T* p = z + map.at(r);
-  const MaxSum a = warp_join(scan<T, 32, 0>(p, cols, c, lane), temperature);
+  const MaxSum a = warp_join(scan<T, 32, 4>(p, cols, c, lane), temperature);
   if (lane == 0) finish_row<T, TI>(a, p, t, r, rows, temperature, lp, stats, q);
 }
 
-constexpr int RING = 4;
-
 // Longer rows: one CTA of G threads each, or, where rows are few, the CTAs of a cluster share one and rank 0 joins their
-// parts through distributed shared memory.  G = 512 reads through the ring, three CTAs on an SM.
+// parts through distributed shared memory.  16-bit rows of 512 threads are bound by the exponentials as much as by memory, so
+// as many threads as fit keep two vectors in flight each; 32-bit ones, with half the exponentials a byte, do better with
+// fewer threads and four vectors.  Over 6973 rows of 151936 bf16, us: two vectors and four CTAs on an SM 398 (5.3 TB/s), two
+// and three 415, four and two 424, rings of asynchronous copies private to a thread 472; 2048 of fp32: 221, 209, 199, 209.
 template <typename T, typename TI, int G>
-__global__ void __launch_bounds__(G, G == 512 ? 3 : 8)
+__global__ void __launch_bounds__(G, G == 512 ? (sizeof(T) == 2 ? 4 : 2) : 8)
 token_rows_kernel(const T* __restrict__ z, RowMap map, const TI* __restrict__ tokens, float* __restrict__ lp,
                   float* __restrict__ stats, long long rows, int cols, long long ignore, float temperature, Scale c,
                   Policy q, int* status, int parts) {
-  extern __shared__ __align__(16) uint8_t ring[];
   __shared__ float2 sh[G / 32];
   __shared__ float2 mine;
   const long long r = blockIdx.x / parts;
@@ -294,7 +257,7 @@ token_rows_kernel(const T* __restrict__ z, RowMap map, const TI* __restrict__ to
     lo = min(part * step, cols);
     n = min(step, cols - lo);
   }
-  MaxSum a = warp_join(scan<T, G, G == 512 ? RING : 0>(p + lo, n, c, threadIdx.x, ring), temperature);
+  MaxSum a = warp_join(scan<T, G, G == 512 && sizeof(T) == 2 ? 2 : 4>(p + lo, n, c, threadIdx.x), temperature);
   if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = make_float2(a.m, a.s);
   __syncthreads();
   if (threadIdx.x < 32) {
@@ -517,14 +480,11 @@ static int rows_forward(const void* z, RowMap map, const void* tokens, float* lp
   // a part has to be worth its cluster barriers: 4096 elements at least
   int parts = 1;
   while (parts < 8 && rows * parts * 2 <= 3 * sms && cols / (parts * 2) >= 4096) parts *= 2;
-  constexpr int smem = RING * 32 * 512;
-  static unsigned long long configured = 0;
-  if (int r = smem_opt_in(token_rows_kernel<T, TI, 512>, smem, configured)) return r;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = parts; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
-  cfg.gridDim = dim3((unsigned)(rows * parts)); cfg.blockDim = dim3(512); cfg.dynamicSmemBytes = smem; cfg.stream = st;
+  cfg.gridDim = dim3((unsigned)(rows * parts)); cfg.blockDim = dim3(512); cfg.stream = st;
   cfg.attrs = attr; cfg.numAttrs = parts > 1 ? 1 : 0;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, token_rows_kernel<T, TI, 512>, (const T*)z, map, (const TI*)tokens, lp, stats, rows,
                                            cols, ignore, temperature, c, q, status, parts);
