@@ -1,27 +1,35 @@
 // Newton-Schulz orthogonalisation of weight updates: the singular values of a matrix are driven to about one by
 //
-//   X = G / (|G|_F + eps),   repeated:  A = X X^T,  B = b A + c A A,  X <- a X + B X          (X: m x n, m <= n)
+//   X = G / (|G|_F + eps),   repeated:  A = X X^T,  B = b A + c A A,  X <- (a I + B) X           (X: m x n, m <= n)
 //
 // i.e. every singular value s goes to a s + b s^3 + c s^5.  A tall G is handled as its transpose.
 //
-// Arithmetic.  The iteration amplifies: with the usual coefficients a small singular value grows by a factor of
-// 3.44 a step, 485 over five, and so does every rounding of X in its direction.  So X is kept in 32 bits, and enters the
-// tensor cores as two fp16 terms, x 2^k = hi + lo, which hold 22 of its 24 bits (k keeps the largest entry near the top
-// of fp16's range, so that lo stays clear of its subnormals: |x_ij| is at most the spectral norm, which the host bounds
-// from the coefficients).  Each product is three of fp16 with fp32 accumulation, hi hi + hi lo + lo hi; a X is added in
-// 32 bits from X itself.  Errors measured against 64 bits (256 x 1024, Gaussian / rank 8 plus noise): 9e-7 / 6e-7, of the
-// products in fp32 1.7e-7 / 5.9e-7, with one fp16 term 1.7e-3, with terms but without X in 32 bits 7e-7 / 4e-6.
+// Products of m x m matrices in place of m x n ones.  With P = a I + B, the next A is P A P, so a block of steps needs X
+// only at its ends: A = X X^T once, then per step  B = b A + c A A,  W = a A + B A,  A <- a W + B W,  and the product of the
+// P's, kept as s I + Q:  Q <- a Q + s B + B Q.  At the end of the block X <- s X + Q X.  All but the last are symmetric.
+// For 896 x 4864 and five steps in blocks of three and two that is 33 GFLOP for the 62 of five products with X each way, and
+// X passes through memory twice instead of five times; for square matrices it is as many operations.  A rounding of A grows
+// by a^2 a step, so blocks are short: simulated over spectra from Gaussian to rank one plus noise, blocks of up to three are
+// as exact as products with X (256 x 1024: 2.4e-6 for 1.5e-6 Gaussian, 0.6e-6 for 0.5e-6 rank 8 plus noise; fp32 products
+// throughout 2.0e-6 and 2.0e-6), five in one lose a digit (5e-6, 21e-6).
 //
-// Work.  A and B are symmetric: only tiles on and below the diagonal are computed, the rest is written as their mirror
-// image by the same epilogue.  A step is three launches over all matrices of a batch, 128 x 128 tiles on persistent CTAs:
+// Arithmetic.  The iteration amplifies: with the usual coefficients a small singular value grows by a factor of
+// 3.44 a step, 485 over five, and so does every rounding of X in its direction.  So X, A and W are kept in 32 bits, and enter
+// the tensor cores as two fp16 terms, x 2^k = hi + lo, which hold 22 of its 24 bits (k keeps the largest entry near the top
+// of fp16's range, so that lo stays clear of its subnormals: an entry is at most the largest eigenvalue, which the host
+// bounds from the coefficients).  Each product is three of fp16 with fp32 accumulation, hi hi + hi lo + lo hi; a X, a A and a W
+// are added in 32 bits from the matrices themselves.  One fp16 term alone loses three digits (1.7e-3).
+//
+// Work.  Of symmetric results only tiles on and below the diagonal are computed, the rest is written as their mirror image by
+// the same epilogue.  A product is one launch over all matrices of a batch (W and Q of a step together), on persistent CTAs:
 //   warp 0 TMA producer, warp 1 issues tcgen05.mma, warps 4-11 epilogue; accumulators in all of tensor memory.
-// A stage holds both terms of both operands for 64 elements of the contraction (64 KB) and feeds three products, so an SM
-// reads 85 bytes a clock from L2 at the full tensor rate, as the single-product GEMM with tiles of 128 x 256 does.
-// Tiles too few to fill the GPU are shared by clusters of up to 8 CTAs, each with a part of the contraction.
+// A block of 64 elements of the contraction brings both terms of both operands and feeds three products.  Tiles too few to
+// fill the GPU are shared by clusters of up to 8 CTAs, each with a part of the contraction; many large ones are worked on by
+// CTA pairs, which read two thirds of the bytes.
 //
 // Sums.  The tensor cores round their accumulator towards zero, which adds up over a long contraction (4864 x 896: 1.6e-5 of
-// the result).  So an accumulator takes up 512 elements of the contraction (256 in tiles of 128 columns) and is then added, rounded to nearest, to the
-// sums that the epilogue's warps hold in registers; the products go on in the next of four accumulators meanwhile.
+// the result).  So an accumulator takes up 512 elements of the contraction (256 in tiles of 128 columns) and is then added,
+// rounded to nearest, to the sums that the epilogue's warps hold in registers; the products go on in the next one meanwhile.
 #include "sm100_ptx.cuh"
 #include "sm100_pair.cuh"
 #include "common.cuh"
@@ -43,22 +51,38 @@ constexpr int SMEM_TOTAL = BARRIER_OFFSET + 256;
 constexpr int THREADS = 384;                          // warps 0 TMA, 1 MMA, 2 and 3 idle, 4-11 epilogue
 constexpr int PARTS = 256;                            // most partial sums of squares per matrix
 
-enum Mode : int { GRAM = 0, SQUARE = 1, APPLY = 2, APPLY_LAST = 3 };
+enum Mode : int { SYM = 0, APPLY = 1, APPLY_LAST = 2 };
+
+// m x m matrices of a batch live in slots: terms [SLOTS][batch][hi, lo][m][lda] and, where they are needed, the matrices
+// themselves in 32 bits [SLOTS][batch][m][lda], on and below the diagonal only.
+constexpr int SLOTS = 5;
+
+// out = f_acc L R + f1 M1 + f2 M2, symmetric
+struct Problem {
+  int left, right;             // slots of L and R (GRAM: X both)
+  int out;                     // slot
+  int m1, m2;                  // slots of M1, M2 or -1
+  int keep;                    // the result in 32 bits is kept too
+  float f_acc, f1, f2;
+  float scale;                 // 2^k of the result's terms
+};
 
 struct Params {
   int* status;
   int m, n, batch;             // X [batch, m, n]
-  int ldx, lda;                // pitch of X and of A, B in elements (multiples of 8)
-  __half* dst;                 // GRAM: A, SQUARE: B, APPLY: the next X; planes [batch][hi, lo][m][ld]
-  const __half* a_planes;      // SQUARE: A
-  float* x;                    // APPLY: X in 32 bits [batch][m][ldx]
-  float f_acc, f_a;            // result = f_acc * accumulator + f_a * (SQUARE: A as stored; APPLY: X)
-  float next_scale;            // APPLY: 2^k of the next X
+  int k;                       // elements of the contraction
+  int ldx, lda;                // pitch of X and of m x m matrices in elements (multiples of 8)
+  int problems;                // SYM: one or two for every matrix of the batch
+  Problem prob[2];             // APPLY: prob[0].left is Q, X <- f_acc Q X + f1 X
+  __half* terms;               // slots
+  float* whole;
+  __half* dst;                 // APPLY: terms of the next X [batch][hi, lo][m][ldx]
+  float* x;                    // X in 32 bits [batch][m][ldx]
   // APPLY_LAST: out[batch] in `out_dtype`, or the weights of an optimizer step through `weights`
   void* out;
   int out_dtype, tall;         // tall: the result goes out transposed, [n, m]
   const long long* weights;    // [batch] addresses of fp32 weights (+ 1 where the weight is tall), or null
-  float lr, decay, scale;      // w <- w (1 - lr decay) - lr o, or scale lr o where it is tall
+  float lr, decay, tall_scale; // w <- w (1 - lr decay) - lr o, or tall_scale lr o where it is tall
   const float* dyn_lr;
   const float* found_inf;
   int splits;                  // CTAs of a cluster that share a tile's contraction (1: whole tiles, persistent CTAs)
@@ -113,46 +137,63 @@ struct Epilogue {
   }
   // symmetric results: blocks of 128 below the diagonal are written twice, those above it not at all
   __device__ __forceinline__ bool outside(int row0, int col0) const {
-    constexpr bool SYM = MODE == GRAM || MODE == SQUARE;
-    return row0 >= p.m || col0 >= (SYM ? p.m : p.n) || (SYM && col0 / BM > row0 / BM);
+    return row0 >= p.m || col0 >= (MODE == SYM ? p.m : p.n) || (MODE == SYM && col0 / BM > row0 / BM);
   }
-  // What a chunk's results are made from besides its sums: X, or both terms of A
-  __device__ __forceinline__ void fetch(uint4 (&in)[8], int z, int row0, int col0) const {
-    const int u = lane & 7, r0 = lane >> 3, col = col0 + 4 * u;
-    if constexpr (MODE != GRAM) {
-      const int rows = outside(row0, col0) || col >= (MODE == SQUARE ? p.m : p.n) ? 0 : p.m - row0 - r0;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        in[i] = make_uint4(0u, 0u, 0u, 0u);
-        if (4 * i >= rows) continue;
-        if constexpr (MODE == SQUARE) {
-          const size_t plane = (size_t)p.m * p.lda;
-          const __half* a = p.a_planes + (size_t)z * 2 * plane + (size_t)(row0 + r0 + 4 * i) * p.lda + col;
-          const uint2 hi = *reinterpret_cast<const uint2*>(a), lo = *reinterpret_cast<const uint2*>(a + plane);
-          in[i] = make_uint4(hi.x, hi.y, lo.x, lo.y);
-        } else {
-          in[i] = *reinterpret_cast<const uint4*>(p.x + ((size_t)z * p.m + row0 + r0 + 4 * i) * p.ldx + col);
-        }
-      }
+  // four elements of row `row` of the 32-bit matrix in slot `slot` of matrix z
+  __device__ __forceinline__ float* whole(int slot, int z, int row, int col) const {
+    return p.whole + (((size_t)slot * p.batch + z) * p.m + row) * p.lda + col;
+  }
+  // What a chunk's results are made from besides its sums: X, or M1
+  __device__ __forceinline__ void fetch(float4 (&in)[8], int z, int row0, int col0) const {
+    const int r0 = lane >> 3, col = col0 + 4 * (lane & 7);
+    int rows = outside(row0, col0) || col >= (MODE == SYM ? p.m : p.n) ? 0 : p.m - row0 - r0;
+    const float* src;
+    size_t pitch;
+    if constexpr (MODE == SYM) {
+      const Problem& q = p.prob[z >= p.batch];
+      if (q.m1 < 0) rows = 0;
+      src = whole(q.m1, z >= p.batch ? z - p.batch : z, row0 + r0, col);
+      pitch = 4 * (size_t)p.lda;
+    } else {
+      src = p.x + ((size_t)z * p.m + row0 + r0) * p.ldx + col;
+      pitch = 4 * (size_t)p.ldx;
     }
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      in[i] = 4 * i < rows ? *reinterpret_cast<const float4*>(src + i * pitch) : make_float4(0.f, 0.f, 0.f, 0.f);
   }
-  __device__ __forceinline__ void run(const float4 (&acc)[8], const uint4 (&in)[8], uint8_t* chunk, int z, int row0, int col0) const {
-    constexpr bool SYM = MODE == GRAM || MODE == SQUARE;
-    const int cols = SYM ? p.m : p.n;
+  __device__ __forceinline__ void run(const float4 (&acc)[8], const float4 (&in)[8], uint8_t* chunk, int z, int row0, int col0) const {
+    const int cols = MODE == SYM ? p.m : p.n;
     if (outside(row0, col0)) return;
     const int u = lane & 7, r0 = lane >> 3, col = col0 + 4 * u;
     const int rows = col < cols ? p.m - row0 - r0 : 0;           // (rows 4 i of this lane below it are inside the matrix)
-    if constexpr (SYM) {
+    const Problem& q = p.prob[MODE == SYM && z >= p.batch];
+    float4 v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = axpby(acc[i], q.f_acc, in[i], q.f1);
+    if constexpr (MODE == SYM) {
+      if (z >= p.batch) z -= p.batch;
       const bool mirror = col0 / BM < row0 / BM;
-      const size_t plane = (size_t)p.m * p.lda, zo = (size_t)z * 2 * plane, at = zo + (size_t)(row0 + r0) * p.lda + col;
       const size_t pitch = 4 * (size_t)p.lda;
+      if (q.m2 >= 0) {
+        const float* src = whole(q.m2, z, row0 + r0, col);
+        float4 w[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = 4 * i < rows ? *reinterpret_cast<const float4*>(src + i * pitch) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = axpby(w[i], q.f2, v[i], 1.f);
+      }
+      if (q.keep) {
+        float* dst = whole(q.out, z, row0 + r0, col);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (4 * i < rows) *reinterpret_cast<float4*>(dst + i * pitch) = v[i];
+      }
+      const size_t plane = (size_t)p.m * p.lda;
+      __half* base = p.terms + ((size_t)q.out * p.batch + z) * 2 * plane;
       uint4 t[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        float v[4] = {acc[i].x * p.f_acc, acc[i].y * p.f_acc, acc[i].z * p.f_acc, acc[i].w * p.f_acc};
-        if constexpr (MODE == SQUARE) add_a(v, make_uint2(in[i].x, in[i].y), make_uint2(in[i].z, in[i].w));
-        t[i] = split4(v[0], v[1], v[2], v[3]);
-      }
+      for (int i = 0; i < 8; ++i) t[i] = split4(v[i].x * q.scale, v[i].y * q.scale, v[i].z * q.scale, v[i].w * q.scale);
       if (mirror) {
         // both terms of an element in the place of its sum; then columns are read as rows
         __syncwarp();
@@ -163,9 +204,10 @@ struct Epilogue {
                          __byte_perm(t[i].y, t[i].w, 0x5410), __byte_perm(t[i].y, t[i].w, 0x7632));
         __syncwarp();
       }
+      __half* dst = base + (size_t)(row0 + r0) * p.lda + col;
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        if (4 * i < rows) put(p.dst + at + i * pitch, plane, t[i]);
+        if (4 * i < rows) put(dst + i * pitch, plane, t[i]);
       if (mirror) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -175,34 +217,25 @@ struct Epilogue {
                             __byte_perm(w[2], w[3], 0x7632));
         }
         const int j = row0 + 4 * u, left = j < p.m ? p.m - col0 - r0 : 0;
-        __half* out = p.dst + zo + (size_t)(col0 + r0) * p.lda + j;
+        __half* out = base + (size_t)(col0 + r0) * p.lda + j;
 #pragma unroll
         for (int i = 0; i < 8; ++i)
           if (4 * i < left) put(out + i * pitch, plane, t[i]);
       }
     } else {
-      float* x = p.x + ((size_t)z * p.m + row0 + r0) * p.ldx + col;
-      const size_t pitch = 4 * (size_t)p.ldx;
-      float4 v[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        v[i] = make_float4(__uint_as_float(in[i].x), __uint_as_float(in[i].y), __uint_as_float(in[i].z), __uint_as_float(in[i].w));
       if constexpr (MODE == APPLY) {
-        const size_t plane = (size_t)p.m * p.ldx;
+        float* x = p.x + ((size_t)z * p.m + row0 + r0) * p.ldx + col;
+        const size_t pitch = 4 * (size_t)p.ldx, plane = (size_t)p.m * p.ldx;
         __half* dst = p.dst + (size_t)z * 2 * plane + (size_t)(row0 + r0) * p.ldx + col;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          v[i] = combine(acc[i], v[i]);
           if (4 * i < rows) {
             *reinterpret_cast<float4*>(x + i * pitch) = v[i];
-            const float f = p.next_scale;
-            put(dst + i * pitch, plane, split4(v[i].x * f, v[i].y * f, v[i].z * f, v[i].w * f));
+            put(dst + i * pitch, plane, split4(v[i].x * q.scale, v[i].y * q.scale, v[i].z * q.scale, v[i].w * q.scale));
           }
         }
       } else {
         const bool across = p.weights != nullptr ? (p.weights[z] & 1) != 0 : p.tall != 0;     // the result is the transpose
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = combine(acc[i], v[i]);
         if (across) {
           __syncwarp();
 #pragma unroll
@@ -220,7 +253,7 @@ struct Epilogue {
         const int left = count > 0 ? (across ? p.n : p.m) - i0 - r0 : 0;
         const size_t at = (size_t)(i0 + r0) * ld + j, lp = 4 * (size_t)ld;
         if (p.weights != nullptr) {
-          if (!skip) apply(reinterpret_cast<float*>(p.weights[z] & ~1ll) + at, lp, left, count, ld, across ? step * p.scale : step, v);
+          if (!skip) apply(reinterpret_cast<float*>(p.weights[z] & ~1ll) + at, lp, left, count, ld, across ? step * p.tall_scale : step, v);
         } else if (p.out_dtype == DT_F32) {
           float* o = reinterpret_cast<float*>(p.out) + (size_t)z * p.m * p.n + at;
 #pragma unroll
@@ -281,20 +314,13 @@ struct Epilogue {
       }
     }
   }
-  __device__ __forceinline__ float4 combine(const float4& a, const float4& x) const {
-    return make_float4(fmaf(a.x, p.f_acc, x.x * p.f_a), fmaf(a.y, p.f_acc, x.y * p.f_a), fmaf(a.z, p.f_acc, x.z * p.f_a),
-                       fmaf(a.w, p.f_acc, x.w * p.f_a));
+  __device__ __forceinline__ float4 axpby(const float4& a, float f, const float4& b, float g) const {
+    return make_float4(fmaf(a.x, f, b.x * g), fmaf(a.y, f, b.y * g), fmaf(a.z, f, b.z * g), fmaf(a.w, f, b.w * g));
   }
   // four rows 4 u .. of column `c` of the chunk
   __device__ __forceinline__ void column(const uint8_t* chunk, int c, int u, uint32_t (&v)[4]) const {
 #pragma unroll
     for (int k = 0; k < 4; ++k) v[k] = *reinterpret_cast<const uint32_t*>(chunk + chunk_at(4 * u + k, c >> 2) + (c & 3) * 4);
-  }
-  __device__ __forceinline__ void add_a(float (&v)[4], const uint2& x, const uint2& y) const {
-    const float2 x0 = __half22float2(*reinterpret_cast<const __half2*>(&x.x)), x1 = __half22float2(*reinterpret_cast<const __half2*>(&x.y));
-    const float2 y0 = __half22float2(*reinterpret_cast<const __half2*>(&y.x)), y1 = __half22float2(*reinterpret_cast<const __half2*>(&y.y));
-    v[0] = fmaf(x0.x + y0.x, p.f_a, v[0]); v[1] = fmaf(x0.y + y0.y, p.f_a, v[1]);
-    v[2] = fmaf(x1.x + y1.x, p.f_a, v[2]); v[3] = fmaf(x1.y + y1.y, p.f_a, v[3]);
   }
   // (the pitch is a multiple of 8, so what lies past the last column is padding)
   __device__ __forceinline__ void put(__half* hi, size_t plane, const uint4& t) const {
@@ -303,7 +329,7 @@ struct Epilogue {
   }
   // What this lane's warp will read of a chunk at its end is fetched into L2 while the products run: one line a lane
   __device__ __forceinline__ void prefetch(int z, int row0, int col0) const {
-    if constexpr (MODE == APPLY || MODE == APPLY_LAST) {
+    if constexpr (MODE != SYM) {
       if (row0 + lane < p.m && col0 < p.n) prefetch_l2(p.x + ((size_t)z * p.m + row0 + lane) * p.ldx + col0);
       if constexpr (MODE == APPLY_LAST) {
         if (p.weights != nullptr) {
@@ -329,9 +355,9 @@ __host__ __device__ constexpr long long tiles_of(bool sym, long long m, long lon
 
 template <int MODE, int BN, int KIND>
 __global__ void __launch_bounds__(THREADS, 1)
-ns_product_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_constant__ CUtensorMap tmapB, const Params p) {
-  constexpr bool SYM = MODE == GRAM || MODE == SQUARE;
-  constexpr bool B_MN = !SYM;                           // X as the right operand: its rows run along the contraction
+ns_product_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_constant__ CUtensorMap tmapB,
+                  const __grid_constant__ Params p) {
+  constexpr bool B_MN = MODE != SYM;                           // X as the right operand: its rows run along the contraction
   constexpr int TM = KIND == PAIR ? 2 * BM : BM;        // rows of a tile
   constexpr int BNC = KIND == PAIR ? BN / 2 : BN;       // columns of the right operand that a CTA loads
   // Ring of half stages: (A hi, B lo) and (A lo, B hi) of a block of the contraction.  The three products of a block run in
@@ -383,9 +409,9 @@ ns_product_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_consta
   wait_for_previous();
 
   const int tm = (p.m + TM - 1) / TM;
-  const int per = (int)tiles_of(SYM, p.m, p.n, TM, BN);
-  const long long total = (long long)per * p.batch;
-  const int kblocks = ((MODE == GRAM ? p.n : p.m) + BK - 1) / BK;
+  const int per = (int)tiles_of(MODE == SYM, p.m, p.n, TM, BN);
+  const long long total = (long long)per * p.batch * p.problems;
+  const int kblocks = (p.k + BK - 1) / BK;
   // this CTA's tiles and its part of their contraction, in blocks of BK
   const int splits = KIND == SPLIT ? p.splits : 1, group = KIND == PAIR ? 2 : splits;
   const long long first = blockIdx.x / group, stride = gridDim.x / group;
@@ -395,7 +421,7 @@ ns_product_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_consta
   auto decode = [&](long long t, int& mi, int& ni, int& z) {
     z = (int)(t / per);
     const int r = (int)(t % per);
-    if constexpr (SYM) {
+    if constexpr (MODE == SYM) {
       if constexpr (BN == TM) {
         mi = (int)((sqrtf(8.f * (float)r + 1.f) - 1.f) * 0.5f);
         while (mi * (mi + 1) / 2 > r) --mi;
@@ -432,6 +458,10 @@ ns_product_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_consta
           int mi, ni, z;
           decode(t, mi, ni, z);
           const int m0 = mi * TM + row_in_tile, n0 = ni * BN + (KIND == PAIR ? rank * BNC : 0);
+          // planes of the operands: two for every matrix of a slot
+          const Problem& pr = p.prob[z >= p.batch];
+          const int zz = z >= p.batch ? z - p.batch : z;
+          const int za = 2 * (pr.left * p.batch + zz), zb = 2 * (pr.right * p.batch + zz);
           bool ok = true;
           for (int kh = 2 * kb0; kh < 2 * kb1; ++kh, ++it) {
             const int s = it % HALVES, k0 = (kh >> 1) * BK, h = kh & 1;      // h: A's term (0 = hi); B's is the other
@@ -441,23 +471,23 @@ ns_product_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_consta
             if constexpr (KIND == PAIR) {
               const uint32_t bar = g2::map_to_cta(smem_u32(&full_bar[s]), 0);
               if (rank == 0) mbar_expect_tx(&full_bar[s], 2 * HALF_BYTES);
-              g2::tma2_load_3d(sa, &tmapA, bar, k0, m0, 2 * z + h);
+              g2::tma2_load_3d(sa, &tmapA, bar, k0, m0, za + h);
               if constexpr (!B_MN) {
-                g2::tma2_load_3d(sb, &tmapB, bar, k0, n0, 2 * z + 1 - h);
+                g2::tma2_load_3d(sb, &tmapB, bar, k0, n0, zb + 1 - h);
               } else {
 #pragma unroll
-                for (int c = 0; c < BNC / 64; ++c) g2::tma2_load_3d(sb + c * (BK * 128), &tmapB, bar, n0 + c * 64, k0, 2 * z + 1 - h);
+                for (int c = 0; c < BNC / 64; ++c) g2::tma2_load_3d(sb + c * (BK * 128), &tmapB, bar, n0 + c * 64, k0, zb + 1 - h);
               }
             } else {
               mbar_expect_tx(&full_bar[s], HALF_BYTES);
-              tma_load_3d(sa, &tmapA, &full_bar[s], k0, m0, 2 * z + h);
+              tma_load_3d(sa, &tmapA, &full_bar[s], k0, m0, za + h);
               if constexpr (!B_MN) {
 #pragma unroll
                 for (int c = 0; c < BNC / 128; ++c)
-                  tma_load_3d(sb + c * A_BYTES, &tmapB, &full_bar[s], k0, n0 + c * 128, 2 * z + 1 - h);
+                  tma_load_3d(sb + c * A_BYTES, &tmapB, &full_bar[s], k0, n0 + c * 128, zb + 1 - h);
               } else {
 #pragma unroll
-                for (int c = 0; c < BNC / 64; ++c) tma_load_3d(sb + c * (BK * 128), &tmapB, &full_bar[s], n0 + c * 64, k0, 2 * z + 1 - h);
+                for (int c = 0; c < BNC / 64; ++c) tma_load_3d(sb + c * (BK * 128), &tmapB, &full_bar[s], n0 + c * 64, k0, zb + 1 - h);
               }
             }
           }
@@ -548,7 +578,7 @@ ns_product_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_consta
       for (int h = 0; h < CHUNKS; ++h)
 #pragma unroll
         for (int j = 0; j < 32; ++j) v[h][j] = 0.f;
-      uint4 in[8];
+      float4 in[8];
       if constexpr (KIND != SPLIT)
         for (int h = 0; h < CHUNKS; ++h) epi.prefetch(z, row0, col0 + h * 32);
       for (int kb = kb0; kb < kb1; kb += DRAIN, ++drains) {
@@ -587,7 +617,7 @@ ns_product_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_consta
         __syncwarp();
         if constexpr (KIND != SPLIT) {
           float4 acc[8];
-          uint4 now[8];
+          float4 now[8];
 #pragma unroll
           for (int i = 0; i < 8; ++i) { acc[i] = *reinterpret_cast<const float4*>(slab + chunk_at(4 * i + (lane >> 3), lane & 7)); now[i] = in[i]; }
           if (h + 1 < CHUNKS) epi.fetch(in, z, row0, col0 + (h + 1) * 32);
@@ -607,7 +637,7 @@ ns_product_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_consta
           __syncwarp();
           const int w = c / CHUNKS;                      // the warp whose chunk this was, and where its rows and columns are
           const int row0 = mi * BM + (w & 3) * 32, col0 = ni * BN + (w >> 2) * (BN / 2) + (c % CHUNKS) * 32;
-          uint4 in[8];
+          float4 in[8];
           epi.fetch(in, z, row0, col0);
           float4 sum[8];
 #pragma unroll
@@ -836,7 +866,7 @@ static int max_clusters(int size) {
   cudaGetDevice(&dev);
   int& n = known[dev & 63][size == 2 ? 1 : size == 4 ? 2 : 3];
   if (n == 0) {
-    auto kern = ns_product_kernel<GRAM, 128, SPLIT>;
+    auto kern = ns_product_kernel<SYM, 128, SPLIT>;
     static unsigned long long configured = 0;
     if (smem_opt_in(kern, SMEM_TOTAL, configured)) return 1;
     cudaLaunchConfig_t cfg = {};
@@ -853,8 +883,7 @@ static int max_clusters(int size) {
 
 template <int MODE>
 static int product(const CUtensorMap& ta, const CUtensorMap& tb, Params p, cudaStream_t st) {
-  constexpr bool SYM = MODE == GRAM || MODE == SQUARE;
-  const long long sms = sm_count(), kblocks = ((MODE == GRAM ? p.n : p.m) + BK - 1) / BK;
+  const long long sms = sm_count(), kblocks = (p.k + BK - 1) / BK, matrices = (long long)p.batch * p.problems;
   // Tiles of 128 x 128 or 128 x 256, whole or shared by the CTAs of a cluster, or of 256 x 256 on pairs: whatever has the
   // fewest clocks on its longest CTA.  A block of the contraction takes 1080 clocks with 128 columns and 1700 with 256,
   // bound by shared memory (213 and 160 bytes a clock at the full tensor rate, of 128), or 2100 where all SMs together
@@ -867,13 +896,13 @@ static int product(const CUtensorMap& ta, const CUtensorMap& tb, Params p, cudaS
     best = clocks; kind = k; bn = width; p.splits = splits; grid = ctas;
   };
   for (int width = 128; width <= 256; width += 128) {
-    const long long total = tiles_of(SYM, p.m, p.n, BM, width) * p.batch, waves = (total + sms - 1) / sms;
+    const long long total = tiles_of(MODE == SYM, p.m, p.n, BM, width) * matrices, waves = (total + sms - 1) / sms;
     const long long block = width == 128 ? 1080 : total >= sms ? 2100 : 1700, ends = width == 128 ? 6000 : 8000;
     offer(waves * kblocks * block + ends, WHOLE, width, 1, total < sms ? total : sms);
     for (int s = 2; s <= 8 && kblocks >= 2 * s && total <= max_clusters(s); s *= 2)      // (one tile each: a single wave)
       offer((kblocks + s - 1) / s * (width == 128 ? 1080 : 1700) + ends + 4000, SPLIT, width, s, total * s);
   }
-  const long long pairs = tiles_of(SYM, p.m, p.n, 2 * BM, 256) * p.batch, at_once = max_clusters(2);
+  const long long pairs = tiles_of(MODE == SYM, p.m, p.n, 2 * BM, 256) * matrices, at_once = max_clusters(2);
   offer((pairs + at_once - 1) / at_once * kblocks * 1600 + 10000, PAIR, 256, 1, 2 * (pairs < at_once ? pairs : at_once));
   const int g = (int)grid;
   if (kind == PAIR) return launch<MODE, 256, PAIR>(ta, tb, p, g, st);
@@ -884,7 +913,7 @@ static int product(const CUtensorMap& ta, const CUtensorMap& tb, Params p, cudaS
 static inline long long up256(long long b) { return (b + 255) & ~255ll; }
 
 struct Workspace {
-  double* partial; float* y; float* x; __half* xp[2]; __half* a; __half* b;
+  double* partial; float* y; float* x; __half* xp[2]; __half* terms; float* whole;
   long long bytes;
   Workspace(uint8_t* base, long long m, long long n, long long batch, bool with_y) {
     const long long ldx = (n + 7) & ~7ll, lda = (m + 7) & ~7ll;
@@ -895,8 +924,8 @@ struct Workspace {
     x = (float*)take(batch * m * ldx * 4);
     xp[0] = (__half*)take(batch * m * ldx * 4);
     xp[1] = (__half*)take(batch * m * ldx * 4);
-    a = (__half*)take(batch * m * lda * 4);
-    b = (__half*)take(batch * m * lda * 4);
+    terms = (__half*)take(SLOTS * batch * m * lda * 4);
+    whole = (float*)take(SLOTS * batch * m * lda * 4);
     bytes = at;
   }
 };
@@ -927,13 +956,15 @@ extern "C" int gb_muon_momentum(const long long* table, int batch, int grad_dt, 
 // Orthogonalises `batch` matrices [m, n], or [n, m] (tall), m <= n.  `src` (contiguous, dtype dt) with `out` of the same type;
 // or src null for the updates that gb_muon_momentum has left in the workspace, which go into the weights whose addresses
 // `weights` [batch] holds (+ 1 for a tall one).
-// exponents [3 steps]: powers of two by which X, A and B of each step are scaled in fp16 (host: from the coefficients).
-extern "C" int gb_newton_schulz(const void* src, void* out, int dt, int m, int n, int tall, int batch, int steps, float a,
-                                float b, float c, double eps, const int* exponents, const long long* weights, float lr,
-                                float decay, float scale, const float* dyn_lr, const float* found_inf, void* workspace,
-                                int* status, cudaStream_t st) {
+// The products to be made are `count` rows of 12 numbers in `program`: kind (0 X X^T, 1 symmetric, 2 the same and to be
+// launched together with the next row, 3 X <- Q X + ..), left, right and out slots, M1 and M2 slots or -1, whether the result
+// is kept in 32 bits, f_acc, f1, f2, the power of two of the result's terms, 0.  The first row's last number: the power of
+// two of the first X's terms.  The last row is of kind 3.
+extern "C" int gb_newton_schulz(const void* src, void* out, int dt, int m, int n, int tall, int batch, const double* program,
+                                int count, double eps, const long long* weights, float lr, float decay, float tall_scale,
+                                const float* dyn_lr, const float* found_inf, void* workspace, int* status, cudaStream_t st) {
   if (batch <= 0 || m <= 0 || n <= 0) return 0;
-  if (batch > 32767 || m > n || steps < 1 || (src == nullptr) != (weights != nullptr) ||
+  if (batch > 6000 || m > n || count < 2 || (src == nullptr) != (weights != nullptr) ||
       (reinterpret_cast<uintptr_t>(workspace) & 255) != 0) return -3;
   const int ldx = (n + 7) & ~7, lda = (m + 7) & ~7;
   const ns::Workspace w((uint8_t*)workspace, m, n, batch, src == nullptr);
@@ -949,29 +980,42 @@ extern "C" int gb_newton_schulz(const void* src, void* out, int dt, int m, int n
   const void* g = src != nullptr ? src : (const void*)w.y;
   const int g_dt = src != nullptr ? dt : (int)DT_F32;
   if (const cudaError_t e = cudaLaunchKernelEx(&cfg, ns::ns_prepare_kernel, g, g_dt, m, n, tall, weights, (const double*)w.partial,
-                                               parts, eps, ldexpf(1.f, exponents[0]), w.x, w.xp[0], ldx)) return (int)e;
-  // maps: X as left or right operand of X X^T, X as right operand of B X (64 rows of the contraction at a time), A, B
-  CUtensorMap mx[2], mxr[2], ma, mb;
+                                               parts, eps, (float)program[11], w.x, w.xp[0], ldx)) return (int)e;
+  // maps: X as left or right operand of X X^T, X as right operand of Q X (64 rows of the contraction at a time), the slots
+  CUtensorMap mx[2], mxr[2], ms;
   int r;
   for (int i = 0; i < 2; ++i) {
     if ((r = make_tmap_3d(&mx[i], w.xp[i], DT_F16, n, m, 2ll * batch, ldx, (long long)m * ldx, 128)) != 0) return 10000 + r;
     if ((r = make_tmap_3d(&mxr[i], w.xp[i], DT_F16, n, m, 2ll * batch, ldx, (long long)m * ldx, 64)) != 0) return 20000 + r;
   }
-  if ((r = make_tmap_3d(&ma, w.a, DT_F16, m, m, 2ll * batch, lda, (long long)m * lda, 128)) != 0) return 30000 + r;
-  if ((r = make_tmap_3d(&mb, w.b, DT_F16, m, m, 2ll * batch, lda, (long long)m * lda, 128)) != 0) return 40000 + r;
+  if ((r = make_tmap_3d(&ms, w.terms, DT_F16, m, m, 2ll * batch * ns::SLOTS, lda, (long long)m * lda, 128)) != 0) return 30000 + r;
   ns::Params p = {};
-  p.status = status; p.m = m; p.n = n; p.batch = batch; p.ldx = ldx; p.lda = lda; p.x = w.x; p.a_planes = w.a;
-  p.out = out; p.out_dtype = dt; p.tall = tall; p.weights = weights; p.lr = lr; p.decay = decay; p.scale = scale;
+  p.status = status; p.m = m; p.n = n; p.batch = batch; p.ldx = ldx; p.lda = lda; p.x = w.x; p.terms = w.terms; p.whole = w.whole;
+  p.out = out; p.out_dtype = dt; p.tall = tall; p.weights = weights; p.lr = lr; p.decay = decay; p.tall_scale = tall_scale;
   p.dyn_lr = dyn_lr; p.found_inf = found_inf;
-  for (int k = 0; k < steps; ++k) {
-    const int sx = exponents[3 * k], sa = exponents[3 * k + 1], sb = exponents[3 * k + 2], cur = k & 1;
-    p.dst = w.a; p.f_acc = ldexpf(1.f, sa - 2 * sx); p.f_a = 0.f;
-    if ((r = ns::product<ns::GRAM>(mx[cur], mx[cur], p, st)) != 0) return r;
-    p.dst = w.b; p.f_acc = ldexpf(c, sb - 2 * sa); p.f_a = ldexpf(b, sb - sa);
-    if ((r = ns::product<ns::SQUARE>(ma, ma, p, st)) != 0) return r;
-    p.dst = w.xp[cur ^ 1]; p.f_acc = ldexpf(1.f, -sb - sx); p.f_a = a;
-    p.next_scale = k + 1 < steps ? ldexpf(1.f, exponents[3 * k + 3]) : 1.f;
-    r = k + 1 < steps ? ns::product<ns::APPLY>(mb, mxr[cur], p, st) : ns::product<ns::APPLY_LAST>(mb, mxr[cur], p, st);
+  int cur = 0;
+  for (int i = 0; i < count; ++i) {
+    int kind = (int)program[12 * i];
+    p.problems = kind == 2 && i + 1 < count ? 2 : 1;
+    for (int j = 0; j < p.problems; ++j) {
+      const double* o = program + 12 * (i + j);
+      for (int k = 1; k <= 5; ++k)
+        if (!(o[k] >= (k > 3 ? -1 : 0) && o[k] < ns::SLOTS)) return -3;
+      p.prob[j] = ns::Problem{(int)o[1], (int)o[2], (int)o[3], (int)o[4], (int)o[5], (int)o[6], (float)o[7], (float)o[8], (float)o[9],
+                              (float)o[10]};
+    }
+    i += p.problems - 1;
+    if (kind == 3) {
+      p.k = m;
+      p.prob[0].right = 0;
+      p.dst = w.xp[cur ^ 1];
+      r = i + 1 < count ? ns::product<ns::APPLY>(ms, mxr[cur], p, st) : ns::product<ns::APPLY_LAST>(ms, mxr[cur], p, st);
+      cur ^= 1;
+    } else {
+      p.k = kind == 0 ? n : m;
+      if (kind == 0) p.prob[0].left = p.prob[0].right = 0;
+      r = kind == 0 ? ns::product<ns::SYM>(mx[cur], mx[cur], p, st) : ns::product<ns::SYM>(ms, ms, p, st);
+    }
     if (r != 0) return r;
   }
   return 0;

@@ -1021,24 +1021,24 @@ def _newton_schulz_torch(x, steps, coefficients, eps):
     return y.transpose(-2, -1) if tall else y
 
 
-def newton_schulz(x, steps, coefficients, eps, exponents):
+def newton_schulz(x, steps, coefficients, eps, program):
     """Orthogonalised matrices of x [batch, rows, cols], in its type."""
     if x.is_cuda:
-        r = N.newton_schulz(contiguous(x), steps, coefficients, eps, exponents)
+        r = N.newton_schulz(contiguous(x), steps, coefficients, eps, program)
         if r is not NotImplemented:
             return r
         _fell("newton_schulz")
     return _newton_schulz_torch(x, steps, coefficients, eps).to(x.dtype).contiguous()
 
 
-def muon_step(params, grads, bufs, shape, lr, momentum, nesterov, weight_decay, scale, steps, coefficients, eps, exponents,
+def muon_step(params, grads, bufs, shape, lr, momentum, nesterov, weight_decay, scale, steps, coefficients, eps, program,
               grad_scale=None, found_inf=None, dyn_lr=None):
     """One Muon step, in place, on matrices of `shape` = (m, n), m <= n, and (n, m), whose update is scaled by `scale`;
     params / grads / bufs are lists of (tensor, index of the matrix in the tensor's leading dimensions).  `grad_scale`,
     `found_inf`: as in `adamw_step`."""
     if params[0][0].is_cuda:
         r = N.muon_step(params, grads, bufs, shape, lr, momentum, nesterov, weight_decay, scale, steps, coefficients, eps,
-                        exponents, grad_scale, found_inf, dyn_lr)
+                        program, grad_scale, found_inf, dyn_lr)
         if r is not NotImplemented:
             return
         _fell("muon_step")

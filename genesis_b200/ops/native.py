@@ -73,7 +73,7 @@ _SIGS = {
     "gb_preference_loss": "pppp" + "lllll" + "l" + "p" + "l" + "ff" + "i" + "pppp" + "ii" + "pp",
     "gb_token_grad": "pppp" + "lllll" + "l" + "f" + "pl" + "pll" + "p" + "f" + "ii" + "p",
     "gb_ns_workspace": "lllip", "gb_muon_momentum": "p" + "iiii" + "f" + "i" + "ppp" + "p",
-    "gb_newton_schulz": "pp" + "iiiiii" + "fff" + "d" + "pp" + "fff" + "pp" + "pp" + "p",
+    "gb_newton_schulz": "pp" + "iiiii" + "p" + "i" + "d" + "p" + "fff" + "pp" + "pp" + "p",
 }
 
 _L = None
@@ -1985,11 +1985,11 @@ def _ns_workspace(m, n, batch, with_y, dev):
 
 
 def _ns_batch(m, n):
-    """Matrices of one pass: the workspace holds 16 bytes per element of them, some GB are enough to fill the GPU."""
-    return max(1, min(4096, (1 << 28) // (m * n)))
+    """Matrices of one pass: the workspace holds 12 bytes per element of them and 40 per element of m x m; some GB fill the GPU."""
+    return max(1, min(4096, (1 << 32) // (12 * m * n + 40 * m * m)))
 
 
-def newton_schulz(x, steps, coefficients, eps, exponents):
+def newton_schulz(x, steps, coefficients, eps, program):
     """Orthogonalised matrices of contiguous x [batch, rows, cols], in its type."""
     if x.dtype not in _FLOATS or not x.is_contiguous():
         return NotImplemented
@@ -1997,18 +1997,17 @@ def newton_schulz(x, steps, coefficients, eps, exponents):
     batch, rows, cols = x.shape
     m, n = min(rows, cols), max(rows, cols)
     per = _ns_batch(m, n)
-    ex = (ctypes.c_int * len(exponents))(*exponents)
     with _on(x.device):
         for i in range(0, batch, per):
             count = min(per, batch - i)
             ws = _ns_workspace(m, n, count, False, x.device)
             _chk(lib().gb_newton_schulz(x[i].data_ptr(), out[i].data_ptr(), _DT[x.dtype], m, n, 1 if rows > cols else 0, count,
-                                        steps, *coefficients, eps, ex, None, 0.0, 0.0, 0.0, None, None, ws.data_ptr(),
+                                        program, len(program) // 12, eps, None, 0.0, 0.0, 0.0, None, None, ws.data_ptr(),
                                         status_tensor(x.device).data_ptr(), _st()), "newton_schulz")
     return out
 
 
-def muon_step(params, grads, bufs, shape, lr, momentum, nesterov, weight_decay, scale, steps, coefficients, eps, exponents,
+def muon_step(params, grads, bufs, shape, lr, momentum, nesterov, weight_decay, scale, steps, coefficients, eps, program,
               grad_scale, found_inf, dyn_lr):
     """One step on matrices of shape (m, n) or (n, m), m <= n.  params / grads / bufs: lists of (tensor, index of the
     matrix in it)."""
@@ -2021,7 +2020,6 @@ def muon_step(params, grads, bufs, shape, lr, momentum, nesterov, weight_decay, 
         return NotImplemented
     dev = params[0][0].device
     per = _ns_batch(m, n)
-    ex = (ctypes.c_int * len(exponents))(*exponents)
 
     def at(pair):
         return pair[0].data_ptr() + pair[1] * m * n * pair[0].element_size()
@@ -2034,7 +2032,7 @@ def muon_step(params, grads, bufs, shape, lr, momentum, nesterov, weight_decay, 
             ws = _ns_workspace(m, n, count, True, dev)
             _chk(lib().gb_muon_momentum(table.data_ptr(), count, _DT[gdt], m, n, float(momentum), 1 if nesterov else 0,
                                         _ptr(grad_scale), _ptr(found_inf), ws.data_ptr(), _st()), "muon_momentum")
-            _chk(lib().gb_newton_schulz(None, None, 0, m, n, 0, count, steps, *coefficients, eps, ex,
+            _chk(lib().gb_newton_schulz(None, None, 0, m, n, 0, count, program, len(program) // 12, eps,
                                         table.data_ptr() + 16 * count, float(lr), float(weight_decay), float(scale),
                                         _ptr(dyn_lr), _ptr(found_inf), ws.data_ptr(), status_tensor(dev).data_ptr(), _st()),
                  "newton_schulz")

@@ -6,6 +6,7 @@
 The orthogonalisation (`csrc/newton_schulz.cu`) works on all matrices of one shape, and its transpose, at once.  Vectors, embeddings and
 output heads are left to AdamW: `Muon` takes tensors of two and more dimensions, whose last two are the matrix.
 """
+import ctypes
 import functools
 import math
 
@@ -19,21 +20,67 @@ from .optimizer import Optimizer
 COEFFICIENTS = (3.4445, -4.7750, 2.0315)
 
 
+# slots of m x m matrices in the kernels' workspace
+_A, _W, _B, _Q = 0, 1, 2, (3, 4)
+
+
 @functools.lru_cache(maxsize=64)
-def _exponents(steps, coefficients):
-    """Powers of two [3 steps] by which X, A = X X^T and B = b A + c A A of every step are scaled before they are rounded to
-    fp16 terms: the largest that keep their entries, which no singular value exceeds, below a quarter of fp16's range."""
+def _program(steps, coefficients):
+    """The products that `gb_newton_schulz` makes, as an array of 12 numbers each (see there and the head of
+    `csrc/newton_schulz.cu`).
+
+    Steps go in blocks of three, or two, between which X is formed anew.  Every matrix is a polynomial in X X^T, so its
+    eigenvalues are followed over all singular values that X may have; the power of two by which its terms are scaled in
+    fp16 is the largest that keeps its entries, which no eigenvalue exceeds, below a quarter of fp16's range."""
     a, b, c = coefficients
-    out, top = [], 1.001
-    for _ in range(steps):
-        s = torch.linspace(0.0, top, 4097, dtype=torch.float64)
-        second = float((b * s ** 2 + c * s ** 4).abs().max())
-        out += [math.floor(math.log2(16384.0 / max(x, 2.0 ** -10))) for x in (top, top * top, second)]
-        top = 1.001 * float((a * s + b * s ** 3 + c * s ** 5).abs().max())
-        if not top < 64.0 or second > 4096.0:
+    rows, top, left = [], 1.001, steps
+
+    def scale(values):
+        peak = float(values.abs().max())
+        if not peak < 4096.0:
             raise ValueError(f"coefficients {coefficients} let singular values grow without bound")
-        top = max(top, 2.0 ** -10)
-    return tuple(out)
+        return 2.0 ** math.floor(math.log2(16384.0 / max(peak, 2.0 ** -10)))
+
+    def row(kind, lhs, rhs, out, f_acc, out_scale, m1=-1, f1=0.0, m2=-1, f2=0.0, keep=True):
+        rows.append([kind, lhs, rhs, out, m1, m2, float(keep), f_acc, f1, f2, out_scale, 0.0])
+
+    while left:
+        block = left if left < 4 else 2 if left == 4 else 3
+        left -= block
+        s = torch.linspace(0.0, top, 4097, dtype=torch.float64)
+        x_scale = scale(s)
+        lam = s * s
+        total = torch.ones_like(s)                       # product of the P's: identity * ident + Q
+        scales, ident, q, old_q = {_A: scale(lam)}, 1.0, _Q[0], None
+        if rows:
+            rows[-1][10] = x_scale                       # the X that the block before has left
+        else:
+            first = x_scale
+        row(0, 0, 0, _A, x_scale ** -2, scales[_A])
+        for k in range(block):
+            B = b * lam + c * lam * lam
+            slot = q if k == 0 else _B
+            scales[slot] = scale(B)
+            row(1, _A, _A, slot, c / scales[_A] ** 2, scales[slot], _A, b)
+            last = k + 1 == block
+            if not last:
+                scales[_W] = scale((a + B) * lam)
+                row(2 if k else 1, slot, _A, _W, 1.0 / (scales[slot] * scales[_A]), scales[_W], _A, a)
+            new = total * (a + B)
+            if k:
+                old_q, q = q, _Q[1 - _Q.index(q)]
+                scales[q] = scale(new - ident * a)
+                row(1, _B, old_q, q, 1.0 / (scales[_B] * scales[old_q]), scales[q], old_q, a, _B, ident)
+            total, ident = new, ident * a
+            if not last:
+                lam = lam * (a + B) ** 2
+                scales[_A] = scale(lam)
+                row(1, slot, _W, _A, 1.0 / (scales[slot] * scales[_W]), scales[_A], _W, a)
+        row(3, q, 0, 0, 1.0 / (scales[q] * x_scale), 1.0, f1=ident)
+        top = max(1.001 * float((s * total).abs().max()), 2.0 ** -10)
+    rows[0][11] = first
+    flat = [x for r in rows for x in r]
+    return (ctypes.c_double * len(flat))(*flat)
 
 
 def _check(steps, coefficients, eps):
@@ -44,7 +91,7 @@ def _check(steps, coefficients, eps):
         raise ValueError(f"coefficients must be three finite numbers, got {coefficients}")
     if not 1e-30 <= float(eps) < math.inf:
         raise ValueError(f"eps must be finite and at least 1e-30, got {eps}")
-    return coefficients, float(eps), _exponents(steps, coefficients)
+    return coefficients, float(eps), _program(steps, coefficients)
 
 
 def orthogonalize(x, steps=5, coefficients=COEFFICIENTS, eps=1e-7):
@@ -59,11 +106,11 @@ def orthogonalize(x, steps=5, coefficients=COEFFICIENTS, eps=1e-7):
         raise ValueError(f"orthogonalize: x must have two dimensions or more, got shape {tuple(x.shape)}")
     if x.requires_grad and grad_mode.is_grad_enabled():
         raise ValueError("orthogonalize is not differentiable: pass a detached Tensor, or call it under no_grad()")
-    coefficients, eps, exponents = _check(steps, coefficients, eps)
+    coefficients, eps, program = _check(steps, coefficients, eps)
     t = x._t
     if t.numel() == 0:
         return Tensor._wrap(torch.empty_like(t))
-    out = K.newton_schulz(t.reshape(-1, *t.shape[-2:]), steps, coefficients, eps, exponents)
+    out = K.newton_schulz(t.reshape(-1, *t.shape[-2:]), steps, coefficients, eps, program)
     return Tensor._wrap(out.reshape(t.shape))
 
 
@@ -123,7 +170,7 @@ class Muon(Optimizer):
         self.t += 1
         if self._dyn_lr_t is not None and not torch.cuda.is_current_stream_capturing():
             self._sync_lr()
-        exponents = _exponents(self.steps, self.coefficients)
+        program = _program(self.steps, self.coefficients)
         groups = {}
         for i in idx:
             p, g = self.params[i]._t, self.params[i].grad._t
@@ -138,6 +185,6 @@ class Muon(Optimizer):
         for (shape, _, _), members in groups.items():
             ps, gs, us = (list(x) for x in zip(*members))
             K.muon_step(ps, gs, us, shape, self.lr, self.momentum, self.nesterov, self.weight_decay,
-                        math.sqrt(shape[1] / shape[0]), self.steps, self.coefficients, self.eps, exponents,
+                        math.sqrt(shape[1] / shape[0]), self.steps, self.coefficients, self.eps, program,
                         self._grad_scale, self._found_inf, self._dyn_lr_t)
         self._touched(idx)

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import genesis_b200 as genesis
-from genesis_b200.optim.muon import COEFFICIENTS, _exponents
+from genesis_b200.optim.muon import COEFFICIENTS, _program
 
 T = genesis.Tensor
 
@@ -71,17 +71,50 @@ def test_refusals():
             call()
 
 
-def test_exponents_keep_entries_in_range():
-    """The scaled entries of X, A, B stay below fp16's largest number for every singular value in reach."""
-    for co in [COEFFICIENTS, (1.5, -0.5, 0.0), (15 / 8, -10 / 8, 3 / 8), (2.0, -1.5, 0.5)]:
-        a, b, c = co
-        s = torch.linspace(0, 1, 100001, dtype=torch.float64)
-        for k in range(6):
-            sx, sa, sb = _exponents(6, co)[3 * k:3 * k + 3]
-            second = b * s ** 2 + c * s ** 4
-            assert float(s.abs().max()) * 2.0 ** sx < 32768
-            assert float(s.max()) ** 2 * 2.0 ** sa < 32768 and float(second.abs().max()) * 2.0 ** sb < 32768
-            s = (a * s + b * s ** 3 + c * s ** 5).abs()
+@pytest.mark.parametrize("steps", [1, 2, 3, 4, 5, 7, 8])
+@pytest.mark.parametrize("coefficients", [COEFFICIENTS, (1.5, -0.5, 0.0), (15 / 8, -10 / 8, 3 / 8), (2.0, -1.5, 0.5)])
+def test_program_of_products(steps, coefficients):
+    """The products that the kernels are told to make, carried out on the eigenvalues of X X^T in 64 bits: they give the
+    iteration, and every scaled entry stays inside fp16's range."""
+    rows = [list(_program(steps, coefficients)[i:i + 12]) for i in range(0, len(_program(steps, coefficients)), 12)]
+    a, b, c = coefficients
+    s = torch.linspace(0, 1, 20001, dtype=torch.float64)
+    want = s.clone()
+    for _ in range(steps):
+        want = a * want + b * want ** 3 + c * want ** 5
+    x, x_scale, slots, kept = s.clone(), rows[0][11], {}, set()
+
+    def fits(v, scale):
+        assert math.log2(scale) == int(math.log2(scale)) and float(v.abs().max()) * scale < 32768
+        return scale
+
+    fits(x, x_scale)
+    assert rows[-1][0] == 3 and rows[0][0] == 0
+    i = 0
+    while i < len(rows):
+        results = []
+        for kind, lhs, rhs, out, m1, m2, keep, f_acc, f1, f2, scale, _ in rows[i:i + (2 if rows[i][0] == 2 else 1)]:
+            if kind == 0:
+                results.append((out, f_acc * (x * x_scale) ** 2, scale, keep))
+            elif kind == 3:
+                q, qs = slots[lhs]
+                x = f_acc * (q * qs) * (x * x_scale) + f1 * x
+                x_scale = fits(x, scale) if i + 1 < len(rows) else 1.0
+            else:
+                (l, ls), (r, rs) = slots[lhs], slots[rhs]
+                v = f_acc * (l * ls) * (r * rs)
+                for m, f in ((m1, f1), (m2, f2)):
+                    if m >= 0:
+                        assert m in kept
+                        v = v + f * slots[m][0]
+                results.append((out, v, scale, keep))
+                # a launch reads its operands while it writes its results
+                assert out not in (lhs, rhs, m2) and out not in [o[2] for o in rows[i:i + (2 if rows[i][0] == 2 else 1)] if o is not rows[i]]
+        for out, v, scale, keep in results:
+            slots[out] = (v, fits(v, scale))
+            (kept.add if keep else kept.discard)(out)
+        i += 2 if rows[i][0] == 2 else 1
+    assert float((x - want).abs().max()) < 1e-12
 
 
 def _manual(ps, gs, us, lr, mu, decay, nesterov):
