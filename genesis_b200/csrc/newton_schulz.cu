@@ -668,6 +668,218 @@ ns_product_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_consta
   }
 }
 
+// A block's products of m x m matrices for m <= 128 in one launch: one CTA per matrix, all matrices in its shared memory.
+// Launched one by one they take 8 us each, of which the products are one; here 2 us (128 x 896: 148 -> ... us).
+// Three slots hold terms, [two halves of the columns][hi, lo][128 rows of 128 bytes], swizzled as the tensor cores read
+// them: R (A, then W in its place, then the next A), B and Q; a result is written where the operand that it replaces has
+// been read from.  A thread keeps half a row of A or W in 32 bits in registers.  Rows and columns past m are zero throughout.
+constexpr int CHAIN_THREADS = 256;
+constexpr int CHAIN_SLOT = 4 * 128 * 128;
+constexpr int CHAIN_BARRIERS = 3 * CHAIN_SLOT;
+constexpr int CHAIN_SMEM = CHAIN_BARRIERS + 64;
+
+struct ChainStep {
+  float sq_acc, sq_a;          // B = sq_acc A A + sq_a A, 2^k of its terms
+  float sq_scale;
+  float w_acc, w_a, w_scale;   // W = w_acc B A + w_a A
+  float a_acc, a_w, a_scale;   // A <- a_acc B W + a_w W
+  float q_acc, q_q, q_b, q_scale;      // Q <- q_acc B Q + q_q Q + q_b B
+};
+struct Chain {
+  int* status;
+  int m, batch, lda, steps;    // up to 3
+  const float* a;              // A in 32 bits (slot 0)
+  __half* q;                   // terms of Q [batch][hi, lo][m][lda]
+  ChainStep step[3];
+};
+
+__global__ void __launch_bounds__(CHAIN_THREADS, 1)
+ns_chain_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_constant__ Chain p) {
+  extern __shared__ __align__(1024) uint8_t smem[];
+  uint64_t* loaded = reinterpret_cast<uint64_t*>(smem + CHAIN_BARRIERS);
+  uint64_t* done = loaded + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const int z = blockIdx.x;
+  if (threadIdx.x == 0) {
+    mbar_init(loaded, 1);
+    mbar_init(done, 1);
+    const bool aligned = (smem_u32(smem) & 1023) == 0;
+    if (!aligned) report_error(p.status, GB_ERR_BAD_ARG, 6, 0);
+    *abort_flag = !aligned || status_poisoned(p.status) ? 1 : 0;
+    mbar_fence_init();
+    tma_prefetch_desc(&tmapA);
+  }
+  if (warp == 0) {
+    tmem_alloc(tmem_slot, 128);
+    tmem_relinquish();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = *tmem_slot;
+  const bool work = *abort_flag == 0;
+  let_next_start();
+  wait_for_previous();
+
+  const int row = (warp & 3) * 32 + lane, half = warp >> 2, col0 = half * 64;      // this thread's half row
+  float whole[64];
+  uint8_t* slot_r = smem;
+  uint8_t* slot_b = smem + CHAIN_SLOT;
+  uint8_t* slot_q = smem + 2 * CHAIN_SLOT;
+  if (work && threadIdx.x == 0) {
+    mbar_expect_tx(loaded, CHAIN_SLOT);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) tma_load_3d(slot_r + i * 16384, &tmapA, loaded, (i >> 1) * 64, 0, 2 * z + (i & 1));
+  }
+  {
+    const float* a = p.a + ((size_t)z * p.m + row) * p.lda + col0;
+#pragma unroll
+    for (int u = 0; u < 16; ++u) {
+      const float4 v = row < p.m && col0 + 4 * u < p.m ? *reinterpret_cast<const float4*>(a + 4 * u) : make_float4(0.f, 0.f, 0.f, 0.f);
+      // (elements of the last vector past m are padding, whatever it holds)
+      whole[4 * u] = v.x;
+      whole[4 * u + 1] = col0 + 4 * u + 1 < p.m ? v.y : 0.f;
+      whole[4 * u + 2] = col0 + 4 * u + 2 < p.m ? v.z : 0.f;
+      whole[4 * u + 3] = col0 + 4 * u + 3 < p.m ? v.w : 0.f;
+    }
+  }
+  const uint32_t idesc = make_idesc(0u, 0u, 0u, 128, 128);
+  uint32_t phase = 0;
+  bool ok = work;
+  // accumulator = L R; every thread waits for it
+  auto multiply = [&](const uint8_t* left, const uint8_t* right) {
+    fence_proxy_async_smem();
+    tc_fence_before_sync();
+    __syncthreads();                                     // operands written, the last accumulator read
+    tc_fence_after_sync();
+    if (warp == 0 && ok) {
+      const uint64_t l = make_smem_desc(smem_u32(left), 16, 1024), r = make_smem_desc(smem_u32(right), 16, 1024);
+      if (elect_one()) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const uint64_t at = (uint64_t)((k >> 2) * 2048 + (k & 3) * 2);      // (16-byte units; 32 KB a half)
+          constexpr uint64_t LO = 1024;
+          umma_f16(tmem, l + at, r + at + LO, idesc, k == 0 ? 0u : 1u);
+          umma_f16(tmem, l + at + LO, r + at, idesc, 1u);
+          umma_f16(tmem, l + at, r + at, idesc, 1u);
+        }
+        umma_commit(done);
+      }
+      __syncwarp();
+    }
+    if (ok) ok = mbar_wait(done, phase, abort_flag, p.status, 410);
+    ok = __syncthreads_and(ok);
+    phase ^= 1;
+    tc_fence_after_sync();
+  };
+  // the thread's 32 columns 32 h .. of the accumulator
+  auto take = [&](int h, uint32_t (&r)[32]) {
+    tmem_ld_32x32b_x32(tmem + ((uint32_t)((warp & 3) * 32) << 16) + col0 + 32 * h, r);
+    tmem_ld_wait();
+  };
+  // unit u (8 columns) of the thread's half row in a slot: hi, and lo 16 KB on
+  auto unit = [&](uint8_t* slot, int u) { return slot + half * 32768 + row * 128 + ((u ^ (row & 7)) << 4); };
+  auto put = [&](uint8_t* slot, int u, const float (&v)[8], float scale) {
+    const uint4 s = split4(v[0] * scale, v[1] * scale, v[2] * scale, v[3] * scale), t = split4(v[4] * scale, v[5] * scale, v[6] * scale, v[7] * scale);
+    uint8_t* at = unit(slot, u);
+    *reinterpret_cast<uint4*>(at) = make_uint4(s.x, s.y, t.x, t.y);
+    *reinterpret_cast<uint4*>(at + 16384) = make_uint4(s.z, s.w, t.z, t.w);
+  };
+  auto get = [&](uint8_t* slot, int u, float (&v)[8], float factor) {
+    const uint8_t* at = unit(slot, u);
+    const uint4 hi = *reinterpret_cast<const uint4*>(at), lo = *reinterpret_cast<const uint4*>(at + 16384);
+    const uint32_t h[4] = {hi.x, hi.y, hi.z, hi.w}, l[4] = {lo.x, lo.y, lo.z, lo.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&h[k])), b = __half22float2(*reinterpret_cast<const __half2*>(&l[k]));
+      v[2 * k] = (a.x + b.x) * factor;
+      v[2 * k + 1] = (a.y + b.y) * factor;
+    }
+  };
+  if (ok) ok = mbar_wait(loaded, 0, abort_flag, p.status, 411);
+  ok = __syncthreads_and(ok);
+  float q_unscale = 1.f;                                 // 1 / 2^k of Q's terms
+  for (int s = 0; s < p.steps; ++s) {
+    const ChainStep& c = p.step[s];
+    uint8_t* into = s == 0 ? slot_q : slot_b;            // the first B is Q
+    multiply(slot_r, slot_r);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      uint32_t r[32];
+      take(h, r);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        float v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = fmaf(__uint_as_float(r[8 * u + k]), c.sq_acc, whole[32 * h + 8 * u + k] * c.sq_a);
+        put(into, 4 * h + u, v, c.sq_scale);
+      }
+    }
+    if (s > 0) {
+      multiply(slot_b, slot_q);
+      const float b_unscale = 1.f / c.sq_scale;          // (powers of two)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t r[32];
+        take(h, r);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          float q[8], b[8];
+          get(slot_q, 4 * h + u, q, q_unscale * c.q_q);
+          get(slot_b, 4 * h + u, b, b_unscale * c.q_b);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) q[k] = fmaf(__uint_as_float(r[8 * u + k]), c.q_acc, q[k]) + b[k];
+          put(slot_q, 4 * h + u, q, c.q_scale);
+        }
+      }
+      q_unscale = 1.f / c.q_scale;
+    } else {
+      q_unscale = 1.f / c.sq_scale;
+    }
+    if (s + 1 == p.steps) break;
+    uint8_t* left = s == 0 ? slot_q : slot_b;            // (B; the next step's products with Q come after its own B)
+#pragma unroll 1
+    for (int twice = 0; twice < 2; ++twice) {            // W in the place of A, then A in the place of W
+      const float acc = twice ? c.a_acc : c.w_acc, own = twice ? c.a_w : c.w_a, scale = twice ? c.a_scale : c.w_scale;
+      multiply(left, slot_r);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t r[32];
+        take(h, r);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          float v[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const int j = 32 * h + 8 * u + k;
+            whole[j] = v[k] = fmaf(__uint_as_float(r[8 * u + k]), acc, whole[j] * own);
+          }
+          put(slot_r, 4 * h + u, v, scale);
+        }
+      }
+    }
+  }
+  if (ok && row < p.m) {
+    __half* q = p.q + ((size_t)z * 2 * p.m + row) * p.lda + col0;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      if (col0 + 8 * u < p.m) {
+        const uint8_t* at = unit(slot_q, u);
+        *reinterpret_cast<uint4*>(q + 8 * u) = *reinterpret_cast<const uint4*>(at);
+        *reinterpret_cast<uint4*>(q + (size_t)p.m * p.lda + 8 * u) = *reinterpret_cast<const uint4*>(at + 16384);
+      }
+    }
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  if (warp == 0) {
+    tc_fence_after_sync();
+    tmem_dealloc(tmem, 128);
+  }
+}
+
 __device__ __forceinline__ double block_sum256(double v, double* sh) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -910,6 +1122,19 @@ static int product(const CUtensorMap& ta, const CUtensorMap& tb, Params p, cudaS
   return bn == 256 ? launch<MODE, 256, WHOLE>(ta, tb, p, g, st) : launch<MODE, 128, WHOLE>(ta, tb, p, g, st);
 }
 
+static int chain(const CUtensorMap& ta, const Chain& c, cudaStream_t st) {
+  static unsigned long long configured = 0;
+  if (int r = smem_opt_in(ns_chain_kernel, CHAIN_SMEM, configured)) return r;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = dim3((unsigned)c.batch); cfg.blockDim = dim3(CHAIN_THREADS); cfg.dynamicSmemBytes = CHAIN_SMEM; cfg.stream = st;
+  cfg.attrs = attr; cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, ns_chain_kernel, ta, c);
+  return e == cudaSuccess ? (int)cudaGetLastError() : (int)e;
+}
+
 static inline long long up256(long long b) { return (b + 255) & ~255ll; }
 
 struct Workspace {
@@ -995,7 +1220,7 @@ extern "C" int gb_newton_schulz(const void* src, void* out, int dt, int m, int n
   p.dyn_lr = dyn_lr; p.found_inf = found_inf;
   int cur = 0;
   for (int i = 0; i < count; ++i) {
-    int kind = (int)program[12 * i];
+    const int kind = (int)program[12 * i];
     p.problems = kind == 2 && i + 1 < count ? 2 : 1;
     for (int j = 0; j < p.problems; ++j) {
       const double* o = program + 12 * (i + j);
@@ -1017,6 +1242,30 @@ extern "C" int gb_newton_schulz(const void* src, void* out, int dt, int m, int n
       r = kind == 0 ? ns::product<ns::SYM>(mx[cur], mx[cur], p, st) : ns::product<ns::SYM>(ms, ms, p, st);
     }
     if (r != 0) return r;
+    if (kind == 0 && m <= 128) {
+      // the rows up to the next X at once; a row is told by its result and operands
+      ns::Chain c = {};
+      c.status = status; c.m = m; c.batch = batch; c.lda = lda; c.a = w.whole;
+      for (++i; i < count && program[12 * i] != 3.0; ++i) {
+        const double* o = program + 12 * i;
+        const int out_slot = (int)o[3];
+        if (o[1] == 0.0 && o[2] == 0.0) {
+          if (c.steps == 3) return -3;
+          ns::ChainStep& t = c.step[c.steps++];
+          t.sq_acc = (float)o[7]; t.sq_a = (float)o[8]; t.sq_scale = (float)o[10];
+        } else {
+          if (c.steps == 0) return -3;
+          ns::ChainStep& t = c.step[c.steps - 1];
+          if (out_slot == 1) { t.w_acc = (float)o[7]; t.w_a = (float)o[8]; t.w_scale = (float)o[10]; }
+          else if (out_slot == 0) { t.a_acc = (float)o[7]; t.a_w = (float)o[8]; t.a_scale = (float)o[10]; }
+          else { t.q_acc = (float)o[7]; t.q_q = (float)o[8]; t.q_b = (float)o[9]; t.q_scale = (float)o[10]; }
+        }
+      }
+      if (i == count || c.steps == 0) return -3;
+      c.q = w.terms + (size_t)program[12 * i + 1] * batch * 2 * m * lda;
+      if ((r = ns::chain(ms, c, st)) != 0) return r;
+      --i;                                               // (the loop goes on with the row of the next X)
+    }
   }
   return 0;
 }
