@@ -11,7 +11,7 @@ torch's (or the native pool's) stream-ordered allocator, so a region that does n
   the capture produced;
 * quantities that are passed to kernels BY VALUE are frozen at capture time (dropout seeds, communication epochs),
   so multi-GPU collectives and dropout stay outside a graph.  Adam/AdamW keep their step count, bias corrections and
-  learning rate in a device vector once `make_capturable()` was called, which is what `GraphedTrainStep` does: a
+  learning rate in a device vector once `make_capturable()` was called (Muon its learning rate), which is what `GraphedTrainStep` does: a
   whole single-GPU training step (forward, backward, optimizer) replays as one launch.
 
 The reference has no counterpart (it launches every Triton kernel from Python).
@@ -123,24 +123,30 @@ class GraphedTrainStep(GraphedCallable):
     list of input tuples is given (real batches) and on `sample_inputs` otherwise; after them
     the step is captured once and every call replays it: inputs are copied into the static buffers, a changed
     `optimizer.lr` is written to the optimizer's device vector, and the returned loss is the static tensor the
-    capture produced (valid until the next call).  Gradients stay readable in `p.grad` after a replay.
+    capture produced (valid until the next call).  Gradients stay readable in `p.grad` after a replay.  `optimizer` may be
+    a list, for steps in which several update their parameters (Muon and AdamW).
     Restrictions: fixed input shapes, no host reads inside `step_fn`, no dropout, one GPU.
     """
 
     def __init__(self, step_fn, optimizer, sample_inputs, warmup=3, warmup_inputs=None):
-        if not hasattr(optimizer, "make_capturable"):
-            raise TypeError("GraphedTrainStep needs an Adam / AdamW optimizer (device-resident step state)")
-        optimizer.make_capturable()
+        self._optimizers = list(optimizer) if isinstance(optimizer, (list, tuple)) else [optimizer]
+        if not self._optimizers or not all(hasattr(o, "make_capturable") for o in self._optimizers):
+            raise TypeError("GraphedTrainStep needs Adam / AdamW / Muon optimizers (device-resident step state)")
+        for o in self._optimizers:
+            o.make_capturable()
         self.optimizer = optimizer
         from ..ops import native
         before = native.launch_count
         super().__init__(step_fn, sample_inputs, warmup, warmup_inputs)
         # kernels per replay = launches recorded while capturing (the last of warmup + 1 runs of step_fn)
         self.kernels_per_step = (native.launch_count - before) // (warmup + 1)
-        optimizer.t -= 1          # the captured call counted a step that did not run
+        for o in self._optimizers:
+            o.t -= 1              # the captured call counted a step that did not run
 
     def __call__(self, *inputs):
-        self.optimizer._sync_lr()
+        for o in self._optimizers:
+            o._sync_lr()
         out = super().__call__(*inputs)
-        self.optimizer.t += 1
+        for o in self._optimizers:
+            o.t += 1
         return out

@@ -1637,7 +1637,7 @@ def policy_loss(logits, tokens, old_log_probs, advantages, ref_log_probs=None, c
     With lp the tokens' log-probabilities (of logits / temperature) and r = exp(lp - old_log_probs), every token's loss is
     max(-A r, -A clamp(r, 1 - clip, 1 + clip_high)) + kl_coef (exp(d) - d - 1), d = ref_log_probs - lp.
     `advantages` has one number per token, or one per sequence ([...] without the last dimension); `clip_high` is `clip`
-    unless given.  Tokens equal to `ignore_index` (prompts, padding) do not count, whatever the other inputs hold there;
+    unless given; a `kl_coef` of 0 leaves the reference out.  Tokens equal to `ignore_index` (prompts, padding) do not count, whatever the other inputs hold there;
     "mean" is over those that do (0 if there are none).  Gradients flow to the logits alone; where both branches are
     equal they flow through the first."""
     name = "policy_loss"
@@ -1648,11 +1648,13 @@ def policy_loss(logits, tokens, old_log_probs, advantages, ref_log_probs=None, c
     lo = 1.0 - _number(name, "clip", clip, 0.0, 1.0)
     hi = 1.0 + _number(name, "clip_high", clip if clip_high is None else clip_high, 0.0, math.inf)
     kl = _number(name, "kl_coef", kl_coef, 0.0, math.inf)
-    if (ref_log_probs is None) != (kl == 0.0):
-        raise ValueError(f"{name}: ref_log_probs and a positive kl_coef go together")
+    if ref_log_probs is None and kl > 0.0:
+        raise ValueError(f"{name}: a positive kl_coef needs ref_log_probs")
     old = _constant(name, "old_log_probs", old_log_probs, (shape,), z)
     adv = _constant(name, "advantages", advantages, (shape, shape[:-1]) if shape else (shape,), z)
     ref = None if ref_log_probs is None else _constant(name, "ref_log_probs", ref_log_probs, (shape,), z)
+    if kl == 0.0:
+        ref = None
     div = 1 if tuple(adv.shape) == shape else _pymax(shape[-1], 1)
     return PolicyLossFunction.apply(logits, t, (old, adv, div, ref, lo, hi, kl), float(temperature), ignore_index, reduction)
 

@@ -154,6 +154,38 @@ def test_repeats_bit_for_bit_and_on_another_stream():
         assert float(torch.linalg.matrix_norm(whole[i].double() - alone[i].double())) < 2 * TOL
 
 
+def test_two_streams_at_once_and_a_captured_call():
+    """Calls that overlap have workspaces of their own; a captured call replays on new values."""
+    xs = [matrix(4, 300, 500, seed=i).cuda() for i in range(4)]
+    want = [genesis.optim.orthogonalize(T(x))._t.clone() for x in xs]
+    streams = [torch.cuda.Stream() for _ in xs]
+    torch.cuda.synchronize()
+    got = [None] * 4
+    for _ in range(3):
+        for i, (x, st) in enumerate(zip(xs, streams)):
+            with torch.cuda.stream(st):
+                got[i] = genesis.optim.orthogonalize(T(x))._t
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    graphed = [genesis.cuda.make_graphed_callable(lambda x: genesis.optim.orthogonalize(x), [T(xs[0])]) for _ in range(2)]
+    for i in (1, 2, 3):
+        a = graphed[0](T(xs[i]))
+        b = graphed[1](T(xs[i - 1]))
+        torch.cuda.synchronize()
+        assert torch.equal(a._t, want[i]) and torch.equal(b._t, want[i - 1])
+
+
+def test_empty_and_zero_gradients():
+    ps = [genesis.nn.Parameter(T(matrix(*s).cuda())) for s in ((30, 40), (0, 40), (40, 30), (5, 6))]
+    opt = genesis.optim.Muon(ps, lr=0.1, weight_decay=0.5)
+    before = [p._t.clone() for p in ps]
+    ps[0].grad, ps[1].grad = T(torch.zeros(30, 40).cuda()), T(torch.zeros(0, 40).cuda())
+    ps[2].grad = T(matrix(40, 30, seed=1).cuda())
+    opt.step()
+    assert torch.allclose(ps[0]._t, before[0] * (1 - 0.1 * 0.5)) and torch.equal(ps[3]._t, before[3])
+    assert float((ps[2]._t - before[2]).abs().max()) > 1e-3
+
+
 def test_grad_scaler():
     shapes, ps = _model_like()
     opt = genesis.optim.Muon(ps, lr=0.1)
@@ -216,14 +248,17 @@ def test_post_training_steps_of_a_model():
     losses = [step(*eager).item() for _ in range(5)]
     assert all(math.isfinite(x) for x in losses) and len(set(losses)) == 5
     graphed = build()
-    graphed[2].make_capturable()
-    run = genesis.cuda.GraphedTrainStep(lambda: step(*graphed), graphed[1], [], warmup=3)
+    run = genesis.cuda.GraphedTrainStep(lambda: step(*graphed), graphed[1:], [], warmup=3)
     again = [run().item() for _ in range(2)]
     # The framework adds up the embedding's gradient in memory in no fixed order, so runs differ in its last bits (eager ones
     # too), and the next step's gradients by some 1e-7 of themselves.  The iteration amplifies that by 485 at most: updates of
     # 2-norm 0.02 * 485 * 1e-7 = 1e-6 for each of the 14 matrices, against gradients of 2-norm 0.5 at most: 7e-6 of the loss.
     assert max(abs(a - b) for a, b in zip(again, losses[3:])) < 1e-5
-    assert graphed[1].t == 5
+    assert graphed[1].t == graphed[2].t == 5
+    # a learning rate changed between replays counts
+    graphed[1].lr, before = 0.0, graphed[1].params[0]._t.clone()
+    run()
+    assert torch.equal(graphed[1].params[0]._t, before)
     # the gradient of one weight against differences of the loss, along the gradient
     model = build()[0]
     pref = T(torch.zeros(4).cuda())
