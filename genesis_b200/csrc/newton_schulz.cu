@@ -27,9 +27,14 @@
 // fill the GPU are shared by clusters of up to 8 CTAs, each with a part of the contraction; many large ones are worked on by
 // CTA pairs, which read two thirds of the bytes.
 //
-// Sums.  The tensor cores round their accumulator towards zero, which adds up over a long contraction (4864 x 896: 1.6e-5 of
-// the result).  So an accumulator takes up 512 elements of the contraction (256 in tiles of 128 columns) and is then added,
-// rounded to nearest, to the sums that the epilogue's warps hold in registers; the products go on in the next one meanwhile.
+// Sums.  The tensor cores round their accumulator towards zero, by 0.5 to 0.8 of a unit in the last place for every 16
+// elements of the contraction: 13 units of a sum of 256 positive terms, 65 of 1024.  In A that shortens the diagonal, and steps
+// with A amplify it.  So in symmetric products an accumulator takes up 128 elements of the contraction, the small products of
+// each block of 64 first, and is then added, rounded to nearest, to the sums that the epilogue's warps hold in registers; in
+// Q X, which nothing amplifies, 256.  The products go on in the next accumulator meanwhile.  Measured error of the result
+// against 64 bits, with 64 / 128 / 256 elements (and of fp32 products): rank 8 plus noise, 16 x 5000 3.6 / 6.3 / 9.6e-6 (0.8e-6),
+// 1024 x 4096 1.9 / 1.7 / 1.7e-6 (3.2e-6); Gaussian, 400 x 4000 1.5 / 2.2 / 3.3e-5 (0.5e-5), 1024 x 1024 7.5 / 7.6 / 9.9e-6
+// (3.1e-6); time of 24 of 4864 x 896 3866 / 3669 / 3592 us.
 #include "sm100_ptx.cuh"
 #include "sm100_pair.cuh"
 #include "common.cuh"
@@ -360,11 +365,12 @@ ns_product_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_consta
   constexpr bool B_MN = MODE != SYM;                           // X as the right operand: its rows run along the contraction
   constexpr int TM = KIND == PAIR ? 2 * BM : BM;        // rows of a tile
   constexpr int BNC = KIND == PAIR ? BN / 2 : BN;       // columns of the right operand that a CTA loads
-  // Ring of half stages: (A hi, B lo) and (A lo, B hi) of a block of the contraction.  The three products of a block run in
-  // the order hi lo, hi hi, lo hi, so the first half is free before the block is done.
+  // Ring of half stages: the high terms of both operands for a block of the contraction, then the low ones.  The products of
+  // a block run in the order hi lo, lo hi, hi hi: while the small ones are summed the accumulator is small and loses little,
+  // and the low terms are free before the block is done.
   constexpr int HALF_BYTES = A_BYTES + BNC * 128, HALVES = RING_BYTES / HALF_BYTES / 2 * 2;
   constexpr int ACCS = 512 / BN;                        // accumulators in tensor memory
-  constexpr int DRAIN = BN == 256 ? 8 : 4;              // blocks of BK that one accumulator takes up: see the header
+  constexpr int DRAIN = MODE == SYM ? 2 : 4;            // blocks of BK that one accumulator takes up: see the header
   constexpr int CHUNKS = BN / 64;                       // of 32 x 32 results, per epilogue warp
   extern __shared__ __align__(1024) uint8_t smem[];
   uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + BARRIER_OFFSET);       // (a pair: those of CTA 0 count both CTAs' loads)
@@ -464,7 +470,7 @@ ns_product_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_consta
           const int za = 2 * (pr.left * p.batch + zz), zb = 2 * (pr.right * p.batch + zz);
           bool ok = true;
           for (int kh = 2 * kb0; kh < 2 * kb1; ++kh, ++it) {
-            const int s = it % HALVES, k0 = (kh >> 1) * BK, h = kh & 1;      // h: A's term (0 = hi); B's is the other
+            const int s = it % HALVES, k0 = (kh >> 1) * BK, h = kh & 1;      // h: 0 = high terms, 1 = low
             if (!mbar_wait(&empty_bar[s], ((it / HALVES) & 1) ^ 1, abort_flag, p.status, 110)) { ok = false; break; }
             uint8_t* sa = smem + s * HALF_BYTES;
             uint8_t* sb = sa + A_BYTES;
@@ -473,10 +479,10 @@ ns_product_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_consta
               if (rank == 0) mbar_expect_tx(&full_bar[s], 2 * HALF_BYTES);
               g2::tma2_load_3d(sa, &tmapA, bar, k0, m0, za + h);
               if constexpr (!B_MN) {
-                g2::tma2_load_3d(sb, &tmapB, bar, k0, n0, zb + 1 - h);
+                g2::tma2_load_3d(sb, &tmapB, bar, k0, n0, zb + h);
               } else {
 #pragma unroll
-                for (int c = 0; c < BNC / 64; ++c) g2::tma2_load_3d(sb + c * (BK * 128), &tmapB, bar, n0 + c * 64, k0, zb + 1 - h);
+                for (int c = 0; c < BNC / 64; ++c) g2::tma2_load_3d(sb + c * (BK * 128), &tmapB, bar, n0 + c * 64, k0, zb + h);
               }
             } else {
               mbar_expect_tx(&full_bar[s], HALF_BYTES);
@@ -484,10 +490,10 @@ ns_product_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_consta
               if constexpr (!B_MN) {
 #pragma unroll
                 for (int c = 0; c < BNC / 128; ++c)
-                  tma_load_3d(sb + c * A_BYTES, &tmapB, &full_bar[s], k0, n0 + c * 128, zb + 1 - h);
+                  tma_load_3d(sb + c * A_BYTES, &tmapB, &full_bar[s], k0, n0 + c * 128, zb + h);
               } else {
 #pragma unroll
-                for (int c = 0; c < BNC / 64; ++c) tma_load_3d(sb + c * (BK * 128), &tmapB, &full_bar[s], n0 + c * 64, k0, zb + 1 - h);
+                for (int c = 0; c < BNC / 64; ++c) tma_load_3d(sb + c * (BK * 128), &tmapB, &full_bar[s], n0 + c * 64, k0, zb + h);
               }
             }
           }
@@ -528,20 +534,18 @@ ns_product_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_consta
           for (int k = kb; k < end; ++k, it += 2) {
             const int s = it % HALVES;                                       // (even: HALVES is)
             const uint32_t ph = (it / HALVES) & 1;
-            if (!__all_sync(0xffffffffu, mbar_wait(&full_bar[s], ph, abort_flag, p.status, 211))) { ok = false; break; }
+            if (!__all_sync(0xffffffffu, mbar_wait(&full_bar[s], ph, abort_flag, p.status, 211) &&
+                                             mbar_wait(&full_bar[s + 1], ph, abort_flag, p.status, 212))) { ok = false; break; }
             tc_fence_after_sync();
             const uint32_t x_addr = smem_u32(smem + s * HALF_BYTES), y_addr = x_addr + HALF_BYTES;
-            const uint64_t a_hi = make_smem_desc(x_addr, 16, 1024), b_lo = b_desc(x_addr + A_BYTES);
-            const uint64_t a_lo = make_smem_desc(y_addr, 16, 1024), b_hi = b_desc(y_addr + A_BYTES);
-            if (elect_one()) multiply(d_tmem, a_hi, b_lo, k == kb);
-            __syncwarp();
-            if (!__all_sync(0xffffffffu, mbar_wait(&full_bar[s + 1], ph, abort_flag, p.status, 212))) { ok = false; break; }
-            tc_fence_after_sync();
+            const uint64_t a_hi = make_smem_desc(x_addr, 16, 1024), b_hi = b_desc(x_addr + A_BYTES);
+            const uint64_t a_lo = make_smem_desc(y_addr, 16, 1024), b_lo = b_desc(y_addr + A_BYTES);
             if (elect_one()) {
-              multiply(d_tmem, a_hi, b_hi, false);
-              commit(&empty_bar[s]);
+              multiply(d_tmem, a_hi, b_lo, k == kb);
               multiply(d_tmem, a_lo, b_hi, false);
               commit(&empty_bar[s + 1]);
+              multiply(d_tmem, a_hi, b_hi, false);
+              commit(&empty_bar[s]);
             }
             __syncwarp();
           }
@@ -712,7 +716,7 @@ ns_chain_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_constant
     tma_prefetch_desc(&tmapA);
   }
   if (warp == 0) {
-    tmem_alloc(tmem_slot, 128);
+    tmem_alloc(tmem_slot, 256);
     tmem_relinquish();
   }
   tc_fence_before_sync();
@@ -757,13 +761,18 @@ ns_chain_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_constant
     if (warp == 0 && ok) {
       const uint64_t l = make_smem_desc(smem_u32(left), 16, 1024), r = make_smem_desc(smem_u32(right), 16, 1024);
       if (elect_one()) {
+        // the small products and half of the large ones in one accumulator, the others in a second one
+        constexpr uint64_t LO = 1024;
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
           const uint64_t at = (uint64_t)((k >> 2) * 2048 + (k & 3) * 2);      // (16-byte units; 32 KB a half)
-          constexpr uint64_t LO = 1024;
           umma_f16(tmem, l + at, r + at + LO, idesc, k == 0 ? 0u : 1u);
           umma_f16(tmem, l + at + LO, r + at, idesc, 1u);
-          umma_f16(tmem, l + at, r + at, idesc, 1u);
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const uint64_t at = (uint64_t)((k >> 2) * 2048 + (k & 3) * 2);
+          umma_f16(tmem + (k >> 2) * 128, l + at, r + at, idesc, k == 4 ? 0u : 1u);
         }
         umma_commit(done);
       }
@@ -775,9 +784,14 @@ ns_chain_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_constant
     tc_fence_after_sync();
   };
   // the thread's 32 columns 32 h .. of the accumulator
-  auto take = [&](int h, uint32_t (&r)[32]) {
-    tmem_ld_32x32b_x32(tmem + ((uint32_t)((warp & 3) * 32) << 16) + col0 + 32 * h, r);
+  auto take = [&](int h, float (&r)[32]) {
+    uint32_t a[32], b[32];
+    const uint32_t at = tmem + ((uint32_t)((warp & 3) * 32) << 16) + col0 + 32 * h;
+    tmem_ld_32x32b_x32(at, a);
+    tmem_ld_32x32b_x32(at + 128, b);
     tmem_ld_wait();
+#pragma unroll
+    for (int j = 0; j < 32; ++j) r[j] = __uint_as_float(a[j]) + __uint_as_float(b[j]);
   };
   // unit u (8 columns) of the thread's half row in a slot: hi, and lo 16 KB on
   auto unit = [&](uint8_t* slot, int u) { return slot + half * 32768 + row * 128 + ((u ^ (row & 7)) << 4); };
@@ -800,6 +814,7 @@ ns_chain_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_constant
   };
   if (ok) ok = mbar_wait(loaded, 0, abort_flag, p.status, 411);
   ok = __syncthreads_and(ok);
+  if (work && !ok && threadIdx.x == 0) drain_copies(loaded, 1, 1);
   float q_unscale = 1.f;                                 // 1 / 2^k of Q's terms
   for (int s = 0; s < p.steps; ++s) {
     const ChainStep& c = p.step[s];
@@ -807,13 +822,13 @@ ns_chain_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_constant
     multiply(slot_r, slot_r);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      uint32_t r[32];
+      float r[32];
       take(h, r);
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         float v[8];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = fmaf(__uint_as_float(r[8 * u + k]), c.sq_acc, whole[32 * h + 8 * u + k] * c.sq_a);
+        for (int k = 0; k < 8; ++k) v[k] = fmaf(r[8 * u + k], c.sq_acc, whole[32 * h + 8 * u + k] * c.sq_a);
         put(into, 4 * h + u, v, c.sq_scale);
       }
     }
@@ -822,7 +837,7 @@ ns_chain_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_constant
       const float b_unscale = 1.f / c.sq_scale;          // (powers of two)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        uint32_t r[32];
+        float r[32];
         take(h, r);
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
@@ -830,7 +845,7 @@ ns_chain_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_constant
           get(slot_q, 4 * h + u, q, q_unscale * c.q_q);
           get(slot_b, 4 * h + u, b, b_unscale * c.q_b);
 #pragma unroll
-          for (int k = 0; k < 8; ++k) q[k] = fmaf(__uint_as_float(r[8 * u + k]), c.q_acc, q[k]) + b[k];
+          for (int k = 0; k < 8; ++k) q[k] = fmaf(r[8 * u + k], c.q_acc, q[k]) + b[k];
           put(slot_q, 4 * h + u, q, c.q_scale);
         }
       }
@@ -846,7 +861,7 @@ ns_chain_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_constant
       multiply(left, slot_r);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        uint32_t r[32];
+        float r[32];
         take(h, r);
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
@@ -854,7 +869,7 @@ ns_chain_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_constant
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
             const int j = 32 * h + 8 * u + k;
-            whole[j] = v[k] = fmaf(__uint_as_float(r[8 * u + k]), acc, whole[j] * own);
+            whole[j] = v[k] = fmaf(r[8 * u + k], acc, whole[j] * own);
           }
           put(slot_r, 4 * h + u, v, scale);
         }
@@ -876,7 +891,7 @@ ns_chain_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_constant
   __syncthreads();
   if (warp == 0) {
     tc_fence_after_sync();
-    tmem_dealloc(tmem, 128);
+    tmem_dealloc(tmem, 256);
   }
 }
 
