@@ -630,7 +630,8 @@ ns_product_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_consta
       }
     }
     if constexpr (KIND == SPLIT) {
-      // the parts of a tile meet: rank k adds up chunks k, k + splits, .., in the order of the ranks, one warp each at a time
+      // the parts of a tile meet: rank k adds up chunks k, k + splits, .., one warp each at a time, its own part first and
+      // the others' in turn (a fixed order for every chunk, and not all ranks at one CTA's shared memory)
       tc_fence_before_sync();
       __syncthreads();
       g2::cluster_sync_all();
@@ -648,7 +649,7 @@ ns_product_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_consta
           for (int i = 0; i < 8; ++i) sum[i] = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
           for (int k = 0; k < splits; ++k) {
-            const uint32_t peer = g2::map_to_cta(smem_u32(smem) + c * CHUNK_BYTES, k);
+            const uint32_t peer = g2::map_to_cta(smem_u32(smem) + c * CHUNK_BYTES, (rank + k) & (splits - 1));
             float4 o[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) o[i] = ld_peer(peer + chunk_at(4 * i + (lane >> 3), lane & 7));
@@ -1114,8 +1115,8 @@ static int product(const CUtensorMap& ta, const CUtensorMap& tb, Params p, cudaS
   // Tiles of 128 x 128 or 128 x 256, whole or shared by the CTAs of a cluster, or of 256 x 256 on pairs: whatever has the
   // fewest clocks on its longest CTA.  A block of the contraction takes 1080 clocks with 128 columns and 1700 with 256,
   // bound by shared memory (213 and 160 bytes a clock at the full tensor rate, of 128), or 2100 where all SMs together
-  // read more than L2 gives (11 TB/s); pairs read two thirds of that and take 1600.  A start and its epilogue are 6000 to
-  // 10000, the exchange of a cluster 4000.
+  // read more than L2 gives (11 TB/s); pairs read two thirds of that and take 1600.  The epilogue of the last tile, which no
+  // products hide, takes 6500 for each chunk of a warp; the parts of a cluster 4000 to meet and 5000 a chunk.
   int kind = WHOLE, bn = 128;
   long long best = -1, grid = 0;
   auto offer = [&](long long clocks, int k, int width, int splits, long long ctas) {
@@ -1124,13 +1125,13 @@ static int product(const CUtensorMap& ta, const CUtensorMap& tb, Params p, cudaS
   };
   for (int width = 128; width <= 256; width += 128) {
     const long long total = tiles_of(MODE == SYM, p.m, p.n, BM, width) * matrices, waves = (total + sms - 1) / sms;
-    const long long block = width == 128 ? 1080 : total >= sms ? 2100 : 1700, ends = width == 128 ? 6000 : 8000;
-    offer(waves * kblocks * block + ends, WHOLE, width, 1, total < sms ? total : sms);
+    const long long block = width == 128 ? 1080 : total >= sms ? 2100 : 1700, chunks = width / 64;
+    offer(waves * kblocks * block + chunks * 6500, WHOLE, width, 1, total < sms ? total : sms);
     for (int s = 2; s <= 8 && kblocks >= 2 * s && total <= max_clusters(s); s *= 2)      // (one tile each: a single wave)
-      offer((kblocks + s - 1) / s * (width == 128 ? 1080 : 1700) + ends + 4000, SPLIT, width, s, total * s);
+      offer((kblocks + s - 1) / s * (width == 128 ? 1080 : 1700) + (chunks + s - 1) / s * 5000 + 4000, SPLIT, width, s, total * s);
   }
   const long long pairs = tiles_of(MODE == SYM, p.m, p.n, 2 * BM, 256) * matrices, at_once = max_clusters(2);
-  offer((pairs + at_once - 1) / at_once * kblocks * 1600 + 10000, PAIR, 256, 1, 2 * (pairs < at_once ? pairs : at_once));
+  offer((pairs + at_once - 1) / at_once * kblocks * 1600 + 4 * 6500, PAIR, 256, 1, 2 * (pairs < at_once ? pairs : at_once));
   const int g = (int)grid;
   if (kind == PAIR) return launch<MODE, 256, PAIR>(ta, tb, p, g, st);
   if (kind == SPLIT) return bn == 256 ? launch<MODE, 256, SPLIT>(ta, tb, p, g, st) : launch<MODE, 128, SPLIT>(ta, tb, p, g, st);
