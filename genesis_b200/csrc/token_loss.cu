@@ -296,11 +296,11 @@ __device__ __forceinline__ double block_sum64(double v, double* sh) {
   return v;
 }
 
-// out[0] = sum of the rows' losses (over the number of rows that count), out[1] = the factor of every row's gradient
+// *out = sum of the rows' losses (over the number of rows that count), *factor = the factor of every row's gradient
 template <typename TI>
 __global__ void __launch_bounds__(1024)
 policy_sum_kernel(const float* __restrict__ loss, const TI* __restrict__ tokens, long long rows, long long cols,
-                  long long ignore, int mean, float* __restrict__ out) {
+                  long long ignore, int mean, float* __restrict__ out, float* __restrict__ factor) {
   __shared__ double sh[32];
   double sum = 0.0, n = 0.0;
   for (long long r = threadIdx.x; r < rows; r += 1024) {
@@ -311,8 +311,8 @@ policy_sum_kernel(const float* __restrict__ loss, const TI* __restrict__ tokens,
   n = block_sum64(n, sh);
   if (threadIdx.x == 0) {
     const double f = mean && n > 0.0 ? 1.0 / n : 1.0;
-    out[0] = (float)(sum * f);
-    out[1] = (float)f;
+    *out = (float)(sum * f);
+    *factor = (float)f;
   }
 }
 
@@ -529,20 +529,20 @@ extern "C" int gb_token_rows(const void* z, const void* tokens, float* lp, float
                       dt, token_i64, status, st);
 }
 
-// The same, and every row's clipped policy loss [rows] and its derivative by lp, coef [rows]; out [2] (or null) receives the
-// sum of the losses (over the number of rows that count with `mean`) and the factor of their gradients.
+// The same, and every row's clipped policy loss [rows] and its derivative by lp, coef [rows]; out (or null) receives the sum
+// of the losses (over the number of rows that count with `mean`), factor that of their gradients.
 extern "C" int gb_policy_loss(const void* z, const void* tokens, float* lp, float* stats, long long rows, long long cols,
                               long long inner, long long s_outer, long long s_inner, long long ignore, float temperature,
                               const float* old, const float* adv, const float* ref, float* loss, float* coef, long long adv_div,
-                              float lo, float hi, float kl, float* out, int mean, int dt, int token_i64, int* status,
+                              float lo, float hi, float kl, float* out, float* factor, int mean, int dt, int token_i64, int* status,
                               cudaStream_t st) {
   if (adv_div < 1) return -3;
   const tl::Policy q{old, adv, ref, loss, coef, adv_div, lo, hi, kl};
   if (const int e = tl::rows_any(z, tokens, lp, stats, rows, cols, tl::RowMap{inner, s_outer, s_inner}, ignore, temperature, q,
                                  dt, token_i64, status, st)) return e;
   if (out == nullptr) return 0;
-  if (token_i64) tl::policy_sum_kernel<long long><<<1, 1024, 0, st>>>(loss, (const long long*)tokens, rows, cols, ignore, mean, out);
-  else tl::policy_sum_kernel<int><<<1, 1024, 0, st>>>(loss, (const int*)tokens, rows, cols, ignore, mean, out);
+  if (token_i64) tl::policy_sum_kernel<long long><<<1, 1024, 0, st>>>(loss, (const long long*)tokens, rows, cols, ignore, mean, out, factor);
+  else tl::policy_sum_kernel<int><<<1, 1024, 0, st>>>(loss, (const int*)tokens, rows, cols, ignore, mean, out, factor);
   return (int)cudaGetLastError();
 }
 

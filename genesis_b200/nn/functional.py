@@ -983,17 +983,17 @@ class PolicyLossFunction(Function):
     @staticmethod
     def forward(ctx, logits, tokens, policy, temperature, ignore_index, reduction):
         logits = K.token_logits(logits)
-        loss, stats, factor = K.policy_loss(logits, tokens, ignore_index, temperature, policy, reduction)
-        ctx.save_for_backward(logits, tokens, stats, factor)
-        ctx.meta = (temperature, ignore_index)
+        loss, stats = K.policy_loss(logits, tokens, ignore_index, temperature, policy, reduction)
+        ctx.save_for_backward(logits, tokens, stats)
+        ctx.meta = (temperature, ignore_index, reduction == "none")
         return loss
 
     @staticmethod
     def backward(ctx, g):
-        logits, tokens, stats, factor = ctx.saved_tensors
-        temperature, ignore_index = ctx.meta
+        logits, tokens, stats = ctx.saved_tensors
+        temperature, ignore_index, each = ctx.meta
         return K.token_grad(logits, tokens, stats, ignore_index, temperature, 1, _as(g, stats.dtype),
-                            g_mod=_pymax(tokens.numel(), 1) if factor is None else 1, dev_scale=factor)
+                            g_mod=_pymax(tokens.numel(), 1) if each else 1, factor_at=0 if each else 3 * tokens.numel())
 
 
 class PreferenceLossFunction(Function):

@@ -636,7 +636,7 @@ def token_rows(logits, tokens, ignore_index, temperature):
 def policy_loss(logits, tokens, ignore_index, temperature, policy, reduction):
     """Clipped policy loss; `policy` = (old log-probabilities, advantages, rows per advantage, reference log-probabilities or
     None, lowest ratio, highest ratio, KL weight).  Returns (loss, the rows' statistics as in `token_rows` followed by the
-    derivatives of their losses by the log-probabilities, a factor of all gradients [1] or None)."""
+    derivatives of their losses by the log-probabilities and, unless reduction is "none", a factor of all gradients)."""
     if logits.is_cuda:
         r = N.policy_loss(logits, tokens, ignore_index, temperature, policy, reduction)
         if r is not NotImplemented:
@@ -658,10 +658,10 @@ def policy_loss(logits, tokens, ignore_index, temperature, policy, reduction):
     loss = torch.where(valid, loss, zero)
     stats = torch.cat((stats, torch.where(valid, coef, zero).reshape(-1)))
     if reduction == "none":
-        return loss, stats, None
+        return loss, stats
     n = int(valid.sum())
     f = 1.0 / n if reduction == "mean" and n else 1.0
-    return (loss.double().sum() * f).to(loss.dtype), stats, torch.tensor([f], dtype=loss.dtype, device=loss.device)
+    return (loss.double().sum() * f).to(loss.dtype), torch.cat((stats, stats.new_tensor([f])))
 
 
 def preference_loss(logits, tokens, ignore_index, ref, beta, smoothing, reduction):
@@ -685,20 +685,20 @@ def preference_loss(logits, tokens, ignore_index, ref, beta, smoothing, reductio
     return (total / (n // 2) if reduction == "mean" and n else total).to(lp.dtype), rewards, stats
 
 
-def token_grad(logits, tokens, stats, ignore_index, temperature, base_div=0, g=None, g_div=1, g_mod=1, dev_scale=None,
+def token_grad(logits, tokens, stats, ignore_index, temperature, base_div=0, g=None, g_div=1, g_mod=1, factor_at=0,
                scale=1.0):
     """Gradient of the logits: row r's derivative by its token's log-probability is
-    base[r // base_div] * g[r // g_div % g_mod] * dev_scale * scale, base being what follows the rows' statistics in `stats`
-    (base_div 0: 1; dev_scale None: 1); zero for ignored rows."""
+    base[r // base_div] * g[r // g_div % g_mod] * factor * scale, base being what follows the rows' statistics in `stats` and
+    factor what stands at `factor_at` there (base_div, factor_at 0: 1); zero for ignored rows."""
     if logits.is_cuda and logits.dtype != torch.float64:
-        return N.token_grad(logits, tokens, stats, ignore_index, temperature, base_div, g, g_div, g_mod, dev_scale, scale)
+        return N.token_grad(logits, tokens, stats, ignore_index, temperature, base_div, g, g_div, g_mod, factor_at, scale)
     rows, V = tokens.numel(), logits.shape[-1]
     r = torch.arange(rows, device=logits.device)
     f = g.reshape(-1)[r // g_div % g_mod] * scale
     if base_div:
         f = f * stats[2 * rows:][r // base_div]
-    if dev_scale is not None:
-        f = f * dev_scale
+    if factor_at:
+        f = f * stats[factor_at]
     flat = tokens.reshape(-1)
     valid = (flat != ignore_index) & (flat >= 0) & (flat < V)
     f = torch.where(valid, f, torch.zeros_like(f)) / temperature

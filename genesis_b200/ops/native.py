@@ -69,7 +69,7 @@ _SIGS = {
     "gb_cast_stack": "ppipip",
     "gb_masked_fill": "pp" + "d" + "ll" + "i" + "p", "gb_fill_elems": "pldip",
     "gb_token_rows": "pppp" + "lllll" + "l" + "f" + "ii" + "pp",
-    "gb_policy_loss": "pppp" + "lllll" + "l" + "f" + "ppppp" + "l" + "fff" + "p" + "iii" + "pp",
+    "gb_policy_loss": "pppp" + "lllll" + "l" + "f" + "ppppp" + "l" + "fff" + "pp" + "iii" + "pp",
     "gb_preference_loss": "pppp" + "lllll" + "l" + "p" + "l" + "ff" + "i" + "pppp" + "ii" + "pp",
     "gb_token_grad": "pppp" + "lllll" + "l" + "f" + "pl" + "pll" + "p" + "f" + "ii" + "p",
     "gb_ns_workspace": "lllip", "gb_muon_momentum": "p" + "iiii" + "f" + "i" + "ppp" + "p",
@@ -1882,6 +1882,8 @@ def masked_fill_(a, mask, value):
 def _row_map(logits):
     """(rows per outer step, outer stride, inner stride) of the rows of [..., V] logits, in elements, or None when they do
     not lie on two strides or a row is not contiguous.  A `logits[:, :-1]` view does, so it is read in place."""
+    if logits.is_contiguous():
+        return logits.numel() // logits.shape[-1] or 1, 0, logits.shape[-1]
     if logits.shape[-1] > 1 and logits.stride(-1) != 1:
         return None
     dims = []                                            # (size, stride) from the outermost, neighbours merged
@@ -1920,25 +1922,25 @@ def token_rows(logits, tokens, ignore_index, temperature):
 
 
 def policy_loss(logits, tokens, ignore_index, temperature, policy, reduction):
-    """(loss, rows' statistics [2, rows] followed by the derivatives of their losses [rows], factor of the gradients [1] or
-    None); `policy` as in `dispatch.policy_loss`."""
+    """(loss, rows' statistics [2, rows] followed by the derivatives of their losses [rows] and a factor of all gradients
+    unless reduction is "none"); `policy` as in `dispatch.policy_loss`."""
     m = _row_map(logits)
     if logits.dtype not in _FLOATS or m is None:
         return NotImplemented
     old, adv, div, ref, lo, hi, kl = policy
     rows, dev = tokens.numel(), logits.device
     each = reduction == "none"
-    # one buffer: statistics, derivatives, log-probabilities, and the losses where they are not asked for
-    buf = torch.empty((4 if each else 5) * rows, dtype=F32, device=dev)
-    out = torch.empty(tokens.shape, dtype=F32, device=dev) if each else torch.empty(2, dtype=F32, device=dev)
+    # one buffer: statistics, derivatives, factor, log-probabilities, and the losses where they are not asked for
+    buf = torch.empty((4 if each else 5) * rows + 1, dtype=F32, device=dev)
+    out = torch.empty(tokens.shape if each else (), dtype=F32, device=dev)
     at, op = buf.data_ptr(), out.data_ptr()
     with _on(dev):
-        _chk(lib().gb_policy_loss(logits.data_ptr(), tokens.data_ptr(), at + 12 * rows, at, rows, logits.shape[-1], *m,
+        _chk(lib().gb_policy_loss(logits.data_ptr(), tokens.data_ptr(), at + 12 * rows + 4, at, rows, logits.shape[-1], *m,
                                   ignore_index, temperature, old.data_ptr(), adv.data_ptr(), _ptr(ref),
-                                  op if each else at + 16 * rows, at + 8 * rows, div, lo, hi, kl, None if each else op,
-                                  1 if reduction == "mean" else 0, _DT[logits.dtype], 1 if tokens.dtype == torch.int64 else 0,
-                                  status_tensor(dev).data_ptr(), _st()), "policy_loss")
-    return (out, buf, None) if each else (out[0], buf, out[1:])
+                                  op if each else at + 16 * rows + 4, at + 8 * rows, div, lo, hi, kl, None if each else op,
+                                  at + 12 * rows, 1 if reduction == "mean" else 0, _DT[logits.dtype],
+                                  1 if tokens.dtype == torch.int64 else 0, status_tensor(dev).data_ptr(), _st()), "policy_loss")
+    return out, buf
 
 
 def preference_loss(logits, tokens, ignore_index, ref, beta, smoothing, reduction):
@@ -1961,10 +1963,10 @@ def preference_loss(logits, tokens, ignore_index, ref, beta, smoothing, reductio
     return out, rewards, buf
 
 
-def token_grad(logits, tokens, stats, ignore_index, temperature, base_div, g, g_div, g_mod, dev_scale, scale):
+def token_grad(logits, tokens, stats, ignore_index, temperature, base_div, g, g_div, g_mod, factor_at, scale):
     """Gradient of [..., V] logits; row r's derivative by its token's log-probability is
-    base[r // base_div] * g[r // g_div % g_mod] * dev_scale * scale, base being what follows the rows' statistics in `stats`
-    (base_div 0: 1; dev_scale None: 1)."""
+    base[r // base_div] * g[r // g_div % g_mod] * factor * scale, base being what follows the rows' statistics in `stats` and
+    factor what stands at `factor_at` there (base_div, factor_at 0: 1)."""
     m = _row_map(logits)
     rows = tokens.numel()
     out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
@@ -1972,7 +1974,7 @@ def token_grad(logits, tokens, stats, ignore_index, temperature, base_div, g, g_
     with _on(logits.device):
         _chk(lib().gb_token_grad(logits.data_ptr(), tokens.data_ptr(), at, out.data_ptr(), rows, logits.shape[-1], *m,
                                  ignore_index, temperature, at + 8 * rows if base_div else None, base_div or 1, g.data_ptr(),
-                                 g_div, g_mod, _ptr(dev_scale), scale, _DT[logits.dtype],
+                                 g_div, g_mod, at + 4 * factor_at if factor_at else None, scale, _DT[logits.dtype],
                                  1 if tokens.dtype == torch.int64 else 0, _st()), "token_grad")
     return out
 
