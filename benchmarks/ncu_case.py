@@ -9,7 +9,8 @@ grouped_gemm (gemm_kernel), attn128_fwd (attn_fwd_kernel), attn128_bwd (attn_bwd
 attn64_fwd, attn64_bwd, attn_decode (attn_decode_kernel), ce (ce_fwd16_kernel / ce_bwd_kernel), softmax (row_stream_kernel / softmax_bwd), rmsnorm (row_stream_kernel / rmsnorm_bwd_kernel),
 addnorm, addnorm_wide (add_rmsnorm_fwd_stream_kernel / rmsnorm_bwd_stream_kernel), moe_combine_bwd (moe_combine_bwd_vec_kernel),
 adam (adam_multi_kernel), swiglu_bwd (swiglu_bwd2d_kernel), rope (rope_vec_kernel),
-reduce_cols (reduce_mid), sort (sort_rows), index (index_get_kernel / index_put_kernel), cat (cat_kernel).
+token_loss (token_rows_kernel / token_grad_kernel), newton_schulz (ns_product_kernel: with -s 4 -c 7 a block of two steps),
+newton_schulz_small (ns_chain_kernel), reduce_cols (reduce_mid), sort (sort_rows), index (index_get_kernel / index_put_kernel), cat (cat_kernel).
 """
 import sys
 import os
@@ -166,7 +167,24 @@ def cat():
     return lambda: K.cat(xs, 1)
 
 
+def token_loss():
+    z, t = rnd(2048, 151936, scale=3.0), torch.randint(0, 151936, (2048,), device=DEV)
+    g = torch.ones(2048, device=DEV)
+
+    def f():
+        _, stats = K.token_rows(z, t, -100, 1.0)
+        K.token_grad(z, t, stats, -100, 1.0, g=g, g_mod=2048)
+    return f
+
+
+def newton_schulz(batch, rows, cols):
+    x = genesis.Tensor(torch.randn(batch, rows, cols, device=DEV))
+    return lambda: genesis.optim.orthogonalize(x, steps=2)
+
+
 CASES = {
+    "token_loss": token_loss, "newton_schulz": lambda: newton_schulz(12, 896, 4864),
+    "newton_schulz_small": lambda: newton_schulz(148, 128, 896),
     "gemm_pair": gemm_pair, "gemm_swiglu": gemm_swiglu, "gemm_swiglu_bwd": gemm_swiglu_bwd, "gemm": gemm, "grouped_gemm": grouped_gemm,
     "attn128_fwd": lambda: _attn(4, 4096, 16, 4, 128, False), "attn128_bwd": lambda: _attn(4, 4096, 16, 4, 128, True),
     "attn64_fwd": lambda: _attn(8, 2048, 14, 2, 64, False), "attn64_bwd": lambda: _attn(8, 2048, 14, 2, 64, True),
