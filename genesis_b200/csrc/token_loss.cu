@@ -190,9 +190,9 @@ __device__ __forceinline__ void finish_row(MaxSum a, const T* p, long long t, lo
     float loss = fmaxf(plain, clipped), coef = plain >= clipped ? plain : 0.f;
     if (plain != plain || clipped != clipped) { loss = plain + clipped; coef = loss; }      // NaN stays NaN
     if (q.ref != nullptr) {
-      const float d = q.ref[r] - lp, e = expf(d);
-      loss += q.kl * (e - d - 1.f);
-      coef += q.kl * (1.f - e);
+      const float d = q.ref[r] - lp, e1 = expm1f(d);               // (exp(d) - 1 would lose what a small d adds)
+      loss += q.kl * (e1 - d);
+      coef -= q.kl * e1;
     }
     q.loss[r] = loss;
     q.coef[r] = coef;

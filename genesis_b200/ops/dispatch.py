@@ -652,9 +652,9 @@ def policy_loss(logits, tokens, ignore_index, temperature, policy, reduction):
     coef = torch.where(torch.isnan(loss), loss, coef)
     if ref is not None:
         d = ref - lp
-        e = torch.exp(d)
-        loss = loss + kl * (e - d - 1)
-        coef = coef + kl * (1 - e)
+        e1 = torch.expm1(d)                              # (exp(d) - 1 would lose what a small d adds)
+        loss = loss + kl * (e1 - d)
+        coef = coef - kl * e1
     loss = torch.where(valid, loss, zero)
     stats = torch.cat((stats, torch.where(valid, coef, zero).reshape(-1)))
     if reduction == "none":

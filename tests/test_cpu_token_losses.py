@@ -127,6 +127,22 @@ def test_what_does_not_count_reaches_nothing():
     assert abs(loss.item() - math.log(2)) < 1e-6 and not rewards._t.any() and not y.grad._t.any()
 
 
+def test_kl_of_a_policy_near_its_reference():
+    """lp is off by 3e-6 at most (its rounding at |lp| < 16 1e-6, the row's log-sum 2e-6), d by that, and exp(d) - 1 - d by
+    |d| of it; exp(d) - 1 has 2^-22 of its own; the loss's rounding 2^-23.  A difference of numbers near one would be off by 1e-7."""
+    g, z, t = make((4, 50), 64, 11, ignored=0.1)
+    lp, on = R.log_probs(z.double(), t)
+    assert float(lp.abs().max()) < 16
+    d = torch.where(torch.rand(t.shape, generator=g) < 0.5, 1.0, -1.0) * 10 ** (-3 + torch.rand(t.shape, generator=g).double())
+    ref, old = (lp + d).float(), lp.float()
+    loss = F.policy_loss(T(z), T(t), T(old), T(torch.zeros(t.shape)), T(ref), kl_coef=0.5, reduction="none")
+    r = R.leaf64(z)
+    each, _ = R.policy(r, t, old, torch.zeros(t.shape), ref, kl=0.5)
+    tol = 0.5 * (d.abs() * 3e-6 + 1e-11 + 2.0 ** -22 * d.abs()) + 2.0 ** -23 * each
+    assert bool(((loss._t.double() - each).abs() <= tol).all())
+    assert float(tol.max()) < 3e-8
+
+
 def test_masked_vocabulary():
     """-inf logits have probability 0 and gradient 0; an answer made of one gives a ratio of 0."""
     g, z, t = make((1, 4), 8, 6, ignored=0.0)
