@@ -338,7 +338,10 @@ preference_kernel(const float* __restrict__ lp, const float* __restrict__ ref, l
     const float h = rewards[i] - rewards[pairs + i];
     // log(1 + exp(-|h|)) is common to both signs: -log sigmoid(h) = max(-h, 0) + it
     const float l1 = log1pf(expf(-fabsf(h)));
-    const float loss = (1.f - smooth) * (fmaxf(-h, 0.f) + l1) + smooth * (fmaxf(h, 0.f) + l1) + (h != h ? h : 0.f);
+    // a side of weight 0 is left out: h is infinite where an answer holds a token of probability 0
+    float loss = h != h ? h : 0.f;
+    if (smooth < 1.f) loss += (1.f - smooth) * (fmaxf(-h, 0.f) + l1);
+    if (smooth > 0.f) loss += smooth * (fmaxf(h, 0.f) + l1);
     const float g = beta * (smooth - 1.f / (1.f + expf(h)));
     gseq[i] = g;
     gseq[pairs + i] = -g;

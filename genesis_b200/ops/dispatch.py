@@ -676,7 +676,11 @@ def preference_loss(logits, tokens, ignore_index, ref, beta, smoothing, reductio
     rewards = (beta * (lp.double().sum(-1) - ref.double())).to(lp.dtype)
     h = rewards[:n // 2] - rewards[n // 2:]
     lse = torch.log1p(torch.exp(-h.abs()))
-    loss = (1 - smoothing) * ((-h).clamp(min=0) + lse) + smoothing * (h.clamp(min=0) + lse)
+    loss = torch.where(torch.isnan(h), h, torch.zeros_like(h))
+    if smoothing < 1:                                    # (h is infinite where an answer holds a token of probability 0)
+        loss = loss + (1 - smoothing) * ((-h).clamp(min=0) + lse)
+    if smoothing > 0:
+        loss = loss + smoothing * (h.clamp(min=0) + lse)
     g = beta * (smoothing - 1 / (1 + torch.exp(h)))
     stats = torch.cat((stats, g, -g))
     if reduction == "none":

@@ -138,9 +138,28 @@ def test_kl_of_a_policy_near_its_reference():
     loss = F.policy_loss(T(z), T(t), T(old), T(torch.zeros(t.shape)), T(ref), kl_coef=0.5, reduction="none")
     r = R.leaf64(z)
     each, _ = R.policy(r, t, old, torch.zeros(t.shape), ref, kl=0.5)
+    each = each.detach()
     tol = 0.5 * (d.abs() * 3e-6 + 1e-11 + 2.0 ** -22 * d.abs()) + 2.0 ** -23 * each
     assert bool(((loss._t.double() - each).abs() <= tol).all())
     assert float(tol.max()) < 3e-8
+
+
+def test_an_answer_of_probability_zero():
+    """Pair 0 rejects one, pair 1 chose one, pair 2 has none."""
+    g, z, t = make((6, 3), 40, 12, ignored=0.0)
+    z[3, 1, t[3, 1]] = -math.inf
+    z[1, 2, t[1, 2]] = -math.inf
+    x = T(z, requires_grad=True)
+    loss, rewards = F.preference_loss(x, T(t), T(torch.zeros(6)), return_rewards=True, reduction="none")
+    assert rewards._t[3] == -math.inf and rewards._t[1] == -math.inf and math.isfinite(float(rewards._t[2]))
+    assert loss._t[0] == 0 and loss._t[1] == math.inf and 0 < float(loss._t[2]) < 10
+    loss.sum().backward()
+    gr = x.grad._t
+    # the pair that is decided asks for nothing; the gradient of the other's rows is beta (onehot - softmax), all finite
+    assert not gr[0].any() and not gr[3].any() and bool(torch.isfinite(gr).all())
+    assert abs(float(gr[1, 2, t[1, 2]]) + 0.1) < 1e-6
+    smooth = F.preference_loss(x, T(t), T(torch.zeros(6)), label_smoothing=0.1, reduction="none")
+    assert smooth._t[0] == math.inf and smooth._t[1] == math.inf
 
 
 def test_masked_vocabulary():
