@@ -1595,6 +1595,8 @@ def _token_args(name, logits, tokens, ignore_index, temperature=1.0):
         raise ValueError(f"{name}: logits are on {z.device}, tokens on {t.device}")
     if isinstance(ignore_index, bool) or not isinstance(ignore_index, int):
         raise TypeError(f"{name}: ignore_index must be an int, got {ignore_index!r}")
+    if not -2 ** 63 <= ignore_index < 2 ** 63:
+        raise ValueError(f"{name}: ignore_index must be a 64-bit number, got {ignore_index}")
     if not 1e-6 <= float(temperature) < math.inf:
         raise ValueError(f"{name}: temperature must be finite and at least 1e-6, got {temperature}")
     if t.dtype not in (torch.int64, torch.int32):

@@ -230,6 +230,13 @@ def test_refusals():
             call()
 
 
+@pytest.mark.parametrize("ignore_index", [2 ** 63, -2 ** 63 - 1, 2 ** 64])
+def test_an_ignore_index_that_no_token_can_be_is_refused(ignore_index):
+    g, z, t = make((2, 4), 10, 8, ignored=0.0)
+    with pytest.raises(ValueError):
+        F.token_log_probs(T(z), T(t), ignore_index=ignore_index)
+
+
 def test_row_map():
     """Rows that lie on two strides are read in place."""
     from genesis_b200.ops.native import _row_map
