@@ -217,20 +217,21 @@ def test_masked_vocabulary_and_extremes(dtype, V):
 
 
 def test_kl_of_a_policy_near_its_reference():
-    """lp is off by 3e-6 at most (its rounding at |lp| < 16 1e-6, the row's log-sum 2e-6), d by that, and exp(d) - 1 - d by
-    |d| of it; exp(d) - 1 has 2^-22 of its own; the loss's rounding 2^-23.  A difference of numbers near one would be off by 1e-7."""
+    """lp is off by 4e-6 at most (its rounding at |lp| < 32 2^-19, the row's log-sum 2e-6), ref by its rounding 2e-6, d by
+    both, and exp(d) - 1 - d by |d| of it; exp(d) - 1 has 2^-22 of its own; the loss's rounding 2^-23.  A difference of
+    numbers near one would be off by 1e-7."""
     g, z, t = make((4, 50), 64, 11, ignored=0.1)
     lp, on = R.log_probs(z.double(), t)
-    assert float(lp.abs().max()) < 16
+    assert float(lp.abs().max()) < 32
     d = torch.where(torch.rand(t.shape, generator=g) < 0.5, 1.0, -1.0) * 10 ** (-3 + torch.rand(t.shape, generator=g).double())
     ref, old = (lp + d).float(), lp.float()
     loss = F.policy_loss(*dev(z, t, old, torch.zeros(t.shape), ref), kl_coef=0.5, reduction="none")
     r = R.leaf64(z)
     each, _ = R.policy(r, t, old, torch.zeros(t.shape), ref, kl=0.5)
     each = each.detach()
-    tol = 0.5 * (d.abs() * 3e-6 + 1e-11 + 2.0 ** -22 * d.abs()) + 2.0 ** -23 * each
+    tol = 0.5 * (d.abs() * 6e-6 + 4e-11 + 2.0 ** -22 * d.abs()) + 2.0 ** -23 * each
     assert bool(((loss._t.cpu().double() - each).abs() <= tol).all())
-    assert float(tol.max()) < 3e-8
+    assert float(tol.max()) < 4e-8
 
 
 def test_an_answer_of_probability_zero():
