@@ -229,12 +229,9 @@ token_rows_warp_kernel(const T* __restrict__ z, RowMap map, const TI* __restrict
 }
 
 // Longer rows: one CTA of G threads each, or, where rows are few, the CTAs of a cluster share one and rank 0 joins their
-// parts through distributed shared memory.  16-bit rows of 512 threads are bound by the exponentials as much as by memory, so
-// as many threads as fit keep two vectors in flight each; 32-bit ones, with half the exponentials a byte, do better with
-// fewer threads and four vectors.  Over 6973 rows of 151936 bf16, us: two vectors and four CTAs on an SM 398 (5.3 TB/s), two
-// and three 415, four and two 424, rings of asynchronous copies private to a thread 472; 2048 of fp32: 221, 209, 199, 209.
-template <typename T, typename TI, int G>
-__global__ void __launch_bounds__(G, G == 512 ? (sizeof(T) == 2 ? 4 : 2) : 8)
+// parts through distributed shared memory.  A thread has U vectors in flight; OCC CTAs fit an SM.
+template <typename T, typename TI, int G, int U, int OCC>
+__global__ void __launch_bounds__(G, OCC)
 token_rows_kernel(const T* __restrict__ z, RowMap map, const TI* __restrict__ tokens, float* __restrict__ lp,
                   float* __restrict__ stats, long long rows, int cols, long long ignore, float temperature, Scale c,
                   Policy q, int* status, int parts) {
@@ -257,7 +254,7 @@ token_rows_kernel(const T* __restrict__ z, RowMap map, const TI* __restrict__ to
     lo = min(part * step, cols);
     n = min(step, cols - lo);
   }
-  MaxSum a = warp_join(scan<T, G, G == 512 && sizeof(T) == 2 ? 2 : 4>(p + lo, n, c, threadIdx.x), temperature);
+  MaxSum a = warp_join(scan<T, G, U>(p + lo, n, c, threadIdx.x), temperature);
   if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = make_float2(a.m, a.s);
   __syncthreads();
   if (threadIdx.x < 32) {
@@ -468,30 +465,38 @@ static int rows_forward(const void* z, RowMap map, const void* tokens, float* lp
                         long long ignore, float temperature, const Policy& q, int* status, cudaStream_t st) {
   const Scale c((double)temperature);
   const long long bytes = (long long)cols * sizeof(T), sms = sm_count();
-  // A warp a row up to 8 KB, 128 threads up to 32 KB, else 512; fewer rows than warps, or CTAs, that the device holds take the
-  // next larger group.
+  // A warp a row up to 8 KB, 128 threads up to 32 KB, as long as these fill the device
   if (bytes <= 2048 || (bytes <= 8192 && rows >= 32 * sms)) {
     token_rows_warp_kernel<T, TI><<<(unsigned)((rows + 7) / 8), 256, 0, st>>>(
         (const T*)z, map, (const TI*)tokens, lp, stats, rows, cols, ignore, temperature, c, q, status);
     return (int)cudaGetLastError();
   }
-  if (bytes <= 8192 || (bytes <= 32768 && rows >= 8 * sms)) {
-    token_rows_kernel<T, TI, 128><<<(unsigned)rows, 128, 0, st>>>(
-        (const T*)z, map, (const TI*)tokens, lp, stats, rows, cols, ignore, temperature, c, q, status, 1);
-    return (int)cudaGetLastError();
-  }
-  // a part has to be worth its cluster barriers: 4096 elements at least
   int parts = 1;
-  while (parts < 8 && rows * parts * 2 <= 3 * sms && cols / (parts * 2) >= 4096) parts *= 2;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = parts; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
-  cfg.gridDim = dim3((unsigned)(rows * parts)); cfg.blockDim = dim3(512); cfg.stream = st;
-  cfg.attrs = attr; cfg.numAttrs = parts > 1 ? 1 : 0;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, token_rows_kernel<T, TI, 512>, (const T*)z, map, (const TI*)tokens, lp, stats, rows,
-                                           cols, ignore, temperature, c, q, status, parts);
-  return e == cudaSuccess ? (int)cudaGetLastError() : (int)e;
+  auto run = [&](auto kernel, int threads) {
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = parts; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    cfg.gridDim = dim3((unsigned)(rows * parts)); cfg.blockDim = dim3(threads); cfg.stream = st;
+    cfg.attrs = attr; cfg.numAttrs = parts > 1 ? 1 : 0;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, (const T*)z, map, (const TI*)tokens, lp, stats, rows, cols, ignore,
+                                             temperature, c, q, status, parts);
+    return e == cudaSuccess ? (int)cudaGetLastError() : (int)e;
+  };
+  if (bytes <= 8192 || (bytes <= 32768 && rows >= 8 * sms)) return run(token_rows_kernel<T, TI, 128, 4, 8>, 128);
+  // Up to two rows an SM: as many threads and vectors in flight as a row can use.  Clusters pay up to one CTA an SM, in parts
+  // that are worth their barriers.  Rows of 151936 bf16, one CTA / clusters of 4, us: 16 rows 18.4 / 12.3, 40 18.4 / 14.3,
+  // 74 18.4 / 20.5; of 24000 8.2 / 10.2.  256 threads instead, 148 rows: 26.7 for 20.5.
+  if (rows <= 2 * sms) {
+    while (parts < 8 && rows * parts * 2 <= sms && cols / (parts * 2) >= 16384) parts *= 2;
+    return run(token_rows_kernel<T, TI, 512, 4, 2>, 512);
+  }
+  // More rows: smaller CTAs, so that fewer threads wait for a row's slowest warp and the last rows spread better.  Of 151936
+  // bf16, 512 / 256 threads: 1000 rows 75.8 / 71.7, 6973 rows 367 / 352 (6.0 TB/s).  16-bit rows are bound by the exponentials
+  // as much as by memory and take all the threads that fit, with two vectors each (four and half as many threads 371);
+  // 32-bit ones, with half the exponentials a byte, four (1000 rows 108 for 125).
+  if (sizeof(T) == 2 && rows > 4 * sms) return run(token_rows_kernel<T, TI, 256, 2, 8>, 256);
+  return run(token_rows_kernel<T, TI, 256, 4, 4>, 256);
 }
 
 template <typename T, typename TI>
