@@ -677,8 +677,9 @@ ns_product_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_consta
 // Launched one by one they take 8 us each, of which the products are one; here 4 us (128 x 896, five steps: 148 -> 92 us).
 // Three slots hold terms, [two halves of the columns][hi, lo][128 rows of 128 bytes], swizzled as the tensor cores read
 // them: R (A, then W in its place, then the next A), B and Q; a result is written where the operand that it replaces has
-// been read from.  A thread keeps half a row of A or W in 32 bits in registers.  Rows and columns past m are zero throughout.
-constexpr int CHAIN_THREADS = 256;
+// been read from.  A thread keeps a quarter of a row of A or W in 32 bits in registers.  Rows and
+// columns past m are zero throughout.
+constexpr int CHAIN_THREADS = 512;
 constexpr int CHAIN_SLOT = 4 * 128 * 128;
 constexpr int CHAIN_BARRIERS = 3 * CHAIN_SLOT;
 constexpr int CHAIN_SMEM = CHAIN_BARRIERS + 64;
@@ -728,8 +729,8 @@ ns_chain_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_constant
   let_next_start();
   wait_for_previous();
 
-  const int row = (warp & 3) * 32 + lane, half = warp >> 2, col0 = half * 64;      // this thread's half row
-  float whole[64];
+  const int row = (warp & 3) * 32 + lane, col0 = (warp >> 2) * 32;       // this thread's part of a row
+  float whole[32];
   uint8_t* slot_r = smem;
   uint8_t* slot_b = smem + CHAIN_SLOT;
   uint8_t* slot_q = smem + 2 * CHAIN_SLOT;
@@ -741,7 +742,7 @@ ns_chain_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_constant
   {
     const float* a = p.a + ((size_t)z * p.m + row) * p.lda + col0;
 #pragma unroll
-    for (int u = 0; u < 16; ++u) {
+    for (int u = 0; u < 8; ++u) {
       const float4 v = row < p.m && col0 + 4 * u < p.m ? *reinterpret_cast<const float4*>(a + 4 * u) : make_float4(0.f, 0.f, 0.f, 0.f);
       // (elements of the last vector past m are padding, whatever it holds)
       whole[4 * u] = v.x;
@@ -784,18 +785,20 @@ ns_chain_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_constant
     phase ^= 1;
     tc_fence_after_sync();
   };
-  // the thread's 32 columns 32 h .. of the accumulator
-  auto take = [&](int h, float (&r)[32]) {
+  // the thread's part of the accumulator
+  auto take = [&](float (&r)[32]) {
     uint32_t a[32], b[32];
-    const uint32_t at = tmem + ((uint32_t)((warp & 3) * 32) << 16) + col0 + 32 * h;
+    const uint32_t at = tmem + ((uint32_t)((warp & 3) * 32) << 16) + col0;
     tmem_ld_32x32b_x32(at, a);
     tmem_ld_32x32b_x32(at + 128, b);
     tmem_ld_wait();
 #pragma unroll
     for (int j = 0; j < 32; ++j) r[j] = __uint_as_float(a[j]) + __uint_as_float(b[j]);
   };
-  // unit u (8 columns) of the thread's half row in a slot: hi, and lo 16 KB on
-  auto unit = [&](uint8_t* slot, int u) { return slot + half * 32768 + row * 128 + ((u ^ (row & 7)) << 4); };
+  // unit u (8 columns) of the thread's part of a row in a slot: hi, and lo 16 KB on
+  auto unit = [&](uint8_t* slot, int u) {
+    return slot + (warp >> 3) * 32768 + row * 128 + ((((warp >> 2) & 1) * 4 + u) ^ (row & 7)) * 16;
+  };
   auto put = [&](uint8_t* slot, int u, const float (&v)[8], float scale) {
     const uint4 s = split4(v[0] * scale, v[1] * scale, v[2] * scale, v[3] * scale), t = split4(v[4] * scale, v[5] * scale, v[6] * scale, v[7] * scale);
     uint8_t* at = unit(slot, u);
@@ -821,34 +824,27 @@ ns_chain_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_constant
     const ChainStep& c = p.step[s];
     uint8_t* into = s == 0 ? slot_q : slot_b;            // the first B is Q
     multiply(slot_r, slot_r);
+    float r[32];
+    take(r);
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      float r[32];
-      take(h, r);
+    for (int u = 0; u < 4; ++u) {
+      float v[8];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        float v[8];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = fmaf(r[8 * u + k], c.sq_acc, whole[32 * h + 8 * u + k] * c.sq_a);
-        put(into, 4 * h + u, v, c.sq_scale);
-      }
+      for (int k = 0; k < 8; ++k) v[k] = fmaf(r[8 * u + k], c.sq_acc, whole[8 * u + k] * c.sq_a);
+      put(into, u, v, c.sq_scale);
     }
     if (s > 0) {
       multiply(slot_b, slot_q);
       const float b_unscale = 1.f / c.sq_scale;          // (powers of two)
+      take(r);
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        float r[32];
-        take(h, r);
+      for (int u = 0; u < 4; ++u) {
+        float q[8], b[8];
+        get(slot_q, u, q, q_unscale * c.q_q);
+        get(slot_b, u, b, b_unscale * c.q_b);
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          float q[8], b[8];
-          get(slot_q, 4 * h + u, q, q_unscale * c.q_q);
-          get(slot_b, 4 * h + u, b, b_unscale * c.q_b);
-#pragma unroll
-          for (int k = 0; k < 8; ++k) q[k] = fmaf(r[8 * u + k], c.q_acc, q[k]) + b[k];
-          put(slot_q, 4 * h + u, q, c.q_scale);
-        }
+        for (int k = 0; k < 8; ++k) q[k] = fmaf(r[8 * u + k], c.q_acc, q[k]) + b[k];
+        put(slot_q, u, q, c.q_scale);
       }
       q_unscale = 1.f / c.q_scale;
     } else {
@@ -860,27 +856,23 @@ ns_chain_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_constant
     for (int twice = 0; twice < 2; ++twice) {            // W in the place of A, then A in the place of W
       const float acc = twice ? c.a_acc : c.w_acc, own = twice ? c.a_w : c.w_a, scale = twice ? c.a_scale : c.w_scale;
       multiply(left, slot_r);
+      take(r);
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        float r[32];
-        take(h, r);
+      for (int u = 0; u < 4; ++u) {
+        float v[8];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          float v[8];
-#pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const int j = 32 * h + 8 * u + k;
-            whole[j] = v[k] = fmaf(r[8 * u + k], acc, whole[j] * own);
-          }
-          put(slot_r, 4 * h + u, v, scale);
+        for (int k = 0; k < 8; ++k) {
+          const int j = 8 * u + k;
+          whole[j] = v[k] = fmaf(r[8 * u + k], acc, whole[j] * own);
         }
+        put(slot_r, u, v, scale);
       }
     }
   }
   if (ok && row < p.m) {
     __half* q = p.q + ((size_t)z * 2 * p.m + row) * p.lda + col0;
 #pragma unroll
-    for (int u = 0; u < 8; ++u) {
+    for (int u = 0; u < 4; ++u) {
       if (col0 + 8 * u < p.m) {
         const uint8_t* at = unit(slot_q, u);
         *reinterpret_cast<uint4*>(q + 8 * u) = *reinterpret_cast<const uint4*>(at);
