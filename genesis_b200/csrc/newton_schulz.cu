@@ -673,12 +673,12 @@ ns_product_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_consta
   }
 }
 
-// A block's products of m x m matrices for m <= 128 in one launch: one CTA per matrix, all matrices in its shared memory.
-// Launched one by one they take 8 us each, of which the products are one; here 4 us (128 x 896, five steps: 148 -> 92 us).
-// Three slots hold terms, [two halves of the columns][hi, lo][128 rows of 128 bytes], swizzled as the tensor cores read
-// them: R (A, then W in its place, then the next A), B and Q; a result is written where the operand that it replaces has
-// been read from.  A thread keeps a quarter of a row of A or W in 32 bits in registers.  Rows and
-// columns past m are zero throughout.
+// A block's products of m x m matrices for m <= 128, and often A = X X^T before them, in one launch: one CTA per matrix, all
+// matrices in its shared memory.  Launched one by one they take 8 us each, of which the products are one; here 2.1 us (128 x 896,
+// five steps: 148 -> 81 us).  Three slots hold terms, [two halves of the columns][hi, lo][128 rows of 128 bytes], swizzled as
+// the tensor cores read them: R (A, then W in its place, then the next A), B and Q; a result is written where the operand that
+// it replaces has been read from.  A thread keeps a quarter of a row of A or W in 32 bits in registers.  Rows and columns past
+// m are zero throughout.
 constexpr int CHAIN_THREADS = 512;
 constexpr int CHAIN_SLOT = 4 * 128 * 128;
 constexpr int CHAIN_BARRIERS = 3 * CHAIN_SLOT;
@@ -694,31 +694,33 @@ struct ChainStep {
 struct Chain {
   int* status;
   int m, batch, lda, steps;    // up to 3
+  int blocks;                  // X in blocks of 128 columns, from which A is formed here; 0: A is there
+  float gram, gram_scale;      // A = gram X X^T, 2^k of its terms
   const float* a;              // A in 32 bits (slot 0)
   __half* q;                   // terms of Q [batch][hi, lo][m][lda]
   ChainStep step[3];
 };
 
 __global__ void __launch_bounds__(CHAIN_THREADS, 1)
-ns_chain_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_constant__ Chain p) {
+ns_chain_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_constant__ CUtensorMap tmapX,
+                const __grid_constant__ Chain p) {
   extern __shared__ __align__(1024) uint8_t smem[];
   uint64_t* loaded = reinterpret_cast<uint64_t*>(smem + CHAIN_BARRIERS);
-  uint64_t* done = loaded + 1;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+  uint64_t* done = loaded + 3;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int z = blockIdx.x;
   if (threadIdx.x == 0) {
-    mbar_init(loaded, 1);
-    mbar_init(done, 1);
+    for (int i = 0; i < 5; ++i) mbar_init(&loaded[i], 1);
     const bool aligned = (smem_u32(smem) & 1023) == 0;
     if (!aligned) report_error(p.status, GB_ERR_BAD_ARG, 6, 0);
     *abort_flag = !aligned || status_poisoned(p.status) ? 1 : 0;
     mbar_fence_init();
-    tma_prefetch_desc(&tmapA);
+    tma_prefetch_desc(p.blocks > 0 ? &tmapX : &tmapA);
   }
   if (warp == 0) {
-    tmem_alloc(tmem_slot, 256);
+    tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
   tc_fence_before_sync();
@@ -734,66 +736,52 @@ ns_chain_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_constant
   uint8_t* slot_r = smem;
   uint8_t* slot_b = smem + CHAIN_SLOT;
   uint8_t* slot_q = smem + 2 * CHAIN_SLOT;
-  if (work && threadIdx.x == 0) {
-    mbar_expect_tx(loaded, CHAIN_SLOT);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) tma_load_3d(slot_r + i * 16384, &tmapA, loaded, (i >> 1) * 64, 0, 2 * z + (i & 1));
-  }
-  {
-    const float* a = p.a + ((size_t)z * p.m + row) * p.lda + col0;
-#pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      const float4 v = row < p.m && col0 + 4 * u < p.m ? *reinterpret_cast<const float4*>(a + 4 * u) : make_float4(0.f, 0.f, 0.f, 0.f);
-      // (elements of the last vector past m are padding, whatever it holds)
-      whole[4 * u] = v.x;
-      whole[4 * u + 1] = col0 + 4 * u + 1 < p.m ? v.y : 0.f;
-      whole[4 * u + 2] = col0 + 4 * u + 2 < p.m ? v.z : 0.f;
-      whole[4 * u + 3] = col0 + 4 * u + 3 < p.m ? v.w : 0.f;
-    }
-  }
   const uint32_t idesc = make_idesc(0u, 0u, 0u, 128, 128);
-  uint32_t phase = 0;
+  uint32_t phase = 0;                                    // of done[0]
   bool ok = work;
-  // accumulator = L R; every thread waits for it
-  auto multiply = [&](const uint8_t* left, const uint8_t* right) {
-    fence_proxy_async_smem();
-    tc_fence_before_sync();
-    __syncthreads();                                     // operands written, the last accumulator read
-    tc_fence_after_sync();
-    if (warp == 0 && ok) {
-      const uint64_t l = make_smem_desc(smem_u32(left), 16, 1024), r = make_smem_desc(smem_u32(right), 16, 1024);
-      if (elect_one()) {
-        // the small products and half of the large ones in one accumulator, the others in a second one
-        constexpr uint64_t LO = 1024;
+  // accumulators `buf` = L R, by warp 0
+  auto issue = [&](const uint8_t* left, const uint8_t* right, int buf) {
+    const uint64_t l = make_smem_desc(smem_u32(left), 16, 1024), r = make_smem_desc(smem_u32(right), 16, 1024);
+    const uint32_t acc = tmem + buf * 256;
+    if (elect_one()) {
+      // the small products and half of the large ones in one accumulator, the others in a second one
+      constexpr uint64_t LO = 1024;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const uint64_t at = (uint64_t)((k >> 2) * 2048 + (k & 3) * 2);      // (16-byte units; 32 KB a half)
-          umma_f16(tmem, l + at, r + at + LO, idesc, k == 0 ? 0u : 1u);
-          umma_f16(tmem, l + at + LO, r + at, idesc, 1u);
-        }
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const uint64_t at = (uint64_t)((k >> 2) * 2048 + (k & 3) * 2);
-          umma_f16(tmem + (k >> 2) * 128, l + at, r + at, idesc, k == 4 ? 0u : 1u);
-        }
-        umma_commit(done);
+      for (int k = 0; k < 8; ++k) {
+        const uint64_t at = (uint64_t)((k >> 2) * 2048 + (k & 3) * 2);      // (16-byte units; 32 KB a half)
+        umma_f16(acc, l + at, r + at + LO, idesc, k == 0 ? 0u : 1u);
+        umma_f16(acc, l + at + LO, r + at, idesc, 1u);
       }
-      __syncwarp();
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const uint64_t at = (uint64_t)((k >> 2) * 2048 + (k & 3) * 2);
+        umma_f16(acc + (k >> 2) * 128, l + at, r + at, idesc, k == 4 ? 0u : 1u);
+      }
+      umma_commit(&done[buf]);
     }
-    if (ok) ok = mbar_wait(done, phase, abort_flag, p.status, 410);
-    ok = __syncthreads_and(ok);
-    phase ^= 1;
-    tc_fence_after_sync();
+    __syncwarp();
   };
-  // the thread's part of the accumulator
-  auto take = [&](float (&r)[32]) {
+  // the thread's part of accumulators `buf`
+  auto take = [&](float (&r)[32], int buf) {
     uint32_t a[32], b[32];
-    const uint32_t at = tmem + ((uint32_t)((warp & 3) * 32) << 16) + col0;
+    const uint32_t at = tmem + buf * 256 + ((uint32_t)((warp & 3) * 32) << 16) + col0;
     tmem_ld_32x32b_x32(at, a);
     tmem_ld_32x32b_x32(at + 128, b);
     tmem_ld_wait();
 #pragma unroll
     for (int j = 0; j < 32; ++j) r[j] = __uint_as_float(a[j]) + __uint_as_float(b[j]);
+  };
+  // accumulators 0 = L R; every thread waits for them
+  auto multiply = [&](const uint8_t* left, const uint8_t* right) {
+    fence_proxy_async_smem();
+    tc_fence_before_sync();
+    __syncthreads();                                     // operands written, the last accumulator read
+    tc_fence_after_sync();
+    if (warp == 0 && ok) issue(left, right, 0);
+    if (ok) ok = mbar_wait(&done[0], phase, abort_flag, p.status, 410);
+    ok = __syncthreads_and(ok);
+    phase ^= 1;
+    tc_fence_after_sync();
   };
   // unit u (8 columns) of the thread's part of a row in a slot: hi, and lo 16 KB on
   auto unit = [&](uint8_t* slot, int u) {
@@ -816,16 +804,81 @@ ns_chain_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_constant
       v[2 * k + 1] = (a.y + b.y) * factor;
     }
   };
-  if (ok) ok = mbar_wait(loaded, 0, abort_flag, p.status, 411);
-  ok = __syncthreads_and(ok);
-  if (work && !ok && threadIdx.x == 0) drain_copies(loaded, 1, 1);
+  if (p.blocks > 0) {
+    // A = X X^T: the slots are a ring of blocks of X; while one is multiplied, the products of the last are added up
+    auto load = [&](int d) {
+      const int i = d % 3;
+      mbar_expect_tx(&loaded[i], CHAIN_SLOT);
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        tma_load_3d(smem + i * CHAIN_SLOT + k * 16384, &tmapX, &loaded[i], d * 128 + (k >> 1) * 64, 0, 2 * z + (k & 1));
+    };
+    int issued = 0;
+    if (work && threadIdx.x == 0)
+      for (; issued < 3 && issued < p.blocks; ++issued) load(issued);
+#pragma unroll
+    for (int j = 0; j < 32; ++j) whole[j] = 0.f;
+    for (int d = 0; d <= p.blocks; ++d) {
+      if (warp == 0 && d < p.blocks && ok) {
+        ok = __all_sync(0xffffffffu, mbar_wait(&loaded[d % 3], (d / 3) & 1, abort_flag, p.status, 411));
+        if (ok) issue(smem + d % 3 * CHAIN_SLOT, smem + d % 3 * CHAIN_SLOT, d & 1);
+      }
+      if (d > 0) {
+        const int e = d - 1;
+        if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&done[e & 1], (e >> 1) & 1, abort_flag, p.status, 412));
+        if (ok) {
+          if (threadIdx.x == 0 && issued < p.blocks) load(issued++);      // into the slot that block e has left
+          __syncwarp();
+          tc_fence_after_sync();
+          float r[32];
+          take(r, e & 1);
+#pragma unroll
+          for (int j = 0; j < 32; ++j) whole[j] += r[j];
+          tc_fence_before_sync();
+        }
+      }
+      ok = __syncthreads_and(ok);
+      tc_fence_after_sync();
+      if (!ok) break;
+    }
+    if (work && !ok && threadIdx.x == 0) drain_copies(loaded, 3, issued);
+    phase = ((p.blocks + 1) / 2) & 1;
+#pragma unroll
+    for (int j = 0; j < 32; ++j) whole[j] *= p.gram;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      float v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = whole[8 * u + k];
+      put(slot_r, u, v, p.gram_scale);
+    }
+  } else {
+    if (work && threadIdx.x == 0) {
+      mbar_expect_tx(loaded, CHAIN_SLOT);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) tma_load_3d(slot_r + i * 16384, &tmapA, loaded, (i >> 1) * 64, 0, 2 * z + (i & 1));
+    }
+    const float* a = p.a + ((size_t)z * p.m + row) * p.lda + col0;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const float4 v = row < p.m && col0 + 4 * u < p.m ? *reinterpret_cast<const float4*>(a + 4 * u) : make_float4(0.f, 0.f, 0.f, 0.f);
+      // (elements of the last vector past m are padding, whatever it holds)
+      whole[4 * u] = v.x;
+      whole[4 * u + 1] = col0 + 4 * u + 1 < p.m ? v.y : 0.f;
+      whole[4 * u + 2] = col0 + 4 * u + 2 < p.m ? v.z : 0.f;
+      whole[4 * u + 3] = col0 + 4 * u + 3 < p.m ? v.w : 0.f;
+    }
+    if (ok) ok = mbar_wait(loaded, 0, abort_flag, p.status, 413);
+    ok = __syncthreads_and(ok);
+    if (work && !ok && threadIdx.x == 0) drain_copies(loaded, 1, 1);
+  }
   float q_unscale = 1.f;                                 // 1 / 2^k of Q's terms
   for (int s = 0; s < p.steps; ++s) {
     const ChainStep& c = p.step[s];
     uint8_t* into = s == 0 ? slot_q : slot_b;            // the first B is Q
     multiply(slot_r, slot_r);
     float r[32];
-    take(r);
+    take(r, 0);
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       float v[8];
@@ -836,7 +889,7 @@ ns_chain_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_constant
     if (s > 0) {
       multiply(slot_b, slot_q);
       const float b_unscale = 1.f / c.sq_scale;          // (powers of two)
-      take(r);
+      take(r, 0);
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         float q[8], b[8];
@@ -856,7 +909,7 @@ ns_chain_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_constant
     for (int twice = 0; twice < 2; ++twice) {            // W in the place of A, then A in the place of W
       const float acc = twice ? c.a_acc : c.w_acc, own = twice ? c.a_w : c.w_a, scale = twice ? c.a_scale : c.w_scale;
       multiply(left, slot_r);
-      take(r);
+      take(r, 0);
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         float v[8];
@@ -884,7 +937,7 @@ ns_chain_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_constant
   __syncthreads();
   if (warp == 0) {
     tc_fence_after_sync();
-    tmem_dealloc(tmem, 256);
+    tmem_dealloc(tmem, 512);
   }
 }
 
@@ -1130,7 +1183,18 @@ static int product(const CUtensorMap& ta, const CUtensorMap& tb, Params p, cudaS
   return bn == 256 ? launch<MODE, 256, WHOLE>(ta, tb, p, g, st) : launch<MODE, 128, WHOLE>(ta, tb, p, g, st);
 }
 
-static int chain(const CUtensorMap& ta, const Chain& c, cudaStream_t st) {
+// Whether ns_chain_kernel forms A = X X^T itself: its one CTA takes 2700 clocks for 128 columns of X; a launch of its own 1080
+// for 64 of them, shared by as many CTAs as there are SMs to a matrix, 8 at most, and 21000 besides (its start, the parts' meeting
+// and A's way through memory).  Five steps, own launch / here, us: 128 x 128 87.7 / 66.3, 128 x 896 88.2 / 82.3, 128 x 2048
+// 91.9 / 107.3, 100 of 128 x 4864 618 / 608.
+static bool folds(int n, int batch) {
+  const int kblocks = (n + BK - 1) / BK;
+  int s = 1;
+  while (s < 8 && kblocks >= 4 * s && (long long)batch * s * 2 <= sm_count()) s *= 2;
+  return (n + 127) / 128 * 2700 <= kblocks * 1080 / s + 21000;
+}
+
+static int chain(const CUtensorMap& ta, const CUtensorMap& tx, const Chain& c, cudaStream_t st) {
   static unsigned long long configured = 0;
   if (int r = smem_opt_in(ns_chain_kernel, CHAIN_SMEM, configured)) return r;
   cudaLaunchConfig_t cfg = {};
@@ -1139,7 +1203,7 @@ static int chain(const CUtensorMap& ta, const Chain& c, cudaStream_t st) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.gridDim = dim3((unsigned)c.batch); cfg.blockDim = dim3(CHAIN_THREADS); cfg.dynamicSmemBytes = CHAIN_SMEM; cfg.stream = st;
   cfg.attrs = attr; cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, ns_chain_kernel, ta, c);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, ns_chain_kernel, ta, tx, c);
   return e == cudaSuccess ? (int)cudaGetLastError() : (int)e;
 }
 
@@ -1227,6 +1291,7 @@ extern "C" int gb_newton_schulz(const void* src, void* out, int dt, int m, int n
   p.out = out; p.out_dtype = dt; p.tall = tall; p.weights = weights; p.lr = lr; p.decay = decay; p.tall_scale = tall_scale;
   p.dyn_lr = dyn_lr; p.found_inf = found_inf;
   int cur = 0;
+  bool fold = false;
   for (int i = 0; i < count; ++i) {
     const int kind = (int)program[12 * i];
     p.problems = kind == 2 && i + 1 < count ? 2 : 1;
@@ -1247,13 +1312,15 @@ extern "C" int gb_newton_schulz(const void* src, void* out, int dt, int m, int n
     } else {
       p.k = kind == 0 ? n : m;
       if (kind == 0) p.prob[0].left = p.prob[0].right = 0;
-      r = kind == 0 ? ns::product<ns::SYM>(mx[cur], mx[cur], p, st) : ns::product<ns::SYM>(ms, ms, p, st);
+      fold = kind == 0 && m <= 128 && ns::folds(n, batch);
+      r = fold ? 0 : kind == 0 ? ns::product<ns::SYM>(mx[cur], mx[cur], p, st) : ns::product<ns::SYM>(ms, ms, p, st);
     }
     if (r != 0) return r;
     if (kind == 0 && m <= 128) {
       // the rows up to the next X at once; a row is told by its result and operands
       ns::Chain c = {};
       c.status = status; c.m = m; c.batch = batch; c.lda = lda; c.a = w.whole;
+      c.blocks = fold ? (n + 127) / 128 : 0; c.gram = p.prob[0].f_acc; c.gram_scale = p.prob[0].scale;
       for (++i; i < count && program[12 * i] != 3.0; ++i) {
         const double* o = program + 12 * i;
         const int out_slot = (int)o[3];
@@ -1271,7 +1338,7 @@ extern "C" int gb_newton_schulz(const void* src, void* out, int dt, int m, int n
       }
       if (i == count || c.steps == 0) return -3;
       c.q = w.terms + (size_t)program[12 * i + 1] * batch * 2 * m * lda;
-      if ((r = ns::chain(ms, c, st)) != 0) return r;
+      if ((r = ns::chain(ms, mx[cur], c, st)) != 0) return r;
       --i;                                               // (the loop goes on with the row of the next X)
     }
   }

@@ -64,6 +64,19 @@ def test_large_and_many(shape):
     assert float(err.max()) < TOL, err
 
 
+@pytest.mark.parametrize("shape", [(1, 100, 250), (2, 128, 380), (1, 77, 500), (3, 128, 641), (1, 1100, 96), (1, 128, 1500),
+                                   (1, 30, 2900), (149, 100, 1300), (160, 24, 4100)])
+def test_short_sides(shape):
+    """Up to 128 rows: A from one to 33 blocks of the long side by the CTA that goes on with it, or by a launch of its own."""
+    x = matrix(*shape, kind="low").cuda()
+    with K.strict_native():
+        o = genesis.optim.orthogonalize(T(x))
+        again = genesis.optim.orthogonalize(T(x))
+    err = torch.linalg.matrix_norm(o._t.double() - iterated(x))
+    assert float(err.max()) < TOL, err
+    assert torch.equal(o._t, again._t)
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("shape", [(60, 90), (90, 60), (2, 131, 77), (1, 7)])
 def test_types(shape, dtype):
