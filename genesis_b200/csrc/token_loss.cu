@@ -176,10 +176,11 @@ __device__ __forceinline__ bool counts(const TI* tokens, long long r, long long 
 
 // One row's results, by one thread
 template <typename T, typename TI>
-__device__ __forceinline__ void finish_row(MaxSum a, const T* p, long long t, long long r, long long rows, float temperature,
+__device__ __forceinline__ void finish_row(MaxSum a, const T* p, long long t, long long r, long long rows, double temperature,
                                            float* lp_out, float* stats, const Policy& q) {
-  // In 64 bits and rounded once.  Differences come before products: z[t] - m is small where the token is likely.
-  const float lp = (float)(((double)Cvt<T>::to_f(p[t]) - (double)a.m) / (double)temperature - log((double)a.s));
+  // In 64 bits and rounded once; the temperature too, which rounded would shift every row by up to 6e-8 of its exponent.
+  // Differences come before products: z[t] - m is small where the token is likely.
+  const float lp = (float)(((double)Cvt<T>::to_f(p[t]) - (double)a.m) / temperature - log((double)a.s));
   lp_out[r] = lp;
   stats[r] = a.m;
   stats[rows + r] = log2f(a.s);
@@ -210,7 +211,7 @@ __device__ __forceinline__ void skip_row(long long r, long long rows, float* lp_
 template <typename T, typename TI>
 __global__ void __launch_bounds__(256)
 token_rows_warp_kernel(const T* __restrict__ z, RowMap map, const TI* __restrict__ tokens, float* __restrict__ lp,
-                       float* __restrict__ stats, long long rows, int cols, long long ignore, float temperature, Scale c,
+                       float* __restrict__ stats, long long rows, int cols, long long ignore, double temperature, Scale c,
                        Policy q, int* status) {
   const int lane = threadIdx.x & 31;
   const long long r = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
@@ -224,7 +225,7 @@ token_rows_warp_kernel(const T* __restrict__ z, RowMap map, const TI* __restrict
     return;
   }
   const T* p = z + map.at(r);
-  const MaxSum a = warp_join(scan<T, 32, 4>(p, cols, c, lane), temperature);
+  const MaxSum a = warp_join(scan<T, 32, 4>(p, cols, c, lane), (float)temperature);
   if (lane == 0) finish_row<T, TI>(a, p, t, r, rows, temperature, lp, stats, q);
 }
 
@@ -233,7 +234,7 @@ token_rows_warp_kernel(const T* __restrict__ z, RowMap map, const TI* __restrict
 template <typename T, typename TI, int G, int U, int OCC>
 __global__ void __launch_bounds__(G, OCC)
 token_rows_kernel(const T* __restrict__ z, RowMap map, const TI* __restrict__ tokens, float* __restrict__ lp,
-                  float* __restrict__ stats, long long rows, int cols, long long ignore, float temperature, Scale c,
+                  float* __restrict__ stats, long long rows, int cols, long long ignore, double temperature, Scale c,
                   Policy q, int* status, int parts) {
   __shared__ float2 sh[G / 32];
   __shared__ float2 mine;
@@ -254,13 +255,13 @@ token_rows_kernel(const T* __restrict__ z, RowMap map, const TI* __restrict__ to
     lo = min(part * step, cols);
     n = min(step, cols - lo);
   }
-  MaxSum a = warp_join(scan<T, G, U>(p + lo, n, c, threadIdx.x), temperature);
+  MaxSum a = warp_join(scan<T, G, U>(p + lo, n, c, threadIdx.x), (float)temperature);
   if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = make_float2(a.m, a.s);
   __syncthreads();
   if (threadIdx.x < 32) {
     a = MaxSum{-INFINITY, 0.f};
     if (threadIdx.x < G / 32) a = MaxSum{sh[threadIdx.x].x, sh[threadIdx.x].y};
-    a = warp_join(a, temperature);
+    a = warp_join(a, (float)temperature);
   }
   if (parts > 1) {
     cg::cluster_group cl = cg::this_cluster();
@@ -269,10 +270,10 @@ token_rows_kernel(const T* __restrict__ z, RowMap map, const TI* __restrict__ to
     if (part == 0 && threadIdx.x == 0) {
       float m = a.m;
       for (int k = 1; k < parts; ++k) m = fmaxf(m, cl.map_shared_rank(&mine, k)->x);
-      float sum = rescale(a, m, temperature);
+      float sum = rescale(a, m, (float)temperature);
       for (int k = 1; k < parts; ++k) {
         const float2 o = *cl.map_shared_rank(&mine, k);
-        sum += rescale(MaxSum{o.x, o.y}, m, temperature);
+        sum += rescale(MaxSum{o.x, o.y}, m, (float)temperature);
       }
       a = MaxSum{m, sum};
     }
@@ -445,7 +446,7 @@ __device__ __forceinline__ void zero_part(T* d, int n, int tid) {
 template <typename T, typename TI, int G>
 __global__ void __launch_bounds__(BWD_THREADS)
 token_grad_kernel(const T* __restrict__ z, RowMap map, const TI* __restrict__ tokens, const float* __restrict__ stats,
-                  T* __restrict__ dz, long long rows, int cols, long long ignore, float temperature, float c, Factor fac,
+                  T* __restrict__ dz, long long rows, int cols, long long ignore, float inv_temperature, float c, Factor fac,
                   int chunk, int chunks) {
   const int tid = threadIdx.x % G;
   const long long item = (long long)blockIdx.x * (BWD_THREADS / G) + threadIdx.x / G;
@@ -455,15 +456,15 @@ token_grad_kernel(const T* __restrict__ z, RowMap map, const TI* __restrict__ to
   const int n = min(chunk, cols - lo);
   T* d = dz + r * cols + lo;
   long long t;
-  const float f = counts(tokens, r, cols, ignore, t) ? fac.at(r) / temperature : 0.f;
+  const float f = counts(tokens, r, cols, ignore, t) ? fac.at(r) * inv_temperature : 0.f;
   if (f == 0.f) { zero_part<T, G>(d, n, tid); return; }
   grad_part<T, G>(z + map.at(r) + lo, d, n, t - lo, stats[r], stats[rows + r], c, f, tid);
 }
 
 template <typename T, typename TI>
 static int rows_forward(const void* z, RowMap map, const void* tokens, float* lp, float* stats, long long rows, int cols,
-                        long long ignore, float temperature, const Policy& q, int* status, cudaStream_t st) {
-  const Scale c((double)temperature);
+                        long long ignore, double temperature, const Policy& q, int* status, cudaStream_t st) {
+  const Scale c(temperature);
   const long long bytes = (long long)cols * sizeof(T), sms = sm_count();
   // A warp a row up to 8 KB, 128 threads up to 32 KB, as long as these fill the device
   if (bytes <= 2048 || (bytes <= 8192 && rows >= 32 * sms)) {
@@ -501,25 +502,25 @@ static int rows_forward(const void* z, RowMap map, const void* tokens, float* lp
 
 template <typename T, typename TI>
 static int rows_backward(const void* z, RowMap map, const void* tokens, const float* stats, void* dz, long long rows, int cols,
-                         long long ignore, float temperature, const Factor& fac, cudaStream_t st) {
-  const float c = (float)(1.4426950408889634 / (double)temperature);
+                         long long ignore, double temperature, const Factor& fac, cudaStream_t st) {
+  const float c = (float)(1.4426950408889634 / temperature), inv = (float)(1.0 / temperature);
   if ((long long)cols * sizeof(T) <= 8192 && (cols <= 1024 || rows >= 32ll * sm_count())) {
     token_grad_kernel<T, TI, 32><<<(unsigned)((rows + 7) / 8), BWD_THREADS, 0, st>>>(
-        (const T*)z, map, (const TI*)tokens, stats, (T*)dz, rows, cols, ignore, temperature, c, fac, cols, 1);
+        (const T*)z, map, (const TI*)tokens, stats, (T*)dz, rows, cols, ignore, inv, c, fac, cols, 1);
     return (int)cudaGetLastError();
   }
   const int chunk = 16384 / (int)sizeof(T) * 2;
   const int chunks = (cols + chunk - 1) / chunk;
   if (rows * chunks > 0x7fffffffll) return -3;
   token_grad_kernel<T, TI, BWD_THREADS><<<(unsigned)(rows * chunks), BWD_THREADS, 0, st>>>(
-      (const T*)z, map, (const TI*)tokens, stats, (T*)dz, rows, cols, ignore, temperature, c, fac, chunk, chunks);
+      (const T*)z, map, (const TI*)tokens, stats, (T*)dz, rows, cols, ignore, inv, c, fac, chunk, chunks);
   return (int)cudaGetLastError();
 }
 
 static int rows_any(const void* z, const void* tokens, float* lp, float* stats, long long rows, long long cols, RowMap map,
-                    long long ignore, float temperature, const Policy& q, int dt, int token_i64, int* status, cudaStream_t st) {
+                    long long ignore, double temperature, const Policy& q, int dt, int token_i64, int* status, cudaStream_t st) {
   if (rows == 0) return 0;
-  if (cols < 1 || cols > 0x7fffffffll || rows > 0x0fffffffll || map.inner < 1 || !(temperature > 0.f)) return -3;
+  if (cols < 1 || cols > 0x7fffffffll || rows > 0x0fffffffll || map.inner < 1 || !(temperature > 0.0)) return -3;
   if (token_i64) GB_DISPATCH_FLOAT(dt, T, return (rows_forward<T, long long>(z, map, tokens, lp, stats, rows, (int)cols, ignore, temperature, q, status, st)));
   GB_DISPATCH_FLOAT(dt, T, return (rows_forward<T, int>(z, map, tokens, lp, stats, rows, (int)cols, ignore, temperature, q, status, st)));
 }
@@ -531,7 +532,7 @@ using namespace gb;
 
 // Log-probabilities lp [rows] of `tokens` and the rows' (max, log2 sum) in stats [2, rows].  Rows: see RowMap.
 extern "C" int gb_token_rows(const void* z, const void* tokens, float* lp, float* stats, long long rows, long long cols,
-                             long long inner, long long s_outer, long long s_inner, long long ignore, float temperature,
+                             long long inner, long long s_outer, long long s_inner, long long ignore, double temperature,
                              int dt, int token_i64, int* status, cudaStream_t st) {
   return tl::rows_any(z, tokens, lp, stats, rows, cols, tl::RowMap{inner, s_outer, s_inner}, ignore, temperature, tl::Policy{},
                       dt, token_i64, status, st);
@@ -540,7 +541,7 @@ extern "C" int gb_token_rows(const void* z, const void* tokens, float* lp, float
 // The same, and every row's clipped policy loss [rows] and its derivative by lp, coef [rows]; out (or null) receives the sum
 // of the losses (over the number of rows that count with `mean`), factor that of their gradients.
 extern "C" int gb_policy_loss(const void* z, const void* tokens, float* lp, float* stats, long long rows, long long cols,
-                              long long inner, long long s_outer, long long s_inner, long long ignore, float temperature,
+                              long long inner, long long s_outer, long long s_inner, long long ignore, double temperature,
                               const float* old, const float* adv, const float* ref, float* loss, float* coef, long long adv_div,
                               float lo, float hi, float kl, float* out, float* factor, int mean, int dt, int token_i64, int* status,
                               cudaStream_t st) {
@@ -560,7 +561,7 @@ extern "C" int gb_preference_loss(const void* z, const void* tokens, float* lp, 
                                   long long inner, long long s_outer, long long s_inner, long long ignore, const float* ref,
                                   long long pairs, float beta, float smooth, int mean, float* loss_each, float* out,
                                   float* rewards, float* gseq, int dt, int token_i64, int* status, cudaStream_t st) {
-  if (const int e = tl::rows_any(z, tokens, lp, stats, rows, cols, tl::RowMap{inner, s_outer, s_inner}, ignore, 1.f, tl::Policy{},
+  if (const int e = tl::rows_any(z, tokens, lp, stats, rows, cols, tl::RowMap{inner, s_outer, s_inner}, ignore, 1.0, tl::Policy{},
                                  dt, token_i64, status, st)) return e;
   tl::preference_kernel<<<1, 1024, 0, st>>>(lp, ref, pairs, pairs > 0 ? rows / (2 * pairs) : 0, beta, smooth, mean, loss_each, out,
                                             rewards, gseq);
@@ -569,12 +570,12 @@ extern "C" int gb_preference_loss(const void* z, const void* tokens, float* lp, 
 
 // Gradient dz [rows, cols] (contiguous); a row's factor: see Factor.
 extern "C" int gb_token_grad(const void* z, const void* tokens, const float* stats, void* dz, long long rows, long long cols,
-                             long long inner, long long s_outer, long long s_inner, long long ignore, float temperature,
+                             long long inner, long long s_outer, long long s_inner, long long ignore, double temperature,
                              const float* base, long long base_div, const float* g, long long g_div, long long g_mod,
                              const float* dev_scale, float scale, int dt, int token_i64, cudaStream_t st) {
   if (rows == 0) return 0;
   if (cols < 1 || cols > 0x7fffffffll || rows > 0x0fffffffll || inner < 1 || base_div < 1 || g_div < 1 || g_mod < 1 ||
-      !(temperature > 0.f)) return -3;
+      !(temperature > 0.0)) return -3;
   const tl::RowMap map{inner, s_outer, s_inner};
   const tl::Factor fac{base, g, dev_scale, base_div, g_div, g_mod, scale};
   if (token_i64) GB_DISPATCH_FLOAT(dt, T, return (tl::rows_backward<T, long long>(z, map, tokens, stats, dz, rows, (int)cols, ignore, temperature, fac, st)));

@@ -68,10 +68,10 @@ _SIGS = {
     "gb_index_put": "pp" + "d" + "ii" + "ppp" + "i" + "pp",
     "gb_cast_stack": "ppipip",
     "gb_masked_fill": "pp" + "d" + "ll" + "i" + "p", "gb_fill_elems": "pldip",
-    "gb_token_rows": "pppp" + "lllll" + "l" + "f" + "ii" + "pp",
-    "gb_policy_loss": "pppp" + "lllll" + "l" + "f" + "ppppp" + "l" + "fff" + "pp" + "iii" + "pp",
+    "gb_token_rows": "pppp" + "lllll" + "l" + "d" + "ii" + "pp",
+    "gb_policy_loss": "pppp" + "lllll" + "l" + "d" + "ppppp" + "l" + "fff" + "pp" + "iii" + "pp",
     "gb_preference_loss": "pppp" + "lllll" + "l" + "p" + "l" + "ff" + "i" + "pppp" + "ii" + "pp",
-    "gb_token_grad": "pppp" + "lllll" + "l" + "f" + "pl" + "pll" + "p" + "f" + "ii" + "p",
+    "gb_token_grad": "pppp" + "lllll" + "l" + "d" + "pl" + "pll" + "p" + "f" + "ii" + "p",
     "gb_ns_workspace": "lllip", "gb_muon_momentum": "p" + "iiii" + "f" + "i" + "ppp" + "p",
     "gb_newton_schulz": "pp" + "iiiii" + "p" + "i" + "d" + "p" + "fff" + "pp" + "pp" + "p",
 }

@@ -216,6 +216,19 @@ def test_masked_vocabulary_and_extremes(dtype, V):
     assert d[0, 0, 20] == 1 and not d[0, 2, : V // 2].any() and not d[0, 3:].any()
 
 
+@pytest.mark.parametrize("temperature", [0.7, 1.3])
+def test_mean_error_at_a_temperature(temperature):
+    """0.7 rounded to 32 bits is 1.7e-8 off, which would shift log-probabilities of -30 by 5e-7, all the same way.  What is left:
+    the hardware exponential is off by less than 1e-7 on average, and the mean of 8000 roundings of up to 2^-19 (of
+    log-probabilities below 64) by 4 * 2^-19 / sqrt(3 * 8000) = 5e-8 at four standard deviations."""
+    g, z, t = make((2, 4000), 300, 13, ignored=0.0, std=6.0)
+    with genesis.no_grad():
+        lp = F.token_log_probs(*dev(z, t), temperature=temperature)
+    ref, _ = R.log_probs(z.double(), t, temperature)
+    assert -64 < float(ref.min()) < float(ref.mean()) < -12
+    assert abs(float((lp._t.cpu().double() - ref).mean())) < 1.5e-7
+
+
 def test_kl_of_a_policy_near_its_reference():
     """lp is off by 4e-6 at most (its rounding at |lp| < 32 2^-19, the row's log-sum 2e-6), ref by its rounding 2e-6, d by
     both, and exp(d) - 1 - d by |d| of it; exp(d) - 1 has 2^-22 of its own; the loss's rounding 2^-23.  A difference of
