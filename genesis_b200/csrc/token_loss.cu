@@ -1,7 +1,7 @@
 // Losses on a language model's logits that need only the log-probability of one token per row: log-probabilities
 // themselves, the clipped policy objective with its KL term, the loss of paired log ratios.
 //
-//   row:         m = max z,  s = sum exp((z - m) / T),  lp = (z[t] - m) / T - log s
+//   row:         m near max z,  s = sum exp((z - m) / T),  lp = (z[t] - m) / T - log s
 //   policy:      r = exp(lp - old),  l = max(-A r, -A clamp(r, 1 - c, 1 + c')) + k (exp(ref - lp) - (ref - lp) - 1)
 //                dl/dlp = (-A r where the unclipped term is the larger, else 0) + k (1 - exp(ref - lp))
 //   preference:  S = sum lp over an answer,  h = beta ((S_c - ref_c) - (S_r - ref_r)),
@@ -10,9 +10,9 @@
 //
 // Three kinds of kernels: one reads every row that counts once and keeps (m, log2 s) of it; one block joins the rows
 // into the loss, in a fixed order and in 64 bits (the sum of an answer's log-probabilities runs into the thousands, its
-// difference to the reference's is of order one); one writes the gradient.  Nothing of the size of the logits is kept
-// between the two passes but the logits.  A row that does not count (its token is the ignored index) is not read, so
-// whatever it holds reaches nothing, and its gradient is zero.
+// difference to the reference's is of order one; there the log-probabilities too are kept in 64 bits); one writes the
+// gradient.  Nothing of the size of the logits is kept between the two passes but the logits.  A row that does not count (its
+// token is the ignored index) is not read, so whatever it holds reaches nothing, and its gradient is zero.
 #include <cooperative_groups.h>
 #include "sm100_ptx.cuh"
 #include "common.cuh"
@@ -38,6 +38,7 @@ struct Policy {
   float* coef;                 // [rows] dl/dlp
   long long adv_div;
   float lo, hi, kl;            // 1 - c, 1 + c', k
+  double* wide;                // [rows] log-probabilities as they are before they are rounded, in place of lp; or null
 };
 
 struct MaxSum { float m, s; };
@@ -46,12 +47,14 @@ struct MaxSum { float m, s; };
 // (z - m) / T, and the sum of an answer's log-probabilities by their number times that.  The high part is rounded down, so
 // that the low one is positive and -inf times either is -inf.
 struct Scale {
-  float hi, lo;
+  float hi, lo, inv, slack;    // inv: 1 / T; slack: what a factor of 2 is among the logits
   explicit Scale(double temperature) {
     const double c = 1.4426950408889634 / temperature;
     hi = (float)c;
     if ((double)hi >= c) hi = nextafterf(hi, 0.f);
     lo = (float)(c - (double)hi);
+    inv = (float)(1.0 / temperature);
+    slack = (float)(1.0 / c);
   }
   __device__ __forceinline__ float operator()(float d) const { return fmaf(d, hi, d * lo); }
 };
@@ -111,14 +114,18 @@ template <typename T, int G, int U>
 __device__ __forceinline__ MaxSum scan(const T* p, int n, const Scale& c, int t) {
   constexpr int V = 16 / sizeof(T), H = V / 2;
   MaxSum a{-INFINITY, 0.f};
+  // The maximum follows when a term passes 2: that is seldom after a thread's first vectors.
   auto raise = [&](float mx) {
-    if (mx > a.m) { a.s *= ex2(c(a.m - mx)); a.m = mx; }
+    if (mx > a.m + c.slack) { a.s *= expf((a.m - mx) * c.inv); a.m = mx; }   // (see rescale)
   };
   auto one = [&](T x) {
     const float z = Cvt<T>::to_f(x);
     raise(z);
     if (z != -INFINITY) a.s += ex2(c(z - a.m));                    // (NaN comes through: NaN - m)
   };
+  // The hardware's exponential is 5e-8 of its result too small on average for negative arguments (2e-8 above -1) and 3.4e-8 too
+  // large for positive ones (above 1).  So one of two neighbours is taken times 2^6: the errors of a sum cancel, where
+  // they shifted the log-probabilities of rows of 151936 by 2.8e-8 each, all the same way.
   const float2 hi = make_float2(c.hi, c.hi), lo = make_float2(c.lo, c.lo);
   auto add = [&](const uint4& v) {
     float2 f[H], sum = make_float2(0.f, 0.f);
@@ -129,10 +136,11 @@ __device__ __forceinline__ MaxSum scan(const T* p, int n, const Scale& c, int t)
     for (int i = 0; i < H; ++i) {
       const float2 d = add2(f[i], nm);
       float2 e = fma2(d, hi, mul2(d, lo));
+      e.y += 6.f;
       e.x = ex2(e.x); e.y = ex2(e.y);
       sum = add2(sum, e);
     }
-    a.s += sum.x + sum.y;
+    a.s += fmaf(sum.y, 0.015625f, sum.x);
   };
   const int mis = (int)((reinterpret_cast<uintptr_t>(p) & 15) / sizeof(T));
   int head = mis ? V - mis : 0;
@@ -180,8 +188,10 @@ __device__ __forceinline__ void finish_row(MaxSum a, const T* p, long long t, lo
                                            float* lp_out, float* stats, const Policy& q) {
   // In 64 bits and rounded once; the temperature too, which rounded would shift every row by up to 6e-8 of its exponent.
   // Differences come before products: z[t] - m is small where the token is likely.
-  const float lp = (float)(((double)Cvt<T>::to_f(p[t]) - (double)a.m) / temperature - log((double)a.s));
-  lp_out[r] = lp;
+  const double wide = ((double)Cvt<T>::to_f(p[t]) - (double)a.m) / temperature - log((double)a.s);
+  const float lp = (float)wide;
+  if (q.wide != nullptr) q.wide[r] = wide;
+  else lp_out[r] = lp;
   stats[r] = a.m;
   stats[rows + r] = log2f(a.s);
   if (q.old != nullptr) {
@@ -201,7 +211,8 @@ __device__ __forceinline__ void finish_row(MaxSum a, const T* p, long long t, lo
 }
 
 __device__ __forceinline__ void skip_row(long long r, long long rows, float* lp_out, float* stats, const Policy& q) {
-  lp_out[r] = 0.f;
+  if (q.wide != nullptr) q.wide[r] = 0.0;
+  else lp_out[r] = 0.f;
   stats[r] = 0.f;
   stats[rows + r] = 0.f;
   if (q.old != nullptr) { q.loss[r] = 0.f; q.coef[r] = 0.f; }
@@ -317,15 +328,15 @@ policy_sum_kernel(const float* __restrict__ loss, const TI* __restrict__ tokens,
 // Pair i: answers i (chosen) and pairs + i (rejected) of `len` rows each.  loss_each [pairs] or null; out[0] = their sum
 // (or mean); rewards [2 pairs] = beta (S - ref); gseq [2 pairs] = dl/dS.
 __global__ void __launch_bounds__(1024)
-preference_kernel(const float* __restrict__ lp, const float* __restrict__ ref, long long pairs, long long len, float beta,
+preference_kernel(const double* __restrict__ lp, const float* __restrict__ ref, long long pairs, long long len, float beta,
                   float smooth, int mean, float* __restrict__ loss_each, float* __restrict__ out, float* __restrict__ rewards,
                   float* __restrict__ gseq) {
   __shared__ double sh[32];
   const int lane = threadIdx.x & 31;
   for (long long s = threadIdx.x >> 5; s < 2 * pairs; s += 32) {
-    const float* p = lp + s * len;
+    const double* p = lp + s * len;
     double sum = 0.0;
-    for (long long i = lane; i < len; i += 32) sum += (double)p[i];
+    for (long long i = lane; i < len; i += 32) sum += p[i];
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (lane == 0) rewards[s] = (float)((double)beta * (sum - (double)ref[s]));
@@ -493,7 +504,8 @@ static int rows_forward(const void* z, RowMap map, const void* tokens, float* lp
     return run(token_rows_kernel<T, TI, 512, 4, 2>, 512);
   }
   // More rows: smaller CTAs, so that fewer threads wait for a row's slowest warp and the last rows spread better.  Of 151936
-  // bf16, 512 / 256 threads: 1000 rows 75.8 / 71.7, 6973 rows 367 / 352 (6.0 TB/s).  16-bit rows are bound by the exponentials
+  // bf16, 512 / 256 threads: 1000 rows 75.8 / 71.7, 6973 rows 367 / 352 (6.0 TB/s; scan's two scales
+  // make it 364).  16-bit rows are bound by the exponentials
   // as much as by memory and take all the threads that fit, with two vectors each (four and half as many threads 371);
   // 32-bit ones, with half the exponentials a byte, four (1000 rows 108 for 125).
   if (sizeof(T) == 2 && rows > 4 * sms) return run(token_rows_kernel<T, TI, 256, 2, 8>, 256);
@@ -555,14 +567,16 @@ extern "C" int gb_policy_loss(const void* z, const void* tokens, float* lp, floa
   return (int)cudaGetLastError();
 }
 
-// Log-probabilities as gb_token_rows gives them, and the loss of `pairs` pairs of answers of rows / (2 pairs) rows each: see
-// preference_kernel.
-extern "C" int gb_preference_loss(const void* z, const void* tokens, float* lp, float* stats, long long rows, long long cols,
+// Log-probabilities as gb_token_rows gives them, but in 64 bits, and the loss of `pairs` pairs of answers of rows / (2 pairs)
+// rows each: see preference_kernel.
+extern "C" int gb_preference_loss(const void* z, const void* tokens, double* lp, float* stats, long long rows, long long cols,
                                   long long inner, long long s_outer, long long s_inner, long long ignore, const float* ref,
                                   long long pairs, float beta, float smooth, int mean, float* loss_each, float* out,
                                   float* rewards, float* gseq, int dt, int token_i64, int* status, cudaStream_t st) {
-  if (const int e = tl::rows_any(z, tokens, lp, stats, rows, cols, tl::RowMap{inner, s_outer, s_inner}, ignore, 1.0, tl::Policy{},
-                                 dt, token_i64, status, st)) return e;
+  tl::Policy q{};
+  q.wide = lp;
+  if (const int e = tl::rows_any(z, tokens, nullptr, stats, rows, cols, tl::RowMap{inner, s_outer, s_inner}, ignore, 1.0, q, dt,
+                                 token_i64, status, st)) return e;
   tl::preference_kernel<<<1, 1024, 0, st>>>(lp, ref, pairs, pairs > 0 ? rows / (2 * pairs) : 0, beta, smooth, mean, loss_each, out,
                                             rewards, gseq);
   return (int)cudaGetLastError();

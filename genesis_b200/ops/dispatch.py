@@ -616,8 +616,8 @@ def token_logits(logits):
 
 
 def token_rows(logits, tokens, ignore_index, temperature):
-    """Log-probabilities of `tokens` [...] under `logits` [..., V] / temperature (0 where ignored), and the rows' maxima and
-    log2 of their sums [2 rows], which the gradient needs."""
+    """Log-probabilities of `tokens` [...] under `logits` [..., V] / temperature (0 where ignored), and what the gradient
+    needs of the rows [2 rows]: m, a number near the row's maximum, and log2 of the sum of exp((z - m) / temperature)."""
     if logits.is_cuda:
         r = N.token_rows(logits, tokens, ignore_index, temperature)
         if r is not NotImplemented:

@@ -1950,14 +1950,15 @@ def preference_loss(logits, tokens, ignore_index, ref, beta, smoothing, reductio
         return NotImplemented
     rows, n, dev = tokens.numel(), ref.numel(), logits.device
     each = reduction == "none"
-    buf = torch.empty(3 * rows + n + 1, dtype=F32, device=dev)
+    # statistics, derivatives, the loss where it is not asked for, and (on a boundary of 8) log-probabilities in 64 bits
+    buf = torch.empty(4 * rows + n + 2, dtype=F32, device=dev)
     out = torch.empty((n // 2,) if each else (), dtype=F32, device=dev)
     rewards = torch.empty(n, dtype=F32, device=dev)
     at, op = buf.data_ptr(), out.data_ptr()
     with _on(dev):
-        _chk(lib().gb_preference_loss(logits.data_ptr(), tokens.data_ptr(), at + 8 * rows + 4 * n, at, rows, logits.shape[-1], *m,
+        _chk(lib().gb_preference_loss(logits.data_ptr(), tokens.data_ptr(), at + 8 * rows + 4 * n + 8, at, rows, logits.shape[-1], *m,
                                       ignore_index, ref.data_ptr(), n // 2, beta, smoothing, 1 if reduction == "mean" else 0,
-                                      op if each else None, at + 12 * rows + 4 * n if each else op, rewards.data_ptr(),
+                                      op if each else None, at + 8 * rows + 4 * n if each else op, rewards.data_ptr(),
                                       at + 8 * rows, _DT[logits.dtype], 1 if tokens.dtype == torch.int64 else 0,
                                       status_tensor(dev).data_ptr(), _st()), "preference_loss")
     return out, rewards, buf
