@@ -504,12 +504,10 @@ static int rows_forward(const void* z, RowMap map, const void* tokens, float* lp
     return run(token_rows_kernel<T, TI, 512, 4, 2>, 512);
   }
   // More rows: smaller CTAs, so that fewer threads wait for a row's slowest warp and the last rows spread better.  Of 151936
-  // bf16, 512 / 256 threads: 1000 rows 75.8 / 71.7, 6973 rows 367 / 352 (6.0 TB/s; scan's two scales
-  // make it 364).  16-bit rows are bound by the exponentials
-  // as much as by memory and take all the threads that fit, with two vectors each (four and half as many threads 371);
-  // 32-bit ones, with half the exponentials a byte, four (1000 rows 108 for 125).
-  if (sizeof(T) == 2 && rows > 4 * sms) return run(token_rows_kernel<T, TI, 256, 2, 8>, 256);
-  return run(token_rows_kernel<T, TI, 256, 4, 4>, 256);
+  // bf16, 512 / 256 threads: 1000 rows 75.8 / 71.7, 6973 rows 367 / 352.  16-bit rows are bound by the exponentials as much as by
+  // memory: five CTAs of 48 registers 354 (6.0 TB/s), four of 60 385, eight of 32, which spill, with two vectors 363; of 50257
+  // fp16, 1250 rows 41.0 / 45.0 / 47.1.  32-bit rows, 2000 of 65536, in the same order: 100, 104, 107, and 1000 of 151936 125, 115, 127.
+  return run(token_rows_kernel<T, TI, 256, 4, sizeof(T) == 2 ? 5 : 4>, 256);
 }
 
 template <typename T, typename TI>
