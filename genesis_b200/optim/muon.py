@@ -155,7 +155,15 @@ class Muon(Optimizer):
             self._dyn_lr = self.lr
 
     def load_state_dict(self, state_dict):
+        kept = self.u
         super().load_state_dict(state_dict)
+        # momenta stay where they are: a captured step goes on with them
+        for i, t in kept.items():
+            if i in self.u:
+                K.copy_(t, self.u[i])
+            else:
+                K.fill_(t, 0)
+            self.u[i] = t
         self.coefficients = tuple(self.coefficients)
         self._sync_lr()
 

@@ -161,6 +161,22 @@ def test_state_dict_and_missing_gradients():
     assert torch.equal(ps[0]._t, other[0]._t)
 
 
+def test_momenta_stay_where_they_are_when_a_state_is_loaded():
+    ps = [genesis.nn.Parameter(T(matrix(4, 6, seed=i))) for i in range(3)]
+    opt = genesis.optim.Muon(ps, lr=0.1)
+    for i in (0, 1):
+        ps[i].grad = T(matrix(4, 6, seed=5 + i))
+    opt.step()
+    state = opt.state_dict()
+    saved = {i: t._t.clone() for i, t in state["u"].items()}
+    state = dict(state, u={0: T(saved[0].clone()), 2: T(saved[1].clone())})
+    held = dict(opt.u)
+    opt.step()
+    opt.load_state_dict(state)
+    assert opt.u[0] is held[0] and opt.u[1] is held[1]
+    assert torch.equal(opt.u[0], saved[0]) and not opt.u[1].any() and torch.equal(opt.u[2], saved[1])
+
+
 def test_grad_scaler_skips_overflow():
     p = genesis.nn.Parameter(T(matrix(4, 6)))
     opt = genesis.optim.Muon([p], lr=0.1)

@@ -188,6 +188,32 @@ def test_two_streams_at_once_and_a_captured_call():
         assert torch.equal(a._t, want[i]) and torch.equal(b._t, want[i - 1])
 
 
+def test_a_captured_step_goes_on_with_a_loaded_state():
+    w = matrix(3, 60, 90).cuda()
+    p = genesis.nn.Parameter(T(w.clone()))
+    x = T(torch.randn(5, 60, device="cuda"))
+    opt = genesis.optim.Muon([p], lr=0.1)
+
+    def step(x):
+        opt.zero_grad()
+        loss = (x @ p[0]).sum() + (p * p).sum()
+        loss.backward()
+        opt.step()
+        return loss
+
+    graphed = genesis.cuda.GraphedTrainStep(step, opt, [x])
+    graphed(x)
+    state = {k: ({i: T(t._t.clone()) for i, t in v.items()} if k == "u" else v) for k, v in opt.state_dict().items()}
+    at = p._t.clone()
+    graphed(x)
+    first = p._t.clone()
+    graphed(x)
+    opt.load_state_dict(state)
+    p._t.copy_(at)
+    graphed(x)
+    assert torch.equal(p._t, first)
+
+
 def test_empty_and_zero_gradients():
     ps = [genesis.nn.Parameter(T(matrix(*s).cuda())) for s in ((30, 40), (0, 40), (40, 30), (5, 6))]
     opt = genesis.optim.Muon(ps, lr=0.1, weight_decay=0.5)
