@@ -119,6 +119,7 @@ class Muon(Optimizer):
     """Momentum with orthogonalised updates, for matrices; see the module's docstring."""
 
     _fused_amp = True       # the kernels take grad_scale / found_inf device scalars (see GradScaler.step)
+    _state_stays = True
 
     def __init__(self, params, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5, coefficients=COEFFICIENTS,
                  eps=1e-7):
@@ -155,15 +156,7 @@ class Muon(Optimizer):
             self._dyn_lr = self.lr
 
     def load_state_dict(self, state_dict):
-        kept = self.u
         super().load_state_dict(state_dict)
-        # momenta stay where they are: a captured step goes on with them
-        for i, t in kept.items():
-            if i in self.u:
-                K.copy_(t, self.u[i])
-            else:
-                K.fill_(t, 0)
-            self.u[i] = t
         self.coefficients = tuple(self.coefficients)
         self._sync_lr()
 

@@ -35,6 +35,9 @@ class Optimizer:
         raise NotImplementedError
 
     _STATE_TENSORS = ("m", "v", "u")
+    # Whether loading a state writes into the buffers that are there: a captured step goes on reading and writing these
+    # (set by the first step that is captured).
+    _state_stays = False
 
     def state_dict(self):
         out = {}
@@ -56,6 +59,12 @@ class Optimizer:
                     raw = t._t if isinstance(t, Tensor) else torch.as_tensor(t)
                     p = self.params[int(i)]._t
                     cur[int(i)] = raw.to(device=p.device, dtype=torch.float32).clone()
+                for i, t in (getattr(self, k, {}) if self._state_stays else {}).items():
+                    if i in cur:
+                        K.copy_(t, cur[i])
+                    else:
+                        K.fill_(t, 0)
+                    cur[i] = t
                 setattr(self, k, cur)
             elif k != "params":
                 setattr(self, k, v)
@@ -76,6 +85,8 @@ class Optimizer:
                     torch.autograd.graph.increment_version(t)
                 except AttributeError:
                     break
+        if ps[0].is_cuda and torch.cuda.is_current_stream_capturing():
+            self._state_stays = True
         ents = getattr(self, "_shadow_entries", None)
         if ents:
             for i in idx:
