@@ -326,11 +326,12 @@ policy_sum_kernel(const float* __restrict__ loss, const TI* __restrict__ tokens,
 }
 
 // Pair i: answers i (chosen) and pairs + i (rejected) of `len` rows each.  loss_each [pairs] or null; out[0] = their sum
-// (or mean); rewards [2 pairs] = beta (S - ref); gseq [2 pairs] = dl/dS.
+// (or mean); rewards [2 pairs] = beta (S - ref); gseq [2 pairs] = dl/dS.  Everything is in 64 bits until it goes out: rewards
+// may be large where their difference is of order one, so that is formed from `wide` [2 pairs], rewards before they are rounded.
 __global__ void __launch_bounds__(1024)
-preference_kernel(const double* __restrict__ lp, const float* __restrict__ ref, long long pairs, long long len, float beta,
-                  float smooth, int mean, float* __restrict__ loss_each, float* __restrict__ out, float* __restrict__ rewards,
-                  float* __restrict__ gseq) {
+preference_kernel(const double* __restrict__ lp, const float* __restrict__ ref, long long pairs, long long len, double beta,
+                  double smooth, int mean, float* __restrict__ loss_each, float* __restrict__ out, float* __restrict__ rewards,
+                  double* __restrict__ wide, float* __restrict__ gseq) {
   __shared__ double sh[32];
   const int lane = threadIdx.x & 31;
   for (long long s = threadIdx.x >> 5; s < 2 * pairs; s += 32) {
@@ -339,23 +340,26 @@ preference_kernel(const double* __restrict__ lp, const float* __restrict__ ref, 
     for (long long i = lane; i < len; i += 32) sum += p[i];
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane == 0) rewards[s] = (float)((double)beta * (sum - (double)ref[s]));
+    if (lane == 0) {
+      wide[s] = beta * (sum - (double)ref[s]);
+      rewards[s] = (float)wide[s];
+    }
   }
   __syncthreads();
   double total = 0.0;
   for (long long i = threadIdx.x; i < pairs; i += 1024) {
-    const float h = rewards[i] - rewards[pairs + i];
+    const double h = wide[i] - wide[pairs + i];
     // log(1 + exp(-|h|)) is common to both signs: -log sigmoid(h) = max(-h, 0) + it
-    const float l1 = log1pf(expf(-fabsf(h)));
+    const double l1 = log1p(exp(-fabs(h)));
     // a side of weight 0 is left out: h is infinite where an answer holds a token of probability 0
-    float loss = h != h ? h : 0.f;
-    if (smooth < 1.f) loss += (1.f - smooth) * (fmaxf(-h, 0.f) + l1);
-    if (smooth > 0.f) loss += smooth * (fmaxf(h, 0.f) + l1);
-    const float g = beta * (smooth - 1.f / (1.f + expf(h)));
+    double loss = h != h ? h : 0.0;
+    if (smooth < 1.0) loss += (1.0 - smooth) * (fmax(-h, 0.0) + l1);
+    if (smooth > 0.0) loss += smooth * (fmax(h, 0.0) + l1);
+    const float g = (float)(beta * (smooth - 1.0 / (1.0 + exp(h))));
     gseq[i] = g;
     gseq[pairs + i] = -g;
-    if (loss_each != nullptr) loss_each[i] = loss;
-    total += (double)loss;
+    if (loss_each != nullptr) loss_each[i] = (float)loss;
+    total += loss;
   }
   total = block_sum64(total, sh);
   if (threadIdx.x == 0) out[0] = (float)(mean && pairs > 0 ? total / (double)pairs : total);
@@ -566,17 +570,17 @@ extern "C" int gb_policy_loss(const void* z, const void* tokens, float* lp, floa
 }
 
 // Log-probabilities as gb_token_rows gives them, but in 64 bits, and the loss of `pairs` pairs of answers of rows / (2 pairs)
-// rows each: see preference_kernel.
+// rows each, in 64 bits too (`wide` [2 pairs] is room for them): see preference_kernel.
 extern "C" int gb_preference_loss(const void* z, const void* tokens, double* lp, float* stats, long long rows, long long cols,
                                   long long inner, long long s_outer, long long s_inner, long long ignore, const float* ref,
-                                  long long pairs, float beta, float smooth, int mean, float* loss_each, float* out,
-                                  float* rewards, float* gseq, int dt, int token_i64, int* status, cudaStream_t st) {
+                                  long long pairs, double beta, double smooth, int mean, float* loss_each, float* out,
+                                  float* rewards, double* wide, float* gseq, int dt, int token_i64, int* status, cudaStream_t st) {
   tl::Policy q{};
   q.wide = lp;
   if (const int e = tl::rows_any(z, tokens, nullptr, stats, rows, cols, tl::RowMap{inner, s_outer, s_inner}, ignore, 1.0, q, dt,
                                  token_i64, status, st)) return e;
   tl::preference_kernel<<<1, 1024, 0, st>>>(lp, ref, pairs, pairs > 0 ? rows / (2 * pairs) : 0, beta, smooth, mean, loss_each, out,
-                                            rewards, gseq);
+                                            rewards, wide, gseq);
   return (int)cudaGetLastError();
 }
 

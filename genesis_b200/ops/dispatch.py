@@ -673,19 +673,19 @@ def preference_loss(logits, tokens, ignore_index, ref, beta, smoothing, reductio
             return r
     lp, stats = token_rows(logits, tokens, ignore_index, 1.0)
     n = ref.numel()
-    rewards = (beta * (lp.double().sum(-1) - ref.double())).to(lp.dtype)
-    h = rewards[:n // 2] - rewards[n // 2:]
+    wide = beta * (lp.double().sum(-1) - ref.double())   # (may be large where the difference of two is of order one)
+    rewards, h = wide.to(lp.dtype), wide[:n // 2] - wide[n // 2:]
     lse = torch.log1p(torch.exp(-h.abs()))
     loss = torch.where(torch.isnan(h), h, torch.zeros_like(h))
     if smoothing < 1:                                    # (h is infinite where an answer holds a token of probability 0)
         loss = loss + (1 - smoothing) * ((-h).clamp(min=0) + lse)
     if smoothing > 0:
         loss = loss + smoothing * (h.clamp(min=0) + lse)
-    g = beta * (smoothing - 1 / (1 + torch.exp(h)))
+    g = (beta * (smoothing - 1 / (1 + torch.exp(h)))).to(lp.dtype)
     stats = torch.cat((stats, g, -g))
     if reduction == "none":
-        return loss, rewards, stats
-    total = loss.double().sum()
+        return loss.to(lp.dtype), rewards, stats
+    total = loss.sum()
     return (total / (n // 2) if reduction == "mean" and n else total).to(lp.dtype), rewards, stats
 
 

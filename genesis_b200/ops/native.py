@@ -70,7 +70,7 @@ _SIGS = {
     "gb_masked_fill": "pp" + "d" + "ll" + "i" + "p", "gb_fill_elems": "pldip",
     "gb_token_rows": "pppp" + "lllll" + "l" + "d" + "ii" + "pp",
     "gb_policy_loss": "pppp" + "lllll" + "l" + "d" + "ppppp" + "l" + "fff" + "pp" + "iii" + "pp",
-    "gb_preference_loss": "pppp" + "lllll" + "l" + "p" + "l" + "ff" + "i" + "pppp" + "ii" + "pp",
+    "gb_preference_loss": "pppp" + "lllll" + "l" + "p" + "l" + "dd" + "i" + "ppppp" + "ii" + "pp",
     "gb_token_grad": "pppp" + "lllll" + "l" + "d" + "pl" + "pll" + "p" + "f" + "ii" + "p",
     "gb_ns_workspace": "lllip", "gb_muon_momentum": "p" + "iiii" + "f" + "i" + "ppp" + "p",
     "gb_newton_schulz": "pp" + "iiiii" + "p" + "i" + "d" + "p" + "fff" + "pp" + "pp" + "p",
@@ -1950,8 +1950,9 @@ def preference_loss(logits, tokens, ignore_index, ref, beta, smoothing, reductio
         return NotImplemented
     rows, n, dev = tokens.numel(), ref.numel(), logits.device
     each = reduction == "none"
-    # statistics, derivatives, the loss where it is not asked for, and (on a boundary of 8) log-probabilities in 64 bits
-    buf = torch.empty(4 * rows + n + 2, dtype=F32, device=dev)
+    # statistics, derivatives, the loss where it is not asked for, and (on a boundary of 8) log-probabilities and rewards in
+    # 64 bits
+    buf = torch.empty(4 * rows + 3 * n + 2, dtype=F32, device=dev)
     out = torch.empty((n // 2,) if each else (), dtype=F32, device=dev)
     rewards = torch.empty(n, dtype=F32, device=dev)
     at, op = buf.data_ptr(), out.data_ptr()
@@ -1959,7 +1960,7 @@ def preference_loss(logits, tokens, ignore_index, ref, beta, smoothing, reductio
         _chk(lib().gb_preference_loss(logits.data_ptr(), tokens.data_ptr(), at + 8 * rows + 4 * n + 8, at, rows, logits.shape[-1], *m,
                                       ignore_index, ref.data_ptr(), n // 2, beta, smoothing, 1 if reduction == "mean" else 0,
                                       op if each else None, at + 8 * rows + 4 * n if each else op, rewards.data_ptr(),
-                                      at + 8 * rows, _DT[logits.dtype], 1 if tokens.dtype == torch.int64 else 0,
+                                      at + 16 * rows + 4 * n + 8, at + 8 * rows, _DT[logits.dtype], 1 if tokens.dtype == torch.int64 else 0,
                                       status_tensor(dev).data_ptr(), _st()), "preference_loss")
     return out, rewards, buf
 
