@@ -326,10 +326,10 @@ policy_sum_kernel(const float* __restrict__ loss, const TI* __restrict__ tokens,
 }
 
 // Pair i: answers i (chosen) and pairs + i (rejected) of `len` rows each.  loss_each [pairs] or null; out[0] = their sum
-// (or mean); rewards [2 pairs] = beta (S - ref); gseq [2 pairs] = dl/dS.  Everything is in 64 bits until it goes out: rewards
+// (or mean); rewards [2 pairs] = beta (S - ref), ref in 32 or 64 bits; gseq [2 pairs] = dl/dS.  Everything is in 64 bits until it goes out: rewards
 // may be large where their difference is of order one, so that is formed from `wide` [2 pairs], rewards before they are rounded.
 __global__ void __launch_bounds__(1024)
-preference_kernel(const double* __restrict__ lp, const float* __restrict__ ref, long long pairs, long long len, double beta,
+preference_kernel(const double* __restrict__ lp, const void* __restrict__ ref, int ref_f64, long long pairs, long long len, double beta,
                   double smooth, int mean, float* __restrict__ loss_each, float* __restrict__ out, float* __restrict__ rewards,
                   double* __restrict__ wide, float* __restrict__ gseq) {
   __shared__ double sh[32];
@@ -341,7 +341,7 @@ preference_kernel(const double* __restrict__ lp, const float* __restrict__ ref, 
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (lane == 0) {
-      wide[s] = beta * (sum - (double)ref[s]);
+      wide[s] = beta * (sum - (ref_f64 ? reinterpret_cast<const double*>(ref)[s] : (double)reinterpret_cast<const float*>(ref)[s]));
       rewards[s] = (float)wide[s];
     }
   }
@@ -572,14 +572,14 @@ extern "C" int gb_policy_loss(const void* z, const void* tokens, float* lp, floa
 // Log-probabilities as gb_token_rows gives them, but in 64 bits, and the loss of `pairs` pairs of answers of rows / (2 pairs)
 // rows each, in 64 bits too (`wide` [2 pairs] is room for them): see preference_kernel.
 extern "C" int gb_preference_loss(const void* z, const void* tokens, double* lp, float* stats, long long rows, long long cols,
-                                  long long inner, long long s_outer, long long s_inner, long long ignore, const float* ref,
+                                  long long inner, long long s_outer, long long s_inner, long long ignore, const void* ref, int ref_f64,
                                   long long pairs, double beta, double smooth, int mean, float* loss_each, float* out,
                                   float* rewards, double* wide, float* gseq, int dt, int token_i64, int* status, cudaStream_t st) {
   tl::Policy q{};
   q.wide = lp;
   if (const int e = tl::rows_any(z, tokens, nullptr, stats, rows, cols, tl::RowMap{inner, s_outer, s_inner}, ignore, 1.0, q, dt,
                                  token_i64, status, st)) return e;
-  tl::preference_kernel<<<1, 1024, 0, st>>>(lp, ref, pairs, pairs > 0 ? rows / (2 * pairs) : 0, beta, smooth, mean, loss_each, out,
+  tl::preference_kernel<<<1, 1024, 0, st>>>(lp, ref, ref_f64, pairs, pairs > 0 ? rows / (2 * pairs) : 0, beta, smooth, mean, loss_each, out,
                                             rewards, wide, gseq);
   return (int)cudaGetLastError();
 }

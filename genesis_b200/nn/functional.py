@@ -1604,8 +1604,9 @@ def _token_args(name, logits, tokens, ignore_index, temperature=1.0):
     return K.contiguous(t)
 
 
-def _constant(name, what, x, shapes, z):
-    """A floating-point input through which no gradient flows, as contiguous numbers of the width the loss is computed in."""
+def _constant(name, what, x, shapes, z, keep_64=False):
+    """A floating-point input through which no gradient flows, as contiguous numbers of the width the loss is computed in
+    (with `keep_64`: of 64 bits where they come in 64)."""
     if not isinstance(x, Tensor) or not x._t.dtype.is_floating_point:
         raise TypeError(f"{name}: {what} must be a floating-point Tensor")
     if x.requires_grad:
@@ -1614,7 +1615,8 @@ def _constant(name, what, x, shapes, z):
         raise ValueError(f"{name}: {what} has shape {tuple(x._t.shape)}, expected {' or '.join(map(str, shapes))}")
     if x._t.device != z.device:
         raise ValueError(f"{name}: logits are on {z.device}, {what} on {x._t.device}")
-    return _as(x._t, torch.float64 if z.dtype == torch.float64 else torch.float32)
+    wide = z.dtype == torch.float64 or (keep_64 and x._t.dtype == torch.float64)
+    return _as(x._t, torch.float64 if wide else torch.float32)
 
 
 def _number(name, what, x, low, high):
@@ -1668,7 +1670,8 @@ def preference_loss(logits, tokens, ref_log_probs, beta=0.1, label_smoothing=0.0
     With S the sums of the answers' log-probabilities (tokens [2 P, T]; those equal to `ignore_index` do not count) and
     reward = beta (S - ref_log_probs [2 P]), a pair's loss is -(1 - e) log sigmoid(h) - e log sigmoid(-h) with
     h = reward(chosen) - reward(rejected) and e = label_smoothing.  "none" gives one loss per pair.  With
-    `return_rewards` also the rewards [2 P], through which no gradient flows."""
+    `return_rewards` also the rewards [2 P], through which no gradient flows.  S and what follows from it are formed in 64 bits;
+    sums of long answers' log-probabilities run into the thousands, so give `ref_log_probs` in 64 bits to lose none of it."""
     name = "preference_loss"
     if reduction not in ("mean", "sum", "none"):
         raise ValueError(f"Invalid reduction mode: {reduction}")
@@ -1678,7 +1681,7 @@ def preference_loss(logits, tokens, ref_log_probs, beta=0.1, label_smoothing=0.0
         raise ValueError(f"{name}: logits must be [2 P, T, V], chosen answers before rejected ones, got {tuple(z.shape)}")
     beta = _number(name, "beta", beta, 0.0, math.inf)
     smoothing = _number(name, "label_smoothing", label_smoothing, 0.0, 1.0)
-    ref = _constant(name, "ref_log_probs", ref_log_probs, ((z.shape[0],),), z)
+    ref = _constant(name, "ref_log_probs", ref_log_probs, ((z.shape[0],),), z, keep_64=True)
     rewards = []
     loss = PreferenceLossFunction.apply(logits, t, ref, beta, smoothing, ignore_index, reduction, rewards)
     return (loss, Tensor._wrap(rewards[0])) if return_rewards else loss

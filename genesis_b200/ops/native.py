@@ -70,7 +70,7 @@ _SIGS = {
     "gb_masked_fill": "pp" + "d" + "ll" + "i" + "p", "gb_fill_elems": "pldip",
     "gb_token_rows": "pppp" + "lllll" + "l" + "d" + "ii" + "pp",
     "gb_policy_loss": "pppp" + "lllll" + "l" + "d" + "ppppp" + "l" + "fff" + "pp" + "iii" + "pp",
-    "gb_preference_loss": "pppp" + "lllll" + "l" + "p" + "l" + "dd" + "i" + "ppppp" + "ii" + "pp",
+    "gb_preference_loss": "pppp" + "lllll" + "l" + "pi" + "l" + "dd" + "i" + "ppppp" + "ii" + "pp",
     "gb_token_grad": "pppp" + "lllll" + "l" + "d" + "pl" + "pll" + "p" + "f" + "ii" + "p",
     "gb_ns_workspace": "lllip", "gb_muon_momentum": "p" + "iiii" + "f" + "i" + "ppp" + "p",
     "gb_newton_schulz": "pp" + "iiiii" + "p" + "i" + "d" + "p" + "fff" + "pp" + "pp" + "p",
@@ -1958,7 +1958,8 @@ def preference_loss(logits, tokens, ignore_index, ref, beta, smoothing, reductio
     at, op = buf.data_ptr(), out.data_ptr()
     with _on(dev):
         _chk(lib().gb_preference_loss(logits.data_ptr(), tokens.data_ptr(), at + 8 * rows + 4 * n + 8, at, rows, logits.shape[-1], *m,
-                                      ignore_index, ref.data_ptr(), n // 2, beta, smoothing, 1 if reduction == "mean" else 0,
+                                      ignore_index, ref.data_ptr(), 1 if ref.dtype == torch.float64 else 0, n // 2, beta, smoothing,
+                                      1 if reduction == "mean" else 0,
                                       op if each else None, at + 8 * rows + 4 * n if each else op, rewards.data_ptr(),
                                       at + 16 * rows + 4 * n + 8, at + 8 * rows, _DT[logits.dtype], 1 if tokens.dtype == torch.int64 else 0,
                                       status_tensor(dev).data_ptr(), _st()), "preference_loss")

@@ -33,3 +33,23 @@ def test_difference_of_large_rewards():
     loss.backward(T(torch.ones(3)))
     each.sum().backward()
     assert float((x.grad._t.double() - r.grad).abs().max()) < 1.1 * (1.1 / 4 * 8e-6 + 1e-6)
+
+
+def with_digits_beyond_32_bits(ref, seed):
+    return ref.double() + torch.rand(ref.shape, generator=torch.Generator().manual_seed(seed)).double() * 2.0 ** -8
+
+
+def test_a_reference_in_64_bits_is_not_rounded():
+    """Sums near -18000, of which 32 bits hold no more than 2^-10: the loss and the gradient are as near as in the test above."""
+    z, t, ref = pairs_of_large_rewards(2)
+    ref = with_digits_beyond_32_bits(ref, 3)
+    assert float((ref - ref.float().double()).abs().max()) > 4e-4
+    x = T(z, requires_grad=True)
+    loss = F.preference_loss(x, T(t), T(ref), beta=1.1, label_smoothing=0.1, reduction="none")
+    r = R.leaf64(z)
+    each, _ = R.preference(r, t, ref, 1.1, 0.1)
+    assert float((loss._t.double() - each.detach()).abs().max()) < 1.1 * 8e-6 + 2.0 ** -24 * 20
+    loss.backward(T(torch.ones(3)))
+    each.sum().backward()
+    assert x.grad._t.dtype == torch.float32
+    assert float((x.grad._t.double() - r.grad).abs().max()) < 1.1 * (1.1 / 4 * 8e-6 + 1e-6)
