@@ -8,7 +8,7 @@
 //                l = -(1 - e) log sigmoid(h) - e log sigmoid(-h),  dl/dh = e - sigmoid(-h)
 //   logits:      dz[j] = g / T ([j = t] - exp((z[j] - m) / T) / s)
 //
-// Three kinds of kernels: one reads every row that counts once and keeps (m, log2 s) of it; one block joins the rows
+// Three kinds of kernels: one reads every row that counts once and keeps m and s (16-bit logits: log2 s) of it; one block joins the rows
 // into the loss, in a fixed order and in 64 bits (the sum of an answer's log-probabilities runs into the thousands, its
 // difference to the reference's is of order one; there the log-probabilities too are kept in 64 bits); one writes the
 // gradient.  Nothing of the size of the logits is kept between the two passes but the logits.  A row that does not count (its
@@ -193,7 +193,7 @@ __device__ __forceinline__ void finish_row(MaxSum a, const T* p, long long t, lo
   if (q.wide != nullptr) q.wide[r] = wide;
   else lp_out[r] = lp;
   stats[r] = a.m;
-  stats[rows + r] = log2f(a.s);
+  stats[rows + r] = sizeof(T) == 4 ? a.s : log2f(a.s);             // (see grad_part)
   if (q.old != nullptr) {
     const float A = q.adv[r / q.adv_div];
     const float ratio = expf(lp - q.old[r]);
@@ -383,10 +383,16 @@ constexpr int BWD_THREADS = 256;
 
 // Gradient of `n` elements of a row by `G` threads; `t` counts from the first of them.
 template <typename T, int G>
-__device__ __forceinline__ void grad_part(const T* p, T* d, int n, long long t, float m, float ls, float c, float f, int tid) {
+__device__ __forceinline__ void grad_part(const T* p, T* d, int n, long long t, float m, float stat, const Scale& c, float f, int tid) {
   constexpr int V = 16 / sizeof(T), H = V / 2, U = 4;
+  // Probabilities of 32-bit logits: the exponential of an argument formed with both parts of log2(e) / T, over s.  With log2 s
+  // in the exponent instead, rounded to 32 bits, all of a row of 151936 would be off by up to 6.6e-7 of themselves, the same
+  // way; 16-bit gradients, rounded to 5e-4 and more, do not show that, and take one instruction where this takes three.
+  constexpr bool EXACT = sizeof(T) == 4;
+  const float hi = c.hi + c.lo, ls = stat, rs = EXACT ? 1.f / stat : 1.f;
   auto one = [&](int j) {
-    const float e = ex2(fmaf(Cvt<T>::to_f(p[j]) - m, c, -ls));
+    const float x = Cvt<T>::to_f(p[j]) - m;
+    const float e = EXACT ? ex2(c(x)) * rs : ex2(fmaf(x, hi, -ls));
     d[j] = Cvt<T>::from_f(f * ((j == t ? 1.f : 0.f) - e));
   };
   const int mis = (int)((reinterpret_cast<uintptr_t>(d) & 15) / sizeof(T));
@@ -396,15 +402,18 @@ __device__ __forceinline__ void grad_part(const T* p, T* d, int n, long long t, 
   const int nv = same ? (n - head) / V : 0;
   const uint4* src = reinterpret_cast<const uint4*>(p + head);
   uint4* dst = reinterpret_cast<uint4*>(d + head);
-  const float2 nm = make_float2(-m, -m), c2 = make_float2(c, c), nl = make_float2(-ls, -ls), nf = make_float2(-f, -f);
+  const float2 nm = make_float2(-m, -m), nf = make_float2(-f, -f), nl = make_float2(-ls, -ls), r2 = make_float2(rs, rs);
+  const float2 c2 = EXACT ? make_float2(c.hi, c.hi) : make_float2(hi, hi), lo = make_float2(c.lo, c.lo);
   const long long tv = t < head ? -1 : (t - head) / V;             // the vector that holds the token
   auto vec = [&](const uint4& x, int i) {
     float2 e[H];
     unpack<T>(x, e);
 #pragma unroll
     for (int k = 0; k < H; ++k) {
-      e[k] = fma2(add2(e[k], nm), c2, nl);
+      const float2 x = add2(e[k], nm);
+      e[k] = fma2(x, c2, EXACT ? mul2(x, lo) : nl);
       e[k].x = ex2(e[k].x); e[k].y = ex2(e[k].y);
+      if constexpr (EXACT) e[k] = mul2(e[k], r2);
     }
     if (i == tv) {
       const int at = (int)((t - head) % V);
@@ -461,7 +470,7 @@ __device__ __forceinline__ void zero_part(T* d, int n, int tid) {
 template <typename T, typename TI, int G>
 __global__ void __launch_bounds__(BWD_THREADS)
 token_grad_kernel(const T* __restrict__ z, RowMap map, const TI* __restrict__ tokens, const float* __restrict__ stats,
-                  T* __restrict__ dz, long long rows, int cols, long long ignore, float inv_temperature, float c, Factor fac,
+                  T* __restrict__ dz, long long rows, int cols, long long ignore, Scale c, Factor fac,
                   int chunk, int chunks) {
   const int tid = threadIdx.x % G;
   const long long item = (long long)blockIdx.x * (BWD_THREADS / G) + threadIdx.x / G;
@@ -471,7 +480,7 @@ token_grad_kernel(const T* __restrict__ z, RowMap map, const TI* __restrict__ to
   const int n = min(chunk, cols - lo);
   T* d = dz + r * cols + lo;
   long long t;
-  const float f = counts(tokens, r, cols, ignore, t) ? fac.at(r) * inv_temperature : 0.f;
+  const float f = counts(tokens, r, cols, ignore, t) ? fac.at(r) * c.inv : 0.f;
   if (f == 0.f) { zero_part<T, G>(d, n, tid); return; }
   grad_part<T, G>(z + map.at(r) + lo, d, n, t - lo, stats[r], stats[rows + r], c, f, tid);
 }
@@ -517,17 +526,17 @@ static int rows_forward(const void* z, RowMap map, const void* tokens, float* lp
 template <typename T, typename TI>
 static int rows_backward(const void* z, RowMap map, const void* tokens, const float* stats, void* dz, long long rows, int cols,
                          long long ignore, double temperature, const Factor& fac, cudaStream_t st) {
-  const float c = (float)(1.4426950408889634 / temperature), inv = (float)(1.0 / temperature);
+  const Scale c(temperature);
   if ((long long)cols * sizeof(T) <= 8192 && (cols <= 1024 || rows >= 32ll * sm_count())) {
     token_grad_kernel<T, TI, 32><<<(unsigned)((rows + 7) / 8), BWD_THREADS, 0, st>>>(
-        (const T*)z, map, (const TI*)tokens, stats, (T*)dz, rows, cols, ignore, inv, c, fac, cols, 1);
+        (const T*)z, map, (const TI*)tokens, stats, (T*)dz, rows, cols, ignore, c, fac, cols, 1);
     return (int)cudaGetLastError();
   }
   const int chunk = 16384 / (int)sizeof(T) * 2;
   const int chunks = (cols + chunk - 1) / chunk;
   if (rows * chunks > 0x7fffffffll) return -3;
   token_grad_kernel<T, TI, BWD_THREADS><<<(unsigned)(rows * chunks), BWD_THREADS, 0, st>>>(
-      (const T*)z, map, (const TI*)tokens, stats, (T*)dz, rows, cols, ignore, inv, c, fac, chunk, chunks);
+      (const T*)z, map, (const TI*)tokens, stats, (T*)dz, rows, cols, ignore, c, fac, chunk, chunks);
   return (int)cudaGetLastError();
 }
 
@@ -544,7 +553,7 @@ static int rows_any(const void* z, const void* tokens, float* lp, float* stats, 
 
 using namespace gb;
 
-// Log-probabilities lp [rows] of `tokens` and the rows' (max, log2 sum) in stats [2, rows].  Rows: see RowMap.
+// Log-probabilities lp [rows] of `tokens` and what gb_token_grad needs of the rows in stats [2, rows].  Rows: see RowMap.
 extern "C" int gb_token_rows(const void* z, const void* tokens, float* lp, float* stats, long long rows, long long cols,
                              long long inner, long long s_outer, long long s_inner, long long ignore, double temperature,
                              int dt, int token_i64, int* status, cudaStream_t st) {

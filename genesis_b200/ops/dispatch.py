@@ -617,7 +617,7 @@ def token_logits(logits):
 
 def token_rows(logits, tokens, ignore_index, temperature):
     """Log-probabilities of `tokens` [...] under `logits` [..., V] / temperature (0 where ignored), and what the gradient
-    needs of the rows [2 rows]: m, a number near the row's maximum, and log2 of the sum of exp((z - m) / temperature)."""
+    needs of the rows [2 rows]: m, a number near the row's maximum, and the sum of exp((z - m) / temperature)."""
     if logits.is_cuda:
         r = N.token_rows(logits, tokens, ignore_index, temperature)
         if r is not NotImplemented:
@@ -627,10 +627,10 @@ def token_rows(logits, tokens, ignore_index, temperature):
     valid = _check_tokens(tokens, logits.shape[-1], ignore_index)
     z = logits.to(acc)
     m = z.max(-1, keepdim=True).values
-    log_sum = torch.logsumexp((z - m) / temperature, -1, keepdim=True)
+    s = torch.exp((z - m) / temperature).sum(-1, keepdim=True)
     tok = torch.where(valid, tokens, torch.zeros_like(tokens)).long().unsqueeze(-1)
-    lp = ((z.gather(-1, tok) - m) / temperature - log_sum).squeeze(-1)
-    return torch.where(valid, lp, torch.zeros_like(lp)), torch.cat((m.reshape(-1), log_sum.reshape(-1) * math.log2(math.e)))
+    lp = ((z.gather(-1, tok) - m) / temperature - torch.log(s)).squeeze(-1)
+    return torch.where(valid, lp, torch.zeros_like(lp)), torch.cat((m.reshape(-1), s.reshape(-1)))
 
 
 def policy_loss(logits, tokens, ignore_index, temperature, policy, reduction):
@@ -707,7 +707,7 @@ def token_grad(logits, tokens, stats, ignore_index, temperature, base_div=0, g=N
     valid = (flat != ignore_index) & (flat >= 0) & (flat < V)
     f = torch.where(valid, f, torch.zeros_like(f)) / temperature
     z = logits.reshape(rows, V).to(stats.dtype)
-    p = torch.exp2((z - stats[:rows, None]) * (math.log2(math.e) / temperature) - stats[rows:2 * rows, None])
+    p = torch.exp((z - stats[:rows, None]) / temperature) / stats[rows:2 * rows, None]
     p.scatter_add_(1, torch.where(valid, flat, torch.zeros_like(flat)).long()[:, None], -torch.ones_like(f)[:, None])
     d = torch.where((f == 0)[:, None], torch.zeros_like(p), p * -f[:, None])
     return d.reshape(logits.shape).to(logits.dtype)
