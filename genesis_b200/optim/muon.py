@@ -181,10 +181,12 @@ class Muon(Optimizer):
             if g.shape != p.shape or g.device != p.device:
                 raise ValueError(f"gradient of shape {tuple(g.shape)} on {g.device} for a parameter of shape "
                                  f"{tuple(p.shape)} on {p.device}")
-            members = groups.setdefault((tuple(sorted(p.shape[-2:])), g.dtype, p.device), [])
+            # (the type and layout of the weight too: those that the kernels do not take must not keep others from them)
+            key = (tuple(sorted(p.shape[-2:])), g.dtype, p.device, p.dtype, p.is_contiguous())
+            members = groups.setdefault(key, [])
             g, u = K.contiguous(g), self._state(self.u, i)
             members += [((p, k), (g, k), (u, k)) for k in range(p.numel() // (p.shape[-2] * p.shape[-1]))]
-        for (shape, _, _), members in groups.items():
+        for (shape, *_), members in groups.items():
             ps, gs, us = (list(x) for x in zip(*members))
             K.muon_step(ps, gs, us, shape, self.lr, self.momentum, self.nesterov, self.weight_decay,
                         math.sqrt(shape[1] / shape[0]), self.steps, self.coefficients, self.eps, program,
