@@ -186,9 +186,11 @@ class Muon(Optimizer):
             members = groups.setdefault(key, [])
             g, u = K.contiguous(g), self._state(self.u, i)
             members += [((p, k), (g, k), (u, k)) for k in range(p.numel() // (p.shape[-2] * p.shape[-1]))]
-        for (shape, *_), members in groups.items():
+        for (shape, _, dev, *_), members in groups.items():
             ps, gs, us = (list(x) for x in zip(*members))
+            # (a kernel reads these on its own device)
+            scalars = [s if s is None or s.device == dev else s.to(dev)
+                       for s in (self._grad_scale, self._found_inf, self._dyn_lr_t)]
             K.muon_step(ps, gs, us, shape, self.lr, self.momentum, self.nesterov, self.weight_decay,
-                        math.sqrt(shape[1] / shape[0]), self.steps, self.coefficients, self.eps, program,
-                        self._grad_scale, self._found_inf, self._dyn_lr_t)
+                        math.sqrt(shape[1] / shape[0]), self.steps, self.coefficients, self.eps, program, *scalars)
         self._touched(idx)

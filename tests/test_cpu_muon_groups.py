@@ -31,3 +31,20 @@ def test_weights_of_other_types_and_layouts_go_by_themselves(monkeypatch):
     for params in seen:
         assert len({p.dtype for p in params}) == 1 and len({p.is_contiguous() for p in params}) == 1
     assert sorted(len(p) for p in seen) == [1, 1, 1, 3]
+
+
+def test_scalars_go_to_the_device_of_the_weights(monkeypatch):
+    """With weights on several devices, the scale, the overflow flag and the learning rate follow each of them: a kernel that was
+    given another device's address would read outside its memory.  ("meta" stands for a second device.)"""
+    ps = [genesis.nn.Parameter(T(matrix(4, 6))), genesis.nn.Parameter(T(matrix(4, 6).to("meta")))]
+    for p in ps:
+        p.grad = T(torch.ones(4, 6, device=p._t.device))
+    opt = genesis.optim.Muon(ps, lr=0.1)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    opt._grad_scale, opt._found_inf, opt._dyn_lr_t = torch.ones(1), torch.zeros(1), torch.tensor([0.1])
+    seen = {}
+    monkeypatch.setattr(K, "muon_step", lambda params, grads, bufs, *a: seen.update({params[0][0].device.type: a[-3:]}))
+    opt.step()
+    assert set(seen) == {"cpu", "meta"}
+    for dev, scalars in seen.items():
+        assert all(s.device.type == dev for s in scalars)
