@@ -644,7 +644,7 @@ def policy_loss(logits, tokens, ignore_index, temperature, policy, reduction):
     old, adv, div, ref, lo, hi, kl = policy
     lp, stats = token_rows(logits, tokens, ignore_index, temperature)
     valid, zero = tokens != ignore_index, torch.zeros_like(lp)
-    A = adv.reshape(-1).repeat_interleave(div).reshape(lp.shape)
+    A = adv if adv.dim() == lp.dim() else adv.unsqueeze(-1)
     ratio = torch.exp(lp - old)
     plain, clipped = -A * ratio, -A * ratio.clamp(lo, hi)
     loss = torch.maximum(plain, clipped)
