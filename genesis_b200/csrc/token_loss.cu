@@ -543,7 +543,7 @@ static int rows_backward(const void* z, RowMap map, const void* tokens, const fl
 static int rows_any(const void* z, const void* tokens, float* lp, float* stats, long long rows, long long cols, RowMap map,
                     long long ignore, double temperature, const Policy& q, int dt, int token_i64, int* status, cudaStream_t st) {
   if (rows == 0) return 0;
-  if (cols < 1 || cols > 0x40000000ll || rows > 0x0fffffffll || map.inner < 1 || !(temperature > 0.0)) return -3;
+  if (cols < 1 || cols > 0x40000000ll || rows > 0x0fffffffll || map.inner < 1 || !(temperature >= 1e-6 && temperature <= 1e20)) return -3;
   if (token_i64) GB_DISPATCH_FLOAT(dt, T, return (rows_forward<T, long long>(z, map, tokens, lp, stats, rows, (int)cols, ignore, temperature, q, status, st)));
   GB_DISPATCH_FLOAT(dt, T, return (rows_forward<T, int>(z, map, tokens, lp, stats, rows, (int)cols, ignore, temperature, q, status, st)));
 }
@@ -600,7 +600,7 @@ extern "C" int gb_token_grad(const void* z, const void* tokens, const float* sta
                              const float* dev_scale, float scale, int dt, int token_i64, cudaStream_t st) {
   if (rows == 0) return 0;
   if (cols < 1 || cols > 0x40000000ll || rows > 0x0fffffffll || inner < 1 || base_div < 1 || g_div < 1 || g_mod < 1 ||
-      !(temperature > 0.0)) return -3;
+      !(temperature >= 1e-6 && temperature <= 1e20)) return -3;
   const tl::RowMap map{inner, s_outer, s_inner};
   const tl::Factor fac{base, g, dev_scale, base_div, g_div, g_mod, scale};
   if (token_i64) GB_DISPATCH_FLOAT(dt, T, return (tl::rows_backward<T, long long>(z, map, tokens, stats, dz, rows, (int)cols, ignore, temperature, fac, st)));

@@ -1597,8 +1597,9 @@ def _token_args(name, logits, tokens, ignore_index, temperature=1.0):
         raise TypeError(f"{name}: ignore_index must be an int, got {ignore_index!r}")
     if not -2 ** 63 <= ignore_index < 2 ** 63:
         raise ValueError(f"{name}: ignore_index must be a 64-bit number, got {ignore_index}")
-    if not 1e-6 <= float(temperature) < math.inf:
-        raise ValueError(f"{name}: temperature must be finite and at least 1e-6, got {temperature}")
+    # (the kernels hold log2(e) / T as two floats, of which the second, down to 2^-53 of it, must not vanish: -inf times it is -inf)
+    if not 1e-6 <= float(temperature) <= 1e20:
+        raise ValueError(f"{name}: temperature must be a number from 1e-6 to 1e20, got {temperature}")
     if t.dtype not in (torch.int64, torch.int32):
         t = t.long()
     return K.contiguous(t)
