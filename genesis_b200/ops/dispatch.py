@@ -612,7 +612,10 @@ def _check_tokens(tokens, vocab, ignore_index):
 
 def token_logits(logits):
     """The logits as the row kernels read them: themselves where their rows lie on two strides, else a copy."""
-    return contiguous(logits) if logits.is_cuda and N._row_map(logits) is None else logits
+    if not (logits.is_cuda and logits.dtype in N._FLOATS):
+        return logits
+    N.check_token_logits(logits)
+    return contiguous(logits) if N._row_map(logits) is None else logits
 
 
 def token_rows(logits, tokens, ignore_index, temperature):

@@ -1903,7 +1903,13 @@ def _row_map(logits):
     return dims[1][0], dims[0][1], dims[1][1]
 
 
-_TOKEN_DT = (torch.int64, torch.int32)
+def check_token_logits(logits):
+    """What the row kernels count in 32 bits: the columns of a row, and rows times the CTAs that share one."""
+    V = logits.shape[-1]
+    rows = logits.numel() // V
+    if V > 1 << 30 or rows >= 1 << 28:
+        raise ValueError(f"losses on tokens' log-probabilities take up to 2^30 logits a row and less than 2^28 rows on CUDA, "
+                         f"got {rows} rows of {V}")
 
 
 def token_rows(logits, tokens, ignore_index, temperature):

@@ -52,3 +52,13 @@ def test_temperatures_that_the_kernels_cannot_hold_are_refused():
         assert min(hi, lo, inv, slack) >= 2.0 ** -126 and math.isfinite(max(hi, lo, inv, slack))
         assert abs(hi + lo - 1.4426950408889634 / temperature) <= 2.0 ** -47 * hi
     F.token_log_probs(x, t, temperature=1e20)
+
+
+def test_rows_beyond_what_the_kernels_count_are_refused_in_words():
+    from genesis_b200.ops import native
+    one = torch.zeros(1)
+    for shape in ((1, 2 ** 30 + 1), (2, 3, 2 ** 31), (2 ** 28, 4), (2 ** 14, 2 ** 14, 1)):
+        with pytest.raises(ValueError, match="2\\^30 logits a row"):
+            native.check_token_logits(one.expand(shape))
+    for shape in ((1, 2 ** 30), (2 ** 28 - 1, 4), (0, 5), (2, 0, 5)):
+        native.check_token_logits(one.expand(shape))
