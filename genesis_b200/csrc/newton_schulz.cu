@@ -1188,10 +1188,10 @@ static int product(const CUtensorMap& ta, const CUtensorMap& tb, Params p, cudaS
 // and A's way through memory).  Five steps, own launch / here, us: 128 x 128 87.7 / 66.3, 128 x 896 88.2 / 82.3, 128 x 2048
 // 91.9 / 107.3, 100 of 128 x 4864 618 / 608.
 static bool folds(int n, int batch) {
-  const int kblocks = (n + BK - 1) / BK;
+  const long long kblocks = (n + BK - 1) / BK;
   int s = 1;
   while (s < 8 && kblocks >= 4 * s && (long long)batch * s * 2 <= sm_count()) s *= 2;
-  return (n + 127) / 128 * 2700 <= kblocks * 1080 / s + 21000;
+  return (n + 127) / 128 * 2700ll <= kblocks * 1080 / s + 21000;
 }
 
 static int chain(const CUtensorMap& ta, const CUtensorMap& tx, const Chain& c, cudaStream_t st) {
@@ -1242,7 +1242,7 @@ extern "C" int gb_ns_workspace(long long m, long long n, long long batch, int wi
 extern "C" int gb_muon_momentum(const long long* table, int batch, int grad_dt, int m, int n, float mu, int nesterov,
                                 const float* grad_scale, const float* found_inf, void* workspace, cudaStream_t st) {
   if (batch <= 0 || m <= 0 || n <= 0) return 0;
-  if (batch > 32767 || m > n) return -3;
+  if (batch > 32767 || m > n || n > (1 << 30)) return -3;
   const ns::Workspace w((uint8_t*)workspace, m, n, batch, true);
   const long long numel = (long long)m * n;
   ns::muon_momentum_kernel<<<dim3(ns::norm_parts(numel), batch), 256, 0, st>>>(table, batch, grad_dt, numel, mu, nesterov,
@@ -1261,7 +1261,7 @@ extern "C" int gb_newton_schulz(const void* src, void* out, int dt, int m, int n
                                 int count, double eps, const long long* weights, float lr, float decay, float tall_scale,
                                 const float* dyn_lr, const float* found_inf, void* workspace, int* status, cudaStream_t st) {
   if (batch <= 0 || m <= 0 || n <= 0) return 0;
-  if (batch > 6000 || m > n || count < 2 || (src == nullptr) != (weights != nullptr) ||
+  if (batch > 6000 || m > n || n > (1 << 30) || count < 2 || (src == nullptr) != (weights != nullptr) ||
       (reinterpret_cast<uintptr_t>(workspace) & 255) != 0) return -3;
   const int ldx = (n + 7) & ~7, lda = (m + 7) & ~7;
   const ns::Workspace w((uint8_t*)workspace, m, n, batch, src == nullptr);

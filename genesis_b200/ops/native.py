@@ -2000,9 +2000,12 @@ def _ns_batch(m, n):
     return max(1, min(4096, (1 << 32) // (12 * m * n + 40 * m * m)))
 
 
+_NS_LONGEST = 1 << 30           # of a matrix's sides: the kernels count rows, columns and their tiles in 32 bits
+
+
 def newton_schulz(x, steps, coefficients, eps, program):
     """Orthogonalised matrices of contiguous x [batch, rows, cols], in its type."""
-    if x.dtype not in _FLOATS or not x.is_contiguous():
+    if x.dtype not in _FLOATS or not x.is_contiguous() or max(x.shape[-2:]) > _NS_LONGEST:
         return NotImplemented
     out = torch.empty_like(x)
     batch, rows, cols = x.shape
@@ -2023,6 +2026,8 @@ def muon_step(params, grads, bufs, shape, lr, momentum, nesterov, weight_decay, 
     """One step on matrices of shape (m, n) or (n, m), m <= n.  params / grads / bufs: lists of (tensor, index of the
     matrix in it)."""
     m, n = shape
+    if n > _NS_LONGEST:
+        return NotImplemented
     for t, _ in params + bufs:
         if t.dtype != F32 or not t.is_contiguous():
             return NotImplemented

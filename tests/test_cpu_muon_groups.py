@@ -48,3 +48,17 @@ def test_scalars_go_to_the_device_of_the_weights(monkeypatch):
     assert set(seen) == {"cpu", "meta"}
     for dev, scalars in seen.items():
         assert all(s.device.type == dev for s in scalars)
+
+
+def test_sides_beyond_32_bits_do_not_reach_the_kernels():
+    """A side of 2^31 and more would arrive there as a negative number, for which nothing is done and the result is whatever the
+    memory held.  Such a matrix goes to the library."""
+    from genesis_b200.ops import native
+    from genesis_b200.optim.muon import _check
+    coefficients, eps, program = _check(1, (1.5, -0.5, 0.0), 1e-7)
+    for shape in ((1, 1, 2 ** 30 + 1), (1, 2 ** 31 + 5, 1)):
+        x = torch.empty(shape, dtype=torch.bfloat16, device="meta")
+        assert native.newton_schulz(x, 1, coefficients, eps, program) is NotImplemented
+        w = [(torch.empty(shape, device="meta"), 0)]
+        assert native.muon_step(w, w, w, (1, max(shape)), 0.1, 0.9, True, 0.0, 1.0, 1, coefficients, eps, program, None, None,
+                                None) is NotImplemented
