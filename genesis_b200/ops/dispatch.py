@@ -1021,7 +1021,8 @@ def _newton_schulz_torch(x, steps, coefficients, eps):
     y = x if x.dtype == torch.float64 else x.to(_F32)
     tall = y.shape[-2] > y.shape[-1]
     y = y.transpose(-2, -1) if tall else y
-    y = y / (torch.linalg.vector_norm(y, dim=(-2, -1), keepdim=True, dtype=torch.float64) + eps).to(y.dtype)
+    # (in 64 bits: the norm of numbers that 32 bits hold may be one that they do not)
+    y = (y.double() / (torch.linalg.vector_norm(y, dim=(-2, -1), keepdim=True, dtype=torch.float64) + eps)).to(y.dtype)
     for _ in range(steps):
         A = y @ y.transpose(-2, -1)
         y = a * y + (b * A + c * (A @ A)) @ y

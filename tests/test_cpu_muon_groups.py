@@ -62,3 +62,11 @@ def test_sides_beyond_32_bits_do_not_reach_the_kernels():
         w = [(torch.empty(shape, device="meta"), 0)]
         assert native.muon_step(w, w, w, (1, max(shape)), 0.1, 0.9, True, 0.0, 1.0, 1, coefficients, eps, program, None, None,
                                 None) is NotImplemented
+
+
+def test_a_norm_beyond_32_bits():
+    """Elements near 1e38: the matrix is the same up to scale, and comes out as that of elements near 1."""
+    x = matrix(20, 30, seed=2).clamp(-3, 3)
+    big = genesis.optim.orthogonalize(T(x * 1e38))._t
+    # scaling rounds each element once more, 2^-24 of it, which the iteration amplifies by 485 at most; as much for the products
+    assert float((big - genesis.optim.orthogonalize(T(x))._t).abs().max()) < 485 * 2.0 ** -24 * 4
