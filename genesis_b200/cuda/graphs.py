@@ -132,6 +132,8 @@ class GraphedTrainStep(GraphedCallable):
         self._optimizers = list(optimizer) if isinstance(optimizer, (list, tuple)) else [optimizer]
         if not self._optimizers or not all(hasattr(o, "make_capturable") for o in self._optimizers):
             raise TypeError("GraphedTrainStep needs Adam / AdamW / Muon optimizers (device-resident step state)")
+        if len({id(o) for o in self._optimizers}) != len(self._optimizers):
+            raise ValueError("GraphedTrainStep: an optimizer is listed twice (its steps would be counted twice)")
         for o in self._optimizers:
             o.make_capturable()
         self.optimizer = optimizer

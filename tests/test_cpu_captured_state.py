@@ -49,3 +49,9 @@ def test_buffers_are_replaced_otherwise(kind):
     other = build(kind)[1]
     opt.load_state_dict(other.state_dict())
     assert torch.equal(aside[name][0]._t, values) and 0 not in getattr(opt, name)
+
+
+def test_an_optimizer_listed_twice_is_refused():
+    ps, opt = build("adamw")
+    with pytest.raises(ValueError, match="twice"):
+        genesis.cuda.GraphedTrainStep(lambda: None, [opt, opt], [])
