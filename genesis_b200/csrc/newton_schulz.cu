@@ -992,10 +992,11 @@ ns_norm_kernel(const void* __restrict__ src, int dt, long long numel, double* __
 }
 
 // Momentum of every matrix of a batch and the update that goes on to the iteration:
-//   u <- mu u + (1 - mu) g,   y = mu u + (1 - mu) g (Nesterov) or u
+//   u <- mu u + nu g,   y = mu u + nu g (Nesterov) or u,   nu = 1 - mu, formed in 64 bits: from mu rounded to 32 it would be
+// 2.4e-7 of itself off at mu = 0.9 or 0.95, and with it every momentum
 // table: addresses of gradients, then of momenta [2, batch]; y [batch, numel], and the partial sums of its squares.
 __global__ void __launch_bounds__(256)
-muon_momentum_kernel(const long long* __restrict__ table, int batch, int grad_dt, long long numel, float mu, int nesterov,
+muon_momentum_kernel(const long long* __restrict__ table, int batch, int grad_dt, long long numel, float mu, float nu, int nesterov,
                      const float* __restrict__ grad_scale, const float* __restrict__ found_inf, float* __restrict__ y,
                      double* __restrict__ partial) {
   __shared__ double sh[8];
@@ -1003,7 +1004,7 @@ muon_momentum_kernel(const long long* __restrict__ table, int batch, int grad_dt
   const void* g = reinterpret_cast<const void*>(table[z]);
   float* u = reinterpret_cast<float*>(table[batch + z]);
   float* yz = y + (size_t)z * numel;
-  const float gs = grad_scale != nullptr ? *grad_scale : 1.f, nu = 1.f - mu;
+  const float gs = grad_scale != nullptr ? *grad_scale : 1.f;
   const bool skip = found_inf != nullptr && *found_inf != 0.f;      // the step is cancelled: momentum stays as it is
   double s = 0.0;
   const long long step = 256ll * gridDim.x, me = (long long)blockIdx.x * 256 + threadIdx.x;
@@ -1239,13 +1240,13 @@ extern "C" int gb_ns_workspace(long long m, long long n, long long batch, int wi
 }
 
 // First half of an optimizer step: see muon_momentum_kernel.  The update and its partial sums stay in the workspace.
-extern "C" int gb_muon_momentum(const long long* table, int batch, int grad_dt, int m, int n, float mu, int nesterov,
+extern "C" int gb_muon_momentum(const long long* table, int batch, int grad_dt, int m, int n, double mu, int nesterov,
                                 const float* grad_scale, const float* found_inf, void* workspace, cudaStream_t st) {
   if (batch <= 0 || m <= 0 || n <= 0) return 0;
   if (batch > 32767 || m > n || n > (1 << 30)) return -3;
   const ns::Workspace w((uint8_t*)workspace, m, n, batch, true);
   const long long numel = (long long)m * n;
-  ns::muon_momentum_kernel<<<dim3(ns::norm_parts(numel), batch), 256, 0, st>>>(table, batch, grad_dt, numel, mu, nesterov,
+  ns::muon_momentum_kernel<<<dim3(ns::norm_parts(numel), batch), 256, 0, st>>>(table, batch, grad_dt, numel, (float)mu, (float)(1.0 - mu), nesterov,
                                                                                grad_scale, found_inf, w.y, w.partial);
   return (int)cudaGetLastError();
 }

@@ -24,3 +24,16 @@ def test_weights_of_other_types_leave_the_others_to_the_kernels():
     opt.step()
     assert torch.equal(mixed[0]._t, alone[0]._t) and torch.equal(mixed[2]._t, alone[1]._t)
     assert all(float((p._t - b).abs().max()) > 1e-3 for p, b in zip(mixed, before))
+
+
+@pytest.mark.parametrize("momentum", [0.9, 0.95, 0.3])
+@pytest.mark.parametrize("shape", [(40, 60), (7, 9)])
+def test_momentum_takes_its_weights_from_64_bits(shape, momentum):
+    """u = (1 - mu) g in the first step: the weight rounded once and the product once, 2^-24 of u each.  1 - mu of a mu that had
+    been rounded before would be off by 2.4e-7."""
+    p = genesis.nn.Parameter(T(matrix(*shape).cuda()))
+    p.grad = T(matrix(*shape, seed=1).cuda())
+    opt = genesis.optim.Muon([p], lr=0.1, momentum=momentum)
+    opt.step()
+    want = (1.0 - momentum) * p.grad._t.double()
+    assert bool(((opt.u[0].double() - want).abs() <= 2.0 ** -23 * 1.001 * want.abs()).all())
