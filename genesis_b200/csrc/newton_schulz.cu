@@ -1155,33 +1155,41 @@ static int max_clusters(int size) {
   return n;
 }
 
-template <int MODE>
-static int product(const CUtensorMap& ta, const CUtensorMap& tb, Params p, cudaStream_t st) {
-  const long long sms = sm_count(), kblocks = (p.k + BK - 1) / BK, matrices = (long long)p.batch * p.problems;
-  // Tiles of 128 x 128 or 128 x 256, whole or shared by the CTAs of a cluster, or of 256 x 256 on pairs: whatever has the
-  // fewest clocks on its longest CTA.  A block of the contraction takes 1080 clocks with 128 columns and 1700 with 256,
-  // bound by shared memory (213 and 160 bytes a clock at the full tensor rate, of 128), or 2100 where all SMs together
-  // read more than L2 gives (11 TB/s); pairs read two thirds of that and take 1600.  The epilogue of the last tile, which no
-  // products hide, takes 6500 for each chunk of a warp; the parts of a cluster 4000 to meet and 5000 a chunk.
-  int kind = WHOLE, bn = 128;
-  long long best = -1, grid = 0;
-  auto offer = [&](long long clocks, int k, int width, int splits, long long ctas) {
-    if (best >= 0 && clocks >= best) return;
-    best = clocks; kind = k; bn = width; p.splits = splits; grid = ctas;
+// How a product is worked on: tiles of 128 x 128 or 128 x 256, whole or shared by the CTAs of a cluster, or of 256 x 256 on
+// pairs: whatever has the fewest clocks on its longest CTA.  A block of the contraction takes 1080 clocks with 128 columns and
+// 1700 with 256, bound by shared memory (213 and 160 bytes a clock at the full tensor rate, of 128), or 2100 where all SMs
+// together read more than L2 gives (11 TB/s); pairs read two thirds of that and take 1600.  The epilogue of the last tile,
+// which no products hide, takes 6500 for each chunk of a warp; the parts of a cluster 4000 to meet and 5000 a chunk.
+struct Plan { int kind, bn, splits, grid; };
+static Plan plan(bool sym, int m, int n, int k, long long matrices) {
+  const long long sms = sm_count(), kblocks = (k + BK - 1) / BK;
+  Plan best{WHOLE, 128, 1, 0};
+  long long least = -1;
+  auto offer = [&](long long clocks, int kind, int width, int splits, long long ctas) {
+    if (least >= 0 && clocks >= least) return;
+    least = clocks;
+    best = Plan{kind, width, splits, (int)ctas};
   };
   for (int width = 128; width <= 256; width += 128) {
-    const long long total = tiles_of(MODE == SYM, p.m, p.n, BM, width) * matrices, waves = (total + sms - 1) / sms;
+    const long long total = tiles_of(sym, m, n, BM, width) * matrices, waves = (total + sms - 1) / sms;
     const long long block = width == 128 ? 1080 : total >= sms ? 2100 : 1700, chunks = width / 64;
     offer(waves * kblocks * block + chunks * 6500, WHOLE, width, 1, total < sms ? total : sms);
     for (int s = 2; s <= 8 && kblocks >= 2 * s && total <= max_clusters(s); s *= 2)      // (one tile each: a single wave)
       offer((kblocks + s - 1) / s * (width == 128 ? 1080 : 1700) + (chunks + s - 1) / s * 5000 + 4000, SPLIT, width, s, total * s);
   }
-  const long long pairs = tiles_of(MODE == SYM, p.m, p.n, 2 * BM, 256) * matrices, at_once = max_clusters(2);
+  const long long pairs = tiles_of(sym, m, n, 2 * BM, 256) * matrices, at_once = max_clusters(2);
   offer((pairs + at_once - 1) / at_once * kblocks * 1600 + 4 * 6500, PAIR, 256, 1, 2 * (pairs < at_once ? pairs : at_once));
-  const int g = (int)grid;
-  if (kind == PAIR) return launch<MODE, 256, PAIR>(ta, tb, p, g, st);
-  if (kind == SPLIT) return bn == 256 ? launch<MODE, 256, SPLIT>(ta, tb, p, g, st) : launch<MODE, 128, SPLIT>(ta, tb, p, g, st);
-  return bn == 256 ? launch<MODE, 256, WHOLE>(ta, tb, p, g, st) : launch<MODE, 128, WHOLE>(ta, tb, p, g, st);
+  return best;
+}
+
+template <int MODE>
+static int product(const CUtensorMap& ta, const CUtensorMap& tb, Params p, cudaStream_t st) {
+  const Plan c = plan(MODE == SYM, p.m, p.n, p.k, (long long)p.batch * p.problems);
+  p.splits = c.splits;
+  if (c.kind == PAIR) return launch<MODE, 256, PAIR>(ta, tb, p, c.grid, st);
+  if (c.kind == SPLIT)
+    return c.bn == 256 ? launch<MODE, 256, SPLIT>(ta, tb, p, c.grid, st) : launch<MODE, 128, SPLIT>(ta, tb, p, c.grid, st);
+  return c.bn == 256 ? launch<MODE, 256, WHOLE>(ta, tb, p, c.grid, st) : launch<MODE, 128, WHOLE>(ta, tb, p, c.grid, st);
 }
 
 // Whether ns_chain_kernel forms A = X X^T itself: its one CTA takes 2700 clocks for 128 columns of X; a launch of its own 1080
@@ -1236,6 +1244,15 @@ using namespace gb;
 // Bytes of workspace that `batch` matrices m x n, m <= n, need (with_y: an optimizer step, which keeps its updates there)
 extern "C" int gb_ns_workspace(long long m, long long n, long long batch, int with_y, long long* bytes) {
   *bytes = ns::Workspace(nullptr, m, n, batch, with_y != 0).bytes;
+  return 0;
+}
+
+// What `plan` chooses on this device for a product with a contraction of k, in which `problems` results are wanted of each of
+// `batch` matrices [m, n]: kind (0 whole tiles, 1 shared by a cluster, 2 CTA pairs), columns of a tile, CTAs that share one
+extern "C" int gb_ns_plan(int sym, int m, int n, int k, int batch, int problems, int* out) {
+  if (m < 1 || n < m || k < 1 || batch < 1 || problems < 1) return -3;
+  const ns::Plan c = ns::plan(sym != 0, m, n, k, (long long)batch * problems);
+  out[0] = c.kind; out[1] = c.bn; out[2] = c.splits;
   return 0;
 }
 

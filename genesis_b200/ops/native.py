@@ -72,7 +72,7 @@ _SIGS = {
     "gb_policy_loss": "pppp" + "lllll" + "l" + "d" + "ppppp" + "l" + "fff" + "pp" + "iii" + "pp",
     "gb_preference_loss": "pppp" + "lllll" + "l" + "pi" + "l" + "dd" + "i" + "ppppp" + "ii" + "pp",
     "gb_token_grad": "pppp" + "lllll" + "l" + "d" + "pl" + "pll" + "p" + "f" + "ii" + "p",
-    "gb_ns_workspace": "lllip", "gb_muon_momentum": "p" + "iiii" + "d" + "i" + "ppp" + "p",
+    "gb_ns_plan": "iiiiiip", "gb_ns_workspace": "lllip", "gb_muon_momentum": "p" + "iiii" + "d" + "i" + "ppp" + "p",
     "gb_newton_schulz": "pp" + "iiiii" + "p" + "i" + "d" + "p" + "fff" + "pp" + "pp" + "p",
 }
 
