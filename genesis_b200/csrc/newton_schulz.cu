@@ -9,9 +9,9 @@
 // P's, kept as s I + Q:  Q <- a Q + s B + B Q.  At the end of the block X <- s X + Q X.  All but the last are symmetric.
 // For 896 x 4864 and five steps in blocks of three and two that is 33 GFLOP for the 62 of five products with X each way, and
 // X passes through memory twice instead of five times; for square matrices it is as many operations.  A rounding of A grows
-// by a^2 a step, so blocks are short: simulated over spectra from Gaussian to rank one plus noise, blocks of up to three are
-// as exact as products with X (256 x 1024: 2.4e-6 for 1.5e-6 Gaussian, 0.6e-6 for 0.5e-6 rank 8 plus noise; fp32 products
-// throughout 2.0e-6 and 2.0e-6), five in one lose a digit (5e-6, 21e-6).
+// by a^2 a step, so blocks are short: simulated over spectra from Gaussian to rank one plus noise, blocks of up to three come
+// within a factor of two of products with X (256 x 1024: 2.4e-6 for 1.5e-6 Gaussian, 0.6e-6 for 0.5e-6 rank 8 plus noise; fp32
+// products throughout 2.0e-6 and 2.0e-6), five in one lose a digit (5e-6, 21e-6).
 //
 // Arithmetic.  The iteration amplifies: with the usual coefficients a small singular value grows by a factor of
 // 3.44 a step, 485 over five, and so does every rounding of X in its direction.  So X, A and W are kept in 32 bits, and enter
@@ -29,12 +29,13 @@
 //
 // Sums.  The tensor cores round their accumulator towards zero, by 0.5 to 0.8 of a unit in the last place for every 16
 // elements of the contraction: 13 units of a sum of 256 positive terms, 65 of 1024.  In A that shortens the diagonal, and steps
-// with A amplify it.  So in symmetric products an accumulator takes up 128 elements of the contraction, the small products of
-// each block of 64 first, and is then added, rounded to nearest, to the sums that the epilogue's warps hold in registers; in
-// Q X, which nothing amplifies, 256.  The products go on in the next accumulator meanwhile.  Measured error of the result
-// against 64 bits, with 64 / 128 / 256 elements (and of fp32 products): rank 8 plus noise, 16 x 5000 3.6 / 6.3 / 9.6e-6 (0.8e-6),
-// 1024 x 4096 1.9 / 1.7 / 1.7e-6 (3.2e-6); Gaussian, 400 x 4000 1.5 / 2.2 / 3.3e-5 (0.5e-5), 1024 x 1024 7.5 / 7.6 / 9.9e-6
-// (3.1e-6); time of 24 of 4864 x 896 3866 / 3669 / 3592 us.
+// with A amplify it.  So in symmetric products an accumulator takes up 64 elements of the contraction where a cluster shares
+// it (matrices with few rows for their length, which lose most, are there; 896 x 4864 267 for 262 us with 128), else 128, the
+// small products of each block of 64 first, and is then added, rounded to nearest, to the sums that the epilogue's warps hold
+// in registers; in Q X, which nothing amplifies, 256.  The products go on in the next accumulator meanwhile.  Measured error
+// of the result against 64 bits, with 64 / 128 / 256 elements throughout (and of fp32 products): rank 8 plus noise, 16 x 5000
+// 3.6 / 6.3 / 9.6e-6 (0.8e-6), 1024 x 4096 1.9 / 1.7 / 1.7e-6 (3.2e-6); Gaussian, 400 x 4000 1.5 / 2.2 / 3.3e-5 (0.5e-5), 1024 x 1024
+// 7.5 / 7.6 / 9.9e-6 (3.1e-6); time of 24 of 4864 x 896 3866 / 3669 / 3592 us.
 #include "sm100_ptx.cuh"
 #include "sm100_pair.cuh"
 #include "common.cuh"
@@ -370,7 +371,8 @@ ns_product_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_consta
   // and the low terms are free before the block is done.
   constexpr int HALF_BYTES = A_BYTES + BNC * 128, HALVES = RING_BYTES / HALF_BYTES / 2 * 2;
   constexpr int ACCS = 512 / BN;                        // accumulators in tensor memory
-  constexpr int DRAIN = MODE == SYM ? 2 : 4;            // blocks of BK that one accumulator takes up: see the header
+  // blocks of BK that one accumulator takes up: see the header
+  constexpr int DRAIN = MODE != SYM ? 4 : KIND == SPLIT ? 1 : 2;
   constexpr int CHUNKS = BN / 64;                       // of 32 x 32 results, per epilogue warp
   extern __shared__ __align__(1024) uint8_t smem[];
   uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + BARRIER_OFFSET);       // (a pair: those of CTA 0 count both CTAs' loads)
