@@ -61,8 +61,8 @@ def _program(steps, coefficients):
             B = b * lam + c * lam * lam
             slot = q if k == 0 else _B
             scales[slot] = scale(B)
-            row(1, _A, _A, slot, c / scales[_A] ** 2, scales[slot], _A, b)
-            last = k + 1 == block
+            last = k + 1 == block                        # (whose Q goes on to X as terms alone: no 32-bit copy of it)
+            row(1, _A, _A, slot, c / scales[_A] ** 2, scales[slot], _A, b, keep=k > 0 or not last)
             if not last:
                 scales[_W] = scale((a + B) * lam)
                 row(2 if k else 1, slot, _A, _W, 1.0 / (scales[slot] * scales[_A]), scales[_W], _A, a)
@@ -70,7 +70,7 @@ def _program(steps, coefficients):
             if k:
                 old_q, q = q, _Q[1 - _Q.index(q)]
                 scales[q] = scale(new - ident * a)
-                row(1, _B, old_q, q, 1.0 / (scales[_B] * scales[old_q]), scales[q], old_q, a, _B, ident)
+                row(1, _B, old_q, q, 1.0 / (scales[_B] * scales[old_q]), scales[q], old_q, a, _B, ident, keep=not last)
             total, ident = new, ident * a
             if not last:
                 lam = lam * (a + B) ** 2

@@ -70,3 +70,20 @@ def test_a_norm_beyond_32_bits():
     big = genesis.optim.orthogonalize(T(x * 1e38))._t
     # scaling rounds each element once more, 2^-24 of it, which the iteration amplifies by 485 at most; as much for the products
     assert float((big - genesis.optim.orthogonalize(T(x))._t).abs().max()) < 485 * 2.0 ** -24 * 4
+
+
+def test_no_result_is_kept_in_32_bits_that_nothing_reads():
+    from genesis_b200.optim.muon import COEFFICIENTS, _program
+    for steps in (1, 2, 3, 4, 5, 7, 8):
+        flat = list(_program(steps, COEFFICIENTS))
+        rows = [flat[i:i + 12] for i in range(0, len(flat), 12)]
+        for i, (kind, _, _, out, _, _, keep, *_) in enumerate(rows):
+            if kind == 3:
+                continue
+            read = False
+            for j in range(i + 1, len(rows)):
+                # the launch that a row of kind 2 shares with the next one reads before either has written
+                read |= out in rows[j][4:6] and not (kind == 2 and j == i + 1)
+                if rows[j][0] in (0, 3) or rows[j][3] == out:
+                    break
+            assert bool(keep) == read, (steps, i)
