@@ -1652,7 +1652,7 @@ def policy_loss(logits, tokens, old_log_probs, advantages, ref_log_probs=None, c
     z, shape = logits._t, tuple(t.shape)
     lo = 1.0 - _number(name, "clip", clip, 0.0, 1.0)
     hi = 1.0 + _number(name, "clip_high", clip if clip_high is None else clip_high, 0.0, math.inf)
-    kl = _number(name, "kl_coef", kl_coef, 0.0, math.inf)
+    kl = _number(name, "kl_coef", kl_coef, 0.0, 1e30)    # (a weight that is infinite in 32 bits would make a term of 0 a NaN)
     if ref_log_probs is None and kl > 0.0:
         raise ValueError(f"{name}: a positive kl_coef needs ref_log_probs")
     old = _constant(name, "old_log_probs", old_log_probs, (shape,), z)
@@ -1680,7 +1680,7 @@ def preference_loss(logits, tokens, ref_log_probs, beta=0.1, label_smoothing=0.0
     z = logits._t
     if z.dim() != 3 or z.shape[0] % 2:
         raise ValueError(f"{name}: logits must be [2 P, T, V], chosen answers before rejected ones, got {tuple(z.shape)}")
-    beta = _number(name, "beta", beta, 0.0, math.inf)
+    beta = _number(name, "beta", beta, 0.0, 1e30)
     smoothing = _number(name, "label_smoothing", label_smoothing, 0.0, 1.0)
     ref = _constant(name, "ref_log_probs", ref_log_probs, ((z.shape[0],),), z, keep_64=True)
     rewards = []

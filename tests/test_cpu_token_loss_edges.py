@@ -62,3 +62,14 @@ def test_rows_beyond_what_the_kernels_count_are_refused_in_words():
             native.check_token_logits(one.expand(shape))
     for shape in ((1, 2 ** 30), (2 ** 28 - 1, 4), (0, 5), (2, 0, 5)):
         native.check_token_logits(one.expand(shape))
+
+
+@pytest.mark.parametrize("weight", [math.inf, 1e39, math.nan, -0.1])
+def test_weights_that_are_not_finite_in_32_bits_are_refused(weight):
+    """0 times infinity would be the loss of tokens that are as likely as the reference's, and of equal answers."""
+    x, t, row = T(torch.randn(2, 3, 5)), T(torch.zeros(2, 3, dtype=torch.int64)), T(torch.zeros(2, 3))
+    with pytest.raises(ValueError):
+        F.policy_loss(x, t, row, row, row, kl_coef=weight)
+    with pytest.raises(ValueError):
+        F.preference_loss(x, t, T(torch.zeros(2)), beta=weight)
+    assert math.isfinite(F.policy_loss(x, t, row, row, clip_high=math.inf).item())
