@@ -124,7 +124,8 @@ class GraphedTrainStep(GraphedCallable):
     the step is captured once and every call replays it: inputs are copied into the static buffers, a changed
     `optimizer.lr` is written to the optimizer's device vector, and the returned loss is the static tensor the
     capture produced (valid until the next call).  Gradients stay readable in `p.grad` after a replay.  `optimizer` may be
-    a list, for steps in which several update their parameters (Muon and AdamW).
+    a list, for steps in which several update their parameters (Muon and AdamW).  `optimizer.load_state_dict` between calls
+    writes into the buffers that the graph reads, so the next call goes on from the loaded state.
     Restrictions: fixed input shapes, no host reads inside `step_fn`, no dropout, one GPU.
     """
 

@@ -5,6 +5,12 @@
 
 The orthogonalisation (`csrc/newton_schulz.cu`) works on all matrices of one shape, and its transpose, at once.  Vectors, embeddings and
 output heads are left to AdamW: `Muon` takes tensors of two and more dimensions, whose last two are the matrix.
+
+On CUDA, contiguous weights in 32 bits take the kernels, with gradients of any floating-point type of up to 32 bits.  Other weights
+(16-bit or 64-bit ones, transposed views) are updated by library products, one matrix at a time, and not in a captured step.
+A call holds workspace: for m x n matrices, m <= n, 12 bytes for each of m n elements (16 in an optimizer's step) and 40 for each of
+m m, for as many matrices at a time as make up 4 GB, or one (8192 x 8192: 3.5 GB, 3.8 in a step).  `Muon` keeps no low-precision
+copies of its weights (`enable_shadows` of AdamW); autocast converts them in every step.
 """
 import ctypes
 import functools
