@@ -10,7 +10,7 @@ attn64_fwd, attn64_bwd, attn_decode (attn_decode_kernel), ce (ce_fwd16_kernel / 
 addnorm, addnorm_wide (add_rmsnorm_fwd_stream_kernel / rmsnorm_bwd_stream_kernel), moe_combine_bwd (moe_combine_bwd_vec_kernel),
 adam (adam_multi_kernel), swiglu_bwd (swiglu_bwd2d_kernel), rope (rope_vec_kernel),
 token_loss (token_rows_kernel / token_grad_kernel), newton_schulz (ns_product_kernel: with -s 4 -c 7 a block of two steps),
-newton_schulz_small (ns_chain_kernel), reduce_cols (reduce_mid), sort (sort_rows), index (index_get_kernel / index_put_kernel), cat (cat_kernel).
+newton_schulz_small (ns_gram_kernel), reduce_cols (reduce_mid), sort (sort_rows), index (index_get_kernel / index_put_kernel), cat (cat_kernel).
 """
 import sys
 import os

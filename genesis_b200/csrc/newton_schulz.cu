@@ -4,14 +4,15 @@
 //
 // i.e. every singular value s goes to a s + b s^3 + c s^5.  A tall G is handled as its transpose.
 //
-// Products of m x m matrices in place of m x n ones.  With P = a I + B, the next A is P A P, so a block of steps needs X
+// Steps are made one by one, with products of X, A X; or, for long and many matrices, in blocks (see one_by_one).
+//
+// Products of m x m matrices in place of m x n ones, in a block.  With P = a I + B, the next A is P A P, so a block of steps needs X
 // only at its ends: A = X X^T once, then per step  B = b A + c A A,  W = a A + B A,  A <- a W + B W,  and the product of the
 // P's, kept as s I + Q:  Q <- a Q + s B + B Q.  At the end of the block X <- s X + Q X.  All but the last are symmetric.
 // For 896 x 4864 and five steps in blocks of three and two that is 33 GFLOP for the 62 of five products with X each way, and
 // X passes through memory twice instead of five times; for square matrices it is as many operations.  A rounding of A grows
-// by a^2 a step, so blocks are short: simulated over spectra from Gaussian to rank one plus noise, blocks of up to three come
-// within a factor of two of products with X (256 x 1024: 2.4e-6 for 1.5e-6 Gaussian, 0.6e-6 for 0.5e-6 rank 8 plus noise; fp32
-// products throughout 2.0e-6 and 2.0e-6), five in one lose a digit (5e-6, 21e-6).
+// by a^2 a step, so blocks are of three at most: five in one lose a digit (256 x 1024, simulated, Gaussian and rank 8 plus noise:
+// 5e-6 and 21e-6), and matrices of few rows, which have few roundings else, go without.
 //
 // Arithmetic.  The iteration amplifies: with the usual coefficients a small singular value grows by a factor of
 // 3.44 a step, 485 over five, and so does every rounding of X in its direction.  So X, A and W are kept in 32 bits, and enter
@@ -21,7 +22,8 @@
 // are added in 32 bits from the matrices themselves.  One fp16 term alone loses three digits (1.7e-3).
 //
 // Work.  Of symmetric results only tiles on and below the diagonal are computed, the rest is written as their mirror image by
-// the same epilogue.  A product is one launch over all matrices of a batch (W and Q of a step together), on persistent CTAs:
+// the same epilogue.  A product is one launch over all matrices of a batch (W and Q of a block's step together; for m <= 128, A and B
+// of a step, which then is two launches), on persistent CTAs:
 //   warp 0 TMA producer, warp 1 issues tcgen05.mma, warps 4-11 epilogue; accumulators in all of tensor memory.
 // A block of 64 elements of the contraction brings both terms of both operands and feeds three products.  Tiles too few to
 // fill the GPU are shared by clusters of up to 8 CTAs, each with a part of the contraction; many large ones are worked on by
@@ -32,8 +34,8 @@
 // with A amplify it.  So in symmetric products an accumulator takes up 64 elements of the contraction where a cluster shares
 // it (matrices with few rows for their length, which lose most, are there; 896 x 4864 267 for 262 us with 128), else 128, the
 // small products of each block of 64 first, and is then added, rounded to nearest, to the sums that the epilogue's warps hold
-// in registers; in Q X, which nothing amplifies, 256.  The products go on in the next accumulator meanwhile.  Measured error
-// of the result against 64 bits, with 64 / 128 / 256 elements throughout (and of fp32 products): rank 8 plus noise, 16 x 5000
+// in registers; in the products with X, 256.  The products go on in the next accumulator meanwhile.  Measured error
+// of the result against 64 bits, in blocks, with 64 / 128 / 256 elements throughout (and of fp32 products): rank 8 plus noise, 16 x 5000
 // 3.6 / 6.3 / 9.6e-6 (0.8e-6), 1024 x 4096 1.9 / 1.7 / 1.7e-6 (3.2e-6); Gaussian, 400 x 4000 1.5 / 2.2 / 3.3e-5 (0.5e-5), 1024 x 1024
 // 7.5 / 7.6 / 9.9e-6 (3.1e-6); time of 24 of 4864 x 896 3866 / 3669 / 3592 us.
 #include "sm100_ptx.cuh"
@@ -675,39 +677,30 @@ ns_product_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_consta
   }
 }
 
-// A block's products of m x m matrices for m <= 128, and often A = X X^T before them, in one launch: one CTA per matrix, all
-// matrices in its shared memory.  Launched one by one they take 8 us each, of which the products are one; here 2.1 us (128 x 896,
-// five steps: 148 -> 81 us).  Three slots hold terms, [two halves of the columns][hi, lo][128 rows of 128 bytes], swizzled as
-// the tensor cores read them: R (A, then W in its place, then the next A), B and Q; a result is written where the operand that
-// it replaces has been read from.  A thread keeps a quarter of a row of A or W in 32 bits in registers.  Rows and columns past
-// m are zero throughout.
-constexpr int CHAIN_THREADS = 512;
-constexpr int CHAIN_SLOT = 4 * 128 * 128;
-constexpr int CHAIN_BARRIERS = 3 * CHAIN_SLOT;
-constexpr int CHAIN_SMEM = CHAIN_BARRIERS + 64;
+// B = b A + c A A for m <= 128, and often A = X X^T before it, in one launch: one CTA per matrix, A in its shared memory.  Launched one
+// by one the two take 8 us each, of which the products are one or two.  Three slots hold terms, [two halves of the columns][hi, lo]
+// [128 rows of 128 bytes], swizzled as the tensor cores read them: blocks of X in turn, then A in the first.  A thread keeps a
+// quarter of a row of A in 32 bits in registers.  Rows and columns past m are zero throughout.
+constexpr int GRAM_THREADS = 512;
+constexpr int GRAM_SLOT = 4 * 128 * 128;
+constexpr int GRAM_BARRIERS = 3 * GRAM_SLOT;
+constexpr int GRAM_SMEM = GRAM_BARRIERS + 64;
 
-struct ChainStep {
-  float sq_acc, sq_a;          // B = sq_acc A A + sq_a A, 2^k of its terms
-  float sq_scale;
-  float w_acc, w_a, w_scale;   // W = w_acc B A + w_a A
-  float a_acc, a_w, a_scale;   // A <- a_acc B W + a_w W
-  float q_acc, q_q, q_b, q_scale;      // Q <- q_acc B Q + q_q Q + q_b B
-};
-struct Chain {
+struct Gram {
   int* status;
-  int m, batch, lda, steps;    // up to 3
+  int m, batch, lda;
   int blocks;                  // X in blocks of 128 columns, from which A is formed here; 0: A is there
   float gram, gram_scale;      // A = gram X X^T, 2^k of its terms
+  float b_acc, b_a, b_scale;   // B = b_acc A A + b_a A, 2^k of its terms
   const float* a;              // A in 32 bits (slot 0)
-  __half* q;                   // terms of Q [batch][hi, lo][m][lda]
-  ChainStep step[3];
+  __half* b;                   // terms of B [batch][hi, lo][m][lda]
 };
 
-__global__ void __launch_bounds__(CHAIN_THREADS, 1)
-ns_chain_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_constant__ CUtensorMap tmapX,
-                const __grid_constant__ Chain p) {
+__global__ void __launch_bounds__(GRAM_THREADS, 1)
+ns_gram_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_constant__ CUtensorMap tmapX,
+                const __grid_constant__ Gram p) {
   extern __shared__ __align__(1024) uint8_t smem[];
-  uint64_t* loaded = reinterpret_cast<uint64_t*>(smem + CHAIN_BARRIERS);
+  uint64_t* loaded = reinterpret_cast<uint64_t*>(smem + GRAM_BARRIERS);
   uint64_t* done = loaded + 3;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -735,15 +728,12 @@ ns_chain_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_constant
 
   const int row = (warp & 3) * 32 + lane, col0 = (warp >> 2) * 32;       // this thread's part of a row
   float whole[32];
-  uint8_t* slot_r = smem;
-  uint8_t* slot_b = smem + CHAIN_SLOT;
-  uint8_t* slot_q = smem + 2 * CHAIN_SLOT;
   const uint32_t idesc = make_idesc(0u, 0u, 0u, 128, 128);
   uint32_t phase = 0;                                    // of done[0]
   bool ok = work;
-  // accumulators `buf` = L R, by warp 0
-  auto issue = [&](const uint8_t* left, const uint8_t* right, int buf) {
-    const uint64_t l = make_smem_desc(smem_u32(left), 16, 1024), r = make_smem_desc(smem_u32(right), 16, 1024);
+  // accumulators `buf` = S S^T for a slot S, by warp 0 (A is its own transpose)
+  auto issue = [&](const uint8_t* slot, int buf) {
+    const uint64_t l = make_smem_desc(smem_u32(slot), 16, 1024), r = l;
     const uint32_t acc = tmem + buf * 256;
     if (elect_one()) {
       // the small products and half of the large ones in one accumulator, the others in a second one
@@ -773,47 +763,21 @@ ns_chain_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_constant
 #pragma unroll
     for (int j = 0; j < 32; ++j) r[j] = __uint_as_float(a[j]) + __uint_as_float(b[j]);
   };
-  // accumulators 0 = L R; every thread waits for them
-  auto multiply = [&](const uint8_t* left, const uint8_t* right) {
-    fence_proxy_async_smem();
-    tc_fence_before_sync();
-    __syncthreads();                                     // operands written, the last accumulator read
-    tc_fence_after_sync();
-    if (warp == 0 && ok) issue(left, right, 0);
-    if (ok) ok = mbar_wait(&done[0], phase, abort_flag, p.status, 410);
-    ok = __syncthreads_and(ok);
-    phase ^= 1;
-    tc_fence_after_sync();
-  };
-  // unit u (8 columns) of the thread's part of a row in a slot: hi, and lo 16 KB on
-  auto unit = [&](uint8_t* slot, int u) {
-    return slot + (warp >> 3) * 32768 + row * 128 + ((((warp >> 2) & 1) * 4 + u) ^ (row & 7)) * 16;
-  };
-  auto put = [&](uint8_t* slot, int u, const float (&v)[8], float scale) {
-    const uint4 s = split4(v[0] * scale, v[1] * scale, v[2] * scale, v[3] * scale), t = split4(v[4] * scale, v[5] * scale, v[6] * scale, v[7] * scale);
-    uint8_t* at = unit(slot, u);
-    *reinterpret_cast<uint4*>(at) = make_uint4(s.x, s.y, t.x, t.y);
-    *reinterpret_cast<uint4*>(at + 16384) = make_uint4(s.z, s.w, t.z, t.w);
-  };
-  auto get = [&](uint8_t* slot, int u, float (&v)[8], float factor) {
-    const uint8_t* at = unit(slot, u);
-    const uint4 hi = *reinterpret_cast<const uint4*>(at), lo = *reinterpret_cast<const uint4*>(at + 16384);
-    const uint32_t h[4] = {hi.x, hi.y, hi.z, hi.w}, l[4] = {lo.x, lo.y, lo.z, lo.w};
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&h[k])), b = __half22float2(*reinterpret_cast<const __half2*>(&l[k]));
-      v[2 * k] = (a.x + b.x) * factor;
-      v[2 * k + 1] = (a.y + b.y) * factor;
-    }
+  // the terms of 8 columns from 8 u on of the thread's part of a row, as they lie in memory: hi, lo
+  auto terms = [&](const float (&v)[32], int u, float scale, uint4& hi, uint4& lo) {
+    const uint4 s = split4(v[8 * u] * scale, v[8 * u + 1] * scale, v[8 * u + 2] * scale, v[8 * u + 3] * scale);
+    const uint4 t = split4(v[8 * u + 4] * scale, v[8 * u + 5] * scale, v[8 * u + 6] * scale, v[8 * u + 7] * scale);
+    hi = make_uint4(s.x, s.y, t.x, t.y);
+    lo = make_uint4(s.z, s.w, t.z, t.w);
   };
   if (p.blocks > 0) {
     // A = X X^T: the slots are a ring of blocks of X; while one is multiplied, the products of the last are added up
     auto load = [&](int d) {
       const int i = d % 3;
-      mbar_expect_tx(&loaded[i], CHAIN_SLOT);
+      mbar_expect_tx(&loaded[i], GRAM_SLOT);
 #pragma unroll
       for (int k = 0; k < 4; ++k)
-        tma_load_3d(smem + i * CHAIN_SLOT + k * 16384, &tmapX, &loaded[i], d * 128 + (k >> 1) * 64, 0, 2 * z + (k & 1));
+        tma_load_3d(smem + i * GRAM_SLOT + k * 16384, &tmapX, &loaded[i], d * 128 + (k >> 1) * 64, 0, 2 * z + (k & 1));
     };
     int issued = 0;
     if (work && threadIdx.x == 0)
@@ -823,7 +787,7 @@ ns_chain_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_constant
     for (int d = 0; d <= p.blocks; ++d) {
       if (warp == 0 && d < p.blocks && ok) {
         ok = __all_sync(0xffffffffu, mbar_wait(&loaded[d % 3], (d / 3) & 1, abort_flag, p.status, 411));
-        if (ok) issue(smem + d % 3 * CHAIN_SLOT, smem + d % 3 * CHAIN_SLOT, d & 1);
+        if (ok) issue(smem + d % 3 * GRAM_SLOT, d & 1);
       }
       if (d > 0) {
         const int e = d - 1;
@@ -847,18 +811,20 @@ ns_chain_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_constant
     phase = ((p.blocks + 1) / 2) & 1;
 #pragma unroll
     for (int j = 0; j < 32; ++j) whole[j] *= p.gram;
+    // A's terms into the first slot: every product has been waited for
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      float v[8];
-#pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] = whole[8 * u + k];
-      put(slot_r, u, v, p.gram_scale);
+      uint4 hi, lo;
+      terms(whole, u, p.gram_scale, hi, lo);
+      uint8_t* at = smem + (warp >> 3) * 32768 + row * 128 + ((((warp >> 2) & 1) * 4 + u) ^ (row & 7)) * 16;
+      *reinterpret_cast<uint4*>(at) = hi;
+      *reinterpret_cast<uint4*>(at + 16384) = lo;
     }
   } else {
     if (work && threadIdx.x == 0) {
-      mbar_expect_tx(loaded, CHAIN_SLOT);
+      mbar_expect_tx(loaded, GRAM_SLOT);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) tma_load_3d(slot_r + i * 16384, &tmapA, loaded, (i >> 1) * 64, 0, 2 * z + (i & 1));
+      for (int i = 0; i < 4; ++i) tma_load_3d(smem + i * 16384, &tmapA, loaded, (i >> 1) * 64, 0, 2 * z + (i & 1));
     }
     const float* a = p.a + ((size_t)z * p.m + row) * p.lda + col0;
 #pragma unroll
@@ -874,64 +840,27 @@ ns_chain_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_constant
     ok = __syncthreads_and(ok);
     if (work && !ok && threadIdx.x == 0) drain_copies(loaded, 1, 1);
   }
-  float q_unscale = 1.f;                                 // 1 / 2^k of Q's terms
-  for (int s = 0; s < p.steps; ++s) {
-    const ChainStep& c = p.step[s];
-    uint8_t* into = s == 0 ? slot_q : slot_b;            // the first B is Q
-    multiply(slot_r, slot_r);
-    float r[32];
-    take(r, 0);
+  fence_proxy_async_smem();
+  tc_fence_before_sync();
+  __syncthreads();                                       // A is there, the last accumulator has been read
+  tc_fence_after_sync();
+  if (warp == 0 && ok) issue(smem, 0);
+  if (ok) ok = mbar_wait(&done[0], phase, abort_flag, p.status, 410);
+  ok = __syncthreads_and(ok);
+  tc_fence_after_sync();
+  float r[32];
+  take(r, 0);
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      float v[8];
-#pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] = fmaf(r[8 * u + k], c.sq_acc, whole[8 * u + k] * c.sq_a);
-      put(into, u, v, c.sq_scale);
-    }
-    if (s > 0) {
-      multiply(slot_b, slot_q);
-      const float b_unscale = 1.f / c.sq_scale;          // (powers of two)
-      take(r, 0);
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        float q[8], b[8];
-        get(slot_q, u, q, q_unscale * c.q_q);
-        get(slot_b, u, b, b_unscale * c.q_b);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) q[k] = fmaf(r[8 * u + k], c.q_acc, q[k]) + b[k];
-        put(slot_q, u, q, c.q_scale);
-      }
-      q_unscale = 1.f / c.q_scale;
-    } else {
-      q_unscale = 1.f / c.sq_scale;
-    }
-    if (s + 1 == p.steps) break;
-    uint8_t* left = s == 0 ? slot_q : slot_b;            // (B; the next step's products with Q come after its own B)
-#pragma unroll 1
-    for (int twice = 0; twice < 2; ++twice) {            // W in the place of A, then A in the place of W
-      const float acc = twice ? c.a_acc : c.w_acc, own = twice ? c.a_w : c.w_a, scale = twice ? c.a_scale : c.w_scale;
-      multiply(left, slot_r);
-      take(r, 0);
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        float v[8];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const int j = 8 * u + k;
-          whole[j] = v[k] = fmaf(r[8 * u + k], acc, whole[j] * own);
-        }
-        put(slot_r, u, v, scale);
-      }
-    }
-  }
+  for (int j = 0; j < 32; ++j) whole[j] = fmaf(r[j], p.b_acc, whole[j] * p.b_a);
   if (ok && row < p.m) {
-    __half* q = p.q + ((size_t)z * 2 * p.m + row) * p.lda + col0;
+    __half* b = p.b + ((size_t)z * 2 * p.m + row) * p.lda + col0;
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      if (col0 + 8 * u < p.m) {
-        const uint8_t* at = unit(slot_q, u);
-        *reinterpret_cast<uint4*>(q + 8 * u) = *reinterpret_cast<const uint4*>(at);
-        *reinterpret_cast<uint4*>(q + (size_t)p.m * p.lda + 8 * u) = *reinterpret_cast<const uint4*>(at + 16384);
+      if (col0 + 8 * u < p.m) {                          // (elements of the last vector past m are zero, and padding)
+        uint4 hi, lo;
+        terms(whole, u, p.b_scale, hi, lo);
+        *reinterpret_cast<uint4*>(b + 8 * u) = hi;
+        *reinterpret_cast<uint4*>(b + (size_t)p.m * p.lda + 8 * u) = lo;
       }
     }
   }
@@ -1162,15 +1091,12 @@ static int max_clusters(int size) {
 // 1700 with 256, bound by shared memory (213 and 160 bytes a clock at the full tensor rate, of 128), or 2100 where all SMs
 // together read more than L2 gives (11 TB/s); pairs read two thirds of that and take 1600.  The epilogue of the last tile,
 // which no products hide, takes 6500 for each chunk of a warp; the parts of a cluster 4000 to meet and 5000 a chunk.
-struct Plan { int kind, bn, splits, grid; };
+struct Plan { int kind, bn, splits, grid; long long clocks; };
 static Plan plan(bool sym, int m, int n, int k, long long matrices) {
   const long long sms = sm_count(), kblocks = (k + BK - 1) / BK;
-  Plan best{WHOLE, 128, 1, 0};
-  long long least = -1;
+  Plan best{WHOLE, 128, 1, 0, -1};
   auto offer = [&](long long clocks, int kind, int width, int splits, long long ctas) {
-    if (least >= 0 && clocks >= least) return;
-    least = clocks;
-    best = Plan{kind, width, splits, (int)ctas};
+    if (best.clocks < 0 || clocks < best.clocks) best = Plan{kind, width, splits, (int)ctas, clocks};
   };
   for (int width = 128; width <= 256; width += 128) {
     const long long total = tiles_of(sym, m, n, BM, width) * matrices, waves = (total + sms - 1) / sms;
@@ -1194,10 +1120,31 @@ static int product(const CUtensorMap& ta, const CUtensorMap& tb, Params p, cudaS
   return c.bn == 256 ? launch<MODE, 256, WHOLE>(ta, tb, p, c.grid, st) : launch<MODE, 128, WHOLE>(ta, tb, p, c.grid, st);
 }
 
-// Whether ns_chain_kernel forms A = X X^T itself: its one CTA takes 2700 clocks for 128 columns of X; a launch of its own 1080
+// The clocks of a program's products (see gb_newton_schulz), each a launch with 10000 to start and to end.
+static long long clocks(const double* program, int count, int m, int n, int batch) {
+  long long total = 0;
+  for (int i = 0; i < count; ++i) {
+    const int kind = (int)program[12 * i], problems = kind == 2 && i + 1 < count ? 2 : 1;
+    total += plan(kind != 3, m, n, kind == 0 ? n : m, (long long)batch * problems).clocks + 10000;
+    i += problems - 1;
+  }
+  return total;
+}
+
+// Whether steps are made one by one, not in blocks.  One by one they are as exact as 32-bit products: X X^T is formed anew for each.
+// In blocks it is carried on, and its roundings with it: error over that of 32-bit products, one by one / in blocks, for gradients of a
+// few strong directions over small ones and for Gaussian matrices: 16 x 5000 1.0 / 5.1 and 1.2 / 2.6, 128 x 896 1.0 / 1.7 and 1.0 / 4.5,
+// 256 x 1024 0.5 / 0.8 and 0.8 / 2.6, 896 x 4864 0.5 / 0.6 and 0.5 / 2.6.  So blocks are for matrices of more than 192 rows, and where
+// they save a tenth of the time: of long and many ones, where operations count.  One by one / in blocks, us: 128 x 896 124 / 83,
+// 256 x 1024 154 / 175, 896 x 896 200 / 219, eight of them 506 / 608, 896 x 4864 316 / 272, 24 of them 4810 / 3242.
+static bool one_by_one(const double* blocks, int blocks_count, const double* single, int single_count, int m, int n, int batch) {
+  return m <= 192 || clocks(single, single_count, m, n, batch) * 9 <= clocks(blocks, blocks_count, m, n, batch) * 10;
+}
+
+// Whether ns_gram_kernel forms A = X X^T itself: its one CTA takes 2700 clocks for 128 columns of X; a launch of its own 1080
 // for 64 of them, shared by as many CTAs as there are SMs to a matrix, 8 at most, and 21000 besides (its start, the parts' meeting
-// and A's way through memory).  Five steps, own launch / here, us: 128 x 128 87.7 / 66.3, 128 x 896 88.2 / 82.3, 128 x 2048
-// 91.9 / 107.3, 100 of 128 x 4864 618 / 608.
+// and A's way through memory).  Five steps, own launch / here, us: 128 x 128 128 / 85, 128 x 896 140 / 124, 128 x 2048 145 / 184,
+// 100 of 128 x 4864 1316 / 1253.
 static bool folds(int n, int batch) {
   const long long kblocks = (n + BK - 1) / BK;
   int s = 1;
@@ -1205,16 +1152,16 @@ static bool folds(int n, int batch) {
   return (n + 127) / 128 * 2700ll <= kblocks * 1080 / s + 21000;
 }
 
-static int chain(const CUtensorMap& ta, const CUtensorMap& tx, const Chain& c, cudaStream_t st) {
+static int gram(const CUtensorMap& ta, const CUtensorMap& tx, const Gram& c, cudaStream_t st) {
   static unsigned long long configured = 0;
-  if (int r = smem_opt_in(ns_chain_kernel, CHAIN_SMEM, configured)) return r;
+  if (int r = smem_opt_in(ns_gram_kernel, GRAM_SMEM, configured)) return r;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.gridDim = dim3((unsigned)c.batch); cfg.blockDim = dim3(CHAIN_THREADS); cfg.dynamicSmemBytes = CHAIN_SMEM; cfg.stream = st;
+  cfg.gridDim = dim3((unsigned)c.batch); cfg.blockDim = dim3(GRAM_THREADS); cfg.dynamicSmemBytes = GRAM_SMEM; cfg.stream = st;
   cfg.attrs = attr; cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, ns_chain_kernel, ta, tx, c);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, ns_gram_kernel, ta, tx, c);
   return e == cudaSuccess ? (int)cudaGetLastError() : (int)e;
 }
 
@@ -1258,6 +1205,12 @@ extern "C" int gb_ns_plan(int sym, int m, int n, int k, int batch, int problems,
   return 0;
 }
 
+// Whether gb_newton_schulz takes the second program
+extern "C" int gb_ns_one_by_one(const double* blocks, int blocks_count, const double* single, int single_count, int m, int n,
+                                int batch) {
+  return ns::one_by_one(blocks, blocks_count, single, single_count, m, n, batch) ? 1 : 0;
+}
+
 // First half of an optimizer step: see muon_momentum_kernel.  The update and its partial sums stay in the workspace.
 extern "C" int gb_muon_momentum(const long long* table, int batch, int grad_dt, int m, int n, double mu, int nesterov,
                                 const float* grad_scale, const float* found_inf, void* workspace, cudaStream_t st) {
@@ -1273,16 +1226,20 @@ extern "C" int gb_muon_momentum(const long long* table, int batch, int grad_dt, 
 // Orthogonalises `batch` matrices [m, n], or [n, m] (tall), m <= n.  `src` (contiguous, dtype dt) with `out` of the same type;
 // or src null for the updates that gb_muon_momentum has left in the workspace, which go into the weights whose addresses
 // `weights` [batch] holds (+ 1 for a tall one).
-// The products to be made are `count` rows of 12 numbers in `program`: kind (0 X X^T, 1 symmetric, 2 the same and to be
+// The products to be made are rows of 12 numbers, in two programs for the same steps: `blocks` of steps, and steps `single`, one by
+// one, which are taken where one_by_one says so, and always for m <= 128.  A row: kind (0 X X^T, 1 symmetric, 2 the same and to be
 // launched together with the next row, 3 X <- Q X + ..), left, right and out slots, M1 and M2 slots or -1, whether the result
 // is kept in 32 bits, f_acc, f1, f2, the power of two of the result's terms, 0.  The first row's last number: the power of
 // two of the first X's terms.  The last row is of kind 3.
-extern "C" int gb_newton_schulz(const void* src, void* out, int dt, int m, int n, int tall, int batch, const double* program,
-                                int count, double eps, const long long* weights, float lr, float decay, float tall_scale,
+extern "C" int gb_newton_schulz(const void* src, void* out, int dt, int m, int n, int tall, int batch, const double* blocks,
+                                int blocks_count, const double* single, int single_count, double eps, const long long* weights, float lr, float decay, float tall_scale,
                                 const float* dyn_lr, const float* found_inf, void* workspace, int* status, cudaStream_t st) {
   if (batch <= 0 || m <= 0 || n <= 0) return 0;
-  if (batch > 6000 || m > n || n > (1 << 30) || count < 2 || (src == nullptr) != (weights != nullptr) ||
+  if (batch > 6000 || m > n || n > (1 << 30) || blocks_count < 2 || single_count < 2 || (src == nullptr) != (weights != nullptr) ||
       (reinterpret_cast<uintptr_t>(workspace) & 255) != 0) return -3;
+  const bool one = ns::one_by_one(blocks, blocks_count, single, single_count, m, n, batch);
+  const double* program = one ? single : blocks;
+  const int count = one ? single_count : blocks_count;
   const int ldx = (n + 7) & ~7, lda = (m + 7) & ~7;
   const ns::Workspace w((uint8_t*)workspace, m, n, batch, src == nullptr);
   const int parts = ns::norm_parts((long long)m * n);
@@ -1337,29 +1294,16 @@ extern "C" int gb_newton_schulz(const void* src, void* out, int dt, int m, int n
     }
     if (r != 0) return r;
     if (kind == 0 && m <= 128) {
-      // the rows up to the next X at once; a row is told by its result and operands
-      ns::Chain c = {};
+      // the next row, B, from A in the same launch, or in one of its own kind
+      if (++i >= count || program[12 * i] != 1.0 || program[12 * i + 1] != 0.0 || program[12 * i + 2] != 0.0) return -3;
+      const double* o = program + 12 * i;
+      if (!(o[3] >= 1 && o[3] < ns::SLOTS)) return -3;
+      ns::Gram c = {};
       c.status = status; c.m = m; c.batch = batch; c.lda = lda; c.a = w.whole;
       c.blocks = fold ? (n + 127) / 128 : 0; c.gram = p.prob[0].f_acc; c.gram_scale = p.prob[0].scale;
-      for (++i; i < count && program[12 * i] != 3.0; ++i) {
-        const double* o = program + 12 * i;
-        const int out_slot = (int)o[3];
-        if (o[1] == 0.0 && o[2] == 0.0) {
-          if (c.steps == 3) return -3;
-          ns::ChainStep& t = c.step[c.steps++];
-          t.sq_acc = (float)o[7]; t.sq_a = (float)o[8]; t.sq_scale = (float)o[10];
-        } else {
-          if (c.steps == 0) return -3;
-          ns::ChainStep& t = c.step[c.steps - 1];
-          if (out_slot == 1) { t.w_acc = (float)o[7]; t.w_a = (float)o[8]; t.w_scale = (float)o[10]; }
-          else if (out_slot == 0) { t.a_acc = (float)o[7]; t.a_w = (float)o[8]; t.a_scale = (float)o[10]; }
-          else { t.q_acc = (float)o[7]; t.q_q = (float)o[8]; t.q_b = (float)o[9]; t.q_scale = (float)o[10]; }
-        }
-      }
-      if (i == count || c.steps == 0) return -3;
-      c.q = w.terms + (size_t)program[12 * i + 1] * batch * 2 * m * lda;
-      if ((r = ns::chain(ms, mx[cur], c, st)) != 0) return r;
-      --i;                                               // (the loop goes on with the row of the next X)
+      c.b_acc = (float)o[7]; c.b_a = (float)o[8]; c.b_scale = (float)o[10];
+      c.b = w.terms + (size_t)o[3] * batch * 2 * m * lda;
+      if ((r = ns::gram(ms, mx[cur], c, st)) != 0) return r;
     }
   }
   return 0;

@@ -73,7 +73,8 @@ _SIGS = {
     "gb_preference_loss": "pppp" + "lllll" + "l" + "pi" + "l" + "dd" + "i" + "ppppp" + "ii" + "pp",
     "gb_token_grad": "pppp" + "lllll" + "l" + "d" + "pl" + "pll" + "p" + "f" + "ii" + "p",
     "gb_ns_plan": "iiiiiip", "gb_ns_workspace": "lllip", "gb_muon_momentum": "p" + "iiii" + "d" + "i" + "ppp" + "p",
-    "gb_newton_schulz": "pp" + "iiiii" + "p" + "i" + "d" + "p" + "fff" + "pp" + "pp" + "p",
+    "gb_ns_one_by_one": "pipiiii",
+    "gb_newton_schulz": "pp" + "iiiii" + "pi" + "pi" + "d" + "p" + "fff" + "pp" + "pp" + "p",
 }
 
 _L = None
@@ -2003,6 +2004,11 @@ def _ns_batch(m, n):
 _NS_LONGEST = 1 << 30           # of a matrix's sides: the kernels count rows, columns and their tiles in 32 bits
 
 
+def _programs(programs):
+    """Both programs of products (`optim.muon._program`), with their numbers of rows."""
+    return [x for p in programs for x in (p, len(p) // 12)]
+
+
 def newton_schulz(x, steps, coefficients, eps, program):
     """Orthogonalised matrices of contiguous x [batch, rows, cols], in its type."""
     if x.dtype not in _FLOATS or not x.is_contiguous() or max(x.shape[-2:]) > _NS_LONGEST:
@@ -2016,7 +2022,7 @@ def newton_schulz(x, steps, coefficients, eps, program):
             count = min(per, batch - i)
             ws = _ns_workspace(m, n, count, False, x.device)
             _chk(lib().gb_newton_schulz(x[i].data_ptr(), out[i].data_ptr(), _DT[x.dtype], m, n, 1 if rows > cols else 0, count,
-                                        program, len(program) // 12, eps, None, 0.0, 0.0, 0.0, None, None, ws.data_ptr(),
+                                        *_programs(program), eps, None, 0.0, 0.0, 0.0, None, None, ws.data_ptr(),
                                         status_tensor(x.device).data_ptr(), _st()), "newton_schulz")
     return out
 
@@ -2048,7 +2054,7 @@ def muon_step(params, grads, bufs, shape, lr, momentum, nesterov, weight_decay, 
             ws = _ns_workspace(m, n, count, True, dev)
             _chk(lib().gb_muon_momentum(table.data_ptr(), count, _DT[gdt], m, n, float(momentum), 1 if nesterov else 0,
                                         _ptr(grad_scale), _ptr(found_inf), ws.data_ptr(), _st()), "muon_momentum")
-            _chk(lib().gb_newton_schulz(None, None, 0, m, n, 0, count, program, len(program) // 12, eps,
+            _chk(lib().gb_newton_schulz(None, None, 0, m, n, 0, count, *_programs(program), eps,
                                         table.data_ptr() + 16 * count, float(lr), float(weight_decay), float(scale),
                                         _ptr(dyn_lr), _ptr(found_inf), ws.data_ptr(), status_tensor(dev).data_ptr(), _st()),
                  "newton_schulz")

@@ -31,11 +31,11 @@ _A, _W, _B, _Q = 0, 1, 2, (3, 4)
 
 
 @functools.lru_cache(maxsize=64)
-def _program(steps, coefficients):
+def _program(steps, coefficients, longest=3):
     """The products that `gb_newton_schulz` makes, as an array of 12 numbers each (see there and the head of
     `csrc/newton_schulz.cu`).
 
-    Steps go in blocks of three, or two, between which X is formed anew.  Every matrix is a polynomial in X X^T, so its
+    Steps go one by one (`longest` 1), or in blocks of three, or two, between which X is formed anew.  Every matrix is a polynomial in X X^T, so its
     eigenvalues are followed over all singular values that X may have; the power of two by which its terms are scaled in
     fp16 is the largest that keeps its entries, which no eigenvalue exceeds, below a quarter of fp16's range."""
     a, b, c = coefficients
@@ -51,7 +51,7 @@ def _program(steps, coefficients):
         rows.append([kind, lhs, rhs, out, m1, m2, float(keep), f_acc, f1, f2, out_scale, 0.0])
 
     while left:
-        block = left if left < 4 else 2 if left == 4 else 3
+        block = min(longest, left if left < 4 else 2 if left == 4 else 3)
         left -= block
         s = torch.linspace(0.0, top, 4097, dtype=torch.float64)
         x_scale = scale(s)
@@ -89,6 +89,10 @@ def _program(steps, coefficients):
     return (ctypes.c_double * len(flat))(*flat)
 
 
+def _programs(steps, coefficients):
+    return _program(steps, coefficients), _program(steps, coefficients, 1)
+
+
 def _check(steps, coefficients, eps):
     if isinstance(steps, bool) or not isinstance(steps, int) or not 1 <= steps <= 64:
         raise ValueError(f"steps must be an int from 1 to 64, got {steps!r}")
@@ -97,7 +101,7 @@ def _check(steps, coefficients, eps):
         raise ValueError(f"coefficients must be three finite numbers, got {coefficients}")
     if not 1e-30 <= float(eps) < math.inf:
         raise ValueError(f"eps must be finite and at least 1e-30, got {eps}")
-    return coefficients, float(eps), _program(steps, coefficients)
+    return coefficients, float(eps), _programs(steps, coefficients)
 
 
 def orthogonalize(x, steps=5, coefficients=COEFFICIENTS, eps=1e-7):
@@ -105,8 +109,8 @@ def orthogonalize(x, steps=5, coefficients=COEFFICIENTS, eps=1e-7):
 
     `steps` times X <- a X + (b A + c A A) X with A = X X^T, from X = x / (|x| + eps); a matrix with more rows than columns
     is handled as its transpose.  Whatever the type, products have 22-bit operands and sums 32 bits; on CUDA the result is
-    some 1e-6 to 4e-5 of its norm off, before it is rounded to x's type: as far as 32-bit products where matrices are large, up to
-    six times as far where they have few rows.  Not differentiable.  A matrix that holds an Inf or
+    some 1e-6 to 4e-5 of its norm off, before it is rounded to x's type: about as far as 32-bit products, up to three times as far
+    where long matrices of more than 192 rows take the steps in blocks.  Not differentiable.  A matrix that holds an Inf or
     NaN comes out as NaN; the others of a batch are not touched by it."""
     if not isinstance(x, Tensor) or not x._t.dtype.is_floating_point:
         raise TypeError("orthogonalize: x must be a floating-point Tensor")
@@ -179,7 +183,7 @@ class Muon(Optimizer):
         self.t += 1
         if self._dyn_lr_t is not None and not torch.cuda.is_current_stream_capturing():
             self._sync_lr()
-        program = _program(self.steps, self.coefficients)
+        program = _programs(self.steps, self.coefficients)
         groups = {}
         for i in idx:
             p, g = self.params[i]._t, self.params[i].grad._t

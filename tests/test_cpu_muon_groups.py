@@ -1,4 +1,5 @@
 """Which matrices a Muon step hands to the kernels together."""
+import pytest
 import torch
 
 import genesis_b200 as genesis
@@ -74,8 +75,8 @@ def test_a_norm_beyond_32_bits():
 
 def test_no_result_is_kept_in_32_bits_that_nothing_reads():
     from genesis_b200.optim.muon import COEFFICIENTS, _program
-    for steps in (1, 2, 3, 4, 5, 7, 8):
-        flat = list(_program(steps, COEFFICIENTS))
+    for steps, longest in [(k, n) for k in (1, 2, 3, 4, 5, 7, 8) for n in (3, 1)]:
+        flat = list(_program(steps, COEFFICIENTS, longest))
         rows = [flat[i:i + 12] for i in range(0, len(flat), 12)]
         for i, (kind, _, _, out, _, _, keep, *_) in enumerate(rows):
             if kind == 3:
@@ -87,3 +88,15 @@ def test_no_result_is_kept_in_32_bits_that_nothing_reads():
                 if rows[j][0] in (0, 3) or rows[j][3] == out:
                     break
             assert bool(keep) == read, (steps, i)
+
+
+@pytest.mark.parametrize("steps", [1, 2, 3, 5, 8])
+@pytest.mark.parametrize("coefficients", [(3.4445, -4.7750, 2.0315), (1.5, -0.5, 0.0), (15 / 8, -10 / 8, 3 / 8), (2.0, -1.5, 0.5)])
+def test_program_of_steps_one_by_one(steps, coefficients, monkeypatch):
+    """The same steps without blocks: for each X X^T, the matrix that X is multiplied by, and the product."""
+    import test_cpu_muon
+    from genesis_b200.optim.muon import _program
+    flat = list(_program(steps, coefficients, 1))
+    assert [flat[i] for i in range(0, len(flat), 12)] == [0, 1, 3] * steps
+    monkeypatch.setattr(test_cpu_muon, "_program", lambda s, c: _program(s, c, 1))
+    test_cpu_muon.test_program_of_products(steps, coefficients)
