@@ -12,7 +12,7 @@
 // For 896 x 4864 and five steps in blocks of three and two that is 33 GFLOP for the 62 of five products with X each way, and
 // X passes through memory twice instead of five times; for square matrices it is as many operations.  A rounding of A grows
 // by a^2 a step, so blocks are of three at most: five in one lose a digit (256 x 1024, simulated, Gaussian and rank 8 plus noise:
-// 5e-6 and 21e-6), and matrices of few rows, which have few roundings else, go without.
+// 5e-6 and 21e-6), and matrices of few rows, which have few roundings else, go without (see one_by_one).
 //
 // Arithmetic.  The iteration amplifies: with the usual coefficients a small singular value grows by a factor of
 // 3.44 a step, 485 over five, and so does every rounding of X in its direction.  So X, A and W are kept in 32 bits, and enter
@@ -1132,13 +1132,14 @@ static long long clocks(const double* program, int count, int m, int n, int batc
 }
 
 // Whether steps are made one by one, not in blocks.  One by one they are as exact as 32-bit products: X X^T is formed anew for each.
-// In blocks it is carried on, and its roundings with it: error over that of 32-bit products, one by one / in blocks, for gradients of a
-// few strong directions over small ones and for Gaussian matrices: 16 x 5000 1.0 / 5.1 and 1.2 / 2.6, 128 x 896 1.0 / 1.7 and 1.0 / 4.5,
-// 256 x 1024 0.5 / 0.8 and 0.8 / 2.6, 896 x 4864 0.5 / 0.6 and 0.5 / 2.6.  So blocks are for matrices of more than 192 rows, and where
-// they save a tenth of the time: of long and many ones, where operations count.  One by one / in blocks, us: 128 x 896 124 / 83,
-// 256 x 1024 154 / 175, 896 x 896 200 / 219, eight of them 506 / 608, 896 x 4864 316 / 272, 24 of them 4810 / 3242.
+// In blocks it is carried on, and its roundings with it.  Error over that of 32-bit products, one by one / in blocks, for gradients of
+// a few strong directions over small ones and for Gaussian matrices: 16 x 5000 1.0 / 5.1 and 1.2 / 2.6, 128 x 896 1.0 / 1.7 and 1.0 / 4.5,
+// batches of 200 x 3000 1.0 / 1.7 and 0.9 / 3.6, of 320 x 2000 0.9 / 1.2 and 1.0 / 5.1, of 512 x 2048 0.7 / 0.9 and 1.1 / 4.4, of 896 x 4864
+// 0.5 / 0.6 and 0.9 / 3.1 (1.2e-5 of the norm).  So blocks are for more than 320 rows, and where they save a tenth of the time:
+// long or many matrices, where operations count.  One by one / in blocks, us: 128 x 896 124 / 83, 256 x 1024 154 / 175, 64 of them
+// 521 / 440, 896 x 896 200 / 219, eight of them 506 / 608, 896 x 4864 316 / 272, 24 of them 4810 / 3242.
 static bool one_by_one(const double* blocks, int blocks_count, const double* single, int single_count, int m, int n, int batch) {
-  return m <= 192 || clocks(single, single_count, m, n, batch) * 9 <= clocks(blocks, blocks_count, m, n, batch) * 10;
+  return m <= 320 || clocks(single, single_count, m, n, batch) * 9 <= clocks(blocks, blocks_count, m, n, batch) * 10;
 }
 
 // Whether ns_gram_kernel forms A = X X^T itself: its one CTA takes 2700 clocks for 128 columns of X; a launch of its own 1080

@@ -109,8 +109,8 @@ def orthogonalize(x, steps=5, coefficients=COEFFICIENTS, eps=1e-7):
 
     `steps` times X <- a X + (b A + c A A) X with A = X X^T, from X = x / (|x| + eps); a matrix with more rows than columns
     is handled as its transpose.  Whatever the type, products have 22-bit operands and sums 32 bits; on CUDA the result is
-    some 1e-6 to 4e-5 of its norm off, before it is rounded to x's type: about as far as 32-bit products, up to three times as far
-    where long matrices of more than 192 rows take the steps in blocks.  Not differentiable.  A matrix that holds an Inf or
+    some 1e-6 to 4e-5 of its norm off, before it is rounded to x's type: about as far as 32-bit products; up to six times as far
+    where long or many matrices of more than 320 rows, which take the steps in blocks, have no strong directions.  Not differentiable.  A matrix that holds an Inf or
     NaN comes out as NaN; the others of a batch are not touched by it."""
     if not isinstance(x, Tensor) or not x._t.dtype.is_floating_point:
         raise TypeError("orthogonalize: x must be a floating-point Tensor")

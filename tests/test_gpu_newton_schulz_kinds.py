@@ -87,25 +87,32 @@ KINDS = [
     (True, 3, (SHARED, 128, 4), 1, 449, 461),
     (True, 3, (SHARED, 256, 2), 5, 323, 551),
     (True, 3, (SHARED, 256, 4), 2, 452, 531),
-    (False, 0, (WHOLE, 256, 1), 26, 265, 1825),
-    (False, 0, (WHOLE, 128, 1), 21, 257, 1415),
-    (False, 0, (SHARED, 256, 8), 6, 196, 4762),
-    (False, 0, (PAIRS, 256, 1), 51, 205, 1513),
-    (False, 1, (WHOLE, 128, 1), 14, 257, 1891),
-    (False, 1, (SHARED, 128, 2), 1, 193, 10047),
+    (True, 3, (WHOLE, 256, 1), 42, 260, 13611),
+    (False, 0, (WHOLE, 128, 1), 13, 394, 1446),
+    (False, 0, (WHOLE, 256, 1), 26, 329, 1843),
+    (False, 0, (SHARED, 128, 2), 10, 329, 1866),
+    (False, 0, (SHARED, 128, 4), 3, 389, 3605),
+    (False, 0, (SHARED, 128, 8), 1, 324, 9851),
+    (False, 0, (SHARED, 256, 2), 15, 330, 1684),
+    (False, 0, (SHARED, 256, 4), 4, 388, 2636),
+    (False, 0, (SHARED, 256, 8), 3, 324, 4117),
+    (False, 0, (PAIRS, 256, 1), 15, 392, 1570),
     (False, 1, (SHARED, 128, 4), 1, 460, 5701),
     (False, 1, (SHARED, 256, 2), 15, 321, 1725),
     (False, 1, (SHARED, 256, 4), 5, 455, 1888),
     (False, 1, (PAIRS, 256, 1), 2, 1474, 3219),
-    (False, 2, (WHOLE, 128, 1), 13, 199, 2420),
-    (False, 2, (SHARED, 128, 2), 1, 193, 10047),
+    (False, 1, (WHOLE, 128, 1), 8, 389, 2359),
+    (False, 1, (WHOLE, 256, 1), 1, 2838, 4687),
+    (False, 1, (SHARED, 128, 2), 1, 324, 9851),
     (False, 2, (SHARED, 128, 4), 1, 460, 5701),
     (False, 2, (SHARED, 256, 2), 7, 331, 2320),
     (False, 2, (SHARED, 256, 4), 1, 642, 3108),
     (False, 2, (PAIRS, 256, 1), 1, 1488, 3227),
-    (False, 3, (WHOLE, 256, 1), 42, 260, 13611),
-    (False, 3, (WHOLE, 128, 1), 1, 193, 10047),
-    (False, 3, (PAIRS, 256, 1), 6, 193, 17510),
+    (False, 2, (WHOLE, 128, 1), 4, 388, 2636),
+    (False, 2, (SHARED, 128, 2), 1, 324, 9851),
+    (False, 3, (WHOLE, 128, 1), 1, 324, 9851),
+    (False, 3, (WHOLE, 256, 1), 38, 326, 12107),
+    (False, 3, (PAIRS, 256, 1), 5, 705, 1846),
 ]
 
 
@@ -126,7 +133,7 @@ def test_each_kind(one, which, how, batch, m, n, kind):
 
 @pytest.mark.parametrize("steps,coefficients", [(1, (3.4445, -4.7750, 2.0315)), (2, (1.5, -0.5, 0.0)), (4, (2.0, -1.5, 0.5)),
                                                 (8, (15 / 8, -10 / 8, 3 / 8))])
-@pytest.mark.parametrize("batch,m,n", [(1, 301, 515), (3, 260, 700), (1, 131, 77), (40, 515, 517), (14, 331, 3320), (6, 196, 6762)])
+@pytest.mark.parametrize("batch,m,n", [(1, 301, 515), (3, 260, 700), (1, 131, 77), (40, 515, 517), (14, 331, 3320), (8, 330, 6762)])
 def test_blocks_of_every_length(batch, m, n, steps, coefficients):
     """One step, blocks of two, of two and two, and of three, three and two; and the same steps one by one."""
     if steps > 1:
@@ -137,22 +144,26 @@ def test_blocks_of_every_length(batch, m, n, steps, coefficients):
     assert distance(o, iterated(x, steps, coefficients)) < TOL
 
 
-@pytest.mark.parametrize("shape", [(16, 16), (16, 2000), (16, 16000), (24, 9000), (64, 300), (128, 128), (128, 896), (130, 600), (256, 1024),
-                                   (400, 4000), (1024, 1024), (896, 4864)])
+@pytest.mark.parametrize("shape", [(1, 16, 16), (1, 16, 2000), (1, 16, 16000), (1, 24, 9000), (1, 64, 300), (1, 128, 128), (1, 128, 896),
+                                   (1, 130, 600), (1, 256, 1024), (20, 200, 3000), (30, 320, 2000), (1, 400, 4000), (1, 1024, 1024),
+                                   (1, 896, 4864), (30, 330, 2500), (24, 512, 2048)])
 @pytest.mark.parametrize("kind", ["normal", "mixed", "low"])
 def test_beside_products_in_32_bits(shape, kind):
-    """As exact as the same iteration in 32-bit products, to within a factor of three on average over inputs; of four where steps
-    are made in blocks, which are for long matrices of more rows than 192 alone."""
+    """As exact as the same iteration in 32-bit products, to within a factor of three on average over inputs, and of 1.5 for the
+    spectra that gradients have.  Steps in blocks, which are for long or many matrices of more than 320 rows, keep the second; of
+    matrices without strong directions they are up to six times as far off."""
+    seeds = range(8 if shape[0] == 1 else 2)
     off = plain = 0.0
-    for seed in range(8):
+    for seed in seeds:
         x = matrix(*shape, seed=seed, kind=kind)
         want = iterated(x)
-        plain += distance(iterated(x, dtype=torch.float32), want) / 8
+        plain += distance(iterated(x, dtype=torch.float32), want) / len(seeds)
         with K.strict_native():
-            off += distance(genesis.optim.orthogonalize(T(x))._t, want) / 8
-    one = one_by_one(1, *shape)
-    assert one == (shape != (896, 4864))
-    assert off < (3 if one else 4) * plain + 2.0 ** -24, (off, plain)
+            off += distance(genesis.optim.orthogonalize(T(x))._t, want) / len(seeds)
+    one = one_by_one(*shape)
+    assert one == (shape[1] <= 320 or shape[0] == 1 and shape != (1, 896, 4864))
+    most = 1.5 if kind == "mixed" else 3 if one or kind == "low" else 6
+    assert off < most * plain + 2.0 ** -24, (off, plain)
 
 
 # (shapes of one batch, with how the wide matrices' last product is worked on: with one row of tiles and more, remainders of
