@@ -16,9 +16,11 @@ import torch
 
 from ..function import Function, AMPPolicy, cast
 from ..tensor import Tensor
-from ..ops import dispatch as K
+from ..ops import dispatch as K, paged as P
+from ..dtypes import to_torch_dtype as _to_torch_dtype
 from ..amp_state import amp_state, shadow_of, stacked_shadow_of
 from .. import random as _random
+from .paged import PagedKVLayer
 
 _pysum, _pymax, _pymin, _pyabs, _pypow = builtins.sum, builtins.max, builtins.min, builtins.abs, builtins.pow
 
@@ -1960,6 +1962,125 @@ def flash_attention(q, k, v, causal=True, scale=None):
     if scale is None:
         scale = 1.0 / math.sqrt(q.shape[-1])
     return FusedAttention.apply(q, k, v, causal, scale)
+
+
+def _paged_args(name, cache, page_table, lengths, counts, B, like):
+    """Checks what the operators on a paged cache have in common; returns the raw (page table, lengths, counts)."""
+    if not isinstance(cache, PagedKVLayer):
+        raise TypeError(f"{name}: cache must be a layer of a PagedKVCache (cache[i]), got {type(cache).__name__}")
+    raw = []
+    for what, t, dims in (("page_table", page_table, 2), ("lengths", lengths, 1), ("counts", counts, 1)):
+        if t is None and what == "counts":
+            raw.append(None)
+            continue
+        if not isinstance(t, Tensor) or t._t.dtype != torch.int32:
+            raise TypeError(f"{name}: {what} must be an int32 Tensor")
+        t = t._t
+        if t.dim() != dims or (B is not None and t.shape[0] != B):
+            raise ValueError(f"{name}: {what} must be [{'B' if B is None else B}{', pages' if dims == 2 else ''}], got {tuple(t.shape)}")
+        B = t.shape[0]
+        if t.device != cache.k.device:
+            raise ValueError(f"{name}: the cache is on {cache.k.device}, {what} on {t.device}")
+        raw.append(t if t.is_contiguous() else K.contiguous(t))
+    if like is not None and like.device != cache.k.device:
+        raise ValueError(f"{name}: the cache is on {cache.k.device}, the tokens on {like.device}")
+    return raw
+
+
+def _paged_tokens(name, what, x, dims, dtype=None):
+    """The raw numbers of a call's tokens.  A cache keeps no graph, so an input that wants a gradient is refused."""
+    from .. import grad_mode
+    if not isinstance(x, Tensor) or x._t.dtype not in (torch.float32, torch.float16, torch.bfloat16):
+        raise TypeError(f"{name}: {what} must be a Tensor of float32, float16 or bfloat16")
+    if x._t.dim() != dims:
+        raise ValueError(f"{name}: {what} must have {dims} dimensions, got {tuple(x._t.shape)}")
+    if dtype is not None and x._t.dtype != dtype:
+        raise TypeError(f"{name}: {what} is {x._t.dtype}, expected {dtype}")
+    if x.requires_grad and grad_mode.is_grad_enabled():
+        raise RuntimeError(f"{name}: no gradient flows through a cache; call it under no_grad or pass a detached {what}")
+    return x._t
+
+
+def paged_kv_write(k, v, cache, page_table, lengths, counts=None):
+    """Puts keys and values k, v [B, S, Hkv, D] into the pages of their sequences, in the type of `cache` (a layer of a
+    `nn.PagedKVCache`).
+
+    `page_table` [B, pages] names each sequence's pages in order, `lengths` [B] counts its tokens with those of this call, and
+    `counts` [B] (all S without it; clipped to 0 .. S) how many of the S are real: token s < counts[b] goes to position
+    lengths[b] - counts[b] + s, and nothing is written for the others or for a negative position (so a slot of the batch that
+    is not in use has length 0).  All three are int32 Tensors on the cache's device.  In 8 bits every token and head gets the smallest power of
+    two with which its largest magnitude is at most 448; infinities and NaN are held as NaN.  A page outside the cache or a
+    position behind the table is skipped and raised as IndexError at the next read of the status word (on the CPU at once).
+    Tokens of one call that share a slot are written in no order."""
+    name = "paged_kv_write"
+    k, v = _paged_tokens(name, "k", k, 4), _paged_tokens(name, "v", v, 4, k._t.dtype if isinstance(k, Tensor) else None)
+    table, lengths, counts = _paged_args(name, cache, page_table, lengths, counts, k.shape[0], k)
+    if k.shape != v.shape or v.device != k.device or tuple(k.shape[2:]) != (cache.num_kv_heads, cache.head_dim):
+        raise ValueError(f"{name}: k and v must be [B, S, {cache.num_kv_heads}, {cache.head_dim}] on one device, got "
+                         f"{tuple(k.shape)} and {tuple(v.shape)}")
+    P.put(None, k, v, None, cache, table, lengths, counts)
+
+
+def paged_qkv_rope(y, cos, sin, cache, page_table, lengths, num_heads, counts=None):
+    """`qkv_rope` into a cache: from a fused projection's y [B, S, (num_heads + 2 Hkv) D], the rotated queries
+    [B, S, num_heads, D], with the rotated keys and the values put into their pages by the same kernel.
+
+    cos, sin [positions, D] float32 (halves equal, as `RotaryEmbedding` keeps them) are read at each token's position in its
+    sequence; keys are rounded once, to the cache's type.  Tokens that are none (see `paged_kv_write`) give queries of zeros."""
+    name = "paged_qkv_rope"
+    y = _paged_tokens(name, "y", y, 3)
+    table, lengths, counts = _paged_args(name, cache, page_table, lengths, counts, y.shape[0], y)
+    Hkv, D = cache.num_kv_heads, cache.head_dim
+    if isinstance(num_heads, bool) or not isinstance(num_heads, int) or num_heads < 1 or num_heads % Hkv:
+        raise ValueError(f"{name}: num_heads must be a positive multiple of {Hkv} KV heads, got {num_heads!r}")
+    if y.shape[2] != (num_heads + 2 * Hkv) * D or D % 2:
+        raise ValueError(f"{name}: y must be [B, S, {(num_heads + 2 * Hkv) * D}] with heads of an even size, got {tuple(y.shape)}")
+    tables = []
+    for what, t in (("cos", cos), ("sin", sin)):
+        if not isinstance(t, Tensor) or t._t.dtype != torch.float32:
+            raise TypeError(f"{name}: {what} must be a float32 Tensor")
+        if t._t.dim() != 2 or t._t.shape[1] != D or t._t.device != y.device:
+            raise ValueError(f"{name}: {what} must be [positions, {D}] on {y.device}, got {tuple(t._t.shape)} on {t._t.device}")
+        tables.append(K.contiguous(t._t))
+    if tables[0].shape != tables[1].shape:
+        raise ValueError(f"{name}: cos and sin differ in shape")
+    x = y.unflatten(-1, (num_heads + 2 * Hkv, D))
+    return Tensor._wrap(P.put(x[:, :, :num_heads], x[:, :, num_heads:num_heads + Hkv], x[:, :, num_heads + Hkv:], tables,
+                              cache, table, lengths, counts))
+
+
+def paged_kv_read(cache, page_table, lengths, max_length, dtype=None):
+    """(k, v) [B, max_length, Hkv, D] of the sequences' first `max_length` tokens, zeros behind each one's end: what the flash attention takes
+    for the next piece of a long prompt.  `dtype`: float32, float16 or bfloat16; the cache's, or bfloat16 for 8 bits (exact)."""
+    name = "paged_kv_read"
+    table, lengths, _ = _paged_args(name, cache, page_table, lengths, None, None, None)
+    if isinstance(max_length, bool) or not isinstance(max_length, int) or not 0 <= max_length < 2 ** 31:
+        raise ValueError(f"{name}: max_length must be a non-negative 32-bit int, got {max_length!r}")
+    held = cache.k.dtype
+    dtype = (torch.bfloat16 if held == P.E4M3 else held) if dtype is None else _to_torch_dtype(dtype)
+    if dtype not in (torch.float32, torch.float16, torch.bfloat16):
+        raise TypeError(f"{name}: dtype must be float32, float16 or bfloat16, got {dtype}")
+    return tuple(Tensor._wrap(t) for t in P.read(cache, table, lengths, max_length, dtype))
+
+
+def paged_attention(q, cache, page_table, lengths, counts=None, scale=None):
+    """Attention of each sequence's newest tokens q [B, S, Hq, D] over its pages -> [B, S, Hq, D] in q's type.
+
+    `lengths` counts the tokens in the cache, those of this call (written before) among them; with `counts` [B] only the first
+    counts[b] of the S are real.  Token s sees the positions up to its own, lengths[b] - counts[b] + s; a token that is none,
+    or whose scores are -inf throughout, gives zeros.  Hkv divides Hq; `scale` is D ** -0.5 unless given.  Probabilities are
+    formed and summed in 32 bits.  Made for few tokens; where S runs into the hundreds the flash attention over what
+    `paged_kv_read` brings back is faster."""
+    name = "paged_attention"
+    q = _paged_tokens(name, "q", q, 4)
+    table, lengths, counts = _paged_args(name, cache, page_table, lengths, counts, q.shape[0], q)
+    Hq, D = q.shape[2:]
+    if D != cache.head_dim or Hq < 1 or Hq % cache.num_kv_heads:
+        raise ValueError(f"{name}: q must be [B, S, heads, {cache.head_dim}] with heads a multiple of {cache.num_kv_heads}, got {tuple(q.shape)}")
+    if q.is_cuda and D > 256:
+        raise ValueError(f"{name}: heads of up to 256 on CUDA, got {D}")
+    scale = D ** -0.5 if scale is None else _number(name, "scale", scale, -1e30, 1e30)
+    return Tensor._wrap(P.attention(q, cache, table, lengths, counts, scale))
 
 
 def scaled_dot_product_attention(q, k, v, attn_mask=None, dropout_p=0.0, is_causal=False, scale=None):

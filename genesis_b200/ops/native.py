@@ -74,6 +74,9 @@ _SIGS = {
     "gb_token_grad": "pppp" + "lllll" + "l" + "d" + "pl" + "pll" + "p" + "f" + "ii" + "p",
     "gb_ns_plan": "iiiiiip", "gb_ns_workspace": "lllip", "gb_muon_momentum": "p" + "iiii" + "d" + "i" + "ppp" + "p",
     "gb_ns_one_by_one": "pipiiii",
+    "gb_paged_put": "plll" * 3 + "ppp" + "i" + "pppp" + "ppp" + "iiiiiiii" + "ii" + "pp",
+    "gb_paged_read": "pppp" + "pp" + "pp" + "iiiiiii" + "ii" + "pp",
+    "gb_paged_attention": "pppppp" + "ppp" + "iiiiiiii" + "f" + "ii" + "pp",
     "gb_newton_schulz": "pp" + "iiiii" + "pi" + "pi" + "d" + "p" + "fff" + "pp" + "pp" + "p",
 }
 
@@ -169,7 +172,8 @@ def _raise_status(rec, what="native kernel"):
     if rec[0] == 4:
         raise IndexError(f"index out of range in a native kernel (site={rec[1]}: 1 row gather / embedding lookup, "
                          f"2 row scatter-add, 3 gather along a dim, 4 scatter along a dim, 5 indexed read, "
-                         f"6 indexed write, 7 token of a row of logits; block={rec[2]}, index={rec[3]}); the access was skipped")
+                         f"6 indexed write, 7 token of a row of logits, 8 page of a key / value cache, 9 position behind a page table or "
+                         f"rotation table; block={rec[2]}, index={rec[3]}); the access was skipped")
     if rec[0] == 3 and rec[1] == 900:
         raise RuntimeError(f"{what}: expert-parallel receive buffer too small: this rank was sent {rec[3]} "
                            f"(tile-padded) rows; raise GENESIS_EP_CAPACITY (multiple of the balanced share)")
