@@ -5,7 +5,24 @@
 // with K and V of KV head h / (Hq / Hkv), and zeros for a row that sees no key (a token that is none, or scores that are -inf
 // throughout).  One pass over the keys with a running maximum and sum in 32 bits; keys behind the end are neither read nor
 // multiplied, so what the rest of a page holds does not matter.
+//
+// Work is shared out by the lengths on the device, so that a captured launch stays right as sequences grow and a long sequence
+// does not leave the GPU to one SM: the chunks of keys of all items (sequence, KV head, tile of query rows) are numbered in
+// order, every warp takes an equal run of them, the warps of a CTA join what they have of an item through shared memory, and
+// a second small kernel joins the items that CTAs share (parts in a fixed order: the same call gives the same bits).
+//   rows     : the query rows of a KV head's group (tokens x heads) are the 8 columns of mma.sync.m16n8k16, 16 keys its rows:
+//              S^T = K Q^T, O^T = V^T P^T.  K and V are read once per 8 or 16 rows.
+//   layout   : fragments straight from global memory, 16 bytes a load and no shared memory in the loop.  The contraction over d
+//              may go in any order that K and Q share, so a lane takes 16 contiguous bytes of its key's row; for V a lane takes
+//              contiguous d of four keys and pairs the keys' numbers with byte permutes.  P^T comes from S^T by movmatrix.
+//   bound    : the bytes of K and V; the next chunk's K is in flight during softmax and P V, its V during the next Q K.
+//   precision: P enters its product as two 16-bit numbers (rounded, and what the rounding lost), or rounding it once to the
+//              type of V would double the error that the output's rounding makes; with 8-bit V it is fp16, whose 11 bits suffice
+//              below a bf16 output.  fp16 P is scaled by 2^7 on top of a maximum that may lag 2^8 behind, so that 2^-31 of the
+//              largest probability is still a number.  e4m3 becomes fp16 exactly; a bf16 q does under a power of two for each
+//              row.  K's powers of two multiply scores, V's multiply P, relative to the largest seen so far.
 #include "paged_common.cuh"
+#include <type_traits>
 
 namespace gb {
 
@@ -19,6 +36,633 @@ struct AttendArgs {
 };
 
 constexpr int PA_WARPS = 4, PA_MAX_D = 256;
+
+// The chunks of all items: items[b] = n(b) * per_seq, in the order of b, then KV head and row tile.
+struct AttendPlan {
+  int per_seq;          // items of a sequence: Hkv * row tiles
+  int tiles;            // row tiles
+  int grid;             // CTAs launched
+  float* parts;         // [grid][2][R][D] sums, then [grid][2][R] maxima and normalisers
+  int* desc;            // [grid][2]: an item that begins in the CTA and goes on behind it (-1: none), and the last CTA that has it
+};
+
+template <typename T, int CDT, int D_, int NQ_>
+struct PA {
+  static constexpr int D = D_, NQ = NQ_, R = 8 * NQ;
+  static constexpr bool E8 = CDT == DT_E4M3, BF = CDT == DT_BF16;
+  static constexpr bool OBF = sizeof(T) == 2 && !std::is_same<T, __half>::value;
+  static constexpr bool SPLIT = !(E8 && OBF);
+  static constexpr int ES = E8 ? 1 : 2;
+  static constexpr int KT = 4096 / (D * ES);            // keys of a chunk: 4 KB of K, 4 KB of V
+  static constexpr int NS = KT / 16;                    // tiles of 16 keys
+  static constexpr int KL = D * ES / 64;                // 16-byte loads of a lane's share of a key's row
+  static constexpr int VW = D * ES / 32;                // words of a lane's share of a value's row
+  static constexpr int MT = D / 16;                     // 16-row tiles of O^T
+  static constexpr int PIECE = R * D;
+  static constexpr int SMEM = 2 * PA_WARPS * PIECE * 4;
+  // first of the two columns d that a lane has of tile mt
+  static __device__ __forceinline__ int column(int g, int mt) {
+    if (E8) return g * (D / 8) + mt * 2;
+    return (g + 8 * (mt >> 2)) * 8 + (mt & 3) * 2;
+  }
+};
+
+__device__ __forceinline__ uint4 ld_stream16(const void* p, bool on) {        // zeros where it is off
+  uint4 v;
+  asm volatile("{\n\t.reg .pred P;\n\tsetp.ne.b32 P, %5, 0;\n\tmov.u32 %0, 0;\n\tmov.u32 %1, 0;\n\tmov.u32 %2, 0;\n\tmov.u32 %3, 0;\n\t"
+               "@P ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];\n\t}"
+               : "=&r"(v.x), "=&r"(v.y), "=&r"(v.z), "=&r"(v.w) : "l"(p), "r"((int)on));
+  return v;
+}
+__device__ __forceinline__ uint2 ld_stream8(const void* p, bool on) {
+  uint2 v;
+  asm volatile("{\n\t.reg .pred P;\n\tsetp.ne.b32 P, %3, 0;\n\tmov.u32 %0, 0;\n\tmov.u32 %1, 0;\n\t"
+               "@P ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];\n\t}" : "=&r"(v.x), "=&r"(v.y) : "l"(p), "r"((int)on));
+  return v;
+}
+// a bit for each 16-bit half of v that is an infinity or NaN
+template <bool BF>
+__device__ __forceinline__ uint32_t not_finite2(uint32_t v) {
+  constexpr uint32_t E = BF ? 0x7f80u : 0x7c00u;
+  return ((v & E) == E ? 1u : 0u) | ((v >> 16 & E) == E ? 2u : 0u);
+}
+__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t v) {        // the low 16 bits
+  uint32_t r;
+  asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(r) : "r"(v));
+  return r;
+}
+__device__ __forceinline__ uint32_t transposed_8x8(uint32_t v) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+template <bool BF>
+__device__ __forceinline__ float2 unpack2(uint32_t v) {
+  if (BF) return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+  return __half22float2(*reinterpret_cast<const __half2*>(&v));
+}
+template <bool BF>
+__device__ __forceinline__ void mma_k16(float (&c)[4], const uint32_t a0, const uint32_t a1, const uint32_t a2, const uint32_t a3, uint32_t b0, uint32_t b1) {
+  if (BF)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float pow2_of(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// weight of a part whose maximum is m against the common maximum
+__device__ __forceinline__ float part_weight(float m, float common) { return m == -INFINITY ? 0.f : pow2_of(m - common); }
+
+// keys that are read of sequence b (none where the call has no token of it), and chunks of KT of them, at least one: an item
+// without keys writes zeros
+__device__ __forceinline__ int attend_keys(const Paged& c, int b) {
+  if (c.count(b) == 0) return 0;
+  const int n = c.length(b), cap = c.capacity();
+  return n < cap ? n : cap;
+}
+__device__ __forceinline__ int attend_chunks(int keys, int kt) { return keys == 0 ? 1 : (keys + kt - 1) / kt; }
+
+// o / l of row r (0 .. S * group - 1) of a group, 4 columns from d on
+template <typename T>
+__device__ __forceinline__ void store_row4(const AttendArgs& a, const Paged& c, int b, int kvh, int r, int d, float4 o, float l) {
+  const int group = a.Hq / c.Hkv;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  T* p = reinterpret_cast<T*>(a.o) + (((long long)b * c.S + r / group) * a.Hq + kvh * group + r % group) * c.D + d;
+  uint2 w;
+  constexpr bool BF = !std::is_same<T, __half>::value;
+  w.x = pack2c<BF>(o.x * inv, o.y * inv);
+  w.y = pack2c<BF>(o.z * inv, o.w * inv);
+  *reinterpret_cast<uint2*>(p) = w;
+}
+
+template <typename T, int CDT, int D, int NQ>
+__global__ void __launch_bounds__(PA_WARPS * 32, NQ == 1 ? 3 : 2)
+paged_attend_kernel(const AttendArgs a, const Paged c, const AttendPlan plan) {
+  using C = PA<T, CDT, D, NQ>;
+  constexpr int R = C::R, KT = C::KT, NS = C::NS, KL = C::KL, VW = C::VW, MT = C::MT, W = PA_WARPS;
+  extern __shared__ __align__(16) float pieces[];                  // [2 W][R][D]
+  __shared__ float piece_m[2 * W][R], piece_l[2 * W][R];
+  __shared__ int piece_item[2 * W], piece_flags[2 * W];
+  __shared__ long long piece_end[2 * W], scan[W], first_chunk[W];
+  __shared__ int first_b[W];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+
+  // ---- the share of this warp -----------------------------------------------------------------------------------------
+  const int each = (c.B + W * 32 - 1) / (W * 32), b0 = min(c.B, (int)threadIdx.x * each), b1 = min(c.B, b0 + each);
+  long long mine = 0;
+  for (int b = b0; b < b1; ++b) mine += attend_chunks(attend_keys(c, b), KT);
+  mine *= plan.per_seq;
+  long long upto = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long x = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += x;
+  }
+  if (lane == 31) scan[warp] = upto;
+  if (threadIdx.x < 2 * W) piece_item[threadIdx.x] = -1;
+  __syncthreads();
+  long long total = 0;
+#pragma unroll
+  for (int w = 0; w < W; ++w) {
+    if (w < warp) upto += scan[w];
+    total += scan[w];
+  }
+  const long long want = (total + W - 1) / W;
+  const int ctas = want < plan.grid ? (int)want : plan.grid, cta = blockIdx.x;
+  auto start_of = [&](long long worker) { return total * worker / ((long long)ctas * W); };
+  if (cta >= ctas) {
+    if (threadIdx.x == 0) plan.desc[2 * cta] = -1;
+    return;
+  }
+#pragma unroll
+  for (int w = 0; w < W; ++w) {
+    const long long u = start_of((long long)cta * W + w);
+    if (u >= upto - mine && u < upto) {
+      long long at = upto - mine;
+      int b = b0;
+      for (;; ++b) {
+        const long long n = (long long)attend_chunks(attend_keys(c, b), KT) * plan.per_seq;
+        if (u < at + n) break;
+        at += n;
+      }
+      first_b[w] = b;
+      first_chunk[w] = at;
+    }
+  }
+  __syncthreads();
+  long long u = start_of((long long)cta * W + warp);
+  const long long u_end = start_of((long long)cta * W + warp + 1);
+  int b = first_b[warp];
+  long long seq_start = first_chunk[warp];
+  int slot = 0;
+  const float sl2 = a.scale * 1.4426950408889634f;
+  const int group = a.Hq / c.Hkv, rows = c.S * group, tpp = c.page / 16;
+
+  while (u < u_end) {
+    // ---- an item's run of chunks ------------------------------------------------------------------------------------
+    const int keys = attend_keys(c, b), n = attend_chunks(keys, KT);
+    const int idx = (int)((u - seq_start) / n);
+    if (idx >= plan.per_seq) { seq_start += (long long)n * plan.per_seq; ++b; continue; }
+    const int c0 = (int)(u - seq_start - (long long)idx * n);
+    const int c1 = (int)min((long long)n, c0 + (u_end - u));
+    const int kvh = idx / plan.tiles, row0 = idx % plan.tiles * R;
+    const int cnt = c.count(b), len = c.length(b);
+    if (len > keys && cnt > 0 && c0 == 0 && lane == 0) report_error(c.status, GB_ERR_BAD_INDEX, SITE_POSITION, len - 1);
+
+    // queries as the B operand: row g, the d that this lane has of a key's row
+    uint32_t qf[NQ][MT][2];
+    float factor[NQ][2];               // of the scores of queries 2t, 2t + 1
+    int end[NQ][2];                    // keys that they see
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) {
+      const int r = row0 + q * 8 + g;
+      const T* p = reinterpret_cast<const T*>(a.q) + (((long long)b * c.S + (r < rows ? r / group : 0)) * a.Hq + kvh * group + (r < rows ? r % group : 0)) * D;
+      float fq = 1.f;
+      if constexpr (!C::E8) {
+#pragma unroll
+        for (int i = 0; i < KL; ++i) {
+          uint4 v = make_uint4(0, 0, 0, 0);
+          if (r < rows) v = *reinterpret_cast<const uint4*>(p + (i * 4 + t) * 8);
+          qf[q][2 * i][0] = v.x; qf[q][2 * i][1] = v.y;
+          qf[q][2 * i + 1][0] = v.z; qf[q][2 * i + 1][1] = v.w;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < KL; ++i)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (r < rows) v = *reinterpret_cast<const uint4*>(p + (i * 4 + t) * 16 + h * 8);
+            qf[q][4 * i + 2 * h][0] = v.x; qf[q][4 * i + 2 * h][1] = v.y;
+            qf[q][4 * i + 2 * h + 1][0] = v.z; qf[q][4 * i + 2 * h + 1][1] = v.w;
+          }
+        if constexpr (C::OBF) {          // bf16 -> fp16 with the row's largest in [2^14, 2^15)
+          uint32_t top = 0;
+#pragma unroll
+          for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const float2 x = unpack2<true>(qf[q][i][h]);
+              top = max(top, max(finite_bits(x.x), finite_bits(x.y)));
+            }
+          top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+          top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+          int e = (int)(top >> 23) - 127 - 14;
+          e = e < -100 ? -100 : e;
+          const float inv = exp2i(-e);
+          fq = exp2i(e);
+#pragma unroll
+          for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const float2 x = unpack2<true>(qf[q][i][h]);
+              qf[q][i][h] = pack2c<false>(x.x * inv, x.y * inv);
+            }
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        factor[q][e] = sl2 * __shfl_sync(0xffffffffu, fq, (2 * t + e) * 4);
+        const int rr = row0 + q * 8 + 2 * t + e, s = rr / group;
+        end[q][e] = rr < rows && s < cnt ? min(keys, max(0, len - cnt + s + 1)) : 0;
+      }
+    }
+
+    float o[NQ][MT][4], m[NQ][2], l[NQ][2];
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) {
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[q][i][e] = 0.f;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) { m[q][e] = -INFINITY; l[q][e] = 0.f; }
+    }
+    int vtop = -1000;                  // the power of two that the accumulators are relative to
+
+    // ---- loads ------------------------------------------------------------------------------------------------------
+    const int* pages = c.table + (size_t)b * c.per;
+    int pg = c0 * NS / tpp, sub = c0 * NS - pg * tpp, tile = c0 * NS;      // the next tile whose page is asked for
+    int id[NS], place[NS];
+    auto ask = [&]() {
+#pragma unroll
+      for (int i = 0; i < NS; ++i) {
+        id[i] = -1;
+        place[i] = -1;
+        if (tile * 16 < keys) { id[i] = pages[pg]; place[i] = sub * 16; }
+        ++tile;
+        if (++sub == tpp) { sub = 0; ++pg; }
+      }
+    };
+    long long row[NS];
+    auto resolve = [&]() {
+#pragma unroll
+      for (int i = 0; i < NS; ++i) {
+        row[i] = -1;
+        if (place[i] < 0) continue;
+        if (id[i] < 0 || id[i] >= c.pages) { if (lane == 0) report_error(c.status, GB_ERR_BAD_INDEX, SITE_PAGE, id[i]); }
+        else row[i] = ((long long)id[i] * c.Hkv + kvh) * c.page + place[i];
+      }
+    };
+    uint4 kr[NS][2][KL];
+    uint32_t vr[NS][4][VW], sc[NS];
+    auto load_k = [&](int chunk) {
+#pragma unroll
+      for (int i = 0; i < NS; ++i) {
+        const int left = keys - (chunk * NS + i) * 16;
+        const char* p = reinterpret_cast<const char*>(a.kpool) + row[i] * (D * C::ES) + t * 16;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int j = 0; j < KL; ++j)
+            kr[i][h][j] = ld_stream16(p + (g + 8 * h) * (D * C::ES) + j * 64, row[i] >= 0 && g + 8 * h < left);
+        if constexpr (C::E8) {         // lanes 0 - 15: K's powers of two, 16 - 31: V's
+          sc[i] = 127;
+          if (row[i] >= 0 && (lane & 15) < left) sc[i] = (lane < 16 ? a.kscale : a.vscale)[row[i] + (lane & 15)];
+        }
+      }
+    };
+    auto load_v = [&](int chunk) {
+#pragma unroll
+      for (int i = 0; i < NS; ++i) {
+        const int left = keys - (chunk * NS + i) * 16;
+        const char* p = reinterpret_cast<const char*>(a.vpool) + row[i] * (D * C::ES);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int key = 2 * t + (k & 1) + (k >> 1) * 8;
+          const bool on = row[i] >= 0 && key < left;
+          if constexpr (VW == 2) {
+            const uint2 v = ld_stream8(p + key * (D * C::ES) + g * 8, on);
+            vr[i][k][0] = v.x; vr[i][k][1] = v.y;
+          } else {
+#pragma unroll
+            for (int j = 0; j < VW / 4; ++j) {
+              const uint4 v = ld_stream16(p + key * (D * C::ES) + (g + 8 * j) * 16, on);
+              vr[i][k][4 * j] = v.x; vr[i][k][4 * j + 1] = v.y; vr[i][k][4 * j + 2] = v.z; vr[i][k][4 * j + 3] = v.w;
+            }
+          }
+        }
+      }
+    };
+    ask();
+    resolve();
+    load_k(c0);
+    load_v(c0);
+    ask();
+
+    for (int ch = c0; ch < c1; ++ch) {
+      // ---- S^T = K Q^T ----------------------------------------------------------------------------------------------
+      float s[NS][NQ][4];
+      bool gone[NS];
+      float ks[NS][2];
+      int ve[NS][2];
+#pragma unroll
+      for (int i = 0; i < NS; ++i) {
+        gone[i] = row[i] < 0;
+#pragma unroll
+        for (int q = 0; q < NQ; ++q)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[i][q][e] = 0.f;
+#pragma unroll
+        for (int j = 0; j < KL; ++j) {
+          const uint32_t lo[4] = {kr[i][0][j].x, kr[i][0][j].y, kr[i][0][j].z, kr[i][0][j].w};
+          const uint32_t hi[4] = {kr[i][1][j].x, kr[i][1][j].y, kr[i][1][j].z, kr[i][1][j].w};
+          if constexpr (!C::E8) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int q = 0; q < NQ; ++q)
+                mma_k16<C::BF>(s[i][q], lo[2 * h], hi[2 * h], lo[2 * h + 1], hi[2 * h + 1], qf[q][2 * j + h][0], qf[q][2 * j + h][1]);
+          } else {
+#pragma unroll
+            for (int h = 0; h < 4; ++h) {
+              const uint32_t a0 = e4m3x2_to_f16x2(lo[h]), a2 = e4m3x2_to_f16x2(lo[h] >> 16);
+              const uint32_t a1 = e4m3x2_to_f16x2(hi[h]), a3 = e4m3x2_to_f16x2(hi[h] >> 16);
+#pragma unroll
+              for (int q = 0; q < NQ; ++q) mma_k16<false>(s[i][q], a0, a1, a2, a3, qf[q][4 * j + h][0], qf[q][4 * j + h][1]);
+            }
+          }
+        }
+        if constexpr (C::E8) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            ks[i][h] = __uint_as_float(__shfl_sync(0xffffffffu, sc[i], g + 8 * h) << 23);
+            ve[i][h] = (int)__shfl_sync(0xffffffffu, sc[i], 16 + g + 8 * h) - 127;
+          }
+        }
+      }
+      const bool more = ch + 1 < c1;
+      if (more) {
+        resolve();
+        load_k(ch + 1);
+        ask();
+      }
+      // ---- probabilities --------------------------------------------------------------------------------------------
+      bool grow = false;
+#pragma unroll
+      for (int i = 0; i < NS; ++i)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int key = (ch * NS + i) * 16 + g + 8 * h;
+          if constexpr (C::E8) {
+            if (gone[i] || key >= keys) ve[i][h] = -1000;
+            grow |= ve[i][h] > vtop;
+          }
+#pragma unroll
+          for (int q = 0; q < NQ; ++q)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              float& x = s[i][q][2 * h + e];
+              x *= factor[q][e];
+              if constexpr (C::E8) x *= ks[i][h];
+              if (gone[i] || key >= end[q][e]) x = -INFINITY;
+              grow |= x > m[q][e] + 8.f;
+            }
+        }
+      if (__any_sync(0xffffffffu, grow)) {
+        float vscale = 1.f;
+        if constexpr (C::E8) {
+          int e = vtop;
+#pragma unroll
+          for (int i = 0; i < NS; ++i) e = max(e, max(ve[i][0], ve[i][1]));
+          e = __reduce_max_sync(0xffffffffu, e);
+          vscale = vtop - e < -126 ? 0.f : exp2i(vtop - e);
+          vtop = e;
+        }
+#pragma unroll
+        for (int q = 0; q < NQ; ++q)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float x = m[q][e];
+#pragma unroll
+            for (int i = 0; i < NS; ++i) x = fmaxf(x, fmaxf(s[i][q][e], s[i][q][2 + e]));
+#pragma unroll
+            for (int w = 4; w < 32; w <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, w));
+            const float alpha = part_weight(m[q][e], x);
+            m[q][e] = x;
+            l[q][e] *= alpha;
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+              o[q][i][e] *= alpha * vscale;
+              o[q][i][2 + e] *= alpha * vscale;
+            }
+          }
+      }
+      uint32_t ph[NS][NQ][2], pl[NS][NQ][2];
+#pragma unroll
+      for (int i = 0; i < NS; ++i)
+#pragma unroll
+        for (int q = 0; q < NQ; ++q)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float p[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              p[e] = pow2_of(s[i][q][2 * h + e] - (m[q][e] == -INFINITY ? 0.f : m[q][e]));
+              l[q][e] += p[e];
+              if constexpr (C::E8) p[e] *= ve[i][h] - vtop + 7 < -126 ? 0.f : exp2i(ve[i][h] - vtop + 7);
+              else if constexpr (!C::BF) p[e] *= 128.f;
+            }
+            const uint32_t w = pack2c<C::BF>(p[0], p[1]);
+            ph[i][q][h] = transposed_8x8(w);
+            if constexpr (C::SPLIT) {
+              const float2 r = unpack2<C::BF>(w);
+              pl[i][q][h] = transposed_8x8(pack2c<C::BF>(p[0] - r.x, p[1] - r.y));
+            }
+          }
+      // ---- O^T += V^T P^T -------------------------------------------------------------------------------------------
+      // rows of a call with several tokens end at different keys; a key that one row sees and another does not is multiplied by
+      // a probability of 0 there, which an infinity or NaN among its values would turn into NaN
+      const bool ragged = c.S > 1 && (ch + 1) * KT > len - cnt;
+#pragma unroll
+      for (int i = 0; i < NS; ++i)
+#pragma unroll
+        for (int j = 0; j < VW * (C::E8 ? 2 : 1); ++j) {
+          uint32_t v[4];
+          if constexpr (!C::E8) {
+            v[0] = __byte_perm(vr[i][0][j], vr[i][1][j], 0x5410);
+            v[1] = __byte_perm(vr[i][0][j], vr[i][1][j], 0x7632);
+            v[2] = __byte_perm(vr[i][2][j], vr[i][3][j], 0x5410);
+            v[3] = __byte_perm(vr[i][2][j], vr[i][3][j], 0x7632);
+          } else {
+            const uint32_t x = __byte_perm(vr[i][0][j / 2], vr[i][1][j / 2], j & 1 ? 0x7362 : 0x5140);
+            const uint32_t y = __byte_perm(vr[i][2][j / 2], vr[i][3][j / 2], j & 1 ? 0x7362 : 0x5140);
+            v[0] = e4m3x2_to_f16x2(x); v[1] = e4m3x2_to_f16x2(x >> 16);
+            v[2] = e4m3x2_to_f16x2(y); v[3] = e4m3x2_to_f16x2(y >> 16);
+          }
+          uint32_t bad = 0;
+          if (ragged) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) bad |= not_finite2<C::BF>(v[k]);
+            bad = __any_sync(0xffffffffu, bad != 0);
+          }
+#pragma unroll
+          for (int q = 0; q < NQ; ++q) {
+            float kept[4];
+            if (bad) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) kept[e] = o[q][j][e];
+            }
+            mma_k16<C::BF>(o[q][j], v[0], v[1], v[2], v[3], ph[i][q][0], ph[i][q][1]);
+            if constexpr (C::SPLIT) mma_k16<C::BF>(o[q][j], v[0], v[1], v[2], v[3], pl[i][q][0], pl[i][q][1]);
+            if (bad) {
+              // the same without those values for the rows that do not see them: how many of them a row sees is a product too
+              uint32_t fine[4], mark[4], sees[2];
+              constexpr uint32_t ONE = C::BF ? 0x3f80u : 0x3c00u;
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const uint32_t f = not_finite2<C::BF>(v[k]);
+                fine[k] = v[k] & ((f & 1 ? 0u : 0xffffu) | (f & 2 ? 0u : 0xffff0000u));
+                mark[k] = (f & 1 ? ONE : 0u) | (f & 2 ? ONE << 16 : 0u);
+              }
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const int key = (ch * NS + i) * 16 + g + 8 * h;
+                sees[h] = transposed_8x8((key < end[q][0] ? ONE : 0u) | (key < end[q][1] ? ONE << 16 : 0u));
+              }
+              float seen[4] = {0.f, 0.f, 0.f, 0.f};
+              mma_k16<C::BF>(seen, mark[0], mark[1], mark[2], mark[3], sees[0], sees[1]);
+              mma_k16<C::BF>(kept, fine[0], fine[1], fine[2], fine[3], ph[i][q][0], ph[i][q][1]);
+              if constexpr (C::SPLIT) mma_k16<C::BF>(kept, fine[0], fine[1], fine[2], fine[3], pl[i][q][0], pl[i][q][1]);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o[q][j][e] = seen[e] == 0.f ? kept[e] : o[q][j][e];
+            }
+          }
+        }
+      if (more) load_v(ch + 1);
+    }
+
+    // ---- the run's result ---------------------------------------------------------------------------------------------
+    float unit = 1.f;
+    if constexpr (C::E8) unit = vtop - 7 < -126 ? 0.f : exp2i(vtop - 7);
+    else if constexpr (!C::BF) unit = 1.f / 128.f;
+#pragma unroll
+    for (int q = 0; q < NQ; ++q)
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int w = 4; w < 32; w <<= 1) l[q][e] += __shfl_xor_sync(0xffffffffu, l[q][e], w);
+    const bool whole = c0 == 0 && c1 == n;
+    const int piece = 2 * warp + slot;
+    if (!whole) {
+      ++slot;
+      if (lane == 0) {
+        piece_item[piece] = b * plan.per_seq + idx;
+        piece_flags[piece] = (c0 == 0 ? 1 : 0) | (c1 == n ? 2 : 0);
+        piece_end[piece] = seq_start + (long long)(idx + 1) * n;
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < NQ; ++q)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int r = q * 8 + 2 * t + e;
+        if (!whole && g == 0) { piece_m[piece][r] = m[q][e]; piece_l[piece][r] = l[q][e]; }
+#pragma unroll
+        for (int i = 0; i < MT; i += 2) {
+          const float4 v = make_float4(o[q][i][e] * unit, o[q][i][2 + e] * unit, o[q][i + 1][e] * unit, o[q][i + 1][2 + e] * unit);
+          const int d = C::column(g, i);
+          if (!whole) *reinterpret_cast<float4*>(pieces + ((size_t)piece * R + r) * D + d) = v;
+          else if (row0 + r < rows) store_row4<T>(a, c, b, kvh, row0 + r, d, v, l[q][e]);
+        }
+      }
+    u += c1 - c0;
+  }
+  __syncthreads();
+
+  // ---- the warps' pieces, item by item ----------------------------------------------------------------------------------
+  int next_item = -1, next_last = 0;
+  for (int p = 0; p < 2 * W;) {
+    const int item = piece_item[p];
+    if (item < 0) { ++p; continue; }
+    int last = p;
+    for (int k = p + 1; k < 2 * W; ++k) {
+      if (piece_item[k] == item) last = k;
+      else if (piece_item[k] >= 0) break;
+    }
+    const bool begins = piece_flags[p] & 1, ends = piece_flags[last] & 2;
+    const int bb = item / plan.per_seq, idx = item % plan.per_seq, kvh = idx / plan.tiles, row0 = idx % plan.tiles * R;
+    const size_t part = (size_t)cta * 2 + (begins ? 1 : 0);
+    for (int e = threadIdx.x; e < R * D / 4; e += W * 32) {
+      const int r = e / (D / 4), d = e % (D / 4) * 4;
+      float mc = -INFINITY, lc = 0.f;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int k = p; k <= last; ++k)
+        if (piece_item[k] == item) mc = fmaxf(mc, piece_m[k][r]);
+      for (int k = p; k <= last; ++k) {
+        if (piece_item[k] != item) continue;
+        const float w = part_weight(piece_m[k][r], mc);
+        const float4 v = *reinterpret_cast<const float4*>(pieces + ((size_t)k * R + r) * D + d);
+        acc.x += w * v.x; acc.y += w * v.y; acc.z += w * v.z; acc.w += w * v.w;
+        lc += w * piece_l[k][r];
+      }
+      if (begins && ends) {
+        if (row0 + r < rows) store_row4<T>(a, c, bb, kvh, row0 + r, d, acc, lc);
+      } else {
+        *reinterpret_cast<float4*>(plan.parts + (part * R + r) * D + d) = acc;
+        if (d == 0) {
+          float* st = plan.parts + (size_t)plan.grid * 2 * R * D + (part * R + r) * 2;
+          st[0] = mc;
+          st[1] = lc;
+        }
+      }
+    }
+    if (begins && !ends) {
+      next_item = item;
+      next_last = (int)((piece_end[last] * ctas - 1) / total);
+    }
+    p = last + 1;
+  }
+  if (threadIdx.x == 0) { plan.desc[2 * cta] = next_item; plan.desc[2 * cta + 1] = next_last; }
+}
+
+// Joins the items that several CTAs have parts of: CTA i takes the one that begins in CTA i of the kernel above and goes on.
+template <typename T, int D, int R>
+__global__ void __launch_bounds__(R * D / 4) paged_join_kernel(const AttendArgs a, const Paged c, const AttendPlan plan) {
+  const int item = plan.desc[2 * blockIdx.x], last = plan.desc[2 * blockIdx.x + 1];
+  if (item < 0) return;
+  const int b = item / plan.per_seq, idx = item % plan.per_seq, kvh = idx / plan.tiles;
+  const int r = threadIdx.x / (D / 4), d = threadIdx.x % (D / 4) * 4, row = idx % plan.tiles * R + r;
+  if (row >= c.S * (a.Hq / c.Hkv)) return;
+  const float* stats = plan.parts + (size_t)plan.grid * 2 * R * D;
+  float m = -INFINITY, l = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int k = blockIdx.x; k <= last; ++k) {
+    const size_t part = (size_t)k * 2 + (k == (int)blockIdx.x ? 1 : 0);
+    const float2 st = *reinterpret_cast<const float2*>(stats + (part * R + r) * 2);
+    const float4 v = *reinterpret_cast<const float4*>(plan.parts + (part * R + r) * D + d);
+    const float mn = fmaxf(m, st.x), wa = part_weight(m, mn), wb = part_weight(st.x, mn);
+    acc.x = acc.x * wa + v.x * wb; acc.y = acc.y * wa + v.y * wb; acc.z = acc.z * wa + v.z * wb; acc.w = acc.w * wa + v.w * wb;
+    l = l * wa + st.y * wb;
+    m = mn;
+  }
+  store_row4<T>(a, c, b, kvh, row, d, acc, l);
+}
+
+template <typename T, int CDT, int D, int NQ>
+static int launch_attend(const AttendArgs& a, const Paged& c, float* parts, int* desc, int grid, cudaStream_t st) {
+  using C = PA<T, CDT, D, NQ>;
+  static unsigned long long cfg = 0;
+  int r;
+  if (C::SMEM > 40 * 1024 && (r = smem_opt_in(paged_attend_kernel<T, CDT, D, NQ>, C::SMEM, cfg)) != 0) return r;
+  AttendPlan plan;
+  plan.tiles = (c.S * (a.Hq / c.Hkv) + C::R - 1) / C::R;
+  plan.per_seq = plan.tiles * c.Hkv;
+  plan.grid = grid;
+  plan.parts = parts;
+  plan.desc = desc;
+  paged_attend_kernel<T, CDT, D, NQ><<<grid, PA_WARPS * 32, C::SMEM, st>>>(a, c, plan);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return (int)e;
+  paged_join_kernel<T, D, C::R><<<grid, C::R * D / 4, 0, st>>>(a, c, plan);
+  return (int)cudaGetLastError();
+}
 
 // Any type and head size: a CTA takes a row of queries, its warps every fourth key, their lanes a share of the head.
 template <typename T, int CDT>
@@ -94,16 +738,46 @@ __global__ void __launch_bounds__(PA_WARPS * 32) paged_attend_any_kernel(const A
 
 using namespace gb;
 
+// Which kernel a call takes, and its CTAs (0: a CTA for every row).  The tensor cores take 16-bit queries of 64 or 128 over caches
+// of their own type or of 8 bits; what remains (32-bit caches and queries, other head sizes) is worked on number by number.
+static int attend_grid(int B, int S, int Hq, int Hkv, int D, int page, int per, int dt, int cdt) {
+  if ((D != 64 && D != 128) || dt == DT_F32 || (cdt != dt && cdt != DT_E4M3) || page % 16) return 0;
+  const int rows = S * (Hq / Hkv), R = rows <= 8 ? 8 : 16;
+  const int kt = 4096 / (D * (cdt == DT_E4M3 ? 1 : 2));
+  const long long tiles = (rows + R - 1) / R, keys = (long long)per * page;
+  const long long chunks = B * Hkv * tiles * (keys <= 0 ? 1 : (keys + kt - 1) / kt);
+  const long long want = (chunks + PA_WARPS - 1) / PA_WARPS, most = (long long)sm_count() * (R == 8 ? 3 : 2);
+  return (int)(want < most ? want : most);
+}
+
+// 32-bit words of workspace that a call needs
+extern "C" int gb_paged_attention_workspace(int B, int S, int Hq, int Hkv, int D, int page, int per, int dt, int cdt) {
+  if (B <= 0 || S <= 0 || Hq <= 0 || Hkv <= 0) return 0;
+  const int R = S * (Hq / Hkv) <= 8 ? 8 : 16;
+  return attend_grid(B, S, Hq, Hkv, D, page, per, dt, cdt) * (2 * R * (D + 2) + 2);
+}
+
 extern "C" int gb_paged_attention(const void* q, void* o, const void* kpool, const void* vpool, const void* kscale,
                                   const void* vscale, const int* table, const int* lengths, const int* counts, int B, int S,
                                   int Hq, int Hkv, int D, int page, int pages, int per, float scale, int dt, int cdt,
-                                  int* status, cudaStream_t st) {
+                                  float* workspace, int* status, cudaStream_t st) {
   if (B <= 0 || S <= 0 || Hq <= 0 || D <= 0) return 0;
   if (D > PA_MAX_D || Hkv <= 0 || Hq % Hkv) return -3;
   AttendArgs a{q, o, kpool, vpool, (const uint8_t*)kscale, (const uint8_t*)vscale, Hq, scale};
   Paged c{table, lengths, counts, status, B, S, Hkv, D, page, pages, per};
   const long long rows = (long long)B * S * Hq;
   if (rows > 0x7fffffff) return -4;
+  const int grid = attend_grid(B, S, Hq, Hkv, D, page, per, dt, cdt);
+  if (grid > 0) {
+    const int R = S * (Hq / Hkv) <= 8 ? 8 : 16;
+    int* desc = reinterpret_cast<int*>(workspace + (size_t)grid * 2 * R * (D + 2));
+#define GB_ATTEND(T, C)                                                                                                    \
+    (D == 64 ? (R == 8 ? launch_attend<T, C, 64, 1>(a, c, workspace, desc, grid, st) : launch_attend<T, C, 64, 2>(a, c, workspace, desc, grid, st)) \
+             : (R == 8 ? launch_attend<T, C, 128, 1>(a, c, workspace, desc, grid, st) : launch_attend<T, C, 128, 2>(a, c, workspace, desc, grid, st)))
+    if (dt == DT_BF16) return cdt == DT_E4M3 ? GB_ATTEND(__nv_bfloat16, DT_E4M3) : GB_ATTEND(__nv_bfloat16, DT_BF16);
+    return cdt == DT_E4M3 ? GB_ATTEND(__half, DT_E4M3) : GB_ATTEND(__half, DT_F16);
+#undef GB_ATTEND
+  }
   GB_DISPATCH_FLOAT(dt, T, GB_DISPATCH_CACHE(cdt, C, paged_attend_any_kernel<T, C><<<(unsigned)rows, PA_WARPS * 32, 0, st>>>(a, c)));
   return (int)cudaGetLastError();
 }

@@ -35,6 +35,15 @@ class PagedKVLayer:
     __slots__ = ("k", "v", "k_scale", "v_scale")
 
     def __init__(self, k, v, k_scale=None, v_scale=None):
+        if k.dim() != 4 or v.shape != k.shape or k.dtype not in CACHE_TYPES or v.dtype != k.dtype or k.shape[2] % 16 or 0 in k.shape:
+            raise ValueError(f"PagedKVLayer: k and v must be pools [pages, KV heads, page size, head dim] of one type, the page size "
+                             f"a multiple of 16, got {tuple(k.shape)} {k.dtype} and {tuple(v.shape)} {v.dtype}")
+        scales = [t for t in (k_scale, v_scale) if t is not None]
+        if len(scales) != (2 if k.dtype == E4M3 else 0) or any(t.shape != k.shape[:3] or t.dtype != torch.uint8 for t in scales):
+            raise ValueError("PagedKVLayer: pools of 8 bits, and no others, have scales [pages, KV heads, page size] of uint8")
+        for t in (k, v, *scales):
+            if not t.is_contiguous() or t.data_ptr() % 16 or t.device != k.device:
+                raise ValueError("PagedKVLayer: pools and scales must be contiguous, start on 16 bytes and be on one device")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
 
     @property

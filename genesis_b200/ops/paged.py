@@ -4,6 +4,8 @@ on the CPU (which is what the tests compare with).
 A layer's pools are k, v [pages, Hkv, page, D] and, for 8 bits, scales [pages, Hkv, page] of uint8: a row stands for its e4m3
 numbers times 2^(scale - 127).  `table` [B, per], `lengths` [B] and `counts` [B] (or None) are int32; token s of sequence b stands
 at position lengths[b] - counts[b] + s, for s < counts[b] (clipped to 0 .. S) and positions from 0 on."""
+import functools
+
 import torch
 
 from . import native as N
@@ -186,19 +188,27 @@ def read(layer, table, lengths, L, dtype):
     return out
 
 
+@functools.lru_cache(maxsize=256)
+def _workspace(device_index, *sizes):
+    return N.lib().gb_paged_attention_workspace(*sizes)
+
+
 def attention(q, layer, table, lengths, counts, scale):
     """softmax(scale q k^T) v of the tokens q [B, S, Hq, D] over the pages of their sequences -> [B, S, Hq, D]."""
     if not q.is_cuda:
         return _attention_cpu(q, layer, table, lengths, counts, scale)
     B, S, Hq, D = q.shape
-    pages, Hkv, page, _ = layer.k.shape
-    dev = q.device
-    q = q if q.is_contiguous() else q.contiguous()
-    out = torch.empty(B, S, Hq, D, dtype=q.dtype, device=dev)
+    k = layer.k
+    pages, Hkv, page, _ = k.shape
+    dev, per, dt, cdt = q.device, table.shape[1], N._DT[q.dtype], CACHE_TYPES[k.dtype]
+    if not q.is_contiguous() or q.data_ptr() % 16:
+        q = q.clone(memory_format=torch.contiguous_format)
+    out = torch.empty_like(q)
     with N._on(dev):
-        N._chk(N.lib().gb_paged_attention(q.data_ptr(), out.data_ptr(), layer.k.data_ptr(), layer.v.data_ptr(),
-                                          N._ptr(layer.k_scale), N._ptr(layer.v_scale), table.data_ptr(), lengths.data_ptr(),
-                                          N._ptr(counts), B, S, Hq, Hkv, D, page, pages, table.shape[1], scale, N._DT[q.dtype],
-                                          CACHE_TYPES[layer.k.dtype], N.status_tensor(dev).data_ptr(), N._st()),
-               "paged_attention")
+        words = _workspace(dev.index, B, S, Hq, Hkv, D, page, per, dt, cdt)
+        work = torch.empty(words, dtype=torch.float32, device=dev) if words else None
+        N._chk(N.lib().gb_paged_attention(q.data_ptr(), out.data_ptr(), k.data_ptr(), layer.v.data_ptr(), N._ptr(layer.k_scale),
+                                          N._ptr(layer.v_scale), table.data_ptr(), lengths.data_ptr(), N._ptr(counts), B, S, Hq,
+                                          Hkv, D, page, pages, per, scale, dt, cdt, N._ptr(work),
+                                          N.status_tensor(dev).data_ptr(), N._st()), "paged_attention")
     return out

@@ -47,6 +47,15 @@ def test_caches_that_are_refused():
                dict(head_dim=True), dict(num_pages=2 ** 31), dict(num_kv_heads=1.0)):
         with pytest.raises(ValueError):
             PagedKVCache(**{**dict(num_pages=2, num_kv_heads=1, head_dim=8), **kw})
+    k = torch.zeros(2, 1, 16, 8)
+    e = torch.zeros(2, 1, 16, 8, dtype=torch.uint8).view(torch.float8_e4m3fn)
+    u = torch.zeros(2, 1, 16, dtype=torch.uint8)
+    genesis.nn.PagedKVLayer(k, k), genesis.nn.PagedKVLayer(e, e, u, u)
+    for wrong in ((k, k[:1]), (k, k.half()), (k.double(), k.double()), (k[:, :, :15], k[:, :, :15]), (k[0], k[0]), (k[:0], k[:0]),
+                  (torch.zeros(2, 1, 8, 16).transpose(2, 3), k), (e, e), (k, k, u, u), (e, e, u, None), (e, e, u[:1], u), (e, e, u.int(), u),
+                  (torch.zeros(257)[1:].view(2, 1, 16, 8), k)):
+        with pytest.raises(ValueError, match="PagedKVLayer"):
+            genesis.nn.PagedKVLayer(*wrong)
     assert PagedKVCache(1, 1, 8, dtype=genesis.bfloat16)[0].k.dtype == torch.bfloat16
     assert PagedKVCache(1, 1, 8, dtype=torch.float8_e4m3fn)[0].k_scale.dtype == torch.uint8
 
@@ -133,6 +142,15 @@ def test_attention(cache, dtype):
     # a length of 2 with three new tokens: the first is none
     short = F.paged_attention(t.tensor(q), t.layer, t.table, t.ints([1, 2, 2, 0, 2, 2]))._t
     assert torch.all(short[:, 0] == 0) and torch.all(short[3] == 0) and not torch.any(torch.all(short[[1, 2], 1] == 0, -1))
+
+
+def test_tokens_that_come_later_do_not_reach_back():
+    t = R.Setup([20], 2, 8, "bf16")
+    q = t.normal(1, 3, 4, 8)
+    clean = F.paged_attention(t.tensor(q), t.layer, t.table, t.lens)._t.clone()
+    t.layer.k[t.pages[0][1], :, 3], t.layer.v[t.pages[0][1], :, 3] = math.nan, math.inf
+    o = F.paged_attention(t.tensor(q), t.layer, t.table, t.lens)._t
+    assert torch.equal(o[:, :2], clean[:, :2]) and not torch.any(torch.isfinite(o[:, 2]))
 
 
 def test_a_prompt_and_single_tokens_give_what_flash_attention_gives():

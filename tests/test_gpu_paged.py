@@ -230,6 +230,30 @@ def test_what_is_not_finite_stays_with_its_rows():
             assert torch.all(o[0] == 0)
 
 
+@pytest.mark.parametrize("S", [3, 9])
+@pytest.mark.parametrize("dtype,cache", TYPES)
+def test_tokens_that_come_later_do_not_reach_back(dtype, cache, S):
+    """Infinities and NaN in the newest token's keys and values belong to the rows that see it."""
+    for D in (64, 128, 48):
+        lengths = [33, 7, 200]
+        t = R.Setup(lengths, 2, D, cache, 16, "cuda")
+        q = t.normal(3, S, 8, D, dtype=dtype)
+        clean = F.paged_attention(t.tensor(q), t.layer, t.table, t.lens)._t.clone()
+        for b, n in enumerate(lengths):
+            if n < S:
+                continue
+            p, at = t.pages[b][(n - 1) // 16], (n - 1) % 16
+            for pool in (t.layer.k, t.layer.v):
+                if cache == "e4m3":
+                    pool.view(torch.uint8)[p, 1, at, 3:9] = 0x7f
+                else:
+                    pool[p, 1, at, 3:6], pool[p, 1, at, 6:9] = math.nan, math.inf
+        o = F.paged_attention(t.tensor(q), t.layer, t.table, t.lens)._t
+        assert torch.equal(o[:, :S - 1], clean[:, :S - 1]) and torch.equal(o[:, S - 1, :4], clean[:, S - 1, :4])
+        hit = [n >= S for n in lengths]
+        assert torch.all(torch.isnan(o[hit][:, S - 1, 4:, 3:6]))
+
+
 def test_the_same_call_gives_the_same_bits():
     for dtype, cache in TYPES:
         t = R.Setup([5000, 1200, 3], 2, 64, cache, 16, "cuda")
