@@ -151,6 +151,7 @@ paged_attend_kernel(const AttendArgs a, const Paged c, const AttendPlan plan) {
   __shared__ long long piece_end[2 * W], scan[W], first_chunk[W];
   __shared__ int first_b[W];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");       // (the join waits for the end of this kernel)
 
   // ---- the share of this warp -----------------------------------------------------------------------------------------
   const int each = (c.B + W * 32 - 1) / (W * 32), b0 = min(c.B, (int)threadIdx.x * each), b1 = min(c.B, b0 + each);
@@ -214,77 +215,6 @@ paged_attend_kernel(const AttendArgs a, const Paged c, const AttendPlan plan) {
     const int cnt = c.count(b), len = c.length(b);
     if (len > keys && cnt > 0 && c0 == 0 && lane == 0) report_error(c.status, GB_ERR_BAD_INDEX, SITE_POSITION, len - 1);
 
-    // queries as the B operand: row g, the d that this lane has of a key's row
-    uint32_t qf[NQ][MT][2];
-    float factor[NQ][2];               // of the scores of queries 2t, 2t + 1
-    int end[NQ][2];                    // keys that they see
-#pragma unroll
-    for (int q = 0; q < NQ; ++q) {
-      const int r = row0 + q * 8 + g;
-      const T* p = reinterpret_cast<const T*>(a.q) + (((long long)b * c.S + (r < rows ? r / group : 0)) * a.Hq + kvh * group + (r < rows ? r % group : 0)) * D;
-      float fq = 1.f;
-      if constexpr (!C::E8) {
-#pragma unroll
-        for (int i = 0; i < KL; ++i) {
-          uint4 v = make_uint4(0, 0, 0, 0);
-          if (r < rows) v = *reinterpret_cast<const uint4*>(p + (i * 4 + t) * 8);
-          qf[q][2 * i][0] = v.x; qf[q][2 * i][1] = v.y;
-          qf[q][2 * i + 1][0] = v.z; qf[q][2 * i + 1][1] = v.w;
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < KL; ++i)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            uint4 v = make_uint4(0, 0, 0, 0);
-            if (r < rows) v = *reinterpret_cast<const uint4*>(p + (i * 4 + t) * 16 + h * 8);
-            qf[q][4 * i + 2 * h][0] = v.x; qf[q][4 * i + 2 * h][1] = v.y;
-            qf[q][4 * i + 2 * h + 1][0] = v.z; qf[q][4 * i + 2 * h + 1][1] = v.w;
-          }
-        if constexpr (C::OBF) {          // bf16 -> fp16 with the row's largest in [2^14, 2^15)
-          uint32_t top = 0;
-#pragma unroll
-          for (int i = 0; i < MT; ++i)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const float2 x = unpack2<true>(qf[q][i][h]);
-              top = max(top, max(finite_bits(x.x), finite_bits(x.y)));
-            }
-          top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-          top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-          int e = (int)(top >> 23) - 127 - 14;
-          e = e < -100 ? -100 : e;
-          const float inv = exp2i(-e);
-          fq = exp2i(e);
-#pragma unroll
-          for (int i = 0; i < MT; ++i)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const float2 x = unpack2<true>(qf[q][i][h]);
-              qf[q][i][h] = pack2c<false>(x.x * inv, x.y * inv);
-            }
-        }
-      }
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        factor[q][e] = sl2 * __shfl_sync(0xffffffffu, fq, (2 * t + e) * 4);
-        const int rr = row0 + q * 8 + 2 * t + e, s = rr / group;
-        end[q][e] = rr < rows && s < cnt ? min(keys, max(0, len - cnt + s + 1)) : 0;
-      }
-    }
-
-    float o[NQ][MT][4], m[NQ][2], l[NQ][2];
-#pragma unroll
-    for (int q = 0; q < NQ; ++q) {
-#pragma unroll
-      for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[q][i][e] = 0.f;
-#pragma unroll
-      for (int e = 0; e < 2; ++e) { m[q][e] = -INFINITY; l[q][e] = 0.f; }
-    }
-    int vtop = -1000;                  // the power of two that the accumulators are relative to
-
     // ---- loads ------------------------------------------------------------------------------------------------------
     const int* pages = c.table + (size_t)b * c.per;
     int pg = c0 * NS / tpp, sub = c0 * NS - pg * tpp, tile = c0 * NS;      // the next tile whose page is asked for
@@ -309,6 +239,21 @@ paged_attend_kernel(const AttendArgs a, const Paged c, const AttendPlan plan) {
         else row[i] = ((long long)id[i] * c.Hkv + kvh) * c.page + place[i];
       }
     };
+    ask();
+    // queries as the B operand: row g, the d that this lane has of a key's row
+    uint32_t qf[NQ][MT][2];
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) {
+      const int r = row0 + q * 8 + g;
+      const T* p = reinterpret_cast<const T*>(a.q) + (((long long)b * c.S + (r < rows ? r / group : 0)) * a.Hq + kvh * group + (r < rows ? r % group : 0)) * D;
+      constexpr int H = C::E8 ? 2 : 1;           // 16-byte loads that go with one of a key's row
+#pragma unroll
+      for (int i = 0; i < KL * H; ++i) {
+        const uint4 v = ld_stream16(p + ((i / H) * 4 + t) * 8 * H + (i % H) * 8, r < rows);
+        qf[q][2 * i][0] = v.x; qf[q][2 * i][1] = v.y;
+        qf[q][2 * i + 1][0] = v.z; qf[q][2 * i + 1][1] = v.w;
+      }
+    }
     uint4 kr[NS][2][KL];
     uint32_t vr[NS][4][VW], sc[NS];
     auto load_k = [&](int chunk) {
@@ -349,11 +294,58 @@ paged_attend_kernel(const AttendArgs a, const Paged c, const AttendPlan plan) {
         }
       }
     };
-    ask();
     resolve();
     load_k(c0);
     load_v(c0);
     ask();
+
+    float factor[NQ][2];               // of the scores of queries 2t, 2t + 1
+    int end[NQ][2];                    // keys that they see
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) {
+      float fq = 1.f;
+      if constexpr (C::E8 && C::OBF) {   // bf16 -> fp16 with the row's largest in [2^14, 2^15)
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float2 x = unpack2<true>(qf[q][i][h]);
+            top = max(top, max(finite_bits(x.x), finite_bits(x.y)));
+          }
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        int e = (int)(top >> 23) - 127 - 14;
+        e = e < -100 ? -100 : e;
+        const float inv = exp2i(-e);
+        fq = exp2i(e);
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float2 x = unpack2<true>(qf[q][i][h]);
+            qf[q][i][h] = pack2c<false>(x.x * inv, x.y * inv);
+          }
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        factor[q][e] = sl2 * __shfl_sync(0xffffffffu, fq, (2 * t + e) * 4);
+        const int rr = row0 + q * 8 + 2 * t + e, s = rr / group;
+        end[q][e] = rr < rows && s < cnt ? min(keys, max(0, len - cnt + s + 1)) : 0;
+      }
+    }
+
+    float o[NQ][MT][4], m[NQ][2], l[NQ][2];
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) {
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[q][i][e] = 0.f;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) { m[q][e] = -INFINITY; l[q][e] = 0.f; }
+    }
+    int vtop = -1000;                  // the power of two that the accumulators are relative to
 
     for (int ch = c0; ch < c1; ++ch) {
       // ---- S^T = K Q^T ----------------------------------------------------------------------------------------------
@@ -622,26 +614,62 @@ paged_attend_kernel(const AttendArgs a, const Paged c, const AttendPlan plan) {
 }
 
 // Joins the items that several CTAs have parts of: CTA i takes the one that begins in CTA i of the kernel above and goes on.
+// The maxima of all parts first, so that the sums are independent loads; groups of threads share the parts.
+constexpr int PJ_THREADS = 512;
 template <typename T, int D, int R>
-__global__ void __launch_bounds__(R * D / 4) paged_join_kernel(const AttendArgs a, const Paged c, const AttendPlan plan) {
-  const int item = plan.desc[2 * blockIdx.x], last = plan.desc[2 * blockIdx.x + 1];
+__global__ void __launch_bounds__(PJ_THREADS) paged_join_kernel(const AttendArgs a, const Paged c, const AttendPlan plan) {
+  constexpr int SLOTS = R * D / 4, GROUPS = PJ_THREADS / SLOTS, WARPS = PJ_THREADS / 32;
+  extern __shared__ float weight[];                    // [parts][R]
+  __shared__ float red[WARPS][R];
+  __shared__ float4 sums[GROUPS > 1 ? GROUPS - 1 : 1][SLOTS];
+  const int first = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int item = plan.desc[2 * first], last = plan.desc[2 * first + 1];
   if (item < 0) return;
-  const int b = item / plan.per_seq, idx = item % plan.per_seq, kvh = idx / plan.tiles;
-  const int r = threadIdx.x / (D / 4), d = threadIdx.x % (D / 4) * 4, row = idx % plan.tiles * R + r;
-  if (row >= c.S * (a.Hq / c.Hkv)) return;
-  const float* stats = plan.parts + (size_t)plan.grid * 2 * R * D;
+  const int parts = last - first + 1;
+  const float2* stats = reinterpret_cast<const float2*>(plan.parts + (size_t)plan.grid * 2 * R * D);
+  auto part = [&](int k) { return (size_t)(first + k) * 2 + (k == 0 ? 1 : 0); };
+  const int r1 = tid % R;
+  // over the threads of the row r1: lanes R apart, then warps
+  auto over_parts = [&](float v, auto op) {
+#pragma unroll
+    for (int w = R; w < 32; w <<= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, w));
+    __syncthreads();
+    if (lane < R) red[warp][lane] = v;
+    __syncthreads();
+  };
   float m = -INFINITY, l = 0.f;
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-  for (int k = blockIdx.x; k <= last; ++k) {
-    const size_t part = (size_t)k * 2 + (k == (int)blockIdx.x ? 1 : 0);
-    const float2 st = *reinterpret_cast<const float2*>(stats + (part * R + r) * 2);
-    const float4 v = *reinterpret_cast<const float4*>(plan.parts + (part * R + r) * D + d);
-    const float mn = fmaxf(m, st.x), wa = part_weight(m, mn), wb = part_weight(st.x, mn);
-    acc.x = acc.x * wa + v.x * wb; acc.y = acc.y * wa + v.y * wb; acc.z = acc.z * wa + v.z * wb; acc.w = acc.w * wa + v.w * wb;
-    l = l * wa + st.y * wb;
-    m = mn;
+  for (int i = tid; i < parts * R; i += PJ_THREADS) m = fmaxf(m, weight[i] = stats[part(i / R) * R + r1].x);
+  over_parts(m, [](float x, float y) { return fmaxf(x, y); });
+  for (int w = 0; w < WARPS; ++w) m = fmaxf(m, red[w][r1]);
+  for (int i = tid; i < parts * R; i += PJ_THREADS) {
+    const float w = part_weight(weight[i], m);
+    weight[i] = w;
+    l += w * stats[part(i / R) * R + r1].y;
   }
+  over_parts(l, [](float x, float y) { return x + y; });
+  const int slot = tid % SLOTS, group = tid / SLOTS, r = slot / (D / 4), d = slot % (D / 4) * 4;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+  for (int k = group; k < parts; k += GROUPS) {
+    const float w = weight[k * R + r];
+    const float4 v = *reinterpret_cast<const float4*>(plan.parts + (part(k) * R + r) * D + d);
+    acc.x += w * v.x; acc.y += w * v.y; acc.z += w * v.z; acc.w += w * v.w;
+  }
+  if constexpr (GROUPS > 1) {
+    if (group > 0) sums[group - 1][slot] = acc;
+    __syncthreads();
+    if (group > 0) return;
+#pragma unroll
+    for (int k = 0; k < GROUPS - 1; ++k) {
+      const float4 v = sums[k][slot];
+      acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
+    }
+  }
+  const int b = item / plan.per_seq, idx = item % plan.per_seq, kvh = idx / plan.tiles, row = idx % plan.tiles * R + r;
+  if (row >= c.S * (a.Hq / c.Hkv)) return;
+  l = 0.f;
+  for (int w = 0; w < WARPS; ++w) l += red[w][r];
   store_row4<T>(a, c, b, kvh, row, d, acc, l);
 }
 
@@ -660,8 +688,18 @@ static int launch_attend(const AttendArgs& a, const Paged& c, float* parts, int*
   paged_attend_kernel<T, CDT, D, NQ><<<grid, PA_WARPS * 32, C::SMEM, st>>>(a, c, plan);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return (int)e;
-  paged_join_kernel<T, D, C::R><<<grid, C::R * D / 4, 0, st>>>(a, c, plan);
-  return (int)cudaGetLastError();
+  cudaLaunchConfig_t lc{};
+  lc.gridDim = dim3(grid);
+  lc.blockDim = dim3(PJ_THREADS);
+  lc.dynamicSmemBytes = (size_t)grid * C::R * 4;
+  lc.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  lc.attrs = at;
+  lc.numAttrs = 1;
+  e = cudaLaunchKernelEx(&lc, paged_join_kernel<T, D, C::R>, a, c, plan);
+  return e != cudaSuccess ? (int)e : (int)cudaGetLastError();
 }
 
 // Any type and head size: a CTA takes a row of queries, its warps every fourth key, their lanes a share of the head.
