@@ -67,17 +67,17 @@ struct PA {
   }
 };
 
-__device__ __forceinline__ uint4 ld_stream16(const void* p, bool on) {        // zeros where it is off
+// keys that are not there are read from here, so that loads need no predicates (and no moves of zeros)
+__device__ const uint4 PA_ZEROS[16] = {};
+
+__device__ __forceinline__ uint4 ld_stream16(const void* p) {
   uint4 v;
-  asm volatile("{\n\t.reg .pred P;\n\tsetp.ne.b32 P, %5, 0;\n\tmov.u32 %0, 0;\n\tmov.u32 %1, 0;\n\tmov.u32 %2, 0;\n\tmov.u32 %3, 0;\n\t"
-               "@P ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];\n\t}"
-               : "=&r"(v.x), "=&r"(v.y), "=&r"(v.z), "=&r"(v.w) : "l"(p), "r"((int)on));
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
   return v;
 }
-__device__ __forceinline__ uint2 ld_stream8(const void* p, bool on) {
+__device__ __forceinline__ uint2 ld_stream8(const void* p) {
   uint2 v;
-  asm volatile("{\n\t.reg .pred P;\n\tsetp.ne.b32 P, %3, 0;\n\tmov.u32 %0, 0;\n\tmov.u32 %1, 0;\n\t"
-               "@P ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];\n\t}" : "=&r"(v.x), "=&r"(v.y) : "l"(p), "r"((int)on));
+  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
   return v;
 }
 // a bit for each 16-bit half of v that is an infinity or NaN
@@ -86,10 +86,10 @@ __device__ __forceinline__ uint32_t not_finite2(uint32_t v) {
   constexpr uint32_t E = BF ? 0x7f80u : 0x7c00u;
   return ((v & E) == E ? 1u : 0u) | ((v >> 16 & E) == E ? 2u : 0u);
 }
-__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t v) {        // the low 16 bits
-  uint32_t r;
-  asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(r) : "r"(v));
-  return r;
+// four e4m3 numbers as two pairs of fp16
+__device__ __forceinline__ void e4m3x4_to_f16(uint32_t v, uint32_t& lo, uint32_t& hi) {
+  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+      : "=r"(lo), "=r"(hi) : "r"(v));
 }
 __device__ __forceinline__ uint32_t transposed_8x8(uint32_t v) {
   uint32_t r;
@@ -140,7 +140,8 @@ __device__ __forceinline__ void store_row4(const AttendArgs& a, const Paged& c, 
   *reinterpret_cast<uint2*>(p) = w;
 }
 
-template <typename T, int CDT, int D, int NQ>
+// MULTI: several tokens a sequence, whose rows end at different keys
+template <typename T, int CDT, int D, int NQ, bool MULTI>
 __global__ void __launch_bounds__(PA_WARPS * 32, NQ == 1 ? 3 : 2)
 paged_attend_kernel(const AttendArgs a, const Paged c, const AttendPlan plan) {
   using C = PA<T, CDT, D, NQ>;
@@ -216,27 +217,17 @@ paged_attend_kernel(const AttendArgs a, const Paged c, const AttendPlan plan) {
     if (len > keys && cnt > 0 && c0 == 0 && lane == 0) report_error(c.status, GB_ERR_BAD_INDEX, SITE_POSITION, len - 1);
 
     // ---- loads ------------------------------------------------------------------------------------------------------
+    const char* const zeros = reinterpret_cast<const char*>(PA_ZEROS);
     const int* pages = c.table + (size_t)b * c.per;
-    int pg = c0 * NS / tpp, sub = c0 * NS - pg * tpp, tile = c0 * NS;      // the next tile whose page is asked for
+    int tile = c0 * NS, pg = tile / tpp, sub = tile - pg * tpp;            // the next tile whose page is asked for
     int id[NS], place[NS];
     auto ask = [&]() {
 #pragma unroll
       for (int i = 0; i < NS; ++i) {
-        id[i] = -1;
         place[i] = -1;
         if (tile * 16 < keys) { id[i] = pages[pg]; place[i] = sub * 16; }
         ++tile;
         if (++sub == tpp) { sub = 0; ++pg; }
-      }
-    };
-    long long row[NS];
-    auto resolve = [&]() {
-#pragma unroll
-      for (int i = 0; i < NS; ++i) {
-        row[i] = -1;
-        if (place[i] < 0) continue;
-        if (id[i] < 0 || id[i] >= c.pages) { if (lane == 0) report_error(c.status, GB_ERR_BAD_INDEX, SITE_PAGE, id[i]); }
-        else row[i] = ((long long)id[i] * c.Hkv + kvh) * c.page + place[i];
       }
     };
     ask();
@@ -249,58 +240,16 @@ paged_attend_kernel(const AttendArgs a, const Paged c, const AttendPlan plan) {
       constexpr int H = C::E8 ? 2 : 1;           // 16-byte loads that go with one of a key's row
 #pragma unroll
       for (int i = 0; i < KL * H; ++i) {
-        const uint4 v = ld_stream16(p + ((i / H) * 4 + t) * 8 * H + (i % H) * 8, r < rows);
+        const uint4 v = ld_stream16(r < rows ? reinterpret_cast<const char*>(p + ((i / H) * 4 + t) * 8 * H + (i % H) * 8) : zeros);
         qf[q][2 * i][0] = v.x; qf[q][2 * i][1] = v.y;
         qf[q][2 * i + 1][0] = v.z; qf[q][2 * i + 1][1] = v.w;
       }
     }
+    long long row[NS];                 // of the pool; -1: no such tile
     uint4 kr[NS][2][KL];
     uint32_t vr[NS][4][VW], sc[NS];
-    auto load_k = [&](int chunk) {
-#pragma unroll
-      for (int i = 0; i < NS; ++i) {
-        const int left = keys - (chunk * NS + i) * 16;
-        const char* p = reinterpret_cast<const char*>(a.kpool) + row[i] * (D * C::ES) + t * 16;
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int j = 0; j < KL; ++j)
-            kr[i][h][j] = ld_stream16(p + (g + 8 * h) * (D * C::ES) + j * 64, row[i] >= 0 && g + 8 * h < left);
-        if constexpr (C::E8) {         // lanes 0 - 15: K's powers of two, 16 - 31: V's
-          sc[i] = 127;
-          if (row[i] >= 0 && (lane & 15) < left) sc[i] = (lane < 16 ? a.kscale : a.vscale)[row[i] + (lane & 15)];
-        }
-      }
-    };
-    auto load_v = [&](int chunk) {
-#pragma unroll
-      for (int i = 0; i < NS; ++i) {
-        const int left = keys - (chunk * NS + i) * 16;
-        const char* p = reinterpret_cast<const char*>(a.vpool) + row[i] * (D * C::ES);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int key = 2 * t + (k & 1) + (k >> 1) * 8;
-          const bool on = row[i] >= 0 && key < left;
-          if constexpr (VW == 2) {
-            const uint2 v = ld_stream8(p + key * (D * C::ES) + g * 8, on);
-            vr[i][k][0] = v.x; vr[i][k][1] = v.y;
-          } else {
-#pragma unroll
-            for (int j = 0; j < VW / 4; ++j) {
-              const uint4 v = ld_stream16(p + key * (D * C::ES) + (g + 8 * j) * 16, on);
-              vr[i][k][4 * j] = v.x; vr[i][k][4 * j + 1] = v.y; vr[i][k][4 * j + 2] = v.z; vr[i][k][4 * j + 3] = v.w;
-            }
-          }
-        }
-      }
-    };
-    resolve();
-    load_k(c0);
-    load_v(c0);
-    ask();
-
     float factor[NQ][2];               // of the scores of queries 2t, 2t + 1
-    int end[NQ][2];                    // keys that they see
+    int end[NQ][2];                    // keys that they see (without MULTI: all, or it is no row)
 #pragma unroll
     for (int q = 0; q < NQ; ++q) {
       float fq = 1.f;
@@ -330,12 +279,17 @@ paged_attend_kernel(const AttendArgs a, const Paged c, const AttendPlan plan) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         factor[q][e] = sl2 * __shfl_sync(0xffffffffu, fq, (2 * t + e) * 4);
-        const int rr = row0 + q * 8 + 2 * t + e, s = rr / group;
-        end[q][e] = rr < rows && s < cnt ? min(keys, max(0, len - cnt + s + 1)) : 0;
+        if constexpr (MULTI) {
+          const int rr = row0 + q * 8 + 2 * t + e, s = rr / group;
+          end[q][e] = rr < rows && s < cnt ? min(keys, max(0, len - cnt + s + 1)) : 0;
+        } else {
+          end[q][e] = keys;
+        }
       }
     }
 
-    float o[NQ][MT][4], m[NQ][2], l[NQ][2];
+    // running maximum m (may lag 2^8 behind), what the exponents are taken off by, normaliser: of this lane's keys
+    float o[NQ][MT][4], m[NQ][2], off[NQ][2], l[NQ][2];
 #pragma unroll
     for (int q = 0; q < NQ; ++q) {
 #pragma unroll
@@ -343,196 +297,263 @@ paged_attend_kernel(const AttendArgs a, const Paged c, const AttendPlan plan) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[q][i][e] = 0.f;
 #pragma unroll
-      for (int e = 0; e < 2; ++e) { m[q][e] = -INFINITY; l[q][e] = 0.f; }
+      for (int e = 0; e < 2; ++e) { m[q][e] = -INFINITY; off[q][e] = 0.f; l[q][e] = 0.f; }
     }
-    int vtop = -1000;                  // the power of two that the accumulators are relative to
+    constexpr float LIFT = !C::E8 && !C::BF ? 7.f : 0.f;      // fp16 P without a scale of its own
+    int vtop = -1000;                  // the power of two of V that the accumulators are relative to
+    const int full = MULTI ? min(keys, max(0, len - cnt + 1)) : keys;      // keys that every token sees
 
-    for (int ch = c0; ch < c1; ++ch) {
+    // one round: scores of chunk ch, K of chunk ch + 1 on its way, probabilities and products of ch, V of ch + 1 on its way
+    for (int ch = c0 - 1; ch < c1; ++ch) {
+      const bool now = ch >= c0, more = ch + 1 < c1;
       // ---- S^T = K Q^T ----------------------------------------------------------------------------------------------
       float s[NS][NQ][4];
-      bool gone[NS];
       float ks[NS][2];
       int ve[NS][2];
+      uint32_t gone = 0;
+      if (now) {
 #pragma unroll
-      for (int i = 0; i < NS; ++i) {
-        gone[i] = row[i] < 0;
+        for (int i = 0; i < NS; ++i) {
+          if (row[i] < 0) gone |= 1u << i;
 #pragma unroll
-        for (int q = 0; q < NQ; ++q)
+          for (int q = 0; q < NQ; ++q)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[i][q][e] = 0.f;
+            for (int e = 0; e < 4; ++e) s[i][q][e] = 0.f;
 #pragma unroll
-        for (int j = 0; j < KL; ++j) {
-          const uint32_t lo[4] = {kr[i][0][j].x, kr[i][0][j].y, kr[i][0][j].z, kr[i][0][j].w};
-          const uint32_t hi[4] = {kr[i][1][j].x, kr[i][1][j].y, kr[i][1][j].z, kr[i][1][j].w};
-          if constexpr (!C::E8) {
+          for (int j = 0; j < KL; ++j) {
+            const uint32_t lo[4] = {kr[i][0][j].x, kr[i][0][j].y, kr[i][0][j].z, kr[i][0][j].w};
+            const uint32_t hi[4] = {kr[i][1][j].x, kr[i][1][j].y, kr[i][1][j].z, kr[i][1][j].w};
+            if constexpr (!C::E8) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
+              for (int h = 0; h < 2; ++h)
 #pragma unroll
-              for (int q = 0; q < NQ; ++q)
-                mma_k16<C::BF>(s[i][q], lo[2 * h], hi[2 * h], lo[2 * h + 1], hi[2 * h + 1], qf[q][2 * j + h][0], qf[q][2 * j + h][1]);
-          } else {
+                for (int q = 0; q < NQ; ++q)
+                  mma_k16<C::BF>(s[i][q], lo[2 * h], hi[2 * h], lo[2 * h + 1], hi[2 * h + 1], qf[q][2 * j + h][0], qf[q][2 * j + h][1]);
+            } else {
 #pragma unroll
-            for (int h = 0; h < 4; ++h) {
-              const uint32_t a0 = e4m3x2_to_f16x2(lo[h]), a2 = e4m3x2_to_f16x2(lo[h] >> 16);
-              const uint32_t a1 = e4m3x2_to_f16x2(hi[h]), a3 = e4m3x2_to_f16x2(hi[h] >> 16);
+              for (int h = 0; h < 4; ++h) {
+                uint32_t a0, a1, a2, a3;
+                e4m3x4_to_f16(lo[h], a0, a2);
+                e4m3x4_to_f16(hi[h], a1, a3);
 #pragma unroll
-              for (int q = 0; q < NQ; ++q) mma_k16<false>(s[i][q], a0, a1, a2, a3, qf[q][4 * j + h][0], qf[q][4 * j + h][1]);
+                for (int q = 0; q < NQ; ++q) mma_k16<false>(s[i][q], a0, a1, a2, a3, qf[q][4 * j + h][0], qf[q][4 * j + h][1]);
+              }
+            }
+          }
+          if constexpr (C::E8) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              ks[i][h] = __uint_as_float(__shfl_sync(0xffffffffu, sc[i], g + 8 * h) << 23);
+              ve[i][h] = (int)__shfl_sync(0xffffffffu, sc[i], 16 + g + 8 * h) - 127;
             }
           }
         }
-        if constexpr (C::E8) {
+      }
+      if (more) {
+#pragma unroll
+        for (int i = 0; i < NS; ++i) {
+          row[i] = -1;
+          if (place[i] >= 0) {
+            if ((unsigned)id[i] >= (unsigned)c.pages) { if (lane == 0) report_error(c.status, GB_ERR_BAD_INDEX, SITE_PAGE, id[i]); }
+            else row[i] = ((long long)id[i] * c.Hkv + kvh) * c.page + place[i];
+          }
+          const int left = row[i] < 0 ? 0 : keys - ((ch + 1) * NS + i) * 16;
+          const char* p = reinterpret_cast<const char*>(a.kpool) + (row[i] + g) * (D * C::ES) + t * 16;
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            ks[i][h] = __uint_as_float(__shfl_sync(0xffffffffu, sc[i], g + 8 * h) << 23);
-            ve[i][h] = (int)__shfl_sync(0xffffffffu, sc[i], 16 + g + 8 * h) - 127;
+            const char* pk = g + 8 * h < left ? p + 8 * h * (D * C::ES) : zeros;
+#pragma unroll
+            for (int j = 0; j < KL; ++j) kr[i][h][j] = ld_stream16(pk + j * 64);
+          }
+          if constexpr (C::E8) {       // lanes 0 - 15: K's powers of two, 16 - 31: V's
+            sc[i] = 0;
+            if ((lane & 15) < left) sc[i] = (lane < 16 ? a.kscale : a.vscale)[row[i] + (lane & 15)];
           }
         }
-      }
-      const bool more = ch + 1 < c1;
-      if (more) {
-        resolve();
-        load_k(ch + 1);
         ask();
       }
-      // ---- probabilities --------------------------------------------------------------------------------------------
-      bool grow = false;
+      if (now) {
+        // ---- probabilities ------------------------------------------------------------------------------------------
+        float top[NQ][2];
 #pragma unroll
-      for (int i = 0; i < NS; ++i)
+        for (int q = 0; q < NQ; ++q)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int key = (ch * NS + i) * 16 + g + 8 * h;
+          for (int e = 0; e < 2; ++e) top[q][e] = -INFINITY;
+        bool grow = false;
+        const bool tail = gone != 0 || (ch + 1) * KT > full;
+#pragma unroll
+        for (int i = 0; i < NS; ++i)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            if constexpr (C::E8) grow |= ve[i][h] > vtop;
+#pragma unroll
+            for (int q = 0; q < NQ; ++q)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                float& x = s[i][q][2 * h + e];
+                x *= C::E8 ? factor[q][e] * ks[i][h] : factor[q][e];
+                if (tail && ((gone >> i & 1) || (ch * NS + i) * 16 + g + 8 * h >= end[q][e])) x = -INFINITY;
+                top[q][e] = fmaxf(top[q][e], x);
+              }
+          }
+#pragma unroll
+        for (int q = 0; q < NQ; ++q)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) grow |= top[q][e] > m[q][e] + 8.f;
+        if (__any_sync(0xffffffffu, grow)) {
+          float vscale = 1.f;
           if constexpr (C::E8) {
-            if (gone[i] || key >= keys) ve[i][h] = -1000;
-            grow |= ve[i][h] > vtop;
+            int e = vtop;
+#pragma unroll
+            for (int i = 0; i < NS; ++i) e = max(e, max(ve[i][0], ve[i][1]));
+            e = __reduce_max_sync(0xffffffffu, e);
+            vscale = vtop - e < -126 ? 0.f : exp2i(vtop - e);
+            vtop = e;
           }
 #pragma unroll
           for (int q = 0; q < NQ; ++q)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              float& x = s[i][q][2 * h + e];
-              x *= factor[q][e];
-              if constexpr (C::E8) x *= ks[i][h];
-              if (gone[i] || key >= end[q][e]) x = -INFINITY;
-              grow |= x > m[q][e] + 8.f;
+              float x = fmaxf(m[q][e], top[q][e]);
+#pragma unroll
+              for (int w = 4; w < 32; w <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, w));
+              const float alpha = part_weight(m[q][e], x);
+              m[q][e] = x;
+              off[q][e] = x == -INFINITY ? 0.f : x - LIFT;
+              l[q][e] *= alpha;
+#pragma unroll
+              for (int i = 0; i < MT; ++i) {
+                o[q][i][e] *= alpha * vscale;
+                o[q][i][2 + e] *= alpha * vscale;
+              }
             }
         }
-      if (__any_sync(0xffffffffu, grow)) {
-        float vscale = 1.f;
-        if constexpr (C::E8) {
-          int e = vtop;
+        uint32_t ph[NS][NQ][2], pl[NS][NQ][2];
 #pragma unroll
-          for (int i = 0; i < NS; ++i) e = max(e, max(ve[i][0], ve[i][1]));
-          e = __reduce_max_sync(0xffffffffu, e);
-          vscale = vtop - e < -126 ? 0.f : exp2i(vtop - e);
-          vtop = e;
-        }
-#pragma unroll
-        for (int q = 0; q < NQ; ++q)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float x = m[q][e];
-#pragma unroll
-            for (int i = 0; i < NS; ++i) x = fmaxf(x, fmaxf(s[i][q][e], s[i][q][2 + e]));
-#pragma unroll
-            for (int w = 4; w < 32; w <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, w));
-            const float alpha = part_weight(m[q][e], x);
-            m[q][e] = x;
-            l[q][e] *= alpha;
-#pragma unroll
-            for (int i = 0; i < MT; ++i) {
-              o[q][i][e] *= alpha * vscale;
-              o[q][i][2 + e] *= alpha * vscale;
-            }
-          }
-      }
-      uint32_t ph[NS][NQ][2], pl[NS][NQ][2];
-#pragma unroll
-      for (int i = 0; i < NS; ++i)
-#pragma unroll
-        for (int q = 0; q < NQ; ++q)
+        for (int i = 0; i < NS; ++i)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            float p[2];
+            const float vs = C::E8 ? exp2i(max(ve[i][h] - vtop + 7, -126)) : 1.f;
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              p[e] = pow2_of(s[i][q][2 * h + e] - (m[q][e] == -INFINITY ? 0.f : m[q][e]));
-              l[q][e] += p[e];
-              if constexpr (C::E8) p[e] *= ve[i][h] - vtop + 7 < -126 ? 0.f : exp2i(ve[i][h] - vtop + 7);
-              else if constexpr (!C::BF) p[e] *= 128.f;
-            }
-            const uint32_t w = pack2c<C::BF>(p[0], p[1]);
-            ph[i][q][h] = transposed_8x8(w);
-            if constexpr (C::SPLIT) {
-              const float2 r = unpack2<C::BF>(w);
-              pl[i][q][h] = transposed_8x8(pack2c<C::BF>(p[0] - r.x, p[1] - r.y));
-            }
-          }
-      // ---- O^T += V^T P^T -------------------------------------------------------------------------------------------
-      // rows of a call with several tokens end at different keys; a key that one row sees and another does not is multiplied by
-      // a probability of 0 there, which an infinity or NaN among its values would turn into NaN
-      const bool ragged = c.S > 1 && (ch + 1) * KT > len - cnt;
+            for (int q = 0; q < NQ; ++q) {
+              float p[2];
 #pragma unroll
-      for (int i = 0; i < NS; ++i)
-#pragma unroll
-        for (int j = 0; j < VW * (C::E8 ? 2 : 1); ++j) {
-          uint32_t v[4];
-          if constexpr (!C::E8) {
-            v[0] = __byte_perm(vr[i][0][j], vr[i][1][j], 0x5410);
-            v[1] = __byte_perm(vr[i][0][j], vr[i][1][j], 0x7632);
-            v[2] = __byte_perm(vr[i][2][j], vr[i][3][j], 0x5410);
-            v[3] = __byte_perm(vr[i][2][j], vr[i][3][j], 0x7632);
-          } else {
-            const uint32_t x = __byte_perm(vr[i][0][j / 2], vr[i][1][j / 2], j & 1 ? 0x7362 : 0x5140);
-            const uint32_t y = __byte_perm(vr[i][2][j / 2], vr[i][3][j / 2], j & 1 ? 0x7362 : 0x5140);
-            v[0] = e4m3x2_to_f16x2(x); v[1] = e4m3x2_to_f16x2(x >> 16);
-            v[2] = e4m3x2_to_f16x2(y); v[3] = e4m3x2_to_f16x2(y >> 16);
-          }
-          uint32_t bad = 0;
-          if (ragged) {
-#pragma unroll
-            for (int k = 0; k < 4; ++k) bad |= not_finite2<C::BF>(v[k]);
-            bad = __any_sync(0xffffffffu, bad != 0);
-          }
-#pragma unroll
-          for (int q = 0; q < NQ; ++q) {
-            float kept[4];
-            if (bad) {
-#pragma unroll
-              for (int e = 0; e < 4; ++e) kept[e] = o[q][j][e];
-            }
-            mma_k16<C::BF>(o[q][j], v[0], v[1], v[2], v[3], ph[i][q][0], ph[i][q][1]);
-            if constexpr (C::SPLIT) mma_k16<C::BF>(o[q][j], v[0], v[1], v[2], v[3], pl[i][q][0], pl[i][q][1]);
-            if (bad) {
-              // the same without those values for the rows that do not see them: how many of them a row sees is a product too
-              uint32_t fine[4], mark[4], sees[2];
-              constexpr uint32_t ONE = C::BF ? 0x3f80u : 0x3c00u;
-#pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                const uint32_t f = not_finite2<C::BF>(v[k]);
-                fine[k] = v[k] & ((f & 1 ? 0u : 0xffffu) | (f & 2 ? 0u : 0xffff0000u));
-                mark[k] = (f & 1 ? ONE : 0u) | (f & 2 ? ONE << 16 : 0u);
+              for (int e = 0; e < 2; ++e) {
+                p[e] = pow2_of(s[i][q][2 * h + e] - off[q][e]);
+                l[q][e] += p[e];
+                if constexpr (C::E8) p[e] *= vs;
               }
-#pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                const int key = (ch * NS + i) * 16 + g + 8 * h;
-                sees[h] = transposed_8x8((key < end[q][0] ? ONE : 0u) | (key < end[q][1] ? ONE << 16 : 0u));
+              const uint32_t w = pack2c<C::BF>(p[0], p[1]);
+              ph[i][q][h] = transposed_8x8(w);
+              if constexpr (C::SPLIT) {
+                const float2 r = unpack2<C::BF>(w);
+                pl[i][q][h] = transposed_8x8(pack2c<C::BF>(p[0] - r.x, p[1] - r.y));
               }
-              float seen[4] = {0.f, 0.f, 0.f, 0.f};
-              mma_k16<C::BF>(seen, mark[0], mark[1], mark[2], mark[3], sees[0], sees[1]);
-              mma_k16<C::BF>(kept, fine[0], fine[1], fine[2], fine[3], ph[i][q][0], ph[i][q][1]);
-              if constexpr (C::SPLIT) mma_k16<C::BF>(kept, fine[0], fine[1], fine[2], fine[3], pl[i][q][0], pl[i][q][1]);
+            }
+          }
+        // ---- O^T += V^T P^T -----------------------------------------------------------------------------------------
 #pragma unroll
-              for (int e = 0; e < 4; ++e) o[q][j][e] = seen[e] == 0.f ? kept[e] : o[q][j][e];
+        for (int i = 0; i < NS; ++i)
+#pragma unroll
+          for (int j = 0; j < VW; ++j) {
+            constexpr int H = C::E8 ? 2 : 1;         // tiles of a word
+            uint32_t v[H][4];
+            if constexpr (!C::E8) {
+              v[0][0] = __byte_perm(vr[i][0][j], vr[i][1][j], 0x5410);
+              v[0][1] = __byte_perm(vr[i][0][j], vr[i][1][j], 0x7632);
+              v[0][2] = __byte_perm(vr[i][2][j], vr[i][3][j], 0x5410);
+              v[0][3] = __byte_perm(vr[i][2][j], vr[i][3][j], 0x7632);
+            } else {
+#pragma unroll
+              for (int h = 0; h < H; ++h) {
+                e4m3x4_to_f16(__byte_perm(vr[i][0][j], vr[i][1][j], h ? 0x7362 : 0x5140), v[h][0], v[h][1]);
+                e4m3x4_to_f16(__byte_perm(vr[i][2][j], vr[i][3][j], h ? 0x7362 : 0x5140), v[h][2], v[h][3]);
+              }
+            }
+#pragma unroll
+            for (int h = 0; h < H; ++h)
+#pragma unroll
+              for (int q = 0; q < NQ; ++q) {
+                float (&acc)[4] = o[q][j * H + h];
+                const uint32_t (&x)[4] = v[h];
+                if constexpr (MULTI) {
+                  // a key that one row sees and another does not is multiplied by a probability of 0 there, which an infinity
+                  // or NaN among its values would turn into NaN
+                  uint32_t bad = 0;
+                  if (tail) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) bad |= not_finite2<C::BF>(x[k]);
+                    bad = __any_sync(0xffffffffu, bad != 0);
+                  }
+                  if (bad) {
+                    // the same without those values for the rows that do not see them; how many of them a row sees is a product too
+                    uint32_t fine[4], mark[4], sees[2];
+                    constexpr uint32_t ONE = C::BF ? 0x3f80u : 0x3c00u;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                      const uint32_t f = not_finite2<C::BF>(x[k]);
+                      fine[k] = x[k] & ((f & 1 ? 0u : 0xffffu) | (f & 2 ? 0u : 0xffff0000u));
+                      mark[k] = (f & 1 ? ONE : 0u) | (f & 2 ? ONE << 16 : 0u);
+                    }
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                      const int key = (ch * NS + i) * 16 + g + 8 * k;
+                      sees[k] = transposed_8x8((key < end[q][0] ? ONE : 0u) | (key < end[q][1] ? ONE << 16 : 0u));
+                    }
+                    float seen[4] = {0.f, 0.f, 0.f, 0.f}, kept[4] = {acc[0], acc[1], acc[2], acc[3]};
+                    mma_k16<C::BF>(seen, mark[0], mark[1], mark[2], mark[3], sees[0], sees[1]);
+                    mma_k16<C::BF>(kept, fine[0], fine[1], fine[2], fine[3], ph[i][q][0], ph[i][q][1]);
+                    if constexpr (C::SPLIT) mma_k16<C::BF>(kept, fine[0], fine[1], fine[2], fine[3], pl[i][q][0], pl[i][q][1]);
+                    mma_k16<C::BF>(acc, x[0], x[1], x[2], x[3], ph[i][q][0], ph[i][q][1]);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[e] = seen[e] == 0.f ? kept[e] : acc[e];
+                    continue;
+                  }
+                }
+                mma_k16<C::BF>(acc, x[0], x[1], x[2], x[3], ph[i][q][0], ph[i][q][1]);
+                if constexpr (C::SPLIT) mma_k16<C::BF>(acc, x[0], x[1], x[2], x[3], pl[i][q][0], pl[i][q][1]);
+              }
+          }
+      }
+      if (more) {
+#pragma unroll
+        for (int i = 0; i < NS; ++i) {
+          const int left = row[i] < 0 ? 0 : keys - ((ch + 1) * NS + i) * 16;
+          const char* p = reinterpret_cast<const char*>(a.vpool) + (row[i] + 2 * t) * (D * C::ES) + g * (VW == 2 ? 8 : 16);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            constexpr int STEP = D * C::ES;
+            const int key = (k & 1) + (k >> 1) * 8;
+            const char* pv = 2 * t + key < left ? p + key * STEP : zeros;
+            if constexpr (VW == 2) {
+              const uint2 v = ld_stream8(pv);
+              vr[i][k][0] = v.x; vr[i][k][1] = v.y;
+            } else {
+#pragma unroll
+              for (int j = 0; j < VW / 4; ++j) {
+                const uint4 v = ld_stream16(pv + 128 * j);
+                vr[i][k][4 * j] = v.x; vr[i][k][4 * j + 1] = v.y; vr[i][k][4 * j + 2] = v.z; vr[i][k][4 * j + 3] = v.w;
+              }
             }
           }
         }
-      if (more) load_v(ch + 1);
+      }
     }
 
     // ---- the run's result ---------------------------------------------------------------------------------------------
-    float unit = 1.f;
-    if constexpr (C::E8) unit = vtop - 7 < -126 ? 0.f : exp2i(vtop - 7);
-    else if constexpr (!C::BF) unit = 1.f / 128.f;
+    const float unit = C::E8 ? (vtop - 7 < -126 ? 0.f : exp2i(vtop - 7)) : 1.f;
+    if constexpr (MULTI) {             // rows that are no tokens (chunks that all tokens see are not masked)
+#pragma unroll
+      for (int q = 0; q < NQ; ++q)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          if (end[q][e] == 0) {
+            m[q][e] = -INFINITY;
+            l[q][e] = 0.f;
+#pragma unroll
+            for (int i = 0; i < MT; ++i) o[q][i][e] = o[q][i][2 + e] = 0.f;
+          }
+    }
 #pragma unroll
     for (int q = 0; q < NQ; ++q)
 #pragma unroll
@@ -554,7 +575,7 @@ paged_attend_kernel(const AttendArgs a, const Paged c, const AttendPlan plan) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int r = q * 8 + 2 * t + e;
-        if (!whole && g == 0) { piece_m[piece][r] = m[q][e]; piece_l[piece][r] = l[q][e]; }
+        if (!whole && g == 0) { piece_m[piece][r] = m[q][e] - LIFT; piece_l[piece][r] = l[q][e]; }
 #pragma unroll
         for (int i = 0; i < MT; i += 2) {
           const float4 v = make_float4(o[q][i][e] * unit, o[q][i][2 + e] * unit, o[q][i + 1][e] * unit, o[q][i + 1][2 + e] * unit);
@@ -673,19 +694,19 @@ __global__ void __launch_bounds__(PJ_THREADS) paged_join_kernel(const AttendArgs
   store_row4<T>(a, c, b, kvh, row, d, acc, l);
 }
 
-template <typename T, int CDT, int D, int NQ>
+template <typename T, int CDT, int D, int NQ, bool MULTI>
 static int launch_attend(const AttendArgs& a, const Paged& c, float* parts, int* desc, int grid, cudaStream_t st) {
   using C = PA<T, CDT, D, NQ>;
   static unsigned long long cfg = 0;
   int r;
-  if (C::SMEM > 40 * 1024 && (r = smem_opt_in(paged_attend_kernel<T, CDT, D, NQ>, C::SMEM, cfg)) != 0) return r;
+  if (C::SMEM > 40 * 1024 && (r = smem_opt_in(paged_attend_kernel<T, CDT, D, NQ, MULTI>, C::SMEM, cfg)) != 0) return r;
   AttendPlan plan;
   plan.tiles = (c.S * (a.Hq / c.Hkv) + C::R - 1) / C::R;
   plan.per_seq = plan.tiles * c.Hkv;
   plan.grid = grid;
   plan.parts = parts;
   plan.desc = desc;
-  paged_attend_kernel<T, CDT, D, NQ><<<grid, PA_WARPS * 32, C::SMEM, st>>>(a, c, plan);
+  paged_attend_kernel<T, CDT, D, NQ, MULTI><<<grid, PA_WARPS * 32, C::SMEM, st>>>(a, c, plan);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return (int)e;
   cudaLaunchConfig_t lc{};
@@ -809,12 +830,12 @@ extern "C" int gb_paged_attention(const void* q, void* o, const void* kpool, con
   if (grid > 0) {
     const int R = S * (Hq / Hkv) <= 8 ? 8 : 16;
     int* desc = reinterpret_cast<int*>(workspace + (size_t)grid * 2 * R * (D + 2));
-#define GB_ATTEND(T, C)                                                                                                    \
-    (D == 64 ? (R == 8 ? launch_attend<T, C, 64, 1>(a, c, workspace, desc, grid, st) : launch_attend<T, C, 64, 2>(a, c, workspace, desc, grid, st)) \
-             : (R == 8 ? launch_attend<T, C, 128, 1>(a, c, workspace, desc, grid, st) : launch_attend<T, C, 128, 2>(a, c, workspace, desc, grid, st)))
+#define GB_ATTEND_(T, C, D_, NQ_) (S > 1 ? launch_attend<T, C, D_, NQ_, true>(a, c, workspace, desc, grid, st) : launch_attend<T, C, D_, NQ_, false>(a, c, workspace, desc, grid, st))
+#define GB_ATTEND(T, C) (D == 64 ? (R == 8 ? GB_ATTEND_(T, C, 64, 1) : GB_ATTEND_(T, C, 64, 2)) : (R == 8 ? GB_ATTEND_(T, C, 128, 1) : GB_ATTEND_(T, C, 128, 2)))
     if (dt == DT_BF16) return cdt == DT_E4M3 ? GB_ATTEND(__nv_bfloat16, DT_E4M3) : GB_ATTEND(__nv_bfloat16, DT_BF16);
     return cdt == DT_E4M3 ? GB_ATTEND(__half, DT_E4M3) : GB_ATTEND(__half, DT_F16);
 #undef GB_ATTEND
+#undef GB_ATTEND_
   }
   GB_DISPATCH_FLOAT(dt, T, GB_DISPATCH_CACHE(cdt, C, paged_attend_any_kernel<T, C><<<(unsigned)rows, PA_WARPS * 32, 0, st>>>(a, c)));
   return (int)cudaGetLastError();
