@@ -42,8 +42,9 @@ struct AttendPlan {
   int per_seq;          // items of a sequence: Hkv * row tiles
   int tiles;            // row tiles
   int grid;             // CTAs launched
-  float* parts;         // [grid][2][R][D] sums, then [grid][2][R] maxima and normalisers
-  int* desc;            // [grid][2]: an item that begins in the CTA and goes on behind it (-1: none), and the last CTA that has it
+  float* parts;         // [grid][2][R][D] sums, then [grid][2][R] maxima and normalisers: of an item that comes from the CTA before,
+                        // and of one that begins in the CTA and goes on behind it
+  int4* spans;          // [grid][2]: that item (-1: none), the first and the last CTA that have it
 };
 
 template <typename T, int CDT, int D_, int NQ_>
@@ -85,11 +86,6 @@ template <bool BF>
 __device__ __forceinline__ uint32_t not_finite2(uint32_t v) {
   constexpr uint32_t E = BF ? 0x7f80u : 0x7c00u;
   return ((v & E) == E ? 1u : 0u) | ((v >> 16 & E) == E ? 2u : 0u);
-}
-// four e4m3 numbers as two pairs of fp16
-__device__ __forceinline__ void e4m3x4_to_f16(uint32_t v, uint32_t& lo, uint32_t& hi) {
-  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
-      : "=r"(lo), "=r"(hi) : "r"(v));
 }
 __device__ __forceinline__ uint32_t transposed_8x8(uint32_t v) {
   uint32_t r;
@@ -149,46 +145,51 @@ paged_attend_kernel(const AttendArgs a, const Paged c, const AttendPlan plan) {
   extern __shared__ __align__(16) float pieces[];                  // [2 W][R][D]
   __shared__ float piece_m[2 * W][R], piece_l[2 * W][R];
   __shared__ int piece_item[2 * W], piece_flags[2 * W];
-  __shared__ long long piece_end[2 * W], scan[W], first_chunk[W];
+  __shared__ unsigned piece_start[2 * W], piece_end[2 * W], scan[W], first_chunk[W];
   __shared__ int first_b[W];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");       // (the join waits for the end of this kernel)
 
   // ---- the share of this warp -----------------------------------------------------------------------------------------
   const int each = (c.B + W * 32 - 1) / (W * 32), b0 = min(c.B, (int)threadIdx.x * each), b1 = min(c.B, b0 + each);
-  long long mine = 0;
+  unsigned mine = 0;                   // (the host has seen to it that all chunks are less than 2^31)
   for (int b = b0; b < b1; ++b) mine += attend_chunks(attend_keys(c, b), KT);
   mine *= plan.per_seq;
-  long long upto = mine;
+  unsigned upto = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const long long x = __shfl_up_sync(0xffffffffu, upto, o);
+    const unsigned x = __shfl_up_sync(0xffffffffu, upto, o);
     if (lane >= o) upto += x;
   }
   if (lane == 31) scan[warp] = upto;
   if (threadIdx.x < 2 * W) piece_item[threadIdx.x] = -1;
   __syncthreads();
-  long long total = 0;
+  unsigned total = 0;
 #pragma unroll
   for (int w = 0; w < W; ++w) {
     if (w < warp) upto += scan[w];
     total += scan[w];
   }
-  const long long want = (total + W - 1) / W;
-  const int ctas = want < plan.grid ? (int)want : plan.grid, cta = blockIdx.x;
-  auto start_of = [&](long long worker) { return total * worker / ((long long)ctas * W); };
+  // the first `rest` warps have a chunk more than the others
+  const int cta = blockIdx.x, ctas = min((unsigned)plan.grid, (total + W - 1) / W);
+  const unsigned workers = ctas * W, share = total / workers, rest = total - share * workers;
+  auto start_of = [&](unsigned worker) { return share * worker + min(worker, rest); };
+  auto cta_of = [&](unsigned chunk) {
+    const unsigned more = rest * (share + 1);
+    return (int)((chunk < more ? chunk / (share + 1) : rest + (chunk - more) / share) / W);
+  };
   if (cta >= ctas) {
-    if (threadIdx.x == 0) plan.desc[2 * cta] = -1;
+    if (threadIdx.x < 2) plan.spans[2 * cta + threadIdx.x] = make_int4(-1, 0, 0, 0);
     return;
   }
 #pragma unroll
   for (int w = 0; w < W; ++w) {
-    const long long u = start_of((long long)cta * W + w);
+    const unsigned u = start_of(cta * W + w);
     if (u >= upto - mine && u < upto) {
-      long long at = upto - mine;
+      unsigned at = upto - mine;
       int b = b0;
       for (;; ++b) {
-        const long long n = (long long)attend_chunks(attend_keys(c, b), KT) * plan.per_seq;
+        const unsigned n = (unsigned)attend_chunks(attend_keys(c, b), KT) * plan.per_seq;
         if (u < at + n) break;
         at += n;
       }
@@ -197,10 +198,10 @@ paged_attend_kernel(const AttendArgs a, const Paged c, const AttendPlan plan) {
     }
   }
   __syncthreads();
-  long long u = start_of((long long)cta * W + warp);
-  const long long u_end = start_of((long long)cta * W + warp + 1);
+  unsigned u = start_of(cta * W + warp);
+  const unsigned u_end = start_of(cta * W + warp + 1);
   int b = first_b[warp];
-  long long seq_start = first_chunk[warp];
+  unsigned seq_start = first_chunk[warp];
   int slot = 0;
   const float sl2 = a.scale * 1.4426950408889634f;
   const int group = a.Hq / c.Hkv, rows = c.S * group, tpp = c.page / 16;
@@ -208,10 +209,10 @@ paged_attend_kernel(const AttendArgs a, const Paged c, const AttendPlan plan) {
   while (u < u_end) {
     // ---- an item's run of chunks ------------------------------------------------------------------------------------
     const int keys = attend_keys(c, b), n = attend_chunks(keys, KT);
-    const int idx = (int)((u - seq_start) / n);
-    if (idx >= plan.per_seq) { seq_start += (long long)n * plan.per_seq; ++b; continue; }
-    const int c0 = (int)(u - seq_start - (long long)idx * n);
-    const int c1 = (int)min((long long)n, c0 + (u_end - u));
+    const int idx = (int)((u - seq_start) / (unsigned)n);
+    if (idx >= plan.per_seq) { seq_start += (unsigned)n * plan.per_seq; ++b; continue; }
+    const int c0 = (int)(u - seq_start - (unsigned)idx * n);
+    const int c1 = min(n, c0 + (int)(u_end - u));
     const int kvh = idx / plan.tiles, row0 = idx % plan.tiles * R;
     const int cnt = c.count(b), len = c.length(b);
     if (len > keys && cnt > 0 && c0 == 0 && lane == 0) report_error(c.status, GB_ERR_BAD_INDEX, SITE_POSITION, len - 1);
@@ -567,7 +568,8 @@ paged_attend_kernel(const AttendArgs a, const Paged c, const AttendPlan plan) {
       if (lane == 0) {
         piece_item[piece] = b * plan.per_seq + idx;
         piece_flags[piece] = (c0 == 0 ? 1 : 0) | (c1 == n ? 2 : 0);
-        piece_end[piece] = seq_start + (long long)(idx + 1) * n;
+        piece_start[piece] = seq_start + (unsigned)idx * n;
+        piece_end[piece] = seq_start + (unsigned)(idx + 1) * n;
       }
     }
 #pragma unroll
@@ -589,7 +591,7 @@ paged_attend_kernel(const AttendArgs a, const Paged c, const AttendPlan plan) {
   __syncthreads();
 
   // ---- the warps' pieces, item by item ----------------------------------------------------------------------------------
-  int next_item = -1, next_last = 0;
+  int4 span[2] = {make_int4(-1, 0, 0, 0), make_int4(-1, 0, 0, 0)};
   for (int p = 0; p < 2 * W;) {
     const int item = piece_item[p];
     if (item < 0) { ++p; continue; }
@@ -625,77 +627,65 @@ paged_attend_kernel(const AttendArgs a, const Paged c, const AttendPlan plan) {
         }
       }
     }
-    if (begins && !ends) {
-      next_item = item;
-      next_last = (int)((piece_end[last] * ctas - 1) / total);
+    if (!(begins && ends)) {
+      const int4 x = make_int4(item, cta_of(piece_start[p]), cta_of(piece_end[p] - 1), 0);
+      if (begins) span[1] = x;
+      else span[0] = x;
     }
     p = last + 1;
   }
-  if (threadIdx.x == 0) { plan.desc[2 * cta] = next_item; plan.desc[2 * cta + 1] = next_last; }
+  if (threadIdx.x == 0) { plan.spans[2 * cta] = span[0]; plan.spans[2 * cta + 1] = span[1]; }
 }
 
-// Joins the items that several CTAs have parts of: CTA i takes the one that begins in CTA i of the kernel above and goes on.
-// The maxima of all parts first, so that the sums are independent loads; groups of threads share the parts.
-constexpr int PJ_THREADS = 512;
+// Joins the items that several CTAs have parts of.  CTA i takes its share of the columns of each item that CTA i of the kernel
+// above has a part of, so that many parts of one item are read by as many CTAs; groups of threads share the parts.
+constexpr int PJ_THREADS = 256;
 template <typename T, int D, int R>
 __global__ void __launch_bounds__(PJ_THREADS) paged_join_kernel(const AttendArgs a, const Paged c, const AttendPlan plan) {
-  constexpr int SLOTS = R * D / 4, GROUPS = PJ_THREADS / SLOTS, WARPS = PJ_THREADS / 32;
-  extern __shared__ float weight[];                    // [parts][R]
-  __shared__ float red[WARPS][R];
-  __shared__ float4 sums[GROUPS > 1 ? GROUPS - 1 : 1][SLOTS];
-  const int first = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  static_assert(R * D / 4 <= 2 * PJ_THREADS, "two CTAs have an item's columns among them");
+  __shared__ float4 sum[PJ_THREADS];
+  __shared__ float2 stat[PJ_THREADS];
+  const int cta = blockIdx.x, tid = threadIdx.x;
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int item = plan.desc[2 * first], last = plan.desc[2 * first + 1];
-  if (item < 0) return;
-  const int parts = last - first + 1;
   const float2* stats = reinterpret_cast<const float2*>(plan.parts + (size_t)plan.grid * 2 * R * D);
-  auto part = [&](int k) { return (size_t)(first + k) * 2 + (k == 0 ? 1 : 0); };
-  const int r1 = tid % R;
-  // over the threads of the row r1: lanes R apart, then warps
-  auto over_parts = [&](float v, auto op) {
-#pragma unroll
-    for (int w = R; w < 32; w <<= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, w));
-    __syncthreads();
-    if (lane < R) red[warp][lane] = v;
-    __syncthreads();
-  };
-  float m = -INFINITY, l = 0.f;
-  for (int i = tid; i < parts * R; i += PJ_THREADS) m = fmaxf(m, weight[i] = stats[part(i / R) * R + r1].x);
-  over_parts(m, [](float x, float y) { return fmaxf(x, y); });
-  for (int w = 0; w < WARPS; ++w) m = fmaxf(m, red[w][r1]);
-  for (int i = tid; i < parts * R; i += PJ_THREADS) {
-    const float w = part_weight(weight[i], m);
-    weight[i] = w;
-    l += w * stats[part(i / R) * R + r1].y;
-  }
-  over_parts(l, [](float x, float y) { return x + y; });
-  const int slot = tid % SLOTS, group = tid / SLOTS, r = slot / (D / 4), d = slot % (D / 4) * 4;
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-  for (int k = group; k < parts; k += GROUPS) {
-    const float w = weight[k * R + r];
-    const float4 v = *reinterpret_cast<const float4*>(plan.parts + (part(k) * R + r) * D + d);
-    acc.x += w * v.x; acc.y += w * v.y; acc.z += w * v.z; acc.w += w * v.w;
-  }
-  if constexpr (GROUPS > 1) {
-    if (group > 0) sums[group - 1][slot] = acc;
-    __syncthreads();
-    if (group > 0) return;
-#pragma unroll
-    for (int k = 0; k < GROUPS - 1; ++k) {
-      const float4 v = sums[k][slot];
-      acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
+  for (int which = 0; which < 2; ++which) {
+    const int4 span = plan.spans[2 * cta + which];
+    if (span.x < 0) continue;
+    const int first = span.y, parts = span.z - first + 1;
+    const int b = span.x / plan.per_seq, idx = span.x % plan.per_seq, kvh = idx / plan.tiles, row0 = idx % plan.tiles * R;
+    const int slots = min(R, c.S * (a.Hq / c.Hkv) - row0) * (D / 4), each = (slots + parts - 1) / parts, s0 = (cta - first) * each;
+    const int mine = min(each, slots - s0);
+    if (mine <= 0) continue;
+    const int P = mine <= 1 ? 1 : 1 << (32 - __clz(mine - 1)), G = PJ_THREADS / P;
+    const int slot = tid & (P - 1), group = tid / P, r = (s0 + slot) / (D / 4), d = (s0 + slot) % (D / 4) * 4;
+    float m = -INFINITY, l = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    auto merge = [&](float2 st, float4 v) {
+      const float mn = fmaxf(m, st.x), wa = part_weight(m, mn), wb = part_weight(st.x, mn);
+      acc.x = acc.x * wa + v.x * wb; acc.y = acc.y * wa + v.y * wb; acc.z = acc.z * wa + v.z * wb; acc.w = acc.w * wa + v.w * wb;
+      l = l * wa + st.y * wb;
+      m = mn;
+    };
+    if (slot < mine) {
+#pragma unroll 2
+      for (int k = group; k < parts; k += G) {
+        const size_t part = (size_t)(first + k) * 2 + (k == 0 ? 1 : 0);
+        merge(stats[part * R + r], *reinterpret_cast<const float4*>(plan.parts + (part * R + r) * D + d));
+      }
     }
+    for (int h = G / 2; h >= 1; h >>= 1) {
+      __syncthreads();
+      sum[tid] = acc;
+      stat[tid] = make_float2(m, l);
+      __syncthreads();
+      if (group < h) merge(stat[tid + h * P], sum[tid + h * P]);
+    }
+    if (group == 0 && slot < mine) store_row4<T>(a, c, b, kvh, row0 + r, d, acc, l);
   }
-  const int b = item / plan.per_seq, idx = item % plan.per_seq, kvh = idx / plan.tiles, row = idx % plan.tiles * R + r;
-  if (row >= c.S * (a.Hq / c.Hkv)) return;
-  l = 0.f;
-  for (int w = 0; w < WARPS; ++w) l += red[w][r];
-  store_row4<T>(a, c, b, kvh, row, d, acc, l);
 }
 
 template <typename T, int CDT, int D, int NQ, bool MULTI>
-static int launch_attend(const AttendArgs& a, const Paged& c, float* parts, int* desc, int grid, cudaStream_t st) {
+static int launch_attend(const AttendArgs& a, const Paged& c, float* parts, int4* spans, int grid, cudaStream_t st) {
   using C = PA<T, CDT, D, NQ>;
   static unsigned long long cfg = 0;
   int r;
@@ -705,14 +695,13 @@ static int launch_attend(const AttendArgs& a, const Paged& c, float* parts, int*
   plan.per_seq = plan.tiles * c.Hkv;
   plan.grid = grid;
   plan.parts = parts;
-  plan.desc = desc;
+  plan.spans = spans;
   paged_attend_kernel<T, CDT, D, NQ, MULTI><<<grid, PA_WARPS * 32, C::SMEM, st>>>(a, c, plan);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return (int)e;
   cudaLaunchConfig_t lc{};
   lc.gridDim = dim3(grid);
   lc.blockDim = dim3(PJ_THREADS);
-  lc.dynamicSmemBytes = (size_t)grid * C::R * 4;
   lc.stream = st;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -784,27 +773,19 @@ __global__ void __launch_bounds__(PA_WARPS * 32) paged_attend_any_kernel(const A
   }
 }
 
-#define GB_DISPATCH_CACHE(cdt, C, ...)                                    \
-  do {                                                                    \
-    if ((cdt) == DT_F32) { constexpr int C = DT_F32; __VA_ARGS__; }       \
-    else if ((cdt) == DT_F16) { constexpr int C = DT_F16; __VA_ARGS__; }  \
-    else if ((cdt) == DT_BF16) { constexpr int C = DT_BF16; __VA_ARGS__; } \
-    else if ((cdt) == DT_E4M3) { constexpr int C = DT_E4M3; __VA_ARGS__; } \
-    else return -2;                                                       \
-  } while (0)
-
 }  // namespace gb
 
 using namespace gb;
 
 // Which kernel a call takes, and its CTAs (0: a CTA for every row).  The tensor cores take 16-bit queries of 64 or 128 over caches
-// of their own type or of 8 bits; what remains (32-bit caches and queries, other head sizes) is worked on number by number.
+// of their own type or of 8 bits; what remains (32-bit caches and queries, other head sizes, more than 2^31 chunks of keys) is worked on number by number.
 static int attend_grid(int B, int S, int Hq, int Hkv, int D, int page, int per, int dt, int cdt) {
   if ((D != 64 && D != 128) || dt == DT_F32 || (cdt != dt && cdt != DT_E4M3) || page % 16) return 0;
   const int rows = S * (Hq / Hkv), R = rows <= 8 ? 8 : 16;
   const int kt = 4096 / (D * (cdt == DT_E4M3 ? 1 : 2));
   const long long tiles = (rows + R - 1) / R, keys = (long long)per * page;
-  const long long chunks = B * Hkv * tiles * (keys <= 0 ? 1 : (keys + kt - 1) / kt);
+  const long long chunks = (long long)B * Hkv * tiles * (keys <= 0 ? 1 : (keys + kt - 1) / kt);
+  if (chunks > 0x7fffffff) return 0;       // (counted in 32 bits)
   const long long want = (chunks + PA_WARPS - 1) / PA_WARPS, most = (long long)sm_count() * (R == 8 ? 3 : 2);
   return (int)(want < most ? want : most);
 }
@@ -813,7 +794,7 @@ static int attend_grid(int B, int S, int Hq, int Hkv, int D, int page, int per, 
 extern "C" int gb_paged_attention_workspace(int B, int S, int Hq, int Hkv, int D, int page, int per, int dt, int cdt) {
   if (B <= 0 || S <= 0 || Hq <= 0 || Hkv <= 0) return 0;
   const int R = S * (Hq / Hkv) <= 8 ? 8 : 16;
-  return attend_grid(B, S, Hq, Hkv, D, page, per, dt, cdt) * (2 * R * (D + 2) + 2);
+  return attend_grid(B, S, Hq, Hkv, D, page, per, dt, cdt) * 2 * (R * (D + 2) + 4);
 }
 
 extern "C" int gb_paged_attention(const void* q, void* o, const void* kpool, const void* vpool, const void* kscale,
@@ -829,8 +810,8 @@ extern "C" int gb_paged_attention(const void* q, void* o, const void* kpool, con
   const int grid = attend_grid(B, S, Hq, Hkv, D, page, per, dt, cdt);
   if (grid > 0) {
     const int R = S * (Hq / Hkv) <= 8 ? 8 : 16;
-    int* desc = reinterpret_cast<int*>(workspace + (size_t)grid * 2 * R * (D + 2));
-#define GB_ATTEND_(T, C, D_, NQ_) (S > 1 ? launch_attend<T, C, D_, NQ_, true>(a, c, workspace, desc, grid, st) : launch_attend<T, C, D_, NQ_, false>(a, c, workspace, desc, grid, st))
+    int4* spans = reinterpret_cast<int4*>(workspace + (size_t)grid * 2 * R * (D + 2));
+#define GB_ATTEND_(T, C, D_, NQ_) (S > 1 ? launch_attend<T, C, D_, NQ_, true>(a, c, workspace, spans, grid, st) : launch_attend<T, C, D_, NQ_, false>(a, c, workspace, spans, grid, st))
 #define GB_ATTEND(T, C) (D == 64 ? (R == 8 ? GB_ATTEND_(T, C, 64, 1) : GB_ATTEND_(T, C, 64, 2)) : (R == 8 ? GB_ATTEND_(T, C, 128, 1) : GB_ATTEND_(T, C, 128, 2)))
     if (dt == DT_BF16) return cdt == DT_E4M3 ? GB_ATTEND(__nv_bfloat16, DT_E4M3) : GB_ATTEND(__nv_bfloat16, DT_BF16);
     return cdt == DT_E4M3 ? GB_ATTEND(__half, DT_E4M3) : GB_ATTEND(__half, DT_F16);

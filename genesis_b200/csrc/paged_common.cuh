@@ -70,4 +70,19 @@ __device__ __forceinline__ float2 from_e4m3x2(uint32_t v) {
   return __half22float2(*reinterpret_cast<const __half2*>(&h));
 }
 
+// four e4m3 numbers as two pairs of fp16
+__device__ __forceinline__ void e4m3x4_to_f16(uint32_t v, uint32_t& lo, uint32_t& hi) {
+  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+      : "=r"(lo), "=r"(hi) : "r"(v));
+}
+
+#define GB_DISPATCH_CACHE(cdt, C, ...)                                    \
+  do {                                                                    \
+    if ((cdt) == DT_F32) { constexpr int C = DT_F32; __VA_ARGS__; }       \
+    else if ((cdt) == DT_F16) { constexpr int C = DT_F16; __VA_ARGS__; }  \
+    else if ((cdt) == DT_BF16) { constexpr int C = DT_BF16; __VA_ARGS__; } \
+    else if ((cdt) == DT_E4M3) { constexpr int C = DT_E4M3; __VA_ARGS__; } \
+    else return -2;                                                       \
+  } while (0)
+
 }  // namespace gb

@@ -25,6 +25,118 @@ struct PutArgs {
   int positions, Hq;
 };
 
+// N numbers (4 or 8) in 32 bits into a pool, in its type; e4m3 under the power of two 1 / inv
+template <int CDT, int N>
+__device__ __forceinline__ void store_numbers(void* pool, long long at, const float (&x)[N], float inv) {
+  if constexpr (CDT == DT_F32) {
+#pragma unroll
+    for (int j = 0; j < N; j += 4) *reinterpret_cast<float4*>(reinterpret_cast<float*>(pool) + at + j) = make_float4(x[j], x[j + 1], x[j + 2], x[j + 3]);
+  } else if constexpr (CDT == DT_E4M3) {
+    uint32_t w[N / 4];
+#pragma unroll
+    for (int j = 0; j < N; j += 4) w[j / 4] = to_e4m3x2(x[j] * inv, x[j + 1] * inv) | to_e4m3x2(x[j + 2] * inv, x[j + 3] * inv) << 16;
+    if constexpr (N == 8) *reinterpret_cast<uint2*>(reinterpret_cast<uint8_t*>(pool) + at) = make_uint2(w[0], w[1]);
+    else *reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(pool) + at) = w[0];
+  } else {
+    uint32_t w[N / 2];
+#pragma unroll
+    for (int j = 0; j < N; j += 2) w[j / 2] = pack2c<CDT == DT_BF16>(x[j], x[j + 1]);
+    if constexpr (N == 8) *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(pool) + at) = make_uint4(w[0], w[1], w[2], w[3]);
+    else *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(pool) + at) = make_uint2(w[0], w[1]);
+  }
+}
+
+// A warp takes a token, or some of its heads where tokens are few (`splits` warps a token): position, page and the lane's part
+// of the rotation tables are looked up once and serve all heads.  A row is 2^log groups of lanes x 16 bytes of each half, so the
+// partner of a rotation is in the same registers, and a row's largest magnitude a few shuffles away.  Two rows of a lane are
+// loaded before the first is worked on.
+template <typename T, int CDT, bool ROPE>
+__global__ void __launch_bounds__(256) paged_put_rows_kernel(const PutArgs a, const Paged c, int log, int splits, int heads) {
+  constexpr int V = 16 / sizeof(T), U = 2;
+  const int lane = threadIdx.x & 31, sub = lane >> log, ch = lane & ((1 << log) - 1), half = c.D / 2, step = 32 >> log;
+  const long long w = (long long)blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
+  const int token = (int)(w / splits), Hq = ROPE ? a.Hq : 0, Ht = Hq + 2 * c.Hkv;
+  if (token >= c.B * c.S) return;
+  const int b = token / c.S, s = token - b * c.S;
+  const int h0 = (int)(w - (long long)token * splits) * heads, h1 = min(Ht, h0 + heads);
+  const int n = c.count(b), pos = c.length(b) - n + s;
+  bool live = s < n && pos >= 0;
+  if (ROPE && live && pos >= a.positions) {
+    if (lane == 0) report_error(c.status, GB_ERR_BAD_INDEX, SITE_POSITION, pos);
+    live = false;
+  }
+  if (!ROPE && !live) return;
+  float cs[V], sn[V];
+  long long row0 = -1;                 // of KV head 0
+  if (live) {
+    if (ROPE) {
+#pragma unroll
+      for (int j = 0; j < V; j += 4) {
+        *reinterpret_cast<float4*>(cs + j) = *reinterpret_cast<const float4*>(a.cosb + (long long)pos * c.D + ch * V + j);
+        *reinterpret_cast<float4*>(sn + j) = *reinterpret_cast<const float4*>(a.sinb + (long long)pos * c.D + ch * V + j);
+      }
+    }
+    row0 = c.row(b, pos, 0);
+  }
+  for (int hb = h0; hb < h1; hb += step * U) {
+    Vec16<T> lo[U], hi[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int h = hb + u * step + sub;
+      if (h < h1 && live) {
+        const bool isq = h < Hq, isk = h < Hq + c.Hkv;
+        const Rows& r = isq ? a.q : isk ? a.k : a.v;
+        const T* x = reinterpret_cast<const T*>(r.p) + b * r.sb + s * r.ss + (isq ? h : isk ? h - Hq : h - Hq - c.Hkv) * r.sh + ch * V;
+        lo[u] = ld16(x);
+        hi[u] = ld16(x + half);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int h = hb + u * step + sub;
+      const bool on = h < h1, isq = h < Hq, isk = !isq && h < Hq + c.Hkv;
+      float x[V], y[V];
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        x[j] = y[j] = 0.f;
+        if (on && live) {
+          x[j] = Cvt<T>::to_f(lo[u].v[j]);
+          y[j] = Cvt<T>::to_f(hi[u].v[j]);
+          if (ROPE && (isq || isk)) {
+            const float p = x[j] * cs[j] - y[j] * sn[j];
+            y[j] = y[j] * cs[j] + x[j] * sn[j];
+            x[j] = p;
+          }
+        }
+      }
+      int e = 0;
+      if constexpr (CDT == DT_E4M3) {
+        uint32_t m = 0;
+#pragma unroll
+        for (int j = 0; j < V; ++j) m = max(m, max(finite_bits(x[j]), finite_bits(y[j])));
+        for (int o = 1 << log >> 1; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+        e = e4m3_exponent(m);
+      }
+      if (!on) continue;
+      if (isq) {
+        Vec16<T> p, q;
+#pragma unroll
+        for (int j = 0; j < V; ++j) { p.v[j] = Cvt<T>::from_f(x[j]); q.v[j] = Cvt<T>::from_f(y[j]); }
+        T* o = reinterpret_cast<T*>(a.q_out) + ((long long)token * Hq + h) * c.D + ch * V;
+        st16(o, p);
+        st16(o + half, q);
+      } else if (row0 >= 0) {
+        const long long row = row0 + (long long)(isk ? h - Hq : h - Hq - c.Hkv) * c.page;
+        void* pool = isk ? a.kpool : a.vpool;
+        const float inv = CDT == DT_E4M3 ? exp2i(-e) : 1.f;
+        store_numbers<CDT, V>(pool, row * c.D + ch * V, x, inv);
+        store_numbers<CDT, V>(pool, row * c.D + ch * V + half, y, inv);
+        if (CDT == DT_E4M3 && ch == 0) (isk ? a.kscale : a.vscale)[row] = (uint8_t)(e + 127);
+      }
+    }
+  }
+}
+
 // Any head size and any alignment: a warp takes a row, once for its largest magnitude and once to write it.
 template <typename T, int CDT>
 __global__ void paged_put_any_kernel(const PutArgs a, const Paged c) {
@@ -100,14 +212,78 @@ __global__ void paged_read_any_kernel(const void* kpool, const void* vpool, cons
   }
 }
 
-#define GB_DISPATCH_CACHE(cdt, C, ...)                                    \
-  do {                                                                    \
-    if ((cdt) == DT_F32) { constexpr int C = DT_F32; __VA_ARGS__; }       \
-    else if ((cdt) == DT_F16) { constexpr int C = DT_F16; __VA_ARGS__; }  \
-    else if ((cdt) == DT_BF16) { constexpr int C = DT_BF16; __VA_ARGS__; } \
-    else if ((cdt) == DT_E4M3) { constexpr int C = DT_E4M3; __VA_ARGS__; } \
-    else return -2;                                                       \
-  } while (0)
+// A block takes 16 positions of a sequence, which lie in one page: per KV head its rows are contiguous there.  A thread takes N
+// numbers of K and of V (16 bytes of e4m3, or what 8 numbers are).
+template <typename T, int CDT, int N>
+__global__ void __launch_bounds__(256) paged_read_rows_kernel(const void* kpool, const void* vpool, const uint8_t* kscale,
+                                                              const uint8_t* vscale, void* kout, void* vout, int L, int log,
+                                                              const Paged c) {
+  const int b = blockIdx.y, p0 = blockIdx.x * 16, groups = 1 << log;      // groups of N numbers in a row
+  const int end = min(L, c.length(b));
+  long long row0 = -1;
+  if (p0 < end) row0 = c.row(b, p0, 0);
+  const int there = row0 < 0 ? 0 : end - p0;
+  for (int i = threadIdx.x; i < c.Hkv * 16 << log; i += 256) {
+    const int g = i & (groups - 1), t = i >> log & 15, h = i >> log >> 4;
+    if (p0 + t >= L) continue;
+    const long long row = row0 + (long long)h * c.page + t, at = row * c.D + g * N;
+    const long long out = (((long long)b * L + p0 + t) * c.Hkv + h) * c.D + g * N;
+    float x[2][N];
+#pragma unroll
+    for (int w = 0; w < 2; ++w)
+#pragma unroll
+      for (int j = 0; j < N; ++j) x[w][j] = 0.f;
+    if (t < there) {
+#pragma unroll
+      for (int w = 0; w < 2; ++w) {
+        const void* pool = w ? vpool : kpool;
+        if constexpr (CDT == DT_E4M3) {
+          uint32_t v[N / 4];
+          if constexpr (N == 16) *reinterpret_cast<uint4*>(v) = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(pool) + at);
+          else *reinterpret_cast<uint2*>(v) = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint8_t*>(pool) + at);
+          const float sc = __uint_as_float((uint32_t)(w ? vscale : kscale)[row] << 23);
+#pragma unroll
+          for (int j = 0; j < N / 4; ++j) {
+            uint32_t lo, hi;
+            e4m3x4_to_f16(v[j], lo, hi);
+            const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&lo)), q = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+            x[w][4 * j] = p.x * sc; x[w][4 * j + 1] = p.y * sc; x[w][4 * j + 2] = q.x * sc; x[w][4 * j + 3] = q.y * sc;
+          }
+        } else if constexpr (CDT == DT_F32) {
+#pragma unroll
+          for (int j = 0; j < N; j += 4) {
+            const float4 v = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(pool) + at + j);
+            x[w][j] = v.x; x[w][j + 1] = v.y; x[w][j + 2] = v.z; x[w][j + 3] = v.w;
+          }
+        } else {
+          uint16_t v[8];
+          *reinterpret_cast<uint4*>(v) = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(pool) + at);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) x[w][j] = half_bits_to_float(v[j], CDT);
+        }
+      }
+    }
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      T* o = reinterpret_cast<T*>(w ? vout : kout) + out;
+      constexpr int V = 16 / sizeof(T);
+#pragma unroll
+      for (int j = 0; j < N; j += V) {
+        Vec16<T> v;
+#pragma unroll
+        for (int k = 0; k < V; ++k) v.v[k] = Cvt<T>::from_f(x[w][j + k]);
+        st16(o + j, v);
+      }
+    }
+  }
+}
+
+// exponent of a power of two; -1: none
+static inline int log2_of(int x) {
+  int l = 0;
+  while (x > 1 << l) ++l;
+  return x == 1 << l ? l : -1;
+}
 
 }  // namespace gb
 
@@ -124,7 +300,23 @@ extern "C" int gb_paged_put(const void* q, long long qb, long long qs, long long
   PutArgs a{{q, qb, qs, qh}, {k, kb, ks, kh}, {v, vb, vs, vh}, q_out, kpool, vpool, (uint8_t*)kscale, (uint8_t*)vscale,
             cosb, sinb, positions, Hq};
   Paged c{table, lengths, counts, status, B, S, Hkv, D, page, pages, per};
-  const long long rows = (long long)B * S * (Hq + 2 * Hkv);
+  const int Ht = Hq + 2 * Hkv;
+  const long long tokens = (long long)B * S;
+  const int V = dt == DT_F32 ? 4 : 8, log = D % (2 * V) == 0 ? log2_of(D / (2 * V)) : -1;
+  auto wide = [&](const Rows& r) { return ((uintptr_t)r.p & 15) == 0 && r.sb % V == 0 && r.ss % V == 0 && r.sh % V == 0; };
+  if (log >= 0 && log <= 5 && wide(a.k) && wide(a.v) && (Hq == 0 || wide(a.q)) && (((uintptr_t)cosb | (uintptr_t)sinb) & 15) == 0 && tokens < 1 << 27) {
+    // heads of a token that a warp takes at once; more warps a token until each SM has some
+    const int once = 2 * (32 >> log), most = (Ht + once - 1) / once;
+    int splits = 1;
+    while (splits < most && tokens * splits < 8 * sm_count()) ++splits;
+    const int heads = (((Ht + splits - 1) / splits) + once - 1) / once * once;
+    splits = (Ht + heads - 1) / heads;
+    const unsigned grid = (unsigned)((tokens * splits + 7) / 8);
+    if (cosb != nullptr) GB_DISPATCH_FLOAT(dt, T, GB_DISPATCH_CACHE(cdt, C, paged_put_rows_kernel<T, C, true><<<grid, 256, 0, st>>>(a, c, log, splits, heads)));
+    else GB_DISPATCH_FLOAT(dt, T, GB_DISPATCH_CACHE(cdt, C, paged_put_rows_kernel<T, C, false><<<grid, 256, 0, st>>>(a, c, log, splits, heads)));
+    return (int)cudaGetLastError();
+  }
+  const long long rows = tokens * Ht;
   GB_DISPATCH_FLOAT(dt, T, GB_DISPATCH_CACHE(cdt, C, paged_put_any_kernel<T, C><<<gb_grid(rows, 8), 256, 0, st>>>(a, c)));
   return (int)cudaGetLastError();
 }
@@ -134,6 +326,15 @@ extern "C" int gb_paged_read(const void* kpool, const void* vpool, const void* k
                              int pages, int per, int dt, int cdt, int* status, cudaStream_t st) {
   if (B <= 0 || L <= 0 || Hkv <= 0 || D <= 0) return 0;
   Paged c{table, lengths, nullptr, status, B, 0, Hkv, D, page, pages, per};
+  const int N = cdt == DT_E4M3 && dt != DT_F32 ? 16 : 8, log = D % N == 0 ? log2_of(D / N) : -1;
+  if (log >= 0 && page % 16 == 0 && B <= 65535 && (long long)Hkv * 16 << log < 1 << 30) {
+    const dim3 grid((L + 15) / 16, B);
+    if (N == 16) GB_DISPATCH_FLOAT(dt, T, paged_read_rows_kernel<T, DT_E4M3, 16><<<grid, 256, 0, st>>>(
+        kpool, vpool, (const uint8_t*)kscale, (const uint8_t*)vscale, kout, vout, L, log, c));
+    else GB_DISPATCH_FLOAT(dt, T, GB_DISPATCH_CACHE(cdt, C, paged_read_rows_kernel<T, C, 8><<<grid, 256, 0, st>>>(
+        kpool, vpool, (const uint8_t*)kscale, (const uint8_t*)vscale, kout, vout, L, log, c)));
+    return (int)cudaGetLastError();
+  }
   const long long total = (long long)B * L * Hkv * D;
   GB_DISPATCH_FLOAT(dt, T, GB_DISPATCH_CACHE(cdt, C, paged_read_any_kernel<T, C><<<gb_grid(total, 256), 256, 0, st>>>(
       kpool, vpool, (const uint8_t*)kscale, (const uint8_t*)vscale, kout, vout, L, c)));
