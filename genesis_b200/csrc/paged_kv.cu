@@ -48,17 +48,27 @@ __device__ __forceinline__ void store_numbers(void* pool, long long at, const fl
 
 // A warp takes a token, or some of its heads where tokens are few (`splits` warps a token): position, page and the lane's part
 // of the rotation tables are looked up once and serve all heads.  A row is 2^log groups of lanes x 16 bytes of each half, so the
-// partner of a rotation is in the same registers, and a row's largest magnitude a few shuffles away.  Two rows of a lane are
-// loaded before the first is worked on.
+// partner of a rotation is in the same registers, and a row's largest magnitude a few shuffles away.  The first rows are asked
+// for before the position is known, each next one before the last is worked on.
 template <typename T, int CDT, bool ROPE>
-__global__ void __launch_bounds__(256) paged_put_rows_kernel(const PutArgs a, const Paged c, int log, int splits, int heads) {
-  constexpr int V = 16 / sizeof(T), U = 2;
+__global__ void __launch_bounds__(256, 4) paged_put_rows_kernel(const PutArgs a, const Paged c, int log, int splits, int heads) {
+  constexpr int V = 16 / sizeof(T);
   const int lane = threadIdx.x & 31, sub = lane >> log, ch = lane & ((1 << log) - 1), half = c.D / 2, step = 32 >> log;
-  const long long w = (long long)blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
+  const unsigned w = blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
   const int token = (int)(w / splits), Hq = ROPE ? a.Hq : 0, Ht = Hq + 2 * c.Hkv;
   if (token >= c.B * c.S) return;
   const int b = token / c.S, s = token - b * c.S;
-  const int h0 = (int)(w - (long long)token * splits) * heads, h1 = min(Ht, h0 + heads);
+  const int h0 = (int)(w - token * splits) * heads, h1 = min(Ht, h0 + heads);
+  Vec16<T> lo, hi;
+  auto load = [&](int h) {
+    if (h >= h1) return;
+    const bool isq = h < Hq, isk = h < Hq + c.Hkv;
+    const Rows& r = isq ? a.q : isk ? a.k : a.v;
+    const T* x = reinterpret_cast<const T*>(r.p) + b * r.sb + s * r.ss + (isq ? h : isk ? h - Hq : h - Hq - c.Hkv) * r.sh + ch * V;
+    lo = ld16(x);
+    hi = ld16(x + half);
+  };
+  load(h0 + sub);
   const int n = c.count(b), pos = c.length(b) - n + s;
   bool live = s < n && pos >= 0;
   if (ROPE && live && pos >= a.positions) {
@@ -78,61 +88,47 @@ __global__ void __launch_bounds__(256) paged_put_rows_kernel(const PutArgs a, co
     }
     row0 = c.row(b, pos, 0);
   }
-  for (int hb = h0; hb < h1; hb += step * U) {
-    Vec16<T> lo[U], hi[U];
+  for (int hb = h0; hb < h1; hb += step) {
+    const int h = hb + sub;
+    const bool on = h < h1, isq = h < Hq, isk = !isq && h < Hq + c.Hkv;
+    float x[V], y[V];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int h = hb + u * step + sub;
-      if (h < h1 && live) {
-        const bool isq = h < Hq, isk = h < Hq + c.Hkv;
-        const Rows& r = isq ? a.q : isk ? a.k : a.v;
-        const T* x = reinterpret_cast<const T*>(r.p) + b * r.sb + s * r.ss + (isq ? h : isk ? h - Hq : h - Hq - c.Hkv) * r.sh + ch * V;
-        lo[u] = ld16(x);
-        hi[u] = ld16(x + half);
-      }
+    for (int j = 0; j < V; ++j) {
+      x[j] = on && live ? Cvt<T>::to_f(lo.v[j]) : 0.f;
+      y[j] = on && live ? Cvt<T>::to_f(hi.v[j]) : 0.f;
     }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int h = hb + u * step + sub;
-      const bool on = h < h1, isq = h < Hq, isk = !isq && h < Hq + c.Hkv;
-      float x[V], y[V];
+    load(h + step);
+    if (ROPE && live && (isq || isk)) {
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        x[j] = y[j] = 0.f;
-        if (on && live) {
-          x[j] = Cvt<T>::to_f(lo[u].v[j]);
-          y[j] = Cvt<T>::to_f(hi[u].v[j]);
-          if (ROPE && (isq || isk)) {
-            const float p = x[j] * cs[j] - y[j] * sn[j];
-            y[j] = y[j] * cs[j] + x[j] * sn[j];
-            x[j] = p;
-          }
-        }
+        const float p = x[j] * cs[j] - y[j] * sn[j];
+        y[j] = y[j] * cs[j] + x[j] * sn[j];
+        x[j] = p;
       }
-      int e = 0;
-      if constexpr (CDT == DT_E4M3) {
-        uint32_t m = 0;
+    }
+    int e = 0;
+    if constexpr (CDT == DT_E4M3) {
+      uint32_t m = 0;
 #pragma unroll
-        for (int j = 0; j < V; ++j) m = max(m, max(finite_bits(x[j]), finite_bits(y[j])));
-        for (int o = 1 << log >> 1; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-        e = e4m3_exponent(m);
-      }
-      if (!on) continue;
-      if (isq) {
-        Vec16<T> p, q;
+      for (int j = 0; j < V; ++j) m = max(m, max(finite_bits(x[j]), finite_bits(y[j])));
+      for (int o = 1 << log >> 1; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+      e = e4m3_exponent(m);
+    }
+    if (!on) continue;
+    if (isq) {
+      Vec16<T> p, q;
 #pragma unroll
-        for (int j = 0; j < V; ++j) { p.v[j] = Cvt<T>::from_f(x[j]); q.v[j] = Cvt<T>::from_f(y[j]); }
-        T* o = reinterpret_cast<T*>(a.q_out) + ((long long)token * Hq + h) * c.D + ch * V;
-        st16(o, p);
-        st16(o + half, q);
-      } else if (row0 >= 0) {
-        const long long row = row0 + (long long)(isk ? h - Hq : h - Hq - c.Hkv) * c.page;
-        void* pool = isk ? a.kpool : a.vpool;
-        const float inv = CDT == DT_E4M3 ? exp2i(-e) : 1.f;
-        store_numbers<CDT, V>(pool, row * c.D + ch * V, x, inv);
-        store_numbers<CDT, V>(pool, row * c.D + ch * V + half, y, inv);
-        if (CDT == DT_E4M3 && ch == 0) (isk ? a.kscale : a.vscale)[row] = (uint8_t)(e + 127);
-      }
+      for (int j = 0; j < V; ++j) { p.v[j] = Cvt<T>::from_f(x[j]); q.v[j] = Cvt<T>::from_f(y[j]); }
+      T* o = reinterpret_cast<T*>(a.q_out) + ((long long)token * Hq + h) * c.D + ch * V;
+      st16(o, p);
+      st16(o + half, q);
+    } else if (row0 >= 0) {
+      const long long row = row0 + (long long)(isk ? h - Hq : h - Hq - c.Hkv) * c.page;
+      void* pool = isk ? a.kpool : a.vpool;
+      const float inv = CDT == DT_E4M3 ? exp2i(-e) : 1.f;
+      store_numbers<CDT, V>(pool, row * c.D + ch * V, x, inv);
+      store_numbers<CDT, V>(pool, row * c.D + ch * V + half, y, inv);
+      if (CDT == DT_E4M3 && ch == 0) (isk ? a.kscale : a.vscale)[row] = (uint8_t)(e + 127);
     }
   }
 }
@@ -306,7 +302,7 @@ extern "C" int gb_paged_put(const void* q, long long qb, long long qs, long long
   auto wide = [&](const Rows& r) { return ((uintptr_t)r.p & 15) == 0 && r.sb % V == 0 && r.ss % V == 0 && r.sh % V == 0; };
   if (log >= 0 && log <= 5 && wide(a.k) && wide(a.v) && (Hq == 0 || wide(a.q)) && (((uintptr_t)cosb | (uintptr_t)sinb) & 15) == 0 && tokens < 1 << 27) {
     // heads of a token that a warp takes at once; more warps a token until each SM has some
-    const int once = 2 * (32 >> log), most = (Ht + once - 1) / once;
+    const int once = 32 >> log, most = (Ht + once - 1) / once;
     int splits = 1;
     while (splits < most && tokens * splits < 8 * sm_count()) ++splits;
     const int heads = (((Ht + splits - 1) / splits) + once - 1) / once * once;

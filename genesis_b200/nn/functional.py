@@ -20,6 +20,7 @@ from ..ops import dispatch as K, paged as P
 from ..dtypes import to_torch_dtype as _to_torch_dtype
 from ..amp_state import amp_state, shadow_of, stacked_shadow_of
 from .. import random as _random
+from .. import grad_mode
 from .paged import PagedKVLayer
 
 _pysum, _pymax, _pymin, _pyabs, _pypow = builtins.sum, builtins.max, builtins.min, builtins.abs, builtins.pow
@@ -1964,41 +1965,47 @@ def flash_attention(q, k, v, causal=True, scale=None):
     return FusedAttention.apply(q, k, v, causal, scale)
 
 
-def _paged_args(name, cache, page_table, lengths, counts, B, like):
-    """Checks what the operators on a paged cache have in common; returns the raw (page table, lengths, counts)."""
+def _paged_args(name, cache, page_table, lengths, counts, B, device):
+    """Checks what the operators on a paged cache have in common; returns the raw (page table, lengths, counts).  `device`:
+    index of the tokens' device (-1: the CPU)."""
     if not isinstance(cache, PagedKVLayer):
         raise TypeError(f"{name}: cache must be a layer of a PagedKVCache (cache[i]), got {type(cache).__name__}")
+    at = cache._call[0]
     raw = []
     for what, t, dims in (("page_table", page_table, 2), ("lengths", lengths, 1), ("counts", counts, 1)):
-        if t is None and what == "counts":
+        if t is None and dims == 1 and what == "counts":
             raw.append(None)
             continue
-        if not isinstance(t, Tensor) or t._t.dtype != torch.int32:
+        if not isinstance(t, Tensor) or t._t.dtype is not torch.int32:
             raise TypeError(f"{name}: {what} must be an int32 Tensor")
         t = t._t
-        if t.dim() != dims or (B is not None and t.shape[0] != B):
+        if B is None and t.dim() == dims:
+            B = t.shape[0]
+        if t.dim() != dims or t.shape[0] != B:
             raise ValueError(f"{name}: {what} must be [{'B' if B is None else B}{', pages' if dims == 2 else ''}], got {tuple(t.shape)}")
-        B = t.shape[0]
-        if t.device != cache.k.device:
+        if t.get_device() != at:
             raise ValueError(f"{name}: the cache is on {cache.k.device}, {what} on {t.device}")
         raw.append(t if t.is_contiguous() else K.contiguous(t))
-    if like is not None and like.device != cache.k.device:
-        raise ValueError(f"{name}: the cache is on {cache.k.device}, the tokens on {like.device}")
+    if device != at:
+        raise ValueError(f"{name}: the cache is on {cache.k.device}, the tokens are not")
     return raw
+
+
+_PAGED_INPUTS = (torch.float32, torch.float16, torch.bfloat16)
 
 
 def _paged_tokens(name, what, x, dims, dtype=None):
     """The raw numbers of a call's tokens.  A cache keeps no graph, so an input that wants a gradient is refused."""
-    from .. import grad_mode
-    if not isinstance(x, Tensor) or x._t.dtype not in (torch.float32, torch.float16, torch.bfloat16):
+    if not isinstance(x, Tensor) or x._t.dtype not in _PAGED_INPUTS:
         raise TypeError(f"{name}: {what} must be a Tensor of float32, float16 or bfloat16")
-    if x._t.dim() != dims:
-        raise ValueError(f"{name}: {what} must have {dims} dimensions, got {tuple(x._t.shape)}")
-    if dtype is not None and x._t.dtype != dtype:
-        raise TypeError(f"{name}: {what} is {x._t.dtype}, expected {dtype}")
+    t = x._t
+    if t.dim() != dims:
+        raise ValueError(f"{name}: {what} must have {dims} dimensions, got {tuple(t.shape)}")
+    if dtype is not None and t.dtype is not dtype:
+        raise TypeError(f"{name}: {what} is {t.dtype}, expected {dtype}")
     if x.requires_grad and grad_mode.is_grad_enabled():
         raise RuntimeError(f"{name}: no gradient flows through a cache; call it under no_grad or pass a detached {what}")
-    return x._t
+    return t
 
 
 def paged_kv_write(k, v, cache, page_table, lengths, counts=None):
@@ -2014,11 +2021,11 @@ def paged_kv_write(k, v, cache, page_table, lengths, counts=None):
     Tokens of one call that share a slot are written in no order."""
     name = "paged_kv_write"
     k, v = _paged_tokens(name, "k", k, 4), _paged_tokens(name, "v", v, 4, k._t.dtype if isinstance(k, Tensor) else None)
-    table, lengths, counts = _paged_args(name, cache, page_table, lengths, counts, k.shape[0], k)
-    if k.shape != v.shape or v.device != k.device or tuple(k.shape[2:]) != (cache.num_kv_heads, cache.head_dim):
+    table, lengths, counts = _paged_args(name, cache, page_table, lengths, counts, k.shape[0], k.get_device())
+    if k.shape != v.shape or v.get_device() != k.get_device() or tuple(k.shape[2:]) != (cache.num_kv_heads, cache.head_dim):
         raise ValueError(f"{name}: k and v must be [B, S, {cache.num_kv_heads}, {cache.head_dim}] on one device, got "
                          f"{tuple(k.shape)} and {tuple(v.shape)}")
-    P.put(None, k, v, None, cache, table, lengths, counts)
+    P.write(k, v, cache, table, lengths, counts)
 
 
 def paged_qkv_rope(y, cos, sin, cache, page_table, lengths, num_heads, counts=None):
@@ -2029,31 +2036,29 @@ def paged_qkv_rope(y, cos, sin, cache, page_table, lengths, num_heads, counts=No
     sequence; keys are rounded once, to the cache's type.  Tokens that are none (see `paged_kv_write`) give queries of zeros."""
     name = "paged_qkv_rope"
     y = _paged_tokens(name, "y", y, 3)
-    table, lengths, counts = _paged_args(name, cache, page_table, lengths, counts, y.shape[0], y)
-    Hkv, D = cache.num_kv_heads, cache.head_dim
+    at = y.get_device()
+    table, lengths, counts = _paged_args(name, cache, page_table, lengths, counts, y.shape[0], at)
+    _, Hkv, _, D = cache._call[2]
     if isinstance(num_heads, bool) or not isinstance(num_heads, int) or num_heads < 1 or num_heads % Hkv:
         raise ValueError(f"{name}: num_heads must be a positive multiple of {Hkv} KV heads, got {num_heads!r}")
     if y.shape[2] != (num_heads + 2 * Hkv) * D or D % 2:
         raise ValueError(f"{name}: y must be [B, S, {(num_heads + 2 * Hkv) * D}] with heads of an even size, got {tuple(y.shape)}")
     tables = []
     for what, t in (("cos", cos), ("sin", sin)):
-        if not isinstance(t, Tensor) or t._t.dtype != torch.float32:
+        if not isinstance(t, Tensor) or t._t.dtype is not torch.float32:
             raise TypeError(f"{name}: {what} must be a float32 Tensor")
-        if t._t.dim() != 2 or t._t.shape[1] != D or t._t.device != y.device:
-            raise ValueError(f"{name}: {what} must be [positions, {D}] on {y.device}, got {tuple(t._t.shape)} on {t._t.device}")
-        tables.append(K.contiguous(t._t))
-    if tables[0].shape != tables[1].shape:
-        raise ValueError(f"{name}: cos and sin differ in shape")
-    x = y.unflatten(-1, (num_heads + 2 * Hkv, D))
-    return Tensor._wrap(P.put(x[:, :, :num_heads], x[:, :, num_heads:num_heads + Hkv], x[:, :, num_heads + Hkv:], tables,
-                              cache, table, lengths, counts))
+        t = t._t
+        if t.dim() != 2 or t.shape[1] != D or t.get_device() != at or (tables and t.shape != tables[0].shape):
+            raise ValueError(f"{name}: {what} must be [positions, {D}] on {y.device}, cos and sin alike, got {tuple(t.shape)} on {t.device}")
+        tables.append(t if t.is_contiguous() else K.contiguous(t))
+    return Tensor._wrap(P.rope_write(y, tables, num_heads, cache, table, lengths, counts))
 
 
 def paged_kv_read(cache, page_table, lengths, max_length, dtype=None):
     """(k, v) [B, max_length, Hkv, D] of the sequences' first `max_length` tokens, zeros behind each one's end: what the flash attention takes
     for the next piece of a long prompt.  `dtype`: float32, float16 or bfloat16; the cache's, or bfloat16 for 8 bits (exact)."""
     name = "paged_kv_read"
-    table, lengths, _ = _paged_args(name, cache, page_table, lengths, None, None, None)
+    table, lengths, _ = _paged_args(name, cache, page_table, lengths, None, None, cache._call[0] if isinstance(cache, PagedKVLayer) else -1)
     if isinstance(max_length, bool) or not isinstance(max_length, int) or not 0 <= max_length < 2 ** 31:
         raise ValueError(f"{name}: max_length must be a non-negative 32-bit int, got {max_length!r}")
     held = cache.k.dtype
@@ -2073,9 +2078,9 @@ def paged_attention(q, cache, page_table, lengths, counts=None, scale=None):
     `paged_kv_read` brings back is faster."""
     name = "paged_attention"
     q = _paged_tokens(name, "q", q, 4)
-    table, lengths, counts = _paged_args(name, cache, page_table, lengths, counts, q.shape[0], q)
+    table, lengths, counts = _paged_args(name, cache, page_table, lengths, counts, q.shape[0], q.get_device())
     Hq, D = q.shape[2:]
-    if D != cache.head_dim or Hq < 1 or Hq % cache.num_kv_heads:
+    if D != cache._call[2][3] or Hq < 1 or Hq % cache._call[2][1]:
         raise ValueError(f"{name}: q must be [B, S, heads, {cache.head_dim}] with heads a multiple of {cache.num_kv_heads}, got {tuple(q.shape)}")
     if q.is_cuda and D > 256:
         raise ValueError(f"{name}: heads of up to 256 on CUDA, got {D}")

@@ -32,7 +32,7 @@ def _positive(name, x):
 class PagedKVLayer:
     """The pools of one decoder layer: raw k, v [pages, KV heads, page size, head dim], and in 8 bits k_scale, v_scale
     [pages, KV heads, page size] (uint8; a row stands for its e4m3 numbers times 2^(scale - 127)), else None."""
-    __slots__ = ("k", "v", "k_scale", "v_scale")
+    __slots__ = ("_k", "_v", "_k_scale", "_v_scale", "_call")
 
     def __init__(self, k, v, k_scale=None, v_scale=None):
         if k.dim() != 4 or v.shape != k.shape or k.dtype not in CACHE_TYPES or v.dtype != k.dtype or k.shape[2] % 16 or 0 in k.shape:
@@ -44,7 +44,15 @@ class PagedKVLayer:
         for t in (k, v, *scales):
             if not t.is_contiguous() or t.data_ptr() % 16 or t.device != k.device:
                 raise ValueError("PagedKVLayer: pools and scales must be contiguous, start on 16 bytes and be on one device")
-        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self._k, self._v, self._k_scale, self._v_scale = k, v, k_scale, v_scale
+        # what every call passes on (so the pools cannot be exchanged): device, addresses, sizes, type
+        self._call = (k.get_device(), tuple(t.data_ptr() if t is not None else None for t in (k, v, k_scale, v_scale)),
+                      tuple(k.shape), CACHE_TYPES[k.dtype])
+
+    k = property(lambda self: self._k)
+    v = property(lambda self: self._v)
+    k_scale = property(lambda self: self._k_scale)
+    v_scale = property(lambda self: self._v_scale)
 
     @property
     def num_pages(self):

@@ -148,44 +148,55 @@ def _dense_last(t):
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
-def put(q, k, v, tables, layer, table, lengths, counts):
-    """Keys and values [B, S, Hkv, D] into their pages; with `tables` (cos, sin [positions, D]) keys are rotated first, and the
-    rotated queries [B, S, Hq, D] returned (zeros for tokens that are none)."""
-    if not k.is_cuda:
-        return _put_cpu(q, k, v, tables, layer, table, lengths, counts)
-    B, S, Hkv, D = k.shape
+def write(k, v, layer, table, lengths, counts):
+    """Keys and values [B, S, Hkv, D] into their pages."""
+    index, (kp, vp, ks, vs), (pages, Hkv, page, D), cdt = layer._call
+    if index < 0:
+        _put_cpu(None, k, v, None, layer, table, lengths, counts)
+        return
     k, v, dev = _dense_last(k), _dense_last(v), k.device
-    status = N.status_tensor(dev).data_ptr()
-    pool = layer.k
-    if tables is None:
-        Hq, out, head, rest = 0, None, (None, 0, 0, 0), (None, None, None, 0)
-    else:
-        q, Hq = _dense_last(q), q.shape[2]
-        out = torch.empty(B, S, Hq, D, dtype=k.dtype, device=dev)
-        head = (q.data_ptr(), *q.stride()[:3])
-        rest = (out.data_ptr(), tables[0].data_ptr(), tables[1].data_ptr(), tables[0].shape[0])
+    B, S = k.shape[:2]
     with N._on(dev):
-        N._chk(N.lib().gb_paged_put(*head, k.data_ptr(), *k.stride()[:3], v.data_ptr(), *v.stride()[:3], *rest,
-                                    pool.data_ptr(), layer.v.data_ptr(), N._ptr(layer.k_scale), N._ptr(layer.v_scale),
-                                    table.data_ptr(), lengths.data_ptr(), N._ptr(counts), B, S, Hq, Hkv, D, pool.shape[2],
-                                    pool.shape[0], table.shape[1], N._DT[k.dtype], CACHE_TYPES[pool.dtype], status, N._st()),
+        N._chk(N.lib().gb_paged_put(None, 0, 0, 0, k.data_ptr(), *k.stride()[:3], v.data_ptr(), *v.stride()[:3], None, None, None, 0,
+                                    kp, vp, ks, vs, table.data_ptr(), lengths.data_ptr(), N._ptr(counts), B, S, 0, Hkv, D, page,
+                                    pages, table.shape[1], N._DT[k.dtype], cdt, N.status_tensor(dev).data_ptr(), N._st()),
                "paged_put")
+
+
+def rope_write(y, tables, Hq, layer, table, lengths, counts):
+    """Rotated queries [B, S, Hq, D] from y [B, S, (Hq + 2 Hkv) D], with the rotated keys and the values put into their pages;
+    zeros for tokens that are none.  `tables`: cos, sin [positions, D] float32."""
+    index, (kp, vp, ks, vs), (pages, Hkv, page, D), cdt = layer._call
+    if index < 0:
+        x = y.unflatten(-1, (Hq + 2 * Hkv, D))
+        return _put_cpu(x[:, :, :Hq], x[:, :, Hq:Hq + Hkv], x[:, :, Hq + Hkv:], tables, layer, table, lengths, counts)
+    y = _dense_last(y)
+    B, S, _ = y.shape
+    sb, ss, _ = y.stride()
+    dev, at, head = y.device, y.data_ptr(), D * y.element_size()
+    cos, sin = tables
+    out = torch.empty(B, S, Hq, D, dtype=y.dtype, device=dev)
+    with N._on(dev):
+        N._chk(N.lib().gb_paged_put(at, sb, ss, D, at + Hq * head, sb, ss, D, at + (Hq + Hkv) * head, sb, ss, D, out.data_ptr(),
+                                    cos.data_ptr(), sin.data_ptr(), cos.shape[0], kp, vp, ks, vs, table.data_ptr(),
+                                    lengths.data_ptr(), N._ptr(counts), B, S, Hq, Hkv, D, page, pages, table.shape[1],
+                                    N._DT[y.dtype], cdt, N.status_tensor(dev).data_ptr(), N._st()), "paged_put")
     return out
 
 
 def read(layer, table, lengths, L, dtype):
     """(k, v) [B, L, Hkv, D] of `dtype`, zeros behind each sequence's end."""
-    if not layer.k.is_cuda:
+    index, (kp, vp, ks, vs), (pages, Hkv, page, D), cdt = layer._call
+    if index < 0:
         return _read_cpu(layer, table, lengths, L, dtype)
-    pages, Hkv, page, D = layer.k.shape
-    B, dev = table.shape[0], layer.k.device
-    out = [torch.empty(B, L, Hkv, D, dtype=dtype, device=dev) for _ in range(2)]
+    B, dev = table.shape[0], table.device
+    k = torch.empty(B, L, Hkv, D, dtype=dtype, device=dev)
+    v = torch.empty_like(k)
     with N._on(dev):
-        N._chk(N.lib().gb_paged_read(layer.k.data_ptr(), layer.v.data_ptr(), N._ptr(layer.k_scale), N._ptr(layer.v_scale),
-                                     out[0].data_ptr(), out[1].data_ptr(), table.data_ptr(), lengths.data_ptr(), B, L, Hkv, D,
-                                     page, pages, table.shape[1], N._DT[dtype], CACHE_TYPES[layer.k.dtype],
-                                     N.status_tensor(dev).data_ptr(), N._st()), "paged_read")
-    return out
+        N._chk(N.lib().gb_paged_read(kp, vp, ks, vs, k.data_ptr(), v.data_ptr(), table.data_ptr(), lengths.data_ptr(), B, L, Hkv,
+                                     D, page, pages, table.shape[1], N._DT[dtype], cdt, N.status_tensor(dev).data_ptr(),
+                                     N._st()), "paged_read")
+    return k, v
 
 
 @functools.lru_cache(maxsize=256)
@@ -195,20 +206,18 @@ def _workspace(device_index, *sizes):
 
 def attention(q, layer, table, lengths, counts, scale):
     """softmax(scale q k^T) v of the tokens q [B, S, Hq, D] over the pages of their sequences -> [B, S, Hq, D]."""
-    if not q.is_cuda:
+    index, (kp, vp, ks, vs), (pages, Hkv, page, D), cdt = layer._call
+    if index < 0:
         return _attention_cpu(q, layer, table, lengths, counts, scale)
-    B, S, Hq, D = q.shape
-    k = layer.k
-    pages, Hkv, page, _ = k.shape
-    dev, per, dt, cdt = q.device, table.shape[1], N._DT[q.dtype], CACHE_TYPES[k.dtype]
+    B, S, Hq, _ = q.shape
+    dev, per, dt = q.device, table.shape[1], N._DT[q.dtype]
     if not q.is_contiguous() or q.data_ptr() % 16:
         q = q.clone(memory_format=torch.contiguous_format)
     out = torch.empty_like(q)
     with N._on(dev):
-        words = _workspace(dev.index, B, S, Hq, Hkv, D, page, per, dt, cdt)
+        words = _workspace(index, B, S, Hq, Hkv, D, page, per, dt, cdt)
         work = torch.empty(words, dtype=torch.float32, device=dev) if words else None
-        N._chk(N.lib().gb_paged_attention(q.data_ptr(), out.data_ptr(), k.data_ptr(), layer.v.data_ptr(), N._ptr(layer.k_scale),
-                                          N._ptr(layer.v_scale), table.data_ptr(), lengths.data_ptr(), N._ptr(counts), B, S, Hq,
-                                          Hkv, D, page, pages, per, scale, dt, cdt, N._ptr(work),
+        N._chk(N.lib().gb_paged_attention(q.data_ptr(), out.data_ptr(), kp, vp, ks, vs, table.data_ptr(), lengths.data_ptr(),
+                                          N._ptr(counts), B, S, Hq, Hkv, D, page, pages, per, scale, dt, cdt, N._ptr(work),
                                           N.status_tensor(dev).data_ptr(), N._st()), "paged_attention")
     return out
