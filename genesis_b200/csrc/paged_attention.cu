@@ -50,26 +50,33 @@ struct AttendPlan {
 template <typename T, int CDT, int D_, int NQ_>
 struct PA {
   static constexpr int D = D_, NQ = NQ_, R = 8 * NQ;
-  static constexpr bool E8 = CDT == DT_E4M3, BF = CDT == DT_BF16;
-  static constexpr bool OBF = sizeof(T) == 2 && !std::is_same<T, __half>::value;
-  static constexpr bool SPLIT = !(E8 && OBF);
-  static constexpr int ES = E8 ? 1 : 2;
-  static constexpr int KT = 4096 / (D * ES);            // keys of a chunk: 4 KB of K, 4 KB of V
+  static constexpr bool E8 = CDT == DT_E4M3, BF = CDT == DT_BF16, F32 = CDT == DT_F32;
+  static constexpr bool OBF = std::is_same<T, __nv_bfloat16>::value;
+  static constexpr bool SPLIT = !(E8 && OBF);           // P in two numbers
+  static constexpr int ES = E8 ? 1 : F32 ? 4 : 2;
+  static constexpr int KT = 4096 / (D * ES) < 16 ? 16 : 4096 / (D * ES);      // keys of a chunk: 4 KB of K and of V, at least a tile
   static constexpr int NS = KT / 16;                    // tiles of 16 keys
   static constexpr int KL = D * ES / 64;                // 16-byte loads of a lane's share of a key's row
   static constexpr int VW = D * ES / 32;                // words of a lane's share of a value's row
   static constexpr int MT = D / 16;                     // 16-row tiles of O^T
+  static constexpr int QS = F32 ? D / 8 : D / 16;       // steps of the contraction over d
+  static constexpr int GP = F32 ? 2 : 1;                // ... and of a tile's over its keys
   static constexpr int PIECE = R * D;
   static constexpr int SMEM = 2 * PA_WARPS * PIECE * 4;
+  static constexpr int CTAS = NQ == 1 && !(F32 && D == 128) ? 3 : 2;          // on an SM
   // first of the two columns d that a lane has of tile mt
   static __device__ __forceinline__ int column(int g, int mt) {
     if (E8) return g * (D / 8) + mt * 2;
+    if (F32) return (g + 8 * (mt >> 1)) * 4 + (mt & 1) * 2;
     return (g + 8 * (mt >> 2)) * 8 + (mt & 3) * 2;
   }
+  // the k-th of the four keys of a tile whose values a lane loads, less its first
+  static __device__ __forceinline__ int first_key(int t) { return F32 ? t : 2 * t; }
+  static __device__ __forceinline__ constexpr int key_step(int k) { return F32 ? 4 * k : (k & 1) + (k >> 1) * 8; }
 };
 
 // keys that are not there are read from here, so that loads need no predicates (and no moves of zeros)
-__device__ const uint4 PA_ZEROS[16] = {};
+__device__ const uint4 PA_ZEROS[32] = {};         // (a row of 128 numbers of 32 bits)
 
 __device__ __forceinline__ uint4 ld_stream16(const void* p) {
   uint4 v;
@@ -80,12 +87,6 @@ __device__ __forceinline__ uint2 ld_stream8(const void* p) {
   uint2 v;
   asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
   return v;
-}
-// a bit for each 16-bit half of v that is an infinity or NaN
-template <bool BF>
-__device__ __forceinline__ uint32_t not_finite2(uint32_t v) {
-  constexpr uint32_t E = BF ? 0x7f80u : 0x7c00u;
-  return ((v & E) == E ? 1u : 0u) | ((v >> 16 & E) == E ? 2u : 0u);
 }
 __device__ __forceinline__ uint32_t transposed_8x8(uint32_t v) {
   uint32_t r;
@@ -105,6 +106,72 @@ __device__ __forceinline__ void mma_k16(float (&c)[4], const uint32_t a0, const 
   else
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
+  asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+}
+// 32 bits as two numbers of 11 bits: what is cut off, rounded (2^-22 at most is lost); nothing of an infinity or NaN
+template <int N>
+__device__ __forceinline__ void split_tf32(const uint32_t (&x)[N], uint32_t (&hi)[N], uint32_t (&lo)[N]) {
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    hi[k] = x[k] & 0xffffe000u;
+    lo[k] = (x[k] & 0x7f800000u) == 0x7f800000u ? 0u : (__float_as_uint(__uint_as_float(x[k]) - __uint_as_float(hi[k])) + 0x1000u) & 0xffffe000u;
+  }
+}
+// c += a b in 32 bits: the three larger of four products
+__device__ __forceinline__ void mma_f32(float (&c)[4], const uint32_t (&a)[4], const uint32_t (&bh)[2], const uint32_t (&bl)[2]) {
+  uint32_t ah[4], al[4];
+  split_tf32(a, ah, al);
+  mma_tf32(c, al, bh);
+  mma_tf32(c, ah, bl);
+  mma_tf32(c, ah, bh);
+}
+// O^T += V^T P^T of a step: P as high and low part
+template <class C>
+__device__ __forceinline__ void mma_pv(float (&acc)[4], const uint32_t (&v)[4], const uint32_t (&hi)[2], const uint32_t (&lo)[2]) {
+  if constexpr (C::F32) {
+    mma_f32(acc, v, hi, lo);
+  } else {
+    mma_k16<C::BF>(acc, v[0], v[1], v[2], v[3], hi[0], hi[1]);
+    if constexpr (C::SPLIT) mma_k16<C::BF>(acc, v[0], v[1], v[2], v[3], lo[0], lo[1]);
+  }
+}
+// The same where rows end at different keys: a key that one row sees and another does not is multiplied by a probability of 0
+// there, which an infinity or NaN among its values would turn into NaN.  If there are any, the product is made again without
+// them for the rows that do not see them; how many of them a row sees is a product too, of ones.
+template <class C, class Sees>
+__device__ __forceinline__ void mma_pv_ragged(float (&acc)[4], const uint32_t (&v)[4], const uint32_t (&hi)[2], const uint32_t (&lo)[2],
+                                              Sees sees) {
+  uint32_t fine[4], mark[4], bad = 0;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    if constexpr (C::F32) {
+      const bool f = (v[k] & 0x7f800000u) == 0x7f800000u;
+      fine[k] = f ? 0u : v[k];
+      mark[k] = f ? 0x3f800000u : 0u;
+    } else {
+      constexpr uint32_t E = C::BF ? 0x7f80u : 0x7c00u, ONE = C::BF ? 0x3f80u : 0x3c00u;
+      const bool f = (v[k] & E) == E, g = (v[k] >> 16 & E) == E;
+      fine[k] = v[k] & ((f ? 0u : 0xffffu) | (g ? 0u : 0xffff0000u));
+      mark[k] = (f ? ONE : 0u) | (g ? ONE << 16 : 0u);
+    }
+    bad |= mark[k];
+  }
+  if (!__any_sync(0xffffffffu, bad != 0)) {
+    mma_pv<C>(acc, v, hi, lo);
+    return;
+  }
+  float seen[4] = {0.f, 0.f, 0.f, 0.f}, kept[4] = {acc[0], acc[1], acc[2], acc[3]};
+  uint32_t ones[2];
+  sees(ones);
+  if constexpr (C::F32) mma_tf32(seen, mark, ones);
+  else mma_k16<C::BF>(seen, mark[0], mark[1], mark[2], mark[3], ones[0], ones[1]);
+  mma_pv<C>(kept, fine, hi, lo);
+  mma_pv<C>(acc, v, hi, lo);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) acc[e] = seen[e] == 0.f ? kept[e] : acc[e];
 }
 __device__ __forceinline__ float pow2_of(float x) {
   float y;
@@ -129,19 +196,20 @@ __device__ __forceinline__ void store_row4(const AttendArgs& a, const Paged& c, 
   const int group = a.Hq / c.Hkv;
   const float inv = l == 0.f ? 0.f : 1.f / l;
   T* p = reinterpret_cast<T*>(a.o) + (((long long)b * c.S + r / group) * a.Hq + kvh * group + r % group) * c.D + d;
-  uint2 w;
-  constexpr bool BF = !std::is_same<T, __half>::value;
-  w.x = pack2c<BF>(o.x * inv, o.y * inv);
-  w.y = pack2c<BF>(o.z * inv, o.w * inv);
-  *reinterpret_cast<uint2*>(p) = w;
+  if constexpr (std::is_same<T, float>::value) {
+    *reinterpret_cast<float4*>(p) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+  } else {
+    constexpr bool BF = std::is_same<T, __nv_bfloat16>::value;
+    *reinterpret_cast<uint2*>(p) = make_uint2(pack2c<BF>(o.x * inv, o.y * inv), pack2c<BF>(o.z * inv, o.w * inv));
+  }
 }
 
 // MULTI: several tokens a sequence, whose rows end at different keys
 template <typename T, int CDT, int D, int NQ, bool MULTI>
-__global__ void __launch_bounds__(PA_WARPS * 32, NQ == 1 ? 3 : 2)
+__global__ void __launch_bounds__(PA_WARPS * 32, PA<T, CDT, D, NQ>::CTAS)
 paged_attend_kernel(const AttendArgs a, const Paged c, const AttendPlan plan) {
   using C = PA<T, CDT, D, NQ>;
-  constexpr int R = C::R, KT = C::KT, NS = C::NS, KL = C::KL, VW = C::VW, MT = C::MT, W = PA_WARPS;
+  constexpr int R = C::R, KT = C::KT, NS = C::NS, KL = C::KL, VW = C::VW, MT = C::MT, QS = C::QS, GP = C::GP, W = PA_WARPS;
   extern __shared__ __align__(16) float pieces[];                  // [2 W][R][D]
   __shared__ float piece_m[2 * W][R], piece_l[2 * W][R];
   __shared__ int piece_item[2 * W], piece_flags[2 * W];
@@ -233,15 +301,15 @@ paged_attend_kernel(const AttendArgs a, const Paged c, const AttendPlan plan) {
     };
     ask();
     // queries as the B operand: row g, the d that this lane has of a key's row
-    uint32_t qf[NQ][MT][2];
+    uint32_t qf[NQ][QS][2];
 #pragma unroll
     for (int q = 0; q < NQ; ++q) {
       const int r = row0 + q * 8 + g;
       const T* p = reinterpret_cast<const T*>(a.q) + (((long long)b * c.S + (r < rows ? r / group : 0)) * a.Hq + kvh * group + (r < rows ? r % group : 0)) * D;
-      constexpr int H = C::E8 ? 2 : 1;           // 16-byte loads that go with one of a key's row
+      constexpr int H = C::E8 ? 2 : 1, E = 16 / sizeof(T);     // 16-byte loads that go with one of a key's row, numbers of each
 #pragma unroll
       for (int i = 0; i < KL * H; ++i) {
-        const uint4 v = ld_stream16(r < rows ? reinterpret_cast<const char*>(p + ((i / H) * 4 + t) * 8 * H + (i % H) * 8) : zeros);
+        const uint4 v = ld_stream16(r < rows ? reinterpret_cast<const char*>(p + ((i / H) * 4 + t) * E * H + (i % H) * E) : zeros);
         qf[q][2 * i][0] = v.x; qf[q][2 * i][1] = v.y;
         qf[q][2 * i + 1][0] = v.z; qf[q][2 * i + 1][1] = v.w;
       }
@@ -300,7 +368,7 @@ paged_attend_kernel(const AttendArgs a, const Paged c, const AttendPlan plan) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) { m[q][e] = -INFINITY; off[q][e] = 0.f; l[q][e] = 0.f; }
     }
-    constexpr float LIFT = !C::E8 && !C::BF ? 7.f : 0.f;      // fp16 P without a scale of its own
+    constexpr float LIFT = !C::E8 && !C::BF && !C::F32 ? 7.f : 0.f;      // fp16 P without a scale of its own
     int vtop = -1000;                  // the power of two of V that the accumulators are relative to
     const int full = MULTI ? min(keys, max(0, len - cnt + 1)) : keys;      // keys that every token sees
 
@@ -324,7 +392,18 @@ paged_attend_kernel(const AttendArgs a, const Paged c, const AttendPlan plan) {
           for (int j = 0; j < KL; ++j) {
             const uint32_t lo[4] = {kr[i][0][j].x, kr[i][0][j].y, kr[i][0][j].z, kr[i][0][j].w};
             const uint32_t hi[4] = {kr[i][1][j].x, kr[i][1][j].y, kr[i][1][j].z, kr[i][1][j].w};
-            if constexpr (!C::E8) {
+            if constexpr (C::F32) {
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const uint32_t x[4] = {lo[2 * h], hi[2 * h], lo[2 * h + 1], hi[2 * h + 1]};
+#pragma unroll
+                for (int q = 0; q < NQ; ++q) {
+                  uint32_t bh[2], bl[2];
+                  split_tf32(qf[q][2 * j + h], bh, bl);
+                  mma_f32(s[i][q], x, bh, bl);
+                }
+              }
+            } else if constexpr (!C::E8) {
 #pragma unroll
               for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -429,7 +508,15 @@ paged_attend_kernel(const AttendArgs a, const Paged c, const AttendPlan plan) {
               }
             }
         }
-        uint32_t ph[NS][NQ][2], pl[NS][NQ][2];
+        uint32_t ph[NS][NQ][GP][2], pl[NS][NQ][GP][2];
+        // 32-bit numbers of keys g (lane's row) and queries 2t, 2t + 1 as the operand of 8 keys: keys t and t + 4 of query g
+        auto turned = [&](float x, float y, uint32_t (&out)[2]) {
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const float p = __shfl_sync(0xffffffffu, x, (t + 4 * k) * 4 + (g >> 1)), q = __shfl_sync(0xffffffffu, y, (t + 4 * k) * 4 + (g >> 1));
+            out[k] = __float_as_uint(g & 1 ? q : p);
+          }
+        };
 #pragma unroll
         for (int i = 0; i < NS; ++i)
 #pragma unroll
@@ -444,88 +531,76 @@ paged_attend_kernel(const AttendArgs a, const Paged c, const AttendPlan plan) {
                 l[q][e] += p[e];
                 if constexpr (C::E8) p[e] *= vs;
               }
-              const uint32_t w = pack2c<C::BF>(p[0], p[1]);
-              ph[i][q][h] = transposed_8x8(w);
-              if constexpr (C::SPLIT) {
-                const float2 r = unpack2<C::BF>(w);
-                pl[i][q][h] = transposed_8x8(pack2c<C::BF>(p[0] - r.x, p[1] - r.y));
+              if constexpr (C::F32) {
+                uint32_t x[2];
+                turned(p[0], p[1], x);
+                split_tf32(x, ph[i][q][h % GP], pl[i][q][h % GP]);
+              } else {
+                const uint32_t w = pack2c<C::BF>(p[0], p[1]);
+                ph[i][q][0][h] = transposed_8x8(w);
+                if constexpr (C::SPLIT) {
+                  const float2 r = unpack2<C::BF>(w);
+                  pl[i][q][0][h] = transposed_8x8(pack2c<C::BF>(p[0] - r.x, p[1] - r.y));
+                }
               }
             }
           }
         // ---- O^T += V^T P^T -----------------------------------------------------------------------------------------
+        auto product = [&](int i, int mt, int gp, const uint32_t (&v)[4]) {
+#pragma unroll
+          for (int q = 0; q < NQ; ++q) {
+            if constexpr (MULTI) {
+              if (tail) {
+                mma_pv_ragged<C>(o[q][mt], v, ph[i][q][gp], pl[i][q][gp], [&](uint32_t (&ones)[2]) {
+                  const int key = (ch * NS + i) * 16 + g + 8 * gp;
+                  if constexpr (C::F32) {
+                    turned(key < end[q][0] ? 1.f : 0.f, key < end[q][1] ? 1.f : 0.f, ones);
+                  } else {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+                      ones[h] = transposed_8x8((key + 8 * h < end[q][0] ? C::BF ? 0x3f80u : 0x3c00u : 0u) | (key + 8 * h < end[q][1] ? C::BF ? 0x3f800000u : 0x3c000000u : 0u));
+                  }
+                });
+                continue;
+              }
+            }
+            mma_pv<C>(o[q][mt], v, ph[i][q][gp], pl[i][q][gp]);
+          }
+        };
 #pragma unroll
         for (int i = 0; i < NS; ++i)
 #pragma unroll
           for (int j = 0; j < VW; ++j) {
-            constexpr int H = C::E8 ? 2 : 1;         // tiles of a word
-            uint32_t v[H][4];
-            if constexpr (!C::E8) {
-              v[0][0] = __byte_perm(vr[i][0][j], vr[i][1][j], 0x5410);
-              v[0][1] = __byte_perm(vr[i][0][j], vr[i][1][j], 0x7632);
-              v[0][2] = __byte_perm(vr[i][2][j], vr[i][3][j], 0x5410);
-              v[0][3] = __byte_perm(vr[i][2][j], vr[i][3][j], 0x7632);
+            if constexpr (C::F32) {
+              if (j & 1) continue;
+#pragma unroll
+              for (int gp = 0; gp < 2; ++gp) {
+                const uint32_t v[4] = {vr[i][2 * gp][j], vr[i][2 * gp][j + 1], vr[i][2 * gp + 1][j], vr[i][2 * gp + 1][j + 1]};
+                product(i, j / 2, gp, v);
+              }
+            } else if constexpr (!C::E8) {
+              const uint32_t v[4] = {__byte_perm(vr[i][0][j], vr[i][1][j], 0x5410), __byte_perm(vr[i][0][j], vr[i][1][j], 0x7632),
+                                     __byte_perm(vr[i][2][j], vr[i][3][j], 0x5410), __byte_perm(vr[i][2][j], vr[i][3][j], 0x7632)};
+              product(i, j, 0, v);
             } else {
 #pragma unroll
-              for (int h = 0; h < H; ++h) {
-                e4m3x4_to_f16(__byte_perm(vr[i][0][j], vr[i][1][j], h ? 0x7362 : 0x5140), v[h][0], v[h][1]);
-                e4m3x4_to_f16(__byte_perm(vr[i][2][j], vr[i][3][j], h ? 0x7362 : 0x5140), v[h][2], v[h][3]);
+              for (int h = 0; h < 2; ++h) {
+                uint32_t v[4];
+                e4m3x4_to_f16(__byte_perm(vr[i][0][j], vr[i][1][j], h ? 0x7362 : 0x5140), v[0], v[1]);
+                e4m3x4_to_f16(__byte_perm(vr[i][2][j], vr[i][3][j], h ? 0x7362 : 0x5140), v[2], v[3]);
+                product(i, 2 * j + h, 0, v);
               }
             }
-#pragma unroll
-            for (int h = 0; h < H; ++h)
-#pragma unroll
-              for (int q = 0; q < NQ; ++q) {
-                float (&acc)[4] = o[q][j * H + h];
-                const uint32_t (&x)[4] = v[h];
-                if constexpr (MULTI) {
-                  // a key that one row sees and another does not is multiplied by a probability of 0 there, which an infinity
-                  // or NaN among its values would turn into NaN
-                  uint32_t bad = 0;
-                  if (tail) {
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) bad |= not_finite2<C::BF>(x[k]);
-                    bad = __any_sync(0xffffffffu, bad != 0);
-                  }
-                  if (bad) {
-                    // the same without those values for the rows that do not see them; how many of them a row sees is a product too
-                    uint32_t fine[4], mark[4], sees[2];
-                    constexpr uint32_t ONE = C::BF ? 0x3f80u : 0x3c00u;
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                      const uint32_t f = not_finite2<C::BF>(x[k]);
-                      fine[k] = x[k] & ((f & 1 ? 0u : 0xffffu) | (f & 2 ? 0u : 0xffff0000u));
-                      mark[k] = (f & 1 ? ONE : 0u) | (f & 2 ? ONE << 16 : 0u);
-                    }
-#pragma unroll
-                    for (int k = 0; k < 2; ++k) {
-                      const int key = (ch * NS + i) * 16 + g + 8 * k;
-                      sees[k] = transposed_8x8((key < end[q][0] ? ONE : 0u) | (key < end[q][1] ? ONE << 16 : 0u));
-                    }
-                    float seen[4] = {0.f, 0.f, 0.f, 0.f}, kept[4] = {acc[0], acc[1], acc[2], acc[3]};
-                    mma_k16<C::BF>(seen, mark[0], mark[1], mark[2], mark[3], sees[0], sees[1]);
-                    mma_k16<C::BF>(kept, fine[0], fine[1], fine[2], fine[3], ph[i][q][0], ph[i][q][1]);
-                    if constexpr (C::SPLIT) mma_k16<C::BF>(kept, fine[0], fine[1], fine[2], fine[3], pl[i][q][0], pl[i][q][1]);
-                    mma_k16<C::BF>(acc, x[0], x[1], x[2], x[3], ph[i][q][0], ph[i][q][1]);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) acc[e] = seen[e] == 0.f ? kept[e] : acc[e];
-                    continue;
-                  }
-                }
-                mma_k16<C::BF>(acc, x[0], x[1], x[2], x[3], ph[i][q][0], ph[i][q][1]);
-                if constexpr (C::SPLIT) mma_k16<C::BF>(acc, x[0], x[1], x[2], x[3], pl[i][q][0], pl[i][q][1]);
-              }
           }
       }
       if (more) {
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
           const int left = row[i] < 0 ? 0 : keys - ((ch + 1) * NS + i) * 16;
-          const char* p = reinterpret_cast<const char*>(a.vpool) + (row[i] + 2 * t) * (D * C::ES) + g * (VW == 2 ? 8 : 16);
+          const char* p = reinterpret_cast<const char*>(a.vpool) + (row[i] + C::first_key(t)) * (D * C::ES) + g * (VW == 2 ? 8 : 16);
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            constexpr int STEP = D * C::ES;
-            const int key = (k & 1) + (k >> 1) * 8;
-            const char* pv = 2 * t + key < left ? p + key * STEP : zeros;
+            const char* pv = C::first_key(t) + C::key_step(k) < left ? p + C::key_step(k) * (D * C::ES) : zeros;
             if constexpr (VW == 2) {
               const uint2 v = ld_stream8(pv);
               vr[i][k][0] = v.x; vr[i][k][1] = v.y;
@@ -777,23 +852,27 @@ __global__ void __launch_bounds__(PA_WARPS * 32) paged_attend_any_kernel(const A
 
 using namespace gb;
 
-// Which kernel a call takes, and its CTAs (0: a CTA for every row).  The tensor cores take 16-bit queries of 64 or 128 over caches
-// of their own type or of 8 bits; what remains (32-bit caches and queries, other head sizes, more than 2^31 chunks of keys) is worked on number by number.
+// Query rows of an item: one operand of 8 columns, or two where there are more rows and registers for them.
+static int attend_rows(int rows, int D, int cdt) { return rows <= 8 || (cdt == DT_F32 && D == 128) ? 8 : 16; }
+
+// Which kernel a call takes, and its CTAs (0: a CTA for every row).  The tensor cores take heads of 64 or 128 over caches of the
+// queries' type, or of 8 bits below 16-bit queries; what remains (other head sizes, types that differ, more than 2^31 chunks of
+// keys) is worked on number by number.
 static int attend_grid(int B, int S, int Hq, int Hkv, int D, int page, int per, int dt, int cdt) {
-  if ((D != 64 && D != 128) || dt == DT_F32 || (cdt != dt && cdt != DT_E4M3) || page % 16) return 0;
-  const int rows = S * (Hq / Hkv), R = rows <= 8 ? 8 : 16;
-  const int kt = 4096 / (D * (cdt == DT_E4M3 ? 1 : 2));
+  if ((D != 64 && D != 128) || (cdt != dt && !(cdt == DT_E4M3 && dt != DT_F32)) || page % 16) return 0;
+  const int rows = S * (Hq / Hkv), R = attend_rows(rows, D, cdt);
+  const int es = cdt == DT_E4M3 ? 1 : cdt == DT_F32 ? 4 : 2, kt = 4096 / (D * es) < 16 ? 16 : 4096 / (D * es);
   const long long tiles = (rows + R - 1) / R, keys = (long long)per * page;
   const long long chunks = (long long)B * Hkv * tiles * (keys <= 0 ? 1 : (keys + kt - 1) / kt);
   if (chunks > 0x7fffffff) return 0;       // (counted in 32 bits)
-  const long long want = (chunks + PA_WARPS - 1) / PA_WARPS, most = (long long)sm_count() * (R == 8 ? 3 : 2);
+  const long long want = (chunks + PA_WARPS - 1) / PA_WARPS, most = (long long)sm_count() * (R == 8 && !(cdt == DT_F32 && D == 128) ? 3 : 2);
   return (int)(want < most ? want : most);
 }
 
 // 32-bit words of workspace that a call needs
 extern "C" int gb_paged_attention_workspace(int B, int S, int Hq, int Hkv, int D, int page, int per, int dt, int cdt) {
   if (B <= 0 || S <= 0 || Hq <= 0 || Hkv <= 0) return 0;
-  const int R = S * (Hq / Hkv) <= 8 ? 8 : 16;
+  const int R = attend_rows(S * (Hq / Hkv), D, cdt);
   return attend_grid(B, S, Hq, Hkv, D, page, per, dt, cdt) * 2 * (R * (D + 2) + 4);
 }
 
@@ -809,12 +888,14 @@ extern "C" int gb_paged_attention(const void* q, void* o, const void* kpool, con
   if (rows > 0x7fffffff) return -4;
   const int grid = attend_grid(B, S, Hq, Hkv, D, page, per, dt, cdt);
   if (grid > 0) {
-    const int R = S * (Hq / Hkv) <= 8 ? 8 : 16;
+    const int R = attend_rows(S * (Hq / Hkv), D, cdt);
     int4* spans = reinterpret_cast<int4*>(workspace + (size_t)grid * 2 * R * (D + 2));
 #define GB_ATTEND_(T, C, D_, NQ_) (S > 1 ? launch_attend<T, C, D_, NQ_, true>(a, c, workspace, spans, grid, st) : launch_attend<T, C, D_, NQ_, false>(a, c, workspace, spans, grid, st))
 #define GB_ATTEND(T, C) (D == 64 ? (R == 8 ? GB_ATTEND_(T, C, 64, 1) : GB_ATTEND_(T, C, 64, 2)) : (R == 8 ? GB_ATTEND_(T, C, 128, 1) : GB_ATTEND_(T, C, 128, 2)))
     if (dt == DT_BF16) return cdt == DT_E4M3 ? GB_ATTEND(__nv_bfloat16, DT_E4M3) : GB_ATTEND(__nv_bfloat16, DT_BF16);
-    return cdt == DT_E4M3 ? GB_ATTEND(__half, DT_E4M3) : GB_ATTEND(__half, DT_F16);
+    if (dt == DT_F16) return cdt == DT_E4M3 ? GB_ATTEND(__half, DT_E4M3) : GB_ATTEND(__half, DT_F16);
+    if (D == 128) return GB_ATTEND_(float, DT_F32, 128, 1);
+    return R == 8 ? GB_ATTEND_(float, DT_F32, 64, 1) : GB_ATTEND_(float, DT_F32, 64, 2);
 #undef GB_ATTEND
 #undef GB_ATTEND_
   }
