@@ -120,19 +120,19 @@ __device__ __forceinline__ void split_tf32(const uint32_t (&x)[N], uint32_t (&hi
     lo[k] = (x[k] & 0x7f800000u) == 0x7f800000u ? 0u : (__float_as_uint(__uint_as_float(x[k]) - __uint_as_float(hi[k])) + 0x1000u) & 0xffffe000u;
   }
 }
-// c += a b in 32 bits: the three larger of four products
-__device__ __forceinline__ void mma_f32(float (&c)[4], const uint32_t (&a)[4], const uint32_t (&bh)[2], const uint32_t (&bl)[2]) {
+// hi + lo += a b in 32 bits: the three larger of four products, the small ones in a sum of their own
+__device__ __forceinline__ void mma_f32(float (&hi)[4], float (&lo)[4], const uint32_t (&a)[4], const uint32_t (&bh)[2], const uint32_t (&bl)[2]) {
   uint32_t ah[4], al[4];
   split_tf32(a, ah, al);
-  mma_tf32(c, al, bh);
-  mma_tf32(c, ah, bl);
-  mma_tf32(c, ah, bh);
+  mma_tf32(lo, al, bh);
+  mma_tf32(lo, ah, bl);
+  mma_tf32(hi, ah, bh);
 }
 // O^T += V^T P^T of a step: P as high and low part
 template <class C>
 __device__ __forceinline__ void mma_pv(float (&acc)[4], const uint32_t (&v)[4], const uint32_t (&hi)[2], const uint32_t (&lo)[2]) {
   if constexpr (C::F32) {
-    mma_f32(acc, v, hi, lo);
+    mma_f32(acc, acc, v, hi, lo);
   } else {
     mma_k16<C::BF>(acc, v[0], v[1], v[2], v[3], hi[0], hi[1]);
     if constexpr (C::SPLIT) mma_k16<C::BF>(acc, v[0], v[1], v[2], v[3], lo[0], lo[1]);
@@ -384,6 +384,7 @@ paged_attend_kernel(const AttendArgs a, const Paged c, const AttendPlan plan) {
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
           if (row[i] < 0) gone |= 1u << i;
+          float small[NQ][4] = {};
 #pragma unroll
           for (int q = 0; q < NQ; ++q)
 #pragma unroll
@@ -394,14 +395,17 @@ paged_attend_kernel(const AttendArgs a, const Paged c, const AttendPlan plan) {
             const uint32_t hi[4] = {kr[i][1][j].x, kr[i][1][j].y, kr[i][1][j].z, kr[i][1][j].w};
             if constexpr (C::F32) {
 #pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                const uint32_t x[4] = {lo[2 * h], hi[2 * h], lo[2 * h + 1], hi[2 * h + 1]};
+              for (int q = 0; q < NQ; ++q) {
+                float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int q = 0; q < NQ; ++q) {
+                for (int h = 0; h < 2; ++h) {
+                  const uint32_t x[4] = {lo[2 * h], hi[2 * h], lo[2 * h + 1], hi[2 * h + 1]};
                   uint32_t bh[2], bl[2];
                   split_tf32(qf[q][2 * j + h], bh, bl);
-                  mma_f32(s[i][q], x, bh, bl);
+                  mma_f32(sum, small[q], x, bh, bl);
                 }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[i][q][e] += sum[e];
               }
             } else if constexpr (!C::E8) {
 #pragma unroll
@@ -419,6 +423,12 @@ paged_attend_kernel(const AttendArgs a, const Paged c, const AttendPlan plan) {
                 for (int q = 0; q < NQ; ++q) mma_k16<false>(s[i][q], a0, a1, a2, a3, qf[q][4 * j + h][0], qf[q][4 * j + h][1]);
               }
             }
+          }
+          if constexpr (C::F32) {
+#pragma unroll
+            for (int q = 0; q < NQ; ++q)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) s[i][q][e] += small[q][e];
           }
           if constexpr (C::E8) {
 #pragma unroll
@@ -546,26 +556,23 @@ paged_attend_kernel(const AttendArgs a, const Paged c, const AttendPlan plan) {
             }
           }
         // ---- O^T += V^T P^T -----------------------------------------------------------------------------------------
-        auto product = [&](int i, int mt, int gp, const uint32_t (&v)[4]) {
+        auto product = [&](float (&acc)[4], int i, int q, int gp, const uint32_t (&v)[4]) {
+          if constexpr (MULTI) {
+            if (tail) {
+              mma_pv_ragged<C>(acc, v, ph[i][q][gp], pl[i][q][gp], [&](uint32_t (&ones)[2]) {
+                const int key = (ch * NS + i) * 16 + g + 8 * gp;
+                if constexpr (C::F32) {
+                  turned(key < end[q][0] ? 1.f : 0.f, key < end[q][1] ? 1.f : 0.f, ones);
+                } else {
 #pragma unroll
-          for (int q = 0; q < NQ; ++q) {
-            if constexpr (MULTI) {
-              if (tail) {
-                mma_pv_ragged<C>(o[q][mt], v, ph[i][q][gp], pl[i][q][gp], [&](uint32_t (&ones)[2]) {
-                  const int key = (ch * NS + i) * 16 + g + 8 * gp;
-                  if constexpr (C::F32) {
-                    turned(key < end[q][0] ? 1.f : 0.f, key < end[q][1] ? 1.f : 0.f, ones);
-                  } else {
-#pragma unroll
-                    for (int h = 0; h < 2; ++h)
-                      ones[h] = transposed_8x8((key + 8 * h < end[q][0] ? C::BF ? 0x3f80u : 0x3c00u : 0u) | (key + 8 * h < end[q][1] ? C::BF ? 0x3f800000u : 0x3c000000u : 0u));
-                  }
-                });
-                continue;
-              }
+                  for (int h = 0; h < 2; ++h)
+                    ones[h] = transposed_8x8((key + 8 * h < end[q][0] ? C::BF ? 0x3f80u : 0x3c00u : 0u) | (key + 8 * h < end[q][1] ? C::BF ? 0x3f800000u : 0x3c000000u : 0u));
+                }
+              });
+              return;
             }
-            mma_pv<C>(o[q][mt], v, ph[i][q][gp], pl[i][q][gp]);
           }
+          mma_pv<C>(acc, v, ph[i][q][gp], pl[i][q][gp]);
         };
 #pragma unroll
         for (int i = 0; i < NS; ++i)
@@ -573,22 +580,29 @@ paged_attend_kernel(const AttendArgs a, const Paged c, const AttendPlan plan) {
           for (int j = 0; j < VW; ++j) {
             if constexpr (C::F32) {
               if (j & 1) continue;
+              const uint32_t v[2][4] = {{vr[i][0][j], vr[i][0][j + 1], vr[i][1][j], vr[i][1][j + 1]},
+                                        {vr[i][2][j], vr[i][2][j + 1], vr[i][3][j], vr[i][3][j + 1]}};
 #pragma unroll
-              for (int gp = 0; gp < 2; ++gp) {
-                const uint32_t v[4] = {vr[i][2 * gp][j], vr[i][2 * gp][j + 1], vr[i][2 * gp + 1][j], vr[i][2 * gp + 1][j + 1]};
-                product(i, j / 2, gp, v);
+              for (int q = 0; q < NQ; ++q) {
+                float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                product(sum, i, q, 0, v[0]);
+                product(sum, i, q, 1, v[1]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[q][j / 2][e] += sum[e];
               }
             } else if constexpr (!C::E8) {
               const uint32_t v[4] = {__byte_perm(vr[i][0][j], vr[i][1][j], 0x5410), __byte_perm(vr[i][0][j], vr[i][1][j], 0x7632),
                                      __byte_perm(vr[i][2][j], vr[i][3][j], 0x5410), __byte_perm(vr[i][2][j], vr[i][3][j], 0x7632)};
-              product(i, j, 0, v);
+#pragma unroll
+              for (int q = 0; q < NQ; ++q) product(o[q][j], i, q, 0, v);
             } else {
 #pragma unroll
               for (int h = 0; h < 2; ++h) {
                 uint32_t v[4];
                 e4m3x4_to_f16(__byte_perm(vr[i][0][j], vr[i][1][j], h ? 0x7362 : 0x5140), v[0], v[1]);
                 e4m3x4_to_f16(__byte_perm(vr[i][2][j], vr[i][3][j], h ? 0x7362 : 0x5140), v[2], v[3]);
-                product(i, 2 * j + h, 0, v);
+#pragma unroll
+                for (int q = 0; q < NQ; ++q) product(o[q][2 * j + h], i, q, 0, v);
               }
             }
           }
