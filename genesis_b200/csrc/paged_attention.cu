@@ -47,14 +47,21 @@ struct AttendPlan {
   int4* spans;          // [grid][2]: that item (-1: none), the first and the last CTA that have it
 };
 
+// Keys of a chunk: 4 KB of K and of V, but a tile of 16 at least and two of them at most (four tiles of 8 bits cost registers:
+// 64 x 4096, 2 KV heads of 64: 36.2 us with four, 33.6 with two; one tile of 128: 71.7 us for 70.1 over 4 KV heads).
+static constexpr int attend_chunk(int D, int bytes) { return 4096 / (D * bytes) < 16 ? 16 : 4096 / (D * bytes) > 32 ? 32 : 4096 / (D * bytes); }
+
 template <typename T, int CDT, int D_, int NQ_>
 struct PA {
   static constexpr int D = D_, NQ = NQ_, R = 8 * NQ;
   static constexpr bool E8 = CDT == DT_E4M3, BF = CDT == DT_BF16, F32 = CDT == DT_F32;
   static constexpr bool OBF = std::is_same<T, __nv_bfloat16>::value;
   static constexpr bool SPLIT = !(E8 && OBF);           // P in two numbers
+  // The tensor cores cut sums off towards zero (2^-24 of them a step on average).  Over thousands of steps that would show in an
+  // output of 11 bits and more, so there a chunk's products are added up apart and then to the accumulators, rounded.
+  static constexpr bool FRESH = !OBF;
   static constexpr int ES = E8 ? 1 : F32 ? 4 : 2;
-  static constexpr int KT = 4096 / (D * ES) < 16 ? 16 : 4096 / (D * ES);      // keys of a chunk: 4 KB of K and of V, at least a tile
+  static constexpr int KT = attend_chunk(D, ES);        // keys of a chunk
   static constexpr int NS = KT / 16;                    // tiles of 16 keys
   static constexpr int KL = D * ES / 64;                // 16-byte loads of a lane's share of a key's row
   static constexpr int VW = D * ES / 32;                // words of a lane's share of a value's row
@@ -138,40 +145,12 @@ __device__ __forceinline__ void mma_pv(float (&acc)[4], const uint32_t (&v)[4], 
     if constexpr (C::SPLIT) mma_k16<C::BF>(acc, v[0], v[1], v[2], v[3], lo[0], lo[1]);
   }
 }
-// The same where rows end at different keys: a key that one row sees and another does not is multiplied by a probability of 0
-// there, which an infinity or NaN among its values would turn into NaN.  If there are any, the product is made again without
-// them for the rows that do not see them; how many of them a row sees is a product too, of ones.
-template <class C, class Sees>
-__device__ __forceinline__ void mma_pv_ragged(float (&acc)[4], const uint32_t (&v)[4], const uint32_t (&hi)[2], const uint32_t (&lo)[2],
-                                              Sees sees) {
-  uint32_t fine[4], mark[4], bad = 0;
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    if constexpr (C::F32) {
-      const bool f = (v[k] & 0x7f800000u) == 0x7f800000u;
-      fine[k] = f ? 0u : v[k];
-      mark[k] = f ? 0x3f800000u : 0u;
-    } else {
-      constexpr uint32_t E = C::BF ? 0x7f80u : 0x7c00u, ONE = C::BF ? 0x3f80u : 0x3c00u;
-      const bool f = (v[k] & E) == E, g = (v[k] >> 16 & E) == E;
-      fine[k] = v[k] & ((f ? 0u : 0xffffu) | (g ? 0u : 0xffff0000u));
-      mark[k] = (f ? ONE : 0u) | (g ? ONE << 16 : 0u);
-    }
-    bad |= mark[k];
-  }
-  if (!__any_sync(0xffffffffu, bad != 0)) {
-    mma_pv<C>(acc, v, hi, lo);
-    return;
-  }
-  float seen[4] = {0.f, 0.f, 0.f, 0.f}, kept[4] = {acc[0], acc[1], acc[2], acc[3]};
-  uint32_t ones[2];
-  sees(ones);
-  if constexpr (C::F32) mma_tf32(seen, mark, ones);
-  else mma_k16<C::BF>(seen, mark[0], mark[1], mark[2], mark[3], ones[0], ones[1]);
-  mma_pv<C>(kept, fine, hi, lo);
-  mma_pv<C>(acc, v, hi, lo);
-#pragma unroll
-  for (int e = 0; e < 4; ++e) acc[e] = seen[e] == 0.f ? kept[e] : acc[e];
+// Bits of a word of V that are infinities or NaN, as a mask.
+template <class C>
+__device__ __forceinline__ uint32_t not_finite(uint32_t w) {
+  if constexpr (C::F32) return (w & 0x7f800000u) == 0x7f800000u ? 0xffffffffu : 0u;
+  else if constexpr (C::E8) return __vcmpeq4(w & 0x7f7f7f7fu, 0x7f7f7f7fu);
+  else return __vcmpeq2(w & (C::BF ? 0x7f807f80u : 0x7c007c00u), C::BF ? 0x7f807f80u : 0x7c007c00u);
 }
 __device__ __forceinline__ float pow2_of(float x) {
   float y;
@@ -370,6 +349,7 @@ paged_attend_kernel(const AttendArgs a, const Paged c, const AttendPlan plan) {
     }
     constexpr float LIFT = !C::E8 && !C::BF && !C::F32 ? 7.f : 0.f;      // fp16 P without a scale of its own
     int vtop = -1000;                  // the power of two of V that the accumulators are relative to
+    int odd_from = 0x7fffffff;         // the first chunk with values left out
     const int full = MULTI ? min(keys, max(0, len - cnt + 1)) : keys;      // keys that every token sees
 
     // one round: scores of chunk ch, K of chunk ch + 1 on its way, probabilities and products of ch, V of ch + 1 on its way
@@ -556,56 +536,68 @@ paged_attend_kernel(const AttendArgs a, const Paged c, const AttendPlan plan) {
             }
           }
         // ---- O^T += V^T P^T -----------------------------------------------------------------------------------------
-        auto product = [&](float (&acc)[4], int i, int q, int gp, const uint32_t (&v)[4]) {
-          if constexpr (MULTI) {
-            if (tail) {
-              mma_pv_ragged<C>(acc, v, ph[i][q][gp], pl[i][q][gp], [&](uint32_t (&ones)[2]) {
-                const int key = (ch * NS + i) * 16 + g + 8 * gp;
-                if constexpr (C::F32) {
-                  turned(key < end[q][0] ? 1.f : 0.f, key < end[q][1] ? 1.f : 0.f, ones);
-                } else {
+        if constexpr (MULTI) {
+          // A key that one row sees and another does not is multiplied by a probability of 0 there, which an infinity or NaN
+          // among its values would turn into NaN.  They are left out here; the rows that see them get them at the end.
+          if (tail) {
+            uint32_t bad = 0;
 #pragma unroll
-                  for (int h = 0; h < 2; ++h)
-                    ones[h] = transposed_8x8((key + 8 * h < end[q][0] ? C::BF ? 0x3f80u : 0x3c00u : 0u) | (key + 8 * h < end[q][1] ? C::BF ? 0x3f800000u : 0x3c000000u : 0u));
+            for (int i = 0; i < NS; ++i)
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+#pragma unroll
+                for (int j = 0; j < VW; ++j) {
+                  const uint32_t f = not_finite<C>(vr[i][k][j]);
+                  bad |= f;
+                  vr[i][k][j] &= ~f;
                 }
-              });
-              return;
-            }
+            if (__any_sync(0xffffffffu, bad != 0) && odd_from > ch) odd_from = ch;
           }
-          mma_pv<C>(acc, v, ph[i][q][gp], pl[i][q][gp]);
-        };
+        }
+        constexpr int TW = C::E8 ? 2 : 1;              // tiles of O^T that a word of V has numbers of
 #pragma unroll
-        for (int i = 0; i < NS; ++i)
+        for (int j = 0; j < VW; j += C::F32 ? 2 : 1) {
+          float sum[TW][NQ][4] = {};
 #pragma unroll
-          for (int j = 0; j < VW; ++j) {
+          for (int i = 0; i < NS; ++i) {
+            uint32_t v[TW * GP][4];
             if constexpr (C::F32) {
-              if (j & 1) continue;
-              const uint32_t v[2][4] = {{vr[i][0][j], vr[i][0][j + 1], vr[i][1][j], vr[i][1][j + 1]},
-                                        {vr[i][2][j], vr[i][2][j + 1], vr[i][3][j], vr[i][3][j + 1]}};
 #pragma unroll
-              for (int q = 0; q < NQ; ++q) {
-                float sum[4] = {0.f, 0.f, 0.f, 0.f};
-                product(sum, i, q, 0, v[0]);
-                product(sum, i, q, 1, v[1]);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) o[q][j / 2][e] += sum[e];
+              for (int k = 0; k < 2; ++k) {
+                v[k][0] = vr[i][2 * k][j]; v[k][1] = vr[i][2 * k][j + 1];
+                v[k][2] = vr[i][2 * k + 1][j]; v[k][3] = vr[i][2 * k + 1][j + 1];
               }
             } else if constexpr (!C::E8) {
-              const uint32_t v[4] = {__byte_perm(vr[i][0][j], vr[i][1][j], 0x5410), __byte_perm(vr[i][0][j], vr[i][1][j], 0x7632),
-                                     __byte_perm(vr[i][2][j], vr[i][3][j], 0x5410), __byte_perm(vr[i][2][j], vr[i][3][j], 0x7632)};
-#pragma unroll
-              for (int q = 0; q < NQ; ++q) product(o[q][j], i, q, 0, v);
+              v[0][0] = __byte_perm(vr[i][0][j], vr[i][1][j], 0x5410);
+              v[0][1] = __byte_perm(vr[i][0][j], vr[i][1][j], 0x7632);
+              v[0][2] = __byte_perm(vr[i][2][j], vr[i][3][j], 0x5410);
+              v[0][3] = __byte_perm(vr[i][2][j], vr[i][3][j], 0x7632);
             } else {
 #pragma unroll
               for (int h = 0; h < 2; ++h) {
-                uint32_t v[4];
-                e4m3x4_to_f16(__byte_perm(vr[i][0][j], vr[i][1][j], h ? 0x7362 : 0x5140), v[0], v[1]);
-                e4m3x4_to_f16(__byte_perm(vr[i][2][j], vr[i][3][j], h ? 0x7362 : 0x5140), v[2], v[3]);
-#pragma unroll
-                for (int q = 0; q < NQ; ++q) product(o[q][2 * j + h], i, q, 0, v);
+                e4m3x4_to_f16(__byte_perm(vr[i][0][j], vr[i][1][j], h ? 0x7362 : 0x5140), v[h][0], v[h][1]);
+                e4m3x4_to_f16(__byte_perm(vr[i][2][j], vr[i][3][j], h ? 0x7362 : 0x5140), v[h][2], v[h][3]);
               }
             }
+#pragma unroll
+            for (int h = 0; h < TW; ++h)
+#pragma unroll
+              for (int q = 0; q < NQ; ++q)
+#pragma unroll
+                for (int gp = 0; gp < GP; ++gp) {
+                  if constexpr (C::FRESH) mma_pv<C>(sum[h][q], v[h + gp], ph[i][q][gp], pl[i][q][gp]);
+                  else mma_pv<C>(o[q][j * TW + h], v[h], ph[i][q][gp], pl[i][q][gp]);
+                }
           }
+          if constexpr (C::FRESH) {
+#pragma unroll
+            for (int h = 0; h < TW; ++h)
+#pragma unroll
+              for (int q = 0; q < NQ; ++q)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[q][C::F32 ? j / 2 : j * TW + h][e] += sum[h][q][e];
+          }
+        }
       }
       if (more) {
 #pragma unroll
@@ -675,6 +667,29 @@ paged_attend_kernel(const AttendArgs a, const Paged c, const AttendPlan plan) {
           else if (row0 + r < rows) store_row4<T>(a, c, b, kvh, row0 + r, d, v, l[q][e]);
         }
       }
+    if constexpr (MULTI) {
+      if (odd_from < c1) {             // infinities and NaN among the values from there on, to the rows that see them
+        __syncwarp();
+        for (int e = lane; e < R * D; e += 32) {
+          const int r = row0 + e / D, d = e % D, s = r / group;
+          if (r >= rows || s >= cnt) continue;
+          const int stop = min(c1 * KT, min(keys, max(0, len - cnt + s + 1)));
+          float sum = 0.f;
+          for (int key = odd_from * KT; key < stop; ++key) {
+            const int i = key / c.page, page = pages[i];
+            if ((unsigned)page >= (unsigned)c.pages) continue;
+            const long long at = (((long long)page * c.Hkv + kvh) * c.page + key - i * c.page) * D + d;
+            float v;
+            if constexpr (C::E8) v = from_e4m3x2(reinterpret_cast<const uint8_t*>(a.vpool)[at]).x;
+            else v = load_as_float(a.vpool, CDT, at);
+            if (!(fabsf(v) < INFINITY)) sum += v;
+          }
+          if (sum == 0.f) continue;
+          if (!whole) pieces[((size_t)piece * R + e / D) * D + d] = sum;
+          else reinterpret_cast<T*>(a.o)[(((long long)b * c.S + s) * a.Hq + kvh * group + r % group) * D + d] = Cvt<T>::from_f(sum);
+        }
+      }
+    }
     u += c1 - c0;
   }
   __syncthreads();
@@ -875,7 +890,7 @@ static int attend_rows(int rows, int D, int cdt) { return rows <= 8 || (cdt == D
 static int attend_grid(int B, int S, int Hq, int Hkv, int D, int page, int per, int dt, int cdt) {
   if ((D != 64 && D != 128) || (cdt != dt && !(cdt == DT_E4M3 && dt != DT_F32)) || page % 16) return 0;
   const int rows = S * (Hq / Hkv), R = attend_rows(rows, D, cdt);
-  const int es = cdt == DT_E4M3 ? 1 : cdt == DT_F32 ? 4 : 2, kt = 4096 / (D * es) < 16 ? 16 : 4096 / (D * es);
+  const int es = cdt == DT_E4M3 ? 1 : cdt == DT_F32 ? 4 : 2, kt = attend_chunk(D, es);
   const long long tiles = (rows + R - 1) / R, keys = (long long)per * page;
   const long long chunks = (long long)B * Hkv * tiles * (keys <= 0 ? 1 : (keys + kt - 1) / kt);
   if (chunks > 0x7fffffff) return 0;       // (counted in 32 bits)
