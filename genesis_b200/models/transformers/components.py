@@ -6,6 +6,7 @@
 `apply_rope` is the fused path on `[B, S, H, D]` (one kernel per tensor instead of ~14).
 """
 import numpy as np
+import torch
 
 from ...tensor import Tensor, tensor
 from ... import nn
@@ -77,3 +78,30 @@ def apply_rope(x, rotary, position_ids=None):
         rotary._build(S)
     pos = None if position_ids is None else position_ids
     return F.rope(x, rotary.cos_cached, rotary.sin_cached, pos)
+
+
+def paged_self_attention(y, rotary, num_heads, cache, page_table, lengths, counts=None, prompt=False):
+    """Self-attention of a fused projection's y [B, S, (num_heads + 2 Hkv) D] through one layer of a paged cache -> [B, S,
+    num_heads * D].  The tokens' keys and values are put into the cache; with `prompt` the sequences have no others, and the
+    flash attention over the call's own keys takes the place of reading them back."""
+    B, S, _ = y.shape
+    room = page_table.shape[1] * cache.page_size
+    if room > rotary.max_seq_len_cached:
+        rotary._build(room)
+    cos, sin = rotary.cos_cached, rotary.sin_cached
+    if prompt:
+        q, k, v = F.qkv_rope(y, cos, sin, None, num_heads, cache.num_kv_heads, cache.head_dim)
+        F.paged_kv_write(k, v, cache, page_table, lengths, counts)
+        o = F.flash_attention(q, k, v, causal=True)
+    else:
+        q = F.paged_qkv_rope(y, cos, sin, cache, page_table, lengths, num_heads, counts)
+        o = F.paged_attention(q, cache, page_table, lengths, counts)
+    return F.reshape(o, (B, S, num_heads * cache.head_dim))
+
+
+def last_tokens(x, counts=None):
+    """[B, S, H] -> [B, 1, H]: each sequence's last real token (its last, without `counts`)."""
+    if counts is None or x.shape[1] == 1:
+        return x[:, x.shape[1] - 1:]
+    at = (counts._t.long() - 1).clamp(0, x.shape[1] - 1)
+    return F.unsqueeze(x[Tensor._wrap(torch.arange(x.shape[0], device=at.device)), Tensor._wrap(at)], 1)

@@ -14,7 +14,7 @@ import torch
 from ... import nn
 from ...nn import functional as F
 from ...tensor import Tensor
-from .components import RotaryEmbedding, apply_rope, find_multiple  # noqa: F401
+from .components import RotaryEmbedding, apply_rope, find_multiple, last_tokens, paged_self_attention  # noqa: F401
 from .config import TransformerConfig, get_transformer_config
 
 ModelArgs = TransformerConfig
@@ -40,11 +40,14 @@ class Attention(nn.Module):
         self.rotary_emb = RotaryEmbedding(self.head_dim, max_position_embeddings=config.max_position_embeddings,
                                           base=config.rope_theta)
 
+    def _projected(self, x):
+        # q, k and v projections as one GEMM over the stacked weights; RoPE reads its head slices in place
+        return F.fused_linear(x, [self.q_proj.weight, self.k_proj.weight, self.v_proj.weight],
+                              [self.q_proj.bias, self.k_proj.bias, self.v_proj.bias])
+
     def forward(self, x, position_ids=None, mask=None):
         B, S, _ = x.shape
-        # q, k and v projections as one GEMM over the stacked weights; RoPE reads its head slices in place
-        y = F.fused_linear(x, [self.q_proj.weight, self.k_proj.weight, self.v_proj.weight],
-                           [self.q_proj.bias, self.k_proj.bias, self.v_proj.bias])
+        y = self._projected(x)
         rot = self.rotary_emb
         if S > rot.max_seq_len_cached:
             rot._build(S)
@@ -52,6 +55,11 @@ class Attention(nn.Module):
                              self.head_dim)
         o = F.flash_attention(q, k, v, causal=True)
         return self.o_proj(F.reshape(o, (B, S, self.num_heads * self.head_dim)))
+
+    def forward_paged(self, x, cache, page_table, lengths, counts=None, prompt=False):
+        """The same over one layer of a paged cache (`components.paged_self_attention`)."""
+        return self.o_proj(paged_self_attention(self._projected(x), self.rotary_emb, self.num_heads, cache, page_table, lengths,
+                                                counts, prompt))
 
 
 class FeedForward(nn.Module):
@@ -95,6 +103,12 @@ class TransformerBlock(nn.Module):
         h, n2 = self.post_attention_layernorm.add_forward(x, self.self_attn(n, position_ids, mask))
         return h, self.mlp(n2)
 
+    def forward_paged(self, stream, branch, *paged):
+        """`forward_deferred` over one layer of a paged cache; `paged` as `Attention.forward_paged` takes it."""
+        x, n = self.input_layernorm.add_forward(stream, branch)
+        h, n2 = self.post_attention_layernorm.add_forward(x, self.self_attn.forward_paged(n, *paged))
+        return h, self.mlp(n2)
+
 
 class QwenModel(nn.Module):
     def __init__(self, config):
@@ -124,6 +138,13 @@ class QwenModel(nn.Module):
     def forward(self, idx, position_ids=None):
         return self.lm_head(self.hidden_states(idx, position_ids))
 
+    def forward_paged(self, idx, cache, page_table, lengths, counts=None, prompt=False, last=True):
+        x, branch = self.embed_tokens(idx), None
+        for i, layer in enumerate(self.layers):
+            x, branch = layer.forward_paged(x, branch, cache[i], page_table, lengths, counts, prompt)
+        h = self.norm.add_forward(x, branch)[1]
+        return self.lm_head(last_tokens(h, counts) if last else h)
+
     @classmethod
     def from_name(cls, name):
         return cls(get_transformer_config(name))
@@ -147,19 +168,34 @@ class QwenForCausalLM(nn.Module):
                                _inplace_backward=not return_logits)
         return (loss, logits) if return_logits else loss
 
-    def generate(self, input_ids, max_new_tokens=100, temperature=1.0, top_k=None, top_p=None):
-        """Appends `max_new_tokens` sampled tokens to `input_ids` [B, S] (temperature 0: greedy).  The prompt is
-        re-encoded every step (no KV cache in this model class, as in the reference)."""
+    def forward_paged(self, idx, cache, page_table, lengths, counts=None, prompt=False, last=True):
+        """Logits of the tokens idx [B, S] that follow what a `nn.PagedKVCache` holds of their sequences, and are put into it.
+
+        `page_table` [B, pages], `lengths` [B] (tokens with those of this call) and `counts` [B] (real ones of the S) are int32
+        Tensors as `nn.functional.paged_attention` takes them.  `prompt`: the sequences had no tokens before.  `last`: logits
+        [B, 1, V] of each sequence's last real token, else [B, S, V].  For inference; nothing here waits for the device, so a
+        step can be captured and replayed while the lengths grow on the device."""
+        return self.model.forward_paged(idx, cache, page_table, lengths, counts, prompt, last)
+
+    def generate(self, input_ids, max_new_tokens=100, temperature=1.0, top_k=None, top_p=None, cache_dtype=None):
+        """Appends `max_new_tokens` sampled tokens to `input_ids` [B, S] (temperature 0: greedy).
+
+        Without `cache_dtype` the prompt is re-encoded every step (as in the reference); with it ("float32", "float16",
+        "bfloat16" or "float8_e4m3fn") keys and values are kept in a paged cache of that type and every step encodes one
+        token of each sequence."""
         from ... import grad_mode
-        from .sampling import sample_next
+        from .sampling import generate_paged, sample_next
         was_training = self.training
         self.eval()
-        out = input_ids
-        with grad_mode.no_grad():
-            for _ in range(max_new_tokens):
-                logits = self(out)
-                tok = sample_next(logits._t[:, -1, :], temperature, top_k, top_p)
-                out = Tensor._wrap(torch.cat((out._t, tok.to(out._t.dtype)), dim=1))
+        if cache_dtype is not None:
+            out = generate_paged(self, input_ids, max_new_tokens, temperature, top_k, top_p, cache_dtype)
+        else:
+            out = input_ids
+            with grad_mode.no_grad():
+                for _ in range(max_new_tokens):
+                    logits = self(out)
+                    tok = sample_next(logits._t[:, -1, :], temperature, top_k, top_p)
+                    out = Tensor._wrap(torch.cat((out._t, tok.to(out._t.dtype)), dim=1))
         if was_training:
             self.train()
         return out

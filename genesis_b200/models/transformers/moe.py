@@ -25,10 +25,10 @@ from ...function import Function, AMPPolicy
 from ...nn import functional as F
 from ...nn.modules.module import Module, Parameter
 from ...ops import dispatch as K
-from .sampling import sample_next
+from .sampling import generate_paged, sample_next
 from ...tensor import Tensor
 from ...amp_state import amp_state
-from .components import RotaryEmbedding, apply_rope
+from .components import RotaryEmbedding, apply_rope, last_tokens, paged_self_attention
 from .config import MoEConfig, get_moe_config
 
 
@@ -366,15 +366,23 @@ class MoEAttention(Module):
         self.rotary_emb = RotaryEmbedding(self.head_dim, max_position_embeddings=config.max_position_embeddings,
                                           base=config.rope_theta)
 
+    def _projected(self, hidden_states):
+        # q, k and v projections as one GEMM over the stacked weights; RoPE reads its head slices in place
+        biases = [self.q_proj.bias, self.k_proj.bias, self.v_proj.bias] if self.q_proj.bias is not None else None
+        return F.fused_linear(hidden_states, [self.q_proj.weight, self.k_proj.weight, self.v_proj.weight], biases)
+
+    def forward_paged(self, hidden_states, cache, page_table, lengths, counts=None, prompt=False):
+        """Self-attention over one layer of a paged cache (`components.paged_self_attention`)."""
+        return self.o_proj(paged_self_attention(self._projected(hidden_states), self.rotary_emb, self.num_heads, cache, page_table,
+                                                lengths, counts, prompt))
+
     def forward(self, hidden_states, attention_mask=None, position_ids=None, past_key_value=None,
                 use_cache=False):
         B, S, _ = hidden_states.shape
         past = 0 if past_key_value is None else past_key_value[0].shape[1]
         if position_ids is None and past > 0:
             position_ids = Tensor._wrap(torch.arange(past, past + S, device=hidden_states._t.device).expand(B, S).contiguous())
-        # q, k and v projections as one GEMM over the stacked weights; RoPE reads its head slices in place
-        biases = [self.q_proj.bias, self.k_proj.bias, self.v_proj.bias] if self.q_proj.bias is not None else None
-        y = F.fused_linear(hidden_states, [self.q_proj.weight, self.k_proj.weight, self.v_proj.weight], biases)
+        y = self._projected(hidden_states)
         rot = self.rotary_emb
         need = S + past if position_ids is None else S + past
         if need > rot.max_seq_len_cached:
@@ -459,6 +467,12 @@ class MoEDecoderLayer(Module):
         h, n2 = self.post_attention_layernorm.add_forward(x, a)
         return h, self.mlp(n2), present
 
+    def forward_paged(self, stream, branch, *paged):
+        """`forward_deferred` over one layer of a paged cache; `paged` as `MoEAttention.forward_paged` takes it."""
+        x, n = self.input_layernorm.add_forward(stream, branch)
+        h, n2 = self.post_attention_layernorm.add_forward(x, self.self_attn.forward_paged(n, *paged))
+        return h, self.mlp(n2)
+
 
 class MoEPreTrainedModel(Module):
     def __init__(self, config):
@@ -508,6 +522,12 @@ class MoEModel(MoEPreTrainedModel):
                 presents.append(present)
         return self.norm.add_forward(h, branch)[1], presents
 
+    def forward_paged(self, input_ids, cache, page_table, lengths, counts=None, prompt=False):
+        h, branch = self.embed_tokens(input_ids), None
+        for i, layer in enumerate(self.layers):
+            h, branch = layer.forward_paged(h, branch, cache[i], page_table, lengths, counts, prompt)
+        return self.norm.add_forward(h, branch)[1]
+
 
 class MoEForCausalLM(MoEPreTrainedModel):
     def __init__(self, config, ep_group=None):
@@ -540,9 +560,19 @@ class MoEForCausalLM(MoEPreTrainedModel):
         config = get_moe_config(config_or_path) if isinstance(config_or_path, str) else config_or_path
         return cls(config)
 
-    def generate(self, input_ids, max_new_tokens=100, temperature=1.0, top_k=None, top_p=None):
+    def forward_paged(self, input_ids, cache, page_table, lengths, counts=None, prompt=False, last=True):
+        """Logits of the tokens [B, S] that follow what a `nn.PagedKVCache` holds of their sequences
+        (`QwenForCausalLM.forward_paged`)."""
+        h = self.model.forward_paged(input_ids, cache, page_table, lengths, counts, prompt)
+        return self.lm_head(last_tokens(h, counts) if last else h)
+
+    def generate(self, input_ids, max_new_tokens=100, temperature=1.0, top_k=None, top_p=None, cache_dtype=None):
+        """Appends `max_new_tokens` sampled tokens to `input_ids` [B, S]; with `cache_dtype` keys and values are kept in a paged
+        cache of that type (`QwenForCausalLM.generate`)."""
         from ... import grad_mode
         self.eval()
+        if cache_dtype is not None:
+            return generate_paged(self, input_ids, max_new_tokens, temperature, top_k, top_p, cache_dtype)
         generated = input_ids
         with grad_mode.no_grad():
             for _ in range(max_new_tokens):

@@ -30,3 +30,29 @@ def sample_next(logits, temperature=1.0, top_k=None, top_p=None):
     u = u.clamp_(1e-20, 1.0 - 1e-7)
     gumbel = -torch.log(-torch.log(u))
     return K.argmax(x + gumbel, -1, True)
+
+
+def generate_paged(model, input_ids, max_new_tokens, temperature, top_k, top_p, cache_dtype, page_size=64):
+    """Appends `max_new_tokens` sampled tokens to `input_ids` [B, S], with keys and values kept in a paged cache of
+    `cache_dtype`: the prompt is encoded once, then one token of each sequence a step.  `model` has a `config` and
+    `forward_paged`."""
+    from ... import grad_mode
+    from ...nn.paged import PagedKVCache
+    from ...tensor import Tensor
+    cfg, out = model.config, input_ids._t
+    B, S = out.shape
+    with grad_mode.no_grad():
+        most = S + max_new_tokens
+        per = -(-most // page_size)
+        cache = PagedKVCache(max(1, B * per), cfg.num_key_value_heads, cfg.head_dim, page_size=page_size,
+                             num_layers=cfg.num_hidden_layers, dtype=cache_dtype, device=out.device)
+        table = cache.page_table(cache.allocate([most] * B))
+        lengths = Tensor._wrap(torch.full((B,), S, dtype=torch.int32, device=out.device))
+        step = out
+        for i in range(max_new_tokens):
+            if i > 0:
+                lengths._t += 1
+            logits = model.forward_paged(Tensor._wrap(step), cache, table, lengths, prompt=i == 0)
+            step = sample_next(logits._t[:, -1, :], temperature, top_k, top_p).to(out.dtype)
+            out = torch.cat((out, step), dim=1)
+    return Tensor._wrap(out)
