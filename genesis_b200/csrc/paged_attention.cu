@@ -21,6 +21,7 @@
 //              below a bf16 output.  fp16 P is scaled by 2^7 on top of a maximum that may lag 2^8 behind, so that 2^-31 of the
 //              largest probability is still a number.  e4m3 becomes fp16 exactly; a bf16 q does under a power of two for each
 //              row.  K's powers of two multiply scores, V's multiply P, relative to the largest seen so far.
+#include "attention_common.cuh"
 #include "paged_common.cuh"
 #include <type_traits>
 
@@ -44,12 +45,16 @@ struct AttendPlan {
   int grid;             // CTAs launched
   float* parts;         // [grid][2][R][D] sums, then [grid][2][R] maxima and normalisers: of an item that comes from the CTA before,
                         // and of one that begins in the CTA and goes on behind it
+  float* spill;         // [grid][PA_WARPS][R][D] sums: pieces that a warp leaves behind before it goes on
   int4* spans;          // [grid][2]: that item (-1: none), the first and the last CTA that have it
 };
 
 // Keys of a chunk: 4 KB of K and of V, but a tile of 16 at least and two of them at most (four tiles of 8 bits cost registers:
 // 64 x 4096, 2 KV heads of 64: 36.2 us with four, 33.6 with two; one tile of 128: 71.7 us for 70.1 over 4 KV heads).
 static constexpr int attend_chunk(int D, int bytes) { return 4096 / (D * bytes) < 16 ? 16 : 4096 / (D * bytes) > 32 ? 32 : 4096 / (D * bytes); }
+
+// Chunks in flight of a warp: 16 KB of them (15 of 8 bits and 64), with three CTAs on an SM.
+static constexpr int attend_stages(int D, int bytes) { return D * bytes == 512 ? 1 : D * bytes == 64 ? 3 : 2; }
 
 template <typename T, int CDT, int D_, int NQ_>
 struct PA {
@@ -69,31 +74,39 @@ struct PA {
   static constexpr int QS = F32 ? D / 8 : D / 16;       // steps of the contraction over d
   static constexpr int GP = F32 ? 2 : 1;                // ... and of a tile's over its keys
   static constexpr int PIECE = R * D;
-  static constexpr int SMEM = 2 * PA_WARPS * PIECE * 4;
-  static constexpr int CTAS = NQ == 1 && !(F32 && D == 128) ? 3 : 2;          // on an SM
+  static constexpr int RB = D * ES, BOX = RB < 128 ? RB : 128;      // bytes of a row, and of a column of the ring's boxes
+  static constexpr int KB = KT * RB, SB = E8 ? NS * 32 : 0;          // a stage: K, V; powers of two (behind all rings)
+  static constexpr int ST = attend_stages(D, ES), RING = ST * 2 * KB;
+  static constexpr int SMEM = PA_WARPS * (RING + ST * SB) + 1024;   // (boxes start on 1024 bytes)
+  static_assert(PIECE * 4 <= RING, "a warp's last piece takes its ring's place");
+  static constexpr int CTAS = 3;                        // on an SM
   // first of the two columns d that a lane has of tile mt
   static __device__ __forceinline__ int column(int g, int mt) {
     if (E8) return g * (D / 8) + mt * 2;
     if (F32) return (g + 8 * (mt >> 1)) * 4 + (mt & 1) * 2;
     return (g + 8 * (mt >> 2)) * 8 + (mt & 3) * 2;
   }
-  // the k-th of the four keys of a tile whose values a lane loads, less its first
-  static __device__ __forceinline__ int first_key(int t) { return F32 ? t : 2 * t; }
-  static __device__ __forceinline__ constexpr int key_step(int k) { return F32 ? 4 * k : (k & 1) + (k >> 1) * 8; }
+  // Row r of an operand of 16 keys is key r ^ 4 where r is odd: then the eight lanes that read shared memory at a time meet eight
+  // different 16-byte units of the swizzled boxes (16 rows of 128 bytes, unit u of row r at u ^ r % 8), for K and for V.
+  static __device__ __forceinline__ int key_of(int r) { return r ^ ((r & 1) << 2); }
+  // where a lane's share of K's row g starts in a tile, and of the first of the four rows whose values it reads (2t, 2t + 1, and 8
+  // on; t, t + 4, t + 8, t + 12 for 32 bits); the others follow by constants
+  static __device__ __forceinline__ int k_unit(int g, int t) {
+    const int key = key_of(g);
+    return RB == 64 ? key * 64 + ((t ^ (key >> 1 & 3)) << 4) : key * 128 + ((t ^ key) << 4);
+  }
+  static __device__ __forceinline__ int first_key(int t) { return F32 ? key_of(t) : 2 * t; }
+  static __device__ __forceinline__ int v_unit(int g, int t) {
+    const int key = first_key(t);
+    return RB == 64 ? key * 64 + (((g >> 1) ^ (key >> 1 & 3)) << 4) + (g & 1) * 8 : key * 128 + ((g ^ key) << 4);
+  }
+  static constexpr int ODD_KEY = F32 ? 4 : 5;           // the second row's key is the first's ^ this: 4, or (2t + 1) ^ 4
+  static constexpr int ODD_UNIT = RB == 64 ? 5 * 64 ^ 2 << 4 : ODD_KEY * 128 ^ ODD_KEY << 4;
 };
 
-// keys that are not there are read from here, so that loads need no predicates (and no moves of zeros)
-__device__ const uint4 PA_ZEROS[32] = {};         // (a row of 128 numbers of 32 bits)
-
-__device__ __forceinline__ uint4 ld_stream16(const void* p) {
-  uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-  return v;
-}
-__device__ __forceinline__ uint2 ld_stream8(const void* p) {
-  uint2 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
-  return v;
+// 16 bytes to shared memory by a bulk copy
+__device__ __forceinline__ void bulk_copy_16(uint32_t dst, const void* src, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], 16, [%2];" ::"r"(dst), "l"(src), "r"(smem_u32(bar)) : "memory");
 }
 __device__ __forceinline__ uint32_t transposed_8x8(uint32_t v) {
   uint32_t r;
@@ -186,10 +199,16 @@ __device__ __forceinline__ void store_row4(const AttendArgs& a, const Paged& c, 
 // MULTI: several tokens a sequence, whose rows end at different keys
 template <typename T, int CDT, int D, int NQ, bool MULTI>
 __global__ void __launch_bounds__(PA_WARPS * 32, PA<T, CDT, D, NQ>::CTAS)
-paged_attend_kernel(const AttendArgs a, const Paged c, const AttendPlan plan) {
+paged_attend_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv, const AttendArgs a, const Paged c,
+                    const AttendPlan plan) {
   using C = PA<T, CDT, D, NQ>;
   constexpr int R = C::R, KT = C::KT, NS = C::NS, KL = C::KL, VW = C::VW, MT = C::MT, QS = C::QS, GP = C::GP, W = PA_WARPS;
-  extern __shared__ __align__(16) float pieces[];                  // [2 W][R][D]
+  extern __shared__ __align__(1024) uint8_t shared[];              // [W][RING], [W][ST][SB]
+  __shared__ uint64_t landed[W][C::ST][2];                           // K's and V's copies of a stage have landed
+  __shared__ int abort_word;
+  volatile int* const abort_flag = &abort_word;
+  uint8_t* const rings = shared + (1024 - (smem_u32(shared) & 1023)) % 1024;
+  __shared__ const float* piece_at[2 * W];                         // [R][D] sums: in the ring of the warp, or in the workspace
   __shared__ float piece_m[2 * W][R], piece_l[2 * W][R];
   __shared__ int piece_item[2 * W], piece_flags[2 * W];
   __shared__ unsigned piece_start[2 * W], piece_end[2 * W], scan[W], first_chunk[W];
@@ -210,6 +229,13 @@ paged_attend_kernel(const AttendArgs a, const Paged c, const AttendPlan plan) {
   }
   if (lane == 31) scan[warp] = upto;
   if (threadIdx.x < 2 * W) piece_item[threadIdx.x] = -1;
+  if (threadIdx.x == 0) {
+    abort_word = 0;
+    for (int i = 0; i < W * C::ST * 2; ++i) mbar_init(&landed[0][0][0] + i, 1);
+    mbar_fence_init();
+    tma_prefetch_desc(&tmk);
+    tma_prefetch_desc(&tmv);
+  }
   __syncthreads();
   unsigned total = 0;
 #pragma unroll
@@ -250,6 +276,10 @@ paged_attend_kernel(const AttendArgs a, const Paged c, const AttendPlan plan) {
   int b = first_b[warp];
   unsigned seq_start = first_chunk[warp];
   int slot = 0;
+  const int k_at = C::k_unit(g, t), v_at = C::v_unit(g, t), gk = C::key_of(g);
+  uint8_t* const ring = rings + warp * C::RING;
+  uint8_t* const powers = rings + W * C::RING + warp * C::ST * C::SB;
+  int put = 0, put_phase = 0, use = 0, use_phase = 0;              // stage of the next chunk that is copied and of the one that is worked on
   const float sl2 = a.scale * 1.4426950408889634f;
   const int group = a.Hq / c.Hkv, rows = c.S * group, tpp = c.page / 16;
 
@@ -264,8 +294,7 @@ paged_attend_kernel(const AttendArgs a, const Paged c, const AttendPlan plan) {
     const int cnt = c.count(b), len = c.length(b);
     if (len > keys && cnt > 0 && c0 == 0 && lane == 0) report_error(c.status, GB_ERR_BAD_INDEX, SITE_POSITION, len - 1);
 
-    // ---- loads ------------------------------------------------------------------------------------------------------
-    const char* const zeros = reinterpret_cast<const char*>(PA_ZEROS);
+    // ---- copies -----------------------------------------------------------------------------------------------------
     const int* pages = c.table + (size_t)b * c.per;
     int tile = c0 * NS, pg = tile / tpp, sub = tile - pg * tpp;            // the next tile whose page is asked for
     int id[NS], place[NS];
@@ -288,54 +317,15 @@ paged_attend_kernel(const AttendArgs a, const Paged c, const AttendPlan plan) {
       constexpr int H = C::E8 ? 2 : 1, E = 16 / sizeof(T);     // 16-byte loads that go with one of a key's row, numbers of each
 #pragma unroll
       for (int i = 0; i < KL * H; ++i) {
-        const uint4 v = ld_stream16(r < rows ? reinterpret_cast<const char*>(p + ((i / H) * 4 + t) * E * H + (i % H) * E) : zeros);
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (r < rows) v = __ldg(reinterpret_cast<const uint4*>(p + ((i / H) * 4 + t) * E * H + (i % H) * E));
         qf[q][2 * i][0] = v.x; qf[q][2 * i][1] = v.y;
         qf[q][2 * i + 1][0] = v.z; qf[q][2 * i + 1][1] = v.w;
       }
     }
-    long long row[NS];                 // of the pool; -1: no such tile
-    uint4 kr[NS][2][KL];
-    uint32_t vr[NS][4][VW], sc[NS];
+    long long row[NS];                 // of the pool, of the chunk that is copied; -1: no such tile
     float factor[NQ][2];               // of the scores of queries 2t, 2t + 1
     int end[NQ][2];                    // keys that they see (without MULTI: all, or it is no row)
-#pragma unroll
-    for (int q = 0; q < NQ; ++q) {
-      float fq = 1.f;
-      if constexpr (C::E8 && C::OBF) {   // bf16 -> fp16 with the row's largest in [2^14, 2^15)
-        uint32_t top = 0;
-#pragma unroll
-        for (int i = 0; i < MT; ++i)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const float2 x = unpack2<true>(qf[q][i][h]);
-            top = max(top, max(finite_bits(x.x), finite_bits(x.y)));
-          }
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        int e = (int)(top >> 23) - 127 - 14;
-        e = e < -100 ? -100 : e;
-        const float inv = exp2i(-e);
-        fq = exp2i(e);
-#pragma unroll
-        for (int i = 0; i < MT; ++i)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const float2 x = unpack2<true>(qf[q][i][h]);
-            qf[q][i][h] = pack2c<false>(x.x * inv, x.y * inv);
-          }
-      }
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        factor[q][e] = sl2 * __shfl_sync(0xffffffffu, fq, (2 * t + e) * 4);
-        if constexpr (MULTI) {
-          const int rr = row0 + q * 8 + 2 * t + e, s = rr / group;
-          end[q][e] = rr < rows && s < cnt ? min(keys, max(0, len - cnt + s + 1)) : 0;
-        } else {
-          end[q][e] = keys;
-        }
-      }
-    }
-
     // running maximum m (may lag 2^8 behind), what the exponents are taken off by, normaliser: of this lane's keys
     float o[NQ][MT][4], m[NQ][2], off[NQ][2], l[NQ][2];
 #pragma unroll
@@ -352,18 +342,60 @@ paged_attend_kernel(const AttendArgs a, const Paged c, const AttendPlan plan) {
     int odd_from = 0x7fffffff;         // the first chunk with values left out
     const int full = MULTI ? min(keys, max(0, len - cnt + 1)) : keys;      // keys that every token sees
 
-    // one round: scores of chunk ch, K of chunk ch + 1 on its way, probabilities and products of ch, V of ch + 1 on its way
-    for (int ch = c0 - 1; ch < c1; ++ch) {
-      const bool now = ch >= c0, more = ch + 1 < c1;
+    // one round: scores of chunk ch, then K of chunk ch + ST into its place; probabilities and products of ch, then V of ch + ST.
+    uint32_t gone_later = 0;           // tiles that are not there, of the chunks in flight
+    for (int ch = c0 - C::ST; ch < c1; ++ch) {
+      const bool now = ch >= c0, more = ch + C::ST < c1;
+      uint8_t* const sk = ring + use * 2 * C::KB;
       // ---- S^T = K Q^T ----------------------------------------------------------------------------------------------
       float s[NS][NQ][4];
       float ks[NS][2];
       int ve[NS][2];
-      uint32_t gone = 0;
+      const uint32_t gone = gone_later & ((1u << NS) - 1);
+      gone_later >>= NS;
+      if (ch == c0) {
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) {
+          float fq = 1.f;
+          if constexpr (C::E8 && C::OBF) {   // bf16 -> fp16 with the row's largest in [2^14, 2^15)
+            uint32_t top = 0;
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const float2 x = unpack2<true>(qf[q][i][h]);
+                top = max(top, max(finite_bits(x.x), finite_bits(x.y)));
+              }
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            int e = (int)(top >> 23) - 127 - 14;
+            e = e < -100 ? -100 : e;
+            const float inv = exp2i(-e);
+            fq = exp2i(e);
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const float2 x = unpack2<true>(qf[q][i][h]);
+                qf[q][i][h] = pack2c<false>(x.x * inv, x.y * inv);
+              }
+          }
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            factor[q][e] = sl2 * __shfl_sync(0xffffffffu, fq, (2 * t + e) * 4);
+            if constexpr (MULTI) {
+              const int rr = row0 + q * 8 + 2 * t + e, s = rr / group;
+              end[q][e] = rr < rows && s < cnt ? min(keys, max(0, len - cnt + s + 1)) : 0;
+            } else {
+              end[q][e] = keys;
+            }
+          }
+        }
+      }
       if (now) {
+        if (!__all_sync(0xffffffffu, mbar_wait(&landed[warp][use][0], use_phase, abort_flag, c.status, 81))) break;
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
-          if (row[i] < 0) gone |= 1u << i;
           float small[NQ][4] = {};
 #pragma unroll
           for (int q = 0; q < NQ; ++q)
@@ -371,8 +403,9 @@ paged_attend_kernel(const AttendArgs a, const Paged c, const AttendPlan plan) {
             for (int e = 0; e < 4; ++e) s[i][q][e] = 0.f;
 #pragma unroll
           for (int j = 0; j < KL; ++j) {
-            const uint32_t lo[4] = {kr[i][0][j].x, kr[i][0][j].y, kr[i][0][j].z, kr[i][0][j].w};
-            const uint32_t hi[4] = {kr[i][1][j].x, kr[i][1][j].y, kr[i][1][j].z, kr[i][1][j].w};
+            const uint8_t* x = sk + i * 16 * C::RB + (j >> 1) * 2048 + (k_at ^ (j & 1) * 64);
+            const uint4 klo = *reinterpret_cast<const uint4*>(x), khi = *reinterpret_cast<const uint4*>(x + 8 * C::BOX);
+            const uint32_t lo[4] = {klo.x, klo.y, klo.z, klo.w}, hi[4] = {khi.x, khi.y, khi.z, khi.w};
             if constexpr (C::F32) {
 #pragma unroll
               for (int q = 0; q < NQ; ++q) {
@@ -413,13 +446,19 @@ paged_attend_kernel(const AttendArgs a, const Paged c, const AttendPlan plan) {
           if constexpr (C::E8) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              ks[i][h] = __uint_as_float(__shfl_sync(0xffffffffu, sc[i], g + 8 * h) << 23);
-              ve[i][h] = (int)__shfl_sync(0xffffffffu, sc[i], 16 + g + 8 * h) - 127;
+              const uint8_t* e = powers + use * C::SB + i * 32 + gk + 8 * h;
+              const bool there = !(gone >> i & 1) && (ch * NS + i) * 16 + gk + 8 * h < keys;
+              ks[i][h] = __uint_as_float((uint32_t)e[0] << 23);
+              ve[i][h] = there ? (int)e[16] - 127 : -127;
             }
           }
         }
       }
+      __syncwarp();                    // all have read
       if (more) {
+        uint64_t* const bar = &landed[warp][put][0];
+        uint8_t* const dk = ring + put * 2 * C::KB;
+        int tiles = 0;
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
           row[i] = -1;
@@ -427,17 +466,20 @@ paged_attend_kernel(const AttendArgs a, const Paged c, const AttendPlan plan) {
             if ((unsigned)id[i] >= (unsigned)c.pages) { if (lane == 0) report_error(c.status, GB_ERR_BAD_INDEX, SITE_PAGE, id[i]); }
             else row[i] = ((long long)id[i] * c.Hkv + kvh) * c.page + place[i];
           }
-          const int left = row[i] < 0 ? 0 : keys - ((ch + 1) * NS + i) * 16;
-          const char* p = reinterpret_cast<const char*>(a.kpool) + (row[i] + g) * (D * C::ES) + t * 16;
+          if (row[i] < 0) gone_later |= 1u << (NS * (C::ST - 1) + i);
+          else ++tiles;
+        }
+        if (lane == 0) {
+          mbar_expect_tx(bar, tiles * (16 * C::RB + (C::E8 ? 32 : 0)));
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const char* pk = g + 8 * h < left ? p + 8 * h * (D * C::ES) : zeros;
+          for (int i = 0; i < NS; ++i) {
+            if (row[i] < 0) continue;
 #pragma unroll
-            for (int j = 0; j < KL; ++j) kr[i][h][j] = ld_stream16(pk + j * 64);
-          }
-          if constexpr (C::E8) {       // lanes 0 - 15: K's powers of two, 16 - 31: V's
-            sc[i] = 0;
-            if ((lane & 15) < left) sc[i] = (lane < 16 ? a.kscale : a.vscale)[row[i] + (lane & 15)];
+            for (int x = 0; x < C::RB / C::BOX; ++x) tma_load_2d(dk + i * 16 * C::RB + x * 2048, &tmk, bar, x * (C::BOX / C::ES), (int)row[i]);
+            if constexpr (C::E8) {
+              bulk_copy_16(smem_u32(powers) + put * C::SB + i * 32, a.kscale + row[i], bar);
+              bulk_copy_16(smem_u32(powers) + put * C::SB + i * 32 + 16, a.vscale + row[i], bar);
+            }
           }
         }
         ask();
@@ -462,7 +504,7 @@ paged_attend_kernel(const AttendArgs a, const Paged c, const AttendPlan plan) {
               for (int e = 0; e < 2; ++e) {
                 float& x = s[i][q][2 * h + e];
                 x *= C::E8 ? factor[q][e] * ks[i][h] : factor[q][e];
-                if (tail && ((gone >> i & 1) || (ch * NS + i) * 16 + g + 8 * h >= end[q][e])) x = -INFINITY;
+                if (tail && ((gone >> i & 1) || (ch * NS + i) * 16 + gk + 8 * h >= end[q][e])) x = -INFINITY;
                 top[q][e] = fmaxf(top[q][e], x);
               }
           }
@@ -536,47 +578,60 @@ paged_attend_kernel(const AttendArgs a, const Paged c, const AttendPlan plan) {
             }
           }
         // ---- O^T += V^T P^T -----------------------------------------------------------------------------------------
-        if constexpr (MULTI) {
-          // A key that one row sees and another does not is multiplied by a probability of 0 there, which an infinity or NaN
-          // among its values would turn into NaN.  They are left out here; the rows that see them get them at the end.
-          if (tail) {
-            uint32_t bad = 0;
+        constexpr int TW = C::E8 ? 2 : 1;              // tiles of O^T that a word of V has numbers of
+        alignas(16) uint32_t vr[NS][4][4];
+        uint32_t bad = 0;
+        if (!__all_sync(0xffffffffu, mbar_wait(&landed[warp][use][1], use_phase, abort_flag, c.status, 82))) break;
+#pragma unroll
+        for (int j = 0; j < VW; j += C::F32 ? 2 : 1) {
+          constexpr int VN = VW == 2 ? 2 : 4;         // words that a lane has of a key side by side
+          if (j % VN == 0) {
 #pragma unroll
             for (int i = 0; i < NS; ++i)
 #pragma unroll
-              for (int k = 0; k < 4; ++k)
+              for (int k = 0; k < 4; ++k) {
+                const uint8_t* x = sk + C::KB + i * 16 * C::RB + j / VN * 2048 + (k >> 1) * 8 * C::BOX + (k & 1 ? v_at ^ C::ODD_UNIT : v_at);
+                if constexpr (VN == 2) *reinterpret_cast<uint2*>(vr[i][k]) = *reinterpret_cast<const uint2*>(x);
+                else *reinterpret_cast<uint4*>(vr[i][k]) = *reinterpret_cast<const uint4*>(x);
+                // What stands behind the end of a sequence or in a tile that is not there is none of it.  With several tokens, a key
+                // that one row sees and another does not is multiplied by a probability of 0 there, which an infinity or NaN among
+                // its values would turn into NaN: those are left out here, and the rows that see them get them at the end.
+                if (tail) {
+                  const int key = (ch * NS + i) * 16 + (k >> 1) * 8 + (k & 1 ? C::first_key(t) ^ C::ODD_KEY : C::first_key(t));
+                  const bool there = !(gone >> i & 1) && key < keys;
 #pragma unroll
-                for (int j = 0; j < VW; ++j) {
-                  const uint32_t f = not_finite<C>(vr[i][k][j]);
-                  bad |= f;
-                  vr[i][k][j] &= ~f;
+                  for (int w = 0; w < VN; ++w) {
+                    if (!there) vr[i][k][w] = 0;
+                    if constexpr (MULTI) {
+                      const uint32_t f = not_finite<C>(vr[i][k][w]);
+                      bad |= f;
+                      vr[i][k][w] &= ~f;
+                    }
+                  }
                 }
-            if (__any_sync(0xffffffffu, bad != 0) && odd_from > ch) odd_from = ch;
+              }
           }
-        }
-        constexpr int TW = C::E8 ? 2 : 1;              // tiles of O^T that a word of V has numbers of
-#pragma unroll
-        for (int j = 0; j < VW; j += C::F32 ? 2 : 1) {
           float sum[TW][NQ][4] = {};
 #pragma unroll
           for (int i = 0; i < NS; ++i) {
             uint32_t v[TW * GP][4];
+            const int w = j % VN;
             if constexpr (C::F32) {
 #pragma unroll
               for (int k = 0; k < 2; ++k) {
-                v[k][0] = vr[i][2 * k][j]; v[k][1] = vr[i][2 * k][j + 1];
-                v[k][2] = vr[i][2 * k + 1][j]; v[k][3] = vr[i][2 * k + 1][j + 1];
+                v[k][0] = vr[i][2 * k][w]; v[k][1] = vr[i][2 * k][w + 1];
+                v[k][2] = vr[i][2 * k + 1][w]; v[k][3] = vr[i][2 * k + 1][w + 1];
               }
             } else if constexpr (!C::E8) {
-              v[0][0] = __byte_perm(vr[i][0][j], vr[i][1][j], 0x5410);
-              v[0][1] = __byte_perm(vr[i][0][j], vr[i][1][j], 0x7632);
-              v[0][2] = __byte_perm(vr[i][2][j], vr[i][3][j], 0x5410);
-              v[0][3] = __byte_perm(vr[i][2][j], vr[i][3][j], 0x7632);
+              v[0][0] = __byte_perm(vr[i][0][w], vr[i][1][w], 0x5410);
+              v[0][1] = __byte_perm(vr[i][0][w], vr[i][1][w], 0x7632);
+              v[0][2] = __byte_perm(vr[i][2][w], vr[i][3][w], 0x5410);
+              v[0][3] = __byte_perm(vr[i][2][w], vr[i][3][w], 0x7632);
             } else {
 #pragma unroll
               for (int h = 0; h < 2; ++h) {
-                e4m3x4_to_f16(__byte_perm(vr[i][0][j], vr[i][1][j], h ? 0x7362 : 0x5140), v[h][0], v[h][1]);
-                e4m3x4_to_f16(__byte_perm(vr[i][2][j], vr[i][3][j], h ? 0x7362 : 0x5140), v[h][2], v[h][3]);
+                e4m3x4_to_f16(__byte_perm(vr[i][0][w], vr[i][1][w], h ? 0x7362 : 0x5140), v[h][0], v[h][1]);
+                e4m3x4_to_f16(__byte_perm(vr[i][2][w], vr[i][3][w], h ? 0x7362 : 0x5140), v[h][2], v[h][3]);
               }
             }
 #pragma unroll
@@ -598,28 +653,41 @@ paged_attend_kernel(const AttendArgs a, const Paged c, const AttendPlan plan) {
                 for (int e = 0; e < 4; ++e) o[q][C::F32 ? j / 2 : j * TW + h][e] += sum[h][q][e];
           }
         }
-      }
-      if (more) {
-#pragma unroll
-        for (int i = 0; i < NS; ++i) {
-          const int left = row[i] < 0 ? 0 : keys - ((ch + 1) * NS + i) * 16;
-          const char* p = reinterpret_cast<const char*>(a.vpool) + (row[i] + C::first_key(t)) * (D * C::ES) + g * (VW == 2 ? 8 : 16);
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const char* pv = C::first_key(t) + C::key_step(k) < left ? p + C::key_step(k) * (D * C::ES) : zeros;
-            if constexpr (VW == 2) {
-              const uint2 v = ld_stream8(pv);
-              vr[i][k][0] = v.x; vr[i][k][1] = v.y;
-            } else {
-#pragma unroll
-              for (int j = 0; j < VW / 4; ++j) {
-                const uint4 v = ld_stream16(pv + 128 * j);
-                vr[i][k][4 * j] = v.x; vr[i][k][4 * j + 1] = v.y; vr[i][k][4 * j + 2] = v.z; vr[i][k][4 * j + 3] = v.w;
-              }
-            }
-          }
+        if constexpr (MULTI) {
+          if (tail && __any_sync(0xffffffffu, bad != 0) && odd_from > ch) odd_from = ch;
         }
       }
+      __syncwarp();
+      if (more) {
+        if (lane == 0) {
+          uint64_t* const bar = &landed[warp][put][1];
+          uint8_t* const dv = ring + put * 2 * C::KB + C::KB;
+          int tiles = 0;
+#pragma unroll
+          for (int i = 0; i < NS; ++i) tiles += row[i] >= 0;
+          mbar_expect_tx(bar, tiles * 16 * C::RB);
+#pragma unroll
+          for (int i = 0; i < NS; ++i) {
+            if (row[i] < 0) continue;
+#pragma unroll
+            for (int x = 0; x < C::RB / C::BOX; ++x) tma_load_2d(dv + i * 16 * C::RB + x * 2048, &tmv, bar, x * (C::BOX / C::ES), (int)row[i]);
+          }
+        }
+        if (++put == C::ST) { put = 0; put_phase ^= 1; }
+      }
+      if (now && ++use == C::ST) { use = 0; use_phase ^= 1; }
+    }
+    if (__any_sync(0xffffffffu, *abort_flag)) {      // gave up: the copies in flight land first, and nothing is kept
+      if (lane == 0) {
+        const uint64_t t0 = globaltimer_ns();
+        for (int i = 0; i < C::ST; ++i)
+          for (int w = 0; w < 2; ++w) {
+            const int phase = i < put ? put_phase : put_phase ^ 1;       // of the last copy into stage i
+            while (!mbar_try_wait(&landed[warp][i][w], phase) && globaltimer_ns() - t0 < 1000000ull) {}
+          }
+      }
+      __syncwarp();
+      break;
     }
 
     // ---- the run's result ---------------------------------------------------------------------------------------------
@@ -644,9 +712,13 @@ paged_attend_kernel(const AttendArgs a, const Paged c, const AttendPlan plan) {
         for (int w = 4; w < 32; w <<= 1) l[q][e] += __shfl_xor_sync(0xffffffffu, l[q][e], w);
     const bool whole = c0 == 0 && c1 == n;
     const int piece = 2 * warp + slot;
+    // a piece that ends the warp's share stays in its ring's place; one that others follow goes to the workspace
+    __syncwarp();
+    float* const sums = u + (c1 - c0) == u_end ? reinterpret_cast<float*>(ring) : plan.spill + ((size_t)cta * W + warp) * C::PIECE;
     if (!whole) {
       ++slot;
       if (lane == 0) {
+        piece_at[piece] = sums;
         piece_item[piece] = b * plan.per_seq + idx;
         piece_flags[piece] = (c0 == 0 ? 1 : 0) | (c1 == n ? 2 : 0);
         piece_start[piece] = seq_start + (unsigned)idx * n;
@@ -663,7 +735,7 @@ paged_attend_kernel(const AttendArgs a, const Paged c, const AttendPlan plan) {
         for (int i = 0; i < MT; i += 2) {
           const float4 v = make_float4(o[q][i][e] * unit, o[q][i][2 + e] * unit, o[q][i + 1][e] * unit, o[q][i + 1][2 + e] * unit);
           const int d = C::column(g, i);
-          if (!whole) *reinterpret_cast<float4*>(pieces + ((size_t)piece * R + r) * D + d) = v;
+          if (!whole) *reinterpret_cast<float4*>(sums + r * D + d) = v;
           else if (row0 + r < rows) store_row4<T>(a, c, b, kvh, row0 + r, d, v, l[q][e]);
         }
       }
@@ -685,7 +757,7 @@ paged_attend_kernel(const AttendArgs a, const Paged c, const AttendPlan plan) {
             if (!(fabsf(v) < INFINITY)) sum += v;
           }
           if (sum == 0.f) continue;
-          if (!whole) pieces[((size_t)piece * R + e / D) * D + d] = sum;
+          if (!whole) sums[e] = sum;
           else reinterpret_cast<T*>(a.o)[(((long long)b * c.S + s) * a.Hq + kvh * group + r % group) * D + d] = Cvt<T>::from_f(sum);
         }
       }
@@ -716,7 +788,7 @@ paged_attend_kernel(const AttendArgs a, const Paged c, const AttendPlan plan) {
       for (int k = p; k <= last; ++k) {
         if (piece_item[k] != item) continue;
         const float w = part_weight(piece_m[k][r], mc);
-        const float4 v = *reinterpret_cast<const float4*>(pieces + ((size_t)k * R + r) * D + d);
+        const float4 v = *reinterpret_cast<const float4*>(piece_at[k] + r * D + d);
         acc.x += w * v.x; acc.y += w * v.y; acc.z += w * v.z; acc.w += w * v.w;
         lc += w * piece_l[k][r];
       }
@@ -788,19 +860,36 @@ __global__ void __launch_bounds__(PJ_THREADS) paged_join_kernel(const AttendArgs
   }
 }
 
+// A pool's rows [pages * Hkv * page, D] in boxes of 16 rows and `box` bytes
+static int pool_map(CUtensorMap* out, const void* pool, const Paged& c, int cdt, int box) {
+  EncodeTiledFn4 enc = encode4();
+  if (enc == nullptr) return -1;
+  const int es = cdt == DT_E4M3 ? 1 : cdt == DT_F32 ? 4 : 2;
+  const cuuint64_t dims[2] = {(cuuint64_t)c.D, (cuuint64_t)c.pages * c.Hkv * c.page}, strides[1] = {(cuuint64_t)c.D * es};
+  const cuuint32_t boxes[2] = {(cuuint32_t)(box / es), 16}, steps[2] = {1, 1};
+  const CUtensorMapDataType type = cdt == DT_E4M3 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : cdt == DT_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                   : cdt == DT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  return (int)enc(out, type, 2, const_cast<void*>(pool), dims, strides, boxes, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  box == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+}
+
 template <typename T, int CDT, int D, int NQ, bool MULTI>
 static int launch_attend(const AttendArgs& a, const Paged& c, float* parts, int4* spans, int grid, cudaStream_t st) {
   using C = PA<T, CDT, D, NQ>;
   static unsigned long long cfg = 0;
   int r;
-  if (C::SMEM > 40 * 1024 && (r = smem_opt_in(paged_attend_kernel<T, CDT, D, NQ, MULTI>, C::SMEM, cfg)) != 0) return r;
+  if ((r = smem_opt_in(paged_attend_kernel<T, CDT, D, NQ, MULTI>, C::SMEM, cfg)) != 0) return r;
   AttendPlan plan;
   plan.tiles = (c.S * (a.Hq / c.Hkv) + C::R - 1) / C::R;
   plan.per_seq = plan.tiles * c.Hkv;
   plan.grid = grid;
   plan.parts = parts;
   plan.spans = spans;
-  paged_attend_kernel<T, CDT, D, NQ, MULTI><<<grid, PA_WARPS * 32, C::SMEM, st>>>(a, c, plan);
+  plan.spill = reinterpret_cast<float*>(spans + 2 * (size_t)grid);
+  CUtensorMap tmk, tmv;
+  if ((r = pool_map(&tmk, a.kpool, c, CDT, C::BOX)) != 0 || (r = pool_map(&tmv, a.vpool, c, CDT, C::BOX)) != 0) return 20000 + r;
+  paged_attend_kernel<T, CDT, D, NQ, MULTI><<<grid, PA_WARPS * 32, C::SMEM, st>>>(tmk, tmv, a, c, plan);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return (int)e;
   cudaLaunchConfig_t lc{};
@@ -886,23 +975,23 @@ static int attend_rows(int rows, int D, int cdt) { return rows <= 8 || (cdt == D
 
 // Which kernel a call takes, and its CTAs (0: a CTA for every row).  The tensor cores take heads of 64 or 128 over caches of the
 // queries' type, or of 8 bits below 16-bit queries; what remains (other head sizes, types that differ, more than 2^31 chunks of
-// keys) is worked on number by number.
-static int attend_grid(int B, int S, int Hq, int Hkv, int D, int page, int per, int dt, int cdt) {
+// keys or rows of the pool) is worked on number by number.
+static int attend_grid(int B, int S, int Hq, int Hkv, int D, int page, int pages, int per, int dt, int cdt) {
   if ((D != 64 && D != 128) || (cdt != dt && !(cdt == DT_E4M3 && dt != DT_F32)) || page % 16) return 0;
   const int rows = S * (Hq / Hkv), R = attend_rows(rows, D, cdt);
   const int es = cdt == DT_E4M3 ? 1 : cdt == DT_F32 ? 4 : 2, kt = attend_chunk(D, es);
   const long long tiles = (rows + R - 1) / R, keys = (long long)per * page;
   const long long chunks = (long long)B * Hkv * tiles * (keys <= 0 ? 1 : (keys + kt - 1) / kt);
-  if (chunks > 0x7fffffff) return 0;       // (counted in 32 bits)
-  const long long want = (chunks + PA_WARPS - 1) / PA_WARPS, most = (long long)sm_count() * (R == 8 && !(cdt == DT_F32 && D == 128) ? 3 : 2);
+  if (chunks > 0x7fffffff || (long long)pages * Hkv * page > 0x7fffffff) return 0;       // (counted in 32 bits)
+  const long long want = (chunks + PA_WARPS - 1) / PA_WARPS, most = (long long)sm_count() * 3;
   return (int)(want < most ? want : most);
 }
 
 // 32-bit words of workspace that a call needs
-extern "C" int gb_paged_attention_workspace(int B, int S, int Hq, int Hkv, int D, int page, int per, int dt, int cdt) {
+extern "C" int gb_paged_attention_workspace(int B, int S, int Hq, int Hkv, int D, int page, int pages, int per, int dt, int cdt) {
   if (B <= 0 || S <= 0 || Hq <= 0 || Hkv <= 0) return 0;
   const int R = attend_rows(S * (Hq / Hkv), D, cdt);
-  return attend_grid(B, S, Hq, Hkv, D, page, per, dt, cdt) * 2 * (R * (D + 2) + 4);
+  return attend_grid(B, S, Hq, Hkv, D, page, pages, per, dt, cdt) * (2 * (R * (D + 2) + 4) + PA_WARPS * R * D);
 }
 
 extern "C" int gb_paged_attention(const void* q, void* o, const void* kpool, const void* vpool, const void* kscale,
@@ -915,7 +1004,7 @@ extern "C" int gb_paged_attention(const void* q, void* o, const void* kpool, con
   Paged c{table, lengths, counts, status, B, S, Hkv, D, page, pages, per};
   const long long rows = (long long)B * S * Hq;
   if (rows > 0x7fffffff) return -4;
-  const int grid = attend_grid(B, S, Hq, Hkv, D, page, per, dt, cdt);
+  const int grid = attend_grid(B, S, Hq, Hkv, D, page, pages, per, dt, cdt);
   if (grid > 0) {
     const int R = attend_rows(S * (Hq / Hkv), D, cdt);
     int4* spans = reinterpret_cast<int4*>(workspace + (size_t)grid * 2 * R * (D + 2));

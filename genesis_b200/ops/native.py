@@ -77,7 +77,7 @@ _SIGS = {
     "gb_paged_put": "plll" * 3 + "ppp" + "i" + "pppp" + "ppp" + "iiiiiiii" + "ii" + "pp",
     "gb_paged_read": "pppp" + "pp" + "pp" + "iiiiiii" + "ii" + "pp",
     "gb_paged_attention": "pppppp" + "ppp" + "iiiiiiii" + "f" + "ii" + "ppp",
-    "gb_paged_attention_workspace": "iiiiiiiii",
+    "gb_paged_attention_workspace": "iiiiiiiiii",
     "gb_newton_schulz": "pp" + "iiiii" + "pi" + "pi" + "d" + "p" + "fff" + "pp" + "pp" + "p",
 }
 

@@ -215,7 +215,7 @@ def attention(q, layer, table, lengths, counts, scale):
         q = q.clone(memory_format=torch.contiguous_format)
     out = torch.empty_like(q)
     with N._on(dev):
-        words = _workspace(index, B, S, Hq, Hkv, D, page, per, dt, cdt)
+        words = _workspace(index, B, S, Hq, Hkv, D, page, pages, per, dt, cdt)
         work = torch.empty(words, dtype=torch.float32, device=dev) if words else None
         N._chk(N.lib().gb_paged_attention(q.data_ptr(), out.data_ptr(), kp, vp, ks, vs, table.data_ptr(), lengths.data_ptr(),
                                           N._ptr(counts), B, S, Hq, Hkv, D, page, pages, per, scale, dt, cdt, N._ptr(work),
