@@ -38,11 +38,23 @@ struct AttendArgs {
 
 constexpr int PA_WARPS = 4, PA_MAX_D = 256;
 
+// n / d for n < 2^31: a division by a number that the host knows is a multiplication (a run of chunks begins with half a dozen)
+struct Div {
+  unsigned mul, shift, d;
+  explicit Div(unsigned x = 1) : d(x) {
+    shift = 0;
+    while (1ull << shift < x) ++shift;
+    mul = (unsigned)(((1ull << 32) * ((1ull << shift) - x)) / x + 1);
+  }
+  __device__ __forceinline__ int by(int n) const { return (int)((__umulhi(mul, (unsigned)n) + (unsigned)n) >> shift); }
+};
+
 // The chunks of all items: items[b] = n(b) * per_seq, in the order of b, then KV head and row tile.
 struct AttendPlan {
   int per_seq;          // items of a sequence: Hkv * row tiles
   int tiles;            // row tiles
   int grid;             // CTAs launched
+  Div seq, tile, group, page;      // by per_seq, tiles, Hq / Hkv, tiles of keys in a page
   float* parts;         // [grid][2][R][D] sums, then [grid][2][R] maxima and normalisers: of an item that comes from the CTA before,
                         // and of one that begins in the CTA and goes on behind it
   float* spill;         // [grid][PA_WARPS][R][D] sums: pieces that a warp leaves behind before it goes on
@@ -53,14 +65,22 @@ struct AttendPlan {
 // 64 x 4096, 2 KV heads of 64: 36.2 us with four, 33.6 with two; one tile of 128: 71.7 us for 70.1 over 4 KV heads).
 static constexpr int attend_chunk(int D, int bytes) { return 4096 / (D * bytes) < 16 ? 16 : 4096 / (D * bytes) > 32 ? 32 : 4096 / (D * bytes); }
 
-// Chunks in flight of a warp: 16 KB of them (15 of 8 bits and 64), with three CTAs on an SM.
-static constexpr int attend_stages(int D, int bytes) { return D * bytes == 512 ? 1 : D * bytes == 64 ? 3 : 2; }
+// CTAs on an SM, by registers: four, three where numbers are split in two or added up apart, two for two operands of rows over 128
+// numbers of 8 bits.  Chunks in flight of a warp, by what shared memory is left; one where registers are spilled, which need the
+// L1 that a larger ring takes (32 sequences of 4096, drafts of 4: 143 us with two, 93 with one).
+static constexpr int attend_ctas(int dt, int cdt, int D, int R) {
+  return R == 16 ? (cdt == DT_E4M3 && D == 128 ? 2 : 3) : cdt == DT_F32 || (cdt == DT_E4M3 && dt == DT_F16) ? 3 : 4;
+}
+static constexpr int attend_stages(int dt, int cdt, int D, int R) {
+  return cdt == DT_E4M3 && D == 64 ? 3 : (cdt == DT_F32 && D == 128) || (R == 16 && cdt != DT_E4M3) ? 1 : 5 - attend_ctas(dt, cdt, D, R);
+}
 
 template <typename T, int CDT, int D_, int NQ_>
 struct PA {
   static constexpr int D = D_, NQ = NQ_, R = 8 * NQ;
   static constexpr bool E8 = CDT == DT_E4M3, BF = CDT == DT_BF16, F32 = CDT == DT_F32;
   static constexpr bool OBF = std::is_same<T, __nv_bfloat16>::value;
+  static constexpr int DT = F32 ? DT_F32 : OBF ? DT_BF16 : DT_F16;
   static constexpr bool SPLIT = !(E8 && OBF);           // P in two numbers
   // The tensor cores cut sums off towards zero (2^-24 of them a step on average).  Over thousands of steps that would show in an
   // output of 11 bits and more, so there a chunk's products are added up apart and then to the accumulators, rounded.
@@ -76,10 +96,10 @@ struct PA {
   static constexpr int PIECE = R * D;
   static constexpr int RB = D * ES, BOX = RB < 128 ? RB : 128;      // bytes of a row, and of a column of the ring's boxes
   static constexpr int KB = KT * RB, SB = E8 ? NS * 32 : 0;          // a stage: K, V; powers of two (behind all rings)
-  static constexpr int ST = attend_stages(D, ES), RING = ST * 2 * KB;
+  static constexpr int ST = attend_stages(DT, CDT, D, R), RING = ST * 2 * KB;
   static constexpr int SMEM = PA_WARPS * (RING + ST * SB) + 1024;   // (boxes start on 1024 bytes)
   static_assert(PIECE * 4 <= RING, "a warp's last piece takes its ring's place");
-  static constexpr int CTAS = 3;                        // on an SM
+  static constexpr int CTAS = attend_ctas(DT, CDT, D, R);
   // first of the two columns d that a lane has of tile mt
   static __device__ __forceinline__ int column(int g, int mt) {
     if (E8) return g * (D / 8) + mt * 2;
@@ -184,10 +204,10 @@ __device__ __forceinline__ int attend_chunks(int keys, int kt) { return keys == 
 
 // o / l of row r (0 .. S * group - 1) of a group, 4 columns from d on
 template <typename T>
-__device__ __forceinline__ void store_row4(const AttendArgs& a, const Paged& c, int b, int kvh, int r, int d, float4 o, float l) {
-  const int group = a.Hq / c.Hkv;
+__device__ __forceinline__ void store_row4(const AttendArgs& a, const Paged& c, const Div& group, int b, int kvh, int r, int d, float4 o, float l) {
+  const int s = group.by(r);
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  T* p = reinterpret_cast<T*>(a.o) + (((long long)b * c.S + r / group) * a.Hq + kvh * group + r % group) * c.D + d;
+  T* p = reinterpret_cast<T*>(a.o) + (((long long)b * c.S + s) * a.Hq + kvh * group.d + r - s * group.d) * c.D + d;
   if constexpr (std::is_same<T, float>::value) {
     *reinterpret_cast<float4*>(p) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
   } else {
@@ -205,19 +225,26 @@ paged_attend_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_consta
   constexpr int R = C::R, KT = C::KT, NS = C::NS, KL = C::KL, VW = C::VW, MT = C::MT, QS = C::QS, GP = C::GP, W = PA_WARPS;
   extern __shared__ __align__(1024) uint8_t shared[];              // [W][RING], [W][ST][SB]
   __shared__ uint64_t landed[W][C::ST][2];                           // K's and V's copies of a stage have landed
-  __shared__ int abort_word;
-  volatile int* const abort_flag = &abort_word;
+  __shared__ int abort_word[W];
   uint8_t* const rings = shared + (1024 - (smem_u32(shared) & 1023)) % 1024;
   __shared__ const float* piece_at[2 * W];                         // [R][D] sums: in the ring of the warp, or in the workspace
   __shared__ float piece_m[2 * W][R], piece_l[2 * W][R];
   __shared__ int piece_item[2 * W], piece_flags[2 * W];
-  __shared__ unsigned piece_start[2 * W], piece_end[2 * W], scan[W], first_chunk[W];
-  __shared__ int first_b[W];
+  __shared__ unsigned piece_start[2 * W], piece_end[2 * W];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");       // (the join waits for the end of this kernel)
 
-  // ---- the share of this warp -----------------------------------------------------------------------------------------
-  const int each = (c.B + W * 32 - 1) / (W * 32), b0 = min(c.B, (int)threadIdx.x * each), b1 = min(c.B, b0 + each);
+  // ---- the share of this warp: every warp finds it by itself ----------------------------------------------------------------
+  if (lane < 2) piece_item[2 * warp + lane] = -1;
+  if (lane == 0) {
+    abort_word[warp] = 0;
+    for (int i = 0; i < C::ST * 2; ++i) mbar_init(&landed[warp][0][0] + i, 1);
+    mbar_fence_init();
+    tma_prefetch_desc(&tmk);
+    tma_prefetch_desc(&tmv);
+  }
+  __syncwarp();
+  const int each = (c.B + 31) / 32, b0 = min(c.B, lane * each), b1 = min(c.B, b0 + each);
   unsigned mine = 0;                   // (the host has seen to it that all chunks are less than 2^31)
   for (int b = b0; b < b1; ++b) mine += attend_chunks(attend_keys(c, b), KT);
   mine *= plan.per_seq;
@@ -227,22 +254,7 @@ paged_attend_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_consta
     const unsigned x = __shfl_up_sync(0xffffffffu, upto, o);
     if (lane >= o) upto += x;
   }
-  if (lane == 31) scan[warp] = upto;
-  if (threadIdx.x < 2 * W) piece_item[threadIdx.x] = -1;
-  if (threadIdx.x == 0) {
-    abort_word = 0;
-    for (int i = 0; i < W * C::ST * 2; ++i) mbar_init(&landed[0][0][0] + i, 1);
-    mbar_fence_init();
-    tma_prefetch_desc(&tmk);
-    tma_prefetch_desc(&tmv);
-  }
-  __syncthreads();
-  unsigned total = 0;
-#pragma unroll
-  for (int w = 0; w < W; ++w) {
-    if (w < warp) upto += scan[w];
-    total += scan[w];
-  }
+  const unsigned total = __shfl_sync(0xffffffffu, upto, 31);
   // the first `rest` warps have a chunk more than the others
   const int cta = blockIdx.x, ctas = min((unsigned)plan.grid, (total + W - 1) / W);
   const unsigned workers = ctas * W, share = total / workers, rest = total - share * workers;
@@ -255,48 +267,36 @@ paged_attend_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_consta
     if (threadIdx.x < 2) plan.spans[2 * cta + threadIdx.x] = make_int4(-1, 0, 0, 0);
     return;
   }
-#pragma unroll
-  for (int w = 0; w < W; ++w) {
-    const unsigned u = start_of(cta * W + w);
-    if (u >= upto - mine && u < upto) {
-      unsigned at = upto - mine;
-      int b = b0;
-      for (;; ++b) {
-        const unsigned n = (unsigned)attend_chunks(attend_keys(c, b), KT) * plan.per_seq;
-        if (u < at + n) break;
-        at += n;
-      }
-      first_b[w] = b;
-      first_chunk[w] = at;
-    }
-  }
-  __syncthreads();
   unsigned u = start_of(cta * W + warp);
   const unsigned u_end = start_of(cta * W + warp + 1);
-  int b = first_b[warp];
-  unsigned seq_start = first_chunk[warp];
+  // the sequence that it begins in (a warp without a share finds one too, or sequence 0)
+  const int owner = max(0, __ffs(__ballot_sync(0xffffffffu, u < upto)) - 1);
+  int b = owner * each;
+  unsigned seq_start = __shfl_sync(0xffffffffu, upto - mine, owner);
   int slot = 0;
   const int k_at = C::k_unit(g, t), v_at = C::v_unit(g, t), gk = C::key_of(g);
+  volatile int* const abort_flag = &abort_word[warp];
   uint8_t* const ring = rings + warp * C::RING;
   uint8_t* const powers = rings + W * C::RING + warp * C::ST * C::SB;
   int put = 0, put_phase = 0, use = 0, use_phase = 0;              // stage of the next chunk that is copied and of the one that is worked on
   const float sl2 = a.scale * 1.4426950408889634f;
-  const int group = a.Hq / c.Hkv, rows = c.S * group, tpp = c.page / 16;
+  const int rows = c.S * plan.group.d;
 
   while (u < u_end) {
     // ---- an item's run of chunks ------------------------------------------------------------------------------------
     const int keys = attend_keys(c, b), n = attend_chunks(keys, KT);
-    const int idx = (int)((u - seq_start) / (unsigned)n);
-    if (idx >= plan.per_seq) { seq_start += (unsigned)n * plan.per_seq; ++b; continue; }
+    if (u - seq_start >= (unsigned)n * plan.per_seq) { seq_start += (unsigned)n * plan.per_seq; ++b; continue; }
+    const int idx = plan.per_seq == 1 ? 0 : (int)((u - seq_start) / (unsigned)n);
     const int c0 = (int)(u - seq_start - (unsigned)idx * n);
     const int c1 = min(n, c0 + (int)(u_end - u));
-    const int kvh = idx / plan.tiles, row0 = idx % plan.tiles * R;
+    const int kvh = plan.tile.by(idx), row0 = (idx - kvh * plan.tiles) * R;
     const int cnt = c.count(b), len = c.length(b);
     if (len > keys && cnt > 0 && c0 == 0 && lane == 0) report_error(c.status, GB_ERR_BAD_INDEX, SITE_POSITION, len - 1);
 
     // ---- copies -----------------------------------------------------------------------------------------------------
     const int* pages = c.table + (size_t)b * c.per;
-    int tile = c0 * NS, pg = tile / tpp, sub = tile - pg * tpp;            // the next tile whose page is asked for
+    const int tpp = plan.page.d;
+    int tile = c0 * NS, pg = plan.page.by(tile), sub = tile - pg * tpp;    // the next tile whose page is asked for
     int id[NS], place[NS];
     auto ask = [&]() {
 #pragma unroll
@@ -312,8 +312,8 @@ paged_attend_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_consta
     uint32_t qf[NQ][QS][2];
 #pragma unroll
     for (int q = 0; q < NQ; ++q) {
-      const int r = row0 + q * 8 + g;
-      const T* p = reinterpret_cast<const T*>(a.q) + (((long long)b * c.S + (r < rows ? r / group : 0)) * a.Hq + kvh * group + (r < rows ? r % group : 0)) * D;
+      const int r = row0 + q * 8 + g, s = plan.group.by(r);
+      const T* p = reinterpret_cast<const T*>(a.q) + (((long long)b * c.S + s) * a.Hq + kvh * plan.group.d + r - s * plan.group.d) * D;
       constexpr int H = C::E8 ? 2 : 1, E = 16 / sizeof(T);     // 16-byte loads that go with one of a key's row, numbers of each
 #pragma unroll
       for (int i = 0; i < KL * H; ++i) {
@@ -338,7 +338,7 @@ paged_attend_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_consta
       for (int e = 0; e < 2; ++e) { m[q][e] = -INFINITY; off[q][e] = 0.f; l[q][e] = 0.f; }
     }
     constexpr float LIFT = !C::E8 && !C::BF && !C::F32 ? 7.f : 0.f;      // fp16 P without a scale of its own
-    int vtop = -1000;                  // the power of two of V that the accumulators are relative to
+    int vtop = -1000;                  // the power of two of V that the accumulators are relative to, as stored
     int odd_from = 0x7fffffff;         // the first chunk with values left out
     const int full = MULTI ? min(keys, max(0, len - cnt + 1)) : keys;      // keys that every token sees
 
@@ -384,7 +384,7 @@ paged_attend_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_consta
           for (int e = 0; e < 2; ++e) {
             factor[q][e] = sl2 * __shfl_sync(0xffffffffu, fq, (2 * t + e) * 4);
             if constexpr (MULTI) {
-              const int rr = row0 + q * 8 + 2 * t + e, s = rr / group;
+              const int rr = row0 + q * 8 + 2 * t + e, s = plan.group.by(rr);
               end[q][e] = rr < rows && s < cnt ? min(keys, max(0, len - cnt + s + 1)) : 0;
             } else {
               end[q][e] = keys;
@@ -447,9 +447,8 @@ paged_attend_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_consta
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               const uint8_t* e = powers + use * C::SB + i * 32 + gk + 8 * h;
-              const bool there = !(gone >> i & 1) && (ch * NS + i) * 16 + gk + 8 * h < keys;
               ks[i][h] = __uint_as_float((uint32_t)e[0] << 23);
-              ve[i][h] = there ? (int)e[16] - 127 : -127;
+              ve[i][h] = e[16];
             }
           }
         }
@@ -486,39 +485,50 @@ paged_attend_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_consta
       }
       if (now) {
         // ---- probabilities ------------------------------------------------------------------------------------------
-        float top[NQ][2];
-#pragma unroll
-        for (int q = 0; q < NQ; ++q)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) top[q][e] = -INFINITY;
-        bool grow = false;
         const bool tail = gone != 0 || (ch + 1) * KT > full;
 #pragma unroll
         for (int i = 0; i < NS; ++i)
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            if constexpr (C::E8) grow |= ve[i][h] > vtop;
+          for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int q = 0; q < NQ; ++q)
 #pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                float& x = s[i][q][2 * h + e];
-                x *= C::E8 ? factor[q][e] * ks[i][h] : factor[q][e];
-                if (tail && ((gone >> i & 1) || (ch * NS + i) * 16 + gk + 8 * h >= end[q][e])) x = -INFINITY;
-                top[q][e] = fmaxf(top[q][e], x);
-              }
-          }
+              for (int e = 0; e < 2; ++e) s[i][q][2 * h + e] *= C::E8 ? factor[q][e] * ks[i][h] : factor[q][e];
+        if (tail) {
+#pragma unroll
+          for (int i = 0; i < NS; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const int key = gone >> i & 1 ? 0x7fffffff : (ch * NS + i) * 16 + gk + 8 * h;
+              if (C::E8 && key >= keys) ve[i][h] = 0;
+#pragma unroll
+              for (int q = 0; q < NQ; ++q)
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                  if (key >= end[q][e]) s[i][q][2 * h + e] = -INFINITY;
+            }
+        }
+        float top[NQ][2];
+        bool grow = false;
 #pragma unroll
         for (int q = 0; q < NQ; ++q)
 #pragma unroll
-          for (int e = 0; e < 2; ++e) grow |= top[q][e] > m[q][e] + 8.f;
+          for (int e = 0; e < 2; ++e) {
+            top[q][e] = fmaxf(s[0][q][e], s[0][q][2 + e]);
+#pragma unroll
+            for (int i = 1; i < NS; ++i) top[q][e] = fmaxf(top[q][e], fmaxf(s[i][q][e], s[i][q][2 + e]));
+            grow |= top[q][e] > m[q][e] + 8.f;
+          }
+        int power = 0;                 // V's largest power of two here, as stored
+        if constexpr (C::E8) {
+#pragma unroll
+          for (int i = 0; i < NS; ++i) power = max(power, max(ve[i][0], ve[i][1]));
+          grow |= power > vtop;
+        }
         if (__any_sync(0xffffffffu, grow)) {
           float vscale = 1.f;
           if constexpr (C::E8) {
-            int e = vtop;
-#pragma unroll
-            for (int i = 0; i < NS; ++i) e = max(e, max(ve[i][0], ve[i][1]));
-            e = __reduce_max_sync(0xffffffffu, e);
+            const int e = __reduce_max_sync(0xffffffffu, max(power, vtop));
             vscale = vtop - e < -126 ? 0.f : exp2i(vtop - e);
             vtop = e;
           }
@@ -553,7 +563,7 @@ paged_attend_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_consta
         for (int i = 0; i < NS; ++i)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const float vs = C::E8 ? exp2i(max(ve[i][h] - vtop + 7, -126)) : 1.f;
+            const float vs = C::E8 ? __uint_as_float((uint32_t)max(ve[i][h] - vtop + 134, 1) << 23) : 1.f;
 #pragma unroll
             for (int q = 0; q < NQ; ++q) {
               float p[2];
@@ -593,10 +603,15 @@ paged_attend_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_consta
                 const uint8_t* x = sk + C::KB + i * 16 * C::RB + j / VN * 2048 + (k >> 1) * 8 * C::BOX + (k & 1 ? v_at ^ C::ODD_UNIT : v_at);
                 if constexpr (VN == 2) *reinterpret_cast<uint2*>(vr[i][k]) = *reinterpret_cast<const uint2*>(x);
                 else *reinterpret_cast<uint4*>(vr[i][k]) = *reinterpret_cast<const uint4*>(x);
-                // What stands behind the end of a sequence or in a tile that is not there is none of it.  With several tokens, a key
-                // that one row sees and another does not is multiplied by a probability of 0 there, which an infinity or NaN among
-                // its values would turn into NaN: those are left out here, and the rows that see them get them at the end.
-                if (tail) {
+              }
+            // What stands behind the end of a sequence or in a tile that is not there is none of it.  With several tokens, a key that
+            // one row sees and another does not is multiplied by a probability of 0 there, which an infinity or NaN among its values
+            // would turn into NaN: those are left out here, and the rows that see them get them at the end.
+            if (tail) {
+#pragma unroll
+              for (int i = 0; i < NS; ++i)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
                   const int key = (ch * NS + i) * 16 + (k >> 1) * 8 + (k & 1 ? C::first_key(t) ^ C::ODD_KEY : C::first_key(t));
                   const bool there = !(gone >> i & 1) && key < keys;
 #pragma unroll
@@ -609,7 +624,7 @@ paged_attend_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_consta
                     }
                   }
                 }
-              }
+            }
           }
           float sum[TW][NQ][4] = {};
 #pragma unroll
@@ -691,7 +706,7 @@ paged_attend_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_consta
     }
 
     // ---- the run's result ---------------------------------------------------------------------------------------------
-    const float unit = C::E8 ? (vtop - 7 < -126 ? 0.f : exp2i(vtop - 7)) : 1.f;
+    const float unit = C::E8 ? (vtop < 8 ? 0.f : exp2i(vtop - 134)) : 1.f;
     if constexpr (MULTI) {             // rows that are no tokens (chunks that all tokens see are not masked)
 #pragma unroll
       for (int q = 0; q < NQ; ++q)
@@ -736,14 +751,14 @@ paged_attend_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_consta
           const float4 v = make_float4(o[q][i][e] * unit, o[q][i][2 + e] * unit, o[q][i + 1][e] * unit, o[q][i + 1][2 + e] * unit);
           const int d = C::column(g, i);
           if (!whole) *reinterpret_cast<float4*>(sums + r * D + d) = v;
-          else if (row0 + r < rows) store_row4<T>(a, c, b, kvh, row0 + r, d, v, l[q][e]);
+          else if (row0 + r < rows) store_row4<T>(a, c, plan.group, b, kvh, row0 + r, d, v, l[q][e]);
         }
       }
     if constexpr (MULTI) {
       if (odd_from < c1) {             // infinities and NaN among the values from there on, to the rows that see them
         __syncwarp();
         for (int e = lane; e < R * D; e += 32) {
-          const int r = row0 + e / D, d = e % D, s = r / group;
+          const int r = row0 + e / D, d = e % D, s = plan.group.by(r);
           if (r >= rows || s >= cnt) continue;
           const int stop = min(c1 * KT, min(keys, max(0, len - cnt + s + 1)));
           float sum = 0.f;
@@ -758,7 +773,7 @@ paged_attend_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_consta
           }
           if (sum == 0.f) continue;
           if (!whole) sums[e] = sum;
-          else reinterpret_cast<T*>(a.o)[(((long long)b * c.S + s) * a.Hq + kvh * group + r % group) * D + d] = Cvt<T>::from_f(sum);
+          else reinterpret_cast<T*>(a.o)[(((long long)b * c.S + s) * a.Hq + kvh * plan.group.d + r - s * plan.group.d) * D + d] = Cvt<T>::from_f(sum);
         }
       }
     }
@@ -777,7 +792,7 @@ paged_attend_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_consta
       else if (piece_item[k] >= 0) break;
     }
     const bool begins = piece_flags[p] & 1, ends = piece_flags[last] & 2;
-    const int bb = item / plan.per_seq, idx = item % plan.per_seq, kvh = idx / plan.tiles, row0 = idx % plan.tiles * R;
+    const int bb = plan.seq.by(item), idx = item - bb * plan.per_seq, kvh = plan.tile.by(idx), row0 = (idx - kvh * plan.tiles) * R;
     const size_t part = (size_t)cta * 2 + (begins ? 1 : 0);
     for (int e = threadIdx.x; e < R * D / 4; e += W * 32) {
       const int r = e / (D / 4), d = e % (D / 4) * 4;
@@ -793,7 +808,7 @@ paged_attend_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_consta
         lc += w * piece_l[k][r];
       }
       if (begins && ends) {
-        if (row0 + r < rows) store_row4<T>(a, c, bb, kvh, row0 + r, d, acc, lc);
+        if (row0 + r < rows) store_row4<T>(a, c, plan.group, bb, kvh, row0 + r, d, acc, lc);
       } else {
         *reinterpret_cast<float4*>(plan.parts + (part * R + r) * D + d) = acc;
         if (d == 0) {
@@ -828,8 +843,8 @@ __global__ void __launch_bounds__(PJ_THREADS) paged_join_kernel(const AttendArgs
     const int4 span = plan.spans[2 * cta + which];
     if (span.x < 0) continue;
     const int first = span.y, parts = span.z - first + 1;
-    const int b = span.x / plan.per_seq, idx = span.x % plan.per_seq, kvh = idx / plan.tiles, row0 = idx % plan.tiles * R;
-    const int slots = min(R, c.S * (a.Hq / c.Hkv) - row0) * (D / 4), each = (slots + parts - 1) / parts, s0 = (cta - first) * each;
+    const int b = plan.seq.by(span.x), idx = span.x - b * plan.per_seq, kvh = plan.tile.by(idx), row0 = (idx - kvh * plan.tiles) * R;
+    const int slots = min(R, c.S * (int)plan.group.d - row0) * (D / 4), each = (slots + parts - 1) / parts, s0 = (cta - first) * each;
     const int mine = min(each, slots - s0);
     if (mine <= 0) continue;
     const int P = mine <= 1 ? 1 : 1 << (32 - __clz(mine - 1)), G = PJ_THREADS / P;
@@ -856,7 +871,7 @@ __global__ void __launch_bounds__(PJ_THREADS) paged_join_kernel(const AttendArgs
       __syncthreads();
       if (group < h) merge(stat[tid + h * P], sum[tid + h * P]);
     }
-    if (group == 0 && slot < mine) store_row4<T>(a, c, b, kvh, row0 + r, d, acc, l);
+    if (group == 0 && slot < mine) store_row4<T>(a, c, plan.group, b, kvh, row0 + r, d, acc, l);
   }
 }
 
@@ -884,6 +899,10 @@ static int launch_attend(const AttendArgs& a, const Paged& c, float* parts, int4
   plan.tiles = (c.S * (a.Hq / c.Hkv) + C::R - 1) / C::R;
   plan.per_seq = plan.tiles * c.Hkv;
   plan.grid = grid;
+  plan.seq = Div(plan.per_seq);
+  plan.tile = Div(plan.tiles);
+  plan.group = Div(a.Hq / c.Hkv);
+  plan.page = Div(c.page / 16);
   plan.parts = parts;
   plan.spans = spans;
   plan.spill = reinterpret_cast<float*>(spans + 2 * (size_t)grid);
@@ -983,7 +1002,7 @@ static int attend_grid(int B, int S, int Hq, int Hkv, int D, int page, int pages
   const long long tiles = (rows + R - 1) / R, keys = (long long)per * page;
   const long long chunks = (long long)B * Hkv * tiles * (keys <= 0 ? 1 : (keys + kt - 1) / kt);
   if (chunks > 0x7fffffff || (long long)pages * Hkv * page > 0x7fffffff) return 0;       // (counted in 32 bits)
-  const long long want = (chunks + PA_WARPS - 1) / PA_WARPS, most = (long long)sm_count() * 3;
+  const long long want = (chunks + PA_WARPS - 1) / PA_WARPS, most = (long long)sm_count() * attend_ctas(dt, cdt, D, R);
   return (int)(want < most ? want : most);
 }
 
