@@ -924,20 +924,24 @@ static int launch_attend(const AttendArgs& a, const Paged& c, float* parts, int4
   return e != cudaSuccess ? (int)e : (int)cudaGetLastError();
 }
 
-// Any type and head size: a CTA takes a row of queries, its warps every fourth key, their lanes a share of the head.
+// Any type and head size: a CTA takes a row of queries and one of `splits` runs of keys, its warps every fourth key, their lanes a
+// share of the head.  Runs are joined below.
 template <typename T, int CDT>
-__global__ void __launch_bounds__(PA_WARPS * 32) paged_attend_any_kernel(const AttendArgs a, const Paged c) {
+__global__ void __launch_bounds__(PA_WARPS * 32) paged_attend_any_kernel(const AttendArgs a, const Paged c, int splits, float* parts) {
   constexpr int N = PA_MAX_D / 32;
   __shared__ float sm_o[PA_WARPS][PA_MAX_D], sm_m[PA_WARPS], sm_l[PA_WARPS];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int h = blockIdx.x % a.Hq, s = blockIdx.x / a.Hq % c.S, b = blockIdx.x / a.Hq / c.S;
+  const int line = blockIdx.x / splits, split = blockIdx.x - line * splits;
+  const int h = line % a.Hq, s = line / a.Hq % c.S, b = line / a.Hq / c.S;
   const int kvh = h / (a.Hq / c.Hkv), n = c.count(b);
   long long end = s < n ? (long long)c.length(b) - n + s + 1 : 0;
   if (end > c.capacity()) {
-    if (threadIdx.x == 0) report_error(c.status, GB_ERR_BAD_INDEX, SITE_POSITION, (int)end - 1);
+    if (threadIdx.x == 0 && split == 0) report_error(c.status, GB_ERR_BAD_INDEX, SITE_POSITION, (int)end - 1);
     end = c.capacity();
   }
-  const T* q = reinterpret_cast<const T*>(a.q) + (((long long)b * c.S + s) * a.Hq + h) * c.D;
+  const int from = (int)(end * split / splits);
+  end = end * (split + 1) / splits;
+  const T* q = reinterpret_cast<const T*>(a.q) + (long long)line * c.D;
   float qv[N], o[N], m = -INFINITY, l = 0.f;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
@@ -949,7 +953,7 @@ __global__ void __launch_bounds__(PA_WARPS * 32) paged_attend_any_kernel(const A
     if constexpr (CDT == DT_E4M3) return from_e4m3x2(reinterpret_cast<const uint8_t*>(pool)[e]).x;
     else return load_as_float(pool, CDT, e);
   };
-  for (int j = warp; j < end; j += PA_WARPS) {
+  for (int j = from + warp; j < end; j += PA_WARPS) {
     const long long row = c.row(b, j, kvh);
     if (row < 0) continue;
     float x = 0.f;
@@ -981,8 +985,37 @@ __global__ void __launch_bounds__(PA_WARPS * 32) paged_attend_any_kernel(const A
   for (int d = threadIdx.x; d < c.D; d += PA_WARPS * 32) {
     float acc = 0.f;
     for (int w = 0; w < PA_WARPS; ++w) acc += sm_o[w][d] * expf(sm_m[w] - base);
-    reinterpret_cast<T*>(a.o)[(((long long)b * c.S + s) * a.Hq + h) * c.D + d] = Cvt<T>::from_f(lc == 0.f ? 0.f : acc / lc);
+    if (splits > 1) parts[(size_t)blockIdx.x * (c.D + 2) + d] = acc;
+    else reinterpret_cast<T*>(a.o)[(long long)line * c.D + d] = Cvt<T>::from_f(lc == 0.f ? 0.f : acc / lc);
   }
+  if (splits > 1 && threadIdx.x == 0) {
+    parts[(size_t)blockIdx.x * (c.D + 2) + c.D] = mc;
+    parts[(size_t)blockIdx.x * (c.D + 2) + c.D + 1] = lc;
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(PA_WARPS * 32) paged_join_any_kernel(void* o, int D, int splits, const float* parts) {
+  const float* p = parts + (size_t)blockIdx.x * splits * (D + 2);
+  float m = -INFINITY;
+  for (int k = 0; k < splits; ++k) m = fmaxf(m, p[k * (D + 2) + D]);
+  const float base = m == -INFINITY ? 0.f : m;
+  for (int d = threadIdx.x; d < D; d += PA_WARPS * 32) {
+    float acc = 0.f, l = 0.f;
+    for (int k = 0; k < splits; ++k) {
+      const float w = expf(p[k * (D + 2) + D] - base);
+      acc += w * p[k * (D + 2) + d];
+      l += w * p[k * (D + 2) + D + 1];
+    }
+    reinterpret_cast<T*>(o)[(long long)blockIdx.x * D + d] = Cvt<T>::from_f(l == 0.f ? 0.f : acc / l);
+  }
+}
+
+// Runs of keys of the kernel for any type: until each SM has sixteen CTAs, of 64 keys at least.
+static int any_splits(long long rows, int page, int per) {
+  const long long keys = (long long)page * per, most = 16ll * sm_count() / (rows > 0 ? rows : 1);
+  const long long n = keys / 64 < most ? keys / 64 : most;
+  return n < 1 ? 1 : n > 256 ? 256 : (int)n;
 }
 
 }  // namespace gb
@@ -1010,6 +1043,11 @@ static int attend_grid(int B, int S, int Hq, int Hkv, int D, int page, int pages
 extern "C" int gb_paged_attention_workspace(int B, int S, int Hq, int Hkv, int D, int page, int pages, int per, int dt, int cdt) {
   if (B <= 0 || S <= 0 || Hq <= 0 || Hkv <= 0) return 0;
   const int R = attend_rows(S * (Hq / Hkv), D, cdt);
+  if (attend_grid(B, S, Hq, Hkv, D, page, pages, per, dt, cdt) == 0) {
+    const long long rows = (long long)B * S * Hq;
+    const int splits = any_splits(rows, page, per);
+    return splits == 1 ? 0 : (int)(rows * splits * (D + 2));
+  }
   return attend_grid(B, S, Hq, Hkv, D, page, pages, per, dt, cdt) * (2 * (R * (D + 2) + 4) + PA_WARPS * R * D);
 }
 
@@ -1036,6 +1074,8 @@ extern "C" int gb_paged_attention(const void* q, void* o, const void* kpool, con
 #undef GB_ATTEND
 #undef GB_ATTEND_
   }
-  GB_DISPATCH_FLOAT(dt, T, GB_DISPATCH_CACHE(cdt, C, paged_attend_any_kernel<T, C><<<(unsigned)rows, PA_WARPS * 32, 0, st>>>(a, c)));
+  const int splits = any_splits(rows, page, per);
+  GB_DISPATCH_FLOAT(dt, T, GB_DISPATCH_CACHE(cdt, C, paged_attend_any_kernel<T, C><<<(unsigned)(rows * splits), PA_WARPS * 32, 0, st>>>(a, c, splits, workspace)));
+  if (splits > 1) GB_DISPATCH_FLOAT(dt, T, paged_join_any_kernel<T><<<(unsigned)rows, PA_WARPS * 32, 0, st>>>(o, D, splits, workspace));
   return (int)cudaGetLastError();
 }
