@@ -38,17 +38,6 @@ struct AttendArgs {
 
 constexpr int PA_WARPS = 4, PA_MAX_D = 256;
 
-// n / d for n < 2^31: a division by a number that the host knows is a multiplication (a run of chunks begins with half a dozen)
-struct Div {
-  unsigned mul, shift, d;
-  explicit Div(unsigned x = 1) : d(x) {
-    shift = 0;
-    while (1ull << shift < x) ++shift;
-    mul = (unsigned)(((1ull << 32) * ((1ull << shift) - x)) / x + 1);
-  }
-  __device__ __forceinline__ int by(int n) const { return (int)((__umulhi(mul, (unsigned)n) + (unsigned)n) >> shift); }
-};
-
 // The chunks of all items: items[b] = n(b) * per_seq, in the order of b, then KV head and row tile.
 struct AttendPlan {
   int per_seq;          // items of a sequence: Hkv * row tiles

@@ -14,6 +14,17 @@ namespace gb {
 constexpr int DT_E4M3 = 8;
 constexpr int SITE_PAGE = 8, SITE_POSITION = 9;
 
+// n / d for n < 2^31: a division by a number that the host knows is a multiplication
+struct Div {
+  unsigned mul, shift, d;
+  explicit Div(unsigned x = 1) : d(x) {
+    shift = 0;
+    while (1ull << shift < x) ++shift;
+    mul = (unsigned)(((1ull << 32) * ((1ull << shift) - x)) / x + 1);
+  }
+  __device__ __forceinline__ int by(int n) const { return (int)((__umulhi(mul, (unsigned)n) + (unsigned)n) >> shift); }
+};
+
 struct Paged {
   const int* table;
   const int* lengths;

@@ -25,16 +25,24 @@ struct PutArgs {
   int positions, Hq;
 };
 
-// N numbers (4 or 8) in 32 bits into a pool, in its type; e4m3 under the power of two 1 / inv
+// N numbers (4 or 8) in 32 bits into a pool, in its type; e4m3 under the power of two 1 / inv, with infinities and NaN among them as
+// NaN where they are `odd`
 template <int CDT, int N>
-__device__ __forceinline__ void store_numbers(void* pool, long long at, const float (&x)[N], float inv) {
+__device__ __forceinline__ void store_numbers(void* pool, long long at, const float (&x)[N], float inv, bool odd) {
   if constexpr (CDT == DT_F32) {
 #pragma unroll
     for (int j = 0; j < N; j += 4) *reinterpret_cast<float4*>(reinterpret_cast<float*>(pool) + at + j) = make_float4(x[j], x[j + 1], x[j + 2], x[j + 3]);
   } else if constexpr (CDT == DT_E4M3) {
     uint32_t w[N / 4];
 #pragma unroll
-    for (int j = 0; j < N; j += 4) w[j / 4] = to_e4m3x2(x[j] * inv, x[j + 1] * inv) | to_e4m3x2(x[j + 2] * inv, x[j + 3] * inv) << 16;
+    for (int j = 0; j < N; j += 4)
+      w[j / 4] = (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(x[j] * inv, x[j + 1] * inv), __NV_SATFINITE, __NV_E4M3) |
+                 (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(x[j + 2] * inv, x[j + 3] * inv), __NV_SATFINITE, __NV_E4M3) << 16;
+    if (odd) {
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        if (!(fabsf(x[j]) < INFINITY)) w[j / 4] |= 0x7fu << j % 4 * 8;
+    }
     if constexpr (N == 8) *reinterpret_cast<uint2*>(reinterpret_cast<uint8_t*>(pool) + at) = make_uint2(w[0], w[1]);
     else *reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(pool) + at) = w[0];
   } else {
@@ -46,90 +54,81 @@ __device__ __forceinline__ void store_numbers(void* pool, long long at, const fl
   }
 }
 
-// A warp takes a token, or some of its heads where tokens are few (`splits` warps a token): position, page and the lane's part
-// of the rotation tables are looked up once and serve all heads.  A row is 2^log groups of lanes x 16 bytes of each half, so the
-// partner of a rotation is in the same registers, and a row's largest magnitude a few shuffles away.  The first rows are asked
-// for before the position is known, each next one before the last is worked on.
+// Rows (token, head) lie one after another: a group of 2^log lanes takes a row, 16 bytes of each of its halves a lane, so the
+// partner of a rotation is in the same registers and a row's largest magnitude a few shuffles away.  The row is asked for before
+// it is known where its token stands.  One row a thread: with two, 8 x 2048 tokens of 14 / 2 heads of 64 took 21.5 us for 17.3 (of
+// 11.8 that their bytes need), 8 x 4096 keys and values of 4 x 128 into 16 bits 28.8 for 25.7.
 template <typename T, int CDT, bool ROPE>
-__global__ void __launch_bounds__(256, 4) paged_put_rows_kernel(const PutArgs a, const Paged c, int log, int splits, int heads) {
+__global__ void __launch_bounds__(256) paged_put_rows_kernel(const PutArgs a, const Paged c, const Div heads, const Div tokens, int rows, int log) {
   constexpr int V = 16 / sizeof(T);
-  const int lane = threadIdx.x & 31, sub = lane >> log, ch = lane & ((1 << log) - 1), half = c.D / 2, step = 32 >> log;
-  const unsigned w = blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
-  const int token = (int)(w / splits), Hq = ROPE ? a.Hq : 0, Ht = Hq + 2 * c.Hkv;
-  if (token >= c.B * c.S) return;
-  const int b = token / c.S, s = token - b * c.S;
-  const int h0 = (int)(w - token * splits) * heads, h1 = min(Ht, h0 + heads);
-  Vec16<T> lo, hi;
-  auto load = [&](int h) {
-    if (h >= h1) return;
-    const bool isq = h < Hq, isk = h < Hq + c.Hkv;
-    const Rows& r = isq ? a.q : isk ? a.k : a.v;
-    const T* x = reinterpret_cast<const T*>(r.p) + b * r.sb + s * r.ss + (isq ? h : isk ? h - Hq : h - Hq - c.Hkv) * r.sh + ch * V;
-    lo = ld16(x);
-    hi = ld16(x + half);
-  };
-  load(h0 + sub);
-  const int n = c.count(b), pos = c.length(b) - n + s;
-  bool live = s < n && pos >= 0;
-  if (ROPE && live && pos >= a.positions) {
-    if (lane == 0) report_error(c.status, GB_ERR_BAD_INDEX, SITE_POSITION, pos);
-    live = false;
-  }
-  if (!ROPE && !live) return;
-  float cs[V], sn[V];
-  long long row0 = -1;                 // of KV head 0
-  if (live) {
-    if (ROPE) {
+  const int ch = threadIdx.x & ((1 << log) - 1), half = c.D / 2;
+  const int Hq = ROPE ? a.Hq : 0, Hk = Hq + c.Hkv;
+  const int r = (int)blockIdx.x * (256 >> log) + (threadIdx.x >> log);
+  const int token = heads.by(r), h = r - token * heads.d, b = tokens.by(token), s = token - b * tokens.d;
+  const bool there = r < rows, isq = h < Hq, isk = !isq && h < Hk;
+  const int hh = isq ? h : isk ? h - Hq : h - Hk;
+  float x[V], y[V];
 #pragma unroll
-      for (int j = 0; j < V; j += 4) {
-        *reinterpret_cast<float4*>(cs + j) = *reinterpret_cast<const float4*>(a.cosb + (long long)pos * c.D + ch * V + j);
-        *reinterpret_cast<float4*>(sn + j) = *reinterpret_cast<const float4*>(a.sinb + (long long)pos * c.D + ch * V + j);
+  for (int j = 0; j < V; ++j) x[j] = y[j] = 0.f;
+  int pos = -1;                        // -1: no token, or one without a rotation
+  long long row = -1;                  // of the pool; -1: nowhere
+  if (there) {
+    const Rows& src = isq ? a.q : isk ? a.k : a.v;
+    const T* p = reinterpret_cast<const T*>(src.p) + b * src.sb + s * src.ss + hh * src.sh + ch * V;
+    const Vec16<T> lo = ld16(p), hi = ld16(p + half);
+    const int n = c.count(b);
+    pos = c.length(b) - n + s;
+    if (s >= n || pos < 0) pos = -1;
+    if (ROPE && pos >= a.positions) {
+      report_error(c.status, GB_ERR_BAD_INDEX, SITE_POSITION, pos);
+      pos = -1;
+    }
+    if (pos >= 0) {
+      if (!isq) row = c.row(b, pos, hh);
+#pragma unroll
+      for (int j = 0; j < V; ++j) { x[j] = Cvt<T>::to_f(lo.v[j]); y[j] = Cvt<T>::to_f(hi.v[j]); }
+      if (ROPE && (isq || isk)) {
+        const float* cp = a.cosb + (long long)pos * c.D + ch * V;
+        const float* sp = a.sinb + (long long)pos * c.D + ch * V;
+        auto turn = [](float& p, float& q, float co, float si) { const float z = p * co - q * si; q = q * co + p * si; p = z; };
+#pragma unroll
+        for (int j = 0; j < V; j += 4) {
+          const float4 cs = *reinterpret_cast<const float4*>(cp + j), sn = *reinterpret_cast<const float4*>(sp + j);
+          turn(x[j], y[j], cs.x, sn.x); turn(x[j + 1], y[j + 1], cs.y, sn.y);
+          turn(x[j + 2], y[j + 2], cs.z, sn.z); turn(x[j + 3], y[j + 3], cs.w, sn.w);
+        }
       }
     }
-    row0 = c.row(b, pos, 0);
   }
-  for (int hb = h0; hb < h1; hb += step) {
-    const int h = hb + sub;
-    const bool on = h < h1, isq = h < Hq, isk = !isq && h < Hq + c.Hkv;
-    float x[V], y[V];
+  int e = 0;
+  bool odd = false;
+  if constexpr (CDT == DT_E4M3) {
+    uint32_t m = 0;
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      x[j] = on && live ? Cvt<T>::to_f(lo.v[j]) : 0.f;
-      y[j] = on && live ? Cvt<T>::to_f(hi.v[j]) : 0.f;
-    }
-    load(h + step);
-    if (ROPE && live && (isq || isk)) {
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const float p = x[j] * cs[j] - y[j] * sn[j];
-        y[j] = y[j] * cs[j] + x[j] * sn[j];
-        x[j] = p;
-      }
-    }
-    int e = 0;
-    if constexpr (CDT == DT_E4M3) {
-      uint32_t m = 0;
+    for (int j = 0; j < V; ++j) m = max(m, max(__float_as_uint(x[j]) & 0x7fffffffu, __float_as_uint(y[j]) & 0x7fffffffu));
+    odd = m >= 0x7f800000u;            // infinities or NaN
+    if (odd) {
+      m = 0;
 #pragma unroll
       for (int j = 0; j < V; ++j) m = max(m, max(finite_bits(x[j]), finite_bits(y[j])));
-      for (int o = 1 << log >> 1; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-      e = e4m3_exponent(m);
     }
-    if (!on) continue;
-    if (isq) {
-      Vec16<T> p, q;
+    for (int o = 1 << log >> 1; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+    e = e4m3_exponent(m);
+  }
+  if (!there) return;
+  if (isq) {
+    Vec16<T> p, q;
 #pragma unroll
-      for (int j = 0; j < V; ++j) { p.v[j] = Cvt<T>::from_f(x[j]); q.v[j] = Cvt<T>::from_f(y[j]); }
-      T* o = reinterpret_cast<T*>(a.q_out) + ((long long)token * Hq + h) * c.D + ch * V;
-      st16(o, p);
-      st16(o + half, q);
-    } else if (row0 >= 0) {
-      const long long row = row0 + (long long)(isk ? h - Hq : h - Hq - c.Hkv) * c.page;
-      void* pool = isk ? a.kpool : a.vpool;
-      const float inv = CDT == DT_E4M3 ? exp2i(-e) : 1.f;
-      store_numbers<CDT, V>(pool, row * c.D + ch * V, x, inv);
-      store_numbers<CDT, V>(pool, row * c.D + ch * V + half, y, inv);
-      if (CDT == DT_E4M3 && ch == 0) (isk ? a.kscale : a.vscale)[row] = (uint8_t)(e + 127);
-    }
+    for (int j = 0; j < V; ++j) { p.v[j] = Cvt<T>::from_f(x[j]); q.v[j] = Cvt<T>::from_f(y[j]); }
+    T* o = reinterpret_cast<T*>(a.q_out) + ((long long)token * Hq + h) * c.D + ch * V;
+    st16(o, p);
+    st16(o + half, q);
+  } else if (row >= 0) {
+    void* pool = isk ? a.kpool : a.vpool;
+    const float inv = CDT == DT_E4M3 ? exp2i(-e) : 1.f;
+    store_numbers<CDT, V>(pool, row * c.D + ch * V, x, inv, odd);
+    store_numbers<CDT, V>(pool, row * c.D + ch * V + half, y, inv, odd);
+    if (CDT == DT_E4M3 && ch == 0) (isk ? a.kscale : a.vscale)[row] = (uint8_t)(e + 127);
   }
 }
 
@@ -211,13 +210,19 @@ __global__ void paged_read_any_kernel(const void* kpool, const void* vpool, cons
 // A block takes 16 positions of a sequence, which lie in one page: per KV head its rows are contiguous there.  A thread takes N
 // numbers of K and of V (16 bytes of e4m3, or what 8 numbers are).
 template <typename T, int CDT, int N>
-__global__ void __launch_bounds__(256) paged_read_rows_kernel(const void* kpool, const void* vpool, const uint8_t* kscale,
-                                                              const uint8_t* vscale, void* kout, void* vout, int L, int log,
-                                                              const Paged c) {
+__global__ void __launch_bounds__(256) paged_read_rows_kernel(const void* __restrict__ kpool, const void* __restrict__ vpool,
+                                                              const uint8_t* __restrict__ kscale, const uint8_t* __restrict__ vscale,
+                                                              void* __restrict__ kout, void* __restrict__ vout, int L, int log,
+                                                              const Paged c, const Div page) {
   const int b = blockIdx.y, p0 = blockIdx.x * 16, groups = 1 << log;      // groups of N numbers in a row
   const int end = min(L, c.length(b));
+  // (the page is asked for before the length is known)
+  const int in_table = page.by(p0), id = in_table < c.per ? c.table[(size_t)b * c.per + in_table] : -1;
   long long row0 = -1;
-  if (p0 < end) row0 = c.row(b, p0, 0);
+  if (p0 < end) {
+    if ((unsigned)id < (unsigned)c.pages) row0 = (long long)id * c.Hkv * c.page + p0 - in_table * c.page;
+    else c.row(b, p0, 0);              // (records what is wrong)
+  }
   const int there = row0 < 0 ? 0 : end - p0;
   for (int i = threadIdx.x; i < c.Hkv * 16 << log; i += 256) {
     const int g = i & (groups - 1), t = i >> log & 15, h = i >> log >> 4;
@@ -300,19 +305,15 @@ extern "C" int gb_paged_put(const void* q, long long qb, long long qs, long long
   const long long tokens = (long long)B * S;
   const int V = dt == DT_F32 ? 4 : 8, log = D % (2 * V) == 0 ? log2_of(D / (2 * V)) : -1;
   auto wide = [&](const Rows& r) { return ((uintptr_t)r.p & 15) == 0 && r.sb % V == 0 && r.ss % V == 0 && r.sh % V == 0; };
-  if (log >= 0 && log <= 5 && wide(a.k) && wide(a.v) && (Hq == 0 || wide(a.q)) && (((uintptr_t)cosb | (uintptr_t)sinb) & 15) == 0 && tokens < 1 << 27) {
-    // heads of a token that a warp takes at once; more warps a token until each SM has some
-    const int once = 32 >> log, most = (Ht + once - 1) / once;
-    int splits = 1;
-    while (splits < most && tokens * splits < 8 * sm_count()) ++splits;
-    const int heads = (((Ht + splits - 1) / splits) + once - 1) / once * once;
-    splits = (Ht + heads - 1) / heads;
-    const unsigned grid = (unsigned)((tokens * splits + 7) / 8);
-    if (cosb != nullptr) GB_DISPATCH_FLOAT(dt, T, GB_DISPATCH_CACHE(cdt, C, paged_put_rows_kernel<T, C, true><<<grid, 256, 0, st>>>(a, c, log, splits, heads)));
-    else GB_DISPATCH_FLOAT(dt, T, GB_DISPATCH_CACHE(cdt, C, paged_put_rows_kernel<T, C, false><<<grid, 256, 0, st>>>(a, c, log, splits, heads)));
+  const long long rows = tokens * Ht;
+  if (log >= 0 && log <= 5 && wide(a.k) && wide(a.v) && (Hq == 0 || wide(a.q)) && (((uintptr_t)cosb | (uintptr_t)sinb) & 15) == 0 && rows < 1 << 30) {
+    const int each = 256 >> log;
+    const unsigned grid = (unsigned)((rows + each - 1) / each);
+    const Div heads(Ht), per(S);
+    if (cosb != nullptr) GB_DISPATCH_FLOAT(dt, T, GB_DISPATCH_CACHE(cdt, C, paged_put_rows_kernel<T, C, true><<<grid, 256, 0, st>>>(a, c, heads, per, (int)rows, log)));
+    else GB_DISPATCH_FLOAT(dt, T, GB_DISPATCH_CACHE(cdt, C, paged_put_rows_kernel<T, C, false><<<grid, 256, 0, st>>>(a, c, heads, per, (int)rows, log)));
     return (int)cudaGetLastError();
   }
-  const long long rows = tokens * Ht;
   GB_DISPATCH_FLOAT(dt, T, GB_DISPATCH_CACHE(cdt, C, paged_put_any_kernel<T, C><<<gb_grid(rows, 8), 256, 0, st>>>(a, c)));
   return (int)cudaGetLastError();
 }
@@ -326,9 +327,9 @@ extern "C" int gb_paged_read(const void* kpool, const void* vpool, const void* k
   if (log >= 0 && page % 16 == 0 && B <= 65535 && (long long)Hkv * 16 << log < 1 << 30) {
     const dim3 grid((L + 15) / 16, B);
     if (N == 16) GB_DISPATCH_FLOAT(dt, T, paged_read_rows_kernel<T, DT_E4M3, 16><<<grid, 256, 0, st>>>(
-        kpool, vpool, (const uint8_t*)kscale, (const uint8_t*)vscale, kout, vout, L, log, c));
+        kpool, vpool, (const uint8_t*)kscale, (const uint8_t*)vscale, kout, vout, L, log, c, Div(page)));
     else GB_DISPATCH_FLOAT(dt, T, GB_DISPATCH_CACHE(cdt, C, paged_read_rows_kernel<T, C, 8><<<grid, 256, 0, st>>>(
-        kpool, vpool, (const uint8_t*)kscale, (const uint8_t*)vscale, kout, vout, L, log, c)));
+        kpool, vpool, (const uint8_t*)kscale, (const uint8_t*)vscale, kout, vout, L, log, c, Div(page))));
     return (int)cudaGetLastError();
   }
   const long long total = (long long)B * L * Hkv * D;
