@@ -752,7 +752,7 @@ paged_attend_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_consta
           const int stop = min(c1 * KT, min(keys, max(0, len - cnt + s + 1)));
           float sum = 0.f;
           for (int key = odd_from * KT; key < stop; ++key) {
-            const int i = key / c.page, page = pages[i];
+            const int i = c.in_page.by(key), page = pages[i];
             if ((unsigned)page >= (unsigned)c.pages) continue;
             const long long at = (((long long)page * c.Hkv + kvh) * c.page + key - i * c.page) * D + d;
             float v;
@@ -1040,14 +1040,15 @@ extern "C" int gb_paged_attention_workspace(int B, int S, int Hq, int Hkv, int D
   return attend_grid(B, S, Hq, Hkv, D, page, pages, per, dt, cdt) * (2 * (R * (D + 2) + 4) + PA_WARPS * R * D);
 }
 
-extern "C" int gb_paged_attention(const void* q, void* o, const void* kpool, const void* vpool, const void* kscale,
-                                  const void* vscale, const int* table, const int* lengths, const int* counts, int B, int S,
-                                  int Hq, int Hkv, int D, int page, int pages, int per, float scale, int dt, int cdt,
-                                  float* workspace, int* status, cudaStream_t st) {
+extern "C" int gb_paged_attention(const void* pools, const void* q, void* o, const int* table, const int* lengths, const int* counts,
+                                  int B, int S, int Hq, int per, float scale, int dt, float* workspace, int* status,
+                                  cudaStream_t st) {
+  const PagedPools& p = *reinterpret_cast<const PagedPools*>(pools);
+  const int Hkv = p.Hkv, D = p.D, page = p.page, pages = p.pages, cdt = p.type;
   if (B <= 0 || S <= 0 || Hq <= 0 || D <= 0) return 0;
   if (D > PA_MAX_D || Hkv <= 0 || Hq % Hkv) return -3;
-  AttendArgs a{q, o, kpool, vpool, (const uint8_t*)kscale, (const uint8_t*)vscale, Hq, scale};
-  Paged c{table, lengths, counts, status, B, S, Hkv, D, page, pages, per};
+  AttendArgs a{q, o, p.k, p.v, p.kscale, p.vscale, Hq, scale};
+  Paged c{table, lengths, counts, status, B, S, Hkv, D, page, pages, per, Div(page)};
   const long long rows = (long long)B * S * Hq;
   if (rows > 0x7fffffff) return -4;
   const int grid = attend_grid(B, S, Hq, Hkv, D, page, pages, per, dt, cdt);

@@ -32,6 +32,7 @@ struct Paged {
   int* status;
   int B, S, Hkv, D;
   int page, pages, per;
+  Div in_page;             // by page
 
   // tokens of sequence b that the table has room for, and how many of this call's S are real
   __device__ __forceinline__ int length(int b) const {
@@ -49,10 +50,17 @@ struct Paged {
   // row of the pool [pages * Hkv * page] that token `pos` of sequence b has at KV head h; -1 (recorded) where there is none
   __device__ __forceinline__ long long row(int b, int pos, int h) const {
     if (pos >= capacity()) { report_error(status, GB_ERR_BAD_INDEX, SITE_POSITION, pos); return -1; }
-    const int i = pos / page, id = table[(size_t)b * per + i];
+    const int i = in_page.by(pos), id = table[(size_t)b * per + i];
     if (id < 0 || id >= pages) { report_error(status, GB_ERR_BAD_INDEX, SITE_PAGE, id); return -1; }
     return ((long long)id * Hkv + h) * page + (pos - i * page);
   }
+};
+
+// One layer's pools, as the caller keeps them (`Pools` in genesis_b200/ops/paged.py has the same fields).
+struct PagedPools {
+  void *k, *v;
+  uint8_t *kscale, *vscale;
+  int pages, Hkv, page, D, type;
 };
 
 // The exponent of a row of e4m3 numbers, from the bits of its largest finite magnitude: the smallest e >= -126 with

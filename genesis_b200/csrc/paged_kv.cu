@@ -213,11 +213,11 @@ template <typename T, int CDT, int N>
 __global__ void __launch_bounds__(256) paged_read_rows_kernel(const void* __restrict__ kpool, const void* __restrict__ vpool,
                                                               const uint8_t* __restrict__ kscale, const uint8_t* __restrict__ vscale,
                                                               void* __restrict__ kout, void* __restrict__ vout, int L, int log,
-                                                              const Paged c, const Div page) {
+                                                              const Paged c) {
   const int b = blockIdx.y, p0 = blockIdx.x * 16, groups = 1 << log;      // groups of N numbers in a row
   const int end = min(L, c.length(b));
   // (the page is asked for before the length is known)
-  const int in_table = page.by(p0), id = in_table < c.per ? c.table[(size_t)b * c.per + in_table] : -1;
+  const int in_table = c.in_page.by(p0), id = in_table < c.per ? c.table[(size_t)b * c.per + in_table] : -1;
   long long row0 = -1;
   if (p0 < end) {
     if ((unsigned)id < (unsigned)c.pages) row0 = (long long)id * c.Hkv * c.page + p0 - in_table * c.page;
@@ -290,50 +290,65 @@ static inline int log2_of(int x) {
 
 using namespace gb;
 
-// q, k, v: [B, S, heads, D] through strides of elements, the last dimension dense; q and the tables null for a write without
-// rotation.  Tokens of one call that share a slot of the cache are written in no order.
-extern "C" int gb_paged_put(const void* q, long long qb, long long qs, long long qh, const void* k, long long kb, long long ks,
-                            long long kh, const void* v, long long vb, long long vs, long long vh, void* q_out,
-                            const float* cosb, const float* sinb, int positions, void* kpool, void* vpool, void* kscale,
-                            void* vscale, const int* table, const int* lengths, const int* counts, int B, int S, int Hq,
-                            int Hkv, int D, int page, int pages, int per, int dt, int cdt, int* status, cudaStream_t st) {
-  if (B <= 0 || S <= 0 || Hkv <= 0 || D <= 0) return 0;
-  PutArgs a{{q, qb, qs, qh}, {k, kb, ks, kh}, {v, vb, vs, vh}, q_out, kpool, vpool, (uint8_t*)kscale, (uint8_t*)vscale,
-            cosb, sinb, positions, Hq};
-  Paged c{table, lengths, counts, status, B, S, Hkv, D, page, pages, per};
-  const int Ht = Hq + 2 * Hkv;
-  const long long tokens = (long long)B * S;
-  const int V = dt == DT_F32 ? 4 : 8, log = D % (2 * V) == 0 ? log2_of(D / (2 * V)) : -1;
+static int paged_put(const PutArgs& a, const Paged& c, const PagedPools& p, int dt, cudaStream_t st) {
+  const int Ht = a.Hq + 2 * p.Hkv;
+  const long long tokens = (long long)c.B * c.S;
+  const int V = dt == DT_F32 ? 4 : 8, log = p.D % (2 * V) == 0 ? log2_of(p.D / (2 * V)) : -1;
   auto wide = [&](const Rows& r) { return ((uintptr_t)r.p & 15) == 0 && r.sb % V == 0 && r.ss % V == 0 && r.sh % V == 0; };
   const long long rows = tokens * Ht;
-  if (log >= 0 && log <= 5 && wide(a.k) && wide(a.v) && (Hq == 0 || wide(a.q)) && (((uintptr_t)cosb | (uintptr_t)sinb) & 15) == 0 && rows < 1 << 30) {
+  if (log >= 0 && log <= 5 && wide(a.k) && wide(a.v) && (a.Hq == 0 || wide(a.q)) && (((uintptr_t)a.cosb | (uintptr_t)a.sinb) & 15) == 0 && rows < 1 << 30) {
     const int each = 256 >> log;
     const unsigned grid = (unsigned)((rows + each - 1) / each);
-    const Div heads(Ht), per(S);
-    if (cosb != nullptr) GB_DISPATCH_FLOAT(dt, T, GB_DISPATCH_CACHE(cdt, C, paged_put_rows_kernel<T, C, true><<<grid, 256, 0, st>>>(a, c, heads, per, (int)rows, log)));
-    else GB_DISPATCH_FLOAT(dt, T, GB_DISPATCH_CACHE(cdt, C, paged_put_rows_kernel<T, C, false><<<grid, 256, 0, st>>>(a, c, heads, per, (int)rows, log)));
+    const Div heads(Ht), per(c.S);
+    if (a.cosb != nullptr) GB_DISPATCH_FLOAT(dt, T, GB_DISPATCH_CACHE(p.type, C, paged_put_rows_kernel<T, C, true><<<grid, 256, 0, st>>>(a, c, heads, per, (int)rows, log)));
+    else GB_DISPATCH_FLOAT(dt, T, GB_DISPATCH_CACHE(p.type, C, paged_put_rows_kernel<T, C, false><<<grid, 256, 0, st>>>(a, c, heads, per, (int)rows, log)));
     return (int)cudaGetLastError();
   }
-  GB_DISPATCH_FLOAT(dt, T, GB_DISPATCH_CACHE(cdt, C, paged_put_any_kernel<T, C><<<gb_grid(rows, 8), 256, 0, st>>>(a, c)));
+  GB_DISPATCH_FLOAT(dt, T, GB_DISPATCH_CACHE(p.type, C, paged_put_any_kernel<T, C><<<gb_grid(rows, 8), 256, 0, st>>>(a, c)));
   return (int)cudaGetLastError();
 }
 
-extern "C" int gb_paged_read(const void* kpool, const void* vpool, const void* kscale, const void* vscale, void* kout,
-                             void* vout, const int* table, const int* lengths, int B, int L, int Hkv, int D, int page,
-                             int pages, int per, int dt, int cdt, int* status, cudaStream_t st) {
-  if (B <= 0 || L <= 0 || Hkv <= 0 || D <= 0) return 0;
-  Paged c{table, lengths, nullptr, status, B, 0, Hkv, D, page, pages, per};
-  const int N = cdt == DT_E4M3 && dt != DT_F32 ? 16 : 8, log = D % N == 0 ? log2_of(D / N) : -1;
-  if (log >= 0 && page % 16 == 0 && B <= 65535 && (long long)Hkv * 16 << log < 1 << 30) {
+// k, v: [B, S, Hkv, D] through strides of elements, the last dimension dense.  Tokens of one call that share a slot of the cache are
+// written in no order.
+extern "C" int gb_paged_write(const void* pools, const void* k, long long kb, long long ks, long long kh, const void* v, long long vb,
+                              long long vs, long long vh, const int* table, const int* lengths, const int* counts, int B, int S,
+                              int per, int dt, int* status, cudaStream_t st) {
+  const PagedPools& p = *reinterpret_cast<const PagedPools*>(pools);
+  if (B <= 0 || S <= 0 || p.Hkv <= 0 || p.D <= 0) return 0;
+  const PutArgs a{{nullptr, 0, 0, 0}, {k, kb, ks, kh}, {v, vb, vs, vh}, nullptr, p.k, p.v, p.kscale, p.vscale, nullptr, nullptr, 0, 0};
+  return paged_put(a, Paged{table, lengths, counts, status, B, S, p.Hkv, p.D, p.page, p.pages, per, Div(p.page)}, p, dt, st);
+}
+
+// y: [B, S, (Hq + 2 Hkv) D] through the strides yb and ys; rotated queries go to q_out [B, S, Hq, D], rotated keys and values to the
+// pages.
+extern "C" int gb_paged_qkv_rope(const void* pools, const void* y, long long yb, long long ys, void* q_out, const float* cosb,
+                                 const float* sinb, int positions, const int* table, const int* lengths, const int* counts, int B,
+                                 int S, int Hq, int per, int dt, int* status, cudaStream_t st) {
+  const PagedPools& p = *reinterpret_cast<const PagedPools*>(pools);
+  if (B <= 0 || S <= 0 || p.Hkv <= 0 || p.D <= 0 || Hq <= 0) return 0;
+  const long long head = (long long)p.D * (dt == DT_F32 ? 4 : 2);
+  const char* x = reinterpret_cast<const char*>(y);
+  const PutArgs a{{x, yb, ys, p.D}, {x + Hq * head, yb, ys, p.D}, {x + (Hq + p.Hkv) * head, yb, ys, p.D}, q_out,
+                  p.k, p.v, p.kscale, p.vscale, cosb, sinb, positions, Hq};
+  return paged_put(a, Paged{table, lengths, counts, status, B, S, p.Hkv, p.D, p.page, p.pages, per, Div(p.page)}, p, dt, st);
+}
+
+extern "C" int gb_paged_read(const void* pools, void* kout, void* vout, const int* table, const int* lengths, int B, int L, int per,
+                             int dt, int* status, cudaStream_t st) {
+  const PagedPools& p = *reinterpret_cast<const PagedPools*>(pools);
+  if (B <= 0 || L <= 0 || p.Hkv <= 0 || p.D <= 0) return 0;
+  const Paged c{table, lengths, nullptr, status, B, 0, p.Hkv, p.D, p.page, p.pages, per, Div(p.page)};
+  const int N = p.type == DT_E4M3 && dt != DT_F32 ? 16 : 8, log = p.D % N == 0 ? log2_of(p.D / N) : -1;
+  if (log >= 0 && p.page % 16 == 0 && B <= 65535 && (long long)p.Hkv * 16 << log < 1 << 30) {
     const dim3 grid((L + 15) / 16, B);
     if (N == 16) GB_DISPATCH_FLOAT(dt, T, paged_read_rows_kernel<T, DT_E4M3, 16><<<grid, 256, 0, st>>>(
-        kpool, vpool, (const uint8_t*)kscale, (const uint8_t*)vscale, kout, vout, L, log, c, Div(page)));
-    else GB_DISPATCH_FLOAT(dt, T, GB_DISPATCH_CACHE(cdt, C, paged_read_rows_kernel<T, C, 8><<<grid, 256, 0, st>>>(
-        kpool, vpool, (const uint8_t*)kscale, (const uint8_t*)vscale, kout, vout, L, log, c, Div(page))));
+        p.k, p.v, p.kscale, p.vscale, kout, vout, L, log, c));
+    else GB_DISPATCH_FLOAT(dt, T, GB_DISPATCH_CACHE(p.type, C, paged_read_rows_kernel<T, C, 8><<<grid, 256, 0, st>>>(
+        p.k, p.v, p.kscale, p.vscale, kout, vout, L, log, c)));
     return (int)cudaGetLastError();
   }
-  const long long total = (long long)B * L * Hkv * D;
-  GB_DISPATCH_FLOAT(dt, T, GB_DISPATCH_CACHE(cdt, C, paged_read_any_kernel<T, C><<<gb_grid(total, 256), 256, 0, st>>>(
-      kpool, vpool, (const uint8_t*)kscale, (const uint8_t*)vscale, kout, vout, L, c)));
+  const long long total = (long long)B * L * p.Hkv * p.D;
+  GB_DISPATCH_FLOAT(dt, T, GB_DISPATCH_CACHE(p.type, C, paged_read_any_kernel<T, C><<<gb_grid(total, 256), 256, 0, st>>>(
+      p.k, p.v, p.kscale, p.vscale, kout, vout, L, c)));
   return (int)cudaGetLastError();
 }

@@ -5,11 +5,13 @@ lengths share one pool, grow page by page, and may share the pages of a common b
 (its MoE attention concatenates the past, `models/transformers/moe.py:504-530`; its dense model encodes its prompt anew for
 every token).  The operators on a layer are `nn.functional.paged_kv_write`, `paged_qkv_rope`, `paged_kv_read` and
 `paged_attention`."""
+import ctypes
+
 import torch
 
 from ..device import as_torch_device
 from ..dtypes import DType
-from ..ops.paged import CACHE_TYPES, E4M3
+from ..ops.paged import CACHE_TYPES, E4M3, pools_of
 from ..tensor import Tensor
 
 
@@ -32,7 +34,7 @@ def _positive(name, x):
 class PagedKVLayer:
     """The pools of one decoder layer: raw k, v [pages, KV heads, page size, head dim], and in 8 bits k_scale, v_scale
     [pages, KV heads, page size] (uint8; a row stands for its e4m3 numbers times 2^(scale - 127)), else None."""
-    __slots__ = ("_k", "_v", "_k_scale", "_v_scale", "_call")
+    __slots__ = ("_k", "_v", "_k_scale", "_v_scale", "_pools", "_call")
 
     def __init__(self, k, v, k_scale=None, v_scale=None):
         if k.dim() != 4 or v.shape != k.shape or k.dtype not in CACHE_TYPES or v.dtype != k.dtype or k.shape[2] % 16 or 0 in k.shape:
@@ -45,9 +47,9 @@ class PagedKVLayer:
             if not t.is_contiguous() or t.data_ptr() % 16 or t.device != k.device:
                 raise ValueError("PagedKVLayer: pools and scales must be contiguous, start on 16 bytes and be on one device")
         self._k, self._v, self._k_scale, self._v_scale = k, v, k_scale, v_scale
-        # what every call passes on (so the pools cannot be exchanged): device, addresses, sizes, type
-        self._call = (k.get_device(), tuple(t.data_ptr() if t is not None else None for t in (k, v, k_scale, v_scale)),
-                      tuple(k.shape), CACHE_TYPES[k.dtype])
+        # what every call passes on (so the pools cannot be exchanged): device, the kernels' description, sizes, type
+        self._pools = pools_of(k, v, k_scale, v_scale)
+        self._call = (k.get_device(), ctypes.addressof(self._pools), tuple(k.shape), CACHE_TYPES[k.dtype])
 
     k = property(lambda self: self._k)
     v = property(lambda self: self._v)

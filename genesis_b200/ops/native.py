@@ -74,9 +74,8 @@ _SIGS = {
     "gb_token_grad": "pppp" + "lllll" + "l" + "d" + "pl" + "pll" + "p" + "f" + "ii" + "p",
     "gb_ns_plan": "iiiiiip", "gb_ns_workspace": "lllip", "gb_muon_momentum": "p" + "iiii" + "d" + "i" + "ppp" + "p",
     "gb_ns_one_by_one": "pipiiii",
-    "gb_paged_put": "plll" * 3 + "ppp" + "i" + "pppp" + "ppp" + "iiiiiiii" + "ii" + "pp",
-    "gb_paged_read": "pppp" + "pp" + "pp" + "iiiiiii" + "ii" + "pp",
-    "gb_paged_attention": "pppppp" + "ppp" + "iiiiiiii" + "f" + "ii" + "ppp",
+    "gb_paged_write": "p" + "plll" * 2 + "ppp" + "iiii" + "pp", "gb_paged_qkv_rope": "ppll" + "pppi" + "ppp" + "iiiii" + "pp",
+    "gb_paged_read": "ppp" + "pp" + "iiii" + "pp", "gb_paged_attention": "ppp" + "ppp" + "iiii" + "f" + "i" + "ppp",
     "gb_paged_attention_workspace": "iiiiiiiiii",
     "gb_newton_schulz": "pp" + "iiiii" + "pi" + "pi" + "d" + "p" + "fff" + "pp" + "pp" + "p",
 }

@@ -4,6 +4,7 @@ on the CPU (which is what the tests compare with).
 A layer's pools are k, v [pages, Hkv, page, D] and, for 8 bits, scales [pages, Hkv, page] of uint8: a row stands for its e4m3
 numbers times 2^(scale - 127).  `table` [B, per], `lengths` [B] and `counts` [B] (or None) are int32; token s of sequence b stands
 at position lengths[b] - counts[b] + s, for s < counts[b] (clipped to 0 .. S) and positions from 0 on."""
+import ctypes
 import functools
 
 import torch
@@ -144,69 +145,82 @@ def _attention_cpu(q, layer, table, lengths, counts, scale):
 # ------------------------------------------------------------------------------------------------
 # the kernels
 # ------------------------------------------------------------------------------------------------
+class Pools(ctypes.Structure):
+    """One layer's pools as the kernels' entry points take them (`PagedPools` in csrc/paged_common.cuh)."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("k", "v", "k_scale", "v_scale")] + \
+               [(n, ctypes.c_int) for n in ("pages", "kv_heads", "page", "head_dim", "type")]
+
+
+def pools_of(k, v, k_scale, v_scale):
+    return Pools(k.data_ptr(), v.data_ptr(), N._ptr(k_scale), N._ptr(v_scale), *k.shape, CACHE_TYPES[k.dtype])
+
+
 def _dense_last(t):
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
+def _launch(what, index, dev, fn, *args):
+    """Calls an entry point that ends in (status, stream) with `dev` as the current device."""
+    if index == torch.cuda.current_device():
+        N._chk(fn(*args, N.status_tensor(dev).data_ptr(), N._st()), what)
+    else:
+        with torch.cuda.device(index):
+            N._chk(fn(*args, N.status_tensor(dev).data_ptr(), N._st()), what)
+
+
 def write(k, v, layer, table, lengths, counts):
     """Keys and values [B, S, Hkv, D] into their pages."""
-    index, (kp, vp, ks, vs), (pages, Hkv, page, D), cdt = layer._call
+    index, pools, _, _ = layer._call
     if index < 0:
         _put_cpu(None, k, v, None, layer, table, lengths, counts)
         return
-    k, v, dev = _dense_last(k), _dense_last(v), k.device
-    B, S = k.shape[:2]
-    with N._on(dev):
-        N._chk(N.lib().gb_paged_put(None, 0, 0, 0, k.data_ptr(), *k.stride()[:3], v.data_ptr(), *v.stride()[:3], None, None, None, 0,
-                                    kp, vp, ks, vs, table.data_ptr(), lengths.data_ptr(), N._ptr(counts), B, S, 0, Hkv, D, page,
-                                    pages, table.shape[1], N._DT[k.dtype], cdt, N.status_tensor(dev).data_ptr(), N._st()),
-               "paged_put")
+    k, v = _dense_last(k), _dense_last(v)
+    (kb, ks, kh, _), (vb, vs, vh, _) = k.stride(), v.stride()
+    _launch("paged_write", index, k.device, N.lib().gb_paged_write, pools, k.data_ptr(), kb, ks, kh, v.data_ptr(), vb, vs, vh,
+            table.data_ptr(), lengths.data_ptr(), N._ptr(counts), k.shape[0], k.shape[1], table.shape[1], N._DT[k.dtype])
 
 
 def rope_write(y, tables, Hq, layer, table, lengths, counts):
     """Rotated queries [B, S, Hq, D] from y [B, S, (Hq + 2 Hkv) D], with the rotated keys and the values put into their pages;
     zeros for tokens that are none.  `tables`: cos, sin [positions, D] float32."""
-    index, (kp, vp, ks, vs), (pages, Hkv, page, D), cdt = layer._call
+    index, pools, (_, Hkv, _, D), _ = layer._call
     if index < 0:
         x = y.unflatten(-1, (Hq + 2 * Hkv, D))
         return _put_cpu(x[:, :, :Hq], x[:, :, Hq:Hq + Hkv], x[:, :, Hq + Hkv:], tables, layer, table, lengths, counts)
     y = _dense_last(y)
     B, S, _ = y.shape
     sb, ss, _ = y.stride()
-    dev, at, head = y.device, y.data_ptr(), D * y.element_size()
     cos, sin = tables
-    out = torch.empty(B, S, Hq, D, dtype=y.dtype, device=dev)
-    with N._on(dev):
-        N._chk(N.lib().gb_paged_put(at, sb, ss, D, at + Hq * head, sb, ss, D, at + (Hq + Hkv) * head, sb, ss, D, out.data_ptr(),
-                                    cos.data_ptr(), sin.data_ptr(), cos.shape[0], kp, vp, ks, vs, table.data_ptr(),
-                                    lengths.data_ptr(), N._ptr(counts), B, S, Hq, Hkv, D, page, pages, table.shape[1],
-                                    N._DT[y.dtype], cdt, N.status_tensor(dev).data_ptr(), N._st()), "paged_put")
+    out = torch.empty(B, S, Hq, D, dtype=y.dtype, device=y.device)
+    _launch("paged_qkv_rope", index, y.device, N.lib().gb_paged_qkv_rope, pools, y.data_ptr(), sb, ss, out.data_ptr(), cos.data_ptr(),
+            sin.data_ptr(), cos.shape[0], table.data_ptr(), lengths.data_ptr(), N._ptr(counts), B, S, Hq, table.shape[1],
+            N._DT[y.dtype])
     return out
 
 
 def read(layer, table, lengths, L, dtype):
     """(k, v) [B, L, Hkv, D] of `dtype`, zeros behind each sequence's end."""
-    index, (kp, vp, ks, vs), (pages, Hkv, page, D), cdt = layer._call
+    index, pools, (_, Hkv, _, D), _ = layer._call
     if index < 0:
         return _read_cpu(layer, table, lengths, L, dtype)
-    B, dev = table.shape[0], table.device
+    B, per = table.shape
+    dev = table.device
     k = torch.empty(B, L, Hkv, D, dtype=dtype, device=dev)
     v = torch.empty_like(k)
-    with N._on(dev):
-        N._chk(N.lib().gb_paged_read(kp, vp, ks, vs, k.data_ptr(), v.data_ptr(), table.data_ptr(), lengths.data_ptr(), B, L, Hkv,
-                                     D, page, pages, table.shape[1], N._DT[dtype], cdt, N.status_tensor(dev).data_ptr(),
-                                     N._st()), "paged_read")
+    _launch("paged_read", index, dev, N.lib().gb_paged_read, pools, k.data_ptr(), v.data_ptr(), table.data_ptr(), lengths.data_ptr(),
+            B, L, per, N._DT[dtype])
     return k, v
 
 
 @functools.lru_cache(maxsize=256)
 def _workspace(device_index, *sizes):
-    return N.lib().gb_paged_attention_workspace(*sizes)
+    with torch.cuda.device(device_index):
+        return N.lib().gb_paged_attention_workspace(*sizes)
 
 
 def attention(q, layer, table, lengths, counts, scale):
     """softmax(scale q k^T) v of the tokens q [B, S, Hq, D] over the pages of their sequences -> [B, S, Hq, D]."""
-    index, (kp, vp, ks, vs), (pages, Hkv, page, D), cdt = layer._call
+    index, at, (pages, Hkv, page, D), cdt = layer._call
     if index < 0:
         return _attention_cpu(q, layer, table, lengths, counts, scale)
     B, S, Hq, _ = q.shape
@@ -214,10 +228,8 @@ def attention(q, layer, table, lengths, counts, scale):
     if not q.is_contiguous() or q.data_ptr() % 16:
         q = q.clone(memory_format=torch.contiguous_format)
     out = torch.empty_like(q)
-    with N._on(dev):
-        words = _workspace(index, B, S, Hq, Hkv, D, page, pages, per, dt, cdt)
-        work = torch.empty(words, dtype=torch.float32, device=dev) if words else None
-        N._chk(N.lib().gb_paged_attention(q.data_ptr(), out.data_ptr(), kp, vp, ks, vs, table.data_ptr(), lengths.data_ptr(),
-                                          N._ptr(counts), B, S, Hq, Hkv, D, page, pages, per, scale, dt, cdt, N._ptr(work),
-                                          N.status_tensor(dev).data_ptr(), N._st()), "paged_attention")
+    words = _workspace(index, B, S, Hq, Hkv, D, page, pages, per, dt, cdt)
+    work = torch.empty(words, dtype=torch.float32, device=dev) if words else None
+    _launch("paged_attention", index, dev, N.lib().gb_paged_attention, at, q.data_ptr(), out.data_ptr(), table.data_ptr(),
+            lengths.data_ptr(), N._ptr(counts), B, S, Hq, per, scale, dt, N._ptr(work))
     return out
