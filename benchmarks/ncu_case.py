@@ -10,7 +10,8 @@ attn64_fwd, attn64_bwd, attn_decode (attn_decode_kernel), ce (ce_fwd16_kernel / 
 addnorm, addnorm_wide (add_rmsnorm_fwd_stream_kernel / rmsnorm_bwd_stream_kernel), moe_combine_bwd (moe_combine_bwd_vec_kernel),
 adam (adam_multi_kernel), swiglu_bwd (swiglu_bwd2d_kernel), rope (rope_vec_kernel),
 token_loss (token_rows_kernel / token_grad_kernel), newton_schulz (ns_product_kernel: with -s 4 -c 7 a block of two steps),
-newton_schulz_small (ns_gram_kernel), reduce_cols (reduce_mid), sort (sort_rows), index (index_get_kernel / index_put_kernel), cat (cat_kernel).
+newton_schulz_small (ns_gram_kernel), paged_attention, paged_attention_8bit (paged_attend_kernel / paged_join_kernel),
+paged_rope (paged_put_rows_kernel), paged_write_read (paged_put_rows_kernel / paged_read_rows_kernel), reduce_cols (reduce_mid), sort (sort_rows), index (index_get_kernel / index_put_kernel), cat (cat_kernel).
 """
 import sys
 import os
@@ -182,7 +183,41 @@ def newton_schulz(batch, rows, cols):
     return lambda: genesis.optim.orthogonalize(x, steps=2)
 
 
+def _paged(B, T, H, D, dtype):
+    cache = genesis.nn.PagedKVCache(B * -(-T // 64), H, D, dtype=dtype, device=DEV)
+    table = cache.page_table(cache.allocate([T] * B))
+    lengths = genesis.Tensor(torch.full((B,), T, dtype=torch.int32, device=DEV))
+    k, v = (genesis.Tensor(rnd(B, T, H, D)) for _ in range(2))
+    genesis.nn.functional.paged_kv_write(k, v, cache[0], table, lengths)
+    return cache[0], table, lengths, k, v
+
+
+def paged_attention(B, T, Hq, H, D, dtype):
+    layer, table, lengths, _, _ = _paged(B, T, H, D, dtype)
+    q = genesis.Tensor(rnd(B, 1, Hq, D))
+    return lambda: genesis.nn.functional.paged_attention(q, layer, table, lengths)
+
+
+def paged_rope():
+    layer, table, lengths, _, _ = _paged(16, 2048, 2, 64, "bfloat16")
+    y = genesis.Tensor(rnd(16, 2048, 18 * 64))
+    cos, sin = (genesis.Tensor(torch.rand(2048, 64, device=DEV)) for _ in range(2))
+    return lambda: genesis.nn.functional.paged_qkv_rope(y, cos, sin, layer, table, lengths, 14)
+
+
+def paged_write_read():
+    layer, table, lengths, k, v = _paged(8, 8192, 4, 128, "float8_e4m3fn")
+
+    def f():
+        genesis.nn.functional.paged_kv_write(k, v, layer, table, lengths)
+        genesis.nn.functional.paged_kv_read(layer, table, lengths, 8192)
+    return f
+
+
 CASES = {
+    "paged_attention": lambda: paged_attention(32, 4096, 32, 4, 128, "bfloat16"),
+    "paged_attention_8bit": lambda: paged_attention(8, 20000, 32, 4, 128, "float8_e4m3fn"),
+    "paged_rope": paged_rope, "paged_write_read": paged_write_read,
     "token_loss": token_loss, "newton_schulz": lambda: newton_schulz(12, 896, 4864),
     "newton_schulz_small": lambda: newton_schulz(148, 128, 896),
     "gemm_pair": gemm_pair, "gemm_swiglu": gemm_swiglu, "gemm_swiglu_bwd": gemm_swiglu_bwd, "gemm": gemm, "grouped_gemm": grouped_gemm,

@@ -12,7 +12,7 @@ ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 sys.path.insert(0, ROOT)
 
 MODULES = [
-    "genesis_b200", "genesis_b200.nn", "genesis_b200.nn.functional", "genesis_b200.nn.utils", "genesis_b200.nn.parallel",
+    "genesis_b200", "genesis_b200.nn", "genesis_b200.nn.functional", "genesis_b200.nn.utils", "genesis_b200.nn.parallel", "genesis_b200.nn.paged",
     "genesis_b200.optim", "genesis_b200.optim.lr_scheduler", "genesis_b200.amp", "genesis_b200.cuda",
     "genesis_b200.distributed", "genesis_b200.distributed.symm", "genesis_b200.distributed.watchdog",
     "genesis_b200.parallel.ep", "genesis_b200.models.transformers", "genesis_b200.serialization",

@@ -2082,8 +2082,8 @@ def paged_attention(q, cache, page_table, lengths, counts=None, scale=None):
     Hq, D = q.shape[2:]
     if D != cache._call[2][3] or Hq < 1 or Hq % cache._call[2][1]:
         raise ValueError(f"{name}: q must be [B, S, heads, {cache.head_dim}] with heads a multiple of {cache.num_kv_heads}, got {tuple(q.shape)}")
-    if q.is_cuda and D > 256:
-        raise ValueError(f"{name}: heads of up to 256 on CUDA, got {D}")
+    if q.is_cuda and (D > 256 or q.shape[0] * q.shape[1] * Hq >= 2 ** 31):
+        raise ValueError(f"{name}: heads of up to 256 and less than 2^31 rows on CUDA, got {tuple(q.shape)}")
     scale = D ** -0.5 if scale is None else _number(name, "scale", scale, -1e30, 1e30)
     return Tensor._wrap(P.attention(q, cache, table, lengths, counts, scale))
 

@@ -173,6 +173,23 @@ def test_attention_over_long_sequences(dtype, cache, Hq, H, D, page):
     _attend(t, lengths, None, 1, Hq, D, dtype, cache, scale=0.31, strengths=3.0)
 
 
+@pytest.mark.parametrize("dtype,cache,Hq,H,D", [("fp32", "e4m3", 14, 2, 64), ("bf16", "fp32", 4, 4, 128), ("fp16", "bf16", 6, 2, 64),
+                                               ("fp32", "bf16", 8, 1, 256), ("bf16", "bf16", 6, 3, 80), ("fp16", "e4m3", 2, 2, 96),
+                                               ("bf16", "e4m3", 4, 1, 1), ("fp32", "fp32", 3, 3, 200)])
+@pytest.mark.parametrize("S", [1, 3])
+def test_attention_of_any_type_and_head(dtype, cache, Hq, H, D, S):
+    lengths = [3000, 1, 0, 64, 65, 700]
+    t = R.Setup(lengths, H, D, cache, 16, "cuda", width=200)
+    _attend(t, lengths, None, S, Hq, D, dtype, cache)
+
+
+@pytest.mark.parametrize("dtype,cache", TYPES)
+def test_scales_of_either_sign_and_none(dtype, cache):
+    t = R.Setup([300, 17], 2, 64, cache, 16, "cuda")
+    for scale in (-0.2, 0.0, 1e-3):
+        _attend(t, [300, 17], None, 1, 14, 64, dtype, cache, scale=scale)
+
+
 @pytest.mark.parametrize("dtype,cache", TYPES)
 def test_attention_of_many_sequences(dtype, cache):
     g = torch.Generator().manual_seed(5)
