@@ -12,10 +12,15 @@
 // a second small kernel joins the items that CTAs share (parts in a fixed order: the same call gives the same bits).
 //   rows     : the query rows of a KV head's group (tokens x heads) are the 8 columns of mma.sync.m16n8k16, 16 keys its rows:
 //              S^T = K Q^T, O^T = V^T P^T.  K and V are read once per 8 or 16 rows.
-//   layout   : fragments straight from global memory, 16 bytes a load and no shared memory in the loop.  The contraction over d
-//              may go in any order that K and Q share, so a lane takes 16 contiguous bytes of its key's row; for V a lane takes
-//              contiguous d of four keys and pairs the keys' numbers with byte permutes.  P^T comes from S^T by movmatrix.
-//   bound    : the bytes of K and V; the next chunk's K is in flight during softmax and P V, its V during the next Q K.
+//   layout   : tiles of 16 keys come by TMA into a ring of each warp (no barrier between warps in the loop), the next chunk's K as
+//              soon as this one's is read, its V behind it.  Fragments are read 16 bytes at a time: the contraction over d may go in any
+//              order that K and Q share, so a lane takes contiguous bytes of its key's row; for V a lane takes contiguous d of four
+//              keys and pairs the keys' numbers with byte permutes.  P^T comes from S^T by movmatrix.
+//   bound    : the bytes of K and V where sequences are long: 64 x 4096 keys, 32 / 4 heads of 128, bf16: 95 us, 5.65 TB/s (6.1 less the 8
+//              that 500 keys take); in 8 bits 59 us, 4.6 TB/s, where converting and the wait for it take as long as the bytes.  8 us of
+//              a call are two launches, finding the share, one round of latencies and the join.
+//   other ways that were measured: fragments by plain loads (bf16 93 us, 8 bits 70), by cp.async (109, 70); fetching ahead into L2 with
+//              plain loads (99 to 110).
 //   precision: P enters its product as two 16-bit numbers (rounded, and what the rounding lost), or rounding it once to the
 //              type of V would double the error that the output's rounding makes; with 8-bit V it is fp16, whose 11 bits suffice
 //              below a bf16 output.  fp16 P is scaled by 2^7 on top of a maximum that may lag 2^8 behind, so that 2^-31 of the
@@ -50,13 +55,15 @@ struct AttendPlan {
   int4* spans;          // [grid][2]: that item (-1: none), the first and the last CTA that have it
 };
 
-// Keys of a chunk: 4 KB of K and of V, but a tile of 16 at least and two of them at most (four tiles of 8 bits cost registers:
-// 64 x 4096, 2 KV heads of 64: 36.2 us with four, 33.6 with two; one tile of 128: 71.7 us for 70.1 over 4 KV heads).
+// Keys of a chunk: 4 KB of K and of V, but a tile of 16 at least and two of them at most: with four of 64 numbers in 8 bits, registers are
+// spilled (64 x 4096, 14 / 2 heads: 45 us for 28.5), with one of 128 the rounds are short (8 x 4096, 32 / 4 heads: 20.3 us for 18.0; only
+// runs of 32768 gain, 57.3 for 58.3).
 static constexpr int attend_chunk(int D, int bytes) { return 4096 / (D * bytes) < 16 ? 16 : 4096 / (D * bytes) > 32 ? 32 : 4096 / (D * bytes); }
 
 // CTAs on an SM, by registers: four, three where numbers are split in two or added up apart, two for two operands of rows over 128
-// numbers of 8 bits.  Chunks in flight of a warp, by what shared memory is left; one where registers are spilled, which need the
-// L1 that a larger ring takes (32 sequences of 4096, drafts of 4: 143 us with two, 93 with one).
+// numbers of 8 bits.  (Three instead of four, 32 / 4 heads of 128: 64 x 4096 bf16 98.7 us for 95.2, in 8 bits 60.7 for 59.2; 8 x 4096 25.3
+// for 23.0, in 8 bits 20.5 for 18.0; 8 x 32768 in 8 bits 57.3 for 58.3.)  Chunks in flight of a warp, by what shared memory is left; one
+// where registers are spilled, which need the L1 that a larger ring takes (32 x 4096, drafts of 4: 144 us with two, 93 with one).
 static constexpr int attend_ctas(int dt, int cdt, int D, int R) {
   return R == 16 ? (cdt == DT_E4M3 && D == 128 ? 2 : 3) : cdt == DT_F32 || (cdt == DT_E4M3 && dt == DT_F16) ? 3 : 4;
 }
@@ -1011,33 +1018,35 @@ static int any_splits(long long rows, int page, int per) {
 
 using namespace gb;
 
-// Query rows of an item: one operand of 8 columns, or two where there are more rows and registers for them.
-static int attend_rows(int rows, int D, int cdt) { return rows <= 8 || (cdt == DT_F32 && D == 128) ? 8 : 16; }
-
-// Which kernel a call takes, and its CTAs (0: a CTA for every row).  The tensor cores take heads of 64 or 128 over caches of the
-// queries' type, or of 8 bits below 16-bit queries; what remains (other head sizes, types that differ, more than 2^31 chunks of
-// keys or rows of the pool) is worked on number by number.
-static int attend_grid(int B, int S, int Hq, int Hkv, int D, int page, int pages, int per, int dt, int cdt) {
-  if ((D != 64 && D != 128) || (cdt != dt && !(cdt == DT_E4M3 && dt != DT_F32)) || page % 16) return 0;
-  const int rows = S * (Hq / Hkv), R = attend_rows(rows, D, cdt);
-  const int es = cdt == DT_E4M3 ? 1 : cdt == DT_F32 ? 4 : 2, kt = attend_chunk(D, es);
-  const long long tiles = (rows + R - 1) / R, keys = (long long)per * page;
-  const long long chunks = (long long)B * Hkv * tiles * (keys <= 0 ? 1 : (keys + kt - 1) / kt);
-  if (chunks > 0x7fffffff || (long long)pages * Hkv * page > 0x7fffffff) return 0;       // (counted in 32 bits)
-  const long long want = (chunks + PA_WARPS - 1) / PA_WARPS, most = (long long)sm_count() * attend_ctas(dt, cdt, D, R);
-  return (int)(want < most ? want : most);
+// Which kernel a call takes: query rows of an item and CTAs (0: the kernel for any type).  The tensor cores take heads of 64 or 128
+// over caches of the queries' type, or of 8 bits below 16-bit queries; what remains (other head sizes, types that differ, more
+// than 2^31 chunks of keys or rows of the pool) is worked on number by number.
+//   rows: two operands of 8 read K and V half as often, and leave half as many chunks to share out.  By what the page table has
+//   room for, two where each warp then has four chunks and more: 32 x 4096, drafts of 4, 32 / 4 heads of 128: 93 us (146 with one), 14 / 2
+//   of 64, drafts of 2: 25.6 (28.7); 8 x 2000, drafts of 8, 12 / 2 of 128: 26.6 with two, 22.9 with one; 4 x 2000, drafts of 5: 17.6, 15.8.
+struct AttendChoice { int R, grid; };
+static AttendChoice attend_choice(int B, int S, int Hq, int Hkv, int D, int page, int pages, int per, int dt, int cdt) {
+  if ((D != 64 && D != 128) || (cdt != dt && !(cdt == DT_E4M3 && dt != DT_F32)) || page % 16) return {8, 0};
+  const int rows = S * (Hq / Hkv), kt = attend_chunk(D, cdt == DT_E4M3 ? 1 : cdt == DT_F32 ? 4 : 2);
+  const long long keys = (long long)per * page, run = keys <= 0 ? 1 : (keys + kt - 1) / kt;
+  auto chunks = [&](int R) { return (long long)B * Hkv * ((rows + R - 1) / R) * run; };
+  // (numbers of 32 bits and 128 have no registers for two)
+  const int R = rows <= 8 || (cdt == DT_F32 && D == 128) || chunks(16) < 4ll * 12 * sm_count() ? 8 : 16;
+  if (chunks(R) > 0x7fffffff || (long long)pages * Hkv * page > 0x7fffffff) return {8, 0};       // (counted in 32 bits)
+  const long long want = (chunks(R) + PA_WARPS - 1) / PA_WARPS, most = (long long)sm_count() * attend_ctas(dt, cdt, D, R);
+  return {R, (int)(want < most ? want : most)};
 }
 
 // 32-bit words of workspace that a call needs
 extern "C" int gb_paged_attention_workspace(int B, int S, int Hq, int Hkv, int D, int page, int pages, int per, int dt, int cdt) {
   if (B <= 0 || S <= 0 || Hq <= 0 || Hkv <= 0) return 0;
-  const int R = attend_rows(S * (Hq / Hkv), D, cdt);
-  if (attend_grid(B, S, Hq, Hkv, D, page, pages, per, dt, cdt) == 0) {
+  const AttendChoice x = attend_choice(B, S, Hq, Hkv, D, page, pages, per, dt, cdt);
+  if (x.grid == 0) {
     const long long rows = (long long)B * S * Hq;
     const int splits = any_splits(rows, page, per);
     return splits == 1 ? 0 : (int)(rows * splits * (D + 2));
   }
-  return attend_grid(B, S, Hq, Hkv, D, page, pages, per, dt, cdt) * (2 * (R * (D + 2) + 4) + PA_WARPS * R * D);
+  return x.grid * (2 * (x.R * (D + 2) + 4) + PA_WARPS * x.R * D);
 }
 
 extern "C" int gb_paged_attention(const void* pools, const void* q, void* o, const int* table, const int* lengths, const int* counts,
@@ -1051,9 +1060,9 @@ extern "C" int gb_paged_attention(const void* pools, const void* q, void* o, con
   Paged c{table, lengths, counts, status, B, S, Hkv, D, page, pages, per, Div(page)};
   const long long rows = (long long)B * S * Hq;
   if (rows > 0x7fffffff) return -4;
-  const int grid = attend_grid(B, S, Hq, Hkv, D, page, pages, per, dt, cdt);
-  if (grid > 0) {
-    const int R = attend_rows(S * (Hq / Hkv), D, cdt);
+  const AttendChoice x = attend_choice(B, S, Hq, Hkv, D, page, pages, per, dt, cdt);
+  if (x.grid > 0) {
+    const int R = x.R, grid = x.grid;
     int4* spans = reinterpret_cast<int4*>(workspace + (size_t)grid * 2 * R * (D + 2));
 #define GB_ATTEND_(T, C, D_, NQ_) (S > 1 ? launch_attend<T, C, D_, NQ_, true>(a, c, workspace, spans, grid, st) : launch_attend<T, C, D_, NQ_, false>(a, c, workspace, spans, grid, st))
 #define GB_ATTEND(T, C) (D == 64 ? (R == 8 ? GB_ATTEND_(T, C, 64, 1) : GB_ATTEND_(T, C, 64, 2)) : (R == 8 ? GB_ATTEND_(T, C, 128, 1) : GB_ATTEND_(T, C, 128, 2)))

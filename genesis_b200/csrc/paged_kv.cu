@@ -248,7 +248,7 @@ __global__ void __launch_bounds__(256) paged_read_rows_kernel(const void* __rest
       for (int w = 0; w < 2; ++w) {
         const void* pool = w ? vpool : kpool;
         if constexpr (CDT == DT_E4M3) {
-          uint32_t v[N / 4];
+          alignas(8) uint32_t v[N / 4];
           *reinterpret_cast<uint2*>(v) = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint8_t*>(pool) + at);
           const float sc = __uint_as_float((uint32_t)(w ? vscale : kscale)[row] << 23);
 #pragma unroll
@@ -265,7 +265,7 @@ __global__ void __launch_bounds__(256) paged_read_rows_kernel(const void* __rest
             x[w][j] = v.x; x[w][j + 1] = v.y; x[w][j + 2] = v.z; x[w][j + 3] = v.w;
           }
         } else {
-          uint16_t v[8];
+          alignas(16) uint16_t v[8];
           *reinterpret_cast<uint4*>(v) = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(pool) + at);
 #pragma unroll
           for (int j = 0; j < 8; ++j) x[w][j] = half_bits_to_float(v[j], CDT);
