@@ -149,16 +149,18 @@ TYPES = [("bf16", "bf16"), ("fp16", "fp16"), ("bf16", "e4m3"), ("fp16", "e4m3"),
 @pytest.mark.parametrize("dtype,cache", TYPES)
 def test_attention_of_single_tokens(Hq, H, D, dtype, cache):
     lengths = [1, 0, 2, 15, 16, 17, 31, 33, 100, 257, 600, -5]
-    t = R.Setup(lengths, H, D, cache, 16, "cuda", width=50)
-    _attend(t, lengths, None, 1, Hq, D, dtype, cache)
+    for width in (50, 10000):
+        t = R.Setup(lengths, H, D, cache, 16, "cuda", width=width)
+        _attend(t, lengths, None, 1, Hq, D, dtype, cache)
 
 
 @pytest.mark.parametrize("Hq,H,D", [(14, 2, 64), (32, 4, 128), (12, 12, 64), (6, 2, 80), (8, 8, 128)])
 @pytest.mark.parametrize("dtype,cache", TYPES)
 @pytest.mark.parametrize("S", [2, 5, 19])
-def test_attention_of_several_tokens(Hq, H, D, dtype, cache, S):
+@pytest.mark.parametrize("width", [0, 4000])         # the rows of an item go by what the table has room for
+def test_attention_of_several_tokens(Hq, H, D, dtype, cache, S, width):
     lengths, counts = [1, 0, 2, 16, 40, 100, 333, 70], [1, 3, 2, S, S, 1, S, 0]
-    t = R.Setup(lengths, H, D, cache, 32, "cuda")
+    t = R.Setup(lengths, H, D, cache, 32, "cuda", width=width)
     _attend(t, lengths, counts, S, Hq, D, dtype, cache)
     _attend(t, lengths, None, S, Hq, D, dtype, cache)         # sequences shorter than the call: rows that see nothing
 
@@ -171,6 +173,8 @@ def test_attention_over_long_sequences(dtype, cache, Hq, H, D, page):
     t = R.Setup(lengths, H, D, cache, page, "cuda")
     _attend(t, lengths, None, 1, Hq, D, dtype, cache)
     _attend(t, lengths, None, 1, Hq, D, dtype, cache, scale=0.31, strengths=3.0)
+    t = R.Setup(lengths, H, D, cache, page, "cuda", width=60000 // page * 16)
+    _attend(t, lengths, None, 3, Hq, D, dtype, cache)
 
 
 @pytest.mark.parametrize("dtype,cache,Hq,H,D", [("fp32", "e4m3", 14, 2, 64), ("bf16", "fp32", 4, 4, 128), ("fp16", "bf16", 6, 2, 64),
@@ -251,9 +255,9 @@ def test_what_is_not_finite_stays_with_its_rows():
 @pytest.mark.parametrize("dtype,cache", TYPES)
 def test_tokens_that_come_later_do_not_reach_back(dtype, cache, S):
     """Infinities and NaN in the newest token's keys and values belong to the rows that see it."""
-    for D in (64, 128, 48):
+    for D, width in ((64, 0), (128, 0), (48, 0), (64, 20000), (128, 20000)):
         lengths = [33, 7, 200]
-        t = R.Setup(lengths, 2, D, cache, 16, "cuda")
+        t = R.Setup(lengths, 2, D, cache, 16, "cuda", width=width)
         q = t.normal(3, S, 8, D, dtype=dtype)
         clean = F.paged_attention(t.tensor(q), t.layer, t.table, t.lens)._t.clone()
         for b, n in enumerate(lengths):
