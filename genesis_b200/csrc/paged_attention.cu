@@ -281,7 +281,11 @@ paged_attend_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_consta
   while (u < u_end) {
     // ---- an item's run of chunks ------------------------------------------------------------------------------------
     const int keys = attend_keys(c, b), n = attend_chunks(keys, KT);
-    if (u - seq_start >= (unsigned)n * plan.per_seq) { seq_start += (unsigned)n * plan.per_seq; ++b; continue; }
+    if (u - seq_start >= (unsigned)n * plan.per_seq) {
+      seq_start += (unsigned)n * plan.per_seq;
+      if (++b >= c.B) break;           // (lengths that change under the kernel's hands give wrong sums, and nothing worse)
+      continue;
+    }
     const int idx = plan.per_seq == 1 ? 0 : (int)((u - seq_start) / (unsigned)n);
     const int c0 = (int)(u - seq_start - (unsigned)idx * n);
     const int c1 = min(n, c0 + (int)(u_end - u));
@@ -340,6 +344,7 @@ paged_attend_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_consta
 
     // one round: scores of chunk ch, then K of chunk ch + ST into its place; probabilities and products of ch, then V of ch + ST.
     uint32_t gone_later = 0;           // tiles that are not there, of the chunks in flight
+    bool ahead = false;                // given up with a K on its way whose V has not been asked for
     for (int ch = c0 - C::ST; ch < c1; ++ch) {
       const bool now = ch >= c0, more = ch + C::ST < c1;
       uint8_t* const sk = ring + use * 2 * C::KB;
@@ -587,7 +592,10 @@ paged_attend_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_consta
         constexpr int TW = C::E8 ? 2 : 1;              // tiles of O^T that a word of V has numbers of
         alignas(16) uint32_t vr[NS][4][4];
         uint32_t bad = 0;
-        if (!__all_sync(0xffffffffu, mbar_wait(&landed[warp][use][1], use_phase, abort_flag, c.status, 82))) break;
+        if (!__all_sync(0xffffffffu, mbar_wait(&landed[warp][use][1], use_phase, abort_flag, c.status, 82))) {
+          ahead = more;
+          break;
+        }
 #pragma unroll
         for (int j = 0; j < VW; j += C::F32 ? 2 : 1) {
           constexpr int VN = VW == 2 ? 2 : 4;         // words that a lane has of a key side by side
@@ -693,7 +701,7 @@ paged_attend_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_consta
         const uint64_t t0 = globaltimer_ns();
         for (int i = 0; i < C::ST; ++i)
           for (int w = 0; w < 2; ++w) {
-            const int phase = i < put ? put_phase : put_phase ^ 1;       // of the last copy into stage i
+            const int phase = i < put || (i == put && w == 0 && ahead) ? put_phase : put_phase ^ 1;       // of the last copy into stage i
             while (!mbar_try_wait(&landed[warp][i][w], phase) && globaltimer_ns() - t0 < 1000000ull) {}
           }
       }

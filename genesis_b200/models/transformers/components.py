@@ -85,8 +85,10 @@ def paged_self_attention(y, rotary, num_heads, cache, page_table, lengths, count
     num_heads * D].  The tokens' keys and values are put into the cache; with `prompt` the sequences have no others, and the
     flash attention over the call's own keys takes the place of reading them back."""
     B, S, _ = y.shape
-    room = page_table.shape[1] * cache.page_size
+    room = max(S, page_table.shape[1] * cache.page_size)
     if room > rotary.max_seq_len_cached:
+        # (a captured step may go on reading the tables that are outgrown)
+        rotary.__dict__.setdefault("_outgrown", []).append((rotary.cos_cached, rotary.sin_cached))
         rotary._build(room)
     cos, sin = rotary.cos_cached, rotary.sin_cached
     if prompt:

@@ -173,7 +173,7 @@ class QwenForCausalLM(nn.Module):
 
         `page_table` [B, pages], `lengths` [B] (tokens with those of this call) and `counts` [B] (real ones of the S) are int32
         Tensors as `nn.functional.paged_attention` takes them.  `prompt`: the sequences had no tokens before.  `last`: logits
-        [B, 1, V] of each sequence's last real token, else [B, S, V].  For inference; nothing here waits for the device, so a
+        [B, 1, V] of each sequence's last real token (of a sequence without one they mean nothing), else [B, S, V].  For inference; nothing here waits for the device, so a
         step can be captured and replayed while the lengths grow on the device."""
         return self.model.forward_paged(idx, cache, page_table, lengths, counts, prompt, last)
 

@@ -51,6 +51,10 @@ class PagedKVLayer:
         self._pools = pools_of(k, v, k_scale, v_scale)
         self._call = (k.get_device(), ctypes.addressof(self._pools), tuple(k.shape), CACHE_TYPES[k.dtype])
 
+    def __reduce__(self):              # (torch does not pickle e4m3)
+        raw = [t.view(torch.uint8) if t.dtype == E4M3 else t for t in (self._k, self._v)]
+        return _layer_of, (*raw, self._k_scale, self._v_scale)
+
     k = property(lambda self: self._k)
     v = property(lambda self: self._v)
     k_scale = property(lambda self: self._k_scale)
@@ -77,6 +81,10 @@ class PagedKVLayer:
                 f"{str(self.k.dtype).replace('torch.', '')}, {self.k.device})")
 
 
+def _layer_of(k, v, k_scale, v_scale):
+    return PagedKVLayer(*((k, v) if k_scale is None else (k.view(E4M3), v.view(E4M3))), k_scale, v_scale)
+
+
 class PagedKVCache:
     """Pages for the keys and values of all layers of a decoder, and which of them are free.
 
@@ -88,8 +96,9 @@ class PagedKVCache:
         ...
         cache.release(pages)
 
-    The pool's memory is what a reader of another stream must wait for like for any tensor's; page numbers are handed out on
-    the host and nothing here waits for the device."""
+    A table may name a page for several sequences (a common beginning), for reading; whose page it is remains the caller's to know.
+    Like any tensor's, the pools' memory is to be waited for by another stream that reads or writes it; page numbers are handed out
+    on the host and nothing here waits for the device."""
 
     def __init__(self, num_pages, num_kv_heads, head_dim, page_size=64, num_layers=1, dtype="bfloat16", device=None):
         P, H, D, page, L = (_positive(n, x) for n, x in (("num_pages", num_pages), ("num_kv_heads", num_kv_heads),

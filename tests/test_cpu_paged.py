@@ -60,6 +60,19 @@ def test_caches_that_are_refused():
     assert PagedKVCache(1, 1, 8, dtype=torch.float8_e4m3fn)[0].k_scale.dtype == torch.uint8
 
 
+def test_copies_have_pools_of_their_own():
+    import copy
+    import pickle
+    c = PagedKVCache(2, 1, 8, page_size=16, dtype="float8_e4m3fn")
+    pages = c.allocate([20])
+    for d in (copy.deepcopy(c), pickle.loads(pickle.dumps(c))):
+        assert d[0].k.data_ptr() != c[0].k.data_ptr() and d.free_pages == 0 and d.dtype == c.dtype
+        F.paged_kv_write(*(genesis.Tensor(torch.ones(1, 20, 1, 8)) for _ in range(2)), d[0], d.page_table(pages), _i(20))
+        assert torch.all(c[0].k.view(torch.uint8) == 0) and int((d[0].k.view(torch.uint8) != 0).sum()) == 160
+    with pytest.raises(AttributeError):
+        c[0].k = torch.zeros(1)
+
+
 # ---- 8 bits --------------------------------------------------------------------------------------
 def test_rows_of_8_bits_are_rounded_once():
     g = torch.Generator().manual_seed(1)

@@ -69,3 +69,23 @@ def test_ragged_prompts_pieces_and_single_tokens(kind):
                 for s in range(n):
                     assert torch.allclose(out[b, s], full[b][have[b] - n + s], atol=1e-4)
     assert have[2] == 40
+
+
+def test_positions_behind_the_rotation_tables():
+    """A page table with more room than the tables: they grow, and the old ones stay for whoever reads them."""
+    m = _model("dense")
+    rot = m.model.layers[0].self_attn.rotary_emb
+    old = rot.cos_cached
+    tokens = torch.randint(0, 97, (1, 70), generator=torch.Generator().manual_seed(3))
+    with genesis.no_grad():
+        cache = PagedKVCache(6, 2, 16, page_size=16, num_layers=2, dtype="float32")
+        table = cache.page_table(cache.allocate([96]))
+        m.forward_paged(genesis.Tensor(tokens[:, :69]), cache, table, _ints(69), prompt=True)
+        out = m.forward_paged(genesis.Tensor(tokens[:, 69:]), cache, table, _ints(70))
+        assert rot.max_seq_len_cached >= 96 and rot._outgrown[0][0] is old
+        assert torch.allclose(out._t[0, 0], m(genesis.Tensor(tokens))._t[0, 69], atol=1e-4)
+        # padding behind the prompt may be longer than the table has room for
+        cache = PagedKVCache(1, 2, 16, page_size=16, num_layers=2, dtype="float32")
+        table = cache.page_table(cache.allocate([5]))
+        short = m.forward_paged(genesis.Tensor(tokens[:, :40]), cache, table, _ints(5), _ints(5), prompt=True)
+        assert torch.allclose(short._t[0, 0], m(genesis.Tensor(tokens[:, :5]))._t[0, 4], atol=1e-4)
