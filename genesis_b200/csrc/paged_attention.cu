@@ -220,7 +220,7 @@ paged_attend_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_consta
   using C = PA<T, CDT, D, NQ>;
   constexpr int R = C::R, KT = C::KT, NS = C::NS, KL = C::KL, VW = C::VW, MT = C::MT, QS = C::QS, GP = C::GP, W = PA_WARPS;
   extern __shared__ __align__(1024) uint8_t shared[];              // [W][RING], [W][ST][SB]
-  __shared__ uint64_t landed[W][C::ST][2];                           // K's and V's copies of a stage have landed
+  __shared__ uint64_t landed[W][2][C::ST];                         // K's and V's copies of a stage have landed
   __shared__ int abort_word[W];
   uint8_t* const rings = shared + (1024 - (smem_u32(shared) & 1023)) % 1024;
   __shared__ const float* piece_at[2 * W];                         // [R][D] sums: in the ring of the warp, or in the workspace
@@ -274,7 +274,8 @@ paged_attend_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_consta
   volatile int* const abort_flag = &abort_word[warp];
   uint8_t* const ring = rings + warp * C::RING;
   uint8_t* const powers = rings + W * C::RING + warp * C::ST * C::SB;
-  int put = 0, put_phase = 0, use = 0, use_phase = 0;              // stage of the next chunk that is copied and of the one that is worked on
+  int put = 0, use = 0, use_phase = 0;                             // stage of the next chunk that is copied and of the one that is worked on
+  unsigned k_copies = 0, v_copies = 0;                             // so far
   const float sl2 = a.scale * 1.4426950408889634f;
   const int rows = c.S * plan.group.d;
 
@@ -344,7 +345,6 @@ paged_attend_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_consta
 
     // one round: scores of chunk ch, then K of chunk ch + ST into its place; probabilities and products of ch, then V of ch + ST.
     uint32_t gone_later = 0;           // tiles that are not there, of the chunks in flight
-    bool ahead = false;                // given up with a K on its way whose V has not been asked for
     for (int ch = c0 - C::ST; ch < c1; ++ch) {
       const bool now = ch >= c0, more = ch + C::ST < c1;
       uint8_t* const sk = ring + use * 2 * C::KB;
@@ -394,7 +394,7 @@ paged_attend_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_consta
         }
       }
       if (now) {
-        if (!__all_sync(0xffffffffu, mbar_wait(&landed[warp][use][0], use_phase, abort_flag, c.status, 81))) break;
+        if (!__all_sync(0xffffffffu, mbar_wait(&landed[warp][0][use], use_phase, abort_flag, c.status, 81))) break;
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
           float small[NQ][4] = {};
@@ -456,7 +456,7 @@ paged_attend_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_consta
       }
       __syncwarp();                    // all have read
       if (more) {
-        uint64_t* const bar = &landed[warp][put][0];
+        uint64_t* const bar = &landed[warp][0][put];
         uint8_t* const dk = ring + put * 2 * C::KB;
         int tiles = 0;
 #pragma unroll
@@ -482,6 +482,7 @@ paged_attend_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_consta
             }
           }
         }
+        ++k_copies;
         ask();
       }
       if (now) {
@@ -592,10 +593,7 @@ paged_attend_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_consta
         constexpr int TW = C::E8 ? 2 : 1;              // tiles of O^T that a word of V has numbers of
         alignas(16) uint32_t vr[NS][4][4];
         uint32_t bad = 0;
-        if (!__all_sync(0xffffffffu, mbar_wait(&landed[warp][use][1], use_phase, abort_flag, c.status, 82))) {
-          ahead = more;
-          break;
-        }
+        if (!__all_sync(0xffffffffu, mbar_wait(&landed[warp][1][use], use_phase, abort_flag, c.status, 82))) break;
 #pragma unroll
         for (int j = 0; j < VW; j += C::F32 ? 2 : 1) {
           constexpr int VN = VW == 2 ? 2 : 4;         // words that a lane has of a key side by side
@@ -679,7 +677,7 @@ paged_attend_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_consta
       __syncwarp();
       if (more) {
         if (lane == 0) {
-          uint64_t* const bar = &landed[warp][put][1];
+          uint64_t* const bar = &landed[warp][1][put];
           uint8_t* const dv = ring + put * 2 * C::KB + C::KB;
           int tiles = 0;
 #pragma unroll
@@ -692,19 +690,14 @@ paged_attend_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_consta
             for (int x = 0; x < C::RB / C::BOX; ++x) tma_load_2d(dv + i * 16 * C::RB + x * 2048, &tmv, bar, x * (C::BOX / C::ES), (int)row[i]);
           }
         }
-        if (++put == C::ST) { put = 0; put_phase ^= 1; }
+        ++v_copies;
+        if (++put == C::ST) put = 0;
       }
       if (now && ++use == C::ST) { use = 0; use_phase ^= 1; }
     }
     if (__any_sync(0xffffffffu, *abort_flag)) {      // gave up: the copies in flight land first, and nothing is kept
-      if (lane == 0) {
-        const uint64_t t0 = globaltimer_ns();
-        for (int i = 0; i < C::ST; ++i)
-          for (int w = 0; w < 2; ++w) {
-            const int phase = i < put || (i == put && w == 0 && ahead) ? put_phase : put_phase ^ 1;       // of the last copy into stage i
-            while (!mbar_try_wait(&landed[warp][i][w], phase) && globaltimer_ns() - t0 < 1000000ull) {}
-          }
-      }
+      drain_copies(&landed[warp][0][0], C::ST, k_copies);
+      drain_copies(&landed[warp][1][0], C::ST, v_copies);
       __syncwarp();
       break;
     }
