@@ -2055,8 +2055,9 @@ def paged_qkv_rope(y, cos, sin, cache, page_table, lengths, num_heads, counts=No
 
 
 def paged_kv_read(cache, page_table, lengths, max_length, dtype=None):
-    """(k, v) [B, max_length, Hkv, D] of the sequences' first `max_length` tokens, zeros behind each one's end: what the flash attention takes
-    for the next piece of a long prompt.  `dtype`: float32, float16 or bfloat16; the cache's, or bfloat16 for 8 bits (exact)."""
+    """(k, v) [B, max_length, Hkv, D] of the sequences' first `max_length` tokens, zeros behind each one's end: what the flash attention
+    takes for the next piece of a long prompt.  `dtype`: float32, float16 or bfloat16; the cache's, or bfloat16 for 8 bits (exact).
+    Tokens whose page or position does not exist come out as zeros, and the error is raised as `paged_kv_write` says."""
     name = "paged_kv_read"
     table, lengths, _ = _paged_args(name, cache, page_table, lengths, None, None, cache._call[0] if isinstance(cache, PagedKVLayer) else -1)
     if isinstance(max_length, bool) or not isinstance(max_length, int) or not 0 <= max_length < 2 ** 31:
@@ -2074,8 +2075,9 @@ def paged_attention(q, cache, page_table, lengths, counts=None, scale=None):
     `lengths` counts the tokens in the cache, those of this call (written before) among them; with `counts` [B] only the first
     counts[b] of the S are real.  Token s sees the positions up to its own, lengths[b] - counts[b] + s; a token that is none,
     or whose scores are -inf throughout, gives zeros.  Hkv divides Hq; `scale` is D ** -0.5 unless given.  Probabilities are
-    formed and summed in 32 bits.  Made for few tokens; where S runs into the hundreds the flash attention over what
-    `paged_kv_read` brings back is faster."""
+    formed and summed in 32 bits.  Keys whose page or position does not exist take no part, and the error is raised as
+    `paged_kv_write` says.  Made for few tokens; where S runs into the hundreds the flash attention over what `paged_kv_read`
+    brings back is faster."""
     name = "paged_attention"
     q = _paged_tokens(name, "q", q, 4)
     table, lengths, counts = _paged_args(name, cache, page_table, lengths, counts, q.shape[0], q.get_device())

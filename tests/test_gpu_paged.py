@@ -296,6 +296,25 @@ def test_queries_that_are_views():
         assert torch.equal(F.paged_attention(genesis.Tensor(x), t.layer, t.table, t.lens)._t, want)
 
 
+@pytest.mark.parametrize("dtype,cache", [("bf16", "bf16"), ("bf16", "e4m3")])
+def test_thousands_of_sequences(dtype, cache):
+    """More sequences than a warp has lanes, a hundred times over; every seventh rests."""
+    g = torch.Generator().manual_seed(8)
+    lengths = torch.randint(1, 60, (3300,), generator=g)
+    lengths[::7] = 0
+    lengths[1234] = 5000
+    t = R.Setup(lengths.tolist(), 1, 64, cache, 16, "cuda")
+    _attend(t, lengths.tolist(), None, 1, 4, 64, dtype, cache)
+
+
+@pytest.mark.parametrize("dtype,cache", [("bf16", "bf16"), ("fp16", "e4m3")])
+def test_one_head_and_many_rows(dtype, cache):
+    """64 query heads on one KV head, four tokens: sixteen tiles of rows that read the same keys."""
+    for width in (0, 30000):
+        t = R.Setup([130, 77], 1, 128, cache, 16, "cuda", width=width)
+        _attend(t, [130, 77], None, 4, 64, 128, dtype, cache)
+
+
 # ---- bad pages, far pages ------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype,cache,D", [("bf16", "bf16", 64), ("fp16", "e4m3", 128), ("fp32", "fp32", 16)])
 def test_bad_pages_are_skipped_and_raised(dtype, cache, D):
