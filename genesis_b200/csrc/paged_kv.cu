@@ -21,8 +21,8 @@ struct PutArgs {
   void* q_out;             // [B, S, Hq, D]
   void *kpool, *vpool;
   uint8_t *kscale, *vscale;
-  const float *cosb, *sinb;     // [positions, D], halves equal; null: no rotation, Hq = 0
-  int positions, Hq;
+  const float *cosb, *sinb;     // [positions, D], halves equal (null where positions is 0)
+  int positions, Hq;            // Hq = 0: keys and values only, not rotated
 };
 
 // N numbers (4 or 8) in 32 bits into a pool, in its type; e4m3 under the power of two 1 / inv, with infinities and NaN among them as
@@ -153,7 +153,7 @@ __global__ void paged_put_any_kernel(const PutArgs a, const Paged c) {
     const int n = c.count(b);
     const long long pos = (long long)c.length(b) - n + s;
     bool live = s < n && pos >= 0;
-    const bool rot = a.cosb != nullptr && (isq || isk);
+    const bool rot = a.Hq > 0 && (isq || isk);
     if (live && rot && pos >= a.positions) {
       if (lane == 0) report_error(c.status, GB_ERR_BAD_INDEX, SITE_POSITION, (int)pos);
       live = false;
@@ -308,7 +308,7 @@ static int paged_put(const PutArgs& a, const Paged& c, const PagedPools& p, int 
     const int each = 256 >> log;
     const unsigned grid = (unsigned)((rows + each - 1) / each);
     const Div heads(Ht), per(c.S);
-    if (a.cosb != nullptr) GB_DISPATCH_FLOAT(dt, T, GB_DISPATCH_CACHE(p.type, C, paged_put_rows_kernel<T, C, true><<<grid, 256, 0, st>>>(a, c, heads, per, (int)rows, log)));
+    if (a.Hq > 0) GB_DISPATCH_FLOAT(dt, T, GB_DISPATCH_CACHE(p.type, C, paged_put_rows_kernel<T, C, true><<<grid, 256, 0, st>>>(a, c, heads, per, (int)rows, log)));
     else GB_DISPATCH_FLOAT(dt, T, GB_DISPATCH_CACHE(p.type, C, paged_put_rows_kernel<T, C, false><<<grid, 256, 0, st>>>(a, c, heads, per, (int)rows, log)));
     return (int)cudaGetLastError();
   }
