@@ -27,12 +27,31 @@ def rotate_half(x):
     return F.cat((-x[..., d:], x[..., :d]), dim=-1)
 
 
+class _Outgrown:
+    """Pairs of tables that larger ones have replaced, held for captured steps that go on reading them.  A module looks for its
+    buffers in lists, tuples and dicts too, and saves, converts and moves what it finds; it does not look in here."""
+    __slots__ = ("_pairs",)
+
+    def __init__(self):
+        self._pairs = []
+
+    def __len__(self):
+        return len(self._pairs)
+
+    def __getitem__(self, i):
+        return self._pairs[i]
+
+    def append(self, pair):
+        self._pairs.append(pair)
+
+
 class RotaryEmbedding(nn.Module):
     def __init__(self, dim, max_position_embeddings=2048, base=10000.0, device=None):
         super().__init__()
         self.dim, self.base = dim, float(base)
         self.max_position_embeddings = max_position_embeddings
         self._device = device
+        self._outgrown = _Outgrown()
         self._build(max_position_embeddings)
 
     def _build(self, seq_len):
@@ -88,7 +107,7 @@ def paged_self_attention(y, rotary, num_heads, cache, page_table, lengths, count
     room = max(S, page_table.shape[1] * cache.page_size)
     if room > rotary.max_seq_len_cached:
         # (a captured step may go on reading the tables that are outgrown)
-        rotary.__dict__.setdefault("_outgrown", []).append((rotary.cos_cached, rotary.sin_cached))
+        rotary._outgrown.append((rotary.cos_cached, rotary.sin_cached))
         rotary._build(room)
     cos, sin = rotary.cos_cached, rotary.sin_cached
     if prompt:

@@ -1,9 +1,12 @@
 """Calls on a paged cache at the edges of what their documentation allows, on the CPU."""
+import copy
+
 import pytest
 import torch
 
 import genesis_b200 as genesis
 import genesis_b200.nn.functional as F
+from genesis_b200.models.transformers import MoEConfig, MoEForCausalLM, QwenForCausalLM, TransformerConfig
 
 import _paged_ref as R
 
@@ -17,3 +20,38 @@ def test_rotation_tables_without_a_position():
     assert torch.equal(R.values(t.layer.k, None).nan_to_num(7e9), before.nan_to_num(7e9))
     q = F.paged_qkv_rope(y, none, none, t.layer, t.table, t.ints([0, 0]), 4)      # no token: nothing to rotate
     assert torch.all(q._t == 0)
+
+
+# ---- rotation tables of a model ------------------------------------------------------------------
+def _model(kind, positions=64, seed=11):
+    genesis.manual_seed(seed)
+    base = dict(vocab_size=97, hidden_size=64, intermediate_size=96, num_hidden_layers=2, num_attention_heads=4,
+                num_key_value_heads=2, head_dim=16, max_position_embeddings=positions, rope_theta=1e4)
+    if kind == "dense":
+        return QwenForCausalLM(TransformerConfig(**base)).eval()
+    return MoEForCausalLM(MoEConfig(**base, num_experts_per_tok=2, num_local_experts=4, moe_intermediate_size=48)).eval()
+
+
+def _rotaries(m):
+    return [layer.self_attn.rotary_emb for layer in m.model.layers]
+
+
+def _tokens(*shape, seed=3):
+    return genesis.Tensor(torch.randint(0, 97, shape, generator=torch.Generator().manual_seed(seed)))
+
+
+@pytest.mark.parametrize("kind", ["dense", "moe"])
+def test_outgrown_tables_are_no_part_of_a_checkpoint(kind):
+    m = _model(kind)
+    keys, buffers = list(m.state_dict()), [n for n, _ in m.named_buffers()]
+    m.generate(_tokens(2, 5), max_new_tokens=70, temperature=0.0, cache_dtype="float32")
+    assert _rotaries(m)[0].max_seq_len_cached > 64
+    assert list(m.state_dict()) == keys and [n for n, _ in m.named_buffers()] == buffers
+    fresh = _model(kind, seed=12)
+    assert fresh.load_state_dict(m.state_dict()) == ([], []) and m.load_state_dict(fresh.state_dict()) == ([], [])
+    twin = copy.deepcopy(m)
+    assert list(twin.state_dict()) == keys
+    # what a captured step reads is neither converted nor moved
+    kept = [(t, t._t) for pair in _rotaries(m)[0]._outgrown for t in pair]
+    m.bfloat16()
+    assert kept and all(t._t is raw for t, raw in kept)
