@@ -63,6 +63,7 @@ class RotaryEmbedding(nn.Module):
         old = self.__dict__.get("cos_cached")
         if old is not None:
             dev = old.device
+            self._outgrown.append((old, self.sin_cached))
         self.max_seq_len_cached = seq_len
         self.register_buffer("inv_freq", tensor(inv.astype(np.float32), device=dev), persistent=False)
         self.register_buffer("cos_cached", tensor(np.cos(emb).astype(np.float32), device=dev), persistent=False)
@@ -106,8 +107,6 @@ def paged_self_attention(y, rotary, num_heads, cache, page_table, lengths, count
     B, S, _ = y.shape
     room = max(S, page_table.shape[1] * cache.page_size)
     if room > rotary.max_seq_len_cached:
-        # (a captured step may go on reading the tables that are outgrown)
-        rotary._outgrown.append((rotary.cos_cached, rotary.sin_cached))
         rotary._build(room)
     cos, sin = rotary.cos_cached, rotary.sin_cached
     if prompt:

@@ -1,5 +1,7 @@
 """Calls on a paged cache at the edges of what their documentation allows, on the CPU."""
 import copy
+import gc
+import weakref
 
 import pytest
 import torch
@@ -7,6 +9,8 @@ import torch
 import genesis_b200 as genesis
 import genesis_b200.nn.functional as F
 from genesis_b200.models.transformers import MoEConfig, MoEForCausalLM, QwenForCausalLM, TransformerConfig
+from genesis_b200.models.transformers.components import apply_rope
+from genesis_b200.nn import PagedKVCache
 
 import _paged_ref as R
 
@@ -32,6 +36,10 @@ def _model(kind, positions=64, seed=11):
     return MoEForCausalLM(MoEConfig(**base, num_experts_per_tok=2, num_local_experts=4, moe_intermediate_size=48)).eval()
 
 
+def _ints(*xs):
+    return genesis.Tensor(torch.tensor(xs, dtype=torch.int32))
+
+
 def _rotaries(m):
     return [layer.self_attn.rotary_emb for layer in m.model.layers]
 
@@ -55,3 +63,24 @@ def test_outgrown_tables_are_no_part_of_a_checkpoint(kind):
     kept = [(t, t._t) for pair in _rotaries(m)[0]._outgrown for t in pair]
     m.bfloat16()
     assert kept and all(t._t is raw for t, raw in kept)
+
+
+@pytest.mark.parametrize("kind", ["dense", "moe"])
+@pytest.mark.parametrize("grow", ["forward", "forward_paged", "rotary", "apply_rope"])
+def test_outgrown_tables_stay_whoever_outgrows_them(kind, grow):
+    """A captured step reads the tables it was captured with, whichever call replaces them."""
+    m = _model(kind)
+    cache = PagedKVCache(8, 2, 16, page_size=16, num_layers=2, dtype="float32")
+    with genesis.no_grad():
+        m.forward_paged(_tokens(1, 5), cache, cache.page_table(cache.allocate([64])), _ints(5), prompt=True)
+        old = [weakref.ref(t._t) for rot in _rotaries(m) for t in (rot.cos_cached, rot.sin_cached)]
+        if grow == "forward":
+            m(_tokens(1, 65))
+        elif grow == "forward_paged":
+            m.forward_paged(_tokens(1, 70), cache, cache.page_table(cache.allocate([5])), _ints(5), _ints(5), prompt=True)
+        else:
+            for rot in _rotaries(m):
+                rot(seq_len=65) if grow == "rotary" else apply_rope(genesis.Tensor(torch.zeros(1, 65, 2, 16)), rot)
+    assert all(rot.max_seq_len_cached >= 65 for rot in _rotaries(m))
+    gc.collect()
+    assert all(r() is not None for r in old)
