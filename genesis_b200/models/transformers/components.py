@@ -69,9 +69,14 @@ class RotaryEmbedding(nn.Module):
         self.register_buffer("cos_cached", tensor(np.cos(emb).astype(np.float32), device=dev), persistent=False)
         self.register_buffer("sin_cached", tensor(np.sin(emb).astype(np.float32), device=dev), persistent=False)
 
+    def reserve(self, seq_len):
+        """Makes the tables reach so many positions.  They at least double, so that all outgrown ones together are no larger."""
+        if seq_len > self.max_seq_len_cached:
+            self._build(max(seq_len, 2 * self.max_seq_len_cached))
+
     def forward(self, x=None, seq_len=None):
-        if seq_len is not None and seq_len > self.max_seq_len_cached:
-            self._build(seq_len)
+        if seq_len is not None:
+            self.reserve(seq_len)
         if seq_len is None:
             return self.cos_cached, self.sin_cached
         return self.cos_cached[:seq_len], self.sin_cached[:seq_len]
@@ -94,8 +99,7 @@ def apply_rotary_pos_emb(q, k, cos, sin, position_ids=None):
 def apply_rope(x, rotary, position_ids=None):
     """Fused rotate-half RoPE on x [B, S, H, D]."""
     S = x.shape[1]
-    if S > rotary.max_seq_len_cached:
-        rotary._build(S)
+    rotary.reserve(S)
     pos = None if position_ids is None else position_ids
     return F.rope(x, rotary.cos_cached, rotary.sin_cached, pos)
 
@@ -105,9 +109,7 @@ def paged_self_attention(y, rotary, num_heads, cache, page_table, lengths, count
     num_heads * D].  The tokens' keys and values are put into the cache; with `prompt` the sequences have no others, and the
     flash attention over the call's own keys takes the place of reading them back."""
     B, S, _ = y.shape
-    room = max(S, page_table.shape[1] * cache.page_size)
-    if room > rotary.max_seq_len_cached:
-        rotary._build(room)
+    rotary.reserve(max(S, page_table.shape[1] * cache.page_size))
     cos, sin = rotary.cos_cached, rotary.sin_cached
     if prompt:
         q, k, v = F.qkv_rope(y, cos, sin, None, num_heads, cache.num_kv_heads, cache.head_dim)

@@ -49,8 +49,7 @@ class Attention(nn.Module):
         B, S, _ = x.shape
         y = self._projected(x)
         rot = self.rotary_emb
-        if S > rot.max_seq_len_cached:
-            rot._build(S)
+        rot.reserve(S)
         q, k, v = F.qkv_rope(y, rot.cos_cached, rot.sin_cached, position_ids, self.num_heads, self.num_kv_heads,
                              self.head_dim)
         o = F.flash_attention(q, k, v, causal=True)

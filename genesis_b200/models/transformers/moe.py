@@ -384,9 +384,7 @@ class MoEAttention(Module):
             position_ids = Tensor._wrap(torch.arange(past, past + S, device=hidden_states._t.device).expand(B, S).contiguous())
         y = self._projected(hidden_states)
         rot = self.rotary_emb
-        need = S + past if position_ids is None else S + past
-        if need > rot.max_seq_len_cached:
-            rot._build(need)
+        rot.reserve(S + past)
         q, k, v = F.qkv_rope(y, rot.cos_cached, rot.sin_cached, position_ids, self.num_heads,
                              self.num_key_value_heads, self.head_dim)
         if past_key_value is not None:

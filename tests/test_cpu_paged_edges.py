@@ -84,3 +84,24 @@ def test_outgrown_tables_stay_whoever_outgrows_them(kind, grow):
     assert all(rot.max_seq_len_cached >= 65 for rot in _rotaries(m))
     gc.collect()
     assert all(r() is not None for r in old)
+
+
+def test_what_is_kept_of_outgrown_tables_is_bounded():
+    """A table of pages that widens page by page: a few pairs, which together are no larger than the present ones."""
+    m = _model("dense", positions=32)
+    cache = PagedKVCache(40, 2, 16, page_size=16, num_layers=2, dtype="float32")
+    pages = cache.allocate([5])
+    with genesis.no_grad():
+        m.forward_paged(_tokens(1, 5), cache, cache.page_table(pages), _ints(5), prompt=True)
+        for n in range(6, 500):
+            cache.extend(pages, [n])
+            if n % 16 == 1:
+                m.forward_paged(_tokens(1, 1), cache, cache.page_table(pages), _ints(n))
+    for rot in _rotaries(m):
+        assert 497 <= rot.max_seq_len_cached <= 1024 and 1 <= len(rot._outgrown) <= 5
+        assert sum(cos.shape[0] for cos, _ in rot._outgrown) <= rot.max_seq_len_cached
+    plain = _model("dense", positions=32)
+    with genesis.no_grad():
+        for n in range(33, 200, 7):
+            plain(_tokens(1, n))
+    assert all(len(rot._outgrown) <= 3 and rot.max_seq_len_cached == 256 for rot in _rotaries(plain))
