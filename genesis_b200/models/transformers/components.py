@@ -27,9 +27,9 @@ def rotate_half(x):
     return F.cat((-x[..., d:], x[..., :d]), dim=-1)
 
 
-class _Outgrown:
-    """Pairs of tables that larger ones have replaced, held for captured steps that go on reading them.  A module looks for its
-    buffers in lists, tuples and dicts too, and saves, converts and moves what it finds; it does not look in here."""
+class _Unseen:
+    """Pairs of tables that are none of a module's buffers.  A module looks for those in lists, tuples and dicts too, and saves,
+    converts and moves what it finds; it does not look in here."""
     __slots__ = ("_pairs",)
 
     def __init__(self):
@@ -51,28 +51,42 @@ class RotaryEmbedding(nn.Module):
         self.dim, self.base = dim, float(base)
         self.max_position_embeddings = max_position_embeddings
         self._device = device
-        self._outgrown = _Outgrown()
+        self._outgrown = _Unseen()      # what larger tables have replaced: captured steps go on reading it
+        self._exact = _Unseen()         # tables in 32 bits of a module that was converted to 16
         self._build(max_position_embeddings)
 
-    def _build(self, seq_len):
+    def _values(self, seq_len, dev):
+        """(inverse frequencies, cos, sin) in 32 bits."""
         inv = 1.0 / (self.base ** (np.arange(0, self.dim, 2, dtype=np.float64) / self.dim))
         t = np.arange(seq_len, dtype=np.float64)
         freqs = np.outer(t, inv)
         emb = np.concatenate([freqs, freqs], axis=-1)
+        return [tensor(x.astype(np.float32), device=dev) for x in (inv, np.cos(emb), np.sin(emb))]
+
+    def _build(self, seq_len):
         dev = self._device
         old = self.__dict__.get("cos_cached")
         if old is not None:
             dev = old.device
             self._outgrown.append((old, self.sin_cached))
         self.max_seq_len_cached = seq_len
-        self.register_buffer("inv_freq", tensor(inv.astype(np.float32), device=dev), persistent=False)
-        self.register_buffer("cos_cached", tensor(np.cos(emb).astype(np.float32), device=dev), persistent=False)
-        self.register_buffer("sin_cached", tensor(np.sin(emb).astype(np.float32), device=dev), persistent=False)
+        for name, values in zip(("inv_freq", "cos_cached", "sin_cached"), self._values(seq_len, dev)):
+            self.register_buffer(name, values, persistent=False)
 
     def reserve(self, seq_len):
         """Makes the tables reach so many positions.  They at least double, so that all outgrown ones together are no larger."""
         if seq_len > self.max_seq_len_cached:
             self._build(max(seq_len, 2 * self.max_seq_len_cached))
+
+    def tables32(self):
+        """(cos, sin) in 32 bits, which the paged operators take, also where the module was converted to 16 (in bfloat16 a cosine
+        is up to 2^-9 off, at every position)."""
+        cos = self.cos_cached
+        if cos._t.dtype is torch.float32:
+            return cos, self.sin_cached
+        if not len(self._exact) or self._exact[-1][0].shape != cos.shape or self._exact[-1][0].device != cos.device:
+            self._exact.append(tuple(self._values(cos.shape[0], cos.device)[1:]))
+        return self._exact[-1]
 
     def forward(self, x=None, seq_len=None):
         if seq_len is not None:
@@ -110,7 +124,7 @@ def paged_self_attention(y, rotary, num_heads, cache, page_table, lengths, count
     flash attention over the call's own keys takes the place of reading them back."""
     B, S, _ = y.shape
     rotary.reserve(max(S, page_table.shape[1] * cache.page_size))
-    cos, sin = rotary.cos_cached, rotary.sin_cached
+    cos, sin = rotary.tables32()
     if prompt:
         q, k, v = F.qkv_rope(y, cos, sin, None, num_heads, cache.num_kv_heads, cache.head_dim)
         F.paged_kv_write(k, v, cache, page_table, lengths, counts)

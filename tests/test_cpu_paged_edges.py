@@ -105,3 +105,31 @@ def test_what_is_kept_of_outgrown_tables_is_bounded():
         for n in range(33, 200, 7):
             plain(_tokens(1, n))
     assert all(len(rot._outgrown) <= 3 and rot.max_seq_len_cached == 256 for rot in _rotaries(plain))
+
+
+@pytest.mark.parametrize("kind", ["dense", "moe"])
+@pytest.mark.parametrize("half", ["bfloat16", "half"])
+def test_models_converted_to_16_bits(kind, half):
+    """forward_paged rotates by tables in 32 bits, whatever the module's buffers were converted to."""
+    answers = []
+    for rebuilt in (False, True):
+        m = getattr(_model(kind), half)()
+        assert _rotaries(m)[0].cos_cached._t.dtype != torch.float32
+        keys = list(m.state_dict())
+        if rebuilt:                                     # the same model with its buffers in 32 bits
+            for rot in _rotaries(m):
+                rot._build(64)
+        cache = PagedKVCache(8, 2, 16, page_size=16, num_layers=2, dtype="float16")
+        table, tokens = cache.page_table(cache.allocate([60, 60])), _tokens(2, 34)
+        with genesis.no_grad():
+            got = [m.forward_paged(tokens[:, :30], cache, table, _ints(30, 30), prompt=True)._t]
+            got += [m.forward_paged(tokens[:, n - 1:n], cache, table, _ints(n, n))._t for n in (31, 32, 33, 34)]
+        answers.append(torch.cat(got, 1))
+        assert list(m.state_dict()) == keys
+        assert all(len(rot._exact) == (0 if rebuilt else 1) for rot in _rotaries(m))
+        out = m.generate(_tokens(2, 5), max_new_tokens=4, temperature=0.0, cache_dtype="bfloat16")
+        assert out.shape == (2, 9)
+        # tables that are outgrown after the conversion
+        assert m.generate(_tokens(1, 70), max_new_tokens=2, temperature=0.0, cache_dtype="float8_e4m3fn").shape == (1, 72)
+    assert answers[0].dtype == getattr(torch, "float16" if half == "half" else half)
+    assert torch.equal(*answers)

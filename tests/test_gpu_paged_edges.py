@@ -97,3 +97,33 @@ def test_a_captured_step_after_a_plain_call_outgrows_the_tables(kind):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out._t, want) and rubbish
+
+
+@pytest.mark.parametrize("kind", ["dense", "moe"])
+@pytest.mark.parametrize("half,cache_dtype", [("bfloat16", "bfloat16"), ("half", "float16"), ("bfloat16", "float8_e4m3fn")])
+def test_models_converted_to_16_bits(kind, half, cache_dtype):
+    """Generation and a captured step of a model in 16 bits; its answers are those of the same model with tables in 32."""
+    answers = []
+    for rebuilt in (False, True):
+        m = getattr(_model(kind), half)()
+        if rebuilt:
+            for layer in m.model.layers:
+                layer.self_attn.rotary_emb._build(256)
+        with genesis.no_grad():
+            cache, table, lengths = _prompted(m, (5, 40), 20, cache_dtype)
+            keep, toks = lengths._t.clone(), genesis.Tensor(_tokens(2, 1, seed=4))
+
+            def step():
+                lengths._t += 1
+                return m.forward_paged(toks, cache, table, lengths)
+
+            want = step()._t.clone()
+            lengths._t.copy_(keep)
+            graph, out = _captured(step, lengths, keep)
+            graph.replay()
+            assert torch.equal(out._t, want)
+            answers.append(want)
+        prompt = genesis.Tensor(_tokens(2, 9))
+        assert m.generate(prompt, max_new_tokens=4, temperature=0.0, cache_dtype=cache_dtype).shape == (2, 13)
+        del graph
+    assert torch.equal(*answers)
