@@ -154,7 +154,7 @@ __global__ void paged_put_any_kernel(const PutArgs a, const Paged c) {
     const long long pos = (long long)c.length(b) - n + s;
     bool live = s < n && pos >= 0;
     const bool rot = a.Hq > 0 && (isq || isk);
-    if (live && rot && pos >= a.positions) {
+    if (live && a.Hq > 0 && pos >= a.positions) {
       if (lane == 0) report_error(c.status, GB_ERR_BAD_INDEX, SITE_POSITION, (int)pos);
       live = false;
     }

@@ -34,6 +34,23 @@ def test_rotation_tables_without_a_position(D, cache):
     assert torch.all(q._t == 0) and all(torch.equal(a, b) for a, b in zip(_bits(t), before))
 
 
+@pytest.mark.parametrize("cache", ["bf16", "e4m3"])
+@pytest.mark.parametrize("D", [64, 6])
+def test_a_token_behind_the_rotation_tables_is_put_nowhere(D, cache):
+    """Neither its key nor its value; the tokens before it are put as ever."""
+    t = R.Setup([20, 4], 2, D, cache, 16, "cuda")
+    y, table = t.tensor(t.normal(2, 3, 8 * D)), t.tensor(torch.ones(18, D))
+    before = _bits(t)
+    F.paged_qkv_rope(y, table, table, t.layer, t.table, t.lens, 4)
+    with pytest.raises(IndexError, match="site=9"):
+        N.check_status()
+    for old, new in zip(before, _bits(t)):
+        same = (old == new).flatten(3).all(-1).all(1).cpu()             # [pages, places]
+        want = torch.ones_like(same)
+        want[t.pages[0][1], 1] = want[t.pages[1][0], 1] = want[t.pages[1][0], 2] = want[t.pages[1][0], 3] = False
+        assert torch.equal(same, want)
+
+
 # ---- models --------------------------------------------------------------------------------------
 def _model(kind, positions=256, head_dim=64):
     genesis.manual_seed(11)
