@@ -26,6 +26,8 @@
 //              below a bf16 output.  fp16 P is scaled by 2^7 on top of a maximum that may lag 2^8 behind, so that 2^-31 of the
 //              largest probability is still a number.  e4m3 becomes fp16 exactly; a bf16 q does under a power of two for each
 //              row.  K's powers of two multiply scores, V's multiply P, relative to the largest seen so far.
+//   infinities and NaN among queries, keys and values come out as the definition has them (a key of score -inf weighs nothing, one
+//              with any weight gives its infinity): a warp that meets some works its share over once more.
 #include "attention_common.cuh"
 #include "paged_common.cuh"
 #include <type_traits>
@@ -202,6 +204,7 @@ __device__ __forceinline__ int attend_chunks(int keys, int kt) { return keys == 
 template <typename T>
 __device__ __forceinline__ void store_row4(const AttendArgs& a, const Paged& c, const Div& group, int b, int kvh, int r, int d, float4 o, float l) {
   const int s = group.by(r);
+  if (l == 0.f) o = make_float4(0.f, 0.f, 0.f, 0.f);       // (scores of -inf throughout, whatever the values hold)
   const float inv = l == 0.f ? 0.f : 1.f / l;
   T* p = reinterpret_cast<T*>(a.o) + (((long long)b * c.S + s) * a.Hq + kvh * group.d + r - s * group.d) * c.D + d;
   if constexpr (std::is_same<T, float>::value) {
@@ -212,11 +215,122 @@ __device__ __forceinline__ void store_row4(const AttendArgs& a, const Paged& c, 
   }
 }
 
+// A warp's share once more, number by number in 32 bits: where keys, values or queries are infinite, what the loop over the
+// tensor cores has made of them is put right, in a run's sums (the last in the ring, others in `spill`, maxima and normalisers
+// at m and l) or in the output.  Only rows and columns that are not finite, or were not to be, are replaced.  A row whose scores are
+// NaN stays so, and is not followed to its end.  About a microsecond a key, which only such numbers pay for.
+template <typename T, int CDT, int D, int R, int KT>
+__device__ __noinline__ void redo_share(const AttendArgs& a, const Paged& c, const AttendPlan& plan, unsigned u, unsigned u_end, float* ring,
+                                        float* spill, float* m, float* l) {
+  constexpr int N = D / 32, G = 8;     // columns of a lane, rows at a time
+  const int lane = threadIdx.x & 31, rows = c.S * (int)plan.group.d;
+  const float sl2 = a.scale * 1.4426950408889634f;
+  int b = 0, slot = 0;
+  unsigned seq_start = 0;
+  auto load = [](const void* pool, long long at) {
+    if constexpr (CDT == DT_E4M3) return from_e4m3x2(reinterpret_cast<const uint8_t*>(pool)[at]).x;
+    else return load_as_float(pool, CDT, at);
+  };
+  auto finite = [](float x) { return fabsf(x) < INFINITY; };
+  while (u < u_end) {
+    const int keys = attend_keys(c, b), n = attend_chunks(keys, KT);
+    if (u - seq_start >= (unsigned)n * plan.per_seq) {
+      seq_start += (unsigned)n * plan.per_seq;
+      if (++b >= c.B) break;
+      continue;
+    }
+    const int idx = (int)((u - seq_start) / (unsigned)n);
+    const int c0 = (int)(u - seq_start - (unsigned)idx * n), c1 = min(n, c0 + (int)(u_end - u));
+    const int kvh = plan.tile.by(idx), row0 = (idx - kvh * plan.tiles) * R, cnt = c.count(b), len = c.length(b);
+    const bool whole = c0 == 0 && c1 == n;
+    float* const sums = u + (c1 - c0) == u_end ? ring : spill;
+    auto line = [&](int r) {           // of row r in q and o
+      const int s = plan.group.by(r);
+      return (((long long)b * c.S + s) * a.Hq + kvh * plan.group.d + r - s * plan.group.d) * D;
+    };
+    for (int r0 = 0; r0 < R && row0 + r0 < rows; r0 += G) {
+      float q[G][N], o[G][N], rm[G], rl[G];
+      int end[G], last = 0;
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        const int r = row0 + r0 + g, s = plan.group.by(r);
+        end[g] = r < rows && s < cnt ? min(min(c1 * KT, keys), len - cnt + s + 1) : 0;
+        last = max(last, end[g]);
+        rm[g] = -INFINITY;
+        rl[g] = 0.f;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          q[g][i] = end[g] > 0 ? Cvt<T>::to_f(reinterpret_cast<const T*>(a.q)[line(r) + i * 32 + lane]) : 0.f;
+          o[g][i] = 0.f;
+        }
+      }
+      for (int key = c0 * KT; key < last; ++key) {
+        const int i = c.in_page.by(key), page = c.table[(size_t)b * c.per + i];
+        if ((unsigned)page >= (unsigned)c.pages) continue;
+        const long long row = ((long long)page * c.Hkv + kvh) * c.page + key - i * c.page;
+        float k[N], v[N], ks = sl2;
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+          k[j] = load(a.kpool, row * D + j * 32 + lane);
+          v[j] = load(a.vpool, row * D + j * 32 + lane);
+        }
+        if constexpr (CDT == DT_E4M3) {
+          ks *= __uint_as_float((uint32_t)a.kscale[row] << 23);
+#pragma unroll
+          for (int j = 0; j < N; ++j) v[j] *= __uint_as_float((uint32_t)a.vscale[row] << 23);
+        }
+        bool on = false;
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+          if (key >= end[g]) continue;
+          float x = 0.f;
+#pragma unroll
+          for (int j = 0; j < N; ++j) x = fmaf(q[g][j], k[j], x);
+          x = warp_sum(x) * ks;
+          const float mn = fmaxf(rm[g], x), base = mn == -INFINITY ? 0.f : mn, w = part_weight(rm[g], base), p = pow2_of(x - base);
+          rm[g] = mn;
+          rl[g] = rl[g] * w + p;
+#pragma unroll
+          for (int j = 0; j < N; ++j) o[g][j] = o[g][j] * w + p * v[j];
+          on |= rl[g] == rl[g];
+        }
+        if (!on) break;                // (NaN in all rows that see this key; the others have ended)
+      }
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        if (end[g] <= 0) continue;
+        const int r = r0 + g;
+        if (whole) {
+          T* out = reinterpret_cast<T*>(a.o) + line(row0 + r);
+#pragma unroll
+          for (int j = 0; j < N; ++j) {
+            const float x = rl[g] == 0.f ? 0.f : o[g][j] / rl[g];
+            if (!finite(x) || !finite(Cvt<T>::to_f(out[j * 32 + lane]))) out[j * 32 + lane] = Cvt<T>::from_f(x);
+          }
+        } else {
+          float &pm = m[slot * R + r], &pl = l[slot * R + r];
+          const bool all = !finite(pl);
+          const float unit = all ? 1.f : pow2_of(rm[g] - pm);
+          __syncwarp();                // (all have read them)
+#pragma unroll
+          for (int j = 0; j < N; ++j) {
+            float& x = sums[r * D + j * 32 + lane];
+            if (all || !finite(o[g][j]) || !finite(x)) x = o[g][j] * unit;
+          }
+          if (all && lane == 0) { pm = rm[g]; pl = rl[g]; }
+        }
+      }
+    }
+    slot += !whole;
+    u += c1 - c0;
+  }
+}
+
 // MULTI: several tokens a sequence, whose rows end at different keys
 template <typename T, int CDT, int D, int NQ, bool MULTI>
 __global__ void __launch_bounds__(PA_WARPS * 32, PA<T, CDT, D, NQ>::CTAS)
-paged_attend_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv, const AttendArgs a, const Paged c,
-                    const AttendPlan plan) {
+paged_attend_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv, const __grid_constant__ AttendArgs a,
+                    const __grid_constant__ Paged c, const __grid_constant__ AttendPlan plan) {
   using C = PA<T, CDT, D, NQ>;
   constexpr int R = C::R, KT = C::KT, NS = C::NS, KL = C::KL, VW = C::VW, MT = C::MT, QS = C::QS, GP = C::GP, W = PA_WARPS;
   extern __shared__ __align__(1024) uint8_t shared[];              // [W][RING], [W][ST][SB]
@@ -227,13 +341,14 @@ paged_attend_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_consta
   __shared__ float piece_m[2 * W][R], piece_l[2 * W][R];
   __shared__ int piece_item[2 * W], piece_flags[2 * W];
   __shared__ unsigned piece_start[2 * W], piece_end[2 * W];
+  __shared__ int again[W];             // a run of the warp has to be worked over once more
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");       // (the join waits for the end of this kernel)
 
   // ---- the share of this warp: every warp finds it by itself ----------------------------------------------------------------
   if (lane < 2) piece_item[2 * warp + lane] = -1;
   if (lane == 0) {
-    abort_word[warp] = 0;
+    abort_word[warp] = again[warp] = 0;
     for (int i = 0; i < C::ST * 2; ++i) mbar_init(&landed[warp][0][0] + i, 1);
     mbar_fence_init();
     tma_prefetch_desc(&tmk);
@@ -340,7 +455,7 @@ paged_attend_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_consta
     }
     constexpr float LIFT = !C::E8 && !C::BF && !C::F32 ? 7.f : 0.f;      // fp16 P without a scale of its own
     int vtop = -1000;                  // the power of two of V that the accumulators are relative to, as stored
-    int odd_from = 0x7fffffff;         // the first chunk with values left out
+    bool left_out = false;             // values of keys that not all tokens see
     const int full = MULTI ? min(keys, max(0, len - cnt + 1)) : keys;      // keys that every token sees
 
     // one round: scores of chunk ch, then K of chunk ch + ST into its place; probabilities and products of ch, then V of ch + ST.
@@ -608,7 +723,7 @@ paged_attend_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_consta
               }
             // What stands behind the end of a sequence or in a tile that is not there is none of it.  With several tokens, a key that
             // one row sees and another does not is multiplied by a probability of 0 there, which an infinity or NaN among its values
-            // would turn into NaN: those are left out here, and the rows that see them get them at the end.
+            // would turn into NaN: those are left out here, and the rows that see them get them in the end.
             if (tail) {
 #pragma unroll
               for (int i = 0; i < NS; ++i)
@@ -671,7 +786,7 @@ paged_attend_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_consta
           }
         }
         if constexpr (MULTI) {
-          if (tail && __any_sync(0xffffffffu, bad != 0) && odd_from > ch) odd_from = ch;
+          left_out |= bad != 0;
         }
       }
       __syncwarp();
@@ -751,30 +866,29 @@ paged_attend_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_consta
           else if (row0 + r < rows) store_row4<T>(a, c, plan.group, b, kvh, row0 + r, d, v, l[q][e]);
         }
       }
-    if constexpr (MULTI) {
-      if (odd_from < c1) {             // infinities and NaN among the values from there on, to the rows that see them
-        __syncwarp();
-        for (int e = lane; e < R * D; e += 32) {
-          const int r = row0 + e / D, d = e % D, s = plan.group.by(r);
-          if (r >= rows || s >= cnt) continue;
-          const int stop = min(c1 * KT, min(keys, max(0, len - cnt + s + 1)));
-          float sum = 0.f;
-          for (int key = odd_from * KT; key < stop; ++key) {
-            const int i = c.in_page.by(key), page = pages[i];
-            if ((unsigned)page >= (unsigned)c.pages) continue;
-            const long long at = (((long long)page * c.Hkv + kvh) * c.page + key - i * c.page) * D + d;
-            float v;
-            if constexpr (C::E8) v = from_e4m3x2(reinterpret_cast<const uint8_t*>(a.vpool)[at]).x;
-            else v = load_as_float(a.vpool, CDT, at);
-            if (!(fabsf(v) < INFINITY)) sum += v;
+    // What is not finite may have met a part of 0 or of the other sign where P, or a number of 32 bits, is split in two.
+    if constexpr (MULTI || !C::E8) {
+      bool odd = left_out;
+      if constexpr (!C::E8) {
+#pragma unroll
+        for (int q = 0; q < NQ; ++q)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float probe = 0.f;
+#pragma unroll
+            for (int i = 0; i < MT; ++i) probe = fmaf(o[q][i][2 + e], 0.f, fmaf(o[q][i][e], 0.f, probe));
+            odd |= probe != 0.f && (C::F32 || l[q][e] > 0.f);
           }
-          if (sum == 0.f) continue;
-          if (!whole) sums[e] = sum;
-          else reinterpret_cast<T*>(a.o)[(((long long)b * c.S + s) * a.Hq + kvh * plan.group.d + r - s * plan.group.d) * D + d] = Cvt<T>::from_f(sum);
-        }
       }
+      if (odd) again[warp] = 1;
     }
     u += c1 - c0;
+  }
+  if constexpr (MULTI || !C::E8) {
+    __syncwarp();
+    if (again[warp] != 0 && *abort_flag == 0)
+      redo_share<T, CDT, D, R, KT>(a, c, plan, start_of(cta * W + warp), u_end, reinterpret_cast<float*>(ring),
+                                   plan.spill + ((size_t)cta * W + warp) * C::PIECE, piece_m[2 * warp], piece_l[2 * warp]);
   }
   __syncthreads();
 

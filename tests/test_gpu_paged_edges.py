@@ -1,4 +1,6 @@
 """Calls on a paged cache at the edges of what their documentation allows, on the GPU."""
+import math
+
 import pytest
 import torch
 
@@ -49,6 +51,114 @@ def test_a_token_behind_the_rotation_tables_is_put_nowhere(D, cache):
         want = torch.ones_like(same)
         want[t.pages[0][1], 1] = want[t.pages[1][0], 1] = want[t.pages[1][0], 2] = want[t.pages[1][0], 3] = False
         assert torch.equal(same, want)
+
+
+# ---- infinities and NaN --------------------------------------------------------------------------
+FAST = [("bf16", "bf16"), ("fp16", "fp16"), ("fp32", "fp32")]                 # (8 bits hold no infinities)
+OTHER = [("bf16", "fp32"), ("fp32", "bf16"), ("fp16", "bf16")]                # number by number
+KINDS = [(a, b, D, w) for a, b in FAST for D in (64, 128, 48) for w in (0, 20000)] + [(a, b, 64, 0) for a, b in OTHER]
+
+
+def _put(t, pool, b, pos, head, columns, x):
+    pool[t.pages[b][pos // t.page], head, pos % t.page, columns] = x
+
+
+def _pair(lengths, D, cache, width, seed=0):
+    return [R.Setup(lengths, 2, D, cache, 16, dev, seed=seed, width=width if dev == "cuda" else 0) for dev in ("cpu", "cuda")]
+
+
+def _kinds(x):
+    """What an element is: 0 finite, 1, -1 an infinity, 2 NaN."""
+    x = x.cpu().double()
+    return torch.where(torch.isnan(x), 2.0, torch.where(torch.isinf(x), x.sign(), torch.zeros_like(x)))
+
+
+@pytest.mark.parametrize("dtype,cache,D,width", KINDS)
+@pytest.mark.parametrize("S", [1, 3, 9])
+def test_infinities_among_the_values(dtype, cache, D, width, S):
+    """A column of a row that sees an infinity is that infinity, one that sees both signs or a NaN is NaN, and all others are
+    what they were, bit by bit; on the CPU alike.  First, middle and last keys, and ones that only later tokens see."""
+    lengths = [1, 40, 700, 17]
+    pair = _pair(lengths, D, cache, width)
+    q = pair[0].normal(4, S, 8, D, dtype=dtype)
+    clean = F.paged_attention(pair[1].tensor(q), pair[1].layer, pair[1].table, pair[1].lens)._t.clone()
+    for t in pair:
+        for b, pos, head, column, x in ((0, 0, 0, 3, math.inf), (0, 0, 1, 4, -math.inf), (0, 0, 1, 5, math.nan),
+                                        (1, 0, 0, 0, math.inf), (1, 39, 0, 1, -math.inf), (1, 0, 0, 2, math.inf), (1, 39, 0, 2, -math.inf),
+                                        (1, 20, 1, 7, math.inf), (1, 38, 1, 8, math.nan), (1, 5, 1, D - 1, -math.inf),
+                                        (2, 0, 0, 6, -math.inf), (2, 699, 0, 9, math.inf), (2, 350, 0, 11, math.inf), (2, 351, 0, 11, math.inf),
+                                        (2, 352, 0, 12, math.inf), (2, 698, 0, 12, -math.inf), (2, 3, 1, 13, math.nan), (2, 4, 1, 13, math.inf)):
+            _put(t, t.layer.v, b, pos, head, column, x)
+    cpu, gpu = (F.paged_attention(t.tensor(q), t.layer, t.table, t.lens)._t.cpu() for t in pair)
+    assert torch.equal(_kinds(gpu), _kinds(cpu)) and int((_kinds(cpu) == 1).sum()) >= 8 and int((_kinds(cpu) == -1).sum()) >= 8
+    fine = _kinds(cpu) == 0
+    assert torch.equal(gpu[fine], clean.cpu()[fine])
+
+
+@pytest.mark.parametrize("dtype,cache,D,width", KINDS)
+@pytest.mark.parametrize("S", [1, 4])
+def test_infinities_among_the_keys(dtype, cache, D, width, S):
+    """Scores of -inf weigh nothing: the rows are those without the key.  Queries of 11 bits and less, and of more."""
+    lengths, drop = [40, 700, 33], [7, 350, 0]
+    pair = _pair(lengths, D, cache, width, seed=2)
+    q = pair[0].normal(3, S, 8, D, dtype=dtype)
+    q[..., 0] = torch.tensor([1.0, 0.5, 3.0, 1 / 3, 2.0 ** -10, 1.0, 1.5, 0.1]).to(q.dtype)
+    for t in pair:
+        for b, pos in enumerate(drop):
+            for head in range(2):
+                _put(t, t.layer.k, b, pos, head, 0, -math.inf)
+    kv = [[torch.cat((x[:pos], x[pos + 1:])) for x in pair[0].kv[b]] for b, pos in enumerate(drop)]
+    want, size, reach = R.attention(q, kv, [n - 1 - S for n in lengths], [S] * 3, D ** -0.5)
+    bound = R.tolerance(q, want, size, reach, 700, cache)
+    for t in pair:
+        o = F.paged_attention(t.tensor(q), t.layer, t.table, t.lens)._t.cpu()
+        assert torch.all((o.double() - want).abs() <= bound)
+    # with an infinity among its values too, such a key gives NaN there: 0 times an infinity
+    for t in pair:
+        for b, pos in enumerate(drop):
+            _put(t, t.layer.v, b, pos, 1, 2, math.inf)
+    cpu, gpu = (F.paged_attention(t.tensor(q), t.layer, t.table, t.lens)._t.cpu() for t in pair)
+    assert torch.all(torch.isnan(cpu[:, :, 4:, 2])) and torch.equal(_kinds(gpu), _kinds(cpu))
+
+
+@pytest.mark.parametrize("dtype,cache,D,width", KINDS)
+@pytest.mark.parametrize("S", [1, 4])
+def test_rows_whose_scores_are_minus_infinity_throughout(dtype, cache, D, width, S):
+    """Zeros, whether keys or the query are infinite, and whatever the values hold."""
+    lengths = [40, 700, 5]
+    pair = _pair(lengths, D, cache, width, seed=3)
+    q = pair[0].normal(3, S, 8, D, dtype=dtype)
+    q[..., 0] = 1.0
+    q[1, :, 0, 0] = -math.inf                # its keys are positive there
+    for t in pair:
+        for b, n in enumerate(lengths):
+            for pos in range(n):
+                if b != 1:
+                    _put(t, t.layer.k, b, pos, 1, 0, -math.inf)
+                else:
+                    _put(t, t.layer.k, b, pos, 0, 0, 1.0 + pos % 3)
+            _put(t, t.layer.v, b, n - 1, 1 if b != 1 else 0, 2, math.inf)
+            _put(t, t.layer.v, b, 0, 1 if b != 1 else 0, 3, -math.inf)
+    cpu, gpu = (F.paged_attention(t.tensor(q), t.layer, t.table, t.lens)._t.cpu() for t in pair)
+    for o in (cpu, gpu):
+        assert torch.all(o[[0, 2]][:, :, 4:] == 0) and torch.all(o[1, :, 0] == 0)
+    assert torch.equal(_kinds(gpu), _kinds(cpu))
+
+
+@pytest.mark.parametrize("dtype,cache", FAST)
+def test_infinities_of_keys_with_little_weight(dtype, cache):
+    """A weight that is no number of fp16 any more is still one; in another part of the sequence, too."""
+    lengths = [600]
+    pair = _pair(lengths, 64, cache, 0, seed=4)
+    q = torch.zeros(1, 1, 2, 64).to(R.TYPES[dtype])
+    q[..., 0] = 8.0
+    for t in pair:
+        for pos in range(600):
+            _put(t, t.layer.k, 0, pos, slice(None), 0, 4.0 if pos == 300 else 0.0)      # weights of e^-32 next to one of 1
+        for i, pos in enumerate((0, 299, 301, 599)):
+            _put(t, t.layer.v, 0, pos, slice(None), i, math.inf)
+    cpu, gpu = (F.paged_attention(t.tensor(q), t.layer, t.table, t.lens, scale=1.0)._t.cpu() for t in pair)
+    assert torch.all(cpu[..., :4] == math.inf) and torch.equal(_kinds(gpu), _kinds(cpu))
 
 
 # ---- models --------------------------------------------------------------------------------------
