@@ -120,8 +120,9 @@ def apply_rope(x, rotary, position_ids=None):
 
 def paged_self_attention(y, rotary, num_heads, cache, page_table, lengths, counts=None, prompt=False):
     """Self-attention of a fused projection's y [B, S, (num_heads + 2 Hkv) D] through one layer of a paged cache -> [B, S,
-    num_heads * D].  The tokens' keys and values are put into the cache; with `prompt` the sequences have no others, and the
-    flash attention over the call's own keys takes the place of reading them back."""
+    num_heads * D].  The tokens' keys and values are put into the cache; with `prompt` the sequences have no others and the real
+    tokens stand first in each row (`prompt_first`), and the flash attention over the call's own keys takes the place of reading
+    them back."""
     B, S, _ = y.shape
     rotary.reserve(max(S, page_table.shape[1] * cache.page_size))
     cos, sin = rotary.tables32()
@@ -135,9 +136,29 @@ def paged_self_attention(y, rotary, num_heads, cache, page_table, lengths, count
     return F.reshape(o, (B, S, num_heads * cache.head_dim))
 
 
+def prompt_first(idx, lengths):
+    """Prompts [B, S] whose real tokens are each row's last lengths[b] -> (idx with them first, how many they are [B], and for
+    `in_places` where each place's token went [B, S]).  Nothing waits for the device."""
+    t = lengths._t if isinstance(lengths, Tensor) else None
+    if t is None or t.shape != idx.shape[:1] or t.device != idx._t.device:
+        return idx, None, None                   # (the operators say what is wrong with them)
+    S = idx.shape[1]
+    n, step = t.clamp(0, S), torch.arange(S, device=t.device)
+    pad = (S - n).long()[:, None]
+    idx = Tensor._wrap(torch.gather(idx._t, 1, (step + pad) % max(S, 1)))
+    return idx, Tensor._wrap(n), Tensor._wrap((step - pad) % max(S, 1))
+
+
 def last_tokens(x, counts=None):
     """[B, S, H] -> [B, 1, H]: each sequence's last real token (its last, without `counts`)."""
     if counts is None or x.shape[1] == 1:
         return x[:, x.shape[1] - 1:]
     at = (counts._t.long() - 1).clamp(0, x.shape[1] - 1)
     return F.unsqueeze(x[Tensor._wrap(torch.arange(x.shape[0], device=at.device)), Tensor._wrap(at)], 1)
+
+
+def in_places(x, places=None):
+    """x [B, S, H] of the tokens that `prompt_first` gave, in the order that it took them from."""
+    if places is None:
+        return x
+    return x[Tensor._wrap(torch.arange(x.shape[0], device=places._t.device).unsqueeze(1)), places]

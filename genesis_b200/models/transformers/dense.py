@@ -14,7 +14,7 @@ import torch
 from ... import nn
 from ...nn import functional as F
 from ...tensor import Tensor
-from .components import RotaryEmbedding, apply_rope, find_multiple, last_tokens, paged_self_attention  # noqa: F401
+from .components import RotaryEmbedding, apply_rope, find_multiple, in_places, last_tokens, paged_self_attention, prompt_first  # noqa: F401
 from .config import TransformerConfig, get_transformer_config
 
 ModelArgs = TransformerConfig
@@ -138,11 +138,14 @@ class QwenModel(nn.Module):
         return self.lm_head(self.hidden_states(idx, position_ids))
 
     def forward_paged(self, idx, cache, page_table, lengths, counts=None, prompt=False, last=True):
+        places = None
+        if prompt and counts is None:
+            idx, counts, places = prompt_first(idx, lengths)
         x, branch = self.embed_tokens(idx), None
         for i, layer in enumerate(self.layers):
             x, branch = layer.forward_paged(x, branch, cache[i], page_table, lengths, counts, prompt)
         h = self.norm.add_forward(x, branch)[1]
-        return self.lm_head(last_tokens(h, counts) if last else h)
+        return self.lm_head(last_tokens(h, counts) if last else in_places(h, places))
 
     @classmethod
     def from_name(cls, name):
@@ -171,9 +174,10 @@ class QwenForCausalLM(nn.Module):
         """Logits of the tokens idx [B, S] that follow what a `nn.PagedKVCache` holds of their sequences, and are put into it.
 
         `page_table` [B, pages], `lengths` [B] (tokens with those of this call) and `counts` [B] (real ones of the S) are int32
-        Tensors as `nn.functional.paged_attention` takes them.  `prompt`: the sequences had no tokens before.  `last`: logits
-        [B, 1, V] of each sequence's last real token (of a sequence without one they mean nothing), else [B, S, V].  For inference; nothing here waits for the device, so a
-        step can be captured and replayed while the lengths grow on the device."""
+        Tensors as `nn.functional.paged_attention` takes them: with `counts` a row's real tokens are its first ones, without, where
+        it is longer than its sequence, its last.  `prompt`: the sequences had no tokens before (lengths are counts).  `last`: logits
+        [B, 1, V] of each sequence's last real token (of a sequence without one they mean nothing), else [B, S, V].  For inference;
+        nothing here waits for the device, so a step can be captured and replayed while the lengths grow on the device."""
         return self.model.forward_paged(idx, cache, page_table, lengths, counts, prompt, last)
 
     def generate(self, input_ids, max_new_tokens=100, temperature=1.0, top_k=None, top_p=None, cache_dtype=None):

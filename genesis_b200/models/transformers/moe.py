@@ -28,7 +28,7 @@ from ...ops import dispatch as K
 from .sampling import generate_paged, sample_next
 from ...tensor import Tensor
 from ...amp_state import amp_state
-from .components import RotaryEmbedding, apply_rope, last_tokens, paged_self_attention
+from .components import RotaryEmbedding, apply_rope, in_places, last_tokens, paged_self_attention, prompt_first
 from .config import MoEConfig, get_moe_config
 
 
@@ -521,10 +521,13 @@ class MoEModel(MoEPreTrainedModel):
         return self.norm.add_forward(h, branch)[1], presents
 
     def forward_paged(self, input_ids, cache, page_table, lengths, counts=None, prompt=False):
+        places = None
+        if prompt and counts is None:
+            input_ids, counts, places = prompt_first(input_ids, lengths)
         h, branch = self.embed_tokens(input_ids), None
         for i, layer in enumerate(self.layers):
             h, branch = layer.forward_paged(h, branch, cache[i], page_table, lengths, counts, prompt)
-        return self.norm.add_forward(h, branch)[1]
+        return in_places(self.norm.add_forward(h, branch)[1], places)
 
 
 class MoEForCausalLM(MoEPreTrainedModel):

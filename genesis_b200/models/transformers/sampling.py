@@ -52,7 +52,7 @@ def generate_paged(model, input_ids, max_new_tokens, temperature, top_k, top_p, 
         for i in range(max_new_tokens):
             if i > 0:
                 lengths._t += 1
-            logits = model.forward_paged(Tensor._wrap(step), cache, table, lengths, prompt=i == 0)
+            logits = model.forward_paged(Tensor._wrap(step), cache, table, lengths, lengths if i == 0 else None, prompt=i == 0)
             step = sample_next(logits._t[:, -1, :], temperature, top_k, top_p).to(out.dtype)
             out = torch.cat((out, step), dim=1)
     return Tensor._wrap(out)

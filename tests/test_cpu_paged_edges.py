@@ -133,3 +133,33 @@ def test_models_converted_to_16_bits(kind, half):
         assert m.generate(_tokens(1, 70), max_new_tokens=2, temperature=0.0, cache_dtype="float8_e4m3fn").shape == (1, 72)
     assert answers[0].dtype == getattr(torch, "float16" if half == "half" else half)
     assert torch.equal(*answers)
+
+
+# ---- prompts -------------------------------------------------------------------------------------
+@pytest.mark.parametrize("kind", ["dense", "moe"])
+@pytest.mark.parametrize("last", [True, False])
+def test_prompts_padded_in_front(kind, last):
+    """Without counts a row's real tokens are its last ones; a prompt is no exception."""
+    m = _model(kind)
+    tokens, S, have = _tokens(4, 20)._t, 9, [9, 5, 0, 1]
+    with genesis.no_grad():
+        full = [m(genesis.Tensor(tokens[b:b + 1]))._t[0] for b in range(4)]
+        cache = PagedKVCache(8, 2, 16, page_size=16, num_layers=2, dtype="float32")
+        table = cache.page_table(cache.allocate([20] * 4))
+        idx = torch.full((4, S), 96)
+        for b, n in enumerate(have):
+            idx[b, S - n:] = tokens[b, :n]
+        out = m.forward_paged(genesis.Tensor(idx), cache, table, _ints(*have), prompt=True, last=last)._t
+        assert out.shape == (4, 1 if last else S, 97)
+        for b, n in enumerate(have):
+            assert torch.allclose(out[b, -min(n, out.shape[1]):][:n], full[b][n - min(n, out.shape[1]):n], atol=1e-4)
+        for _ in range(3):                                 # what has been put into the cache goes on
+            nxt = torch.stack([tokens[b, n:n + 1] for b, n in enumerate(have)])
+            have = [n + 1 for n in have]
+            out = m.forward_paged(genesis.Tensor(nxt), cache, table, _ints(*have))._t
+            for b, n in enumerate(have):
+                assert torch.allclose(out[b, 0], full[b][n - 1], atol=1e-4)
+        with pytest.raises(TypeError, match="lengths must be an int32 Tensor"):
+            m.forward_paged(genesis.Tensor(idx), cache, table, [9, 5, 0, 1], prompt=True)
+        with pytest.raises(ValueError, match="lengths must be"):
+            m.forward_paged(genesis.Tensor(idx), cache, table, _ints(9, 5), prompt=True)

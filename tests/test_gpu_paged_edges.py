@@ -254,3 +254,29 @@ def test_models_converted_to_16_bits(kind, half, cache_dtype):
         assert m.generate(prompt, max_new_tokens=4, temperature=0.0, cache_dtype=cache_dtype).shape == (2, 13)
         del graph
     assert torch.equal(*answers)
+
+
+@pytest.mark.parametrize("kind", ["dense", "moe"])
+def test_prompts_padded_in_front_and_behind(kind):
+    """The same bits, whichever side the padding is on."""
+    m = _model(kind)
+    toks, have, S = _tokens(3, 40), (40, 7, 23), 40
+    rows = torch.zeros(2, 3, S, dtype=torch.int64, device="cuda")
+    for b, n in enumerate(have):
+        rows[0, b, :n] = rows[1, b, S - n:] = toks[b, :n]
+    rows[1, 1, :S - 7] = 5
+    for last in (True, False):
+        outs = []
+        for idx, counts in ((rows[0], _ints(*have)), (rows[1], None)):
+            cache = PagedKVCache(12, 2, 64, page_size=16, num_layers=2, dtype="bfloat16", device="cuda")
+            table = cache.page_table(cache.allocate([41, 41, 41]))
+            with genesis.no_grad(), genesis.amp.autocast(dtype=genesis.bfloat16):
+                out = m.forward_paged(genesis.Tensor(idx), cache, table, _ints(*have), counts, prompt=True, last=last)._t
+                nxt = m.forward_paged(genesis.Tensor(toks[:, :1]), cache, table, _ints(*(n + 1 for n in have)))._t
+            outs.append((out, nxt))
+        (a, x), (b, y) = outs
+        assert torch.equal(x, y)
+        if last:
+            assert torch.equal(a, b)
+        else:
+            assert all(torch.equal(a[i, :n], b[i, S - n:]) for i, n in enumerate(have))
