@@ -190,18 +190,19 @@ class QwenForCausalLM(nn.Module):
         from .sampling import generate_paged, sample_next
         was_training = self.training
         self.eval()
-        if cache_dtype is not None:
-            out = generate_paged(self, input_ids, max_new_tokens, temperature, top_k, top_p, cache_dtype)
-        else:
+        try:
+            if cache_dtype is not None:
+                return generate_paged(self, input_ids, max_new_tokens, temperature, top_k, top_p, cache_dtype)
             out = input_ids
             with grad_mode.no_grad():
                 for _ in range(max_new_tokens):
                     logits = self(out)
                     tok = sample_next(logits._t[:, -1, :], temperature, top_k, top_p)
                     out = Tensor._wrap(torch.cat((out._t, tok.to(out._t.dtype)), dim=1))
-        if was_training:
-            self.train()
-        return out
+            return out
+        finally:
+            if was_training:
+                self.train()
 
     def load_state_dict(self, state_dict, strict=True):
         sd = dict(state_dict)

@@ -571,16 +571,22 @@ class MoEForCausalLM(MoEPreTrainedModel):
         """Appends `max_new_tokens` sampled tokens to `input_ids` [B, S]; with `cache_dtype` keys and values are kept in a paged
         cache of that type (`QwenForCausalLM.generate`)."""
         from ... import grad_mode
+        was_training = self.training
         self.eval()
-        if cache_dtype is not None:
-            return generate_paged(self, input_ids, max_new_tokens, temperature, top_k, top_p, cache_dtype)
-        generated = input_ids
-        with grad_mode.no_grad():
-            for _ in range(max_new_tokens):
-                logits = self(generated)
-                tok = sample_next(logits._t[:, -1, :], temperature, top_k, top_p)
-                generated = Tensor._wrap(torch.cat((generated._t, tok.to(generated._t.dtype)), dim=1))
-        return generated
+        try:
+            if cache_dtype is not None:
+                return generate_paged(self, input_ids, max_new_tokens, temperature, top_k, top_p, cache_dtype)
+            generated = input_ids
+            with grad_mode.no_grad():
+                for _ in range(max_new_tokens):
+                    logits = self(generated)
+                    tok = sample_next(logits._t[:, -1, :], temperature, top_k, top_p)
+                    generated = Tensor._wrap(torch.cat((generated._t, tok.to(generated._t.dtype)), dim=1))
+            return generated
+        except BaseException:
+            if was_training:           # (a call that answers leaves the model in eval mode)
+                self.train()
+            raise
 
 
 class MoETransformerBlock(MoEDecoderLayer):

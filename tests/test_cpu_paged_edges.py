@@ -163,3 +163,18 @@ def test_prompts_padded_in_front(kind, last):
             m.forward_paged(genesis.Tensor(idx), cache, table, [9, 5, 0, 1], prompt=True)
         with pytest.raises(ValueError, match="lengths must be"):
             m.forward_paged(genesis.Tensor(idx), cache, table, _ints(9, 5), prompt=True)
+
+
+@pytest.mark.parametrize("kind", ["dense", "moe"])
+def test_a_refused_generation_leaves_the_mode_as_it_was(kind):
+    m = _model(kind).train()
+    with pytest.raises(ValueError, match="a cache holds one of"):
+        m.generate(_tokens(1, 3), max_new_tokens=1, cache_dtype="int8")
+    assert m.training and all(x.training for x in m.modules())
+    with pytest.raises(Exception):
+        m.generate(_tokens(3), max_new_tokens=1, cache_dtype="float32")          # no [B, S]
+    assert m.training
+    m.eval()
+    with pytest.raises(ValueError):
+        m.generate(_tokens(1, 3), max_new_tokens=1, cache_dtype="int8")
+    assert not m.training
