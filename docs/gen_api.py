@@ -45,7 +45,7 @@ def main():
             out.append(doc)
         out.append("")
         rows = []
-        for n in sorted(dir(m)):
+        for n in sorted(getattr(m, "__all__", dir(m))):
             if n.startswith("_"):
                 continue
             o = getattr(m, n)

@@ -16,12 +16,12 @@ import torch
 
 from ..function import Function, AMPPolicy, cast
 from ..tensor import Tensor
-from ..ops import dispatch as K, paged as P
+from ..ops import dispatch as K, paged as _P
 from ..dtypes import to_torch_dtype as _to_torch_dtype
 from ..amp_state import amp_state, shadow_of, stacked_shadow_of
 from .. import random as _random
-from .. import grad_mode
-from .paged import PagedKVLayer
+from .. import grad_mode as _grad_mode
+from .paged import PagedKVLayer as _PagedKVLayer
 
 _pysum, _pymax, _pymin, _pyabs, _pypow = builtins.sum, builtins.max, builtins.min, builtins.abs, builtins.pow
 
@@ -1968,7 +1968,7 @@ def flash_attention(q, k, v, causal=True, scale=None):
 def _paged_args(name, cache, page_table, lengths, counts, B, device):
     """Checks what the operators on a paged cache have in common; returns the raw (page table, lengths, counts).  `device`:
     index of the tokens' device (-1: the CPU)."""
-    if not isinstance(cache, PagedKVLayer):
+    if not isinstance(cache, _PagedKVLayer):
         raise TypeError(f"{name}: cache must be a layer of a PagedKVCache (cache[i]), got {type(cache).__name__}")
     at = cache._call[0]
     raw = []
@@ -2003,7 +2003,7 @@ def _paged_tokens(name, what, x, dims, dtype=None):
         raise ValueError(f"{name}: {what} must have {dims} dimensions, got {tuple(t.shape)}")
     if dtype is not None and t.dtype is not dtype:
         raise TypeError(f"{name}: {what} is {t.dtype}, expected {dtype}")
-    if x.requires_grad and grad_mode.is_grad_enabled():
+    if x.requires_grad and _grad_mode.is_grad_enabled():
         raise RuntimeError(f"{name}: no gradient flows through a cache; call it under no_grad or pass a detached {what}")
     return t
 
@@ -2025,7 +2025,7 @@ def paged_kv_write(k, v, cache, page_table, lengths, counts=None):
     if k.shape != v.shape or v.get_device() != k.get_device() or tuple(k.shape[2:]) != (cache.num_kv_heads, cache.head_dim):
         raise ValueError(f"{name}: k and v must be [B, S, {cache.num_kv_heads}, {cache.head_dim}] on one device, got "
                          f"{tuple(k.shape)} and {tuple(v.shape)}")
-    P.write(k, v, cache, table, lengths, counts)
+    _P.write(k, v, cache, table, lengths, counts)
 
 
 def paged_qkv_rope(y, cos, sin, cache, page_table, lengths, num_heads, counts=None):
@@ -2051,7 +2051,7 @@ def paged_qkv_rope(y, cos, sin, cache, page_table, lengths, num_heads, counts=No
         if t.dim() != 2 or t.shape[1] != D or t.get_device() != at or (tables and t.shape != tables[0].shape):
             raise ValueError(f"{name}: {what} must be [positions, {D}] on {y.device}, cos and sin alike, got {tuple(t.shape)} on {t.device}")
         tables.append(t if t.is_contiguous() else K.contiguous(t))
-    return Tensor._wrap(P.rope_write(y, tables, num_heads, cache, table, lengths, counts))
+    return Tensor._wrap(_P.rope_write(y, tables, num_heads, cache, table, lengths, counts))
 
 
 def paged_kv_read(cache, page_table, lengths, max_length, dtype=None):
@@ -2059,14 +2059,14 @@ def paged_kv_read(cache, page_table, lengths, max_length, dtype=None):
     takes for the next piece of a long prompt.  `dtype`: float32, float16 or bfloat16; the cache's, or bfloat16 for 8 bits (exact).
     Tokens whose page or position does not exist come out as zeros, and the error is raised as `paged_kv_write` says."""
     name = "paged_kv_read"
-    table, lengths, _ = _paged_args(name, cache, page_table, lengths, None, None, cache._call[0] if isinstance(cache, PagedKVLayer) else -1)
+    table, lengths, _ = _paged_args(name, cache, page_table, lengths, None, None, cache._call[0] if isinstance(cache, _PagedKVLayer) else -1)
     if isinstance(max_length, bool) or not isinstance(max_length, int) or not 0 <= max_length < 2 ** 31:
         raise ValueError(f"{name}: max_length must be a non-negative 32-bit int, got {max_length!r}")
     held = cache.k.dtype
-    dtype = (torch.bfloat16 if held == P.E4M3 else held) if dtype is None else _to_torch_dtype(dtype)
+    dtype = (torch.bfloat16 if held == _P.E4M3 else held) if dtype is None else _to_torch_dtype(dtype)
     if dtype not in (torch.float32, torch.float16, torch.bfloat16):
         raise TypeError(f"{name}: dtype must be float32, float16 or bfloat16, got {dtype}")
-    return tuple(Tensor._wrap(t) for t in P.read(cache, table, lengths, max_length, dtype))
+    return tuple(Tensor._wrap(t) for t in _P.read(cache, table, lengths, max_length, dtype))
 
 
 def paged_attention(q, cache, page_table, lengths, counts=None, scale=None):
@@ -2087,7 +2087,7 @@ def paged_attention(q, cache, page_table, lengths, counts=None, scale=None):
     if q.is_cuda and (D > 256 or q.shape[0] * q.shape[1] * Hq >= 2 ** 31):
         raise ValueError(f"{name}: heads of up to 256 and less than 2^31 rows on CUDA, got {tuple(q.shape)}")
     scale = D ** -0.5 if scale is None else _number(name, "scale", scale, -1e30, 1e30)
-    return Tensor._wrap(P.attention(q, cache, table, lengths, counts, scale))
+    return Tensor._wrap(_P.attention(q, cache, table, lengths, counts, scale))
 
 
 def scaled_dot_product_attention(q, k, v, attn_mask=None, dropout_p=0.0, is_causal=False, scale=None):

@@ -14,6 +14,8 @@ from ..dtypes import DType
 from ..ops.paged import CACHE_TYPES, E4M3, pools_of
 from ..tensor import Tensor
 
+__all__ = ["PagedKVCache", "PagedKVLayer"]
+
 
 def _cache_dtype(dtype):
     names = {str(t).replace("torch.", ""): t for t in CACHE_TYPES}

@@ -178,3 +178,12 @@ def test_a_refused_generation_leaves_the_mode_as_it_was(kind):
     with pytest.raises(ValueError):
         m.generate(_tokens(1, 3), max_new_tokens=1, cache_dtype="int8")
     assert not m.training
+
+
+def test_names_of_the_package():
+    """The operators are functions of nn.functional and of the package; what their module imports is neither's."""
+    for name in ("paged_attention", "paged_kv_read", "paged_kv_write", "paged_qkv_rope"):
+        assert getattr(genesis, name) is getattr(F, name)
+    assert not any(hasattr(genesis, name) or hasattr(F, name) for name in ("PagedKVLayer", "PagedKVCache", "pools_of"))
+    assert not hasattr(F, "grad_mode") and not hasattr(F, "P")
+    assert sorted(genesis.nn.paged.__all__) == ["PagedKVCache", "PagedKVLayer"]
