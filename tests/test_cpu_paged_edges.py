@@ -187,3 +187,28 @@ def test_names_of_the_package():
     assert not any(hasattr(genesis, name) or hasattr(F, name) for name in ("PagedKVLayer", "PagedKVCache", "pools_of"))
     assert not hasattr(F, "grad_mode") and not hasattr(F, "P")
     assert sorted(genesis.nn.paged.__all__) == ["PagedKVCache", "PagedKVLayer"]
+
+
+@pytest.mark.parametrize("kind", ["dense", "moe"])
+def test_slots_that_rest(kind):
+    """Lengths advance by the slots that are active, which are the step's counts: a slot out of use stays so."""
+    m = _model(kind)
+    tokens = _tokens(3, 20)._t
+    cache = PagedKVCache(4, 2, 16, page_size=16, num_layers=2, dtype="float32")
+    table = cache.page_table(cache.allocate([20, 0, 20]))
+    lengths, active = _ints(5, 0, 7), _ints(1, 0, 1)
+    with genesis.no_grad():
+        full = [m(genesis.Tensor(tokens[b:b + 1]))._t[0] for b in range(3)]
+        m.forward_paged(genesis.Tensor(tokens[:, :7]), cache, table, lengths, lengths, prompt=True)
+        have = [5, 0, 7]
+        for step in range(6):
+            if step == 3:
+                active._t[2] = 0                            # this one rests with what it has
+            nxt = torch.stack([tokens[b, n:n + 1] for b, n in enumerate(have)])
+            have = [n + int(a) for n, a in zip(have, active._t)]
+            lengths._t += active._t
+            out = m.forward_paged(genesis.Tensor(nxt), cache, table, lengths, active)._t
+            for b in range(3):
+                if int(active._t[b]):
+                    assert torch.allclose(out[b, 0], full[b][have[b] - 1], atol=1e-4)
+    assert lengths._t.tolist() == [11, 0, 10]

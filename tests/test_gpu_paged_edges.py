@@ -280,3 +280,46 @@ def test_prompts_padded_in_front_and_behind(kind):
             assert torch.equal(a, b)
         else:
             assert all(torch.equal(a[i, :n], b[i, S - n:]) for i, n in enumerate(have))
+
+
+def test_slots_that_rest_in_a_captured_step():
+    """A slot out of use and one that comes to rest, through replays: no error is recorded, the lengths and pages of both stay, and
+    the others go on as without them."""
+    m = _model("dense")
+    toks = _tokens(6, 3, 1, seed=8)
+    with genesis.no_grad(), genesis.amp.autocast(dtype=genesis.bfloat16):
+        cache = PagedKVCache(12, 2, 64, page_size=16, num_layers=2, dtype="bfloat16", device="cuda")
+        table, lengths, active = cache.page_table(cache.allocate([60, 0, 60])), _ints(5, 0, 40), _ints(1, 0, 1)
+        m.forward_paged(genesis.Tensor(_tokens(3, 40, seed=5)), cache, table, lengths, lengths, prompt=True)
+        state = [x.clone() for layer in cache.layers for x in (layer.k, layer.v)]
+        idx = genesis.Tensor(toks[0].clone())
+
+        def step():
+            lengths._t += active._t
+            return m.forward_paged(idx, cache, table, lengths, active)
+
+        graph, out = _captured(step, lengths, lengths._t.clone())
+        N.check_status()
+        for i in range(6):
+            active._t[2] = int(i < 3)
+            idx._t.copy_(toks[i])
+            graph.replay()
+            if i == 2:
+                kept = [x.clone() for layer in cache.layers for x in (layer.k, layer.v)]
+        N.check_status()
+        assert lengths._t.tolist() == [11, 0, 43]
+        mine = [p for p in range(12) if p in table._t[2].tolist()]
+        assert all(torch.equal(a[mine], b[mine]) for a, b in zip(kept, [x for layer in cache.layers for x in (layer.k, layer.v)]))
+        got = out._t[0].clone()
+        # the first sequence alone
+        for x, y in zip([x for layer in cache.layers for x in (layer.k, layer.v)], state):
+            x.copy_(y)
+        one, alone = _ints(5), None
+        for i in range(6):
+            one._t += 1
+            alone = m.forward_paged(genesis.Tensor(toks[i, :1]), cache, genesis.Tensor(table._t[:1].contiguous()), one)._t
+        q = genesis.Tensor(torch.randn(3, 1, 4, 64, device="cuda").bfloat16())
+        assert torch.all(F.paged_attention(q, cache[0], table, lengths, active)._t[1:] == 0)
+        # (products over other numbers of rows may be split otherwise: a dozen roundings to bf16 in each of two layers, 2^-9 on average)
+        assert float((got.float() - alone[0].float()).norm() / alone[0].float().norm()) < 2 * 12 * 2.0 ** -9
+    N.check_status()
