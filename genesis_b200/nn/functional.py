@@ -2055,9 +2055,12 @@ def paged_qkv_rope(y, cos, sin, cache, page_table, lengths, num_heads, counts=No
 
 
 def paged_kv_read(cache, page_table, lengths, max_length, dtype=None):
-    """(k, v) [B, max_length, Hkv, D] of the sequences' first `max_length` tokens, zeros behind each one's end: what the flash attention
-    takes for the next piece of a long prompt.  `dtype`: float32, float16 or bfloat16; the cache's, or bfloat16 for 8 bits (exact).
-    Tokens whose page or position does not exist come out as zeros, and the error is raised as `paged_kv_write` says."""
+    """(k, v) [B, max_length, Hkv, D] of the sequences' first `max_length` tokens, zeros behind each one's end.
+
+    `dtype`: float32, float16 or bfloat16; the cache's, or bfloat16 for 8 bits (exact).  Tokens whose page or position does not
+    exist come out as zeros, and the error is raised as `paged_kv_write` says.  Where all sequences are `max_length` long, the
+    flash attention takes the result for the next piece of their prompts (its last query sees its last key); of sequences of
+    different lengths it would take the zeros for keys, so those go through `paged_attention`, or one by one."""
     name = "paged_kv_read"
     table, lengths, _ = _paged_args(name, cache, page_table, lengths, None, None, cache._call[0] if isinstance(cache, _PagedKVLayer) else -1)
     if isinstance(max_length, bool) or not isinstance(max_length, int) or not 0 <= max_length < 2 ** 31:
@@ -2076,8 +2079,8 @@ def paged_attention(q, cache, page_table, lengths, counts=None, scale=None):
     counts[b] of the S are real.  Token s sees the positions up to its own, lengths[b] - counts[b] + s; a token that is none,
     or whose scores are -inf throughout, gives zeros.  Hkv divides Hq; `scale` is D ** -0.5 unless given.  Probabilities are
     formed and summed in 32 bits.  Keys whose page or position does not exist take no part, and the error is raised as
-    `paged_kv_write` says.  Made for few tokens; where S runs into the hundreds the flash attention over what `paged_kv_read`
-    brings back is faster."""
+    `paged_kv_write` says.  Made for few tokens; where S runs into the hundreds and the sequences are equally long, the
+    flash attention over what `paged_kv_read` brings back is faster."""
     name = "paged_attention"
     q = _paged_tokens(name, "q", q, 4)
     table, lengths, counts = _paged_args(name, cache, page_table, lengths, counts, q.shape[0], q.get_device())

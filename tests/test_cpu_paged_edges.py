@@ -212,3 +212,19 @@ def test_slots_that_rest(kind):
                 if int(active._t[b]):
                     assert torch.allclose(out[b, 0], full[b][have[b] - 1], atol=1e-4)
     assert lengths._t.tolist() == [11, 0, 10]
+
+
+def test_pieces_read_back_for_flash_attention():
+    """Of sequences that are equally long, and of each one alone where they are not."""
+    B, Hq, H, D, S = 3, 4, 2, 16, 5
+    for lengths in ([30, 30, 30], [30, 17, 9]):
+        t = R.Setup(lengths, H, D, "fp32")
+        q = t.tensor(t.normal(B, S, Hq, D, dtype="fp32"))
+        want = F.paged_attention(q, t.layer, t.table, t.lens)._t
+        if len(set(lengths)) == 1:
+            k, v = F.paged_kv_read(t.layer, t.table, t.lens, lengths[0])
+            assert torch.allclose(F.flash_attention(q, k, v, causal=True)._t, want, atol=1e-5)
+        for b, n in enumerate(lengths):
+            one = t.tensor(t.table._t[b:b + 1]), t.ints([n])
+            k, v = F.paged_kv_read(t.layer, *one, n)
+            assert torch.allclose(F.flash_attention(q[b:b + 1], k, v, causal=True)._t, want[b:b + 1], atol=1e-5)
