@@ -68,10 +68,12 @@ class RotaryEmbedding(nn.Module):
         old = self.__dict__.get("cos_cached")
         if old is not None:
             dev = old.device
+        values = self._values(seq_len, dev)      # (nothing changes where this fails, as it does while a stream is captured)
+        if old is not None:
             self._outgrown.append((old, self.sin_cached))
         self.max_seq_len_cached = seq_len
-        for name, values in zip(("inv_freq", "cos_cached", "sin_cached"), self._values(seq_len, dev)):
-            self.register_buffer(name, values, persistent=False)
+        for name, t in zip(("inv_freq", "cos_cached", "sin_cached"), values):
+            self.register_buffer(name, t, persistent=False)
 
     def reserve(self, seq_len):
         """Makes the tables reach so many positions.  They at least double, so that all outgrown ones together are no larger."""

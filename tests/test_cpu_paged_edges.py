@@ -9,7 +9,7 @@ import torch
 import genesis_b200 as genesis
 import genesis_b200.nn.functional as F
 from genesis_b200.models.transformers import MoEConfig, MoEForCausalLM, QwenForCausalLM, TransformerConfig
-from genesis_b200.models.transformers.components import apply_rope
+from genesis_b200.models.transformers.components import RotaryEmbedding, apply_rope
 from genesis_b200.nn import PagedKVCache
 
 import _paged_ref as R
@@ -228,3 +228,15 @@ def test_pieces_read_back_for_flash_attention():
             one = t.tensor(t.table._t[b:b + 1]), t.ints([n])
             k, v = F.paged_kv_read(t.layer, *one, n)
             assert torch.allclose(F.flash_attention(q[b:b + 1], k, v, causal=True)._t, want[b:b + 1], atol=1e-5)
+
+
+def test_tables_that_cannot_grow_stay_as_they_are(monkeypatch):
+    """As while a stream is captured: the next call tries again, and none reads behind the tables' end."""
+    rot = RotaryEmbedding(16, 32)
+    cos, sin = rot.cos_cached, rot.sin_cached
+    with monkeypatch.context() as patch:
+        patch.setattr(RotaryEmbedding, "_values", lambda *a: (_ for _ in ()).throw(RuntimeError("capturing")))
+        with pytest.raises(RuntimeError, match="capturing"):
+            rot.reserve(33)
+    assert rot.max_seq_len_cached == 32 and rot.cos_cached is cos and rot.sin_cached is sin and len(rot._outgrown) == 0
+    assert F.rope(genesis.Tensor(torch.ones(1, 33, 2, 16)), *rot(seq_len=33)).shape == (1, 33, 2, 16)
