@@ -43,9 +43,10 @@ struct Paged {
     const int c = counts != nullptr ? counts[b] : S;
     return c < 0 ? 0 : c > S ? S : c;
   }
+  // (the last positions of 2^31 are left out, so that keys can be counted in whole chunks, and one chunk ahead, in 31 bits)
   __device__ __forceinline__ int capacity() const {
     const long long c = (long long)per * page;
-    return c > 0x7fffffff ? 0x7fffffff : (int)c;
+    return c > 0x7fffff00 ? 0x7fffff00 : (int)c;
   }
   // row of the pool [pages * Hkv * page] that token `pos` of sequence b has at KV head h; -1 (recorded) where there is none
   __device__ __forceinline__ long long row(int b, int pos, int h) const {

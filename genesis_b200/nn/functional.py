@@ -2015,10 +2015,11 @@ def paged_kv_write(k, v, cache, page_table, lengths, counts=None):
     `page_table` [B, pages] names each sequence's pages in order, `lengths` [B] counts its tokens with those of this call, and
     `counts` [B] (all S without it; clipped to 0 .. S) how many of the S are real: token s < counts[b] goes to position
     lengths[b] - counts[b] + s, and nothing is written for the others or for a negative position (so a slot of the batch that
-    is not in use has length 0).  All three are int32 Tensors on the cache's device.  In 8 bits every token and head gets the smallest power of
-    two with which its largest magnitude is at most 448; infinities and NaN are held as NaN.  A page outside the cache or a
-    position behind the table is skipped and raised as IndexError at the next read of the status word (on the CPU at once).
-    Tokens of one call that share a slot are written in no order."""
+    is not in use has length 0).  All three are int32 Tensors on the cache's device.  In 8 bits every token and head gets the
+    smallest power of two with which its largest magnitude is at most 448; infinities and NaN are held as NaN.  A page outside
+    the cache or a position behind the table (on CUDA, the last 256 of 2^31 too) is skipped and raised as IndexError at the next
+    read of the status word (on the CPU at once).  Tokens of one call that share a slot are written in no order: it may be left
+    with part of one and part of another."""
     name = "paged_kv_write"
     k, v = _paged_tokens(name, "k", k, 4), _paged_tokens(name, "v", v, 4, k._t.dtype if isinstance(k, Tensor) else None)
     table, lengths, counts = _paged_args(name, cache, page_table, lengths, counts, k.shape[0], k.get_device())

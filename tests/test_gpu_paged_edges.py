@@ -15,6 +15,10 @@ import _paged_ref as R
 pytestmark = pytest.mark.gpu
 
 
+def _ints(*xs):
+    return genesis.Tensor(torch.tensor(xs, dtype=torch.int32, device="cuda"))
+
+
 def _bits(t):
     return [x.clone().view(torch.uint8) for x in (t.layer.k, t.layer.v)]
 
@@ -51,6 +55,40 @@ def test_a_token_behind_the_rotation_tables_is_put_nowhere(D, cache):
         want = torch.ones_like(same)
         want[t.pages[0][1], 1] = want[t.pages[1][0], 1] = want[t.pages[1][0], 2] = want[t.pages[1][0], 3] = False
         assert torch.equal(same, want)
+
+
+def test_positions_next_to_31_bits():
+    """One page of 2^20 tokens that a table names 2048 times.  Keys are counted in 31 bits, so the last 256 positions are behind
+    the table; up to them, keys seen over and over weigh what they weigh once."""
+    D, page = 64, 2 ** 20
+    layer = genesis.nn.PagedKVCache(1, 1, D, page_size=page, dtype="float16", device="cuda")[0]
+    g = torch.Generator("cuda").manual_seed(6)
+    layer.k.copy_(torch.randn(1, 1, page, D, device="cuda", generator=g))
+    layer.v.fill_(1)
+    layer.v[:, :, ::3, 1::2] = 0
+    table = genesis.Tensor(torch.zeros(1, 2048, dtype=torch.int32, device="cuda"))
+    q = genesis.Tensor(torch.randn(1, 1, 1, D, device="cuda", generator=g).half())
+    once = F.paged_attention(q, layer, genesis.Tensor(table._t[:, :1].contiguous()), _ints(page))._t.float()
+    N.check_status()
+    assert torch.all((once[..., ::2] - 1).abs() <= 2.0 ** -10) and torch.all((once[..., 1::2] - 2 / 3).abs() <= 0.05)
+    for n in (2 ** 31 - 256, 2 ** 31 - 255, 2 ** 31 - 1):
+        o = F.paged_attention(q, layer, table, _ints(n))._t.float()
+        if n > 2 ** 31 - 256:
+            with pytest.raises(IndexError, match="site=9"):
+                N.check_status()
+        N.check_status()
+        # a warp adds up 2^26 / 2368 chunks, each addition off by 2^-24 of the sum at most, in the sums and in the normaliser: 2^-8.2;
+        # two results are rounded to 11 bits
+        assert torch.all((o - once).abs() <= 2.0 ** -8.2 + 2.0 ** -10)
+    x = genesis.Tensor(torch.full((1, 1, 1, D), 3.0, device="cuda").half())
+    before = layer.k.clone()
+    F.paged_kv_write(x, x, layer, table, _ints(2 ** 31 - 1))
+    with pytest.raises(IndexError, match="site=9"):
+        N.check_status()
+    assert torch.equal(layer.k, before)
+    F.paged_kv_write(x, x, layer, table, _ints(2 ** 31 - 256))             # position 2^31 - 257 = 257 before the page's end
+    N.check_status()
+    assert torch.all(layer.k[0, 0, page - 257] == 3) and torch.equal(layer.k[0, 0, :page - 257], before[0, 0, :page - 257])
 
 
 # ---- infinities and NaN --------------------------------------------------------------------------
@@ -169,10 +207,6 @@ def _model(kind, positions=256, head_dim=64):
     if kind == "dense":
         return QwenForCausalLM(TransformerConfig(**base)).eval().cuda()
     return MoEForCausalLM(MoEConfig(**base, num_experts_per_tok=2, num_local_experts=4, moe_intermediate_size=256)).eval().cuda()
-
-
-def _ints(*xs):
-    return genesis.Tensor(torch.tensor(xs, dtype=torch.int32, device="cuda"))
 
 
 def _tokens(*shape, seed=3):
