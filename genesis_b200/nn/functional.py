@@ -2064,8 +2064,8 @@ def paged_kv_read(cache, page_table, lengths, max_length, dtype=None):
     different lengths it would take the zeros for keys, so those go through `paged_attention`, or one by one."""
     name = "paged_kv_read"
     table, lengths, _ = _paged_args(name, cache, page_table, lengths, None, None, cache._call[0] if isinstance(cache, _PagedKVLayer) else -1)
-    if isinstance(max_length, bool) or not isinstance(max_length, int) or not 0 <= max_length < 2 ** 31:
-        raise ValueError(f"{name}: max_length must be a non-negative 32-bit int, got {max_length!r}")
+    if isinstance(max_length, bool) or not isinstance(max_length, int) or not 0 <= max_length <= 2 ** 31 - 16:
+        raise ValueError(f"{name}: max_length must be a non-negative int of at most 2^31 - 16, got {max_length!r}")
     held = cache.k.dtype
     dtype = (torch.bfloat16 if held == _P.E4M3 else held) if dtype is None else _to_torch_dtype(dtype)
     if dtype not in (torch.float32, torch.float16, torch.bfloat16):

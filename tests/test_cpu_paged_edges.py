@@ -240,3 +240,10 @@ def test_tables_that_cannot_grow_stay_as_they_are(monkeypatch):
             rot.reserve(33)
     assert rot.max_seq_len_cached == 32 and rot.cos_cached is cos and rot.sin_cached is sin and len(rot._outgrown) == 0
     assert F.rope(genesis.Tensor(torch.ones(1, 33, 2, 16)), *rot(seq_len=33)).shape == (1, 33, 2, 16)
+
+
+def test_lengths_that_blocks_of_16_cannot_count():
+    t = R.Setup([3], 1, 8, "fp32")
+    for n in (2 ** 31 - 15, 2 ** 31 - 1, 2 ** 40):
+        with pytest.raises(ValueError, match="max_length"):
+            F.paged_kv_read(t.layer, t.table, t.lens, n)
