@@ -818,7 +818,7 @@ paged_attend_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_consta
     }
 
     // ---- the run's result ---------------------------------------------------------------------------------------------
-    const float unit = C::E8 ? (vtop < 8 ? 0.f : exp2i(vtop - 134)) : 1.f;
+    const float unit = !C::E8 ? 1.f : vtop >= 8 ? exp2i(vtop - 134) : vtop > 0 ? __uint_as_float(1u << (vtop + 15)) : 0.f;
     if constexpr (MULTI) {             // rows that are no tokens (chunks that all tokens see are not masked)
 #pragma unroll
       for (int q = 0; q < NQ; ++q)

@@ -199,6 +199,27 @@ def test_infinities_of_keys_with_little_weight(dtype, cache):
     assert torch.all(cpu[..., :4] == math.inf) and torch.equal(_kinds(gpu), _kinds(cpu))
 
 
+# ---- 8 bits --------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype,S", [("bf16", 1), ("bf16", 3), ("fp32", 1)])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("power", [-126, -121, -119, -110, 100])
+def test_values_of_the_smallest_and_large_powers_of_two(dtype, S, D, power):
+    """Rows whose power of two is next to the smallest, whose unit is no normal number of 32 bits any more."""
+    t = R.Setup([40, 700], 2, D, "e4m3", 16, "cuda", seed=7)
+    q = t.normal(2, S, 8, D, dtype=dtype)
+    small = R.Setup([40, 700], 2, D, "e4m3", 16, "cuda", seed=7)
+    for x in (t, small):
+        x.layer.v_scale.fill_(127)
+    small.layer.v_scale.fill_(127 + power)
+    one, tiny = (F.paged_attention(x.tensor(q), x.layer, x.table, x.lens)._t.cpu().double() for x in (t, small))
+    want = one * 2.0 ** power
+    # the same numbers under another power of two: equal but for what falls below the smallest subnormal number of the output, or
+    # of 32 bits before the last division (2^-149, once a warp and once a join: a handful), and a rounding that this tips over
+    # (number by number, a weight is multiplied by the power first: 2^-150 off below 2^-126, times a value of up to 448, for each key)
+    step = 2.0 ** -133 if dtype == "bf16" else 2.0 ** -149 + 700 * 448 * 2.0 ** -150
+    assert torch.all((tiny - want).abs() <= step + 16 * 2.0 ** -149 + want.abs() * R.HALF[R.TYPES[dtype]] * 2) and torch.any(tiny != 0)
+
+
 # ---- models --------------------------------------------------------------------------------------
 def _model(kind, positions=256, head_dim=64):
     genesis.manual_seed(11)
