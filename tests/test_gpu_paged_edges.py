@@ -199,6 +199,37 @@ def test_infinities_of_keys_with_little_weight(dtype, cache):
     assert torch.all(cpu[..., :4] == math.inf) and torch.equal(_kinds(gpu), _kinds(cpu))
 
 
+# ---- digits of 32-bit attention over long sequences ----------------------------------------------
+@pytest.mark.parametrize("Hq,H,D", [(14, 2, 64), (32, 4, 128), (12, 12, 64), (6, 2, 80)])
+@pytest.mark.parametrize("S,width", [(1, 0), (3, 0), (3, 20000)])
+def test_long_sequences_in_32_bits_keep_their_digits(Hq, H, D, S, width):
+    """The error of a whole output, not of single numbers at their worst: weights that miss their low parts would show."""
+    lengths = [9000, 4097, 700]
+    t = R.Setup(lengths, H, D, "fp32", 16, "cuda", seed=9, width=width)
+    q = t.normal(3, S, Hq, D, dtype="fp32") * 3
+    o = F.paged_attention(t.tensor(q), t.layer, t.table, t.lens)._t.cpu().double()
+    want, size, _ = R.attention(q, t.kv, [n - S for n in lengths], [S] * 3, D ** -0.5)
+
+    def rms(x):
+        return float(x.square().mean().sqrt())
+
+    # A score is the sum of D products of 22 bits each, 3 D^-1/2 in size on average: 2^-22 of 3 together, and as much again from sums
+    # that are cut off at 2^-24 in each of D / 8 steps; the exponent's own rounding is 2^-24 of scores of up to 16, 2^-20.  Products
+    # of weights and values and their sums add 2^-22 each.  In all below 2^-19 of the magnitudes that are added up.
+    bound = 2.0 ** -19 * rms(size)
+    assert rms(o - want) <= bound
+    # what the bound is for: the same with weights of 11 bits
+    cut = torch.zeros_like(want)
+    for b, n in enumerate(lengths):
+        for s in range(S):
+            k, v = (x[:n - S + s + 1].repeat_interleave(Hq // H, 1) for x in t.kv[b])
+            z = torch.einsum("hd,nhd->hn", q[b, s].double(), k) * D ** -0.5
+            p = torch.exp(z - z.amax(-1, keepdim=True))
+            step = torch.ldexp(torch.ones_like(p), torch.frexp(p)[1] - 11)
+            cut[b, s] = torch.einsum("hn,nhd->hd", torch.round(p / step) * step, v) / p.sum(-1)[:, None]
+    assert rms(cut - want) > 2 * bound
+
+
 # ---- 8 bits --------------------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype,S", [("bf16", 1), ("bf16", 3), ("fp32", 1)])
 @pytest.mark.parametrize("D", [64, 128])
@@ -378,3 +409,67 @@ def test_slots_that_rest_in_a_captured_step():
         # (products over other numbers of rows may be split otherwise: a dozen roundings to bf16 in each of two layers, 2^-9 on average)
         assert float((got.float() - alone[0].float()).norm() / alone[0].float().norm()) < 2 * 12 * 2.0 ** -9
     N.check_status()
+
+
+def _sharp(kind, head_dim):
+    """A model whose scores matter: queries and keys of several times the usual size."""
+    m = _model(kind, head_dim=head_dim)
+    for layer in m.model.layers:
+        for w in (layer.self_attn.q_proj.weight, layer.self_attn.k_proj.weight):
+            w._t.mul_(5.0)
+    return m
+
+
+def _decoded(m, tokens, head_dim, dtype, ahead=0):
+    """Logits of the tokens 99 .. 111 of 120 over a paged cache: a prompt, single tokens, a piece.  `ahead`: what single tokens'
+    lengths are off by."""
+    cache = PagedKVCache(10, 2, head_dim, page_size=32, num_layers=2, dtype=dtype, device="cuda")
+    table = cache.page_table(cache.allocate([130, 130]))
+    got = [m.forward_paged(genesis.Tensor(tokens[:, :100]), cache, table, _ints(100, 100), prompt=True)._t]
+    for n in range(101, 106):
+        got.append(m.forward_paged(genesis.Tensor(tokens[:, n - 1:n]), cache, table, _ints(n + ahead, n + ahead))._t)
+    got.append(m.forward_paged(genesis.Tensor(tokens[:, 105:112]), cache, table, _ints(112 + ahead, 112 + ahead), last=False)._t)
+    return torch.cat(got, 1).float()
+
+
+def _off(got, want):
+    return float((got - want).norm() / want.norm())
+
+
+@pytest.mark.parametrize("kind", ["dense", "moe"])
+@pytest.mark.parametrize("head_dim", [64, 128])
+def test_decoding_against_encoding_everything_in_32_bits(kind, head_dim):
+    """Both models, in 32 bits throughout, and what a position that is off by one would do."""
+    m, tokens = _sharp(kind, head_dim), _tokens(2, 112)
+    with genesis.no_grad():
+        want = m(genesis.Tensor(tokens))._t[:, 99:112].float()
+        # matrix products round their operands to 11 bits.  Operands that differ by 2^-20 round apart one time in 2^9, by 2^-11: 2^-15.5 of
+        # each of 14 products' results in two layers and the head, on either side, were they all of one sign: below 2^-10
+        assert _off(_decoded(m, tokens, head_dim, "float32"), want) < 2.0 ** -10
+        assert _off(_decoded(m, tokens, head_dim, "float32", ahead=1), want) > 2.0 ** -8
+
+
+@pytest.mark.parametrize("kind", ["dense", "moe"])
+@pytest.mark.parametrize("head_dim", [64, 128])
+@pytest.mark.parametrize("cache_dtype,slack", [("bfloat16", 0.0), ("float16", 0.0), ("float8_e4m3fn", 2.0 ** -4)])
+def test_decoding_in_mixed_types_over_caches_of_all_types(kind, head_dim, cache_dtype, slack):
+    """Queries in 32 bits over 16- and 8-bit caches, which a model outside autocast asks for; against a cache in 32 bits."""
+    m, tokens = _sharp(kind, head_dim), _tokens(2, 112)
+    with genesis.no_grad():
+        want = _decoded(m, tokens, head_dim, "float32")
+        # keys and values lose 2^-9 (fp16: 2^-12; 8 bits: 2^-5 each on average, 2^-4 in all) in two layers; scores of up to 16 carry that on
+        bound = 2 * 2.0 ** -9 * 4 + slack * 4
+        assert _off(_decoded(m, tokens, head_dim, cache_dtype), want) < bound
+
+
+@pytest.mark.parametrize("head_dim", [64, 128])
+def test_decoding_in_bf16_against_encoding_everything(head_dim):
+    """Under autocast; a position that is off by one is further off than the roundings allow."""
+    m, tokens = _sharp("dense", head_dim), _tokens(2, 112)
+    with genesis.no_grad(), genesis.amp.autocast(dtype=genesis.bfloat16):
+        want = m(genesis.Tensor(tokens))._t[:, 99:112].float()
+        # a dozen roundings to bf16 a layer, 2^-9 / 3^1/2 of a number each and independent of one another, on either side, carried on
+        # by scores of several times the usual size
+        bound = 4 * (2 * 2 * 12) ** 0.5 * 2.0 ** -9 / 3 ** 0.5
+        assert _off(_decoded(m, tokens, head_dim, "bfloat16"), want) < bound
+        assert _off(_decoded(m, tokens, head_dim, "bfloat16", ahead=1), want) > 2 * bound
