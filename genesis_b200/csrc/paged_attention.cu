@@ -3,8 +3,8 @@
 //   o[b, s, h] = sum_j p_j v_j,  p = softmax of scale * q . k_j over the j < lengths[b] - counts[b] + s + 1
 //
 // with K and V of KV head h / (Hq / Hkv), and zeros for a row that sees no key (a token that is none, or scores that are -inf
-// throughout).  One pass over the keys with a running maximum and sum in 32 bits; keys behind the end are neither read nor
-// multiplied, so what the rest of a page holds does not matter.
+// throughout).  One pass over the keys with a running maximum and sum in 32 bits.  Tiles of 16 keys are read whole; scores and values
+// of keys behind the end are cleared in the last one, so what the rest of a page holds does not matter.
 //
 // Work is shared out by the lengths on the device, so that a captured launch stays right as sequences grow and a long sequence
 // does not leave the GPU to one SM: the chunks of keys of all items (sequence, KV head, tile of query rows) are numbered in
@@ -17,8 +17,9 @@
 //              order that K and Q share, so a lane takes contiguous bytes of its key's row; for V a lane takes contiguous d of four
 //              keys and pairs the keys' numbers with byte permutes.  P^T comes from S^T by movmatrix.
 //   bound    : the bytes of K and V where sequences are long: 64 x 4096 keys, 32 / 4 heads of 128, bf16: 95 us, 5.65 TB/s (6.1 less the 8
-//              that 500 keys take); in 8 bits 59 us, 4.6 TB/s, where converting and the wait for it take as long as the bytes.  8 us of
-//              a call are two launches, finding the share, one round of latencies and the join.
+//              that 500 keys take).  In 8 bits 59 us, 4.6 TB/s, where nothing is at its limit (DRAM 51 %, issue slots 54 %): 16 warps an SM
+//              with one chunk in flight wait for it, at 128 registers of which some are spilled.  8 us of a call are two launches,
+//              finding the share, one round of latencies and the join.
 //   other ways that were measured: fragments by plain loads (bf16 93 us, 8 bits 70), by cp.async (109, 70); fetching ahead into L2 with
 //              plain loads (99 to 110).
 //   precision: P enters its product as two 16-bit numbers (rounded, and what the rounding lost), or rounding it once to the
@@ -65,7 +66,8 @@ static constexpr int attend_chunk(int D, int bytes) { return 4096 / (D * bytes) 
 // CTAs on an SM, by registers: four, three where numbers are split in two or added up apart, two for two operands of rows over 128
 // numbers of 8 bits.  (Three instead of four, 32 / 4 heads of 128: 64 x 4096 bf16 98.7 us for 95.2, in 8 bits 60.7 for 59.2; 8 x 4096 25.3
 // for 23.0, in 8 bits 20.5 for 18.0; 8 x 32768 in 8 bits 57.3 for 58.3.)  Chunks in flight of a warp, by what shared memory is left; one
-// where registers are spilled, which need the L1 that a larger ring takes (32 x 4096, drafts of 4: 144 us with two, 93 with one).
+// where the spilled registers are many, which need the L1 that a larger ring takes (32 x 4096, drafts of 4: 144 us with two, 93 with one).
+// (29 of the 38 kernels spill, 4 to 292 bytes a thread; those of two operands over 16 bits the most.)
 static constexpr int attend_ctas(int dt, int cdt, int D, int R) {
   return R == 16 ? (cdt == DT_E4M3 && D == 128 ? 2 : 3) : cdt == DT_F32 || (cdt == DT_E4M3 && dt == DT_F16) ? 3 : 4;
 }
@@ -218,7 +220,8 @@ __device__ __forceinline__ void store_row4(const AttendArgs& a, const Paged& c, 
 // A warp's share once more, number by number in 32 bits: where keys, values or queries are infinite, what the loop over the
 // tensor cores has made of them is put right, in a run's sums (the last in the ring, others in `spill`, maxima and normalisers
 // at m and l) or in the output.  Only rows and columns that are not finite, or were not to be, are replaced.  A row whose scores are
-// NaN stays so, and is not followed to its end.  About a microsecond a key, which only such numbers pay for.
+// NaN stays so, and is not followed to its end.  About two microseconds a key of the share, which only such numbers pay for (an infinity
+// among the values, 64 x 4096, 32 / 4 heads of 128, bf16: 0.9 ms for 0.1); that the code is there costs others 0 to 0.3 us a call.
 template <typename T, int CDT, int D, int R, int KT>
 __device__ __noinline__ void redo_share(const AttendArgs& a, const Paged& c, const AttendPlan& plan, unsigned u, unsigned u_end, float* ring,
                                         float* spill, float* m, float* l) {
@@ -1139,6 +1142,8 @@ using namespace gb;
 //   rows: two operands of 8 read K and V half as often, and leave half as many chunks to share out.  By what the page table has
 //   room for, two where each warp then has four chunks and more: 32 x 4096, drafts of 4, 32 / 4 heads of 128: 93 us (146 with one), 14 / 2
 //   of 64, drafts of 2: 25.6 (28.7); 8 x 2000, drafts of 8, 12 / 2 of 128: 26.6 with two, 22.9 with one; 4 x 2000, drafts of 5: 17.6, 15.8.
+//   The sequences' own lengths are known on the device only.  A table with room for 32768 over 8 sequences of 200 (drafts of 4, 32 / 4 of
+//   128) takes two operands for one and 15.8 us for 14.0; single tokens 11.7 for 11.2; over 32 of 2000 nothing changes.
 struct AttendChoice { int R, grid; };
 static AttendChoice attend_choice(int B, int S, int Hq, int Hkv, int D, int page, int pages, int per, int dt, int cdt) {
   if ((D != 64 && D != 128) || (cdt != dt && !(cdt == DT_E4M3 && dt != DT_F32)) || page % 16) return {8, 0};
