@@ -17,7 +17,7 @@
 //              order that K and Q share, so a lane takes contiguous bytes of its key's row; for V a lane takes contiguous d of four
 //              keys and pairs the keys' numbers with byte permutes.  P^T comes from S^T by movmatrix.
 //   bound    : the bytes of K and V where sequences are long: 64 x 4096 keys, 32 / 4 heads of 128, bf16: 95 us, 5.65 TB/s (6.1 less the 8
-//              that 500 keys take).  In 8 bits 59 us, 4.6 TB/s, where nothing is at its limit (DRAM 51 %, issue slots 54 %): 16 warps an SM
+//              that 500 keys take).  In 8 bits 59 us, 4.6 TB/s, where nothing is at its limit (DRAM 49 %, issue slots 54 %): 16 warps an SM
 //              with one chunk in flight wait for it, at 128 registers of which some are spilled.  8 us of a call are two launches,
 //              finding the share, one round of latencies and the join.
 //   other ways that were measured: fragments by plain loads (bf16 93 us, 8 bits 70), by cp.async (109, 70); fetching ahead into L2 with
