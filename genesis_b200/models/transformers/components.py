@@ -70,7 +70,7 @@ class RotaryEmbedding(nn.Module):
             dev = old.device
         values = self._values(seq_len, dev)      # (nothing changes where this fails, as it does while a stream is captured)
         if old is not None:
-            self._outgrown.append((old, self.sin_cached))
+            self.__dict__.setdefault("_outgrown", _Unseen()).append((old, self.sin_cached))     # (a module that was pickled without)
         self.max_seq_len_cached = seq_len
         for name, t in zip(("inv_freq", "cos_cached", "sin_cached"), values):
             self.register_buffer(name, t, persistent=False)
@@ -86,9 +86,10 @@ class RotaryEmbedding(nn.Module):
         cos = self.cos_cached
         if cos._t.dtype is torch.float32:
             return cos, self.sin_cached
-        if not len(self._exact) or self._exact[-1][0].shape != cos.shape or self._exact[-1][0].device != cos.device:
-            self._exact.append(tuple(self._values(cos.shape[0], cos.device)[1:]))
-        return self._exact[-1]
+        kept = self.__dict__.setdefault("_exact", _Unseen())
+        if not len(kept) or kept[-1][0].shape != cos.shape or kept[-1][0].device != cos.device:
+            kept.append(tuple(self._values(cos.shape[0], cos.device)[1:]))
+        return kept[-1]
 
     def forward(self, x=None, seq_len=None):
         if seq_len is not None:

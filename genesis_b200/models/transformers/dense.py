@@ -14,7 +14,8 @@ import torch
 from ... import nn
 from ...nn import functional as F
 from ...tensor import Tensor
-from .components import RotaryEmbedding, apply_rope, find_multiple, in_places, last_tokens, paged_self_attention, prompt_first  # noqa: F401
+from .components import (RotaryEmbedding, apply_rope, find_multiple, in_places, last_tokens,  # noqa: F401
+                         paged_self_attention, prompt_first)
 from .config import TransformerConfig, get_transformer_config
 
 ModelArgs = TransformerConfig

@@ -2078,13 +2078,14 @@ def paged_attention(q, cache, page_table, lengths, counts=None, scale=None):
 
     `lengths` counts the tokens in the cache, those of this call (written before) among them; with `counts` [B] only the first
     counts[b] of the S are real.  Token s sees the positions up to its own, lengths[b] - counts[b] + s; a token that is none,
-    or whose scores are -inf throughout, gives zeros.  Hkv divides Hq; `scale` is D ** -0.5 unless given.  Scores, probabilities and
-    sums are held in 32 bits.  On CUDA, heads of 64 and 128 go through the tensor cores: probabilities then enter their product with
-    the values in two 16-bit numbers (17 bits of them below bfloat16, 22 below float16), or in one of 11 bits where the cache holds 8 and q
-    is bfloat16, and float32 numbers as two of 11 bits (a relative 2^-22 is lost of each); other heads, and types that differ
-    (float32 q over 8 or 16 bits), are worked on in 32 bits, number by number.  Keys whose page or position does not exist take no part, and the error is raised as
-    `paged_kv_write` says.  Made for few tokens; where S runs into the hundreds and the sequences are equally long, the
-    flash attention over what `paged_kv_read` brings back is faster."""
+    or whose scores are -inf throughout, gives zeros.  Hkv divides Hq; `scale` is D ** -0.5 unless given.  Keys whose page or
+    position does not exist take no part, and the error is raised as `paged_kv_write` says.  Made for few tokens; where S runs
+    into the hundreds and the sequences are equally long, the flash attention over what `paged_kv_read` brings back is faster.
+
+    Scores, probabilities and sums are held in 32 bits.  On CUDA, heads of 64 and 128 go through the tensor cores: probabilities
+    then enter their product with the values in two 16-bit numbers (17 bits of them below bfloat16, 22 below float16), or in one
+    of 11 bits where the cache holds 8 and q is bfloat16, and float32 numbers as two of 11 bits (a relative 2^-22 is lost of
+    each); other heads, and types that differ (float32 q over 8 or 16 bits), are worked on in 32 bits, number by number."""
     name = "paged_attention"
     q = _paged_tokens(name, "q", q, 4)
     table, lengths, counts = _paged_args(name, cache, page_table, lengths, counts, q.shape[0], q.get_device())

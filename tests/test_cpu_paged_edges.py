@@ -247,3 +247,14 @@ def test_lengths_that_blocks_of_16_cannot_count():
     for n in (2 ** 31 - 15, 2 ** 31 - 1, 2 ** 40):
         with pytest.raises(ValueError, match="max_length"):
             F.paged_kv_read(t.layer, t.table, t.lens, n)
+
+
+def test_modules_that_were_pickled_without_a_place_for_old_tables():
+    rot = RotaryEmbedding(16, 32)
+    del rot._outgrown, rot._exact
+    rot.reserve(40)
+    assert rot.max_seq_len_cached == 64 and len(rot._outgrown) == 1
+    rot.bfloat16()
+    del rot._exact
+    cos, _ = rot.tables32()
+    assert cos._t.dtype == torch.float32 and cos.shape == (64, 16) and rot.tables32()[0] is cos
